@@ -109,6 +109,11 @@ HIP_SYMBOLS = {
     "dali_hip_argsort_i32": (_i, [H, C.c_int64, C.c_int32, H, H]),
     "dali_hip_argsort_i32_noalloc": (_i, [H, C.c_int64, C.c_int32, H, H]),
     "dali_hip_topk_rows": (_i, [H, _i, C.c_int64, C.c_int32, C.c_int32, _i, _i, H]),
+    "dali_hip_layer_norm": (_i, [_i, C.c_int64, _i, H, C.c_int64, H, H, C.c_double, H, H, H]),
+    "dali_hip_layer_norm_backward": (_i, [_i, C.c_int64, _i, H, C.c_int64, H, C.c_int64, H, H, H, H, H, H]),
+    "dali_hip_token_log_probs": (_i, [_i, C.c_int64, _i, H, C.c_int64, H, _i, H, H, H, H, H]),
+    "dali_hip_token_log_probs_backward": (_i, [_i, C.c_int64, _i, H, H, H, C.c_int64, H, H, H, H]),
+    "dali_hip_clip_by_global_norm": (_i, [_i, _i, C.POINTER(H), C.POINTER(H), C.POINTER(C.c_int64), C.c_double, H]),
     "dali_hip_capture_begin": (_i, []),
     "dali_hip_capture_end": (_i, [C.POINTER(H)]),
     "dali_hip_graph_launch": (_i, [H]),
@@ -197,6 +202,11 @@ FRONT_SYMBOLS = {
     "dali_fe_gru_sequence": (_i, [H, H, H, H, H, _HP, _HP]),
     "dali_fe_stacked_lstm_step": (_i, [H, _i, _HP, _HP, _HP, _HP, _HP, _i, _HP, _HP]),
     "dali_fe_stacked_lstm_sequence": (_i, [H, _i, _HP, _HP, _HP, _HP, _HP, _i, _HP, _HP, _HP]),
+    "dali_fe_layer_norm": (_i, [H, H, H, C.c_double, _HP, _HP, _HP]),
+    "dali_fe_layer_norm_backward": (_i, [H, H, H, H, H, _HP, _HP, _HP]),
+    "dali_fe_token_log_probs": (_i, [H, H, _i, _HP, _HP, _HP, _HP, _HP]),
+    "dali_fe_token_log_probs_backward": (_i, [H, H, H, H, H, H, _HP]),
+    "dali_fe_clip_by_global_norm": (_i, [_HP, _i, C.c_double, _HP, _HP]),
     "dali_fe_eval": (_i, [H]),
     "dali_fe_eval_together": (_i, [_HP, _i]),
     "dali_fe_assign": (_i, [H, _i, H]),

@@ -262,6 +262,49 @@ dali_array_t dali_fe_gru_step(dali_array_t x, dali_array_t h, dali_array_t W, da
     FE_TRY(return wrap(dali::op::gru_step(A(x), A(h), A(W), A(U), A(b)));, nullptr)
 }
 
+// an operand that may be absent
+static Array maybe(dali_array_t h) { return h ? *(Array*)h : Array(); }
+// a destination that may be absent, and its handle once it is not
+static Array given(const dali_array_t* h) { return h && *h ? *(Array*)*h : Array(); }
+static void deliver(dali_array_t* h, const Array& a) {
+    if (h && !*h && !a.is_stateless()) *h = wrap(a);
+}
+
+int dali_fe_layer_norm(dali_array_t x, dali_array_t gamma, dali_array_t beta, double epsilon, dali_array_t* y, dali_array_t* mean, dali_array_t* rstd) {
+    FE_TRY(auto r = dali::op::layer_norm(A(x), maybe(gamma), maybe(beta), epsilon, {given(y), given(mean), given(rstd)}); deliver(y, r.y); deliver(mean, r.mean);
+           deliver(rstd, r.rstd); return 0;
+           , 1)
+}
+int dali_fe_layer_norm_backward(dali_array_t dy, dali_array_t x, dali_array_t mean, dali_array_t rstd, dali_array_t gamma, dali_array_t* dx, dali_array_t* dgamma,
+                                dali_array_t* dbeta) {
+    FE_TRY(auto r = dali::op::layer_norm_backward(A(dy), A(x), A(mean), A(rstd), maybe(gamma), {given(dx), given(dgamma), given(dbeta)}); deliver(dx, r.x);
+           deliver(dgamma, r.gamma); deliver(dbeta, r.beta); return 0;
+           , 1)
+}
+int dali_fe_token_log_probs(dali_array_t logits, dali_array_t tokens, int k, dali_array_t* log_probs, dali_array_t* entropy, dali_array_t* lse, dali_array_t* top_log_probs,
+                            dali_array_t* top_tokens) {
+    FE_TRY(auto r = dali::op::token_log_probs(A(logits), A(tokens), k, {given(log_probs), given(entropy), given(lse), given(top_log_probs), given(top_tokens)});
+           deliver(log_probs, r.log_probs); deliver(entropy, r.entropy); deliver(lse, r.lse); deliver(top_log_probs, r.top_log_probs); deliver(top_tokens, r.top_tokens);
+           return 0;
+           , 1)
+}
+int dali_fe_token_log_probs_backward(dali_array_t d_log_probs, dali_array_t d_entropy, dali_array_t logits, dali_array_t tokens, dali_array_t lse, dali_array_t entropy,
+                                     dali_array_t* d_logits) {
+    FE_TRY(deliver(d_logits, dali::op::token_log_probs_backward(A(d_log_probs), maybe(d_entropy), A(logits), A(tokens), A(lse), maybe(entropy), given(d_logits))); return 0;, 1)
+}
+int dali_fe_clip_by_global_norm(const dali_array_t* arrays, int count, double max_norm, dali_array_t* clipped, dali_array_t* norm) {
+    FE_TRY(std::vector<Array> in; for (int i = 0; i < count; ++i) in.push_back(A(arrays[i]));
+           if (!clipped) { deliver(norm, dali::op::global_norm(in, given(norm))); return 0; }
+           dali::op::ClippedArrays out; bool any = false;
+           for (int i = 0; i < count; ++i) { out.arrays.push_back(given(&clipped[i])); any = any || clipped[i]; }
+           if (!any) out.arrays.clear();
+           out.norm = given(norm);
+           auto r = dali::op::clip_by_global_norm(in, max_norm, out);
+           for (int i = 0; i < count; ++i) deliver(&clipped[i], r.arrays[i]);
+           deliver(norm, r.norm); return 0;
+           , 1)
+}
+
 int dali_fe_eval(dali_array_t a) { FE_TRY(A(a).eval(); return 0;, 1) }
 int dali_fe_eval_together(dali_array_t* roots, int n) {
     FE_TRY(std::vector<Array> r; for (int i = 0; i < n; ++i) r.push_back(A(roots[i])); Array::eval_together(r); return 0;, 1)

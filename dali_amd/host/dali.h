@@ -390,6 +390,37 @@ struct GRUSequence {
     Array states, last;
 };
 GRUSequence gru_sequence(const Array& xs, const Array& h0, const Array& W, const Array& U, const Array& b);
+
+// Layer normalisation along the last axis: y = (x - mean) rstd gamma + beta, with the statistics that its gradient needs (shape of x without its last
+// axis). gamma and beta may be stateless (1 and 0). Here and below: float or double, evaluated when called, and the members of `out` that are not stateless
+// are the destinations (dense buffers of the result's shape; y may be x itself).
+struct LayerNorm {
+    Array y, mean, rstd;
+};
+LayerNorm layer_norm(const Array& x, const Array& gamma = Array(), const Array& beta = Array(), double epsilon = 1e-5, const LayerNorm& out = LayerNorm());
+// The gradients of x, gamma and beta from dy, that of y. A stateless gamma stands for 1, and the gradients of the weights are then not formed. x's may be dy or x itself.
+struct LayerNormGradient {
+    Array x, gamma, beta;
+};
+LayerNormGradient layer_norm_backward(const Array& dy, const Array& x, const Array& mean, const Array& rstd, const Array& gamma = Array(),
+                                      const LayerNormGradient& out = LayerNormGradient());
+// Log probabilities of one given token per row of logits [..., V] under softmax(logits), the entropy of the row, its log-sum-exp, and the k best entries with
+// their log probabilities (the lower position first among equals). A token outside [0, V) stands for none: log probability 0.
+struct TokenLogProbs {
+    Array log_probs, entropy, lse, top_log_probs, top_tokens;
+};
+TokenLogProbs token_log_probs(const Array& logits, const Array& tokens, int k = 0, const TokenLogProbs& out = TokenLogProbs());
+// The gradient of the logits from those of log_probs and entropy (stateless: none); it may take the logits' place
+Array token_log_probs_backward(const Array& d_log_probs, const Array& d_entropy, const Array& logits, const Array& tokens, const Array& lse, const Array& entropy,
+                               const Array& out = Array());
+// sqrt of the sum of the squares of all values of all arrays, summed in double
+Array global_norm(const std::vector<Array>& arrays, const Array& out = Array());
+// the arrays times min(1, max_norm / norm), and the norm; arrays come back as they are where the norm is not finite. Destinations may be the arrays themselves
+struct ClippedArrays {
+    std::vector<Array> arrays;
+    Array norm;
+};
+ClippedArrays clip_by_global_norm(const std::vector<Array>& arrays, double max_norm, const ClippedArrays& out = ClippedArrays());
 }  // namespace op
 
 // Named scopes (dali/utils/scope.h:11-34): DALI_SCOPE(name) opens a scope that lasts to the end of the block when

@@ -10,6 +10,7 @@
 #define PY_SSIZE_T_CLEAN
 #include <Python.h>
 
+#include <deque>
 #include <vector>
 
 #include "../../include/dali_front.h"
@@ -359,10 +360,178 @@ PyObject* f_lstm_step(PyObject*, PyObject* const* args, Py_ssize_t n) {
     return status != 0 ? fail("lstm_step") : wrapped(r, 2, "lstm_step");
 }
 
+// Destinations that the program gives: None (new arrays), or a sequence of arrays and None. The results come back as a tuple: the destinations themselves
+// where they were given, new arrays elsewhere, None for what was not formed.
+struct Destinations {
+    PyObject* given = nullptr;
+    std::vector<dali_array_t> handles;
+    Destinations() = default;
+    Destinations(const Destinations&) = delete;
+    Destinations& operator=(const Destinations&) = delete;
+    ~Destinations() { Py_XDECREF(given); }
+    bool set(PyObject* out, Py_ssize_t n, const char* what) {
+        handles.assign(n, nullptr);
+        if (out == Py_None) return true;
+        given = PySequence_Tuple(out);
+        if (!given) return false;
+        if (PyTuple_GET_SIZE(given) != n) {
+            PyErr_Format(PyExc_TypeError, "%s: out must hold %zd arrays (got %zd)", what, n, PyTuple_GET_SIZE(given));
+            return false;
+        }
+        for (Py_ssize_t i = 0; i < n; ++i) {
+            PyObject* o = PyTuple_GET_ITEM(given, i);
+            if (o == Py_None) continue;
+            if (!PyObject_TypeCheck(o, &HandleType)) {
+                PyErr_Format(PyExc_TypeError, "%s: out holds something that is no Array", what);
+                return false;
+            }
+            handles[i] = ((ArrayObject*)o)->handle;
+            if (!handles[i]) {
+                PyErr_Format(PyExc_TypeError, "%s: out holds an Array without a handle", what);
+                return false;
+            }
+        }
+        return true;
+    }
+    PyObject* given_at(Py_ssize_t i) const {
+        PyObject* o = given ? PyTuple_GET_ITEM(given, i) : Py_None;
+        return o == Py_None ? nullptr : o;
+    }
+    // gives up the new handles, also where it fails
+    PyObject* results(const char* what) {
+        const Py_ssize_t n = (Py_ssize_t)handles.size();
+        PyObject* t = PyTuple_New(n);
+        for (Py_ssize_t i = 0; i < n; ++i) {
+            PyObject* o = given_at(i);
+            const bool fresh = !o && handles[i];
+            if (!t) {
+                if (fresh) release(handles[i]);
+                continue;
+            }
+            if (fresh) {
+                o = wrap(handles[i], what);
+                if (!o) Py_CLEAR(t);
+                else PyTuple_SET_ITEM(t, i, o);
+                continue;
+            }
+            o = o ? o : Py_None;
+            Py_INCREF(o);
+            PyTuple_SET_ITEM(t, i, o);
+        }
+        return t;
+    }
+};
+
+// an operand that may be None
+bool optional(Operand& a, PyObject* o) { return o == Py_None || a.set(o); }
+
+bool number(PyObject* o, double* v) {
+    *v = PyFloat_AsDouble(o);
+    return *v != -1.0 || !PyErr_Occurred();
+}
+
+// x, gamma, beta, epsilon, out
+PyObject* f_layer_norm(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    Operand x, gamma, beta;
+    Destinations out;
+    double epsilon;
+    if (!count_is(n, 5, "layer_norm") || !x.set(args[0]) || !optional(gamma, args[1]) || !optional(beta, args[2]) || !number(args[3], &epsilon) ||
+        !out.set(args[4], 3, "layer_norm"))
+        return nullptr;
+    dali_array_t* r = out.handles.data();
+    const int status = unlocked([&] { return dali_fe_layer_norm(x.handle, gamma.handle, beta.handle, epsilon, &r[0], &r[1], &r[2]); });
+    return status != 0 ? fail("layer_norm") : out.results("layer_norm");
+}
+
+// dy, x, mean, rstd, gamma, out
+PyObject* f_layer_norm_backward(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    Operand dy, x, mean, rstd, gamma;
+    Destinations out;
+    if (!count_is(n, 6, "layer_norm_backward") || !dy.set(args[0]) || !x.set(args[1]) || !mean.set(args[2]) || !rstd.set(args[3]) || !optional(gamma, args[4]) ||
+        !out.set(args[5], 3, "layer_norm_backward"))
+        return nullptr;
+    dali_array_t* r = out.handles.data();
+    const int status = unlocked([&] { return dali_fe_layer_norm_backward(dy.handle, x.handle, mean.handle, rstd.handle, gamma.handle, &r[0], &r[1], &r[2]); });
+    return status != 0 ? fail("layer_norm_backward") : out.results("layer_norm_backward");
+}
+
+// logits, tokens, k, out
+PyObject* f_token_log_probs(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    Operand logits, tokens;
+    Destinations out;
+    int k;
+    if (!count_is(n, 4, "token_log_probs") || !logits.set(args[0]) || !tokens.set(args[1]) || !whole_number(args[2], &k) || !out.set(args[3], 5, "token_log_probs")) return nullptr;
+    dali_array_t* r = out.handles.data();
+    const int status = unlocked([&] { return dali_fe_token_log_probs(logits.handle, tokens.handle, k, &r[0], &r[1], &r[2], &r[3], &r[4]); });
+    return status != 0 ? fail("token_log_probs") : out.results("token_log_probs");
+}
+
+// d_log_probs, d_entropy, logits, tokens, lse, entropy, out (one array or None)
+PyObject* f_token_log_probs_backward(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    const char* what = "token_log_probs_backward";
+    Operand a[6];
+    Destinations out;
+    if (!count_is(n, 7, what)) return nullptr;
+    for (int i = 0; i < 6; ++i)
+        if (i == 1 || i == 5 ? !optional(a[i], args[i]) : !a[i].set(args[i])) return nullptr;
+    PyObject* one = PyTuple_Pack(1, args[6]);
+    const bool ok = one && out.set(one, 1, what);
+    Py_XDECREF(one);
+    if (!ok) return nullptr;
+    dali_array_t* r = out.handles.data();
+    const int status = unlocked([&] { return dali_fe_token_log_probs_backward(a[0].handle, a[1].handle, a[2].handle, a[3].handle, a[4].handle, a[5].handle, &r[0]); });
+    PyObject* t = status != 0 ? fail(what) : out.results(what);
+    if (!t) return nullptr;
+    PyObject* d = PyTuple_GET_ITEM(t, 0);
+    Py_INCREF(d);
+    Py_DECREF(t);
+    return d;
+}
+
+// arrays, max_norm (None: the norm alone), destinations of the arrays, destination of the norm -> (tuple of arrays, norm), or the norm
+PyObject* f_clip_by_global_norm(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    const char* what = "clip_by_global_norm";
+    if (!count_is(n, 4, what)) return nullptr;
+    const bool clip = args[1] != Py_None;
+    double max_norm = 0;
+    if (clip && !number(args[1], &max_norm)) return nullptr;
+    PyObject* arrays = PySequence_Tuple(args[0]);
+    if (!arrays) return nullptr;
+    const Py_ssize_t count = PyTuple_GET_SIZE(arrays);
+    std::deque<Operand> operands;
+    std::vector<dali_array_t> in;
+    Destinations out, norm;
+    PyObject* one = PyTuple_Pack(1, args[3]);
+    bool ok = one && norm.set(one, 1, what) && out.set(args[2], clip ? count : 0, what);
+    Py_XDECREF(one);
+    for (Py_ssize_t i = 0; ok && i < count; ++i) {
+        operands.emplace_back();
+        ok = operands.back().set(PyTuple_GET_ITEM(arrays, i));
+        in.push_back(operands.back().handle);
+    }
+    Py_DECREF(arrays);
+    if (!ok) return nullptr;
+    const int status = unlocked([&] { return dali_fe_clip_by_global_norm(in.data(), (int)count, max_norm, clip ? out.handles.data() : nullptr, norm.handles.data()); });
+    if (status != 0) return fail(clip ? what : "global_norm");
+    PyObject* t = norm.results(what);
+    if (!t) return nullptr;
+    PyObject* d = PyTuple_GET_ITEM(t, 0);
+    Py_INCREF(d);
+    Py_DECREF(t);
+    if (!clip) return d;
+    PyObject* results = out.results(what);
+    PyObject* pair = results ? PyTuple_Pack(2, results, d) : nullptr;
+    Py_XDECREF(results);
+    Py_DECREF(d);
+    return pair;
+}
+
 #define FUNCTION(name) {#name, (PyCFunction)(void (*)(void))f_##name, METH_FASTCALL, nullptr}
 PyMethodDef functions[] = {FUNCTION(register),        FUNCTION(unary),     FUNCTION(binary),  FUNCTION(all_reduce), FUNCTION(axis_reduce),
                            FUNCTION(arg_axis_reduce), FUNCTION(softmax),   FUNCTION(dot),     FUNCTION(gather),     FUNCTION(gather_from_rows),
                            FUNCTION(transpose),       FUNCTION(assign),    FUNCTION(softmax_cross_entropy),         FUNCTION(lstm_step),
+                           FUNCTION(layer_norm),      FUNCTION(layer_norm_backward),   FUNCTION(token_log_probs),    FUNCTION(token_log_probs_backward),
+                           FUNCTION(clip_by_global_norm),
                            {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_bind", nullptr, -1, functions, nullptr, nullptr, nullptr, nullptr};
 

@@ -216,6 +216,48 @@ def softmax_cross_entropy(logits, targets):
     return _bind.softmax_cross_entropy(logits, targets)
 
 
+# Operators of language models. They are evaluated when called, take float or double arrays, and write into new arrays or, with ``out``, into destinations that the
+# program keeps: dense buffers of the results' shapes (None in the place of one: a new array). A destination may take the place of the operand that is named
+# for it and must not overlap anything else.
+def layer_norm(x, gamma=None, beta=None, epsilon=1e-5, out=None):
+    """(y, mean, rstd) of the normalisation along the last axis: mean and rstd = 1 / sqrt(mean((x - mean)^2) + epsilon) have the shape of x without that axis,
+    y = (x - mean) rstd gamma + beta. gamma and beta are vectors, None stands for 1 and 0. y may be x itself."""
+    return _bind.layer_norm(x, gamma, beta, epsilon, out)
+
+
+def layer_norm_backward(dy, x, mean, rstd, gamma=None, out=None):
+    """(dx, dgamma, dbeta) from dy, the gradient of y, and the statistics that ``layer_norm`` left. Without gamma there are no weights: (dx, None, None).
+    dx may be dy or x itself. Gradients of the weights are summed in an order that depends on the shape alone."""
+    return _bind.layer_norm_backward(dy, x, mean, rstd, gamma, out)
+
+
+def token_log_probs(logits, tokens, k=0, out=None):
+    """(log_probs, entropy, lse, top_log_probs, top_tokens) of softmax(logits) along the last axis: the log probability of one given token per row (int32), the
+    entropy of the row, ln sum e^x, and the k (at most 64) best entries, the lower position first among equals; k = 0: None for both.
+
+    A logit of -inf has probability 0. A row of nothing else has lse = log_probs = -inf and entropy 0. A NaN or +inf makes its row's values NaN (a NaN
+    ranks last among the alternatives). A token outside the vocabulary (-1, say) marks a row without one: log probability 0."""
+    return _bind.token_log_probs(logits, tokens, k, out)
+
+
+def token_log_probs_backward(d_log_probs, d_entropy, logits, tokens, lse, entropy, out=None):
+    """The gradient of the logits from those of log_probs and entropy: d_log_probs (one_hot - p) - d_entropy p (ln p + entropy). d_entropy (and entropy
+    with it) may be None. A row of -inf alone gets zeros; a row without a token has none through its log probability. The gradient may take the logits' place."""
+    return _bind.token_log_probs_backward(d_log_probs, d_entropy, logits, tokens, lse, entropy, out)
+
+
+def global_norm(arrays, out=None):
+    """sqrt of the sum of the squares of all values of all arrays (of one type), summed in double; a scalar array."""
+    return _bind.clip_by_global_norm(arrays, None, None, out)
+
+
+def clip_by_global_norm(arrays, max_norm, out=None):
+    """(arrays times min(1, max_norm / norm), norm) with the norm of ``global_norm``. ``out``: (destinations or None, destination of the norm or None); the
+    arrays themselves may be their destinations. Where the norm is not finite the arrays come back as they are."""
+    destinations, norm = (None, None) if out is None else out
+    return _bind.clip_by_global_norm(arrays, float(max_norm), destinations, norm)
+
+
 def lstm_step(x, h, c, W, U, b):
     """One LSTM cell step; returns (c', h') already evaluated."""
     return _bind.lstm_step(x, h, c, W, U, b)

@@ -151,6 +151,22 @@ dali_array_t dali_fe_gru_step(dali_array_t x, dali_array_t h, dali_array_t W, da
  * [T, B, H] and the last one; the input half of all steps is one product */
 int dali_fe_gru_sequence(dali_array_t xs, dali_array_t h0, dali_array_t W, dali_array_t U, dali_array_t b, dali_array_t* states, dali_array_t* last);
 
+/* Layer normalisation along the last axis, its gradient, log probabilities of tokens and clipping by the global norm; see op.layer_norm and what follows it in
+ * dali_amd/op.py. Evaluated when called. Every result is passed by the address of a handle: NULL there receives a new array, a handle is the
+ * destination (a dense buffer of the result's shape and type) and stays. gamma, beta, tokens' and entropy's gradient may be NULL where that is said. */
+int dali_fe_layer_norm(dali_array_t x, dali_array_t gamma, dali_array_t beta, double epsilon, dali_array_t* y, dali_array_t* mean, dali_array_t* rstd);
+/* gamma NULL: dgamma and dbeta are not formed and their handles left alone */
+int dali_fe_layer_norm_backward(dali_array_t dy, dali_array_t x, dali_array_t mean, dali_array_t rstd, dali_array_t gamma, dali_array_t* dx, dali_array_t* dgamma,
+                                dali_array_t* dbeta);
+/* k = 0: the handles of the alternatives are left alone */
+int dali_fe_token_log_probs(dali_array_t logits, dali_array_t tokens, int k, dali_array_t* log_probs, dali_array_t* entropy, dali_array_t* lse, dali_array_t* top_log_probs,
+                            dali_array_t* top_tokens);
+/* d_entropy NULL: entropy may be NULL too */
+int dali_fe_token_log_probs_backward(dali_array_t d_log_probs, dali_array_t d_entropy, dali_array_t logits, dali_array_t tokens, dali_array_t lse, dali_array_t entropy,
+                                     dali_array_t* d_logits);
+/* clipped: `count` handles, or NULL for the norm alone */
+int dali_fe_clip_by_global_norm(const dali_array_t* arrays, int count, double max_norm, dali_array_t* clipped, dali_array_t* norm);
+
 /* evaluation, assignment, host access */
 int dali_fe_eval(dali_array_t a);
 int dali_fe_eval_together(dali_array_t* roots, int n);

@@ -347,6 +347,47 @@ int dali_hip_gru_recurrent_persistent_supported(int batch, int hidden);
 int dali_hip_softmax_axis(const float* x, float* out, long long outer, int extent, long long inner);
 int dali_hip_softmax_axis_supported(long long outer, int extent, long long inner);
 
+/* ------------------------------------------------------------- layer normalisation */
+/*
+ * Rows of `width` values, x_stride values apart (x may be a view of wider rows): mean = sum(x) / width, rstd = 1 / sqrt(mean((x - mean)^2) + epsilon),
+ * y = (x - mean) rstd gamma + beta. dtype: DALI_HIP_FLOAT or DALI_HIP_DOUBLE, of every operand. gamma and beta [width] may be NULL (1 and 0). y
+ * [rows, width], mean and rstd [rows] are dense; y may be x itself where that is dense, any other overlap is refused. The reference has none.
+ */
+int dali_hip_layer_norm(int dtype, int64_t rows, int width, const void* x, int64_t x_stride, const void* gamma, const void* beta, double epsilon, void* y, void* mean,
+                        void* rstd);
+/*
+ * Its gradient, from the gradient dy of y and the mean and rstd that the forward pass left: with u = (x - mean) rstd and a = dy gamma,
+ * dx = rstd (a - mean(a) - u mean(a u)), dgamma = sum over the rows of dy u, dbeta = that of dy. gamma may be NULL (1). dgamma and dbeta [width] come
+ * together; both NULL: not formed. dx [rows, width] is dense and may be x or dy itself. Sums over rows are formed in an order that depends on the extents alone.
+ */
+int dali_hip_layer_norm_backward(int dtype, int64_t rows, int width, const void* dy, int64_t dy_stride, const void* x, int64_t x_stride, const void* mean, const void* rstd,
+                                 const void* gamma, void* dx, void* dgamma, void* dbeta);
+
+/* ------------------------------------------------------------- log probabilities of tokens */
+#define DALI_HIP_MAX_ALTERNATIVES 64
+/*
+ * Per row of logits [rows, vocab] (rows `stride` values apart): lse = ln sum e^x, log_probs = x[token] - lse, entropy = -sum p ln p with p = e^(x - lse),
+ * and the k best entries as top_tokens [rows, k] (lower position first among equals) with their log probabilities top_log_probs [rows, k]; k = 0: none, at most
+ * DALI_HIP_MAX_ALTERNATIVES. A logit of -inf has probability 0. A row of -inf alone: lse and log_probs -inf, entropy 0. A NaN or +inf makes the row's
+ * values NaN (among the alternatives a NaN ranks as -inf). A token outside [0, vocab) stands for none: log_probs 0. Destinations must not overlap anything.
+ */
+int dali_hip_token_log_probs(int dtype, int64_t rows, int vocab, const void* logits, int64_t stride, const int32_t* tokens, int k, void* log_probs, void* entropy, void* lse,
+                             void* top_log_probs, int32_t* top_tokens);
+/*
+ * The gradient of both: d_logits = d_log_probs (delta_token - p) - d_entropy p (ln p + entropy), from the lse and entropy of the forward pass. d_entropy may be NULL (entropy
+ * is not read then). d_logits [rows, vocab] is dense and may be the logits themselves. Rows of -inf alone get zeros, a token outside [0, vocab) no gradient through it.
+ */
+int dali_hip_token_log_probs_backward(int dtype, int64_t rows, int vocab, const void* d_log_probs, const void* d_entropy, const void* logits, int64_t stride,
+                                      const int32_t* tokens, const void* lse, const void* entropy, void* d_logits);
+
+/* ------------------------------------------------------------- the norm of many arrays */
+/*
+ * *norm = sqrt(sum of the squares of all values of `count` arrays of sizes[i] values each), summed in double whatever the type; with `out`, out[i] = in[i] * min(1,
+ * max_norm / norm). out[i] may be in[i]; other overlaps are refused. Where the norm is not finite nothing is scaled. in, out and sizes are host arrays, read before the
+ * call returns; norm is a device scalar of the arrays' type.
+ */
+int dali_hip_clip_by_global_norm(int dtype, int count, const void* const* in, void* const* out, const int64_t* sizes, double max_norm, void* norm);
+
 /* ------------------------------------------------------------- scatter */
 /*
  * Stable ordering of n int32 keys held in device memory: sorted_keys[p] is the p-th smallest key and
