@@ -19,26 +19,106 @@ struct Vec {
     typedef T type __attribute__((ext_vector_type(16 / sizeof(T)), aligned(sizeof(T))));
 };
 
-// one value of every thread -> the same fold of all in every thread, in an order that depends on nothing but the thread numbers.
-// `scratch` holds one T per wave; it may be used again at once.
-template <typename T>
-__device__ __forceinline__ T wave_sum(T v) {
-#pragma unroll
-    for (int d = 1; d < 64; d *= 2) v += __shfl_xor(v, d, 64);
-    return v;
+// The value of the lane that is D away in the binary numbering of a wave, for folds that have already joined the lanes closer than D: `a` and `b` are
+// the two halves' values, the same pair in both. Steps inside 16 lanes are data moves of the vector unit (within a quad, the mirror image of 8 and of 16 lanes),
+// the others exchange half rows between two registers; none goes through LDS.
+template <int D>
+__device__ __forceinline__ void halves(unsigned v, unsigned& a, unsigned& b) {
+    if constexpr (D <= 8) {
+        constexpr int control = D == 1 ? 0xB1 : D == 2 ? 0x4E : D == 4 ? 0x141 : 0x140;
+        a = v;
+        b = (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, control, 0xf, 0xf, true);
+    } else if constexpr (D == 16) {
+        const auto r = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+        a = r[0], b = r[1];
+    } else {
+        const auto r = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+        a = r[0], b = r[1];
+    }
 }
 
-template <int THREADS, typename T>
-__device__ __forceinline__ T block_sum(T v, T* scratch) {
-    v = wave_sum(v);
-    if (THREADS == 64) return v;
+template <int D, typename T>
+__device__ __forceinline__ void halves_of(T v, T& a, T& b) {
+    if constexpr (sizeof(T) == 4) {
+        unsigned x, y;
+        halves<D>(__builtin_bit_cast(unsigned, v), x, y);
+        a = __builtin_bit_cast(T, x), b = __builtin_bit_cast(T, y);
+    } else {
+        const unsigned long long bits = __builtin_bit_cast(unsigned long long, v);
+        unsigned x0, y0, x1, y1;
+        halves<D>((unsigned)bits, x0, y0);
+        halves<D>((unsigned)(bits >> 32), x1, y1);
+        a = __builtin_bit_cast(T, (unsigned long long)x1 << 32 | x0);
+        b = __builtin_bit_cast(T, (unsigned long long)y1 << 32 | y0);
+    }
+}
+
+// the fold of LANES neighbouring lanes' values, the same in each of them; `op` is commutative, so the bits do not depend on the lane
+template <int LANES, int D = 1, typename T, typename Op>
+__device__ __forceinline__ T fold_lanes(T v, Op op) {
+    if constexpr (D >= LANES) {
+        return v;
+    } else {
+        T a, b;
+        halves_of<D>(v, a, b);
+        return fold_lanes<LANES, D * 2>(op(a, b), op);
+    }
+}
+
+struct Sum {
+    template <typename T>
+    __device__ __forceinline__ T operator()(T a, T b) const {
+        return a + b;
+    }
+};
+// (a NaN loses against a number)
+struct Max {
+    __device__ __forceinline__ float operator()(float a, float b) const { return fmaxf(a, b); }
+    __device__ __forceinline__ double operator()(double a, double b) const { return fmax(a, b); }
+};
+
+// the fold of one value of every thread, the same in each of them, in an order that depends on nothing but the thread numbers. `scratch` holds one T per wave;
+// it may be used again at once.
+template <int THREADS, typename T, typename Op>
+__device__ __forceinline__ T fold_block(T v, T* scratch, Op op) {
+    v = fold_lanes<64>(v, op);
+    if constexpr (THREADS == 64) return v;
     __syncthreads();
     if ((threadIdx.x & 63) == 0) scratch[threadIdx.x >> 6] = v;
     __syncthreads();
     T s = scratch[0];
 #pragma unroll
-    for (int w = 1; w < THREADS / 64; ++w) s += scratch[w];
+    for (int w = 1; w < THREADS / 64; ++w) s = op(s, scratch[w]);
     return s;
+}
+
+template <int THREADS, typename T>
+__device__ __forceinline__ T block_sum(T v, T* scratch) {
+    return fold_block<THREADS>(v, scratch, Sum());
+}
+
+// Results that another workgroup of the same launch reads: stored past the caches of this one's die, awaited, and announced with a ticket
+template <typename T>
+__device__ __forceinline__ void publish(T* p, T v) {
+    __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+template <typename T>
+__device__ __forceinline__ T observe(const T* p) {
+    return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+// Whether the calling workgroup is the last of `members` to arrive at the counter, which it then leaves at zero. All threads call it; `shared` is theirs. What
+// any thread published before is acknowledged by memory before the ticket is drawn.
+__device__ __forceinline__ bool last_to_arrive(unsigned* counter, unsigned members, unsigned* shared) {
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        const unsigned ticket = __hip_atomic_fetch_add(counter, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        if (ticket == members - 1) __hip_atomic_store(counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        *shared = ticket;
+    }
+    __syncthreads();
+    asm volatile("" ::: "memory");
+    return *shared == members - 1;
 }
 
 // ------------------------------------------------------------------------------------------------ arguments (host)
