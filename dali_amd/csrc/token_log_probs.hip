@@ -33,6 +33,82 @@ struct Real<double> {
     static __device__ __forceinline__ double ln(double s) { return log(s); }
 };
 
+// An entry of a row (or the best of a group of entries, by the group's number): of two the better has the larger value, or among equals the lower position. A NaN
+// counts as -inf. Of fp32 it is one whole number that grows with the value and falls with the position; there a zero is a zero of either sign.
+template <typename T>
+struct Entry;
+template <>
+struct Entry<float> {
+    unsigned long long key;
+    static __device__ __forceinline__ Entry of(float v, int position) {
+        const unsigned b = __builtin_bit_cast(unsigned, fmaxf(v, -INFINITY) + 0.0f);
+        return {(unsigned long long)(b ^ ((unsigned)((int)b >> 31) | 0x80000000u)) << 32 | (0xffffffffu - (unsigned)position)};
+    }
+    static __device__ __forceinline__ Entry none() { return {0}; }  // worse than any
+    static __device__ __forceinline__ Entry either(bool first, const Entry& a, const Entry& b) { return {first ? a.key : b.key}; }
+    __device__ __forceinline__ float value() const {
+        const unsigned b = (unsigned)(key >> 32);
+        return __builtin_bit_cast(float, b ^ ((unsigned)((int)~b >> 31) | 0x80000000u));
+    }
+    __device__ __forceinline__ int position() const { return (int)(0xffffffffu - (unsigned)key); }
+    __device__ __forceinline__ bool better(const Entry& o) const { return key > o.key; }
+    template <int D>
+    __device__ __forceinline__ void halves(Entry& a, Entry& b) const {
+        halves_of<D>(key, a.key, b.key);
+    }
+    __device__ __forceinline__ Entry lane(int l) const {
+        return {(unsigned long long)(unsigned)__builtin_amdgcn_readlane((int)(key >> 32), l) << 32 | (unsigned)__builtin_amdgcn_readlane((int)key, l)};
+    }
+    __device__ __forceinline__ void publish(Entry* p) const { dali_hip::publish(&p->key, key); }
+    static __device__ __forceinline__ Entry observe(const Entry* p) { return {dali_hip::observe(&p->key)}; }
+};
+template <>
+struct Entry<double> {
+    double v;
+    long at;
+    static __device__ __forceinline__ Entry of(double v, int position) { return {fmax(v, -(double)INFINITY), position}; }
+    static __device__ __forceinline__ Entry none() { return {-INFINITY, 1L << 40}; }
+    static __device__ __forceinline__ Entry either(bool first, const Entry& a, const Entry& b) { return {first ? a.v : b.v, first ? a.at : b.at}; }
+    __device__ __forceinline__ double value() const { return v; }
+    __device__ __forceinline__ int position() const { return (int)at; }
+    __device__ __forceinline__ bool better(const Entry& o) const { return v > o.v || (v == o.v && at < o.at); }
+    template <int D>
+    __device__ __forceinline__ void halves(Entry& a, Entry& b) const {
+        halves_of<D>(v, a.v, b.v);
+        halves_of<D>(at, a.at, b.at);
+    }
+    static __device__ __forceinline__ long word(long w, int l) {
+        return (long)((unsigned long long)(unsigned)__builtin_amdgcn_readlane((int)(w >> 32), l) << 32 | (unsigned)__builtin_amdgcn_readlane((int)w, l));
+    }
+    __device__ __forceinline__ Entry lane(int l) const { return {__builtin_bit_cast(double, word(__builtin_bit_cast(long, v), l)), word(at, l)}; }
+    __device__ __forceinline__ void publish(Entry* p) const {
+        dali_hip::publish(&p->v, v);
+        dali_hip::publish(&p->at, at);
+    }
+    static __device__ __forceinline__ Entry observe(const Entry* p) { return {dali_hip::observe(&p->v), dali_hip::observe(&p->at)}; }
+};
+
+// the best entry that LANES neighbouring lanes hold
+template <int LANES, int D = 1, typename T>
+__device__ __forceinline__ Entry<T> best_of_lanes(const Entry<T>& e) {
+    if constexpr (D >= LANES) {
+        return e;
+    } else {
+        Entry<T> a, b;
+        e.template halves<D>(a, b);
+        return best_of_lanes<LANES, D * 2>(Entry<T>::either(a.better(b), a, b));
+    }
+}
+
+// how many of a wave's entries are better than the lane's own: its place among them
+template <typename T>
+__device__ __forceinline__ int place_in_wave(const Entry<T>& e) {
+    int place = 0;
+#pragma unroll 16
+    for (int l = 0; l < 64; ++l) place += e.lane(l).better(e) ? 1 : 0;
+    return place;
+}
+
 template <typename T>
 struct LogProbArgs {
     const T* logits;
@@ -44,38 +120,10 @@ struct LogProbArgs {
     // rows in segments: `per` groups of Vec<T>::N logits to a segment
     int segments, per;
     T* sums;         // [rows][segments][3]
-    T* best;         // [rows][segments][k]
-    int* positions;  // the same
+    Entry<T>* best;  // [rows][segments][k], in order
     unsigned* counters;
     int counter_step;
 };
-
-// of two entries the better: the larger value, the lower position among equals
-template <typename T>
-__device__ __forceinline__ bool better(T v, int i, T w, int j) {
-    return v > w || (v == w && i < j);
-}
-
-// a NaN counts as -inf among the alternatives
-template <typename T>
-__device__ __forceinline__ T ranked(T v) {
-    return Max()(v, T(-INFINITY));
-}
-
-// the best entry that LANES neighbouring lanes hold
-template <int LANES, int D = 1, typename T>
-__device__ __forceinline__ void best_of_lanes(T& v, int& i) {
-    if constexpr (D < LANES) {
-        T va, vb;
-        int ia, ib;
-        halves_of<D>(v, va, vb);
-        halves_of<D>(i, ia, ib);
-        const bool first = better(va, ia, vb, ib);
-        v = first ? va : vb;
-        i = first ? ia : ib;
-        best_of_lanes<LANES, D * 2>(v, i);
-    }
-}
 
 template <typename T>
 __host__ __device__ __forceinline__ int groups_of(int vocab) {
@@ -153,79 +201,241 @@ __global__ __launch_bounds__(kThreads) void log_prob_short(LogProbArgs<T> a) {
 #pragma unroll
         for (int i = 0; i < N; ++i) unnamed |= ((l + e * LANES) * N + i < a.vocab ? 1u : 0u) << (e * N + i);
     for (int n = 0; n < a.k; ++n) {
-        T bv = -INFINITY;
-        int at = 0x7fffffff, slot = 0;
+        Entry<T> best = Entry<T>::none();
+        int slot = 0;
 #pragma unroll
         for (int e = 0; e < E; ++e)
 #pragma unroll
             for (int i = 0; i < N; ++i) {
-                const T w = ranked(v[e][i]);
-                const bool take = (unnamed >> (e * N + i) & 1) && (w > bv || at == 0x7fffffff);
-                bv = take ? w : bv;
-                at = take ? (l + e * LANES) * N + i : at;
+                const Entry<T> w = Entry<T>::of(v[e][i], (l + e * LANES) * N + i);
+                const bool take = (unnamed >> (e * N + i) & 1) && w.better(best);
+                best = Entry<T>::either(take, w, best);
                 slot = take ? e * N + i : slot;
             }
-        const int mine = at;
-        best_of_lanes<LANES>(bv, at);
+        const int mine = best.position();
+        best = best_of_lanes<LANES>(best);
+        const int at = best.position();
         if (mine == at) unnamed &= ~(1u << slot);
         if (l == 0 && row < a.rows) {
+            const T bv = best.value();
             a.top[r * a.k + n] = q.nothing ? T(-INFINITY) : bv == T(-INFINITY) ? x[at] - q.lse : bv - q.lse;
             a.top_tokens[r * a.k + n] = at;
         }
     }
 }
 
-constexpr int kList = 512;   // entries that may be ranked at once
-constexpr int kQuads = kThreads / 4;
+constexpr int kList = 512;    // entries that are ranked at once
+constexpr int kMerge = 64;    // segments of a row, one to a lane of the wave that joins them
+constexpr int kByQuads = 48;  // up to so many alternatives, 64 quads of threads bound them; beyond, the threads themselves
 
-// The k best of `n` entries in LDS, in order: an entry's place is the number of better ones
-template <typename T, typename Put>
-__device__ __forceinline__ void rank_list(const T* value, const int* position, int n, int k, Put put) {
-    for (int i = threadIdx.x; i < n; i += kThreads) {
-        const T v = value[i];
-        const int p = position[i];
-        int place = 0;
-        for (int j = 0; j < n; ++j) place += better(value[j], position[j], v, p) ? 1 : 0;
-        if (place < k) put(place, v, p);
+// The running sums of a row or a part of it: the maximum, the weights relative to it and their product with the exponents
+template <typename T>
+struct Sums {
+    T m = Real<T>::lowest, s = 0, t = 0;
+    __device__ __forceinline__ void raise(T to) {
+        const T by = Max()(m - to, Real<T>::under), w = Real<T>::weight(by);
+        t = w * (t + by * s);
+        s *= w;
+        m = to;
+    }
+    __device__ __forceinline__ void add(T v) {
+        const T d = v - m, w = Real<T>::weight(d);
+        s += w;
+        t += w * Max()(d, Real<T>::under);
+    }
+    __device__ __forceinline__ void over_wave() {
+        raise(fold_lanes<64>(m, Max()));
+        s = fold_lanes<64>(s, Sum());
+        t = fold_lanes<64>(t, Sum());
+    }
+    __device__ __forceinline__ void join(Sums o) {
+        const T high = Max()(m, o.m);
+        raise(high);
+        o.raise(high);
+        s += o.s;
+        t += o.t;
+    }
+};
+
+// What the workgroups of the long forms share
+template <typename T, bool TOP>
+struct Shared {
+    T sums[kThreads / 64][3];
+    unsigned arrived;
+    int count;
+    Entry<T> list[TOP ? kList : 1], key[TOP ? kThreads : 1], bound;
+    int unit[TOP ? DALI_HIP_MAX_ALTERNATIVES : 1];
+};
+
+template <typename T, bool TOP>
+__device__ __forceinline__ void over_block(Sums<T>& q, Shared<T, TOP>& sh) {
+    q.over_wave();
+    if ((threadIdx.x & 63) == 0) {
+        T* p = sh.sums[threadIdx.x >> 6];
+        p[0] = q.m, p[1] = q.s, p[2] = q.t;
+    }
+    __syncthreads();
+    q.m = sh.sums[0][0], q.s = sh.sums[0][1], q.t = sh.sums[0][2];
+#pragma unroll
+    for (int w = 1; w < kThreads / 64; ++w) {
+        Sums<T> o;
+        o.m = sh.sums[w][0], o.s = sh.sums[w][1], o.t = sh.sums[w][2];
+        q.join(o);
     }
 }
 
-// One workgroup per row, or per segment of a row: a thread walks its groups once with a running maximum, the sum of weights below it and the sum of weights
-// times exponents, which are rescaled when the maximum rises (once per four groups). For the alternatives it also keeps its best group. Of the k units (quads of threads,
-// or threads where more than 16 alternatives are asked for) with the best groups, the k-th best group's value and position bound the k best entries from below, and
-// entries above that bound lie in those units alone: they are read again, what passes the bound is collected and ranked.
+// The k best groups of 64 units (quads of threads, or threads), from each thread's best group: the k-th of them is sh.bound, the units are sh.unit. The k best
+// entries of all are no worse than the bound (k groups hold an entry that good) and lie in those units (of any other unit every entry is worse).
+template <typename T>
+__device__ __forceinline__ void find_bound(Entry<T> mine, int k, Shared<T, true>& sh) {
+    const int tid = threadIdx.x;
+    if (k <= kByQuads) {
+        mine = best_of_lanes<4>(mine);
+        if ((tid & 3) == 0) sh.key[tid >> 2] = mine;
+        if (tid == 0) sh.count = 0;
+        __syncthreads();
+        if (tid < 64) {
+            const Entry<T> e = sh.key[tid];
+            const int place = place_in_wave(e);
+            if (place < k) sh.unit[place] = tid;
+            if (place == k - 1) sh.bound = e;
+        }
+    } else {
+        sh.key[tid] = mine;
+        if (tid == 0) sh.count = 0;
+        __syncthreads();
+        int place = 0;
+#pragma unroll 8
+        for (int i = 0; i < kThreads; ++i) place += sh.key[i].better(mine) ? 1 : 0;
+        if (place < k) sh.unit[place] = tid;
+        if (place == k - 1) sh.bound = mine;
+    }
+    __syncthreads();
+}
+
+// the entries of group g that pass the bound join the list
+template <typename T>
+__device__ __forceinline__ void collect(const T (&v)[Vec<T>::N], int g, int vocab, const Entry<T>& bound, Shared<T, true>& sh) {
+#pragma unroll
+    for (int e = 0; e < Vec<T>::N; ++e) {
+        // (the bound's position is a group's: any of its entries may be the one)
+        const Entry<T> w = Entry<T>::of(v[e], g);
+        if (g * Vec<T>::N + e < vocab && !bound.better(w)) {
+            const int slot = atomicAdd(&sh.count, 1);
+            if (slot < kList) sh.list[slot] = Entry<T>::of(v[e], g * Vec<T>::N + e);
+        }
+    }
+}
+
+// The k best of `n` entries of the list, in order: an entry's place is the number of better ones
+template <typename T, typename Put>
+__device__ __forceinline__ void rank_list(const Shared<T, true>& sh, int n, int k, Put put) {
+    for (int i = threadIdx.x; i < n; i += kThreads) {
+        const Entry<T> e = sh.list[i];
+        int place = 0;
+#pragma unroll 8
+        for (int j = 0; j < n; ++j) place += sh.list[j].better(e) ? 1 : 0;
+        if (place < k) put(place, e);
+    }
+}
+
+template <typename T>
+__device__ __forceinline__ void write_alternative(const LogProbArgs<T>& a, long r, const T* x, const RowResult<T>& q, int place, const Entry<T>& e) {
+    const T v = e.value();
+    const int p = e.position();
+    // (a NaN was ranked as -inf)
+    a.top[r * a.k + place] = q.nothing ? T(-INFINITY) : v == T(-INFINITY) ? x[p] - q.lse : v - q.lse;
+    a.top_tokens[r * a.k + place] = p;
+}
+
+// So many of the best side by side in few units that the list does not hold them: one after the other over all groups, into the list
+template <typename T>
+__device__ __forceinline__ void one_by_one(const LogProbArgs<T>& a, const T* x, int begin, int end, Shared<T, true>& sh) {
+    Entry<T> last = Entry<T>::none();
+    for (int n = 0; n < a.k; ++n) {
+        Entry<T> best = Entry<T>::none();
+        for (long c = (long)begin * Vec<T>::N + threadIdx.x; c < min((long)a.vocab, (long)end * Vec<T>::N); c += kThreads) {
+            const Entry<T> w = Entry<T>::of(x[c], (int)c);
+            if ((n == 0 || last.better(w)) && w.better(best)) best = w;
+        }
+        best = best_of_lanes<64>(best);
+        __syncthreads();
+        if ((threadIdx.x & 63) == 0) sh.key[threadIdx.x >> 6] = best;
+        __syncthreads();
+        for (int w = 0; w < kThreads / 64; ++w)
+            if (sh.key[w].better(best)) best = sh.key[w];
+        if (threadIdx.x == 0) sh.list[n] = best;
+        last = best;
+    }
+    __syncthreads();
+}
+
+// The end of a row: straight to the results, or by way of the workspace where the row has several segments, whose last workgroup joins them. `found` entries
+// of the list hold the k best of the segment.
+template <typename T, bool TOP>
+__device__ __forceinline__ void finish(const LogProbArgs<T>& a, long r, int segment, const T* x, Sums<T> q, int found, int token, T own, Shared<T, TOP>& sh) {
+    const int tid = threadIdx.x;
+    if (a.segments == 1) {
+        const RowResult<T> done = result_of(q.m, q.s);
+        if (tid == 0) write_row(a, r, done, q.s, q.t, token, own);
+        if constexpr (TOP) rank_list(sh, found, a.k, [&](int place, const Entry<T>& e) { write_alternative(a, r, x, done, place, e); });
+        return;
+    }
+    const long cell = r * a.segments + segment;
+    if (tid == 0) {
+        publish(a.sums + cell * 3, q.m);
+        publish(a.sums + cell * 3 + 1, q.s);
+        publish(a.sums + cell * 3 + 2, q.t);
+    }
+    if constexpr (TOP) rank_list(sh, found, a.k, [&](int place, const Entry<T>& e) { e.publish(a.best + cell * a.k + place); });
+    if (!last_to_arrive(a.counters + r * a.counter_step, (unsigned)a.segments, &sh.arrived)) return;
+    if constexpr (TOP)
+        for (int i = tid; i < a.segments * a.k; i += kThreads) sh.list[i] = Entry<T>::observe(a.best + r * a.segments * a.k + i);
+    Sums<T> all;
+    if ((tid & 63) < a.segments) {
+        const T* p = a.sums + (r * a.segments + (tid & 63)) * 3;
+        all.m = observe(p), all.s = observe(p + 1), all.t = observe(p + 2);
+    }
+    all.over_wave();
+    const RowResult<T> done = result_of(all.m, all.s);
+    if (tid == 0) write_row(a, r, done, all.s, all.t, token, own);
+    if constexpr (TOP) {
+        __syncthreads();
+        if (tid >= 64) return;
+        // the segments' lists are in order: a lane stands at the head of one, and the best head is next
+        int at = 0;
+        Entry<T> head = tid < a.segments ? sh.list[tid * a.k] : Entry<T>::none(), kept = Entry<T>::none();
+        for (int n = 0; n < a.k; ++n) {
+            const Entry<T> best = best_of_lanes<64>(head);
+            if (n == tid) kept = best;
+            if (tid < a.segments && !best.better(head)) head = ++at < a.k ? sh.list[tid * a.k + at] : Entry<T>::none();
+        }
+        if (tid < a.k) write_alternative(a, r, x, done, tid, kept);
+    }
+}
+
+// One workgroup per row, or per segment of a row: a thread walks its groups once with running sums, which are rescaled when the maximum rises (once per four
+// groups), and its best group. What passes the bound that the best groups give lies in k units; their groups are read again and collected.
 template <typename T, bool TOP>
 __global__ __launch_bounds__(kThreads) void log_prob_long(LogProbArgs<T> a) {
     constexpr int N = Vec<T>::N, U = 4;
-    __shared__ T scratch[4], list[kList], key[TOP ? kThreads : 1], bound;
-    __shared__ int places[kList], group[TOP ? kThreads : 1], unit[TOP ? DALI_HIP_MAX_ALTERNATIVES : 1], bound_group, count;
-    __shared__ unsigned arrived;
-    const int tid = threadIdx.x, lane = tid & 63;
+    __shared__ Shared<T, TOP> sh;
+    const int tid = threadIdx.x;
     const long r = blockIdx.x / (unsigned)a.segments;
     const int segment = (int)(blockIdx.x - (unsigned)r * (unsigned)a.segments);
     const T* x = a.logits + r * a.stride;
     const int groups = groups_of<T>(a.vocab), begin = segment * a.per, end = min(groups, begin + a.per), whole = min(end, a.vocab / N);
     const int token = a.tokens[r];
     const T own = token >= 0 && token < a.vocab ? x[token] : T(0);
-    T m = Real<T>::lowest, s = 0, t = 0, top = -INFINITY;
-    int top_group = begin + tid < end ? begin + tid : 0x7fffffff;
-    auto raise = [&](T to) {
-        const T by = Max()(m - to, Real<T>::under), w = Real<T>::weight(by);
-        t = w * (t + by * s);
-        s *= w;
-        m = to;
-    };
-    auto add = [&](T v) {
-        const T d = v - m, w = Real<T>::weight(d);
-        s += w;
-        t += w * Max()(d, Real<T>::under);
-    };
+    Sums<T> q;
+    T top = -INFINITY;
+    int top_group = begin + tid;
     int j = begin + tid;
     for (; j + (U - 1) * kThreads < whole; j += U * kThreads) {
         typename Vec<T>::type v[U];
 #pragma unroll
         for (int u = 0; u < U; ++u) v[u] = *reinterpret_cast<const typename Vec<T>::type*>(x + (long)(j + u * kThreads) * N);
-        T high = m;
+        T high = q.m;
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             T g = v[u][0];
@@ -234,11 +444,11 @@ __global__ __launch_bounds__(kThreads) void log_prob_long(LogProbArgs<T> a) {
             high = Max()(high, g);
             if (TOP && g > top) top = g, top_group = j + u * kThreads;
         }
-        raise(high);
+        q.raise(high);
 #pragma unroll
         for (int u = 0; u < U; ++u)
 #pragma unroll
-            for (int i = 0; i < N; ++i) add(v[u][i]);
+            for (int i = 0; i < N; ++i) q.add(v[u][i]);
     }
     for (; j < end; j += kThreads) {
         T v[N];
@@ -247,133 +457,86 @@ __global__ __launch_bounds__(kThreads) void log_prob_long(LogProbArgs<T> a) {
 #pragma unroll
         for (int i = 1; i < N; ++i) g = Max()(g, v[i]);
         if (TOP && g > top) top = g, top_group = j;
-        raise(Max()(m, g));
+        q.raise(Max()(q.m, g));
 #pragma unroll
-        for (int i = 0; i < N; ++i) add(v[i]);
+        for (int i = 0; i < N; ++i) q.add(v[i]);
     }
-    // the workgroup's sums
-    const T mine = m;
-    m = fold_block<kThreads>(m, scratch, Max());
-    {
-        const T by = Max()(mine - m, Real<T>::under), w = Real<T>::weight(by);
-        t = block_sum<kThreads>(w * (t + by * s), scratch);
-        s = block_sum<kThreads>(w * s, scratch);
-    }
+    over_block(q, sh);
     int found = 0;
     if constexpr (TOP) {
-        const bool quads = a.k <= 16;
-        if (quads) {
-            best_of_lanes<4>(top, top_group);
-            if ((tid & 3) == 0) key[tid >> 2] = top, group[tid >> 2] = top_group;
-        } else {
-            key[tid] = top, group[tid] = top_group;
-        }
-        if (tid == 0) count = 0;
-        __syncthreads();
-        if (quads) {
-            if (tid < 64) {
-                T kv = key[lane];
-                int kg = group[lane];
-                for (int n = 0; n < a.k; ++n) {
-                    T bv = kv;
-                    int bg = kg;
-                    best_of_lanes<64>(bv, bg);
-                    if (kg == bg) {  // (a group belongs to one unit)
-                        unit[n] = lane;
-                        if (n == a.k - 1) bound = bv, bound_group = bg;
-                        kv = -INFINITY, kg = 0x7fffffff;
-                    }
-                }
-            }
-        } else {
-            int place = 0;
-            for (int i = 0; i < kThreads; ++i) place += better(key[i], group[i], top, top_group) ? 1 : 0;
-            if (place < a.k) unit[place] = tid;
-            if (place == a.k - 1) bound = top, bound_group = top_group;
-        }
-        __syncthreads();
-        // the units' entries again
-        const T low = bound;
-        const int low_group = bound_group, wide = quads ? 4 : 1, walks = (end - begin + kThreads - 1) / kThreads * wide;
+        find_bound(begin + tid < end ? Entry<T>::of(top, top_group) : Entry<T>::none(), a.k, sh);
+        const Entry<T> bound = sh.bound;
+        const int wide = a.k <= kByQuads ? 4 : 1, walks = (end - begin + kThreads - 1) / kThreads * wide;
         for (int i = tid; i < a.k * walks; i += kThreads) {
             const int n = i / walks, step = i - n * walks;
-            const int g = begin + unit[n] * wide + (quads ? (step & 3) + (step >> 2) * kThreads : step * kThreads);
+            const int g = begin + sh.unit[n] * wide + (wide == 4 ? (step & 3) + (step >> 2) * kThreads : step * kThreads);
             if (g >= end) continue;
             T v[N];
             load_group(x, g * N, a.vocab, v);
-#pragma unroll
-            for (int e = 0; e < N; ++e) {
-                const T w = ranked(v[e]);
-                if (g * N + e < a.vocab && (w > low || (w == low && g <= low_group))) {
-                    const int slot = atomicAdd(&count, 1);
-                    if (slot < kList) list[slot] = w, places[slot] = g * N + e;
-                }
-            }
+            collect(v, g, a.vocab, bound, sh);
         }
         __syncthreads();
-        found = count;
+        found = sh.count;
         if (found > kList) {
-            // (so many of the best side by side in few units: one after the other over the whole segment)
-            T last = INFINITY;
-            int last_at = -1;
-            for (int n = 0; n < a.k; ++n) {
-                T bv = -INFINITY;
-                int at = 0x7fffffff;
-                for (long c = (long)begin * N + tid; c < min((long)a.vocab, (long)end * N); c += kThreads) {
-                    const T w = ranked(x[c]);
-                    if (better(last, last_at, w, (int)c) && better(w, (int)c, bv, at)) bv = w, at = (int)c;
-                }
-                best_of_lanes<64>(bv, at);
-                __syncthreads();
-                if (lane == 0) key[tid >> 6] = bv, group[tid >> 6] = at;
-                __syncthreads();
-                for (int w = 0; w < kThreads / 64; ++w)
-                    if (better(key[w], group[w], bv, at)) bv = key[w], at = group[w];
-                if (tid == 0) list[n] = bv, places[n] = at;
-                last = bv;
-                last_at = at;
-            }
+            one_by_one(a, x, begin, end, sh);
             found = a.k;
-            __syncthreads();
         }
     }
-    if (a.segments > 1) {
-        const long cell = r * a.segments + segment;
-        if (tid == 0) {
-            publish(a.sums + cell * 3, m);
-            publish(a.sums + cell * 3 + 1, s);
-            publish(a.sums + cell * 3 + 2, t);
+    finish(a, r, segment, x, q, found, token, own, sh);
+}
+
+// Segments that a workgroup holds in registers, E groups to a thread: all of them are loaded at once and nothing is read again.
+template <typename T, bool TOP, int E>
+__global__ __launch_bounds__(kThreads) void log_prob_segments(LogProbArgs<T> a) {
+    constexpr int N = Vec<T>::N;
+    __shared__ Shared<T, TOP> sh;
+    const int tid = threadIdx.x;
+    const long r = blockIdx.x / (unsigned)a.segments;
+    const int segment = (int)(blockIdx.x - (unsigned)r * (unsigned)a.segments);
+    const T* x = a.logits + r * a.stride;
+    const int begin = segment * a.per, end = min(groups_of<T>(a.vocab), begin + a.per);
+    T v[E][N];
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+        const int g = begin + tid + e * kThreads;
+        load_group(x, g < end ? g * N : a.vocab, a.vocab, v[e]);
+    }
+    const int token = a.tokens[r];
+    const T own = token >= 0 && token < a.vocab ? x[token] : T(0);
+    Sums<T> q;
+    T top = -INFINITY, high = q.m;
+    int top_group = begin + tid;
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+        T g = v[e][0];
+#pragma unroll
+        for (int i = 1; i < N; ++i) g = Max()(g, v[e][i]);
+        high = Max()(high, g);
+        if (TOP && g > top) top = g, top_group = begin + tid + e * kThreads;
+    }
+    q.m = high;
+#pragma unroll
+    for (int e = 0; e < E; ++e)
+#pragma unroll
+        for (int i = 0; i < N; ++i) q.add(v[e][i]);
+    over_block(q, sh);
+    int found = 0;
+    if constexpr (TOP) {
+        find_bound(begin + tid < end ? Entry<T>::of(top, top_group) : Entry<T>::none(), a.k, sh);
+        const Entry<T> bound = sh.bound;
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            const int g = begin + tid + e * kThreads;
+            if (g < end) collect(v[e], g, a.vocab, bound, sh);
         }
-        if constexpr (TOP)
-            rank_list(list, places, found, a.k, [&](int place, T v, int p) {
-                publish(a.best + cell * a.k + place, v);
-                publish(a.positions + cell * a.k + place, p);
-            });
-        if (!last_to_arrive(a.counters + r * a.counter_step, (unsigned)a.segments, &arrived)) return;
-        // the row's sums and candidates, from all segments
-        const T* sums = a.sums + r * a.segments * 3;
-        const bool have = lane < a.segments;
-        m = have ? observe(sums + lane * 3) : Real<T>::lowest;
-        s = have ? observe(sums + lane * 3 + 1) : T(0);
-        t = have ? observe(sums + lane * 3 + 2) : T(0);
-        if constexpr (TOP) {
-            found = a.segments * a.k;
-            for (int i = tid; i < found; i += kThreads) list[i] = observe(a.best + r * found + i), places[i] = observe(a.positions + r * found + i);
-        }
-        const T part = m;
-        m = fold_lanes<64>(m, Max());
-        const T by = Max()(part - m, Real<T>::under), w = Real<T>::weight(by);
-        t = fold_lanes<64>(w * (t + by * s), Sum());
-        s = fold_lanes<64>(w * s, Sum());
         __syncthreads();
+        found = sh.count;
+        if (found > kList) {
+            one_by_one(a, x, begin, end, sh);
+            found = a.k;
+        }
     }
-    const RowResult<T> q = result_of(m, s);
-    if (tid == 0) write_row(a, r, q, s, t, token, own);
-    if constexpr (TOP)
-        rank_list(list, places, found, a.k, [&](int place, T v, int p) {
-            a.top[r * a.k + place] = q.nothing ? T(-INFINITY) : v == T(-INFINITY) ? x[p] - q.lse : v - q.lse;
-            a.top_tokens[r * a.k + place] = p;
-        });
+    finish(a, r, segment, x, q, found, token, own, sh);
 }
 
 template <typename T>
@@ -498,21 +661,26 @@ int forward(LogProbArgs<T> all) {
             });
             continue;
         }
-        // Few rows are cut into segments of at least 512 groups, two for a thread, until there are 512 workgroups or so; their candidates are ranked in one list
-        const long cut = std::min({512L / a.rows, (long)groups / 512, (long)kList / std::max(a.k, 1), 64L});
+        // Few rows are cut into segments of at least 512 groups, two for a thread, until there are 512 workgroups or so. The segments' alternatives are joined in one
+        // list, and a lane of one wave stands for a segment.
+        const long cut = std::min({512L / a.rows, (long)groups / 512, (long)kList / std::max(a.k, 1), (long)kMerge});
         if (cut > 1) {
             a.segments = (int)cut;
             a.per = (groups + a.segments - 1) / a.segments;
             a.segments = (groups + a.per - 1) / a.per;
             a.counters = (unsigned*)workspace();
             a.counter_step = counter_step(a.rows);
-            a.sums = (T*)(workspace() + kWorkspaceCounterBytes);
-            a.best = a.sums + a.rows * a.segments * 3;
-            a.positions = (int*)(a.best + a.rows * a.segments * a.k);
+            a.best = (Entry<T>*)(workspace() + kWorkspaceCounterBytes);
+            a.sums = (T*)(a.best + a.rows * a.segments * a.k);
         }
         const dim3 grid((unsigned)(a.rows * a.segments));
-        if (a.k) hipLaunchKernelGGL((log_prob_long<T, true>), grid, dim3(kThreads), 0, stream(), a);
-        else hipLaunchKernelGGL((log_prob_long<T, false>), grid, dim3(kThreads), 0, stream(), a);
+        auto launch = [&](auto top) {
+            constexpr bool TOP = decltype(top)::value;
+            if (a.per <= 4 * kThreads) hipLaunchKernelGGL((log_prob_segments<T, TOP, 4>), grid, dim3(kThreads), 0, stream(), a);
+            else hipLaunchKernelGGL((log_prob_long<T, TOP>), grid, dim3(kThreads), 0, stream(), a);
+        };
+        if (a.k) launch(std::true_type());
+        else launch(std::false_type());
     }
     return launched("dali_hip_token_log_probs");
 }
