@@ -33,6 +33,12 @@ struct Real<double> {
     static __device__ __forceinline__ double ln(double s) { return log(s); }
 };
 
+// a NaN counts as -inf among the alternatives
+template <typename T>
+__device__ __forceinline__ T ranked(T v) {
+    return Max()(v, T(-INFINITY));
+}
+
 // An entry of a row (or the best of a group of entries, by the group's number): of two the better has the larger value, or among equals the lower position. A NaN
 // counts as -inf. Of fp32 it is one whole number that grows with the value and falls with the position; there a zero is a zero of either sign.
 template <typename T>
@@ -162,13 +168,132 @@ __device__ __forceinline__ void write_row(const LogProbArgs<T>& a, long r, const
     a.log_probs[r] = token < 0 || token >= a.vocab ? T(0) : q.nothing ? T(-INFINITY) : (own - q.m) - q.ln;
 }
 
-// Rows that LANES lanes hold in registers, E groups each: every statistic is exact after one reading, and an alternative is one fold over what is left.
-template <typename T, int LANES, int E>
+template <typename T>
+__device__ __forceinline__ void write_alternative(const LogProbArgs<T>& a, long r, const T* x, const RowResult<T>& q, int place, const Entry<T>& e) {
+    const T v = e.value();
+    const int p = e.position();
+    // (a NaN was ranked as -inf)
+    a.top[r * a.k + place] = q.nothing ? T(-INFINITY) : v == T(-INFINITY) ? x[p] - q.lse : v - q.lse;
+    a.top_tokens[r * a.k + place] = p;
+}
+
+// Entries of one wave that are ranked at once
+constexpr int kWaveList = 128;
+
+// The k best of the entries that a wave holds in registers, E groups to a lane, E > 1: the k-th best of the lanes' own best bounds them, what passes it is collected
+// and ranked. False where the list does not hold them.
+template <typename T, int E, typename Put>
+__device__ __forceinline__ bool best_by_bound(const T (&v)[E][Vec<T>::N], int l, int vocab, int k, Entry<T>* list, int* count, Put put) {
+    constexpr int N = Vec<T>::N;
+    T top = -INFINITY;
+    int at = l * N;
+#pragma unroll
+    for (int e = 0; e < E; ++e)
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+            if (v[e][i] > top) top = v[e][i], at = (l + e * 64) * N + i;
+    const Entry<T> mine = l * N < vocab ? Entry<T>::of(top, at) : Entry<T>::none();
+    const unsigned long long last = __ballot(place_in_wave(mine) == k - 1);
+    const Entry<T> bound = mine.lane(__builtin_ctzll(last));
+    const T low = bound.value();
+    if (l == 0) *count = 0;
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+#pragma unroll
+    for (int e = 0; e < E; ++e)
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            if (ranked(v[e][i]) < low) continue;
+            const int c = (l + e * 64) * N + i;
+            const Entry<T> w = Entry<T>::of(v[e][i], c);
+            if (c < vocab && !bound.better(w)) {
+                const int slot = atomicAdd(count, 1);
+                if (slot < kWaveList) list[slot] = w;
+            }
+        }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    const int n = __builtin_amdgcn_readfirstlane(*(volatile int*)count);
+    if (n > kWaveList) return false;
+    for (int i = l; i < n; i += 64) {
+        const Entry<T> e = list[i];
+        int place = 0;
+#pragma unroll 4
+        for (int j = 0; j < n; ++j) place += list[j].better(e) ? 1 : 0;
+        if (place < k) put(place, e);
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    return true;
+}
+
+// One alternative after the other of the entries that LANES lanes hold: an entry that has been named is no longer free
+template <typename T, int LANES, int E, typename Put>
+__device__ __forceinline__ void best_one_by_one(const T (&v)[E][Vec<T>::N], int l, int vocab, int k, Put put) {
+    constexpr int N = Vec<T>::N;
+    unsigned long long unnamed = 0;
+#pragma unroll
+    for (int e = 0; e < E; ++e)
+#pragma unroll
+        for (int i = 0; i < N; ++i) unnamed |= ((l + e * LANES) * N + i < vocab ? 1ull : 0ull) << (e * N + i);
+    for (int n = 0; n < k; ++n) {
+        Entry<T> best = Entry<T>::none();
+        int slot = 0;
+#pragma unroll
+        for (int e = 0; e < E; ++e)
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                const Entry<T> w = Entry<T>::of(v[e][i], (l + e * LANES) * N + i);
+                const bool take = (unnamed >> (e * N + i) & 1) && w.better(best);
+                best = Entry<T>::either(take, w, best);
+                slot = take ? e * N + i : slot;
+            }
+        const int mine = best.position();
+        best = best_of_lanes<LANES>(best);
+        if (mine == best.position()) unnamed &= ~(1ull << slot);
+        if (l == 0) put(n, best);
+    }
+}
+
+// The same for fp32 rows of one group to a lane, where the lanes lie in the order of the positions: each orders its four once, and the next alternative is the
+// head of the first lane whose head is the largest of all heads.
+template <int LANES, typename Put>
+__device__ __forceinline__ void best_by_heads(const float (&v)[1][4], int l, int vocab, int k, Put put) {
+    unsigned key[4];
+    int at[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        key[i] = l * 4 + i < vocab ? (unsigned)(Entry<float>::of(v[0][i], 0).key >> 32) : 0u;  // (0 is worse than any entry's)
+        at[i] = l * 4 + i;
+    }
+    auto order = [&](int i, int j) {
+        const bool swap = key[j] > key[i] || (key[j] == key[i] && at[j] < at[i]);
+        const unsigned hi = swap ? key[j] : key[i], lo = swap ? key[i] : key[j];
+        const int p = swap ? at[j] : at[i], q = swap ? at[i] : at[j];
+        key[i] = hi, key[j] = lo, at[i] = p, at[j] = q;
+    };
+    order(0, 1), order(2, 3), order(0, 2), order(1, 3), order(1, 2);
+    const int lane = threadIdx.x & 63, base = lane & ~(LANES - 1);
+    const unsigned long long team = (LANES == 64 ? ~0ull : ((1ull << (LANES % 64)) - 1)) << base;
+    for (int n = 0; n < k; ++n) {
+        const unsigned high = fold_lanes<LANES>(key[0], [](unsigned a, unsigned b) { return a > b ? a : b; });
+        const bool first = __builtin_ctzll(__ballot(key[0] == high) & team) == lane;
+        if (first) {
+            put(n, Entry<float>{(unsigned long long)key[0] << 32 | (0xffffffffu - (unsigned)at[0])});
+            key[0] = key[1], key[1] = key[2], key[2] = key[3], key[3] = 0;
+            at[0] = at[1], at[1] = at[2], at[2] = at[3];
+        }
+    }
+}
+
+// Rows that LANES lanes hold in registers, E groups each: every statistic is exact after one reading.
+template <typename T, int LANES, int E, bool TOP>
 __global__ __launch_bounds__(kThreads) void log_prob_short(LogProbArgs<T> a) {
     constexpr int N = Vec<T>::N;
+    constexpr bool LIST = TOP && E > 1;
+    __shared__ Entry<T> lists[LIST ? kThreads / 64 : 1][LIST ? kWaveList : 1];
+    __shared__ int counts[LIST ? kThreads / 64 : 1];
     const int l = threadIdx.x % LANES;
     const long row = (long)blockIdx.x * (kThreads / LANES) + threadIdx.x / LANES;
-    const long r = row < a.rows ? row : a.rows - 1;  // (lanes without a row go along with the last)
+    const bool live = row < a.rows;
+    const long r = live ? row : a.rows - 1;  // (lanes without a row go along with the last)
     const T* x = a.logits + r * a.stride;
     T v[E][N];
 #pragma unroll
@@ -193,40 +318,25 @@ __global__ __launch_bounds__(kThreads) void log_prob_short(LogProbArgs<T> a) {
     s = fold_lanes<LANES>(s, Sum());
     t = fold_lanes<LANES>(t, Sum());
     const RowResult<T> q = result_of(m, s);
-    if (l == 0 && row < a.rows) write_row(a, r, q, s, t, token, own);
-    // one alternative after the other; an entry that has been named is no longer free
-    unsigned unnamed = 0;
-#pragma unroll
-    for (int e = 0; e < E; ++e)
-#pragma unroll
-        for (int i = 0; i < N; ++i) unnamed |= ((l + e * LANES) * N + i < a.vocab ? 1u : 0u) << (e * N + i);
-    for (int n = 0; n < a.k; ++n) {
-        Entry<T> best = Entry<T>::none();
-        int slot = 0;
-#pragma unroll
-        for (int e = 0; e < E; ++e)
-#pragma unroll
-            for (int i = 0; i < N; ++i) {
-                const Entry<T> w = Entry<T>::of(v[e][i], (l + e * LANES) * N + i);
-                const bool take = (unnamed >> (e * N + i) & 1) && w.better(best);
-                best = Entry<T>::either(take, w, best);
-                slot = take ? e * N + i : slot;
-            }
-        const int mine = best.position();
-        best = best_of_lanes<LANES>(best);
-        const int at = best.position();
-        if (mine == at) unnamed &= ~(1u << slot);
-        if (l == 0 && row < a.rows) {
-            const T bv = best.value();
-            a.top[r * a.k + n] = q.nothing ? T(-INFINITY) : bv == T(-INFINITY) ? x[at] - q.lse : bv - q.lse;
-            a.top_tokens[r * a.k + n] = at;
+    if (l == 0 && live) write_row(a, r, q, s, t, token, own);
+    if constexpr (TOP) {
+        auto put = [&](int place, const Entry<T>& e) {
+            if (live) write_alternative(a, r, x, q, place, e);
+        };
+        if constexpr (E == 1 && sizeof(T) == 4) {
+            best_by_heads<LANES>(v, l, a.vocab, a.k, put);
+        } else if constexpr (E == 1) {
+            best_one_by_one<T, LANES, E>(v, l, a.vocab, a.k, put);
+        } else {
+            const int wave = threadIdx.x >> 6;
+            if (a.k <= 2 || !best_by_bound<T, E>(v, l, a.vocab, a.k, lists[wave], &counts[wave], put)) best_one_by_one<T, LANES, E>(v, l, a.vocab, a.k, put);
         }
     }
 }
 
 constexpr int kList = 512;    // entries that are ranked at once
 constexpr int kMerge = 64;    // segments of a row, one to a lane of the wave that joins them
-constexpr int kByQuads = 48;  // up to so many alternatives, 64 quads of threads bound them; beyond, the threads themselves
+constexpr int kByQuads = 32;  // up to so many alternatives, the best of 64 quads of threads bound them; beyond, those of the threads themselves
 
 // The running sums of a row or a part of it: the maximum, the weights relative to it and their product with the exponents
 template <typename T>
@@ -262,9 +372,9 @@ template <typename T, bool TOP>
 struct Shared {
     T sums[kThreads / 64][3];
     unsigned arrived;
-    int count;
+    int count, units;
     Entry<T> list[TOP ? kList : 1], key[TOP ? kThreads : 1], bound;
-    int unit[TOP ? DALI_HIP_MAX_ALTERNATIVES : 1];
+    int unit[TOP ? kThreads : 1];
 };
 
 template <typename T, bool TOP>
@@ -284,40 +394,38 @@ __device__ __forceinline__ void over_block(Sums<T>& q, Shared<T, TOP>& sh) {
     }
 }
 
-// The k best groups of 64 units (quads of threads, or threads), from each thread's best group: the k-th of them is sh.bound, the units are sh.unit. The k best
-// entries of all are no worse than the bound (k groups hold an entry that good) and lie in those units (of any other unit every entry is worse).
+// The k-th best of the best groups that the quads of threads hold (or the threads): k groups have an entry that good, so the k best entries of all are no worse
 template <typename T>
-__device__ __forceinline__ void find_bound(Entry<T> mine, int k, Shared<T, true>& sh) {
+__device__ __forceinline__ Entry<T> find_bound(const Entry<T>& mine, int k, Shared<T, true>& sh) {
     const int tid = threadIdx.x;
+    if (tid == 0) sh.count = sh.units = 0;
     if (k <= kByQuads) {
-        mine = best_of_lanes<4>(mine);
-        if ((tid & 3) == 0) sh.key[tid >> 2] = mine;
-        if (tid == 0) sh.count = 0;
+        const Entry<T> quad = best_of_lanes<4>(mine);
+        if ((tid & 3) == 0) sh.key[tid >> 2] = quad;
         __syncthreads();
         if (tid < 64) {
             const Entry<T> e = sh.key[tid];
-            const int place = place_in_wave(e);
-            if (place < k) sh.unit[place] = tid;
-            if (place == k - 1) sh.bound = e;
+            if (place_in_wave(e) == k - 1) sh.bound = e;
         }
     } else {
         sh.key[tid] = mine;
-        if (tid == 0) sh.count = 0;
         __syncthreads();
         int place = 0;
 #pragma unroll 8
         for (int i = 0; i < kThreads; ++i) place += sh.key[i].better(mine) ? 1 : 0;
-        if (place < k) sh.unit[place] = tid;
         if (place == k - 1) sh.bound = mine;
     }
     __syncthreads();
+    return sh.bound;
 }
 
 // the entries of group g that pass the bound join the list
 template <typename T>
 __device__ __forceinline__ void collect(const T (&v)[Vec<T>::N], int g, int vocab, const Entry<T>& bound, Shared<T, true>& sh) {
+    const T low = bound.value();
 #pragma unroll
     for (int e = 0; e < Vec<T>::N; ++e) {
+        if (ranked(v[e]) < low) continue;
         // (the bound's position is a group's: any of its entries may be the one)
         const Entry<T> w = Entry<T>::of(v[e], g);
         if (g * Vec<T>::N + e < vocab && !bound.better(w)) {
@@ -337,15 +445,6 @@ __device__ __forceinline__ void rank_list(const Shared<T, true>& sh, int n, int 
         for (int j = 0; j < n; ++j) place += sh.list[j].better(e) ? 1 : 0;
         if (place < k) put(place, e);
     }
-}
-
-template <typename T>
-__device__ __forceinline__ void write_alternative(const LogProbArgs<T>& a, long r, const T* x, const RowResult<T>& q, int place, const Entry<T>& e) {
-    const T v = e.value();
-    const int p = e.position();
-    // (a NaN was ranked as -inf)
-    a.top[r * a.k + place] = q.nothing ? T(-INFINITY) : v == T(-INFINITY) ? x[p] - q.lse : v - q.lse;
-    a.top_tokens[r * a.k + place] = p;
 }
 
 // So many of the best side by side in few units that the list does not hold them: one after the other over all groups, into the list
@@ -415,7 +514,7 @@ __device__ __forceinline__ void finish(const LogProbArgs<T>& a, long r, int segm
 }
 
 // One workgroup per row, or per segment of a row: a thread walks its groups once with running sums, which are rescaled when the maximum rises (once per four
-// groups), and its best group. What passes the bound that the best groups give lies in k units; their groups are read again and collected.
+// groups), and its best group. What passes the bound that the best groups give lies in the few threads whose own best passes it; their groups are read again.
 template <typename T, bool TOP>
 __global__ __launch_bounds__(kThreads) void log_prob_long(LogProbArgs<T> a) {
     constexpr int N = Vec<T>::N, U = 4;
@@ -464,12 +563,12 @@ __global__ __launch_bounds__(kThreads) void log_prob_long(LogProbArgs<T> a) {
     over_block(q, sh);
     int found = 0;
     if constexpr (TOP) {
-        find_bound(begin + tid < end ? Entry<T>::of(top, top_group) : Entry<T>::none(), a.k, sh);
-        const Entry<T> bound = sh.bound;
-        const int wide = a.k <= kByQuads ? 4 : 1, walks = (end - begin + kThreads - 1) / kThreads * wide;
-        for (int i = tid; i < a.k * walks; i += kThreads) {
-            const int n = i / walks, step = i - n * walks;
-            const int g = begin + sh.unit[n] * wide + (wide == 4 ? (step & 3) + (step >> 2) * kThreads : step * kThreads);
+        const Entry<T> mine = begin + tid < end ? Entry<T>::of(top, top_group) : Entry<T>::none(), bound = find_bound(mine, a.k, sh);
+        if (!bound.better(mine)) sh.unit[atomicAdd(&sh.units, 1)] = tid;
+        __syncthreads();
+        const int walks = (end - begin + kThreads - 1) / kThreads, all = sh.units * walks;
+        for (int i = tid; i < all; i += kThreads) {
+            const int n = i / walks, g = begin + sh.unit[n] + (i - n * walks) * kThreads;
             if (g >= end) continue;
             T v[N];
             load_group(x, g * N, a.vocab, v);
@@ -522,8 +621,7 @@ __global__ __launch_bounds__(kThreads) void log_prob_segments(LogProbArgs<T> a) 
     over_block(q, sh);
     int found = 0;
     if constexpr (TOP) {
-        find_bound(begin + tid < end ? Entry<T>::of(top, top_group) : Entry<T>::none(), a.k, sh);
-        const Entry<T> bound = sh.bound;
+        const Entry<T> bound = find_bound(begin + tid < end ? Entry<T>::of(top, top_group) : Entry<T>::none(), a.k, sh);
 #pragma unroll
         for (int e = 0; e < E; ++e) {
             const int g = begin + tid + e * kThreads;
@@ -626,23 +724,31 @@ __global__ __launch_bounds__(kThreads) void log_prob_backward_long(LogProbBackwa
     }
 }
 
-// lanes and groups per lane that hold a row of `groups` groups; false: none
-template <typename F>
+// lanes and groups per lane that hold a row of `groups` groups, up to `most` of them; false: none
+template <int MOST, typename F>
 bool short_rows(int groups, F launch) {
-    if (groups <= 8) launch(std::integral_constant<int, 8>(), std::integral_constant<int, 1>());
-    else if (groups <= 16) launch(std::integral_constant<int, 16>(), std::integral_constant<int, 1>());
-    else if (groups <= 32) launch(std::integral_constant<int, 32>(), std::integral_constant<int, 1>());
-    else if (groups <= 64) launch(std::integral_constant<int, 64>(), std::integral_constant<int, 1>());
-    else if (groups <= 128) launch(std::integral_constant<int, 64>(), std::integral_constant<int, 2>());
-    else if (groups <= 256) launch(std::integral_constant<int, 64>(), std::integral_constant<int, 4>());
-    else return false;
-    return true;
+    auto with = [&](auto lanes, auto e) {
+        launch(lanes, e);
+        return true;
+    };
+    if (groups <= 8) return with(std::integral_constant<int, 8>(), std::integral_constant<int, 1>());
+    if (groups <= 16) return with(std::integral_constant<int, 16>(), std::integral_constant<int, 1>());
+    if (groups <= 32) return with(std::integral_constant<int, 32>(), std::integral_constant<int, 1>());
+    if (groups <= 64) return with(std::integral_constant<int, 64>(), std::integral_constant<int, 1>());
+    if (groups <= 128) return with(std::integral_constant<int, 64>(), std::integral_constant<int, 2>());
+    if (groups <= 256) return with(std::integral_constant<int, 64>(), std::integral_constant<int, 4>());
+    if constexpr (MOST > 256) {
+        if (groups <= 512) return with(std::integral_constant<int, 64>(), std::integral_constant<int, 8>());
+        if (groups <= 1024) return with(std::integral_constant<int, 64>(), std::integral_constant<int, 16>());
+    }
+    return false;
 }
 
 template <typename T>
 int forward(LogProbArgs<T> all) {
     const int groups = groups_of<T>(all.vocab);
-    const bool is_short = groups <= 256;
+    // A wave per row up to 1024 groups, where there are rows enough for all waves; else a workgroup above 256
+    const bool is_short = groups <= 256 || (groups <= 1024 && all.rows >= 1024);
     // a launch numbers its workgroups in 31 bits
     for (long done = 0; done < all.rows;) {
         LogProbArgs<T> a = all;
@@ -655,9 +761,11 @@ int forward(LogProbArgs<T> all) {
         a.segments = 1;
         a.per = groups;
         if (is_short) {
-            short_rows(groups, [&](auto lanes, auto e) {
-                constexpr int per = kThreads / decltype(lanes)::value;
-                hipLaunchKernelGGL((log_prob_short<T, decltype(lanes)::value, decltype(e)::value>), dim3((unsigned)((a.rows + per - 1) / per)), dim3(kThreads), 0, stream(), a);
+            short_rows<1024>(groups, [&](auto lanes, auto e) {
+                constexpr int LANES = decltype(lanes)::value, E = decltype(e)::value, per = kThreads / LANES;
+                const dim3 grid((unsigned)((a.rows + per - 1) / per));
+                if (a.k) hipLaunchKernelGGL((log_prob_short<T, LANES, E, true>), grid, dim3(kThreads), 0, stream(), a);
+                else hipLaunchKernelGGL((log_prob_short<T, LANES, E, false>), grid, dim3(kThreads), 0, stream(), a);
             });
             continue;
         }
@@ -699,7 +807,7 @@ int backward(LogProbBackwardArgs<T> all) {
         if (a.d_entropy) a.d_entropy += done, a.entropy += done;
         done += a.rows;
         a.pieces = (int)pieces;
-        if (short_rows(groups, [&](auto lanes, auto e) {
+        if (short_rows<256>(groups, [&](auto lanes, auto e) {
                 constexpr int per = kThreads / decltype(lanes)::value;
                 hipLaunchKernelGGL((log_prob_backward_short<T, decltype(lanes)::value, decltype(e)::value>), dim3((unsigned)((a.rows + per - 1) / per)), dim3(kThreads), 0, stream(), a);
             }))
