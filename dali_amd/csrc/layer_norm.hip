@@ -6,6 +6,7 @@
 // Sums are held in the operands' own type (32 bits or more). The variance is the mean of squared distances from the mean, with the mean's own
 // rounding error taken out again (x - mean sums to delta n where the mean is off by delta): rows far from zero keep their digits.
 #include <algorithm>
+#include <type_traits>
 
 #include "row_math.h"
 
@@ -23,27 +24,150 @@ struct NormArgs {
     T epsilon;
 };
 
+// Sums over the team of TEAM threads that holds a row: lanes of a wave, or a workgroup of whole waves, which meets once per call. `scratch` has two halves that take
+// turns, so that a wave may write the next sums while another still reads these.
+template <typename T, int TEAM>
+struct TeamScratch {
+    T v[TEAM > 64 ? 2 : 1][TEAM > 64 ? TEAM / 64 : 1][2];
+};
+template <int TEAM, typename T>
+__device__ __forceinline__ void team_sum(T& p, T& q, TeamScratch<T, TEAM>& scratch, int& turn) {
+    p = fold_lanes<(TEAM < 64 ? TEAM : 64)>(p, Sum());
+    q = fold_lanes<(TEAM < 64 ? TEAM : 64)>(q, Sum());
+    if constexpr (TEAM > 64) {
+        auto& s = scratch.v[turn];
+        turn ^= 1;
+        if ((threadIdx.x & 63) == 0) s[threadIdx.x >> 6][0] = p, s[threadIdx.x >> 6][1] = q;
+        __syncthreads();
+        p = s[0][0], q = s[0][1];
+#pragma unroll
+        for (int w = 1; w < TEAM / 64; ++w) p += s[w][0], q += s[w][1];
+    }
+}
+
 template <typename T>
-__global__ __launch_bounds__(kThreads) void norm_rows(NormArgs<T> a) {
-    __shared__ T scratch[kThreads / 64];
+__device__ __forceinline__ T root_of(T variance, T epsilon) {
+    // (below zero by rounding alone; a NaN stays)
+    return T(1) / sqrt((variance < T(0) ? T(0) : variance) + epsilon);
+}
+
+// A team of TEAM threads per row, which lives in their registers, E groups of 16 bytes to a thread: read once, written once. WHOLE: the teams' groups are the
+// row exactly. The weights stay in registers from row to row where they fit.
+template <typename T, int TEAM, int E, bool WHOLE>
+__global__ __launch_bounds__(TEAM > kThreads ? TEAM : kThreads) void norm_team(NormArgs<T> a) {
+    constexpr int N = Vec<T>::N, BLOCK = TEAM > kThreads ? TEAM : kThreads, TEAMS = BLOCK / TEAM;
+    constexpr bool HOLD = E * N <= 16;
+    __shared__ TeamScratch<T, TEAM> scratch;
+    int turn = 0;
+    const int l = threadIdx.x % TEAM;
+    const T count = a.width;
+    T gamma[HOLD ? E : 1][N], beta[HOLD ? E : 1][N];
+    auto weights = [&](int e, T (&g)[N], T (&b)[N]) {
+        const int c = (l + e * TEAM) * N;
+        if (a.gamma) {
+            load_group(a.gamma, c, a.width, T(0), g);
+        } else {
+#pragma unroll
+            for (int i = 0; i < N; ++i) g[i] = T(1);
+        }
+        if (a.beta) {
+            load_group(a.beta, c, a.width, T(0), b);
+        } else {
+#pragma unroll
+            for (int i = 0; i < N; ++i) b[i] = T(0);
+        }
+    };
+    if constexpr (HOLD) {
+#pragma unroll
+        for (int e = 0; e < E; ++e) weights(e, gamma[e], beta[e]);
+    }
+    for (long first = (long)blockIdx.x * TEAMS; first < a.rows; first += (long)gridDim.x * TEAMS) {
+        const long row = first + threadIdx.x / TEAM, r = row < a.rows ? row : a.rows - 1;  // (a team without a row goes along with the last)
+        const T* x = a.x + r * a.stride;
+        T v[E][N];
+        T s = 0, none = 0;
+#pragma unroll
+        for (int e = 0; e < E; ++e) load_group(x, (l + e * TEAM) * N, a.width, T(0), v[e]);
+#pragma unroll
+        for (int e = 0; e < E; ++e)
+#pragma unroll
+            for (int i = 0; i < N; ++i) s += v[e][i];
+        team_sum<TEAM>(s, none, scratch, turn);
+        const T near = s / count;
+        T off = 0, square = 0;
+#pragma unroll
+        for (int e = 0; e < E; ++e)
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                v[e][i] -= near;
+                const T d = WHOLE || (l + e * TEAM) * N + i < a.width ? v[e][i] : T(0);
+                off += d;
+                square += d * d;
+            }
+        team_sum<TEAM>(off, square, scratch, turn);
+        off /= count;
+        const T rstd = root_of(square / count - off * off, a.epsilon);
+        if (row < a.rows) {
+            if (l == 0) {
+                a.mean[r] = near + off;
+                a.rstd[r] = rstd;
+            }
+#pragma unroll
+            for (int e = 0; e < E; ++e) {
+                T g[N], b[N];
+                if constexpr (!HOLD) weights(e, g, b);
+#pragma unroll
+                for (int i = 0; i < N; ++i) {
+                    const T gi = HOLD ? gamma[HOLD ? e : 0][i] : g[i], bi = HOLD ? beta[HOLD ? e : 0][i] : b[i];
+                    v[e][i] = (v[e][i] - off) * rstd * gi + bi;
+                }
+                store_group(a.y + r * a.width, (l + e * TEAM) * N, a.width, v[e]);
+            }
+        }
+    }
+}
+
+// Rows that no workgroup's registers hold: a workgroup walks each three times
+template <typename T>
+__global__ __launch_bounds__(1024) void norm_rows(NormArgs<T> a) {
+    constexpr int N = Vec<T>::N, BLOCK = 1024;
+    __shared__ TeamScratch<T, BLOCK> scratch;
+    int turn = 0;
+    const int groups = groups_of<T>(a.width);
+    const T count = a.width;
     for (long r = blockIdx.x; r < a.rows; r += gridDim.x) {
         const T* x = a.x + r * a.stride;
-        T s = 0;
-        for (int c = threadIdx.x; c < a.width; c += kThreads) s += x[c];
-        const T near = block_sum<kThreads>(s, scratch) / a.width;
-        T off = 0, sq = 0;
-        for (int c = threadIdx.x; c < a.width; c += kThreads) {
-            const T d = x[c] - near;
-            off += d;
-            sq += d * d;
-        }
-        off = block_sum<kThreads>(off, scratch) / a.width;
-        sq = block_sum<kThreads>(sq, scratch) / a.width - off * off;
-        const T rstd = T(1) / sqrt((sq > 0 || sq != sq ? sq : T(0)) + a.epsilon);
         T* y = a.y + r * a.width;
-        for (int c = threadIdx.x; c < a.width; c += kThreads) {
-            const T u = ((x[c] - near) - off) * rstd;
-            y[c] = u * (a.gamma ? a.gamma[c] : T(1)) + (a.beta ? a.beta[c] : T(0));
+        T s = 0, none = 0, v[N], g[N], b[N];
+        for (int j = threadIdx.x; j < groups; j += BLOCK) {
+            load_group(x, j * N, a.width, T(0), v);
+#pragma unroll
+            for (int i = 0; i < N; ++i) s += v[i];
+        }
+        team_sum<BLOCK>(s, none, scratch, turn);
+        const T near = s / count;
+        T off = 0, square = 0;
+        for (int j = threadIdx.x; j < groups; j += BLOCK) {
+            load_group(x, j * N, a.width, near, v);
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                const T d = v[i] - near;
+                off += d;
+                square += d * d;
+            }
+        }
+        team_sum<BLOCK>(off, square, scratch, turn);
+        off /= count;
+        const T rstd = root_of(square / count - off * off, a.epsilon);
+        for (int j = threadIdx.x; j < groups; j += BLOCK) {
+            load_group(x, j * N, a.width, T(0), v);
+#pragma unroll
+            for (int i = 0; i < N; ++i) g[i] = T(1), b[i] = T(0);
+            if (a.gamma) load_group(a.gamma, j * N, a.width, T(0), g);
+            if (a.beta) load_group(a.beta, j * N, a.width, T(0), b);
+#pragma unroll
+            for (int i = 0; i < N; ++i) v[i] = ((v[i] - near) - off) * rstd * g[i] + b[i];
+            store_group(y, j * N, a.width, v);
         }
         if (threadIdx.x == 0) {
             a.mean[r] = near + off;
@@ -61,34 +185,166 @@ struct NormBackwardArgs {
     int width, parts;
 };
 
-template <typename T>
-__global__ __launch_bounds__(kThreads) void norm_backward_rows(NormBackwardArgs<T> a) {
-    __shared__ T scratch[kThreads / 64];
-    for (long r = blockIdx.x; r < a.rows; r += gridDim.x) {
-        const T *x = a.x + r * a.x_stride, *dy = a.dy + r * a.dy_stride;
-        const T mean = a.mean[r], rstd = a.rstd[r];
-        T level = 0, along = 0;
-        for (int c = threadIdx.x; c < a.width; c += kThreads) {
-            const T g = dy[c] * (a.gamma ? a.gamma[c] : T(1));
-            level += g;
-            along += g * ((x[c] - mean) * rstd);
-        }
-        level = block_sum<kThreads>(level, scratch) / a.width;
-        along = block_sum<kThreads>(along, scratch) / a.width;
-        T* dx = a.dx + r * a.width;
-        for (int c = threadIdx.x; c < a.width; c += kThreads) {
-            const T g = dy[c] * (a.gamma ? a.gamma[c] : T(1));
-            dx[c] = rstd * ((g - level) - (x[c] - mean) * rstd * along);
+// the value of the lane D further on in its half (D = 8: of 16 lanes) or in the other half, without a condition on closer lanes
+template <int D, typename T>
+__device__ __forceinline__ T plus_across(T v) {
+    if constexpr (D >= 16) {
+        T a, b;
+        halves_of<D>(v, a, b);
+        return a + b;
+    } else {
+        static_assert(D == 8, "lanes 8, 16 or 32 apart");
+        const auto rotated = [](unsigned w) { return (unsigned)__builtin_amdgcn_update_dpp(0, (int)w, 0x128, 0xf, 0xf, true); };
+        if constexpr (sizeof(T) == 4) {
+            return v + __builtin_bit_cast(T, rotated(__builtin_bit_cast(unsigned, v)));
+        } else {
+            const unsigned long long w = __builtin_bit_cast(unsigned long long, v);
+            return v + __builtin_bit_cast(T, (unsigned long long)rotated((unsigned)(w >> 32)) << 32 | rotated((unsigned)w));
         }
     }
 }
 
-// columns of one strip over one part of the rows, then the parts in order
+// The gradient with the rows in registers as above; a thread also keeps the sums of its columns over all rows that its team takes. At the end the teams of a
+// workgroup are joined, lanes first and then waves through LDS, in halves, and the workgroup leaves one row of partial sums for each weight.
+template <typename T, int TEAM, int E, bool WHOLE, bool WEIGHTS>
+__global__ __launch_bounds__(TEAM > 512 ? TEAM : 512) void norm_backward_team(NormBackwardArgs<T> a) {
+    constexpr int N = Vec<T>::N, BLOCK = TEAM > 512 ? TEAM : 512, TEAMS = BLOCK / TEAM;
+    // (waves that hold the same columns; LDS for half of them)
+    constexpr int SPAN = TEAM > 64 ? TEAM : 64, SAME = BLOCK / SPAN;
+    __shared__ TeamScratch<T, TEAM> scratch;
+    __shared__ T joined[WEIGHTS && SAME > 1 ? SAME / 2 : 1][WEIGHTS && SAME > 1 ? 2 * E * N : 1][WEIGHTS && SAME > 1 ? SPAN : 1];
+    static_assert(TEAM <= 64 || TEAMS == 1, "a team of several waves is a workgroup");
+    int turn = 0;
+    const int l = threadIdx.x % TEAM;
+    const T count = a.width;
+    T gamma[E][N], dgamma[E][N], dbeta[E][N];
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) gamma[e][i] = T(1), dgamma[e][i] = dbeta[e][i] = T(0);
+        if (a.gamma) load_group(a.gamma, (l + e * TEAM) * N, a.width, T(0), gamma[e]);
+    }
+    for (long first = (long)blockIdx.x * TEAMS; first < a.rows; first += (long)gridDim.x * TEAMS) {
+        const long row = first + threadIdx.x / TEAM, r = row < a.rows ? row : a.rows - 1;
+        const bool live = row < a.rows;  // (a team without a row goes along with the last, and adds nothing)
+        const T *x = a.x + r * a.x_stride, *dy = a.dy + r * a.dy_stride;
+        T u[E][N], d[E][N];
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            load_group(x, (l + e * TEAM) * N, a.width, T(0), u[e]);
+            load_group(dy, (l + e * TEAM) * N, a.width, T(0), d[e]);
+        }
+        const T mean = a.mean[r], rstd = a.rstd[r];
+        T level = 0, along = 0;
+#pragma unroll
+        for (int e = 0; e < E; ++e)
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                const bool in = WHOLE || (l + e * TEAM) * N + i < a.width;
+                u[e][i] = in ? (u[e][i] - mean) * rstd : T(0);
+                if constexpr (WEIGHTS) {
+                    dgamma[e][i] += live ? d[e][i] * u[e][i] : T(0);
+                    dbeta[e][i] += live ? d[e][i] : T(0);
+                }
+                d[e][i] *= gamma[e][i];
+                level += d[e][i];
+                along += d[e][i] * u[e][i];
+            }
+        team_sum<TEAM>(level, along, scratch, turn);
+        level /= count;
+        along /= count;
+        if (live) {
+#pragma unroll
+            for (int e = 0; e < E; ++e) {
+#pragma unroll
+                for (int i = 0; i < N; ++i) d[e][i] = rstd * ((d[e][i] - level) - u[e][i] * along);
+                store_group(a.dx + r * a.width, (l + e * TEAM) * N, a.width, d[e]);
+            }
+        }
+    }
+    if constexpr (WEIGHTS) {
+        auto every = [&](auto&& f) {
+#pragma unroll
+            for (int e = 0; e < E; ++e)
+#pragma unroll
+                for (int i = 0; i < N; ++i) f(dgamma[e][i], 2 * (e * N + i)), f(dbeta[e][i], 2 * (e * N + i) + 1);
+        };
+        if constexpr (TEAM < 64) {
+            every([&](T& v, int) {
+                if constexpr (TEAM <= 8) v = plus_across<8>(v);
+                if constexpr (TEAM <= 16) v = plus_across<16>(v);
+                v = plus_across<32>(v);
+            });
+        }
+        const int at = threadIdx.x % SPAN, group = threadIdx.x / SPAN;
+#pragma unroll
+        for (int half = SAME / 2; half >= 1; half /= 2) {
+            __syncthreads();
+            if (group >= half && group < 2 * half) every([&](T& v, int k) { joined[group - half][k][at] = v; });
+            __syncthreads();
+            if (group < half) every([&](T& v, int k) { v += joined[group][k][at]; });
+        }
+        if (threadIdx.x < TEAM) {
+            T* g = a.parts == 1 ? a.dgamma : a.partial + (long)blockIdx.x * 2 * a.width;
+            T* b = a.parts == 1 ? a.dbeta : g + a.width;
+#pragma unroll
+            for (int e = 0; e < E; ++e) {
+                store_group(g, (l + e * TEAM) * N, a.width, dgamma[e]);
+                store_group(b, (l + e * TEAM) * N, a.width, dbeta[e]);
+            }
+        }
+    }
+}
+
+// Longer rows: dx by a workgroup that walks each row twice ...
+template <typename T>
+__global__ __launch_bounds__(1024) void norm_backward_rows(NormBackwardArgs<T> a) {
+    constexpr int N = Vec<T>::N, BLOCK = 1024;
+    __shared__ TeamScratch<T, BLOCK> scratch;
+    int turn = 0;
+    const int groups = groups_of<T>(a.width);
+    const T count = a.width;
+    for (long r = blockIdx.x; r < a.rows; r += gridDim.x) {
+        const T *x = a.x + r * a.x_stride, *dy = a.dy + r * a.dy_stride;
+        T* dx = a.dx + r * a.width;
+        const T mean = a.mean[r], rstd = a.rstd[r];
+        T level = 0, along = 0, u[N], d[N], g[N];
+        auto load = [&](int j) {
+            load_group(x, j * N, a.width, mean, u);
+            load_group(dy, j * N, a.width, T(0), d);
+#pragma unroll
+            for (int i = 0; i < N; ++i) g[i] = T(1);
+            if (a.gamma) load_group(a.gamma, j * N, a.width, T(0), g);
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                u[i] = (u[i] - mean) * rstd;
+                d[i] *= g[i];
+            }
+        };
+        for (int j = threadIdx.x; j < groups; j += BLOCK) {
+            load(j);
+#pragma unroll
+            for (int i = 0; i < N; ++i) level += d[i], along += d[i] * u[i];
+        }
+        team_sum<BLOCK>(level, along, scratch, turn);
+        level /= count;
+        along /= count;
+        for (int j = threadIdx.x; j < groups; j += BLOCK) {
+            load(j);
+#pragma unroll
+            for (int i = 0; i < N; ++i) d[i] = rstd * ((d[i] - level) - u[i] * along);
+            store_group(dx, j * N, a.width, d);
+        }
+    }
+}
+
+// ... and the weights by columns, over one part of the rows
 template <typename T>
 __global__ __launch_bounds__(kThreads) void norm_weights(NormBackwardArgs<T> a) {
     const int c = blockIdx.x * kThreads + threadIdx.x;
     if (c >= a.width) return;
     T g = 0, b = 0;
+#pragma unroll 4
     for (long r = blockIdx.y; r < a.rows; r += a.parts) {
         const T d = a.dy[r * a.dy_stride + c];
         g += d * ((a.x[r * a.x_stride + c] - a.mean[r]) * a.rstd[r]);
@@ -104,37 +360,95 @@ __global__ __launch_bounds__(kThreads) void norm_weights(NormBackwardArgs<T> a) 
     p[a.width] = b;
 }
 
+// The parts in order: 16 threads of a column take every 16th part each, and are joined in a tree. Partial rows of dgamma and dbeta lie one behind the other, so
+// both are columns of one matrix [parts, 2 width].
 template <typename T>
 __global__ __launch_bounds__(kThreads) void norm_fold(NormBackwardArgs<T> a) {
-    const int c = blockIdx.x * kThreads + threadIdx.x;
-    if (c >= a.width) return;
-    T g = 0, b = 0;
-    for (int i = 0; i < a.parts; ++i) {
-        g += a.partial[(long)i * 2 * a.width + c];
-        b += a.partial[(long)i * 2 * a.width + a.width + c];
+    __shared__ T joined[16][17];
+    const int i = threadIdx.x & 15, p = threadIdx.x >> 4;
+    const long c = (long)blockIdx.x * 16 + i, columns = 2L * a.width;
+    T s = 0;
+    if (c < columns) {
+        const T* from = a.partial + c;
+#pragma unroll 8
+        for (int k = p; k < a.parts; k += 16) s += from[k * columns];
     }
-    a.dgamma[c] = g;
-    a.dbeta[c] = b;
+    joined[p][i] = s;
+#pragma unroll
+    for (int half = 8; half >= 1; half /= 2) {
+        __syncthreads();
+        if (p < half) joined[p][i] += joined[p + half][i];
+    }
+    __syncthreads();
+    if (p == 0 && c < columns) (c < a.width ? a.dgamma[c] : a.dbeta[c - a.width]) = joined[0][i];
+}
+
+// threads to a row and groups to a thread that hold a row of `groups` groups; false: none up to `most`
+template <int MOST, typename F>
+bool team_for(int groups, F launch) {
+    auto with = [&](auto team, auto e) {
+        launch(team, e);
+        return true;
+    };
+    using std::integral_constant;
+    if (groups <= 8) return with(integral_constant<int, 8>(), integral_constant<int, 1>());
+    if (groups <= 16) return with(integral_constant<int, 16>(), integral_constant<int, 1>());
+    if (groups <= 32) return with(integral_constant<int, 32>(), integral_constant<int, 1>());
+    if (groups <= 64) return with(integral_constant<int, 64>(), integral_constant<int, 1>());
+    if (groups <= 128) return with(integral_constant<int, 64>(), integral_constant<int, 2>());
+    if (groups <= 192) return with(integral_constant<int, 64>(), integral_constant<int, 3>());
+    if (groups <= 256) return with(integral_constant<int, 64>(), integral_constant<int, 4>());
+    if (groups <= 512) return with(integral_constant<int, 512>(), integral_constant<int, 1>());
+    if (groups <= 1024) return with(integral_constant<int, 512>(), integral_constant<int, 2>());
+    if (groups <= 2048) return with(integral_constant<int, 512>(), integral_constant<int, 4>());
+    if (groups <= 4096) return with(integral_constant<int, 1024>(), integral_constant<int, 4>());
+    if constexpr (MOST > 4096)
+        if (groups <= 8192) return with(integral_constant<int, 1024>(), integral_constant<int, 8>());
+    return false;
 }
 
 template <typename T>
 int forward(NormArgs<T> a) {
-    hipLaunchKernelGGL(norm_rows<T>, dim3((unsigned)std::min(a.rows, 65536L)), dim3(kThreads), 0, stream(), a);
+    const bool held = team_for<8192>(groups_of<T>(a.width), [&](auto team, auto e) {
+        constexpr int TEAM = decltype(team)::value, E = decltype(e)::value, BLOCK = TEAM > kThreads ? TEAM : kThreads, TEAMS = BLOCK / TEAM;
+        const dim3 grid((unsigned)std::min((a.rows + TEAMS - 1) / TEAMS, 8192L * kThreads / BLOCK));
+        if (a.width == TEAM * E * Vec<T>::N) hipLaunchKernelGGL((norm_team<T, TEAM, E, true>), grid, dim3(BLOCK), 0, stream(), a);
+        else hipLaunchKernelGGL((norm_team<T, TEAM, E, false>), grid, dim3(BLOCK), 0, stream(), a);
+    });
+    if (!held) hipLaunchKernelGGL(norm_rows<T>, dim3((unsigned)std::min(a.rows, 65536L)), dim3(1024), 0, stream(), a);
     return launched("dali_hip_layer_norm");
 }
 
 template <typename T>
 int backward(NormBackwardArgs<T> a) {
-    // (the weights first: dx may take the place of x or dy)
-    if (a.dgamma) {
-        const long fit = (long)(kWorkspacePartialBytes / (2 * sizeof(T) * (size_t)a.width));
-        a.parts = (int)std::max(1L, std::min({64L, a.rows, fit}));
-        a.partial = (T*)(workspace() + kWorkspaceCounterBytes);
-        const dim3 grid((a.width + kThreads - 1) / kThreads, a.parts);
-        hipLaunchKernelGGL(norm_weights<T>, grid, dim3(kThreads), 0, stream(), a);
-        if (a.parts > 1) hipLaunchKernelGGL(norm_fold<T>, dim3(grid.x), dim3(kThreads), 0, stream(), a);
+    const long fit = (long)(kWorkspacePartialBytes / (2 * sizeof(T) * (size_t)a.width));  // rows of partial sums that the workspace holds
+    a.partial = (T*)(workspace() + kWorkspaceCounterBytes);
+    a.parts = 1;
+    if (a.rows == 0) {
+        if (a.dgamma) hipLaunchKernelGGL(norm_weights<T>, dim3((a.width + kThreads - 1) / kThreads), dim3(kThreads), 0, stream(), a);
+        return launched("dali_hip_layer_norm_backward");
     }
-    if (a.rows > 0) hipLaunchKernelGGL(norm_backward_rows<T>, dim3((unsigned)std::min(a.rows, 65536L)), dim3(kThreads), 0, stream(), a);
+    const bool held = team_for<4096>(groups_of<T>(a.width), [&](auto team, auto e) {
+        constexpr int TEAM = decltype(team)::value, E = decltype(e)::value, BLOCK = TEAM > 512 ? TEAM : 512, TEAMS = BLOCK / TEAM;
+        // two workgroups to a compute unit, or one of 1024 threads, each with all the rows that fall to it: few partial sums
+        a.parts = (int)std::max(1L, std::min({(a.rows + TEAMS - 1) / TEAMS, 512L * 512 / BLOCK, fit}));
+        const dim3 grid((unsigned)a.parts);
+        const bool whole = a.width == TEAM * E * Vec<T>::N;
+        auto launch = [&](auto w, auto g) {
+            hipLaunchKernelGGL((norm_backward_team<T, TEAM, E, decltype(w)::value, decltype(g)::value>), grid, dim3(BLOCK), 0, stream(), a);
+        };
+        using std::false_type;
+        using std::true_type;
+        if (a.dgamma) whole ? launch(true_type(), true_type()) : launch(false_type(), true_type());
+        else whole ? launch(true_type(), false_type()) : launch(false_type(), false_type());
+    });
+    if (!held && a.dgamma) {
+        // (the weights first: dx may take the place of x or dy)
+        a.parts = (int)std::max(1L, std::min({64L, a.rows, fit}));
+        hipLaunchKernelGGL(norm_weights<T>, dim3((a.width + kThreads - 1) / kThreads, a.parts), dim3(kThreads), 0, stream(), a);
+    }
+    if (a.dgamma && a.parts > 1) hipLaunchKernelGGL(norm_fold<T>, dim3((unsigned)((2L * a.width + 15) / 16)), dim3(kThreads), 0, stream(), a);
+    if (!held) hipLaunchKernelGGL(norm_backward_rows<T>, dim3((unsigned)std::min(a.rows, 65536L)), dim3(1024), 0, stream(), a);
     return launched("dali_hip_layer_norm_backward");
 }
 

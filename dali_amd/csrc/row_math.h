@@ -19,6 +19,41 @@ struct Vec {
     typedef T type __attribute__((ext_vector_type(16 / sizeof(T)), aligned(sizeof(T))));
 };
 
+// groups of 16 bytes in a row
+template <typename T>
+__host__ __device__ __forceinline__ int groups_of(int width) {
+    return width / Vec<T>::N + (width % Vec<T>::N != 0);
+}
+
+// the group of values that begins at c, with `fill` in the place of what lies past the row's end
+template <typename T>
+__device__ __forceinline__ void load_group(const T* x, int c, int width, T fill, T (&v)[Vec<T>::N]) {
+    constexpr int N = Vec<T>::N;
+    if (c <= width - N) {
+        const typename Vec<T>::type g = *reinterpret_cast<const typename Vec<T>::type*>(x + c);
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[i] = g[i];
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[i] = c + i < width ? x[c + i] : fill;
+    }
+}
+
+template <typename T>
+__device__ __forceinline__ void store_group(T* out, int c, int width, const T (&v)[Vec<T>::N]) {
+    constexpr int N = Vec<T>::N;
+    if (c <= width - N) {
+        typename Vec<T>::type g;
+#pragma unroll
+        for (int i = 0; i < N; ++i) g[i] = v[i];
+        *reinterpret_cast<typename Vec<T>::type*>(out + c) = g;
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+            if (c + i < width) out[c + i] = v[i];
+    }
+}
+
 // The value of the lane that is D away in the binary numbering of a wave, for folds that have already joined the lanes closer than D: `a` and `b` are
 // the two halves' values, the same pair in both. Steps inside 16 lanes are data moves of the vector unit (within a quad, the mirror image of 8 and of 16 lanes),
 // the others exchange half rows between two registers; none goes through LDS.

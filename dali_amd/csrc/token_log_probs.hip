@@ -131,25 +131,6 @@ struct LogProbArgs {
     int counter_step;
 };
 
-template <typename T>
-__host__ __device__ __forceinline__ int groups_of(int vocab) {
-    return vocab / Vec<T>::N + (vocab % Vec<T>::N != 0);
-}
-
-// group c / N of the row, with -inf in the place of what lies past its end
-template <typename T>
-__device__ __forceinline__ void load_group(const T* x, int c, int vocab, T (&v)[Vec<T>::N]) {
-    constexpr int N = Vec<T>::N;
-    if (c <= vocab - N) {
-        const typename Vec<T>::type g = *reinterpret_cast<const typename Vec<T>::type*>(x + c);
-#pragma unroll
-        for (int i = 0; i < N; ++i) v[i] = g[i];
-    } else {
-#pragma unroll
-        for (int i = 0; i < N; ++i) v[i] = c + i < vocab ? x[c + i] : T(-INFINITY);
-    }
-}
-
 // what a row's sums come to
 template <typename T>
 struct RowResult {
@@ -297,7 +278,7 @@ __global__ __launch_bounds__(kThreads) void log_prob_short(LogProbArgs<T> a) {
     const T* x = a.logits + r * a.stride;
     T v[E][N];
 #pragma unroll
-    for (int e = 0; e < E; ++e) load_group(x, (l + e * LANES) * N, a.vocab, v[e]);
+    for (int e = 0; e < E; ++e) load_group(x, (l + e * LANES) * N, a.vocab, T(-INFINITY), v[e]);
     const int token = a.tokens[r];
     const T own = token >= 0 && token < a.vocab ? x[token] : T(0);
     T m = Real<T>::lowest;
@@ -551,7 +532,7 @@ __global__ __launch_bounds__(kThreads) void log_prob_long(LogProbArgs<T> a) {
     }
     for (; j < end; j += kThreads) {
         T v[N];
-        load_group(x, j * N, a.vocab, v);
+        load_group(x, j * N, a.vocab, T(-INFINITY), v);
         T g = v[0];
 #pragma unroll
         for (int i = 1; i < N; ++i) g = Max()(g, v[i]);
@@ -571,7 +552,7 @@ __global__ __launch_bounds__(kThreads) void log_prob_long(LogProbArgs<T> a) {
             const int n = i / walks, g = begin + sh.unit[n] + (i - n * walks) * kThreads;
             if (g >= end) continue;
             T v[N];
-            load_group(x, g * N, a.vocab, v);
+            load_group(x, g * N, a.vocab, T(-INFINITY), v);
             collect(v, g, a.vocab, bound, sh);
         }
         __syncthreads();
@@ -598,7 +579,7 @@ __global__ __launch_bounds__(kThreads) void log_prob_segments(LogProbArgs<T> a) 
 #pragma unroll
     for (int e = 0; e < E; ++e) {
         const int g = begin + tid + e * kThreads;
-        load_group(x, g < end ? g * N : a.vocab, a.vocab, v[e]);
+        load_group(x, g < end ? g * N : a.vocab, a.vocab, T(-INFINITY), v[e]);
     }
     const int token = a.tokens[r];
     const T own = token >= 0 && token < a.vocab ? x[token] : T(0);
@@ -666,21 +647,6 @@ struct RowGradient {
     }
 };
 
-template <typename T>
-__device__ __forceinline__ void store_group(T* out, int c, int vocab, const T (&v)[Vec<T>::N]) {
-    constexpr int N = Vec<T>::N;
-    if (c <= vocab - N) {
-        typename Vec<T>::type g;
-#pragma unroll
-        for (int i = 0; i < N; ++i) g[i] = v[i];
-        *reinterpret_cast<typename Vec<T>::type*>(out + c) = g;
-    } else {
-#pragma unroll
-        for (int i = 0; i < N; ++i)
-            if (c + i < vocab) out[c + i] = v[i];
-    }
-}
-
 // LANES lanes to a row
 template <typename T, int LANES, int E>
 __global__ __launch_bounds__(kThreads) void log_prob_backward_short(LogProbBackwardArgs<T> a) {
@@ -691,7 +657,7 @@ __global__ __launch_bounds__(kThreads) void log_prob_backward_short(LogProbBackw
     const T* x = a.logits + r * a.stride;
     T v[E][N];
 #pragma unroll
-    for (int e = 0; e < E; ++e) load_group(x, (l + e * LANES) * N, a.vocab, v[e]);
+    for (int e = 0; e < E; ++e) load_group(x, (l + e * LANES) * N, a.vocab, T(-INFINITY), v[e]);
     const RowGradient<T> q(a, r);
 #pragma unroll
     for (int e = 0; e < E; ++e) {
@@ -713,7 +679,7 @@ __global__ __launch_bounds__(kThreads) void log_prob_backward_long(LogProbBackwa
     const int first = (piece * U * kThreads + (int)threadIdx.x) * N;  // (the last group of the longest row ends at 2^31 - 1)
     T v[U][N];
 #pragma unroll
-    for (int u = 0; u < U; ++u) load_group(x, min((long)first + u * kThreads * N, (long)a.vocab), a.vocab, v[u]);
+    for (int u = 0; u < U; ++u) load_group(x, min((long)first + u * kThreads * N, (long)a.vocab), a.vocab, T(-INFINITY), v[u]);
 #pragma unroll
     for (int u = 0; u < U; ++u) {
         const long c = (long)first + u * kThreads * N;
