@@ -2,8 +2,9 @@
 //
 //   norm = sqrt(sum over all arrays of sum of squares),  scale = max_norm / norm where norm > max_norm, else 1
 //
-// Squares are summed in double (an fp32 value's square neither overflows nor vanishes there). Every workgroup sums one chunk and leaves one
-// partial; one workgroup folds the partials in the order of the chunks, so the norm does not depend on scheduling. A norm that is not finite
+// Squares are summed in double (an fp32 value's square neither overflows nor vanishes there). A workgroup sums the chunks that fall to it and leaves one
+// partial; every workgroup of the second launch folds all partials in the same order before it scales, so the norm does not depend on scheduling and needs no
+// launch of its own. The second launch walks the chunks backwards: what the first read last is still in the cache. A norm that is not finite
 // scales nothing: the arrays come back as they are and the norm says so.
 #include <algorithm>
 #include <vector>
@@ -14,17 +15,20 @@ namespace dali_hip {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kBatch = 96;  // arrays per launch: their addresses travel with it (kernel arguments hold 4 KiB)
+constexpr int kBatch = 96;       // arrays per launch: their addresses travel with it (kernel arguments hold 4 KiB)
+constexpr int kPartials = 1024;  // workgroups of the first launch, as far as one launch goes
+constexpr int kUnroll = 4;       // groups of 16 bytes that a thread has in flight
 
 struct Batch {
     const void* in[kBatch];
     void* out[kBatch];
     long n[kBatch];
     int first[kBatch + 1];  // number of an array's first chunk in this launch
-    int arrays;
-    long chunk;
-    double* partial;  // of this launch's first chunk
-    double* result;   // {scale}
+    int arrays, chunk;      // values to a chunk
+    double* partial;        // first launch: of its first workgroup
+    int partials;           // second launch: all of them
+    double max_norm;
+    void* norm;             // written by the second launch, if this is its first batch (else NULL)
 };
 
 // the array that chunk b belongs to
@@ -38,54 +42,67 @@ __device__ __forceinline__ int array_of(const Batch& a, int b) {
     return lo;
 }
 
+// the groups of chunk b, four to a thread at a time: f(array, where in it, values, how many of them)
+template <typename T, typename F>
+__device__ __forceinline__ void walk(const Batch& a, int b, F f) {
+    constexpr int N = Vec<T>::N, STEP = kThreads * N;
+    const int i = array_of(a, b);
+    const long begin = (long)(b - a.first[i]) * a.chunk;
+    const int count = (int)min((long)a.chunk, a.n[i] - begin);
+    const T* x = (const T*)a.in[i] + begin;
+    for (int c = threadIdx.x * N; c < count; c += kUnroll * STEP) {
+        T v[kUnroll][N];
+#pragma unroll
+        for (int u = 0; u < kUnroll; ++u) load_group(x, min(c + u * STEP, count), count, T(0), v[u]);
+#pragma unroll
+        for (int u = 0; u < kUnroll; ++u) f(i, begin, c + u * STEP, count, v[u]);
+    }
+}
+
 template <typename T>
 __global__ __launch_bounds__(kThreads) void squares(Batch a) {
     __shared__ double scratch[kThreads / 64];
-    const int i = array_of(a, blockIdx.x);
-    const long begin = (blockIdx.x - a.first[i]) * a.chunk, end = min(begin + a.chunk, a.n[i]);
-    const T* x = (const T*)a.in[i];
     double s = 0;
-    for (long c = begin + threadIdx.x; c < end; c += kThreads) s += (double)x[c] * (double)x[c];
+    for (int b = blockIdx.x; b < a.first[a.arrays]; b += gridDim.x)
+        walk<T>(a, b, [&](int, long, int, int, const T(&v)[Vec<T>::N]) {
+#pragma unroll
+            for (int k = 0; k < Vec<T>::N; ++k) s += (double)v[k] * (double)v[k];
+        });
     s = block_sum<kThreads>(s, scratch);
     if (threadIdx.x == 0) a.partial[blockIdx.x] = s;
 }
 
 template <typename T>
-__global__ __launch_bounds__(kThreads) void fold(const double* partial, int count, double max_norm, T* norm, double* scale) {
+__global__ __launch_bounds__(kThreads) void rescale(Batch a) {
     __shared__ double scratch[kThreads / 64];
     double s = 0;
-    for (int i = threadIdx.x; i < count; i += kThreads) s += partial[i];
+    for (int i = threadIdx.x; i < a.partials; i += kThreads) s += a.partial[i];
     s = sqrt(block_sum<kThreads>(s, scratch));
-    if (threadIdx.x == 0) {
-        *norm = (T)s;
-        *scale = s > max_norm && s < (double)INFINITY ? max_norm / s : 1.0;
-    }
-}
-
-template <typename T>
-__global__ __launch_bounds__(kThreads) void rescale(Batch a) {
-    const int i = array_of(a, blockIdx.x);
-    const long begin = (blockIdx.x - a.first[i]) * a.chunk, end = min(begin + a.chunk, a.n[i]);
-    const T* x = (const T*)a.in[i];
-    T* y = (T*)a.out[i];
+    if (a.norm && blockIdx.x == 0 && threadIdx.x == 0) *(T*)a.norm = (T)s;
     // (in double: where the norm passes the largest float, the scale would lose its digits in one)
-    const double scale = *a.result;
-    for (long c = begin + threadIdx.x; c < end; c += kThreads) y[c] = (T)((double)x[c] * scale);
+    const double scale = s > a.max_norm && s < (double)INFINITY ? a.max_norm / s : 1.0;
+    for (int b = a.first[a.arrays] - 1 - (int)blockIdx.x; b >= 0; b -= gridDim.x)
+        walk<T>(a, b, [&](int i, long begin, int c, int count, T(&v)[Vec<T>::N]) {
+#pragma unroll
+            for (int k = 0; k < Vec<T>::N; ++k) v[k] = (T)((double)v[k] * scale);
+            if (c < count) store_group((T*)a.out[i] + begin, c, count, v);
+        });
 }
 
 template <typename T>
 int clip(int count, const void* const* in, void* const* out, const int64_t* sizes, double max_norm, T* norm) {
+    double* partial = (double*)(workspace() + kWorkspaceCounterBytes);
     long total = 0;
     for (int i = 0; i < count; ++i) total += sizes[i];
-    const long chunk = std::max(1024L, (total / 4096 + 1023) / 1024 * 1024);
-    double* partial = (double*)(workspace() + kWorkspaceCounterBytes);
-    double* scale = partial;
-    ++partial;
-    int done = 0;
-    auto batches = [&](auto&& launch) {
-        done = 0;
+    constexpr int STEP = kThreads * Vec<T>::N * kUnroll;
+    // chunks of one step of a workgroup where there are few, of four where there are many: an array's end costs less of them
+    const int chunk = total < 4096L * STEP ? STEP : 4 * STEP;
+    const int batches = (count + kBatch - 1) / kBatch, most = std::max(kPartials / std::max(batches, 1), 16);
+    Batch b;
+    b.chunk = chunk;
+    b.max_norm = max_norm;
+    auto each = [&](auto&& launch) {
         for (int at = 0; at < count;) {
-            Batch b;
             b.arrays = 0;
             b.first[0] = 0;
             for (; at < count && b.arrays < kBatch; ++at) {
@@ -96,17 +113,29 @@ int clip(int count, const void* const* in, void* const* out, const int64_t* size
                 b.first[b.arrays + 1] = b.first[b.arrays] + (int)((sizes[at] + chunk - 1) / chunk);
                 ++b.arrays;
             }
-            if (b.arrays == 0) continue;
-            b.chunk = chunk;
-            b.partial = partial + done;
-            b.result = scale;
-            launch(b, b.first[b.arrays]);
-            done += b.first[b.arrays];
+            if (b.arrays) launch(b.first[b.arrays]);
         }
     };
-    batches([&](const Batch& b, int blocks) { hipLaunchKernelGGL(squares<T>, dim3(blocks), dim3(kThreads), 0, stream(), b); });
-    hipLaunchKernelGGL(fold<T>, dim3(1), dim3(kThreads), 0, stream(), partial, done, max_norm, norm, scale);
-    if (out) batches([&](const Batch& b, int blocks) { hipLaunchKernelGGL(rescale<T>, dim3(blocks), dim3(kThreads), 0, stream(), b); });
+    int partials = 0;
+    each([&](int chunks) {
+        const int blocks = std::min(chunks, most);
+        b.partial = partial + partials;
+        hipLaunchKernelGGL(squares<T>, dim3(blocks), dim3(kThreads), 0, stream(), b);
+        partials += blocks;
+    });
+    b.partial = partial;
+    b.partials = partials;
+    b.norm = norm;
+    if (out)
+        each([&](int chunks) {
+            hipLaunchKernelGGL(rescale<T>, dim3(std::min(chunks, 2048)), dim3(kThreads), 0, stream(), b);
+            b.norm = nullptr;
+        });
+    if (b.norm) {  // the norm alone, or nothing to scale
+        b.arrays = 0;
+        b.first[0] = 0;
+        hipLaunchKernelGGL(rescale<T>, dim3(1), dim3(kThreads), 0, stream(), b);
+    }
     return launched("dali_hip_clip_by_global_norm");
 }
 
@@ -123,8 +152,8 @@ extern "C" int dali_hip_clip_by_global_norm(int dtype, int count, const void* co
     const size_t size = dtype == DALI_HIP_FLOAT ? 4 : 8;
     for (int i = 0; i < count; ++i)
         if (sizes[i] < 0 || (sizes[i] > 0 && (!in[i] || (out && !out[i])))) return fail("%s: array %d has no memory or a negative size", what, i);
-    // (one partial per chunk: at most 4096, and one more for each array)
-    if (((size_t)count + 4096 + 2) * sizeof(double) > kWorkspacePartialBytes) return fail("%s: %d arrays are more than the workspace has room for", what, count);
+    // (partial sums: kPartials, or 16 for every launch of kBatch arrays; chunks are numbered in 31 bits)
+    if (count > (1 << 24)) return fail("%s: %d arrays are more than the workspace has room for", what, count);
     if (ensure_init()) return DALI_HIP_ERROR;
     const Span result("norm", norm, 1, size);
     for (int i = 0; i < count; ++i) {
