@@ -16,7 +16,7 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kBatch = 96;       // arrays per launch: their addresses travel with it (kernel arguments hold 4 KiB)
-constexpr int kPartials = 1024;  // workgroups of the first launch, as far as one launch goes
+constexpr int kPartials = 2048;  // workgroups of the first launch, as far as one launch goes
 constexpr int kUnroll = 4;       // groups of 16 bytes that a thread has in flight
 
 struct Batch {
@@ -62,17 +62,20 @@ __device__ __forceinline__ void walk(const Batch& a, int b, F f) {
 template <typename T>
 __global__ __launch_bounds__(kThreads) void squares(Batch a) {
     __shared__ double scratch[kThreads / 64];
-    double s = 0;
+    double part[Vec<T>::N] = {};
     for (int b = blockIdx.x; b < a.first[a.arrays]; b += gridDim.x)
         walk<T>(a, b, [&](int, long, int, int, const T(&v)[Vec<T>::N]) {
 #pragma unroll
-            for (int k = 0; k < Vec<T>::N; ++k) s += (double)v[k] * (double)v[k];
+            for (int k = 0; k < Vec<T>::N; ++k) part[k] += (double)v[k] * (double)v[k];
         });
+    double s = part[0];
+#pragma unroll
+    for (int k = 1; k < Vec<T>::N; ++k) s += part[k];
     s = block_sum<kThreads>(s, scratch);
     if (threadIdx.x == 0) a.partial[blockIdx.x] = s;
 }
 
-template <typename T>
+template <typename T, bool PAST>
 __global__ __launch_bounds__(kThreads) void rescale(Batch a) {
     __shared__ double scratch[kThreads / 64];
     double s = 0;
@@ -85,7 +88,7 @@ __global__ __launch_bounds__(kThreads) void rescale(Batch a) {
         walk<T>(a, b, [&](int i, long begin, int c, int count, T(&v)[Vec<T>::N]) {
 #pragma unroll
             for (int k = 0; k < Vec<T>::N; ++k) v[k] = (T)((double)v[k] * scale);
-            if (c < count) store_group((T*)a.out[i] + begin, c, count, v);
+            if (c < count) store_group<PAST>((T*)a.out[i] + begin, c, count, v);
         });
 }
 
@@ -128,13 +131,14 @@ int clip(int count, const void* const* in, void* const* out, const int64_t* size
     b.norm = norm;
     if (out)
         each([&](int chunks) {
-            hipLaunchKernelGGL(rescale<T>, dim3(std::min(chunks, 2048)), dim3(kThreads), 0, stream(), b);
+            either_way(past_caches(2.0 * sizeof(T) * total),
+                       [&](auto p) { hipLaunchKernelGGL((rescale<T, decltype(p)::value>), dim3(std::min(chunks, 2048)), dim3(kThreads), 0, stream(), b); });
             b.norm = nullptr;
         });
     if (b.norm) {  // the norm alone, or nothing to scale
         b.arrays = 0;
         b.first[0] = 0;
-        hipLaunchKernelGGL(rescale<T>, dim3(1), dim3(kThreads), 0, stream(), b);
+        hipLaunchKernelGGL((rescale<T, false>), dim3(1), dim3(kThreads), 0, stream(), b);
     }
     return launched("dali_hip_clip_by_global_norm");
 }

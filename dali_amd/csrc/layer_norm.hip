@@ -53,7 +53,7 @@ __device__ __forceinline__ T root_of(T variance, T epsilon) {
 
 // A team of TEAM threads per row, which lives in their registers, E groups of 16 bytes to a thread: read once, written once. WHOLE: the teams' groups are the
 // row exactly. The weights stay in registers from row to row where they fit.
-template <typename T, int TEAM, int E, bool WHOLE>
+template <typename T, int TEAM, int E, bool WHOLE, bool PAST>
 __global__ __launch_bounds__(TEAM > kThreads ? TEAM : kThreads) void norm_team(NormArgs<T> a) {
     constexpr int N = Vec<T>::N, BLOCK = TEAM > kThreads ? TEAM : kThreads, TEAMS = BLOCK / TEAM;
     constexpr bool HOLD = E * N <= 16;
@@ -121,14 +121,14 @@ __global__ __launch_bounds__(TEAM > kThreads ? TEAM : kThreads) void norm_team(N
                     const T gi = HOLD ? gamma[HOLD ? e : 0][i] : g[i], bi = HOLD ? beta[HOLD ? e : 0][i] : b[i];
                     v[e][i] = (v[e][i] - off) * rstd * gi + bi;
                 }
-                store_group(a.y + r * a.width, (l + e * TEAM) * N, a.width, v[e]);
+                store_group<PAST>(a.y + r * a.width, (l + e * TEAM) * N, a.width, v[e]);
             }
         }
     }
 }
 
 // Rows that no workgroup's registers hold: a workgroup walks each three times
-template <typename T>
+template <typename T, bool PAST>
 __global__ __launch_bounds__(1024) void norm_rows(NormArgs<T> a) {
     constexpr int N = Vec<T>::N, BLOCK = 1024;
     __shared__ TeamScratch<T, BLOCK> scratch;
@@ -167,7 +167,7 @@ __global__ __launch_bounds__(1024) void norm_rows(NormArgs<T> a) {
             if (a.beta) load_group(a.beta, j * N, a.width, T(0), b);
 #pragma unroll
             for (int i = 0; i < N; ++i) v[i] = ((v[i] - near) - off) * rstd * g[i] + b[i];
-            store_group(y, j * N, a.width, v);
+            store_group<PAST>(y, j * N, a.width, v);
         }
         if (threadIdx.x == 0) {
             a.mean[r] = near + off;
@@ -206,7 +206,7 @@ __device__ __forceinline__ T plus_across(T v) {
 
 // The gradient with the rows in registers as above; a thread also keeps the sums of its columns over all rows that its team takes. At the end the teams of a
 // workgroup are joined, lanes first and then waves through LDS, in halves, and the workgroup leaves one row of partial sums for each weight.
-template <typename T, int TEAM, int E, bool WHOLE, bool WEIGHTS>
+template <typename T, int TEAM, int E, bool WHOLE, bool WEIGHTS, bool PAST>
 __global__ __launch_bounds__(TEAM > 512 ? TEAM : 512) void norm_backward_team(NormBackwardArgs<T> a) {
     constexpr int N = Vec<T>::N, BLOCK = TEAM > 512 ? TEAM : 512, TEAMS = BLOCK / TEAM;
     // (waves that hold the same columns; LDS for half of them)
@@ -258,7 +258,7 @@ __global__ __launch_bounds__(TEAM > 512 ? TEAM : 512) void norm_backward_team(No
             for (int e = 0; e < E; ++e) {
 #pragma unroll
                 for (int i = 0; i < N; ++i) d[e][i] = rstd * ((d[e][i] - level) - u[e][i] * along);
-                store_group(a.dx + r * a.width, (l + e * TEAM) * N, a.width, d[e]);
+                store_group<PAST>(a.dx + r * a.width, (l + e * TEAM) * N, a.width, d[e]);
             }
         }
     }
@@ -297,7 +297,7 @@ __global__ __launch_bounds__(TEAM > 512 ? TEAM : 512) void norm_backward_team(No
 }
 
 // Longer rows: dx by a workgroup that walks each row twice ...
-template <typename T>
+template <typename T, bool PAST>
 __global__ __launch_bounds__(1024) void norm_backward_rows(NormBackwardArgs<T> a) {
     constexpr int N = Vec<T>::N, BLOCK = 1024;
     __shared__ TeamScratch<T, BLOCK> scratch;
@@ -333,7 +333,7 @@ __global__ __launch_bounds__(1024) void norm_backward_rows(NormBackwardArgs<T> a
             load(j);
 #pragma unroll
             for (int i = 0; i < N; ++i) d[i] = rstd * ((d[i] - level) - u[i] * along);
-            store_group(dx, j * N, a.width, d);
+            store_group<PAST>(dx, j * N, a.width, d);
         }
     }
 }
@@ -409,18 +409,24 @@ bool team_for(int groups, F launch) {
 
 template <typename T>
 int forward(NormArgs<T> a) {
+    const bool past = past_caches(2.0 * sizeof(T) * a.rows * a.width);
     const bool held = team_for<8192>(groups_of<T>(a.width), [&](auto team, auto e) {
         constexpr int TEAM = decltype(team)::value, E = decltype(e)::value, BLOCK = TEAM > kThreads ? TEAM : kThreads, TEAMS = BLOCK / TEAM;
         const dim3 grid((unsigned)std::min((a.rows + TEAMS - 1) / TEAMS, 8192L * kThreads / BLOCK));
-        if (a.width == TEAM * E * Vec<T>::N) hipLaunchKernelGGL((norm_team<T, TEAM, E, true>), grid, dim3(BLOCK), 0, stream(), a);
-        else hipLaunchKernelGGL((norm_team<T, TEAM, E, false>), grid, dim3(BLOCK), 0, stream(), a);
+        either_way(past, [&](auto p) {
+            either_way(a.width == TEAM * E * Vec<T>::N, [&](auto whole) {
+                hipLaunchKernelGGL((norm_team<T, TEAM, E, decltype(whole)::value, decltype(p)::value>), grid, dim3(BLOCK), 0, stream(), a);
+            });
+        });
     });
-    if (!held) hipLaunchKernelGGL(norm_rows<T>, dim3((unsigned)std::min(a.rows, 65536L)), dim3(1024), 0, stream(), a);
+    if (!held)
+        either_way(past, [&](auto p) { hipLaunchKernelGGL((norm_rows<T, decltype(p)::value>), dim3((unsigned)std::min(a.rows, 65536L)), dim3(1024), 0, stream(), a); });
     return launched("dali_hip_layer_norm");
 }
 
 template <typename T>
 int backward(NormBackwardArgs<T> a) {
+    const bool past = past_caches(3.0 * sizeof(T) * a.rows * a.width);
     const long fit = (long)(kWorkspacePartialBytes / (2 * sizeof(T) * (size_t)a.width));  // rows of partial sums that the workspace holds
     a.partial = (T*)(workspace() + kWorkspaceCounterBytes);
     a.parts = 1;
@@ -433,14 +439,13 @@ int backward(NormBackwardArgs<T> a) {
         // two workgroups to a compute unit, or one of 1024 threads, each with all the rows that fall to it: few partial sums
         a.parts = (int)std::max(1L, std::min({(a.rows + TEAMS - 1) / TEAMS, 512L * 512 / BLOCK, fit}));
         const dim3 grid((unsigned)a.parts);
-        const bool whole = a.width == TEAM * E * Vec<T>::N;
-        auto launch = [&](auto w, auto g) {
-            hipLaunchKernelGGL((norm_backward_team<T, TEAM, E, decltype(w)::value, decltype(g)::value>), grid, dim3(BLOCK), 0, stream(), a);
-        };
-        using std::false_type;
-        using std::true_type;
-        if (a.dgamma) whole ? launch(true_type(), true_type()) : launch(false_type(), true_type());
-        else whole ? launch(true_type(), false_type()) : launch(false_type(), false_type());
+        either_way(past, [&](auto p) {
+            either_way(a.width == TEAM * E * Vec<T>::N, [&](auto whole) {
+                either_way(a.dgamma != nullptr, [&](auto weights) {
+                    hipLaunchKernelGGL((norm_backward_team<T, TEAM, E, decltype(whole)::value, decltype(weights)::value, decltype(p)::value>), grid, dim3(BLOCK), 0, stream(), a);
+                });
+            });
+        });
     });
     if (!held && a.dgamma) {
         // (the weights first: dx may take the place of x or dy)
@@ -448,7 +453,8 @@ int backward(NormBackwardArgs<T> a) {
         hipLaunchKernelGGL(norm_weights<T>, dim3((a.width + kThreads - 1) / kThreads, a.parts), dim3(kThreads), 0, stream(), a);
     }
     if (a.dgamma && a.parts > 1) hipLaunchKernelGGL(norm_fold<T>, dim3((unsigned)((2L * a.width + 15) / 16)), dim3(kThreads), 0, stream(), a);
-    if (!held) hipLaunchKernelGGL(norm_backward_rows<T>, dim3((unsigned)std::min(a.rows, 65536L)), dim3(1024), 0, stream(), a);
+    if (!held)
+        either_way(past, [&](auto p) { hipLaunchKernelGGL((norm_backward_rows<T, decltype(p)::value>), dim3((unsigned)std::min(a.rows, 65536L)), dim3(1024), 0, stream(), a); });
     return launched("dali_hip_layer_norm_backward");
 }
 

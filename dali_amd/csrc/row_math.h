@@ -7,6 +7,7 @@
 
 #include <cstdint>
 #include <initializer_list>
+#include <type_traits>
 
 #include "runtime.h"
 
@@ -39,14 +40,17 @@ __device__ __forceinline__ void load_group(const T* x, int c, int width, T fill,
     }
 }
 
-template <typename T>
+// (PAST: without taking room in the caches, for results that they would not hold until somebody reads them. A condition at run time does not do: the
+// compiler merges the two stores into the ordinary one)
+template <bool PAST = false, typename T>
 __device__ __forceinline__ void store_group(T* out, int c, int width, const T (&v)[Vec<T>::N]) {
     constexpr int N = Vec<T>::N;
     if (c <= width - N) {
         typename Vec<T>::type g;
 #pragma unroll
         for (int i = 0; i < N; ++i) g[i] = v[i];
-        *reinterpret_cast<typename Vec<T>::type*>(out + c) = g;
+        if constexpr (PAST) __builtin_nontemporal_store(g, reinterpret_cast<typename Vec<T>::type*>(out + c));
+        else *reinterpret_cast<typename Vec<T>::type*>(out + c) = g;
     } else {
 #pragma unroll
         for (int i = 0; i < N; ++i)
@@ -130,6 +134,16 @@ __device__ __forceinline__ T fold_block(T v, T* scratch, Op op) {
 template <int THREADS, typename T>
 __device__ __forceinline__ T block_sum(T v, T* scratch) {
     return fold_block<THREADS>(v, scratch, Sum());
+}
+
+// Whether a pass moves so much that the caches (256 MiB) would not hold its result until somebody reads it
+inline bool past_caches(double bytes) { return bytes >= (double)(256L << 20); }
+
+// f(true_type) or f(false_type)
+template <typename F>
+void either_way(bool condition, F f) {
+    if (condition) f(std::true_type());
+    else f(std::false_type());
 }
 
 // Results that another workgroup of the same launch reads: stored past the caches of this one's die, awaited, and announced with a ticket

@@ -648,7 +648,7 @@ struct RowGradient {
 };
 
 // LANES lanes to a row
-template <typename T, int LANES, int E>
+template <typename T, int LANES, int E, bool PAST>
 __global__ __launch_bounds__(kThreads) void log_prob_backward_short(LogProbBackwardArgs<T> a) {
     constexpr int N = Vec<T>::N;
     const int l = threadIdx.x % LANES;
@@ -664,12 +664,12 @@ __global__ __launch_bounds__(kThreads) void log_prob_backward_short(LogProbBackw
         const int c = (l + e * LANES) * N;
 #pragma unroll
         for (int i = 0; i < N; ++i) v[e][i] = q.of(v[e][i], c + i);
-        store_group(a.d_logits + r * a.vocab, c, a.vocab, v[e]);
+        store_group<PAST>(a.d_logits + r * a.vocab, c, a.vocab, v[e]);
     }
 }
 
 // a workgroup to a piece of a row, four groups to a thread
-template <typename T>
+template <typename T, bool PAST>
 __global__ __launch_bounds__(kThreads) void log_prob_backward_long(LogProbBackwardArgs<T> a) {
     constexpr int N = Vec<T>::N, U = 4;
     const long r = blockIdx.x / (unsigned)a.pieces;
@@ -686,7 +686,7 @@ __global__ __launch_bounds__(kThreads) void log_prob_backward_long(LogProbBackwa
         if (c >= a.vocab) break;
 #pragma unroll
         for (int i = 0; i < N; ++i) v[u][i] = q.of(v[u][i], (int)c + i);
-        store_group(a.d_logits + r * a.vocab, (int)c, a.vocab, v[u]);
+        store_group<PAST>(a.d_logits + r * a.vocab, (int)c, a.vocab, v[u]);
     }
 }
 
@@ -761,6 +761,7 @@ int forward(LogProbArgs<T> all) {
 
 template <typename T>
 int backward(LogProbBackwardArgs<T> all) {
+    const bool past = past_caches(2.0 * sizeof(T) * all.rows * all.vocab);
     const int groups = groups_of<T>(all.vocab);
     const long pieces = ((long)groups + 4 * kThreads - 1) / (4 * kThreads);
     for (long done = 0; done < all.rows;) {
@@ -775,10 +776,13 @@ int backward(LogProbBackwardArgs<T> all) {
         a.pieces = (int)pieces;
         if (short_rows<256>(groups, [&](auto lanes, auto e) {
                 constexpr int per = kThreads / decltype(lanes)::value;
-                hipLaunchKernelGGL((log_prob_backward_short<T, decltype(lanes)::value, decltype(e)::value>), dim3((unsigned)((a.rows + per - 1) / per)), dim3(kThreads), 0, stream(), a);
+                either_way(past, [&](auto p) {
+                    hipLaunchKernelGGL((log_prob_backward_short<T, decltype(lanes)::value, decltype(e)::value, decltype(p)::value>), dim3((unsigned)((a.rows + per - 1) / per)),
+                                       dim3(kThreads), 0, stream(), a);
+                });
             }))
             continue;
-        hipLaunchKernelGGL(log_prob_backward_long<T>, dim3((unsigned)(a.rows * pieces)), dim3(kThreads), 0, stream(), a);
+        either_way(past, [&](auto p) { hipLaunchKernelGGL((log_prob_backward_long<T, decltype(p)::value>), dim3((unsigned)(a.rows * pieces)), dim3(kThreads), 0, stream(), a); });
     }
     return launched("dali_hip_token_log_probs_backward");
 }
