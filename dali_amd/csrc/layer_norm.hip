@@ -224,17 +224,34 @@ __global__ __launch_bounds__(TEAM > 512 ? TEAM : 512) void norm_backward_team(No
         for (int i = 0; i < N; ++i) gamma[e][i] = T(1), dgamma[e][i] = dbeta[e][i] = T(0);
         if (a.gamma) load_group(a.gamma, (l + e * TEAM) * N, a.width, T(0), gamma[e]);
     }
-    for (long first = (long)blockIdx.x * TEAMS; first < a.rows; first += (long)gridDim.x * TEAMS) {
-        const long row = first + threadIdx.x / TEAM, r = row < a.rows ? row : a.rows - 1;
-        const bool live = row < a.rows;  // (a team without a row goes along with the last, and adds nothing)
+    // The next row is under way while one is worked on, where the registers hold both
+    constexpr bool AHEAD = TEAM <= 512 || E <= 2;
+    T u[E][N], d[E][N], next_u[AHEAD ? E : 1][N], next_d[AHEAD ? E : 1][N], mean, rstd, next_mean, next_rstd;
+    const long stride = (long)gridDim.x * TEAMS;
+    auto ask = [&](long row, auto& into_u, auto& into_d, T& into_mean, T& into_rstd) {
+        const long r = row < a.rows ? row : a.rows - 1;
         const T *x = a.x + r * a.x_stride, *dy = a.dy + r * a.dy_stride;
-        T u[E][N], d[E][N];
 #pragma unroll
         for (int e = 0; e < E; ++e) {
-            load_group(x, (l + e * TEAM) * N, a.width, T(0), u[e]);
-            load_group(dy, (l + e * TEAM) * N, a.width, T(0), d[e]);
+            load_group(x, (l + e * TEAM) * N, a.width, T(0), into_u[e]);
+            load_group(dy, (l + e * TEAM) * N, a.width, T(0), into_d[e]);
         }
-        const T mean = a.mean[r], rstd = a.rstd[r];
+        into_mean = a.mean[r], into_rstd = a.rstd[r];
+    };
+    if constexpr (AHEAD) ask((long)blockIdx.x * TEAMS + threadIdx.x / TEAM, next_u, next_d, next_mean, next_rstd);
+    for (long first = (long)blockIdx.x * TEAMS; first < a.rows; first += stride) {
+        const long row = first + threadIdx.x / TEAM, r = row < a.rows ? row : a.rows - 1;
+        const bool live = row < a.rows;  // (a team without a row goes along with the last, and adds nothing)
+        if constexpr (AHEAD) {
+#pragma unroll
+            for (int e = 0; e < E; ++e)
+#pragma unroll
+                for (int i = 0; i < N; ++i) u[e][i] = next_u[e][i], d[e][i] = next_d[e][i];
+            mean = next_mean, rstd = next_rstd;
+            if (first + stride < a.rows) ask(row + stride, next_u, next_d, next_mean, next_rstd);
+        } else {
+            ask(row, u, d, mean, rstd);
+        }
         T level = 0, along = 0;
 #pragma unroll
         for (int e = 0; e < E; ++e)
@@ -370,7 +387,7 @@ __global__ __launch_bounds__(kThreads) void norm_fold(NormBackwardArgs<T> a) {
     T s = 0;
     if (c < columns) {
         const T* from = a.partial + c;
-#pragma unroll 8
+#pragma unroll 16
         for (int k = p; k < a.parts; k += 16) s += from[k * columns];
     }
     joined[p][i] = s;
@@ -400,7 +417,7 @@ bool team_for(int groups, F launch) {
     if (groups <= 256) return with(integral_constant<int, 64>(), integral_constant<int, 4>());
     if (groups <= 512) return with(integral_constant<int, 512>(), integral_constant<int, 1>());
     if (groups <= 1024) return with(integral_constant<int, 512>(), integral_constant<int, 2>());
-    if (groups <= 2048) return with(integral_constant<int, 512>(), integral_constant<int, 4>());
+    if (groups <= 2048) return with(integral_constant<int, 1024>(), integral_constant<int, 2>());
     if (groups <= 4096) return with(integral_constant<int, 1024>(), integral_constant<int, 4>());
     if constexpr (MOST > 4096)
         if (groups <= 8192) return with(integral_constant<int, 1024>(), integral_constant<int, 8>());
@@ -436,8 +453,10 @@ int backward(NormBackwardArgs<T> a) {
     }
     const bool held = team_for<4096>(groups_of<T>(a.width), [&](auto team, auto e) {
         constexpr int TEAM = decltype(team)::value, E = decltype(e)::value, BLOCK = TEAM > 512 ? TEAM : 512, TEAMS = BLOCK / TEAM;
-        // two workgroups to a compute unit, or one of 1024 threads, each with all the rows that fall to it: few partial sums
-        a.parts = (int)std::max(1L, std::min({(a.rows + TEAMS - 1) / TEAMS, 512L * 512 / BLOCK, fit}));
+        // As many workgroups as the registers let run at once, each with all the rows that fall to it; rows of two groups to a thread of 512 have half of that
+        // where there are rows enough, for fewer partial sums
+        const int per_unit = TEAM <= 64 ? (E == 4 ? 1 : TEAM == 64 && E == 1 ? 4 : 2) : TEAM == 512 && (E == 1 || (E == 2 && a.rows < 8192)) ? 2 : 1;
+        a.parts = (int)std::max(1L, std::min({(a.rows + TEAMS - 1) / TEAMS, 256L * per_unit, fit}));
         const dim3 grid((unsigned)a.parts);
         either_way(past, [&](auto p) {
             either_way(a.width == TEAM * E * Vec<T>::N, [&](auto whole) {
