@@ -51,11 +51,15 @@ __device__ __forceinline__ void walk(const Batch& a, int b, F f) {
     const int count = (int)min((long)a.chunk, a.n[i] - begin);
     const T* x = (const T*)a.in[i] + begin;
     for (int c = threadIdx.x * N; c < count; c += kUnroll * STEP) {
-        T v[kUnroll][N];
+        typename Vec<T>::type g[kUnroll];
 #pragma unroll
-        for (int u = 0; u < kUnroll; ++u) load_group(x, min(c + u * STEP, count), count, T(0), v[u]);
+        for (int u = 0; u < kUnroll; ++u) g[u] = ask_group(x, c + u * STEP, count);
 #pragma unroll
-        for (int u = 0; u < kUnroll; ++u) f(i, begin, c + u * STEP, count, v[u]);
+        for (int u = 0; u < kUnroll; ++u) {
+            T v[N];
+            take_group(g[u], c + u * STEP, count, T(0), v);
+            f(i, begin, c + u * STEP, count, v);
+        }
     }
 }
 

@@ -56,7 +56,7 @@ __device__ __forceinline__ T root_of(T variance, T epsilon) {
 template <typename T, int TEAM, int E, bool WHOLE, bool PAST>
 __global__ __launch_bounds__(TEAM > kThreads ? TEAM : kThreads) void norm_team(NormArgs<T> a) {
     constexpr int N = Vec<T>::N, BLOCK = TEAM > kThreads ? TEAM : kThreads, TEAMS = BLOCK / TEAM;
-    constexpr bool HOLD = E * N <= 16;
+    constexpr bool HOLD = E * N <= 16, LONG = TEAM > 8;  // (8 threads are given the shortest rows)
     __shared__ TeamScratch<T, TEAM> scratch;
     int turn = 0;
     const int l = threadIdx.x % TEAM;
@@ -84,14 +84,17 @@ __global__ __launch_bounds__(TEAM > kThreads ? TEAM : kThreads) void norm_team(N
     for (long first = (long)blockIdx.x * TEAMS; first < a.rows; first += (long)gridDim.x * TEAMS) {
         const long row = first + threadIdx.x / TEAM, r = row < a.rows ? row : a.rows - 1;  // (a team without a row goes along with the last)
         const T* x = a.x + r * a.stride;
+        typename Vec<T>::type group[E];
         T v[E][N];
         T s = 0, none = 0;
 #pragma unroll
-        for (int e = 0; e < E; ++e) load_group(x, (l + e * TEAM) * N, a.width, T(0), v[e]);
+        for (int e = 0; e < E; ++e) group[e] = ask_group<LONG, WHOLE>(x, (l + e * TEAM) * N, a.width);
 #pragma unroll
-        for (int e = 0; e < E; ++e)
+        for (int e = 0; e < E; ++e) {
+            take_group<LONG, WHOLE>(group[e], (l + e * TEAM) * N, a.width, T(0), v[e]);
 #pragma unroll
             for (int i = 0; i < N; ++i) s += v[e][i];
+        }
         team_sum<TEAM>(s, none, scratch, turn);
         const T near = s / count;
         T off = 0, square = 0;
@@ -209,6 +212,7 @@ __device__ __forceinline__ T plus_across(T v) {
 template <typename T, int TEAM, int E, bool WHOLE, bool WEIGHTS, bool PAST>
 __global__ __launch_bounds__(TEAM > 512 ? TEAM : 512) void norm_backward_team(NormBackwardArgs<T> a) {
     constexpr int N = Vec<T>::N, BLOCK = TEAM > 512 ? TEAM : 512, TEAMS = BLOCK / TEAM;
+    constexpr bool LONG = TEAM > 8;  // (8 threads are given the shortest rows)
     // (waves that hold the same columns; LDS for half of them)
     constexpr int SPAN = TEAM > 64 ? TEAM : 64, SAME = BLOCK / SPAN;
     __shared__ TeamScratch<T, TEAM> scratch;
@@ -226,39 +230,39 @@ __global__ __launch_bounds__(TEAM > 512 ? TEAM : 512) void norm_backward_team(No
     }
     // The next row is under way while one is worked on, where the registers hold both
     constexpr bool AHEAD = TEAM <= 512 || E <= 2;
-    T u[E][N], d[E][N], next_u[AHEAD ? E : 1][N], next_d[AHEAD ? E : 1][N], mean, rstd, next_mean, next_rstd;
+    typename Vec<T>::type asked_x[E], asked_dy[E];
+    T mean, rstd;
     const long stride = (long)gridDim.x * TEAMS;
-    auto ask = [&](long row, auto& into_u, auto& into_d, T& into_mean, T& into_rstd) {
+    auto ask = [&](long row) {
         const long r = row < a.rows ? row : a.rows - 1;
-        const T *x = a.x + r * a.x_stride, *dy = a.dy + r * a.dy_stride;
 #pragma unroll
         for (int e = 0; e < E; ++e) {
-            load_group(x, (l + e * TEAM) * N, a.width, T(0), into_u[e]);
-            load_group(dy, (l + e * TEAM) * N, a.width, T(0), into_d[e]);
+            asked_x[e] = ask_group<LONG, WHOLE>(a.x + r * a.x_stride, (l + e * TEAM) * N, a.width);
+            asked_dy[e] = ask_group<LONG, WHOLE>(a.dy + r * a.dy_stride, (l + e * TEAM) * N, a.width);
         }
-        into_mean = a.mean[r], into_rstd = a.rstd[r];
+        mean = a.mean[r], rstd = a.rstd[r];
     };
-    if constexpr (AHEAD) ask((long)blockIdx.x * TEAMS + threadIdx.x / TEAM, next_u, next_d, next_mean, next_rstd);
+    if constexpr (AHEAD) ask((long)blockIdx.x * TEAMS + threadIdx.x / TEAM);
     for (long first = (long)blockIdx.x * TEAMS; first < a.rows; first += stride) {
         const long row = first + threadIdx.x / TEAM, r = row < a.rows ? row : a.rows - 1;
         const bool live = row < a.rows;  // (a team without a row goes along with the last, and adds nothing)
-        if constexpr (AHEAD) {
+        if constexpr (!AHEAD) ask(row);
+        const T row_mean = mean, row_rstd = rstd;
+        T u[E][N], d[E][N];
 #pragma unroll
-            for (int e = 0; e < E; ++e)
-#pragma unroll
-                for (int i = 0; i < N; ++i) u[e][i] = next_u[e][i], d[e][i] = next_d[e][i];
-            mean = next_mean, rstd = next_rstd;
-            if (first + stride < a.rows) ask(row + stride, next_u, next_d, next_mean, next_rstd);
-        } else {
-            ask(row, u, d, mean, rstd);
+        for (int e = 0; e < E; ++e) {
+            take_group<LONG, WHOLE>(asked_x[e], (l + e * TEAM) * N, a.width, T(0), u[e]);
+            take_group<LONG, WHOLE>(asked_dy[e], (l + e * TEAM) * N, a.width, T(0), d[e]);
         }
+        if constexpr (AHEAD)
+            if (first + stride < a.rows) ask(row + stride);
         T level = 0, along = 0;
 #pragma unroll
         for (int e = 0; e < E; ++e)
 #pragma unroll
             for (int i = 0; i < N; ++i) {
                 const bool in = WHOLE || (l + e * TEAM) * N + i < a.width;
-                u[e][i] = in ? (u[e][i] - mean) * rstd : T(0);
+                u[e][i] = in ? (u[e][i] - row_mean) * row_rstd : T(0);
                 if constexpr (WEIGHTS) {
                     dgamma[e][i] += live ? d[e][i] * u[e][i] : T(0);
                     dbeta[e][i] += live ? d[e][i] : T(0);
@@ -274,7 +278,7 @@ __global__ __launch_bounds__(TEAM > 512 ? TEAM : 512) void norm_backward_team(No
 #pragma unroll
             for (int e = 0; e < E; ++e) {
 #pragma unroll
-                for (int i = 0; i < N; ++i) d[e][i] = rstd * ((d[e][i] - level) - u[e][i] * along);
+                for (int i = 0; i < N; ++i) d[e][i] = row_rstd * ((d[e][i] - level) - u[e][i] * along);
                 store_group<PAST>(a.dx + r * a.width, (l + e * TEAM) * N, a.width, d[e]);
             }
         }

@@ -26,18 +26,40 @@ __host__ __device__ __forceinline__ int groups_of(int width) {
     return width / Vec<T>::N + (width % Vec<T>::N != 0);
 }
 
-// the group of values that begins at c, with `fill` in the place of what lies past the row's end
+// The group of values that begins at c, in two steps: the access, which reads the row's last whole group where c lies past its beginning, so that it needs no
+// branch and many are under way at once; and the values, moved to their places, with `fill` past the row's end. Rows shorter than a group are read one by one;
+// LONG: the row is known not to be, WHOLE: nor to end inside a group or before c.
+template <bool LONG = false, bool WHOLE = false, typename T>
+__device__ __forceinline__ typename Vec<T>::type ask_group(const T* x, int c, int width) {
+    constexpr int N = Vec<T>::N;
+    if constexpr (WHOLE) return *reinterpret_cast<const typename Vec<T>::type*>(x + c);
+    if (LONG || width >= N) return *reinterpret_cast<const typename Vec<T>::type*>(x + min(c, width - N));
+    typename Vec<T>::type g;
+#pragma unroll
+    for (int i = 0; i < N; ++i) g[i] = c + i < width ? x[c + i] : T(0);
+    return g;
+}
+template <bool LONG = false, bool WHOLE = false, typename T>
+__device__ __forceinline__ void take_group(const typename Vec<T>::type& g, int c, int width, T fill, T (&v)[Vec<T>::N]) {
+    constexpr int N = Vec<T>::N;
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = g[i];
+    if constexpr (WHOLE) return;
+    const int off = c - (width - N);
+    if (off <= 0) return;
+    if (LONG || width >= N) {
+#pragma unroll
+        for (int bit = 1; bit < N; bit *= 2)
+            if (off & bit)
+#pragma unroll
+                for (int i = 0; i < N; ++i) v[i] = i + bit < N ? v[i + bit < N ? i + bit : 0] : fill;
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = c + i < width ? v[i] : fill;
+}
 template <typename T>
 __device__ __forceinline__ void load_group(const T* x, int c, int width, T fill, T (&v)[Vec<T>::N]) {
-    constexpr int N = Vec<T>::N;
-    if (c <= width - N) {
-        const typename Vec<T>::type g = *reinterpret_cast<const typename Vec<T>::type*>(x + c);
-#pragma unroll
-        for (int i = 0; i < N; ++i) v[i] = g[i];
-    } else {
-#pragma unroll
-        for (int i = 0; i < N; ++i) v[i] = c + i < width ? x[c + i] : fill;
-    }
+    take_group(ask_group(x, c, width), c, width, fill, v);
 }
 
 // (PAST: without taking room in the caches, for results that they would not hold until somebody reads them. A condition at run time does not do: the

@@ -276,9 +276,12 @@ __global__ __launch_bounds__(kThreads) void log_prob_short(LogProbArgs<T> a) {
     const bool live = row < a.rows;
     const long r = live ? row : a.rows - 1;  // (lanes without a row go along with the last)
     const T* x = a.logits + r * a.stride;
+    typename Vec<T>::type g[E];
     T v[E][N];
 #pragma unroll
-    for (int e = 0; e < E; ++e) load_group(x, (l + e * LANES) * N, a.vocab, T(-INFINITY), v[e]);
+    for (int e = 0; e < E; ++e) g[e] = ask_group<(LANES > 8)>(x, (l + e * LANES) * N, a.vocab);
+#pragma unroll
+    for (int e = 0; e < E; ++e) take_group<(LANES > 8)>(g[e], (l + e * LANES) * N, a.vocab, T(-INFINITY), v[e]);
     const int token = a.tokens[r];
     const T own = token >= 0 && token < a.vocab ? x[token] : T(0);
     T m = Real<T>::lowest;
@@ -575,12 +578,13 @@ __global__ __launch_bounds__(kThreads) void log_prob_segments(LogProbArgs<T> a) 
     const int segment = (int)(blockIdx.x - (unsigned)r * (unsigned)a.segments);
     const T* x = a.logits + r * a.stride;
     const int begin = segment * a.per, end = min(groups_of<T>(a.vocab), begin + a.per);
+    typename Vec<T>::type asked[E];
     T v[E][N];
+    auto at = [&](int e) { return begin + tid + e * kThreads < end ? (begin + tid + e * kThreads) * N : a.vocab; };
 #pragma unroll
-    for (int e = 0; e < E; ++e) {
-        const int g = begin + tid + e * kThreads;
-        load_group(x, g < end ? g * N : a.vocab, a.vocab, T(-INFINITY), v[e]);
-    }
+    for (int e = 0; e < E; ++e) asked[e] = ask_group<true>(x, at(e), a.vocab);
+#pragma unroll
+    for (int e = 0; e < E; ++e) take_group<true>(asked[e], at(e), a.vocab, T(-INFINITY), v[e]);
     const int token = a.tokens[r];
     const T own = token >= 0 && token < a.vocab ? x[token] : T(0);
     Sums<T> q;
@@ -655,16 +659,18 @@ __global__ __launch_bounds__(kThreads) void log_prob_backward_short(LogProbBackw
     const long r = (long)blockIdx.x * (kThreads / LANES) + threadIdx.x / LANES;
     if (r >= a.rows) return;
     const T* x = a.logits + r * a.stride;
-    T v[E][N];
+    typename Vec<T>::type g[E];
 #pragma unroll
-    for (int e = 0; e < E; ++e) load_group(x, (l + e * LANES) * N, a.vocab, T(-INFINITY), v[e]);
+    for (int e = 0; e < E; ++e) g[e] = ask_group<(LANES > 8)>(x, (l + e * LANES) * N, a.vocab);
     const RowGradient<T> q(a, r);
 #pragma unroll
     for (int e = 0; e < E; ++e) {
         const int c = (l + e * LANES) * N;
+        T v[N];
+        take_group<(LANES > 8)>(g[e], c, a.vocab, T(-INFINITY), v);
 #pragma unroll
-        for (int i = 0; i < N; ++i) v[e][i] = q.of(v[e][i], c + i);
-        store_group<PAST>(a.d_logits + r * a.vocab, c, a.vocab, v[e]);
+        for (int i = 0; i < N; ++i) v[i] = q.of(v[i], c + i);
+        store_group<PAST>(a.d_logits + r * a.vocab, c, a.vocab, v);
     }
 }
 
@@ -677,16 +683,18 @@ __global__ __launch_bounds__(kThreads) void log_prob_backward_long(LogProbBackwa
     const T* x = a.logits + r * a.stride;
     const RowGradient<T> q(a, r);
     const int first = (piece * U * kThreads + (int)threadIdx.x) * N;  // (the last group of the longest row ends at 2^31 - 1)
-    T v[U][N];
+    typename Vec<T>::type g[U];
 #pragma unroll
-    for (int u = 0; u < U; ++u) load_group(x, min((long)first + u * kThreads * N, (long)a.vocab), a.vocab, T(-INFINITY), v[u]);
+    for (int u = 0; u < U; ++u) g[u] = ask_group<true>(x, (int)min((long)first + u * kThreads * N, (long)a.vocab), a.vocab);
 #pragma unroll
     for (int u = 0; u < U; ++u) {
         const long c = (long)first + u * kThreads * N;
         if (c >= a.vocab) break;
+        T v[N];
+        take_group<true>(g[u], (int)c, a.vocab, T(-INFINITY), v);
 #pragma unroll
-        for (int i = 0; i < N; ++i) v[u][i] = q.of(v[u][i], (int)c + i);
-        store_group<PAST>(a.d_logits + r * a.vocab, (int)c, a.vocab, v[u]);
+        for (int i = 0; i < N; ++i) v[i] = q.of(v[i], (int)c + i);
+        store_group<PAST>(a.d_logits + r * a.vocab, (int)c, a.vocab, v);
     }
 }
 
