@@ -67,17 +67,19 @@ const void* read(const Array& a) { return a.is_stateless() ? nullptr : a.device_
 // (what a destination held stays if the call is refused)
 void* write(const Array& a) { return a.is_stateless() ? nullptr : a.device_ptr(memory::AM_MUTABLE); }
 
-// issues the launch now and, while a recording is open, on every replay; `keep`: all that it reads and writes
-void issue(const char* kind, const std::vector<Array>& keep, const std::vector<Array>& written, const std::function<int()>& launch) {
-    if (g_dry_run) return;
+// Issues the launch now and, while a recording is open, on every replay. `keep`: makes the list of all arrays that it reads, and of those that it writes.
+template <typename Launch, typename Keep>
+void issue(const char* kind, const Launch& launch, const Keep& keep) {
     DALI_SCOPE(kind);
     check_hip(launch(), kind);
     jit_stats().kernels_launched++;
     jit_stats().last_kernel_kinds = kind;
     if (!g_recording) return;
-    for (const Array& a : written)
+    std::vector<Array> reads, writes;
+    keep(reads, writes);
+    for (const Array& a : writes)
         if (!a.is_stateless()) note_recorded_write(a.expression()->memory);
-    g_recording->push_back([kind, keep, written, launch]() { check_hip(launch(), kind); });
+    g_recording->push_back([kind, reads, writes, launch]() { check_hip(launch(), kind); });
 }
 
 }  // namespace
@@ -100,7 +102,9 @@ LayerNorm layer_norm(const Array& x, const Array& gamma, const Array& beta, doub
     void *yp = write(r.y), *mp = write(r.mean), *sp = write(r.rstd);
     const int64_t rows = in.rows, stride = in.stride;
     const int width = in.width;
-    issue(what, {in.array, g, b}, {r.y, r.mean, r.rstd}, [=]() { return dali_hip_layer_norm(dtype, rows, width, xp, stride, gp, bp, epsilon, yp, mp, sp); });
+    issue(
+        what, [=]() { return dali_hip_layer_norm(dtype, rows, width, xp, stride, gp, bp, epsilon, yp, mp, sp); },
+        [&](std::vector<Array>& reads, std::vector<Array>& writes) { reads = {in.array, g, b}, writes = {r.y, r.mean, r.rstd}; });
     return r;
 }
 
@@ -127,8 +131,9 @@ LayerNormGradient layer_norm_backward(const Array& dy, const Array& x, const Arr
     void *dxp = write(r.x), *dgp = write(r.gamma), *dbp = write(r.beta);
     const int64_t rows = in.rows, x_stride = in.stride, dy_stride = gy.stride;
     const int width = in.width;
-    issue(what, {gy.array, in.array, m, s, g}, {r.x, r.gamma, r.beta},
-          [=]() { return dali_hip_layer_norm_backward(dtype, rows, width, dyp, dy_stride, xp, x_stride, mp, sp, gp, dxp, dgp, dbp); });
+    issue(
+        what, [=]() { return dali_hip_layer_norm_backward(dtype, rows, width, dyp, dy_stride, xp, x_stride, mp, sp, gp, dxp, dgp, dbp); },
+        [&](std::vector<Array>& reads, std::vector<Array>& writes) { reads = {gy.array, in.array, m, s, g}, writes = {r.x, r.gamma, r.beta}; });
     return r;
 }
 
@@ -158,8 +163,9 @@ TokenLogProbs token_log_probs(const Array& logits, const Array& tokens, int k, c
     void *pp = write(r.log_probs), *ep = write(r.entropy), *lp = write(r.lse), *vp = write(r.top_log_probs), *ip = write(r.top_tokens);
     const int64_t rows = in.rows, stride = in.stride;
     const int vocab = in.width;
-    issue(what, {in.array, t}, {r.log_probs, r.entropy, r.lse, r.top_log_probs, r.top_tokens},
-          [=]() { return dali_hip_token_log_probs(dtype, rows, vocab, xp, stride, (const int32_t*)tp, k, pp, ep, lp, vp, (int32_t*)ip); });
+    issue(
+        what, [=]() { return dali_hip_token_log_probs(dtype, rows, vocab, xp, stride, (const int32_t*)tp, k, pp, ep, lp, vp, (int32_t*)ip); },
+        [&](std::vector<Array>& reads, std::vector<Array>& writes) { reads = {in.array, t}, writes = {r.log_probs, r.entropy, r.lse, r.top_log_probs, r.top_tokens}; });
     return r;
 }
 
@@ -187,33 +193,43 @@ Array token_log_probs_backward(const Array& d_log_probs, const Array& d_entropy,
     void* rp = write(r);
     const int64_t rows = in.rows, stride = in.stride;
     const int vocab = in.width;
-    issue(what, {in.array, g, t, l, h, e}, {r},
-          [=]() { return dali_hip_token_log_probs_backward(dtype, rows, vocab, gp, hp, xp, stride, (const int32_t*)tp, lp, ep, rp); });
+    issue(
+        what, [=]() { return dali_hip_token_log_probs_backward(dtype, rows, vocab, gp, hp, xp, stride, (const int32_t*)tp, lp, ep, rp); },
+        [&](std::vector<Array>& reads, std::vector<Array>& writes) { reads = {in.array, g, t, l, h, e}, writes = {r}; });
     return r;
 }
 
 static Array norm_of(const char* what, const std::vector<Array>& arrays, double max_norm, const std::vector<Array>* clipped, const Array& out) {
     DALI_ASSERT(!arrays.empty(), make_message(what, ": needs at least one array"));
+    const size_t count = arrays.size();
     const DType dtype = arrays[0].dtype();
-    std::vector<Array> in;
-    std::vector<const void*> from;
-    std::vector<void*> to;
-    std::vector<int64_t> sizes;
-    for (const Array& a : arrays) {
-        DALI_ASSERT(is_real(a) && a.dtype() == dtype, make_message(what, ": the arrays must be float or double, all of one type"));
-        in.push_back(dense(a));
-        sizes.push_back(a.number_of_elements());
-    }
+    std::vector<Array> laid_out;  // of arrays that are not dense
+    std::vector<void*> pointers(2 * count);
+    std::vector<int64_t> sizes(count);
+    for (const Array& a : arrays) DALI_ASSERT(is_real(a) && a.dtype() == dtype, make_message(what, ": the arrays must be float or double, all of one type"));
     const Array norm = destination(what, "the norm", out, {}, dtype);
     if (g_dry_run) return norm;
-    for (const Array& a : in) from.push_back(read(a));
+    for (size_t i = 0; i < count; ++i) {
+        const Array a = dense(arrays[i]);
+        sizes[i] = a.number_of_elements();
+        pointers[i] = a.device_ptr();
+        if (a.state_ != arrays[i].state_) laid_out.push_back(a);
+    }
     if (clipped)
-        for (const Array& a : *clipped) to.push_back(write(a));
+        for (size_t i = 0; i < count; ++i) pointers[count + i] = write((*clipped)[i]);
     void* np = write(norm);
-    std::vector<Array> written = clipped ? *clipped : std::vector<Array>();
-    written.push_back(norm);
-    issue(what, in, written,
-          [=]() { return dali_hip_clip_by_global_norm(dtype, (int)from.size(), from.data(), to.empty() ? nullptr : to.data(), sizes.data(), max_norm, np); });
+    const bool clip = clipped != nullptr;
+    issue(
+        what,
+        [dtype, count, pointers, sizes, max_norm, clip, np]() {
+            return dali_hip_clip_by_global_norm(dtype, (int)count, pointers.data(), clip ? pointers.data() + count : nullptr, sizes.data(), max_norm, np);
+        },
+        [&](std::vector<Array>& reads, std::vector<Array>& writes) {
+            reads = arrays;
+            reads.insert(reads.end(), laid_out.begin(), laid_out.end());
+            if (clipped) writes = *clipped;
+            writes.push_back(norm);
+        });
     return norm;
 }
 
