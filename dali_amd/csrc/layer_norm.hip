@@ -24,14 +24,14 @@ struct NormArgs {
     T epsilon;
 };
 
-// Sums over the team of TEAM threads that holds a row: lanes of a wave, or a workgroup of whole waves, which meets once per call. `scratch` has two halves that take
-// turns, so that a wave may write the next sums while another still reads these.
-template <typename T, int TEAM>
+// Sums over the team of TEAM threads that holds a row: lanes of a wave, or whole waves of a workgroup, all of which meet once per call. `scratch` has two halves
+// that take turns, so that a wave may write the next sums while another still reads these.
+template <typename T, int TEAM, int TEAMS = 1>
 struct TeamScratch {
-    T v[TEAM > 64 ? 2 : 1][TEAM > 64 ? TEAM / 64 : 1][2];
+    T v[TEAM > 64 ? 2 : 1][TEAM > 64 ? TEAMS * TEAM / 64 : 1][2];
 };
-template <int TEAM, typename T>
-__device__ __forceinline__ void team_sum(T& p, T& q, TeamScratch<T, TEAM>& scratch, int& turn) {
+template <int TEAM, typename T, int TEAMS>
+__device__ __forceinline__ void team_sum(T& p, T& q, TeamScratch<T, TEAM, TEAMS>& scratch, int& turn) {
     p = fold_lanes<(TEAM < 64 ? TEAM : 64)>(p, Sum());
     q = fold_lanes<(TEAM < 64 ? TEAM : 64)>(q, Sum());
     if constexpr (TEAM > 64) {
@@ -39,9 +39,10 @@ __device__ __forceinline__ void team_sum(T& p, T& q, TeamScratch<T, TEAM>& scrat
         turn ^= 1;
         if ((threadIdx.x & 63) == 0) s[threadIdx.x >> 6][0] = p, s[threadIdx.x >> 6][1] = q;
         __syncthreads();
-        p = s[0][0], q = s[0][1];
+        const int from = TEAMS == 1 ? 0 : threadIdx.x / TEAM * (TEAM / 64);
+        p = s[from][0], q = s[from][1];
 #pragma unroll
-        for (int w = 1; w < TEAM / 64; ++w) p += s[w][0], q += s[w][1];
+        for (int w = 1; w < TEAM / 64; ++w) p += s[from + w][0], q += s[from + w][1];
     }
 }
 
@@ -209,15 +210,14 @@ __device__ __forceinline__ T plus_across(T v) {
 
 // The gradient with the rows in registers as above; a thread also keeps the sums of its columns over all rows that its team takes. At the end the teams of a
 // workgroup are joined, lanes first and then waves through LDS, in halves, and the workgroup leaves one row of partial sums for each weight.
-template <typename T, int TEAM, int E, bool WHOLE, bool WEIGHTS, bool PAST>
-__global__ __launch_bounds__(TEAM > 512 ? TEAM : 512) void norm_backward_team(NormBackwardArgs<T> a) {
-    constexpr int N = Vec<T>::N, BLOCK = TEAM > 512 ? TEAM : 512, TEAMS = BLOCK / TEAM;
+template <typename T, int TEAM, int TEAMS, int E, bool WHOLE, bool WEIGHTS, bool PAST>
+__global__ __launch_bounds__(TEAM * TEAMS) void norm_backward_team(NormBackwardArgs<T> a) {
+    constexpr int N = Vec<T>::N, BLOCK = TEAM * TEAMS;
     constexpr bool LONG = TEAM > 8;  // (8 threads are given the shortest rows)
     // (waves that hold the same columns; LDS for half of them)
     constexpr int SPAN = TEAM > 64 ? TEAM : 64, SAME = BLOCK / SPAN;
-    __shared__ TeamScratch<T, TEAM> scratch;
+    __shared__ TeamScratch<T, TEAM, TEAMS> scratch;
     __shared__ T joined[WEIGHTS && SAME > 1 ? SAME / 2 : 1][WEIGHTS && SAME > 1 ? 2 * E * N : 1][WEIGHTS && SAME > 1 ? SPAN : 1];
-    static_assert(TEAM <= 64 || TEAMS == 1, "a team of several waves is a workgroup");
     int turn = 0;
     const int l = threadIdx.x % TEAM;
     const T count = a.width;
@@ -456,19 +456,29 @@ int backward(NormBackwardArgs<T> a) {
         return launched("dali_hip_layer_norm_backward");
     }
     const bool held = team_for<4096>(groups_of<T>(a.width), [&](auto team, auto e) {
-        constexpr int TEAM = decltype(team)::value, E = decltype(e)::value, BLOCK = TEAM > 512 ? TEAM : 512, TEAMS = BLOCK / TEAM;
-        // As many workgroups as the registers let run at once, each with all the rows that fall to it; rows of two groups to a thread of 512 have half of that
-        // where there are rows enough, for fewer partial sums
-        const int per_unit = TEAM <= 64 ? (E == 4 ? 1 : TEAM == 64 && E == 1 ? 4 : 2) : TEAM == 512 && (E == 1 || (E == 2 && a.rows < 8192)) ? 2 : 1;
-        a.parts = (int)std::max(1L, std::min({(a.rows + TEAMS - 1) / TEAMS, 256L * per_unit, fit}));
-        const dim3 grid((unsigned)a.parts);
-        either_way(past, [&](auto p) {
-            either_way(a.width == TEAM * E * Vec<T>::N, [&](auto whole) {
-                either_way(a.dgamma != nullptr, [&](auto weights) {
-                    hipLaunchKernelGGL((norm_backward_team<T, TEAM, E, decltype(whole)::value, decltype(weights)::value, decltype(p)::value>), grid, dim3(BLOCK), 0, stream(), a);
+        constexpr int TEAM = decltype(team)::value, E = decltype(e)::value;
+        // as many workgroups as the registers let run at once, each with all the rows that fall to it
+        auto run = [&](auto teams) {
+            constexpr int TEAMS = decltype(teams)::value, per_unit = TEAM > 64 || E == 4 ? 1 : TEAM == 64 && E == 1 ? 4 : 2;
+            a.parts = (int)std::max(1L, std::min({(a.rows + TEAMS - 1) / TEAMS, 256L * per_unit, fit}));
+            const dim3 grid((unsigned)a.parts);
+            either_way(past, [&](auto p) {
+                either_way(a.width == TEAM * E * Vec<T>::N, [&](auto whole) {
+                    either_way(a.dgamma != nullptr, [&](auto weights) {
+                        hipLaunchKernelGGL((norm_backward_team<T, TEAM, TEAMS, E, decltype(whole)::value, decltype(weights)::value, decltype(p)::value>), grid, dim3(TEAM * TEAMS), 0,
+                                           stream(), a);
+                    });
                 });
             });
-        });
+        };
+        // Two teams of 512 threads share a workgroup and its partial sums; where rows are many and a team holds two groups to a thread, one team to a compute unit
+        // streams faster (32768x4096: 280 us, two teams 305; 4000x4096: 46 and 43)
+        if constexpr (TEAM == 512) {
+            if (E == 2 && a.rows >= 8192) run(std::integral_constant<int, 1>());
+            else run(std::integral_constant<int, 2>());
+        } else {
+            run(std::integral_constant<int, (TEAM > 512 ? 1 : 512 / TEAM)>());
+        }
     });
     if (!held && a.dgamma) {
         // (the weights first: dx may take the place of x or dy)
