@@ -419,6 +419,11 @@ bool team_for(int groups, F launch) {
     if (groups <= 128) return with(integral_constant<int, 64>(), integral_constant<int, 2>());
     if (groups <= 192) return with(integral_constant<int, 64>(), integral_constant<int, 3>());
     if (groups <= 256) return with(integral_constant<int, 64>(), integral_constant<int, 4>());
+    if constexpr (MOST > 4096) {
+        if (groups <= 512) return with(integral_constant<int, 256>(), integral_constant<int, 2>());
+        if (groups <= 1024) return with(integral_constant<int, 256>(), integral_constant<int, 4>());
+        if (groups <= 2048) return with(integral_constant<int, 512>(), integral_constant<int, 4>());
+    }
     if (groups <= 512) return with(integral_constant<int, 512>(), integral_constant<int, 1>());
     if (groups <= 1024) return with(integral_constant<int, 512>(), integral_constant<int, 2>());
     if (groups <= 2048) return with(integral_constant<int, 1024>(), integral_constant<int, 2>());
