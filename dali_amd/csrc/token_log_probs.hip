@@ -115,6 +115,18 @@ __device__ __forceinline__ int place_in_wave(const Entry<T>& e) {
     return place;
 }
 
+// The k-th best of a wave's entries, in every lane: a few by taking the best away one after the other, more by counting places
+constexpr int kOneByOne = 12;
+template <typename T>
+__device__ __forceinline__ Entry<T> kth_of_wave(Entry<T> e, int k) {
+    if (k > kOneByOne) return e.lane(__builtin_ctzll(__ballot(place_in_wave(e) == k - 1)));
+    for (int n = 1; n < k; ++n) {
+        const Entry<T> best = best_of_lanes<64>(e);
+        e = Entry<T>::either(best.better(e), e, Entry<T>::none());
+    }
+    return best_of_lanes<64>(e);
+}
+
 template <typename T>
 struct LogProbArgs {
     const T* logits;
@@ -161,36 +173,32 @@ __device__ __forceinline__ void write_alternative(const LogProbArgs<T>& a, long 
 // Entries of one wave that are ranked at once
 constexpr int kWaveList = 128;
 
-// The k best of the entries that a wave holds in registers, E groups to a lane, E > 1: the k-th best of the lanes' own best bounds them, what passes it is collected
-// and ranked. False where the list does not hold them.
+// The k best of the entries that a wave holds in registers, E groups to a lane, E > 1: the k-th best of the lanes' best groups (`top`, and the group's number) bounds
+// them, what passes it is collected and ranked. False where the list does not hold them.
 template <typename T, int E, typename Put>
-__device__ __forceinline__ bool best_by_bound(const T (&v)[E][Vec<T>::N], int l, int vocab, int k, Entry<T>* list, int* count, Put put) {
+__device__ __forceinline__ bool best_by_bound(const T (&v)[E][Vec<T>::N], T top, int top_group, int l, int vocab, int k, Entry<T>* list, int* count, Put put) {
     constexpr int N = Vec<T>::N;
-    T top = -INFINITY;
-    int at = l * N;
-#pragma unroll
-    for (int e = 0; e < E; ++e)
-#pragma unroll
-        for (int i = 0; i < N; ++i)
-            if (v[e][i] > top) top = v[e][i], at = (l + e * 64) * N + i;
-    const Entry<T> mine = l * N < vocab ? Entry<T>::of(top, at) : Entry<T>::none();
-    const unsigned long long last = __ballot(place_in_wave(mine) == k - 1);
-    const Entry<T> bound = mine.lane(__builtin_ctzll(last));
+    const Entry<T> mine = l * N < vocab ? Entry<T>::of(top, top_group) : Entry<T>::none();
+    const Entry<T> bound = kth_of_wave(mine, k);
     const T low = bound.value();
     if (l == 0) *count = 0;
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
 #pragma unroll
-    for (int e = 0; e < E; ++e)
+    for (int e = 0; e < E; ++e) {
+        T g = ranked(v[e][0]);
+#pragma unroll
+        for (int i = 1; i < N; ++i) g = Max()(g, v[e][i]);
+        if (g < low) continue;
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-            if (ranked(v[e][i]) < low) continue;
             const int c = (l + e * 64) * N + i;
-            const Entry<T> w = Entry<T>::of(v[e][i], c);
-            if (c < vocab && !bound.better(w)) {
+            // (the bound's position is a group's: any of its entries may be the one)
+            if (c < vocab && !bound.better(Entry<T>::of(v[e][i], l + e * 64))) {
                 const int slot = atomicAdd(count, 1);
-                if (slot < kWaveList) list[slot] = w;
+                if (slot < kWaveList) list[slot] = Entry<T>::of(v[e][i], c);
             }
         }
+    }
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     const int n = __builtin_amdgcn_readfirstlane(*(volatile int*)count);
     if (n > kWaveList) return false;
@@ -234,9 +242,9 @@ __device__ __forceinline__ void best_one_by_one(const T (&v)[E][Vec<T>::N], int 
 }
 
 // The same for fp32 rows of one group to a lane, where the lanes lie in the order of the positions: each orders its four once, and the next alternative is the
-// head of the first lane whose head is the largest of all heads.
-template <int LANES, typename Put>
-__device__ __forceinline__ void best_by_heads(const float (&v)[1][4], int l, int vocab, int k, Put put) {
+// head of the first lane whose head is the largest of all heads. They go into `list` in order.
+template <int LANES>
+__device__ __forceinline__ void best_by_heads(const float (&v)[1][4], int l, int vocab, int k, Entry<float>* list) {
     unsigned key[4];
     int at[4];
 #pragma unroll
@@ -255,21 +263,23 @@ __device__ __forceinline__ void best_by_heads(const float (&v)[1][4], int l, int
     const unsigned long long team = (LANES == 64 ? ~0ull : ((1ull << (LANES % 64)) - 1)) << base;
     for (int n = 0; n < k; ++n) {
         const unsigned high = fold_lanes<LANES>(key[0], [](unsigned a, unsigned b) { return a > b ? a : b; });
-        const bool first = __builtin_ctzll(__ballot(key[0] == high) & team) == lane;
-        if (first) {
-            put(n, Entry<float>{(unsigned long long)key[0] << 32 | (0xffffffffu - (unsigned)at[0])});
+        if (__builtin_ctzll(__ballot(key[0] == high) & team) == lane) {
+            list[n].key = (unsigned long long)key[0] << 32 | (0xffffffffu - (unsigned)at[0]);
             key[0] = key[1], key[1] = key[2], key[2] = key[3], key[3] = 0;
             at[0] = at[1], at[1] = at[2], at[2] = at[3];
         }
     }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
 }
 
 // Rows that LANES lanes hold in registers, E groups each: every statistic is exact after one reading.
 template <typename T, int LANES, int E, bool TOP>
 __global__ __launch_bounds__(kThreads) void log_prob_short(LogProbArgs<T> a) {
     constexpr int N = Vec<T>::N;
-    constexpr bool LIST = TOP && E > 1;
-    __shared__ Entry<T> lists[LIST ? kThreads / 64 : 1][LIST ? kWaveList : 1];
+    // lists: of a wave that bounds its best, or of a row whose lanes' heads are compared
+    constexpr bool HEADS = TOP && E == 1 && sizeof(T) == 4, LIST = TOP && (E > 1 || HEADS);
+    constexpr int LISTS = HEADS ? kThreads / LANES : kThreads / 64, LENGTH = HEADS ? (LANES * N < DALI_HIP_MAX_ALTERNATIVES ? LANES * N : DALI_HIP_MAX_ALTERNATIVES) : kWaveList;
+    __shared__ Entry<T> lists[LIST ? LISTS : 1][LIST ? LENGTH : 1];
     __shared__ int counts[LIST ? kThreads / 64 : 1];
     const int l = threadIdx.x % LANES;
     const long row = (long)blockIdx.x * (kThreads / LANES) + threadIdx.x / LANES;
@@ -284,11 +294,16 @@ __global__ __launch_bounds__(kThreads) void log_prob_short(LogProbArgs<T> a) {
     for (int e = 0; e < E; ++e) take_group<(LANES > 8)>(g[e], (l + e * LANES) * N, a.vocab, T(-INFINITY), v[e]);
     const int token = a.tokens[r];
     const T own = token >= 0 && token < a.vocab ? x[token] : T(0);
-    T m = Real<T>::lowest;
+    T m = Real<T>::lowest, top = -INFINITY;
+    int top_group = l;
 #pragma unroll
-    for (int e = 0; e < E; ++e)
+    for (int e = 0; e < E; ++e) {
+        T h = v[e][0];
 #pragma unroll
-        for (int i = 0; i < N; ++i) m = Max()(m, v[e][i]);
+        for (int i = 1; i < N; ++i) h = Max()(h, v[e][i]);
+        m = Max()(m, h);
+        if (TOP && E > 1 && h > top) top = h, top_group = l + e * LANES;
+    }
     m = fold_lanes<LANES>(m, Max());
     T s = 0, t = 0;
 #pragma unroll
@@ -308,12 +323,14 @@ __global__ __launch_bounds__(kThreads) void log_prob_short(LogProbArgs<T> a) {
             if (live) write_alternative(a, r, x, q, place, e);
         };
         if constexpr (E == 1 && sizeof(T) == 4) {
-            best_by_heads<LANES>(v, l, a.vocab, a.k, put);
+            Entry<T>* list = lists[threadIdx.x / LANES];
+            best_by_heads<LANES>(v, l, a.vocab, a.k, list);
+            for (int n = l; n < a.k; n += LANES) put(n, list[n]);
         } else if constexpr (E == 1) {
             best_one_by_one<T, LANES, E>(v, l, a.vocab, a.k, put);
         } else {
             const int wave = threadIdx.x >> 6;
-            if (a.k <= 2 || !best_by_bound<T, E>(v, l, a.vocab, a.k, lists[wave], &counts[wave], put)) best_one_by_one<T, LANES, E>(v, l, a.vocab, a.k, put);
+            if (!best_by_bound<T, E>(v, top, top_group, l, a.vocab, a.k, lists[wave], &counts[wave], put)) best_one_by_one<T, LANES, E>(v, l, a.vocab, a.k, put);
         }
     }
 }
@@ -389,8 +406,8 @@ __device__ __forceinline__ Entry<T> find_bound(const Entry<T>& mine, int k, Shar
         if ((tid & 3) == 0) sh.key[tid >> 2] = quad;
         __syncthreads();
         if (tid < 64) {
-            const Entry<T> e = sh.key[tid];
-            if (place_in_wave(e) == k - 1) sh.bound = e;
+            const Entry<T> kth = kth_of_wave(sh.key[tid], k);
+            if (tid == 0) sh.bound = kth;
         }
     } else {
         sh.key[tid] = mine;
@@ -511,7 +528,8 @@ __device__ __forceinline__ void finish(const LogProbArgs<T>& a, long r, int segm
         if (tid < 64) {
             const int segments = a.segments, place = tid / segments, from = tid - place * segments;
             const Entry<T> e = place < a.k ? sh.list[from * a.k + place] : Entry<T>::none();
-            if (place_in_wave(e) == a.k - 1) sh.bound = e;
+            const Entry<T> kth = kth_of_wave(e, a.k);
+            if (tid == 0) sh.bound = kth;
         }
         __syncthreads();
         const Entry<T> bound = sh.bound;
