@@ -269,7 +269,8 @@ extern "C" int dali_hip_clip_by_global_norm(int dtype, int count, const void* co
         if (sizes[i] < 0 || (sizes[i] > 0 && (!in[i] || (out && !out[i])))) return fail("%s: array %d has no memory or a negative size", what, i);
     // (partial sums: kPartials, or 16 for every launch of kBatch arrays; chunks are numbered in 31 bits)
     if (count > (1 << 24)) return fail("%s: %d arrays are more than the workspace has room for", what, count);
-    if (ensure_init()) return DALI_HIP_ERROR;
+    for (int i = 0; i < count; ++i)
+        if (off_elements({in[i], out ? out[i] : nullptr, norm}, size)) return fail("%s: an address is off its type's size", what);
     const Span result("norm", norm, 1, size);
     for (int i = 0; i < count; ++i) {
         const Span a("an array", in[i], sizes[i], size);
@@ -299,6 +300,7 @@ extern "C" int dali_hip_clip_by_global_norm(int dtype, int count, const void* co
                 if (r->i != i || r->lo != lo) return fail("%s: result %d overlaps array %d", what, r->i, i);
         }
     }
+    if (ensure_init()) return DALI_HIP_ERROR;
     if (dtype == DALI_HIP_FLOAT) return clip<float>(count, in, out, sizes, max_norm, (float*)norm);
     return clip<double>(count, in, out, sizes, max_norm, (double*)norm);
 }

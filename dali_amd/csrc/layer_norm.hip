@@ -513,6 +513,7 @@ extern "C" int dali_hip_layer_norm(int dtype, int64_t rows, int width, const voi
     if (check_spans(what, {Span("y", y, rows * width, size), Span("mean", mean, rows, size), Span("rstd", rstd, rows, size)},
                     {Span("x", x, rows, width, x_stride, size), Span("gamma", gamma, width, size), Span("beta", beta, width, size)}, 1))
         return DALI_HIP_ERROR;
+    if (off_elements({x, gamma, beta, y, mean, rstd}, size)) return fail("%s: an address is off its type's size", what);
     if (ensure_init()) return DALI_HIP_ERROR;
     if (dtype == DALI_HIP_FLOAT)
         return forward<float>({(const float*)x, (const float*)gamma, (const float*)beta, (float*)y, (float*)mean, (float*)rstd, (long)rows, (long)x_stride, width, (float)epsilon});
@@ -532,6 +533,7 @@ extern "C" int dali_hip_layer_norm_backward(int dtype, int64_t rows, int width, 
                      Span("gamma", gamma, width, size)},
                     2))
         return DALI_HIP_ERROR;
+    if (off_elements({dy, x, mean, rstd, gamma, dx, dgamma, dbeta}, size)) return fail("%s: an address is off its type's size", what);
     if (ensure_init()) return DALI_HIP_ERROR;
     if (dtype == DALI_HIP_FLOAT)
         return backward<float>({(const float*)dy, (const float*)x, (const float*)mean, (const float*)rstd, (const float*)gamma, (float*)dx, (float*)dgamma, (float*)dbeta, nullptr,

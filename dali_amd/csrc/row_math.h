@@ -222,6 +222,12 @@ inline int check_spans(const char* what, std::initializer_list<Span> outs, std::
     return DALI_HIP_OK;
 }
 
+inline bool off_elements(std::initializer_list<const void*> pointers, size_t size) {
+    for (const void* p : pointers)
+        if ((uintptr_t)p % size != 0) return true;
+    return false;
+}
+
 inline bool is_real(int dtype) { return dtype == DALI_HIP_FLOAT || dtype == DALI_HIP_DOUBLE; }
 
 inline int launched(const char* what) {

@@ -21,14 +21,14 @@ struct Real;
 template <>
 struct Real<float> {
     static constexpr float lowest = -3.402823466e+38f;  // where a running maximum begins: finite, so that no difference to it is NaN
-    static constexpr float under = -1e30f;              // an exponent whose weight is 0: what an infinite one is replaced by where it meets a weight
+    static constexpr float under = -200.0f;             // an exponent whose weight is 0: what a lower one is replaced by where it meets a weight or a gradient
     static __device__ __forceinline__ float weight(float d) { return __builtin_amdgcn_exp2f(d * 1.44269504088896341f); }
     static __device__ __forceinline__ float ln(float s) { return logf(s); }
 };
 template <>
 struct Real<double> {
     static constexpr double lowest = -1.7976931348623157e+308;
-    static constexpr double under = -1e300;
+    static constexpr double under = -1000.0;
     static __device__ __forceinline__ double weight(double d) { return exp(d); }
     static __device__ __forceinline__ double ln(double s) { return log(s); }
 };
@@ -859,6 +859,7 @@ extern "C" int dali_hip_token_log_probs(int dtype, int64_t rows, int vocab, cons
                      Span("top_log_probs", top_log_probs, rows * k, size), Span("top_tokens", top_tokens, rows * k, 4)},
                     {Span("logits", logits, rows, vocab, stride, size), Span("tokens", tokens, rows, 4)}, 0))
         return DALI_HIP_ERROR;
+    if (off_elements({logits, log_probs, entropy, lse, top_log_probs}, size) || off_elements({tokens, top_tokens}, 4)) return fail("%s: an address is off its type's size", what);
     if (ensure_init()) return DALI_HIP_ERROR;
     if (dtype == DALI_HIP_FLOAT)
         return forward<float>({(const float*)logits, tokens, (float*)log_probs, (float*)entropy, (float*)lse, (float*)top_log_probs, top_tokens, (long)rows, (long)stride, vocab, k});
@@ -879,6 +880,7 @@ extern "C" int dali_hip_token_log_probs_backward(int dtype, int64_t rows, int vo
                      Span("tokens", tokens, rows, 4), Span("lse", lse, rows, size), Span("entropy", entropy, rows, size)},
                     1))
         return DALI_HIP_ERROR;
+    if (off_elements({d_log_probs, d_entropy, logits, lse, entropy, d_logits}, size) || off_elements({tokens}, 4)) return fail("%s: an address is off its type's size", what);
     if (ensure_init()) return DALI_HIP_ERROR;
     if (dtype == DALI_HIP_FLOAT)
         return backward<float>({(const float*)d_log_probs, (const float*)d_entropy, (const float*)logits, (const float*)lse, (const float*)entropy, tokens, (float*)d_logits,

@@ -459,8 +459,11 @@ PyObject* f_layer_norm_backward(PyObject*, PyObject* const* args, Py_ssize_t n) 
 PyObject* f_token_log_probs(PyObject*, PyObject* const* args, Py_ssize_t n) {
     Operand logits, tokens;
     Destinations out;
-    int k;
-    if (!count_is(n, 4, "token_log_probs") || !logits.set(args[0]) || !tokens.set(args[1]) || !whole_number(args[2], &k) || !out.set(args[3], 5, "token_log_probs")) return nullptr;
+    if (!count_is(n, 4, "token_log_probs") || !logits.set(args[0]) || !tokens.set(args[1]) || !out.set(args[3], 5, "token_log_probs")) return nullptr;
+    int too_large = 0;
+    const long asked = PyLong_AsLongAndOverflow(args[2], &too_large);  // (a count that is not one of an int is refused, not cut)
+    if (asked == -1 && PyErr_Occurred()) return nullptr;
+    const int k = too_large || asked != (int)asked ? -1 : (int)asked;
     dali_array_t* r = out.handles.data();
     const int status = unlocked([&] { return dali_fe_token_log_probs(logits.handle, tokens.handle, k, &r[0], &r[1], &r[2], &r[3], &r[4]); });
     return status != 0 ? fail("token_log_probs") : out.results("token_log_probs");

@@ -131,6 +131,20 @@ def test_clustered_entries(gpu, D, rng, vocab, rows):
         check(x, tokens, k, call(D, x, tokens, k))
 
 
+@pytest.mark.parametrize("rows,vocab,stride", [(5, 4000, 256), (1, 40000, 256), (1, 1000000, 256), (600, 20000, 256), (1030, 4000, 64), (1030, 400, 64)])
+@pytest.mark.parametrize("dtype", [np.float32, np.float64])
+def test_more_good_entries_than_are_ranked_at_once(gpu, D, rows, vocab, stride, dtype):
+    """Nearly all of the best lie in the groups of few threads: `stride` groups of 16 bytes apart, in every segment."""
+    rng = np.random.RandomState(vocab)
+    group = np.arange(vocab) * np.dtype(dtype).itemsize // 16
+    x = rng.randn(rows, vocab).astype(dtype)
+    x[:, group % stride < (50 if stride == 256 else 40)] += 100
+    x[:, ::7] = np.round(x[:, ::7])  # (with ties)
+    tokens = rng.randint(0, vocab, rows).astype(np.int32)
+    for k in (12, 20, 64):
+        check(x, tokens, k, call(D, x, tokens, k))
+
+
 @pytest.mark.parametrize("vocab", [5, 97, 1100, 40000])
 def test_infinities_and_nan_stay_in_their_rows(gpu, D, rng, vocab):
     x = (rng.randn(8, vocab) * 3).astype(np.float32)
@@ -215,6 +229,19 @@ def test_backward_of_masked_rows(gpu, D, rng, vocab):
     g, h = rng.randn(8).astype(np.float32), rng.randn(8).astype(np.float32)
     got = check_backward(D, x, tokens, g, h)
     assert not got[0].any()
+
+
+@pytest.mark.parametrize("vocab", [40, 1500, 9000])
+def test_large_gradients_of_masked_rows(gpu, D, rng, vocab):
+    """A masked entry's gradient is 0 whatever comes from above (but for the given token's own part, which does not ask for its probability)."""
+    x = rng.randn(5, vocab).astype(np.float32)
+    x[:4, rng.rand(vocab) < 0.5] = -np.inf
+    x[2] = -np.inf
+    x[3, 1:] = np.finfo(np.float32).min
+    x[:2, 0] = x[4, 0] = 1.0
+    g, h = np.array([1e30, -1e30, 1e30, 1e20, 0], np.float32), np.array([1e30, 1e32, -1e30, 1e30, 1e30], np.float32)
+    got = check_backward(D, x, np.zeros(5, np.int32), g, h)
+    assert (got[:, 1:][np.isneginf(x[:, 1:])] == 0).all()
 
 
 @pytest.mark.parametrize("vocab", [2, 97, 1500, 9000])

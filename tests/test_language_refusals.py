@@ -38,6 +38,7 @@ def test_token_log_probs(D):
     for call, text in ((lambda: op.token_log_probs(whole, tokens), "float or double"), (lambda: op.token_log_probs(x, per_row), "tokens must be int"),
                        (lambda: op.token_log_probs(x, whole), "tokens must be int"), (lambda: op.token_log_probs(x, tokens, -1), "k must be from 0 to 6"),
                        (lambda: op.token_log_probs(x, tokens, 7), "k must be from 0 to 6"), (lambda: op.token_log_probs(D.Array.empty((4, 900)), tokens, 65), "k must be from 0 to 64"),
+                       (lambda: op.token_log_probs(x, tokens, 2 ** 32 + 1), "k must be from 0 to 6"), (lambda: op.token_log_probs(x, tokens, 10 ** 30), "k must be from 0 to 6"),
                        (lambda: op.token_log_probs(D.Array.empty((4, 0)), tokens), "last axis"), (lambda: op.token_log_probs(x, tokens, 2, out=(None, None, None, x, None)), "top_log_probs must be"),
                        (lambda: op.token_log_probs(x, tokens, 2, out=(None, None, None, None, D.Array.empty((4, 2)))), "top_tokens must be int"),
                        (lambda: op.token_log_probs_backward(vector, None, x, tokens, per_row, None), "d_log_probs must be"),
@@ -90,6 +91,12 @@ def test_entries_of_the_library(D):
     refused(hip.dali_hip_token_log_probs(0, 1, 400, p, 4, p, 65, p, p, p, p, p), "65 alternatives")
     refused(hip.dali_hip_token_log_probs(0, 1, 4, p, 4, p, 2, at(8), at(9), at(10), None, None), "NULL")
     refused(hip.dali_hip_token_log_probs_backward(0, 1, 4, p, p, p, 4, p, p, None, p), "NULL")
+    odd = lambda i: C.c_void_p(C.addressof(host) + 8 * i + 2)  # noqa: E731
+    refused(hip.dali_hip_layer_norm(0, 1, 4, odd(0), 4, None, None, 1e-5, at(8), at(16), at(17)), "off its type's size")
+    refused(hip.dali_hip_layer_norm_backward(0, 1, 4, at(0), 4, at(8), 4, at(16), at(17), at(20), odd(24), at(28), at(32)), "off its type's size")
+    refused(hip.dali_hip_token_log_probs(0, 1, 4, at(0), 4, odd(8), 0, at(10), at(11), at(12), None, None), "off its type's size")
+    refused(hip.dali_hip_token_log_probs_backward(0, 1, 4, at(6), None, at(0), 4, at(8), at(9), None, odd(10)), "off its type's size")
+    refused(hip.dali_hip_clip_by_global_norm(0, 1, (C.c_void_p * 1)(odd(0).value), None, (C.c_int64 * 1)(3), 1.0, at(9)), "off its type's size")
     sizes, pointers = (C.c_int64 * 1)(-3), (C.c_void_p * 1)(C.addressof(host))
     refused(hip.dali_hip_clip_by_global_norm(0, 1, pointers, None, sizes, 1.0, at(9)), "negative size")
     refused(hip.dali_hip_clip_by_global_norm(0, 1, pointers, pointers, (C.c_int64 * 1)(3), float("nan"), at(9)), "negative")
