@@ -558,10 +558,17 @@ __global__ __launch_bounds__(kThreads) void log_prob_long(LogProbArgs<T> a) {
     T top = -INFINITY;
     int top_group = begin + tid;
     int j = begin + tid;
+    typename Vec<T>::type next[U];
+    auto ask = [&](int from) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) next[u] = *reinterpret_cast<const typename Vec<T>::type*>(x + (long)(from + u * kThreads) * N);
+    };
+    if (j + (U - 1) * kThreads < whole) ask(j);
     for (; j + (U - 1) * kThreads < whole; j += U * kThreads) {
         typename Vec<T>::type v[U];
 #pragma unroll
-        for (int u = 0; u < U; ++u) v[u] = *reinterpret_cast<const typename Vec<T>::type*>(x + (long)(j + u * kThreads) * N);
+        for (int u = 0; u < U; ++u) v[u] = next[u];
+        if (j + (2 * U - 1) * kThreads < whole) ask(j + U * kThreads);  // (under way while these are worked on)
         T high = q.m;
 #pragma unroll
         for (int u = 0; u < U; ++u) {
