@@ -116,7 +116,7 @@ __device__ __forceinline__ int place_in_wave(const Entry<T>& e) {
 }
 
 // The k-th best of a wave's entries, in every lane: a few by taking the best away one after the other, more by counting places
-constexpr int kOneByOne = 12;
+constexpr int kOneByOne = 10;  // (65536x1000 with 4, 8, 12, 16 alternatives: 62, 76, 92, 110 us one by one, 85, 89, 91, 93 by places)
 template <typename T>
 __device__ __forceinline__ Entry<T> kth_of_wave(Entry<T> e, int k) {
     if (k > kOneByOne) return e.lane(__builtin_ctzll(__ballot(place_in_wave(e) == k - 1)));
@@ -338,7 +338,8 @@ __global__ __launch_bounds__(kThreads) void log_prob_short(LogProbArgs<T> a) {
 constexpr int kList = 512;    // entries that are ranked at once
 constexpr int kMerge = 64;    // segments of a row, one to a lane of the wave that joins them
 constexpr int kByHeads = 8;   // up to so many alternatives, the segments' lists are joined one after the other
-constexpr int kByQuads = 32;  // up to so many alternatives, the best of 64 quads of threads bound them; beyond, those of the threads themselves
+constexpr int kByQuads = 32;  // up to so many alternatives, the best of 64 quads of threads bound them; beyond, those of the threads themselves, which bound them closer but
+                              // take longer to compare (quads and threads, 8192x32000: 236 and 232 us with 24, 283 and 268 with 48; 1x50257: 10.6 and 13.0, 12.6 and 14.1)
 
 // The running sums of a row or a part of it: the maximum, the weights relative to it and their product with the exponents
 template <typename T>
@@ -764,7 +765,6 @@ bool short_rows(int groups, F launch) {
     if (groups <= 256) return with(std::integral_constant<int, 64>(), std::integral_constant<int, 4>());
     if constexpr (MOST > 256) {
         if (groups <= 512) return with(std::integral_constant<int, 64>(), std::integral_constant<int, 8>());
-        if (groups <= 1024) return with(std::integral_constant<int, 64>(), std::integral_constant<int, 16>());
     }
     return false;
 }
@@ -772,8 +772,9 @@ bool short_rows(int groups, F launch) {
 template <typename T>
 int forward(LogProbArgs<T> all) {
     const int groups = groups_of<T>(all.vocab);
-    // A wave per row up to 1024 groups, where there are rows enough for all waves; else a workgroup above 256
-    const bool is_short = groups <= 256 || (groups <= 1024 && all.rows >= 1024);
+    // A wave per row up to 256 groups, and to 512 where there are rows enough for all waves, a workgroup above. Wave and workgroup, with 5 alternatives (us): 256x2000 5.8 and
+    // 5.1, 1023x2000 5.8 and 6.7, 8192x2000 18 and 27, 8192x4000 37 and 30, 65536x3000 234 and 199.
+    const bool is_short = groups <= 256 || (groups <= 512 && all.rows >= 1024);
     // a launch numbers its workgroups in 31 bits
     for (long done = 0; done < all.rows;) {
         LogProbArgs<T> a = all;
@@ -786,7 +787,7 @@ int forward(LogProbArgs<T> all) {
         a.segments = 1;
         a.per = groups;
         if (is_short) {
-            short_rows<1024>(groups, [&](auto lanes, auto e) {
+            short_rows<512>(groups, [&](auto lanes, auto e) {
                 constexpr int LANES = decltype(lanes)::value, E = decltype(e)::value, per = kThreads / LANES;
                 const dim3 grid((unsigned)((a.rows + per - 1) / per));
                 if (a.k) hipLaunchKernelGGL((log_prob_short<T, LANES, E, true>), grid, dim3(kThreads), 0, stream(), a);
@@ -794,9 +795,11 @@ int forward(LogProbArgs<T> all) {
             });
             continue;
         }
-        // Few rows are cut into segments of at least 512 groups, two for a thread, until there are 512 workgroups or so. The segments' alternatives are joined in one
-        // list, and a lane of one wave stands for a segment.
-        const long cut = std::min({512L / a.rows, (long)groups / 512, (long)kList / std::max(a.k, 1), (long)kMerge});
+        // Few long rows are cut into segments of at least 512 groups, two for a thread, 512 workgroups or so together. The segments' alternatives are joined in one list,
+        // and a lane of one wave stands for a segment. Cut and whole, with 5 alternatives (us): 8x32000 7.3 and 9.1, 64x32000 8.1 and 9.1, 130x32000 10.8 and 9.1, 100x8000
+        // 7.7 and 6.3, 130x100000 15.2 and 16.9, 250x200000 42.2 and 45.9.
+        const bool cuts = (a.rows <= 128 && groups >= 4096) || (a.rows <= 256 && groups >= 16384);
+        const long cut = cuts ? std::min({512L / a.rows, (long)groups / 512, (long)kList / std::max(a.k, 1), (long)kMerge}) : 1;
         if (cut > 1) {
             a.segments = (int)cut;
             a.per = (groups + a.segments - 1) / a.segments;
