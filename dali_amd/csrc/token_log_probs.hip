@@ -337,6 +337,7 @@ __global__ __launch_bounds__(kThreads) void log_prob_short(LogProbArgs<T> a) {
 
 constexpr int kList = 512;    // entries that are ranked at once
 constexpr int kMerge = 64;    // segments of a row, one to a lane of the wave that joins them
+constexpr int kParts = 4;     // of a thread's walk, each with a best group
 constexpr int kByHeads = 8;   // up to so many alternatives, the segments' lists are joined one after the other
 constexpr int kByQuads = 32;  // up to so many alternatives, the best of 64 quads of threads bound them; beyond, those of the threads themselves, which bound them closer but
                               // take longer to compare (quads and threads, 8192x32000: 236 and 232 us with 24, 283 and 268 with 48; 1x50257: 10.6 and 13.0, 12.6 and 14.1)
@@ -377,7 +378,7 @@ struct Shared {
     unsigned arrived;
     int count, units;
     Entry<T> list[TOP ? kList : 1], key[TOP ? kThreads : 1], bound;
-    int unit[TOP ? kThreads : 1];
+    unsigned short unit[TOP ? kParts * kThreads : 1];
 };
 
 template <typename T, bool TOP>
@@ -543,55 +544,68 @@ __device__ __forceinline__ void finish(const LogProbArgs<T>& a, long r, int segm
 }
 
 // One workgroup per row, or per segment of a row: a thread walks its groups once with running sums, which are rescaled when the maximum rises (once per four
-// groups), and its best group. What passes the bound that the best groups give lies in the few threads whose own best passes it; their groups are read again.
+// groups). For the alternatives it keeps the best group of each quarter of its walk. What passes the bound that the best groups give lies in the few quarters whose own best
+// passes it; their groups are read again: a line of the cache for 16 bytes each time, which is why they are quarters (8192x32000 with 5 alternatives read 1.15 times the
+// logits with whole walks, 184 us).
 template <typename T, bool TOP>
 __global__ __launch_bounds__(kThreads) void log_prob_long(LogProbArgs<T> a) {
-    constexpr int N = Vec<T>::N, U = 4;
+    constexpr int N = Vec<T>::N, U = 4, STEP = U * kThreads, PARTS = TOP ? kParts : 1;
     __shared__ Shared<T, TOP> sh;
     const int tid = threadIdx.x;
     const long r = blockIdx.x / (unsigned)a.segments;
     const int segment = (int)(blockIdx.x - (unsigned)r * (unsigned)a.segments);
     const T* x = a.logits + r * a.stride;
     const int groups = groups_of<T>(a.vocab), begin = segment * a.per, end = min(groups, begin + a.per), whole = min(end, a.vocab / N);
+    const int span = ((end - begin - 1) / (STEP * PARTS) + 1) * STEP;  // groups of the segment in a part, whole steps of all threads
     const int token = a.tokens[r];
     const T own = token >= 0 && token < a.vocab ? x[token] : T(0);
     Sums<T> q;
-    T top = -INFINITY;
-    int top_group = begin + tid;
+    T top[PARTS];
+    int top_group[PARTS];
     int j = begin + tid;
     typename Vec<T>::type next[U];
     auto ask = [&](int from) {
 #pragma unroll
         for (int u = 0; u < U; ++u) next[u] = *reinterpret_cast<const typename Vec<T>::type*>(x + (long)(from + u * kThreads) * N);
     };
-    if (j + (U - 1) * kThreads < whole) ask(j);
-    for (; j + (U - 1) * kThreads < whole; j += U * kThreads) {
-        typename Vec<T>::type v[U];
+    if (j + STEP - kThreads < whole) ask(j);
 #pragma unroll
-        for (int u = 0; u < U; ++u) v[u] = next[u];
-        if (j + (2 * U - 1) * kThreads < whole) ask(j + U * kThreads);  // (under way while these are worked on)
-        T high = q.m;
+    for (int part = 0; part < PARTS; ++part) {
+        top[part] = -INFINITY;
+        top_group[part] = begin + tid + part * span;
+        const int limit = PARTS == 1 ? whole : (int)min((long)whole, (long)begin + tid + (part + 1L) * span);  // (a step ends below it or begins at it)
+        for (; j + STEP - kThreads < whole && j < limit; j += STEP) {
+            typename Vec<T>::type v[U];
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            T g = v[u][0];
+            for (int u = 0; u < U; ++u) v[u] = next[u];
+            if (j + 2 * STEP - kThreads < whole) ask(j + STEP);  // (under way while these are worked on)
+            T high = q.m;
 #pragma unroll
-            for (int i = 1; i < N; ++i) g = Max()(g, v[u][i]);
-            high = Max()(high, g);
-            if (TOP && g > top) top = g, top_group = j + u * kThreads;
+            for (int u = 0; u < U; ++u) {
+                T g = v[u][0];
+#pragma unroll
+                for (int i = 1; i < N; ++i) g = Max()(g, v[u][i]);
+                high = Max()(high, g);
+                if (TOP && g > top[part]) top[part] = g, top_group[part] = j + u * kThreads;
+            }
+            q.raise(high);
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+#pragma unroll
+                for (int i = 0; i < N; ++i) q.add(v[u][i]);
         }
-        q.raise(high);
-#pragma unroll
-        for (int u = 0; u < U; ++u)
-#pragma unroll
-            for (int i = 0; i < N; ++i) q.add(v[u][i]);
     }
+    // (what is left is less than a step and lies in one part)
+    const int rest = (j - begin - tid) / span;
     for (; j < end; j += kThreads) {
         T v[N];
         load_group(x, j * N, a.vocab, T(-INFINITY), v);
         T g = v[0];
 #pragma unroll
         for (int i = 1; i < N; ++i) g = Max()(g, v[i]);
-        if (TOP && g > top) top = g, top_group = j;
+#pragma unroll
+        for (int part = 0; part < PARTS; ++part)
+            if (TOP && part == rest && g > top[part]) top[part] = g, top_group[part] = j;
         q.raise(Max()(q.m, g));
 #pragma unroll
         for (int i = 0; i < N; ++i) q.add(v[i]);
@@ -599,16 +613,25 @@ __global__ __launch_bounds__(kThreads) void log_prob_long(LogProbArgs<T> a) {
     over_block(q, sh);
     int found = 0;
     if constexpr (TOP) {
-        const Entry<T> mine = begin + tid < end ? Entry<T>::of(top, top_group) : Entry<T>::none(), bound = find_bound(mine, a.k, sh);
-        if (!bound.better(mine)) sh.unit[atomicAdd(&sh.units, 1)] = tid;
+        Entry<T> best[PARTS], mine = Entry<T>::none();
+#pragma unroll
+        for (int part = 0; part < PARTS; ++part) {
+            best[part] = (long)begin + tid + (long)part * span < end ? Entry<T>::of(top[part], top_group[part]) : Entry<T>::none();
+            mine = Entry<T>::either(best[part].better(mine), best[part], mine);
+        }
+        const Entry<T> bound = find_bound(mine, a.k, sh);
+#pragma unroll
+        for (int part = 0; part < PARTS; ++part)
+            if (!bound.better(best[part])) sh.unit[atomicAdd(&sh.units, 1)] = (unsigned short)(part * kThreads + tid);
         __syncthreads();
-        const int walks = (end - begin + kThreads - 1) / kThreads, all = sh.units * walks;
+        const int walks = span / kThreads, all = sh.units * walks;
         for (int i = tid; i < all; i += kThreads) {
-            const int n = i / walks, g = begin + sh.unit[n] + (i - n * walks) * kThreads;
+            const int n = i / walks, unit = sh.unit[n];
+            const long g = (long)begin + (unit & (kThreads - 1)) + (long)(unit / kThreads) * span + (i - n * walks) * kThreads;
             if (g >= end) continue;
             T v[N];
-            load_group(x, g * N, a.vocab, T(-INFINITY), v);
-            collect(v, g, a.vocab, bound, sh);
+            load_group(x, (int)g * N, a.vocab, T(-INFINITY), v);
+            collect(v, (int)g, a.vocab, bound, sh);
         }
         __syncthreads();
         found = sh.count;
@@ -812,8 +835,15 @@ int forward(LogProbArgs<T> all) {
         const dim3 grid((unsigned)(a.rows * a.segments));
         auto launch = [&](auto top) {
             constexpr bool TOP = decltype(top)::value;
-            if (a.per <= 4 * kThreads) hipLaunchKernelGGL((log_prob_segments<T, TOP, 4>), grid, dim3(kThreads), 0, stream(), a);
-            else hipLaunchKernelGGL((log_prob_long<T, TOP>), grid, dim3(kThreads), 0, stream(), a);
+            auto held = [&](auto e) {
+                if (a.per > decltype(e)::value * kThreads) return false;
+                hipLaunchKernelGGL((log_prob_segments<T, TOP, decltype(e)::value>), grid, dim3(kThreads), 0, stream(), a);
+                return true;
+            };
+            if (held(std::integral_constant<int, 2>()) || held(std::integral_constant<int, 3>()) || held(std::integral_constant<int, 4>()) ||
+                held(std::integral_constant<int, 5>()) || held(std::integral_constant<int, 6>()) || held(std::integral_constant<int, 8>()))
+                return;
+            hipLaunchKernelGGL((log_prob_long<T, TOP>), grid, dim3(kThreads), 0, stream(), a);
         };
         if (a.k) launch(std::true_type());
         else launch(std::false_type());
