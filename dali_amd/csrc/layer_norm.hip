@@ -52,8 +52,9 @@ __device__ __forceinline__ T root_of(T variance, T epsilon) {
     return T(1) / sqrt((variance < T(0) ? T(0) : variance) + epsilon);
 }
 
-// A team of TEAM threads per row, which lives in their registers, E groups of 16 bytes to a thread: read once, written once. WHOLE: the teams' groups are the
-// row exactly. The weights stay in registers from row to row where they fit.
+// A team of TEAM threads per row, which lives in their registers, E groups of 16 bytes to a thread: read once, written once, which bounds it. WHOLE: the teams' groups are
+// the row exactly. The weights stay in registers from row to row where they fit. 8192x1024 11.5 us (5.8 TB/s), 65536x1024 89 us (6.0), 32768x4096 187 us (5.7); 8x1024 4.4 us
+// among others, 2.9 of them on the device.
 template <typename T, int TEAM, int E, bool WHOLE, bool PAST>
 __global__ __launch_bounds__(TEAM > kThreads ? TEAM : kThreads) void norm_team(NormArgs<T> a) {
     constexpr int N = Vec<T>::N, BLOCK = TEAM > kThreads ? TEAM : kThreads, TEAMS = BLOCK / TEAM;
@@ -131,7 +132,7 @@ __global__ __launch_bounds__(TEAM > kThreads ? TEAM : kThreads) void norm_team(N
     }
 }
 
-// Rows that no workgroup's registers hold: a workgroup walks each three times
+// Rows that no workgroup's registers hold: a workgroup walks each three times, the later ones in the caches
 template <typename T, bool PAST>
 __global__ __launch_bounds__(1024) void norm_rows(NormArgs<T> a) {
     constexpr int N = Vec<T>::N, BLOCK = 1024;
@@ -209,7 +210,9 @@ __device__ __forceinline__ T plus_across(T v) {
 }
 
 // The gradient with the rows in registers as above; a thread also keeps the sums of its columns over all rows that its team takes. At the end the teams of a
-// workgroup are joined, lanes first and then waves through LDS, in halves, and the workgroup leaves one row of partial sums for each weight.
+// workgroup are joined, lanes first and then waves through LDS, in halves, and the workgroup leaves one row of partial sums for each weight. So x and dy are read once for all
+// three gradients. Bound by memory: 32768x4096 280 us (5.7 TB/s), 65536x1024 148 us (5.4); 8192x1024 22.3 us, of which 18 to 20 are this launch (a wave has two rows) and 2
+// to 4 the fold; 3001x2047 in double 36 us. The next row is asked for before this one is worked on (8192x1024 24.2 without, 65536x1024 154).
 template <typename T, int TEAM, int TEAMS, int E, bool WHOLE, bool WEIGHTS, bool PAST>
 __global__ __launch_bounds__(TEAM * TEAMS) void norm_backward_team(NormBackwardArgs<T> a) {
     constexpr int N = Vec<T>::N, BLOCK = TEAM * TEAMS;
@@ -404,7 +407,8 @@ __global__ __launch_bounds__(kThreads) void norm_fold(NormBackwardArgs<T> a) {
     if (p == 0 && c < columns) (c < a.width ? a.dgamma[c] : a.dbeta[c - a.width]) = joined[0][i];
 }
 
-// threads to a row and groups to a thread that hold a row of `groups` groups; false: none up to `most`
+// Threads to a row and groups to a thread that hold a row of `groups` groups; false: none up to MOST. The forward pass, which holds a row and no sums, takes fewer threads
+// with more groups (256 threads with 2, 512 with 1: 32768x1500 73 and 87 us; 256 with 4, 512 with 2: 32768x3000 143 and 149; 512 with 4, 1024 with 2: 16384x8192 182 and 188).
 template <int MOST, typename F>
 bool team_for(int groups, F launch) {
     auto with = [&](auto team, auto e) {

@@ -158,7 +158,9 @@ __device__ __forceinline__ T block_sum(T v, T* scratch) {
     return fold_block<THREADS>(v, scratch, Sum());
 }
 
-// Whether a pass moves so much that the caches (256 MiB) would not hold its result until somebody reads it
+// Whether a pass moves so much that the caches (256 MiB) would not hold its result until somebody reads it. Ordinary stores and those past the caches (us): gradient of log
+// probabilities 8192x32000 408 and 392, layer norm 65536x1024 91.7 and 89.1, clipping 52 million values, whose second launch finds more of what the first read, 127 and 105.
+// Smaller passes gain little (8192x1024 11.5 and 11.4, its gradient 24.2 and 22.6), and the next kernel would have to fetch their result.
 inline bool past_caches(double bytes) { return bytes >= (double)(256L << 20); }
 
 // f(true_type) or f(false_type)

@@ -272,7 +272,9 @@ __device__ __forceinline__ void best_by_heads(const float (&v)[1][4], int l, int
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
 }
 
-// Rows that LANES lanes hold in registers, E groups each: every statistic is exact after one reading.
+// Rows that LANES lanes hold in registers, E groups each: every statistic is exact after one reading, and no workgroup meets. Bound by memory without alternatives
+// (65536x1500 66 us, 5.9 TB/s; 51200x97 7.6 us, where the launch is half of it), by arithmetic with them (51200x97 with 5 14.5 us, 65536x1000 64 us, 4.1 TB/s: a
+// comparison of all lanes costs a row as much as its exponentials).
 template <typename T, int LANES, int E, bool TOP>
 __global__ __launch_bounds__(kThreads) void log_prob_short(LogProbArgs<T> a) {
     constexpr int N = Vec<T>::N;
@@ -546,7 +548,8 @@ __device__ __forceinline__ void finish(const LogProbArgs<T>& a, long r, int segm
 // One workgroup per row, or per segment of a row: a thread walks its groups once with running sums, which are rescaled when the maximum rises (once per four
 // groups). For the alternatives it keeps the best group of each quarter of its walk. What passes the bound that the best groups give lies in the few quarters whose own best
 // passes it; their groups are read again: a line of the cache for 16 bytes each time, which is why they are quarters (8192x32000 with 5 alternatives read 1.15 times the
-// logits with whole walks, 184 us).
+// logits with whole walks, 184 us). Bound by memory: 8192x32000 175 us (6.0 TB/s), with 5, 20 and 64 alternatives 182, 190 and 222 us. One reading with running sums
+// instead of a maximum first and the sums after it: the row is larger than what the registers of a workgroup hold.
 template <typename T, bool TOP>
 __global__ __launch_bounds__(kThreads) void log_prob_long(LogProbArgs<T> a) {
     constexpr int N = Vec<T>::N, U = 4, STEP = U * kThreads, PARTS = TOP ? kParts : 1;
@@ -643,7 +646,9 @@ __global__ __launch_bounds__(kThreads) void log_prob_long(LogProbArgs<T> a) {
     finish(a, r, segment, x, q, found, token, own, sh);
 }
 
-// Segments that a workgroup holds in registers, E groups to a thread: all of them are loaded at once and nothing is read again.
+// Segments that a workgroup holds in registers, E groups to a thread: all of them are loaded at once and nothing is read again. 65536x3000 128 us (6.2 TB/s), with 5
+// alternatives 187; 32768x8000 170 and 181 us. A single row of 50257 in 25 segments takes 7.0 us with 5 alternatives and 10.1 with 20, 4.6 without: a chain of one reading,
+// the folds, the bound, two trips to memory for what the segments found and its ranking.
 template <typename T, bool TOP, int E>
 __global__ __launch_bounds__(kThreads) void log_prob_segments(LogProbArgs<T> a) {
     constexpr int N = Vec<T>::N;
@@ -726,7 +731,8 @@ struct RowGradient {
     }
 };
 
-// LANES lanes to a row
+// The gradient is a map once a row's lse is known: one reading, one writing, bound by memory. LANES lanes to a row: 51200x97 9.5 us (4.3 TB/s, an odd length costs lanes
+// and whole lines), 65536x613 57 us (5.7 TB/s)
 template <typename T, int LANES, int E, bool PAST>
 __global__ __launch_bounds__(kThreads) void log_prob_backward_short(LogProbBackwardArgs<T> a) {
     constexpr int N = Vec<T>::N;
@@ -749,7 +755,7 @@ __global__ __launch_bounds__(kThreads) void log_prob_backward_short(LogProbBackw
     }
 }
 
-// a workgroup to a piece of a row, four groups to a thread
+// a workgroup to a piece of a row, four groups to a thread: 8192x32000 393 us (5.3 TB/s, above a plain copy of that size)
 template <typename T, bool PAST>
 __global__ __launch_bounds__(kThreads) void log_prob_backward_long(LogProbBackwardArgs<T> a) {
     constexpr int N = Vec<T>::N, U = 4;
@@ -795,8 +801,8 @@ bool short_rows(int groups, F launch) {
 template <typename T>
 int forward(LogProbArgs<T> all) {
     const int groups = groups_of<T>(all.vocab);
-    // A wave per row up to 256 groups, and to 512 where there are rows enough for all waves, a workgroup above. Wave and workgroup, with 5 alternatives (us): 256x2000 5.8 and
-    // 5.1, 1023x2000 5.8 and 6.7, 8192x2000 18 and 27, 8192x4000 37 and 30, 65536x3000 234 and 199.
+    // A wave per row up to 256 groups, and to 512 where there are rows enough for all waves, a workgroup above. Wave and workgroup, with 5 alternatives (us): 256x2000 5.9 and
+    // 4.8, 1023x2000 6.0 and 6.1, 8192x2000 18 and 23, 65536x2000 107 and 164; above 512 groups 65536x3000 234 and 187.
     const bool is_short = groups <= 256 || (groups <= 512 && all.rows >= 1024);
     // a launch numbers its workgroups in 31 bits
     for (long done = 0; done < all.rows;) {
