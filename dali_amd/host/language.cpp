@@ -118,6 +118,7 @@ LayerNormGradient layer_norm_backward(const Array& dy, const Array& x, const Arr
     check_shape(what, "rstd", rstd, leading(x), dtype);
     const bool weights = !gamma.is_stateless();
     if (weights) check_shape(what, "gamma", gamma, vector, dtype);
+    DALI_ASSERT(weights || (out.gamma.is_stateless() && out.beta.is_stateless()), make_message(what, ": without gamma there are no gradients of weights to write"));
     LayerNormGradient r;
     r.x = destination(what, "dx", out.x, x.shape(), dtype);
     if (weights) {
@@ -146,6 +147,7 @@ TokenLogProbs token_log_probs(const Array& logits, const Array& tokens, int k, c
     check_shape(what, "tokens", tokens, rows_shape, DTYPE_INT32);
     DALI_ASSERT(k >= 0 && k <= DALI_HIP_MAX_ALTERNATIVES && k <= logits.shape().back(),
                 make_message(what, ": k must be from 0 to ", std::min(DALI_HIP_MAX_ALTERNATIVES, logits.shape().back()), " here (got ", k, ")"));
+    DALI_ASSERT(k > 0 || (out.top_log_probs.is_stateless() && out.top_tokens.is_stateless()), make_message(what, ": with k = 0 there are no alternatives to write"));
     TokenLogProbs r;
     r.log_probs = destination(what, "log_probs", out.log_probs, rows_shape, dtype);
     r.entropy = destination(what, "entropy", out.entropy, rows_shape, dtype);

@@ -21,6 +21,7 @@ def test_layer_norm(D):
                        (lambda: op.layer_norm_backward(x, x, vector, per_row), "mean must be"), (lambda: op.layer_norm_backward(x, x, per_row, vector), "rstd must be"),
                        (lambda: op.layer_norm_backward(double, x, per_row, per_row), "dy must be"), (lambda: op.layer_norm_backward(x.T, x, per_row, per_row), "dy must be"),
                        (lambda: op.layer_norm_backward(x, x, per_row, per_row, per_row), "gamma must be"),
+                       (lambda: op.layer_norm_backward(x, x, per_row, per_row, out=(None, vector, None)), "without gamma"),
                        (lambda: op.layer_norm_backward(x, x, per_row, per_row, vector, out=(None, None, per_row)), "dbeta must be")):
         with pytest.raises(D.DaliError, match=text):
             call()
@@ -39,7 +40,8 @@ def test_token_log_probs(D):
                        (lambda: op.token_log_probs(x, whole), "tokens must be int"), (lambda: op.token_log_probs(x, tokens, -1), "k must be from 0 to 6"),
                        (lambda: op.token_log_probs(x, tokens, 7), "k must be from 0 to 6"), (lambda: op.token_log_probs(D.Array.empty((4, 900)), tokens, 65), "k must be from 0 to 64"),
                        (lambda: op.token_log_probs(x, tokens, 2 ** 32 + 1), "k must be from 0 to 6"), (lambda: op.token_log_probs(x, tokens, 10 ** 30), "k must be from 0 to 6"),
-                       (lambda: op.token_log_probs(D.Array.empty((4, 0)), tokens), "last axis"), (lambda: op.token_log_probs(x, tokens, 2, out=(None, None, None, x, None)), "top_log_probs must be"),
+                       (lambda: op.token_log_probs(D.Array.empty((4, 0)), tokens), "last axis"),
+                       (lambda: op.token_log_probs(x, tokens, 0, out=(None, None, None, x, None)), "with k = 0"), (lambda: op.token_log_probs(x, tokens, 2, out=(None, None, None, x, None)), "top_log_probs must be"),
                        (lambda: op.token_log_probs(x, tokens, 2, out=(None, None, None, None, D.Array.empty((4, 2)))), "top_tokens must be int"),
                        (lambda: op.token_log_probs_backward(vector, None, x, tokens, per_row, None), "d_log_probs must be"),
                        (lambda: op.token_log_probs_backward(per_row, per_row, x, tokens, per_row, None), "needs the entropy"),
