@@ -165,8 +165,8 @@ template <typename T>
 __device__ __forceinline__ void write_alternative(const LogProbArgs<T>& a, long r, const T* x, const RowResult<T>& q, int place, const Entry<T>& e) {
     const T v = e.value();
     const int p = e.position();
-    // (a NaN was ranked as -inf)
-    a.top[r * a.k + place] = q.nothing ? T(-INFINITY) : v == T(-INFINITY) ? x[p] - q.lse : v - q.lse;
+    // (as the given token's is written: lse would round away digits of rows far from 0. A NaN was ranked as -inf)
+    a.top[r * a.k + place] = q.nothing ? T(-INFINITY) : ((v == T(-INFINITY) ? x[p] : v) - q.m) - q.ln;
     a.top_tokens[r * a.k + place] = p;
 }
 

@@ -343,3 +343,18 @@ def test_device_refusals(gpu, D, rng):
     with pytest.raises(D.DaliError, match="d_logits overlaps logits"):
         op.token_log_probs_backward(one, None, buf[:8], tokens, one, None, out=buf[1:9])
     assert np.array_equal(buf.numpy(), before)
+
+
+@pytest.mark.parametrize("dtype", [np.float32, np.float64])
+@pytest.mark.parametrize("rows,vocab", [(7, 5), (9, 97), (5, 300), (1030, 1300), (300, 3001), (2, 50257), (140, 12345)])
+def test_an_alternative_has_the_given_tokens_log_probability(gpu, D, rng, rows, vocab, dtype):
+    # rows far from 0, where a difference to lse would lose digits that the difference to the maximum keeps
+    x = (rng.randint(-64, 64, (rows, vocab)) / 16.0 + 30000.0).astype(dtype)
+    k = 5
+    order = best(x, k)
+    X = D.Array.from_numpy(x)
+    for place in range(k):
+        tokens = np.ascontiguousarray(order[:, place]).astype(np.int32)
+        log_probs, _, _, top, top_tokens = D.op.token_log_probs(X, D.Array.from_numpy(tokens), k)
+        assert np.array_equal(top_tokens.numpy()[:, place], tokens)
+        assert np.array_equal(top.numpy()[:, place], log_probs.numpy())
