@@ -365,7 +365,7 @@ __global__ __launch_bounds__(1024) void norm_backward_rows(NormBackwardArgs<T> a
 // ... and the weights by columns, over one part of the rows
 template <typename T>
 __global__ __launch_bounds__(kThreads) void norm_weights(NormBackwardArgs<T> a) {
-    const int c = blockIdx.x * kThreads + threadIdx.x;
+    const long c = (long)blockIdx.x * kThreads + threadIdx.x;  // (may pass 31 bits in the last workgroup)
     if (c >= a.width) return;
     T g = 0, b = 0;
 #pragma unroll 4
@@ -461,7 +461,7 @@ int backward(NormBackwardArgs<T> a) {
     a.partial = (T*)(workspace() + kWorkspaceCounterBytes);
     a.parts = 1;
     if (a.rows == 0) {
-        if (a.dgamma) hipLaunchKernelGGL(norm_weights<T>, dim3((a.width + kThreads - 1) / kThreads), dim3(kThreads), 0, stream(), a);
+        if (a.dgamma) hipLaunchKernelGGL(norm_weights<T>, dim3((unsigned)(((long)a.width + kThreads - 1) / kThreads)), dim3(kThreads), 0, stream(), a);
         return launched("dali_hip_layer_norm_backward");
     }
     const bool held = team_for<4096>(groups_of<T>(a.width), [&](auto team, auto e) {
@@ -492,7 +492,7 @@ int backward(NormBackwardArgs<T> a) {
     if (!held && a.dgamma) {
         // (the weights first: dx may take the place of x or dy)
         a.parts = (int)std::max(1L, std::min({64L, a.rows, fit}));
-        hipLaunchKernelGGL(norm_weights<T>, dim3((a.width + kThreads - 1) / kThreads, a.parts), dim3(kThreads), 0, stream(), a);
+        hipLaunchKernelGGL(norm_weights<T>, dim3((unsigned)(((long)a.width + kThreads - 1) / kThreads), a.parts), dim3(kThreads), 0, stream(), a);
     }
     if (a.dgamma && a.parts > 1) hipLaunchKernelGGL(norm_fold<T>, dim3((unsigned)((2L * a.width + 15) / 16)), dim3(kThreads), 0, stream(), a);
     if (!held)
