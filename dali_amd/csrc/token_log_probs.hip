@@ -798,16 +798,20 @@ bool short_rows(int groups, F launch) {
     return false;
 }
 
+// Workgroups of a launch: HIP takes fewer than 2^32 threads along an axis. More rows take several launches, of which a failed one is the last.
+constexpr long kMostBlocks = 1L << 23;
+static_assert(kMostBlocks * kThreads < 1L << 32, "threads of a launch");
+
 template <typename T>
 int forward(LogProbArgs<T> all) {
+    const char* what = "dali_hip_token_log_probs";
     const int groups = groups_of<T>(all.vocab);
     // A wave per row up to 256 groups, and to 512 where there are rows enough for all waves, a workgroup above. Wave and workgroup, with 5 alternatives (us): 256x2000 5.9 and
     // 4.8, 1023x2000 6.0 and 6.1, 8192x2000 18 and 23, 65536x2000 107 and 164; above 512 groups 65536x3000 234 and 187.
     const bool is_short = groups <= 256 || (groups <= 512 && all.rows >= 1024);
-    // a launch numbers its workgroups in 31 bits
     for (long done = 0; done < all.rows;) {
         LogProbArgs<T> a = all;
-        a.rows = std::min(all.rows - done, 1L << 24);
+        a.rows = std::min(all.rows - done, kMostBlocks);
         a.logits += done * a.stride;
         a.tokens += done;
         a.log_probs += done, a.entropy += done, a.lse += done;
@@ -822,6 +826,7 @@ int forward(LogProbArgs<T> all) {
                 if (a.k) hipLaunchKernelGGL((log_prob_short<T, LANES, E, true>), grid, dim3(kThreads), 0, stream(), a);
                 else hipLaunchKernelGGL((log_prob_short<T, LANES, E, false>), grid, dim3(kThreads), 0, stream(), a);
             });
+            if (launched(what)) return DALI_HIP_ERROR;
             continue;
         }
         // Few long rows are cut into segments of at least 512 groups, two for a thread, 512 workgroups or so together. The segments' alternatives are joined in one list,
@@ -853,8 +858,9 @@ int forward(LogProbArgs<T> all) {
         };
         if (a.k) launch(std::true_type());
         else launch(std::false_type());
+        if (launched(what)) return DALI_HIP_ERROR;
     }
-    return launched("dali_hip_token_log_probs");
+    return DALI_HIP_OK;
 }
 
 template <typename T>
@@ -864,7 +870,7 @@ int backward(LogProbBackwardArgs<T> all) {
     const long pieces = ((long)groups + 4 * kThreads - 1) / (4 * kThreads);
     for (long done = 0; done < all.rows;) {
         LogProbBackwardArgs<T> a = all;
-        a.rows = std::min(all.rows - done, std::max(1L, (1L << 24) / pieces));
+        a.rows = std::min(all.rows - done, std::max(1L, kMostBlocks / pieces));
         a.logits += done * a.stride;
         a.d_logits += done * a.vocab;
         a.tokens += done;
@@ -872,17 +878,18 @@ int backward(LogProbBackwardArgs<T> all) {
         if (a.d_entropy) a.d_entropy += done, a.entropy += done;
         done += a.rows;
         a.pieces = (int)pieces;
-        if (short_rows<256>(groups, [&](auto lanes, auto e) {
-                constexpr int per = kThreads / decltype(lanes)::value;
-                either_way(past, [&](auto p) {
-                    hipLaunchKernelGGL((log_prob_backward_short<T, decltype(lanes)::value, decltype(e)::value, decltype(p)::value>), dim3((unsigned)((a.rows + per - 1) / per)),
-                                       dim3(kThreads), 0, stream(), a);
-                });
-            }))
-            continue;
-        either_way(past, [&](auto p) { hipLaunchKernelGGL((log_prob_backward_long<T, decltype(p)::value>), dim3((unsigned)(a.rows * pieces)), dim3(kThreads), 0, stream(), a); });
+        const bool is_short = short_rows<256>(groups, [&](auto lanes, auto e) {
+            constexpr int per = kThreads / decltype(lanes)::value;
+            either_way(past, [&](auto p) {
+                hipLaunchKernelGGL((log_prob_backward_short<T, decltype(lanes)::value, decltype(e)::value, decltype(p)::value>), dim3((unsigned)((a.rows + per - 1) / per)),
+                                   dim3(kThreads), 0, stream(), a);
+            });
+        });
+        if (!is_short)
+            either_way(past, [&](auto p) { hipLaunchKernelGGL((log_prob_backward_long<T, decltype(p)::value>), dim3((unsigned)(a.rows * pieces)), dim3(kThreads), 0, stream(), a); });
+        if (launched("dali_hip_token_log_probs_backward")) return DALI_HIP_ERROR;
     }
-    return launched("dali_hip_token_log_probs_backward");
+    return DALI_HIP_OK;
 }
 
 }  // namespace
