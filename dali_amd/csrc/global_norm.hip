@@ -4,7 +4,7 @@
 //
 // Squares are summed in double (an fp32 value's square neither overflows nor vanishes there). A workgroup sums the chunks that fall to it and leaves one
 // partial; every workgroup of the second launch folds all partials in the same order before it scales, so the norm does not depend on scheduling and needs no
-// launch of its own. The second launch walks the chunks backwards: what the first read last is still in the cache. A norm that is not finite
+// launch of its own. (The partials lie where no other kernel writes until the second launch has been issued: Carried, runtime.h.) The second launch walks the chunks backwards: what the first read last is still in the cache. A norm that is not finite
 // scales nothing: the arrays come back as they are and the norm says so, and arrays that are their own destinations are left alone whenever nothing is scaled.
 // Bound by memory: 52 million fp32 values in 24 arrays 103 us, 38 for the norm (5.4 TB/s) and 64 to 68 for the scaling (6.3 TB/s read and written, half of the reading from
 // the cache); 45 thousand in 12 arrays 11 us, where two launches and the host are all there is.
@@ -20,6 +20,8 @@ constexpr int kThreads = 256;
 constexpr int kBatch = 96;       // arrays per launch: their addresses travel with it (kernel arguments hold 4 KiB); up to kFew of them in a smaller form
 constexpr int kFew = 16;
 constexpr int kPartials = 2048;  // workgroups of the first launch, as far as one launch goes
+constexpr int kMostArrays = 1 << 24;
+static_assert((kMostArrays / kBatch + 1L) * 16 * sizeof(double) <= kCarriedBytes, "partial sums of as many launches");
 constexpr int kUnroll = 4;       // groups of 16 bytes that a thread has in flight
 
 template <int MOST>
@@ -188,7 +190,8 @@ bool taken_by_one(int count, const void* const* in, void* const* out, const int6
 
 template <typename T, int MOST>
 int clip_batches(int count, const void* const* in, void* const* out, const int64_t* sizes, double max_norm, T* norm) {
-    double* partial = (double*)(workspace() + kWorkspaceCounterBytes);
+    const Carried carried;
+    double* partial = (double*)carried.data();
     long total = 0;
     for (int i = 0; i < count; ++i) total += sizes[i];
     constexpr int STEP = kThreads * Vec<T>::N * kUnroll;
@@ -269,7 +272,7 @@ extern "C" int dali_hip_clip_by_global_norm(int dtype, int count, const void* co
     for (int i = 0; i < count; ++i)
         if (sizes[i] < 0 || (sizes[i] > 0 && (!in[i] || (out && !out[i])))) return fail("%s: array %d has no memory or a negative size", what, i);
     // (partial sums: kPartials, or 16 for every launch of kBatch arrays; chunks are numbered in 31 bits)
-    if (count > (1 << 24)) return fail("%s: %d arrays are more than the workspace has room for", what, count);
+    if (count > kMostArrays) return fail("%s: %d arrays are more than there is room for", what, count);
     for (int i = 0; i < count; ++i)
         if (off_elements({in[i], out ? out[i] : nullptr, norm}, size)) return fail("%s: an address is off its type's size", what);
     const Span result("norm", norm, 1, size);

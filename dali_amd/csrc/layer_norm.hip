@@ -457,8 +457,9 @@ int forward(NormArgs<T> a) {
 template <typename T>
 int backward(NormBackwardArgs<T> a) {
     const bool past = past_caches(3.0 * sizeof(T) * a.rows * a.width);
-    const long fit = (long)(kWorkspacePartialBytes / (2 * sizeof(T) * (size_t)a.width));  // rows of partial sums that the workspace holds
-    a.partial = (T*)(workspace() + kWorkspaceCounterBytes);
+    const long fit = (long)(kCarriedBytes / (2 * sizeof(T) * (size_t)a.width));  // rows of partial sums that there is room for
+    const Carried carried;  // (to the launch that folds them)
+    a.partial = (T*)carried.data();
     a.parts = 1;
     if (a.rows == 0) {
         if (a.dgamma) hipLaunchKernelGGL(norm_weights<T>, dim3((unsigned)(((long)a.width + kThreads - 1) / kThreads)), dim3(kThreads), 0, stream(), a);

@@ -53,7 +53,7 @@ struct Runtime {
     hipStream_t copy_stream = nullptr;
     hipEvent_t order_event = nullptr;
     std::string arch = "gfx950";
-    // workspace: [counters | partials]
+    // workspace: [counters | partials | what launches carry to the next]
     char* ws = nullptr;
     // bank: size class -> parked blocks. Blocks up to kSlabBlockMax are carved out of large slabs (a driver
     // allocation costs tens to hundreds of microseconds whatever its size); larger ones are driver allocations
@@ -85,6 +85,10 @@ static Runtime& rt() {
 
 hipStream_t stream() { return rt().stream; }
 char* workspace() { return rt().ws; }
+
+static std::mutex g_carried;
+Carried::Carried() : lock_(g_carried) {}
+
 int bound_device() { return rt().ready ? rt().device : -1; }
 
 int ensure_init() {
@@ -208,7 +212,7 @@ int dali_hip_init(int device) {
     if (colon != std::string::npos) arch = arch.substr(0, colon);
     r.arch = arch;
     HIP_TRY(hipStreamCreateWithFlags(&r.stream, hipStreamNonBlocking));
-    HIP_TRY(hipMalloc((void**)&r.ws, kWorkspaceBytes));
+    HIP_TRY(hipMalloc((void**)&r.ws, kWorkspaceBytes + kCarriedBytes));
     HIP_TRY(hipMemsetAsync(r.ws, 0, kWorkspaceBytes, r.stream));
     HIP_TRY(hipStreamSynchronize(r.stream));
     if (sort_scratch_init(device)) return DALI_HIP_ERROR;
@@ -788,6 +792,7 @@ int dali_hip_capture_end(void** graph_exec) {
 }
 
 int dali_hip_graph_launch(void* graph_exec) {
+    const Carried carried;  // (the graph may hold launches that carry partial results to the next, and is put on the stream node by node)
     HIP_TRY(hipGraphLaunch((hipGraphExec_t)graph_exec, rt().stream));
     return DALI_HIP_OK;
 }

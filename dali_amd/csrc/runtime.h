@@ -4,6 +4,7 @@
 
 #include <hip/hip_runtime.h>
 
+#include <mutex>
 #include <string>
 
 #include "../../include/dali_hip.h"
@@ -17,6 +18,8 @@ constexpr int kWorkspaceCounters = 16384;
 constexpr size_t kWorkspaceCounterBytes = (size_t)kWorkspaceCounters * 4;
 constexpr size_t kWorkspacePartialBytes = (size_t)32 << 20;
 constexpr size_t kWorkspaceBytes = kWorkspaceCounterBytes + kWorkspacePartialBytes;
+// Behind it, partial results that one launch leaves for another of the same entry point
+constexpr size_t kCarriedBytes = (size_t)32 << 20;
 // Words between n of the counters that are drawn from at the same time: memory takes an arrival every 12 ns or so at one cache line,
 // whichever word it goes to, so they lie 256 bytes apart as far as there is room.
 inline int counter_step(long n) {
@@ -30,6 +33,15 @@ int fail_str(const std::string& s);
 int ensure_init();
 hipStream_t stream();
 char* workspace();
+// The block of partial results that launches carry to the next one, for whoever holds it: from before the first launch until the last is issued, so that
+// another host thread's launches that use it come before or after both. What finishes with the workspace within one launch may come between them.
+class Carried {
+    std::lock_guard<std::mutex> lock_;
+
+   public:
+    Carried();
+    char* data() const { return workspace() + kWorkspaceBytes; }
+};
 // device the library is bound to, -1 before dali_hip_init
 int bound_device();
 // sort.hip: looks up the device address of its built-in scratch array; called by dali_hip_init with `device` current

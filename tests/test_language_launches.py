@@ -1,5 +1,5 @@
-"""What the operators of language models launch, written down by a program that answers for the device: sizes of the launches and what a failed one
-stops."""
+"""What the operators of language models launch, written down by a program that answers for the device: sizes of the launches, what a failed one stops, and launches
+that belong together."""
 import os
 import subprocess
 
@@ -44,3 +44,20 @@ def test_a_failed_launch_is_the_last(recorder, op, extent):
     for failing in (0, 1):
         (_, status, launches, _, _), = recorder("one", op, 0, 5 << 24, extent, 0, failing)
         assert int(status) != 0 and int(launches) == failing + 1
+
+
+def test_two_threads_do_not_part_what_belongs_together(recorder):
+    """The partial sums that one launch leaves are read by the next: what another thread launches between the two must not be such a pair's half."""
+    assert [k for k, in recorder("threads", "squares")] == ["squares", "rescale", "norm_backward_team", "norm_fold"]
+    assert [k for k, in recorder("threads", "norm_backward_team")] == ["norm_backward_team", "norm_fold", "squares", "rescale"]
+    assert [k for k, in recorder("threads", "graph")] == ["graph_begins", "graph_ends", "squares", "rescale"]
+
+
+def test_partial_sums_that_wait_for_another_launch_have_a_place_of_their_own(recorder):
+    """Kernels that finish with the workspace within one launch may come between the two of a pair."""
+    lines = recorder("places")
+    assert all(int(status) == 0 for _, status, *_ in lines)
+    places = {kind: sorted({int(p) for k, _, *found in lines if k == kind for p in found}) for kind in ("one", "two")}
+    assert len(places["one"]) >= 2 and places["two"]
+    partials = 65536 + (32 << 20)  # counters and the partial sums of single launches
+    assert places["one"][-1] < partials <= places["two"][0]
