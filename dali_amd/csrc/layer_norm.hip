@@ -4,7 +4,8 @@
 //   u = (x - mean) rstd,  a = dy gamma,  dx = rstd (a - mean(a) - u mean(a u)),  dgamma = sum over rows of dy u,  dbeta = that of dy
 //
 // Sums are held in the operands' own type (32 bits or more). The variance is the mean of squared distances from the mean, with the mean's own
-// rounding error taken out again (x - mean sums to delta n where the mean is off by delta): rows far from zero keep their digits.
+// rounding error taken out again (x - mean sums to delta n where the mean is off by delta): rows far from zero keep their digits. Rows for which
+// this is not enough, because delta is most of the distances or because sums pass the type's range, are taken again (norm_apart).
 #include <algorithm>
 #include <type_traits>
 
@@ -30,7 +31,8 @@ template <typename T, int TEAM, int TEAMS = 1>
 struct TeamScratch {
     T v[TEAM > 64 ? 2 : 1][TEAM > 64 ? TEAMS * TEAM / 64 : 1][2];
 };
-template <int TEAM, typename T, int TEAMS>
+// (AT_ONCE: waves whose sums are read side by side, in as many registers)
+template <int TEAM, int AT_ONCE = 16, typename T, int TEAMS>
 __device__ __forceinline__ void team_sum(T& p, T& q, TeamScratch<T, TEAM, TEAMS>& scratch, int& turn) {
     p = fold_lanes<(TEAM < 64 ? TEAM : 64)>(p, Sum());
     q = fold_lanes<(TEAM < 64 ? TEAM : 64)>(q, Sum());
@@ -41,7 +43,7 @@ __device__ __forceinline__ void team_sum(T& p, T& q, TeamScratch<T, TEAM, TEAMS>
         __syncthreads();
         const int from = TEAMS == 1 ? 0 : threadIdx.x / TEAM * (TEAM / 64);
         p = s[from][0], q = s[from][1];
-#pragma unroll
+#pragma unroll AT_ONCE
         for (int w = 1; w < TEAM / 64; ++w) p += s[from + w][0], q += s[from + w][1];
     }
 }
@@ -52,11 +54,91 @@ __device__ __forceinline__ T root_of(T variance, T epsilon) {
     return T(1) / sqrt((variance < T(0) ? T(0) : variance) + epsilon);
 }
 
+// Whether a row's variance can be taken as the mean square `spread` of its distances from the mean less the square of their own mean `off`: that keeps its digits (three
+// quarters of the spread are left, or what is lost is nothing beside epsilon), and nothing has passed the type's range.
+template <typename T>
+__device__ __forceinline__ bool settled(T off, T spread, T epsilon) {
+    return (off * off <= T(0.25) * spread + T(1.0 / 4096) * epsilon) & (spread < T(INFINITY));
+}
+
+// A row that is not is marked by an rstd below 0 and taken again once its team is through with all others: its y is not written until then, so it is still there where
+// y takes its place, and the kernels' registers stay those of ordinary rows (as further passes over a row in registers 72 became 76 to 100, and
+// 65536x200 took 24.0 us instead of 21.4).
+template <typename T>
+__device__ __forceinline__ T mark(T spread) {
+    return spread < T(INFINITY) ? T(-1) : T(-2);
+}
+
+// The row is read times a power of two where something passed the range (so 2^31 of the largest squares do not), and the distances are made good by their mean
+// before the squares are taken: they are small multiples of the values' last place where that matters, so both differences are exact, and a row
+// of one value has distances of 0. Four readings a value at a time, the later ones in the caches: 8192x1024 of nothing but such rows 27 us, of others 11.7.
+template <typename T>
+struct Scaled;
+template <>
+struct Scaled<float> {
+    static constexpr float down = 0x1p-81f, up = 0x1p81f;
+};
+template <>
+struct Scaled<double> {
+    static constexpr double down = 0x1p-540, up = 0x1p540;
+};
+template <int TEAM, typename T, typename Scratch>
+__device__ __forceinline__ void norm_apart(const NormArgs<T>& a, long r, int l, T down, Scratch& scratch, int& turn) {
+    const T* x = a.x + r * a.stride;
+    const T count = a.width;
+    T s = 0, off = 0, rest = 0, square = 0, none = 0;
+#pragma unroll 1
+    for (long c = l; c < a.width; c += TEAM) s += x[c] * down;
+    team_sum<TEAM, 1>(s, none, scratch, turn);
+    const T near = s / count;
+#pragma unroll 1
+    for (long c = l; c < a.width; c += TEAM) off += x[c] * down - near;
+    team_sum<TEAM, 1>(off, none, scratch, turn);
+    off /= count;
+#pragma unroll 1
+    for (long c = l; c < a.width; c += TEAM) {
+        const T d = (x[c] * down - near) - off;
+        rest += d;
+        square += d * d;
+    }
+    team_sum<TEAM, 1>(rest, square, scratch, turn);
+    rest /= count;
+    T variance = square / count - rest * rest;
+    variance = variance < T(0) ? T(0) : variance;
+    // (scaled down, epsilon may vanish: beside any variance that is not 0 it is nothing)
+    const T unit = variance == T(0) ? root_of(variance, a.epsilon) : root_of(variance, a.epsilon * down * down);
+    T* y = a.y + r * a.width;
+#pragma unroll 1
+    for (long c = l; c < a.width; c += TEAM) {
+        const T u = (((x[c] * down - near) - off) - rest) * unit;
+        y[c] = u * (a.gamma ? a.gamma[c] : T(1)) + (a.beta ? a.beta[c] : T(0));
+    }
+    if (l == 0) {
+        const T mean = (near + off) + rest;
+        a.mean[r] = down < T(1) ? mean * Scaled<T>::up : mean;
+        a.rstd[r] = variance == T(0) ? unit : unit * down;
+    }
+}
+template <int TEAM, int TEAMS, typename T, typename Scratch>
+__device__ __forceinline__ void norm_marked(const NormArgs<T>& a, Scratch& scratch, int& turn) {
+    int l = threadIdx.x % TEAM;
+    asm volatile("" : "+v"(l)::"memory");  // (no address is kept in registers for this)
+#pragma unroll 1
+    for (long first = (long)blockIdx.x * TEAMS; first < a.rows; first += (long)gridDim.x * TEAMS) {
+        const long r = first + threadIdx.x / TEAM;
+        if (r >= a.rows) continue;
+        T marked = l == 0 ? a.rstd[r] : T(0), none = 0;  // (of the thread that wrote it)
+        team_sum<TEAM, 1>(marked, none, scratch, turn);
+        if (marked < T(0)) norm_apart<TEAM>(a, r, l, marked == mark(T(0)) ? T(1) : Scaled<T>::down, scratch, turn);
+    }
+}
+
 // A team of TEAM threads per row, which lives in their registers, E groups of 16 bytes to a thread: read once, written once, which bounds it. WHOLE: the teams' groups are
 // the row exactly. The weights stay in registers from row to row where they fit. 8192x1024 11.5 us (5.8 TB/s), 65536x1024 89 us (6.0), 32768x4096 187 us (5.7); 8x1024 4.4 us
 // among others, 2.9 of them on the device.
+// (the bound on waves: of 3001x2047 in double 18.4 us, without it 19.5; of 32768x2999 in float 150, without it 141)
 template <typename T, int TEAM, int E, bool WHOLE, bool PAST>
-__global__ __launch_bounds__(TEAM > kThreads ? TEAM : kThreads) void norm_team(NormArgs<T> a) {
+__global__ __launch_bounds__(TEAM > kThreads ? TEAM : kThreads, TEAM == 256 && E == 4 && sizeof(T) == 8 ? 5 : 1) void norm_team(NormArgs<T> a) {
     constexpr int N = Vec<T>::N, BLOCK = TEAM > kThreads ? TEAM : kThreads, TEAMS = BLOCK / TEAM;
     constexpr bool HOLD = E * N <= 16, LONG = TEAM > 8;  // (8 threads are given the shortest rows)
     __shared__ TeamScratch<T, TEAM> scratch;
@@ -83,6 +165,7 @@ __global__ __launch_bounds__(TEAM > kThreads ? TEAM : kThreads) void norm_team(N
 #pragma unroll
         for (int e = 0; e < E; ++e) weights(e, gamma[e], beta[e]);
     }
+    bool apart = false;
     for (long first = (long)blockIdx.x * TEAMS; first < a.rows; first += (long)gridDim.x * TEAMS) {
         const long row = first + threadIdx.x / TEAM, r = row < a.rows ? row : a.rows - 1;  // (a team without a row goes along with the last)
         const T* x = a.x + r * a.stride;
@@ -111,12 +194,16 @@ __global__ __launch_bounds__(TEAM > kThreads ? TEAM : kThreads) void norm_team(N
             }
         team_sum<TEAM>(off, square, scratch, turn);
         off /= count;
-        const T rstd = root_of(square / count - off * off, a.epsilon);
+        const T spread = square / count;
+        const bool plain = settled(off, spread, a.epsilon);
+        apart |= !plain;
+        const T rstd = root_of(spread - off * off, a.epsilon);
         if (row < a.rows) {
             if (l == 0) {
                 a.mean[r] = near + off;
-                a.rstd[r] = rstd;
+                a.rstd[r] = plain ? rstd : mark(spread);
             }
+            if (!plain) continue;
 #pragma unroll
             for (int e = 0; e < E; ++e) {
                 T g[N], b[N];
@@ -130,9 +217,10 @@ __global__ __launch_bounds__(TEAM > kThreads ? TEAM : kThreads) void norm_team(N
             }
         }
     }
+    if (__builtin_amdgcn_ballot_w64(apart) != 0) norm_marked<TEAM, TEAMS>(a, scratch, turn);
 }
 
-// Rows that no workgroup's registers hold: a workgroup walks each three times, the later ones in the caches
+// Rows that no workgroup's registers hold, or not without spilling: a workgroup walks each three times, the later ones in the caches
 template <typename T, bool PAST>
 __global__ __launch_bounds__(1024) void norm_rows(NormArgs<T> a) {
     constexpr int N = Vec<T>::N, BLOCK = 1024;
@@ -140,6 +228,7 @@ __global__ __launch_bounds__(1024) void norm_rows(NormArgs<T> a) {
     int turn = 0;
     const int groups = groups_of<T>(a.width);
     const T count = a.width;
+    bool apart = false;
     for (long r = blockIdx.x; r < a.rows; r += gridDim.x) {
         const T* x = a.x + r * a.stride;
         T* y = a.y + r * a.width;
@@ -163,7 +252,13 @@ __global__ __launch_bounds__(1024) void norm_rows(NormArgs<T> a) {
         }
         team_sum<BLOCK>(off, square, scratch, turn);
         off /= count;
-        const T rstd = root_of(square / count - off * off, a.epsilon);
+        const T spread = square / count;
+        if (!settled(off, spread, a.epsilon)) {
+            apart = true;
+            if (threadIdx.x == 0) a.rstd[r] = mark(spread);
+            continue;
+        }
+        const T rstd = root_of(spread - off * off, a.epsilon);
         for (int j = threadIdx.x; j < groups; j += BLOCK) {
             load_group(x, j * N, a.width, T(0), v);
 #pragma unroll
@@ -179,6 +274,7 @@ __global__ __launch_bounds__(1024) void norm_rows(NormArgs<T> a) {
             a.rstd[r] = rstd;
         }
     }
+    if (__builtin_amdgcn_ballot_w64(apart) != 0) norm_marked<BLOCK, 1>(a, scratch, turn);
 }
 
 template <typename T>
@@ -440,12 +536,17 @@ bool team_for(int groups, F launch) {
 template <typename T>
 int forward(NormArgs<T> a) {
     const bool past = past_caches(2.0 * sizeof(T) * a.rows * a.width);
-    const bool held = team_for<8192>(groups_of<T>(a.width), [&](auto team, auto e) {
+    const int groups = groups_of<T>(a.width);
+    // Rows of more than 4096 groups that are not whole do not fit the registers without spilling some. Held and walked three times (us): 4096x20000 180 and 155, 4096x31000 226
+    // and 261, 8x20000 10.3 and 7.3; in double 4096x9001 227 and 158, 4096x15000 272 and 254, and whole 4096x16384 198 and 291.
+    const bool walked = groups > 4096 && a.width != 8192 * Vec<T>::N && (groups <= 6144 || sizeof(T) == 8);
+    const bool held = !walked && team_for<8192>(groups, [&](auto team, auto e) {
         constexpr int TEAM = decltype(team)::value, E = decltype(e)::value, BLOCK = TEAM > kThreads ? TEAM : kThreads, TEAMS = BLOCK / TEAM;
         const dim3 grid((unsigned)std::min((a.rows + TEAMS - 1) / TEAMS, 8192L * kThreads / BLOCK));
         either_way(past, [&](auto p) {
             either_way(a.width == TEAM * E * Vec<T>::N, [&](auto whole) {
-                hipLaunchKernelGGL((norm_team<T, TEAM, E, decltype(whole)::value, decltype(p)::value>), grid, dim3(BLOCK), 0, stream(), a);
+                if constexpr (E < 8 || sizeof(T) == 4 || decltype(whole)::value)
+                    hipLaunchKernelGGL((norm_team<T, TEAM, E, decltype(whole)::value, decltype(p)::value>), grid, dim3(BLOCK), 0, stream(), a);
             });
         });
     });

@@ -350,8 +350,9 @@ int dali_hip_softmax_axis_supported(long long outer, int extent, long long inner
 /* ------------------------------------------------------------- layer normalisation */
 /*
  * Rows of `width` values, x_stride values apart (x may be a view of wider rows): mean = sum(x) / width, rstd = 1 / sqrt(mean((x - mean)^2) + epsilon),
- * y = (x - mean) rstd gamma + beta. dtype: DALI_HIP_FLOAT or DALI_HIP_DOUBLE, of every operand. gamma and beta [width] may be NULL (1 and 0). y
- * [rows, width], mean and rstd [rows] are dense; y may be x itself where that is dense, any other overlap is refused. The reference has none.
+ * y = (x - mean) rstd gamma + beta. dtype: DALI_HIP_FLOAT or DALI_HIP_DOUBLE, of every operand. Rows of any finite values are served, whether their sums and
+ * squares fit the type or not. gamma and beta [width] may be NULL (1 and 0). y [rows, width], mean and rstd [rows] are dense; y may be x itself where that is
+ * dense, any other overlap is refused. The reference has none.
  */
 int dali_hip_layer_norm(int dtype, int64_t rows, int width, const void* x, int64_t x_stride, const void* gamma, const void* beta, double epsilon, void* y, void* mean,
                         void* rstd);
