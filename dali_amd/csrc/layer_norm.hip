@@ -286,6 +286,15 @@ struct NormBackwardArgs {
     int width, parts;
 };
 
+// u = (x - mean) rstd of a row, from halves: x - mean may pass the type's range where x and mean do not. (Nothing is lost by it: what halving rounds off is
+// below the smallest normal number, and an rstd that is finite stands for a deviation far above.)
+template <typename T>
+struct Normalised {
+    T mean, twice;
+    __device__ __forceinline__ Normalised(T row_mean, T rstd) : mean(row_mean * T(0.5)), twice(rstd * T(2)) {}
+    __device__ __forceinline__ T operator()(T x) const { return (x * T(0.5) - mean) * twice; }
+};
+
 // the value of the lane D further on in its half (D = 8: of 16 lanes) or in the other half, without a condition on closer lanes
 template <int D, typename T>
 __device__ __forceinline__ T plus_across(T v) {
@@ -346,7 +355,8 @@ __global__ __launch_bounds__(TEAM * TEAMS) void norm_backward_team(NormBackwardA
         const long row = first + threadIdx.x / TEAM, r = row < a.rows ? row : a.rows - 1;
         const bool live = row < a.rows;  // (a team without a row goes along with the last, and adds nothing)
         if constexpr (!AHEAD) ask(row);
-        const T row_mean = mean, row_rstd = rstd;
+        const Normalised<T> normalised(mean, rstd);
+        const T row_rstd = rstd;
         T u[E][N], d[E][N];
 #pragma unroll
         for (int e = 0; e < E; ++e) {
@@ -361,7 +371,7 @@ __global__ __launch_bounds__(TEAM * TEAMS) void norm_backward_team(NormBackwardA
 #pragma unroll
             for (int i = 0; i < N; ++i) {
                 const bool in = WHOLE || (l + e * TEAM) * N + i < a.width;
-                u[e][i] = in ? (u[e][i] - row_mean) * row_rstd : T(0);
+                u[e][i] = in ? normalised(u[e][i]) : T(0);
                 if constexpr (WEIGHTS) {
                     dgamma[e][i] += live ? d[e][i] * u[e][i] : T(0);
                     dbeta[e][i] += live ? d[e][i] : T(0);
@@ -428,6 +438,7 @@ __global__ __launch_bounds__(1024) void norm_backward_rows(NormBackwardArgs<T> a
         const T *x = a.x + r * a.x_stride, *dy = a.dy + r * a.dy_stride;
         T* dx = a.dx + r * a.width;
         const T mean = a.mean[r], rstd = a.rstd[r];
+        const Normalised<T> normalised(mean, rstd);
         T level = 0, along = 0, u[N], d[N], g[N];
         auto load = [&](int j) {
             load_group(x, j * N, a.width, mean, u);
@@ -437,7 +448,7 @@ __global__ __launch_bounds__(1024) void norm_backward_rows(NormBackwardArgs<T> a
             if (a.gamma) load_group(a.gamma, j * N, a.width, T(0), g);
 #pragma unroll
             for (int i = 0; i < N; ++i) {
-                u[i] = (u[i] - mean) * rstd;
+                u[i] = normalised(u[i]);
                 d[i] *= g[i];
             }
         };
@@ -467,7 +478,7 @@ __global__ __launch_bounds__(kThreads) void norm_weights(NormBackwardArgs<T> a) 
 #pragma unroll 4
     for (long r = blockIdx.y; r < a.rows; r += a.parts) {
         const T d = a.dy[r * a.dy_stride + c];
-        g += d * ((a.x[r * a.x_stride + c] - a.mean[r]) * a.rstd[r]);
+        g += d * Normalised<T>(a.mean[r], a.rstd[r])(a.x[r * a.x_stride + c]);
         b += d;
     }
     if (a.parts == 1) {

@@ -3,7 +3,7 @@
 import numpy as np
 import pytest
 
-from test_gpu_layer_norm import U, depth, oracle
+from test_gpu_layer_norm import U, backward_bounds, depth, oracle
 
 pytestmark = pytest.mark.gpu
 
@@ -110,3 +110,20 @@ def test_a_row_does_not_depend_on_the_others(gpu, D, rng, width):
     place = D.Array.from_numpy(odd)
     D.op.layer_norm(place, out=(place, None, None))
     assert np.array_equal(place.numpy(), norm(D, odd)[0], equal_nan=True)
+
+
+@pytest.mark.parametrize("width", [2, 3, 64, 97, 250, 1024, 5000, 20000, 50001])
+@pytest.mark.parametrize("dtype", [np.float32, np.float64])
+def test_gradient_at_the_ends_of_the_range(gpu, D, rng, width, dtype):
+    """x - mean passes the type's range where x does not; u = (x - mean) rstd is an ordinary number."""
+    big, u, rows = np.finfo(dtype).max, U[dtype], 40
+    x = np.where(rng.rand(rows, width) < 0.2, big, -big).astype(dtype)
+    x[:, 0], x[:, 1] = big, -big
+    x[1::2] *= dtype(0.2)
+    dy, gamma = rng.randn(rows, width).astype(dtype), (1 + 0.2 * rng.randn(width)).astype(dtype)
+    _, mean, rstd = (v.astype(dtype) for v in oracle(x, gamma, 0 * gamma, 1e-5))
+    got = [v.numpy() for v in D.op.layer_norm_backward(*[D.Array.from_numpy(v) for v in (dy, x, mean, rstd, gamma)])]
+    # (the statistics are operands: what they were rounded to is not the kernel's error)
+    for g, (want, bound) in zip(got, backward_bounds(dy, x, mean, rstd, gamma)):
+        assert np.isfinite(bound.astype(dtype)).all()
+        assert (np.abs(g - want) <= bound + 4 * np.finfo(dtype).smallest_subnormal).all()
