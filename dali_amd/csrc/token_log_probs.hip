@@ -726,8 +726,9 @@ struct RowGradient {
         entropy = a.d_entropy ? a.entropy[r] : T(0);
     }
     __device__ __forceinline__ T of(T x, int c) const {
-        const T d = x - lse;
-        return (c == token ? g : T(0)) - Real<T>::weight(d) * (g + h * (Max()(d, Real<T>::under) + entropy));
+        // (the weight first: an exponent whose weight is small or 0 would carry a large gradient past the type's range)
+        const T d = x - lse, w = Real<T>::weight(d);
+        return (c == token ? g : T(0)) - (w * g + (w * h) * (Max()(d, Real<T>::under) + entropy));
     }
 };
 
