@@ -2,8 +2,9 @@
 //
 //   norm = sqrt(sum over all arrays of sum of squares),  scale = max_norm / norm where norm > max_norm, else 1
 //
-// Squares are summed in double (an fp32 value's square neither overflows nor vanishes there). A workgroup sums the chunks that fall to it and leaves one
-// partial; every workgroup of the second launch folds all partials in the same order before it scales, so the norm does not depend on scheduling and needs no
+// Squares are summed in double (an fp32 value's square neither overflows nor vanishes there; squares of doubles go into three sums by the value's size, those of
+// large and of small values scaled by a power of two: Squares). A workgroup sums the chunks that fall to it and leaves its
+// partial sums; every workgroup of the second launch folds all partials in the same order before it scales, so the norm does not depend on scheduling and needs no
 // launch of its own. (The partials lie where no other kernel writes until the second launch has been issued: Carried, runtime.h.) The second launch walks the chunks backwards: what the first read last is still in the cache. A norm that is not finite
 // scales nothing: the arrays come back as they are and the norm says so, and arrays that are their own destinations are left alone whenever nothing is scaled.
 // Bound by memory: 52 million fp32 values in 24 arrays 103 us, 38 for the norm (5.4 TB/s) and 64 to 68 for the scaling (6.3 TB/s read and written, half of the reading from
@@ -21,8 +22,70 @@ constexpr int kBatch = 96;       // arrays per launch: their addresses travel wi
 constexpr int kFew = 16;
 constexpr int kPartials = 2048;  // workgroups of the first launch, as far as one launch goes
 constexpr int kMostArrays = 1 << 24;
-static_assert((kMostArrays / kBatch + 1L) * 16 * sizeof(double) <= kCarriedBytes, "partial sums of as many launches");
+constexpr int kLeast = 5;        // workgroups of a launch among many
+constexpr long kOther = 1 << 20;  // partial sums before the others of their workgroups
+static_assert((kMostArrays / kBatch + 1L) * kLeast <= kOther && 3 * kOther * sizeof(double) <= kCarriedBytes, "partial sums of as many launches");
 constexpr int kUnroll = 4;       // groups of 16 bytes that a thread has in flight
+
+// The sum of squares of fp32 values, or of doubles: those from 2^501 on times 2^-600, those below 2^-500 times 2^600, and the others, each in a sum of its own. 2^40 of
+// them pass no sum's range, and none vanishes in it. (mid, large, small)
+template <typename T>
+struct Squares {
+    static constexpr int SUMS = sizeof(T) == 4 ? 1 : 3;
+    double sum[SUMS] = {};
+    __device__ __forceinline__ void add(float v) { sum[0] += (double)v * (double)v; }
+    __device__ __forceinline__ void add(double v) {
+        const unsigned exponent = (unsigned)(__builtin_bit_cast(unsigned long long, v) >> 52) & 0x7ff;
+        if (__builtin_expect(exponent - (1023 - 500) <= 1000, 1)) sum[0] += v * v;
+        else if (exponent < 1023) sum[2] += (v * 0x1p600) * (v * 0x1p600);  // (zeros too)
+        else sum[1] += (v * 0x1p-600) * (v * 0x1p-600);  // (infinities and NaN too)
+    }
+    __device__ __forceinline__ void join(const Squares& o) {
+#pragma unroll
+        for (int i = 0; i < SUMS; ++i) sum[i] += o.sum[i];
+    }
+    __device__ __forceinline__ double norm() const {
+        if constexpr (SUMS == 1) {
+            return sqrt(sum[0]);
+        } else {
+            if (ordinary()) return sqrt(sum[0]);
+            const double s = sqrt(sum[2]) * 0x1p-600, m = sqrt(sum[0]) * 0x1p-600;
+            if (sum[1] != 0) return sqrt(sum[1] + m * m) * 0x1p600;
+            return sum[0] == 0 ? s : sqrt(sum[0] + s * s);
+        }
+    }
+    __device__ __forceinline__ bool ordinary() const { return SUMS == 1 || (sum[SUMS > 1 ? 1 : 0] == 0 && sum[SUMS > 1 ? 2 : 0] == 0); }
+    // over a workgroup, the same in each of its threads
+    template <int THREADS>
+    __device__ __forceinline__ void fold(double (&scratch)[THREADS / 64][SUMS]) {
+#pragma unroll
+        for (int i = 0; i < SUMS; ++i) sum[i] = fold_lanes<64>(sum[i], Sum());
+        if ((threadIdx.x & 63) == 0)
+#pragma unroll
+            for (int i = 0; i < SUMS; ++i) scratch[threadIdx.x >> 6][i] = sum[i];
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < SUMS; ++i) sum[i] = scratch[0][i];
+#pragma unroll
+        for (int w = 1; w < THREADS / 64; ++w)
+#pragma unroll
+            for (int i = 0; i < SUMS; ++i) sum[i] += scratch[w][i];
+    }
+};
+
+// What the arrays are multiplied by, in two factors: the first is 1 but where the product of both is below the normal numbers and would lose its digits. (In double: where the norm
+// passes the largest float, the scale would lose them in one.) `none`: nothing is scaled.
+struct Scale {
+    double first = 1, second = 1;
+    bool none;
+    __device__ __forceinline__ Scale(double norm, double max_norm) : none(!(norm > max_norm && norm < (double)INFINITY)) {
+        if (none) return;
+        second = max_norm / norm;
+        if (second < 0x1p-1000) first = 0x1p-600, second = max_norm / (norm * 0x1p-600);
+    }
+    __device__ __forceinline__ float of(float v) const { return (float)((double)v * second); }  // (a second factor below 2^-1000 leaves nothing of a float)
+    __device__ __forceinline__ double of(double v) const { return (v * first) * second; }
+};
 
 template <int MOST>
 struct Batch {
@@ -31,7 +94,7 @@ struct Batch {
     long n[MOST];
     int first[MOST + 1];  // number of an array's first chunk in this launch
     int arrays, chunk;      // values to a chunk
-    double* partial;        // first launch: of its first workgroup
+    double *partial, *other;  // first launch: of its first workgroup (of doubles: their ordinary values; two sums more)
     int partials;           // second launch: all of them
     bool leave;             // second launch: nothing to scale, arrays in their own places stay as they are
     double max_norm;
@@ -74,34 +137,45 @@ __device__ __forceinline__ void walk(const Batch<MOST>& a, int b, F f) {
 
 template <typename T, int MOST>
 __global__ __launch_bounds__(kThreads) void squares(Batch<MOST> a) {
-    __shared__ double scratch[kThreads / 64];
-    double part[Vec<T>::N] = {};
+    __shared__ double scratch[kThreads / 64][Squares<T>::SUMS];
+    Squares<T> part[Vec<T>::N];
     for (int b = blockIdx.x; b < a.first[a.arrays]; b += gridDim.x)
         walk<T>(a, b, [&](int, long, int, int, const T(&v)[Vec<T>::N]) {
 #pragma unroll
-            for (int k = 0; k < Vec<T>::N; ++k) part[k] += (double)v[k] * (double)v[k];
+            for (int k = 0; k < Vec<T>::N; ++k) part[k].add(v[k]);
         });
-    double s = part[0];
 #pragma unroll
-    for (int k = 1; k < Vec<T>::N; ++k) s += part[k];
-    s = block_sum<kThreads>(s, scratch);
-    if (threadIdx.x == 0) a.partial[blockIdx.x] = s;
+    for (int k = 1; k < Vec<T>::N; ++k) part[0].join(part[k]);
+    part[0].template fold<kThreads>(scratch);
+    if (threadIdx.x == 0) {
+        // (a sum below 0 says that the others are there to be read: a third of the bytes for the next launch, all of whose workgroups read them)
+        a.partial[blockIdx.x] = part[0].ordinary() ? part[0].sum[0] : -part[0].sum[0];
+        if constexpr (Squares<T>::SUMS > 1) {
+            a.other[2 * (long)blockIdx.x] = part[0].sum[1];
+            a.other[2 * (long)blockIdx.x + 1] = part[0].sum[2];
+        }
+    }
 }
 
 template <typename T, int MOST, bool PAST>
 __global__ __launch_bounds__(kThreads) void rescale(Batch<MOST> a) {
-    __shared__ double scratch[kThreads / 64];
-    double s = 0;
-    for (int i = threadIdx.x; i < a.partials; i += kThreads) s += a.partial[i];
-    s = sqrt(block_sum<kThreads>(s, scratch));
-    if (a.norm && blockIdx.x == 0 && threadIdx.x == 0) *(T*)a.norm = (T)s;
-    // (in double: where the norm passes the largest float, the scale would lose its digits in one)
-    const double scale = s > a.max_norm && s < (double)INFINITY ? a.max_norm / s : 1.0;
-    a.leave = scale == 1.0;
+    __shared__ double scratch[kThreads / 64][Squares<T>::SUMS];
+    Squares<T> all;
+    for (int i = threadIdx.x; i < a.partials; i += kThreads) {
+        const double mid = a.partial[i];
+        all.sum[0] += fabs(mid);
+        if constexpr (Squares<T>::SUMS > 1)
+            if (signbit(mid)) all.sum[1] += a.other[2 * (long)i], all.sum[2] += a.other[2 * (long)i + 1];
+    }
+    all.template fold<kThreads>(scratch);
+    const double norm = all.norm();
+    if (a.norm && blockIdx.x == 0 && threadIdx.x == 0) *(T*)a.norm = (T)norm;
+    const Scale scale(norm, a.max_norm);
+    a.leave = scale.none;
     for (int b = a.first[a.arrays] - 1 - (int)blockIdx.x; b >= 0; b -= gridDim.x)
         walk<T>(a, b, [&](int i, long begin, int c, int count, T(&v)[Vec<T>::N]) {
 #pragma unroll
-            for (int k = 0; k < Vec<T>::N; ++k) v[k] = (T)((double)v[k] * scale);
+            for (int k = 0; k < Vec<T>::N; ++k) v[k] = scale.of(v[k]);
             if (c < count) store_group<PAST>((T*)a.out[i] + begin, c, count, v);
         });
 }
@@ -149,20 +223,21 @@ __device__ __forceinline__ void walk_units(const FewArrays& a, F f) {
 template <typename T>
 __global__ __launch_bounds__(64 * kWaves) void clip_few(FewArrays a, double max_norm, T* norm) {
     constexpr int N = Vec<T>::N;
-    __shared__ double scratch[kWaves];
-    double s = 0;
+    __shared__ double scratch[kWaves][Squares<T>::SUMS];
+    Squares<T> all;
     walk_units<T>(a, [&](int, int, int, const T(&v)[N]) {
 #pragma unroll
-        for (int k = 0; k < N; ++k) s += (double)v[k] * (double)v[k];
+        for (int k = 0; k < N; ++k) all.add(v[k]);
     });
-    s = sqrt(block_sum<64 * kWaves>(s, scratch));
-    if (threadIdx.x == 0) *norm = (T)s;
-    const double scale = s > max_norm && s < (double)INFINITY ? max_norm / s : 1.0;
+    all.template fold<64 * kWaves>(scratch);
+    const double length = all.norm();
+    if (threadIdx.x == 0) *norm = (T)length;
+    const Scale scale(length, max_norm);
     walk_units<T>(a, [&](int i, int c, int n, T(&v)[N]) {
         T* out = (T*)a.out[i];
-        if (!out || (scale == 1.0 && a.in[i] == out)) return;
+        if (!out || (scale.none && a.in[i] == out)) return;
 #pragma unroll
-        for (int k = 0; k < N; ++k) v[k] = (T)((double)v[k] * scale);
+        for (int k = 0; k < N; ++k) v[k] = scale.of(v[k]);
         store_group(out, c, n, v);
     });
 }
@@ -191,12 +266,12 @@ bool taken_by_one(int count, const void* const* in, void* const* out, const int6
 template <typename T, int MOST>
 int clip_batches(int count, const void* const* in, void* const* out, const int64_t* sizes, double max_norm, T* norm) {
     const Carried carried;
-    double* partial = (double*)carried.data();
+    double *partial = (double*)carried.data(), *other = partial + kOther;
     long total = 0;
     for (int i = 0; i < count; ++i) total += sizes[i];
     constexpr int STEP = kThreads * Vec<T>::N * kUnroll;
     const int chunk = STEP;  // (of two, four, eight steps: 52 million values 103, 105, 113 us, this way 104; 4 million 12.6, 13.8, 18.5 and 13.1; 45 thousand 12.2, 12.6, 13.9 and 11.0)
-    const int batches = (count + MOST - 1) / MOST, most = std::max(kPartials / std::max(batches, 1), 16);
+    const int batches = (count + MOST - 1) / MOST, most = std::max(kPartials / std::max(batches, 1), kLeast);
     Batch<MOST> b;
     b.chunk = chunk;
     b.leave = false;
@@ -227,10 +302,12 @@ int clip_batches(int count, const void* const* in, void* const* out, const int64
     each([&](int chunks) {
         const int blocks = std::min(chunks, most);
         b.partial = partial + partials;
+        b.other = other + 2 * partials;
         hipLaunchKernelGGL((squares<T, MOST>), dim3(blocks), dim3(kThreads), 0, stream(), b);
         partials += blocks;
     });
     b.partial = partial;
+    b.other = other;
     b.partials = partials;
     b.norm = norm;
     if (out)
@@ -271,7 +348,7 @@ extern "C" int dali_hip_clip_by_global_norm(int dtype, int count, const void* co
     const size_t size = dtype == DALI_HIP_FLOAT ? 4 : 8;
     for (int i = 0; i < count; ++i)
         if (sizes[i] < 0 || (sizes[i] > 0 && (!in[i] || (out && !out[i])))) return fail("%s: array %d has no memory or a negative size", what, i);
-    // (partial sums: kPartials, or 16 for every launch of kBatch arrays; chunks are numbered in 31 bits)
+    // (partial sums: of kPartials workgroups, or of kLeast for every launch of kBatch arrays; chunks are numbered in 31 bits)
     if (count > kMostArrays) return fail("%s: %d arrays are more than there is room for", what, count);
     for (int i = 0; i < count; ++i)
         if (off_elements({in[i], out ? out[i] : nullptr, norm}, size)) return fail("%s: an address is off its type's size", what);

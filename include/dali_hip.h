@@ -383,8 +383,9 @@ int dali_hip_token_log_probs_backward(int dtype, int64_t rows, int vocab, const 
 
 /* ------------------------------------------------------------- the norm of many arrays */
 /*
- * *norm = sqrt(sum of the squares of all values of `count` arrays of sizes[i] values each), summed in double whatever the type; with `out`, out[i] = in[i] * min(1,
- * max_norm / norm). out[i] may be in[i]; other overlaps are refused. Where the norm is not finite nothing is scaled. in, out and sizes are host arrays, read before the
+ * *norm = sqrt(sum of the squares of all values of `count` arrays of sizes[i] values each), summed in double whatever the type, also where the squares of doubles are no
+ * doubles; with `out`, out[i] = in[i] * min(1, max_norm / norm). out[i] may be in[i]; other overlaps are refused. Where the norm is not finite in double nothing is
+ * scaled (one of fp32 arrays that passes the largest float is reported as infinite and scales by what it is). in, out and sizes are host arrays, read before the
  * call returns; norm is a device scalar of the arrays' type.
  */
 int dali_hip_clip_by_global_norm(int dtype, int count, const void* const* in, void* const* out, const int64_t* sizes, double max_norm, void* norm);
