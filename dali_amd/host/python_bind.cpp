@@ -422,8 +422,13 @@ struct Destinations {
     }
 };
 
-// an operand that may be None
-bool optional(Operand& a, PyObject* o) { return o == Py_None || a.set(o); }
+// an operand that may be None (an array without a handle is not: it would be taken for none)
+bool optional(Operand& a, PyObject* o) {
+    if (o == Py_None) return true;
+    if (!a.set(o)) return false;
+    if (!a.handle) PyErr_SetString(PyExc_TypeError, "an operand is an Array without a handle");
+    return a.handle != nullptr;
+}
 
 bool number(PyObject* o, double* v) {
     *v = PyFloat_AsDouble(o);

@@ -105,3 +105,20 @@ def test_entries_of_the_library(D):
     refused(hip.dali_hip_clip_by_global_norm(0, 1, pointers, None, (C.c_int64 * 1)(3), 1.0, None), "NULL")
     assert hip.dali_hip_layer_norm(0, 0, 4, None, 4, None, None, 1e-5, None, None, None) == 0  # nothing to do
     assert hip.dali_hip_token_log_probs(0, 0, 4, None, 4, None, 0, None, None, None, None, None) == 0
+
+
+def test_operands_without_a_handle(D):
+    """An array whose handle was given up is no absent weight."""
+    op = D.op
+    x, per_row, vector, tokens, double, whole = arrays(D)
+    gone = D.Array.from_numpy(np.zeros(6, np.float32))
+    handle, gone._h = gone._h, None
+    try:
+        for call in (lambda: op.layer_norm(x, gone), lambda: op.layer_norm(x, vector, gone), lambda: op.layer_norm_backward(x, x, per_row, per_row, gone),
+                     lambda: op.token_log_probs_backward(per_row, gone, x, tokens, per_row, None), lambda: op.token_log_probs_backward(per_row, per_row, x, tokens, per_row, gone)):
+            with pytest.raises(TypeError, match="without a handle"):
+                call()
+        with pytest.raises(D.DaliError, match="NULL array handle"):
+            op.layer_norm(gone)
+    finally:
+        gone._h = handle
