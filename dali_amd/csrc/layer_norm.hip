@@ -623,7 +623,7 @@ extern "C" int dali_hip_layer_norm(int dtype, int64_t rows, int width, const voi
     const char* what = "dali_hip_layer_norm";
     if (!is_real(dtype)) return fail("%s: dtype %d is neither float nor double", what, dtype);
     if (rows < 0 || width < 1) return fail("%s: %lld rows of %d values", what, (long long)rows, width);
-    if (!(epsilon >= 0) || epsilon > 1e30) return fail("%s: epsilon must be a number that is not negative (got %g)", what, epsilon);
+    if (!(epsilon >= 0) || epsilon > 1e30) return fail("%s: epsilon must be from 0 to 1e30 (got %g)", what, epsilon);
     if (rows == 0) return DALI_HIP_OK;
     if (!x || !y || !mean || !rstd) return fail("%s: NULL argument", what);
     const size_t size = dtype == DALI_HIP_FLOAT ? 4 : 8;

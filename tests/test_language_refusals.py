@@ -122,3 +122,13 @@ def test_operands_without_a_handle(D):
             op.layer_norm(gone)
     finally:
         gone._h = handle
+
+
+@pytest.mark.parametrize("epsilon", [-1e-5, -np.inf, np.nan, 2e30, np.inf])
+def test_epsilon(D, epsilon):
+    from dali_amd._native import hip
+    host = (C.c_double * 64)()
+    at = lambda i: C.c_void_p(C.addressof(host) + 8 * i)  # noqa: E731
+    for dtype in (0, 1):
+        assert hip.dali_hip_layer_norm(dtype, 1, 4, at(0), 4, None, None, epsilon, at(8), at(16), at(17)) != 0
+        assert "epsilon must be from 0 to 1e30" in hip.dali_hip_last_error().decode()
