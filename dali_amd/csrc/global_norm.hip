@@ -265,6 +265,7 @@ bool taken_by_one(int count, const void* const* in, void* const* out, const int6
 
 template <typename T, int MOST>
 int clip_batches(int count, const void* const* in, void* const* out, const int64_t* sizes, double max_norm, T* norm) {
+    const char* what = "dali_hip_clip_by_global_norm";
     const Carried carried;
     double *partial = (double*)carried.data(), *other = partial + kOther;
     long total = 0;
@@ -295,33 +296,37 @@ int clip_batches(int count, const void* const* in, void* const* out, const int64
                 }
                 filled = true;
             }
-            if (b.arrays) launch(b.first[b.arrays]);
+            if (!b.arrays) continue;
+            launch(b.first[b.arrays]);
+            if (launched(what)) return false;  // (and nothing is scaled by a norm that was not formed)
         }
+        return true;
     };
     int partials = 0;
-    each([&](int chunks) {
+    const bool summed = each([&](int chunks) {
         const int blocks = std::min(chunks, most);
         b.partial = partial + partials;
         b.other = other + 2 * partials;
         hipLaunchKernelGGL((squares<T, MOST>), dim3(blocks), dim3(kThreads), 0, stream(), b);
         partials += blocks;
     });
+    if (!summed) return DALI_HIP_ERROR;
     b.partial = partial;
     b.other = other;
     b.partials = partials;
     b.norm = norm;
-    if (out)
-        each([&](int chunks) {
+    if (out && !each([&](int chunks) {
             either_way(past_caches(2.0 * sizeof(T) * total),
                        [&](auto p) { hipLaunchKernelGGL((rescale<T, MOST, decltype(p)::value>), dim3(std::min(chunks, 2048)), dim3(kThreads), 0, stream(), b); });
             b.norm = nullptr;
-        });
+        }))
+        return DALI_HIP_ERROR;
     if (b.norm) {  // the norm alone, or nothing to scale
         b.arrays = 0;
         b.first[0] = 0;
         hipLaunchKernelGGL((rescale<T, MOST, false>), dim3(1), dim3(kThreads), 0, stream(), b);
     }
-    return launched("dali_hip_clip_by_global_norm");
+    return launched(what);
 }
 
 template <typename T>

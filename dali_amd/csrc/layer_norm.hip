@@ -568,6 +568,7 @@ int forward(NormArgs<T> a) {
 
 template <typename T>
 int backward(NormBackwardArgs<T> a) {
+    const char* what = "dali_hip_layer_norm_backward";
     const bool past = past_caches(3.0 * sizeof(T) * a.rows * a.width);
     const long fit = (long)(kCarriedBytes / (2 * sizeof(T) * (size_t)a.width));  // rows of partial sums that there is room for
     const Carried carried;  // (to the launch that folds them)
@@ -575,7 +576,7 @@ int backward(NormBackwardArgs<T> a) {
     a.parts = 1;
     if (a.rows == 0) {
         if (a.dgamma) hipLaunchKernelGGL(norm_weights<T>, dim3((unsigned)(((long)a.width + kThreads - 1) / kThreads)), dim3(kThreads), 0, stream(), a);
-        return launched("dali_hip_layer_norm_backward");
+        return launched(what);
     }
     const bool held = team_for<4096>(groups_of<T>(a.width), [&](auto team, auto e) {
         constexpr int TEAM = decltype(team)::value, E = decltype(e)::value;
@@ -607,10 +608,12 @@ int backward(NormBackwardArgs<T> a) {
         a.parts = (int)std::max(1L, std::min({64L, a.rows, fit}));
         hipLaunchKernelGGL(norm_weights<T>, dim3((unsigned)(((long)a.width + kThreads - 1) / kThreads), a.parts), dim3(kThreads), 0, stream(), a);
     }
+    if (launched(what)) return DALI_HIP_ERROR;
     if (a.dgamma && a.parts > 1) hipLaunchKernelGGL(norm_fold<T>, dim3((unsigned)((2L * a.width + 15) / 16)), dim3(kThreads), 0, stream(), a);
+    if (launched(what)) return DALI_HIP_ERROR;
     if (!held)
         either_way(past, [&](auto p) { hipLaunchKernelGGL((norm_backward_rows<T, decltype(p)::value>), dim3((unsigned)std::min(a.rows, 65536L)), dim3(1024), 0, stream(), a); });
-    return launched("dali_hip_layer_norm_backward");
+    return launched(what);
 }
 
 }  // namespace

@@ -174,7 +174,7 @@ int main(int argc, char** argv) {
         const long rows = std::atol(argv[4]);
         if (argc > 7) g_fail_at = std::atoi(argv[7]);
         const int status = op == "log_probs" ? log_probs(dtype, rows, extent, std::atoi(argv[6])) : op == "log_probs_backward" ? log_probs_backward(dtype, rows, extent) :
-                           op == "norm" ? norm(dtype, rows, extent) : norm_backward(dtype, rows, extent);
+                           op == "clip" ? clip(dtype, std::vector<int64_t>(rows, extent)) : op == "norm" ? norm(dtype, rows, extent) : norm_backward(dtype, rows, extent);
         report(op.c_str(), status);
     } else if (what == "threads") {  // the kernel whose launch waits
         g_pause_at = argv[2];

@@ -46,6 +46,16 @@ def test_a_failed_launch_is_the_last(recorder, op, extent):
         assert int(status) != 0 and int(launches) == failing + 1
 
 
+@pytest.mark.parametrize("op,rows,extent", [("clip", 3, 100000), ("clip", 300, 100000), ("norm_backward", 5000, 1024), ("norm_backward", 5000, 40000)])
+@pytest.mark.parametrize("dtype", [0, 1])
+def test_nothing_is_made_of_partial_sums_that_no_launch_left(recorder, op, rows, extent, dtype):
+    (_, status, launches, _, _), = recorder("one", op, dtype, rows, extent, 0)
+    assert int(status) == 0 and int(launches) > 1
+    for failing in range(int(launches)):
+        (_, status, made, _, _), = recorder("one", op, dtype, rows, extent, 0, failing)
+        assert int(status) != 0 and int(made) == failing + 1
+
+
 def test_two_threads_do_not_part_what_belongs_together(recorder):
     """The partial sums that one launch leaves are read by the next: what another thread launches between the two must not be such a pair's half."""
     assert [k for k, in recorder("threads", "squares")] == ["squares", "rescale", "norm_backward_team", "norm_fold"]
