@@ -367,7 +367,8 @@ int dali_hip_layer_norm_backward(int dtype, int64_t rows, int width, const void*
 /* ------------------------------------------------------------- log probabilities of tokens */
 #define DALI_HIP_MAX_ALTERNATIVES 64
 /*
- * Per row of logits [rows, vocab] (rows `stride` values apart): lse = ln sum e^x, log_probs = x[token] - lse, entropy = -sum p ln p with p = e^(x - lse),
+ * Per row of logits [rows, vocab] (rows `stride` values apart): lse = ln sum e^x = m + ln S with the maximum m and S = sum e^(x - m), log_probs = (x[token] - m) - ln S
+ * (which the size of the logits costs no digits; lse is rounded to its own), entropy = -sum p ln p with p = e^(x - lse),
  * and the k best entries as top_tokens [rows, k] (lower position first among equals) with their log probabilities top_log_probs [rows, k]; k = 0: none, at most
  * DALI_HIP_MAX_ALTERNATIVES. A logit of -inf has probability 0. A row of -inf alone: lse and log_probs -inf, entropy 0. A NaN or +inf makes the row's
  * values NaN (among the alternatives a NaN ranks as -inf). A token outside [0, vocab) stands for none: log_probs 0. Destinations must not overlap anything.
@@ -376,7 +377,8 @@ int dali_hip_token_log_probs(int dtype, int64_t rows, int vocab, const void* log
                              void* top_log_probs, int32_t* top_tokens);
 /*
  * The gradient of both: d_logits = d_log_probs (delta_token - p) - d_entropy p (ln p + entropy), from the lse and entropy of the forward pass. d_entropy may be NULL (entropy
- * is not read then). d_logits [rows, vocab] is dense and may be the logits themselves. Rows of -inf alone get zeros, a token outside [0, vocab) no gradient through it.
+ * is not read then). p is e^(x - lse) with lse as it was rounded: its relative error holds half a unit in the last place of lse, 1e-3 for fp32 logits near 30000. d_logits
+ * [rows, vocab] is dense and may be the logits themselves. Rows of -inf alone get zeros, a token outside [0, vocab) no gradient through it.
  */
 int dali_hip_token_log_probs_backward(int dtype, int64_t rows, int vocab, const void* d_log_probs, const void* d_entropy, const void* logits, int64_t stride,
                                       const int32_t* tokens, const void* lse, const void* entropy, void* d_logits);
