@@ -10,6 +10,7 @@
 // Bound by memory: 52 million fp32 values in 24 arrays 103 us, 38 for the norm (5.4 TB/s) and 64 to 68 for the scaling (6.3 TB/s read and written, half of the reading from
 // the cache); 45 thousand in 12 arrays 11 us, where two launches and the host are all there is.
 #include <algorithm>
+#include <new>
 #include <vector>
 
 #include "row_math.h"
@@ -340,13 +341,7 @@ int clip(int count, const void* const* in, void* const* out, const int64_t* size
     return clip_batches<T, kBatch>(count, in, out, sizes, max_norm, norm);
 }
 
-}  // namespace
-}  // namespace dali_hip
-
-using namespace dali_hip;
-
-extern "C" int dali_hip_clip_by_global_norm(int dtype, int count, const void* const* in, void* const* out, const int64_t* sizes, double max_norm, void* norm) {
-    const char* what = "dali_hip_clip_by_global_norm";
+int checked(const char* what, int dtype, int count, const void* const* in, void* const* out, const int64_t* sizes, double max_norm, void* norm) {
     if (!is_real(dtype)) return fail("%s: dtype %d is neither float nor double", what, dtype);
     if (count < 0 || !norm || (count > 0 && (!in || !sizes))) return fail("%s: NULL argument", what);
     if (out && !(max_norm >= 0)) return fail("%s: the largest norm must not be negative (got %g)", what, max_norm);
@@ -389,4 +384,18 @@ extern "C" int dali_hip_clip_by_global_norm(int dtype, int count, const void* co
     if (ensure_init()) return DALI_HIP_ERROR;
     if (dtype == DALI_HIP_FLOAT) return clip<float>(count, in, out, sizes, max_norm, (float*)norm);
     return clip<double>(count, in, out, sizes, max_norm, (double*)norm);
+}
+
+}  // namespace
+}  // namespace dali_hip
+
+using namespace dali_hip;
+
+extern "C" int dali_hip_clip_by_global_norm(int dtype, int count, const void* const* in, void* const* out, const int64_t* sizes, double max_norm, void* norm) {
+    const char* what = "dali_hip_clip_by_global_norm";
+    try {
+        return checked(what, dtype, count, in, out, sizes, max_norm, norm);
+    } catch (const std::bad_alloc&) {  // (the list of results)
+        return fail("%s: no host memory for %d arrays", what, count);
+    }
 }

@@ -1,6 +1,7 @@
 // Runs entry points of the library on a machine without a device: the runtime's calls that they make are answered here (a program's own definitions come before
 // those of the libraries that it loads), launches are written down and launch nothing. What is printed is checked by test_language_launches.py.
 #include <hip/hip_runtime_api.h>
+#include <sys/resource.h>
 
 #include <atomic>
 #include <chrono>
@@ -189,6 +190,18 @@ int main(int argc, char** argv) {
         for (const Launch& l : g_launches)
             for (const char* k : {"graph_begins", "graph_ends", "squares", "rescale", "norm_backward_team", "norm_weights", "norm_fold"})
                 if (l.kernel.find(k) != std::string::npos) std::printf("%s\n", k);
+    } else if (what == "memory") {  // many arrays, and then no memory for what the call notes about them
+        if (dali_hip_init(0)) return 1;
+        const size_t count = 1 << 23;
+        std::vector<const void*> in(count, at(1));
+        std::vector<void*> out(count, at(2));
+        const std::vector<int64_t> sizes(count, 0);
+        rlimit limit;
+        getrlimit(RLIMIT_AS, &limit);
+        limit.rlim_cur = 64 << 20;  // (less than is in use: nothing more is given)
+        if (setrlimit(RLIMIT_AS, &limit)) return 1;
+        const int status = dali_hip_clip_by_global_norm(0, (int)count, in.data(), out.data(), sizes.data(), 1.0, at(3));
+        std::printf("%d %s\n", status, dali_hip_last_error());
     } else if (what == "places") {
         if (dali_hip_init(0)) return 1;
         // (searched: what the launches' arguments hold at least)

@@ -56,6 +56,12 @@ def test_nothing_is_made_of_partial_sums_that_no_launch_left(recorder, op, rows,
         assert int(status) != 0 and int(made) == failing + 1
 
 
+def test_a_call_without_memory_for_its_notes_fails(recorder):
+    """An exception does not leave an entry of the library."""
+    (status, *message), = recorder("memory")
+    assert int(status) != 0 and "memory" in message
+
+
 def test_two_threads_do_not_part_what_belongs_together(recorder):
     """The partial sums that one launch leaves are read by the next: what another thread launches between the two must not be such a pair's half."""
     assert [k for k, in recorder("threads", "squares")] == ["squares", "rescale", "norm_backward_team", "norm_fold"]
