@@ -134,7 +134,7 @@ __device__ __forceinline__ void norm_marked(const NormArgs<T>& a, Scratch& scrat
 }
 
 // A team of TEAM threads per row, which lives in their registers, E groups of 16 bytes to a thread: read once, written once, which bounds it. WHOLE: the teams' groups are
-// the row exactly. The weights stay in registers from row to row where they fit. 8192x1024 11.5 us (5.8 TB/s), 65536x1024 89 us (6.0), 32768x4096 187 us (5.7); 8x1024 4.4 us
+// the row exactly. The weights stay in registers from row to row where they fit. 8192x1024 11.6 us (5.8 TB/s), 65536x1024 89 us (6.0), 32768x4096 183 us (5.9); 8x1024 4.2 us
 // among others, 2.9 of them on the device.
 // (the bound on waves: of 3001x2047 in double 18.4 us, without it 19.5; of 32768x2999 in float 150, without it 141)
 template <typename T, int TEAM, int E, bool WHOLE, bool PAST>
@@ -316,7 +316,7 @@ __device__ __forceinline__ T plus_across(T v) {
 
 // The gradient with the rows in registers as above; a thread also keeps the sums of its columns over all rows that its team takes. At the end the teams of a
 // workgroup are joined, lanes first and then waves through LDS, in halves, and the workgroup leaves one row of partial sums for each weight. So x and dy are read once for all
-// three gradients. Bound by memory: 32768x4096 280 us (5.7 TB/s), 65536x1024 148 us (5.4); 8192x1024 22.3 us, of which 18 to 20 are this launch (a wave has two rows) and 2
+// three gradients. Bound by memory: 32768x4096 280 us (5.7 TB/s), 65536x1024 148 us (5.4); 8192x1024 22.3 us, of which 18 to 20 are this launch (a wave has four rows) and 2
 // to 4 the fold; 3001x2047 in double 36 us. The next row is asked for before this one is worked on (8192x1024 24.2 without, 65536x1024 154).
 template <typename T, int TEAM, int TEAMS, int E, bool WHOLE, bool WEIGHTS, bool PAST>
 __global__ __launch_bounds__(TEAM * TEAMS) void norm_backward_team(NormBackwardArgs<T> a) {

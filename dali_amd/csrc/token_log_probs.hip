@@ -4,6 +4,7 @@
 //   lse = m + ln S,  log p(t) = x_t - lse,  entropy = -sum p ln p = ln S - T / S
 //   d x = d log p(t) (delta_t - p) - d entropy p (ln p + entropy)
 //
+// Log probabilities are written as (x - m) - ln S, which keeps the digits of rows far from 0; p of the gradient is e^(x - lse) with lse as it was rounded.
 // A value of -inf (or far below m) has weight 0 and adds nothing to the entropy. A row of -inf alone has lse = -inf, entropy 0 and no gradient.
 // A NaN or +inf makes its row's results NaN. A token outside [0, vocab) stands for none: its log probability is 0 and has no gradient.
 #include <algorithm>
@@ -647,7 +648,7 @@ __global__ __launch_bounds__(kThreads) void log_prob_long(LogProbArgs<T> a) {
 }
 
 // Segments that a workgroup holds in registers, E groups to a thread: all of them are loaded at once and nothing is read again. 65536x3000 128 us (6.2 TB/s), with 5
-// alternatives 187; 32768x8000 170 and 181 us. A single row of 50257 in 25 segments takes 7.0 us with 5 alternatives and 10.1 with 20, 4.6 without: a chain of one reading,
+// alternatives 187; 32768x8000 170 and 181 us. A single row of 50257 in 24 segments takes 7.0 us with 5 alternatives and 10.2 with 20, 4.6 without: a chain of one reading,
 // the folds, the bound, two trips to memory for what the segments found and its ranking.
 template <typename T, bool TOP, int E>
 __global__ __launch_bounds__(kThreads) void log_prob_segments(LogProbArgs<T> a) {
@@ -732,7 +733,7 @@ struct RowGradient {
     }
 };
 
-// The gradient is a map once a row's lse is known: one reading, one writing, bound by memory. LANES lanes to a row: 51200x97 9.5 us (4.3 TB/s, an odd length costs lanes
+// The gradient is a map once a row's lse is known: one reading, one writing, bound by memory. LANES lanes to a row: 51200x97 9.2 us (4.3 TB/s, an odd length costs lanes
 // and whole lines), 65536x613 57 us (5.7 TB/s)
 template <typename T, int LANES, int E, bool PAST>
 __global__ __launch_bounds__(kThreads) void log_prob_backward_short(LogProbBackwardArgs<T> a) {
@@ -830,7 +831,7 @@ int forward(LogProbArgs<T> all) {
             if (launched(what)) return DALI_HIP_ERROR;
             continue;
         }
-        // Few long rows are cut into segments of at least 512 groups, two for a thread, 512 workgroups or so together. The segments' alternatives are joined in one list,
+        // Few long rows are cut into segments of at least 512 groups, two or three for a thread, 512 workgroups or so together. The segments' alternatives are joined in one list,
         // and a lane of one wave stands for a segment. Cut and whole, with 5 alternatives (us): 8x32000 7.3 and 9.1, 64x32000 8.1 and 9.1, 130x32000 10.8 and 9.1, 100x8000
         // 7.7 and 6.3, 130x100000 15.2 and 16.9, 250x200000 42.2 and 45.9.
         const bool cuts = (a.rows <= 128 && groups >= 4096) || (a.rows <= 256 && groups >= 16384);
