@@ -82,7 +82,7 @@ struct Scale {
     __device__ __forceinline__ Scale(double norm, double max_norm) : none(!(norm > max_norm && norm < (double)INFINITY)) {
         if (none) return;
         second = max_norm / norm;
-        if (second < 0x1p-1000) first = 0x1p-600, second = max_norm / (norm * 0x1p-600);
+        if (second < 0x1p-1000 && max_norm > 0) first = 0x1p-600, second = max_norm / (norm * 0x1p-600);  // (the norm is above 2^-74 then)
     }
     __device__ __forceinline__ float of(float v) const { return (float)((double)v * second); }  // (a second factor below 2^-1000 leaves nothing of a float)
     __device__ __forceinline__ double of(double v) const { return (v * first) * second; }

@@ -54,3 +54,13 @@ def test_a_norm_of_doubles_that_is_not_finite(gpu, D, rng, value, n):
     arrays = [np.full(n, 1.7e308), np.full(17, 1.0)]
     got, got_norm = D.op.clip_by_global_norm([D.Array.from_numpy(a) for a in arrays], 0.1)
     assert np.isinf(got_norm.numpy()) and all(np.array_equal(g.numpy(), a) for g, a in zip(got, arrays))
+
+
+@pytest.mark.parametrize("n", [1, 7, 3000, 300000])
+@pytest.mark.parametrize("dtype", [np.float32, np.float64])
+def test_a_largest_norm_of_0(gpu, D, rng, n, dtype):
+    """Everything is scaled to 0, however small it is."""
+    for size in {np.float32: [1.0, 1e-44, 1e38], np.float64: [1.0, 1e-150, 1e-200, 1e-320, 1e300]}[dtype]:
+        a = np.abs(rng.randn(n)) + 1
+        got, norm = D.op.clip_by_global_norm([D.Array.from_numpy((a / a.max() * size).astype(dtype))], 0.0)
+        assert norm.numpy() > 0 and not got[0].numpy().any()
