@@ -8,7 +8,7 @@
 // second launch has been issued: Carried, runtime.h.) The second launch walks the chunks backwards: what the first read last is still in the cache. A norm that is not
 // finite scales nothing: the arrays come back as they are and the norm says so, and arrays that are their own destinations are left alone whenever nothing is scaled.
 // Bound by memory: 52 million fp32 values in 24 arrays 103 us, 38 for the norm (5.4 TB/s) and 64 to 68 for the scaling (6.3 TB/s read and written, half of the reading from
-// the cache), in double 217 (5.8 TB/s read twice and written); 45 thousand in 12 arrays 11.8 us, where two launches and the host are all there is.
+// the cache), in double 213 (5.9 TB/s read twice and written); 45 thousand in 12 arrays 11.8 us, where two launches and the host are all there is.
 #include <algorithm>
 #include <new>
 #include <vector>
@@ -60,7 +60,8 @@ struct Squares {
     template <int THREADS>
     __device__ __forceinline__ void fold(double (&scratch)[THREADS / 64][SUMS]) {
 #pragma unroll
-        for (int i = 0; i < SUMS; ++i) sum[i] = fold_lanes<64>(sum[i], Sum());
+        for (int i = 0; i < SUMS; ++i)
+            if (i == 0 || __builtin_amdgcn_ballot_w64(sum[i] != 0) != 0) sum[i] = fold_lanes<64>(sum[i], Sum());  // (seldom)
         if ((threadIdx.x & 63) == 0)
 #pragma unroll
             for (int i = 0; i < SUMS; ++i) scratch[threadIdx.x >> 6][i] = sum[i];
