@@ -113,6 +113,15 @@ HIP_SYMBOLS = {
     "dali_hip_layer_norm_backward": (_i, [_i, C.c_int64, _i, H, C.c_int64, H, C.c_int64, H, H, H, H, H, H]),
     "dali_hip_token_log_probs": (_i, [_i, C.c_int64, _i, H, C.c_int64, H, _i, H, H, H, H, H]),
     "dali_hip_token_log_probs_backward": (_i, [_i, C.c_int64, _i, H, H, H, C.c_int64, H, H, H, H]),
+    "dali_hip_embedding": (_i, [_i, C.c_int64, _i, _i, H, C.c_int64, H, C.c_double, H]),
+    "dali_hip_embedding_backward_workspace": (_i, [_i, C.c_int64, _i, _i, C.POINTER(C.c_size_t)]),
+    "dali_hip_embedding_backward": (_i, [_i, C.c_int64, _i, _i, H, C.c_int64, H, C.c_double, H, H]),
+    "dali_hip_cross_attention_workspace": (_i, [_i] * 8 + [C.POINTER(C.c_size_t)]),
+    "dali_hip_cross_attention": (_i, [_i] * 7 + [H, C.POINTER(C.c_int64)] * 3 + [H, C.c_double, H, H, H]),
+    "dali_hip_cross_attention_backward": (_i, [_i] * 7 + [H, C.POINTER(C.c_int64)] * 4 + [H, H, H, C.c_double, H, H, H, H]),
+    "dali_hip_projected_cross_entropy_workspace": (_i, [_i, C.c_int64, _i, _i, _i, _i, C.POINTER(C.c_size_t)]),
+    "dali_hip_projected_cross_entropy": (_i, [_i, C.c_int64, _i, _i, H, C.c_int64, H, C.c_int64, _i, H, H, H, H, H]),
+    "dali_hip_projected_cross_entropy_backward": (_i, [_i, C.c_int64, _i, _i, H, H, C.c_int64, H, C.c_int64, _i, H, H, H, H, H, _i, H, H]),
     "dali_hip_clip_by_global_norm": (_i, [_i, _i, C.POINTER(H), C.POINTER(H), C.POINTER(C.c_int64), C.c_double, H]),
     "dali_hip_capture_begin": (_i, []),
     "dali_hip_capture_end": (_i, [C.POINTER(H)]),
@@ -207,6 +216,12 @@ FRONT_SYMBOLS = {
     "dali_fe_token_log_probs": (_i, [H, H, _i, _HP, _HP, _HP, _HP, _HP]),
     "dali_fe_token_log_probs_backward": (_i, [H, H, H, H, H, H, _HP]),
     "dali_fe_clip_by_global_norm": (_i, [_HP, _i, C.c_double, _HP, _HP]),
+    "dali_fe_embedding": (_i, [H, H, C.c_double, _HP]),
+    "dali_fe_embedding_backward": (_i, [H, H, _i, C.c_double, _HP]),
+    "dali_fe_cross_attention": (_i, [H, H, H, H, C.c_double, _HP, _HP]),
+    "dali_fe_cross_attention_backward": (_i, [H, H, H, H, H, H, H, C.c_double, _HP, _HP, _HP]),
+    "dali_fe_projected_cross_entropy": (_i, [H, H, H, H, _HP, _HP]),
+    "dali_fe_projected_cross_entropy_backward": (_i, [H, H, H, H, H, H, _HP, _HP, _HP]),
     "dali_fe_eval": (_i, [H]),
     "dali_fe_eval_together": (_i, [_HP, _i]),
     "dali_fe_assign": (_i, [H, _i, H]),

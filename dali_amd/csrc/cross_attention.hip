@@ -1,0 +1,996 @@
+// Attention of a decoder's positions to an encoder's states, and its gradients. Beyond the reference.
+//
+// q [batch, queries, heads, width]; k, v [batch, keys, kv_heads, width]; head h looks at the states of kv head h / (heads / kv_heads); sequence b has counts[b] states,
+// what lies behind them is not read. s = scale q.k, lse = ln sum e^s, p = e^(s - lse), y = sum p v. With delta = dy.y: ds = p (dy.v - delta), dq = scale sum ds k,
+// dk = scale sum ds q, dv = sum p dy. The scores are never kept: they are formed tile by tile beside a running maximum and sum, and again on the way back.
+//
+// The positions of all heads that share a kv head are the rows of one problem, whose states are read once for all of them: row r is position r / group of head r % group.
+//
+// Everything is formed transposed, states by rows: a 16x16 tile of s comes out of the matrix instruction with one row of the problem to a lane (lane % 16) and four
+// states to its registers, which is what the next product takes as its right operand if its inner extent is walked in the order (register, lane / 16). So
+// the weights never leave their registers, a lane's running maximum, sum and rescaling are of one row, and maxima over the states are folded over two
+// exchanges of half rows. The left operands are tiles of states in LDS, read 16 bytes at a time both along a state (for s) and across states (for y).
+#include <algorithm>
+#include <cmath>
+
+#include "row_math.h"
+
+namespace dali_hip {
+namespace {
+
+typedef float floatx4 __attribute__((ext_vector_type(4)));
+typedef double doublex4 __attribute__((ext_vector_type(4)));
+
+// The 16x16x4 matrix instruction: lane l holds a[l % 16][l / 16] and b[l / 16][l % 16], and of the result column l % 16, rows row_of(0..3, l / 16).
+// Exponents are those of 2 in fp32 (the instruction's base) and of e in fp64.
+template <typename T>
+struct Matrix;
+template <>
+struct Matrix<float> {
+    typedef floatx4 acc;
+    static constexpr float lowest = -3.402823466e+38f;
+    static constexpr double base = 1.4426950408889634074;  // exponents are counted in powers of 2
+    static __device__ __forceinline__ int row_of(int v, int g) { return 4 * g + v; }
+    static __device__ __forceinline__ acc mul(float a, float b, acc c) { return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0); }
+    static __device__ __forceinline__ float weight(float d) { return __builtin_amdgcn_exp2f(d); }
+    static __device__ __forceinline__ float lse(float top, float sum) { return (top + log2f(sum)) * 0.693147180559945309f; }
+};
+template <>
+struct Matrix<double> {
+    typedef doublex4 acc;
+    static constexpr double lowest = -1.7976931348623157e+308;
+    static constexpr double base = 1.0;
+    static __device__ __forceinline__ int row_of(int v, int g) { return 4 * v + g; }
+    static __device__ __forceinline__ acc mul(double a, double b, acc c) { return __builtin_amdgcn_mfma_f64_16x16x4f64(a, b, c, 0, 0, 0); }
+    static __device__ __forceinline__ double weight(double d) { return exp(d); }
+    static __device__ __forceinline__ double lse(double top, double sum) { return top + log(sum); }
+};
+
+struct Operand {
+    const void* p;
+    int64_t batch, row, head;  // strides in values
+};
+
+struct Args {
+    int batch, queries, keys, heads, kv_heads, width, group, rows;  // group: heads that share a kv head; rows: queries * group
+    Operand q, k, v, dy;
+    const int32_t* counts;
+    const void *y, *lse;  // dense
+    double scale;
+    void *y_out, *lse_out, *dq, *dk, *dv;  // dense
+    void* delta;                            // [batch, queries, heads]
+    // results of parts of the states (or rows): [part][problem][row][D], and maxima and sums [part][problem][row]
+    void *parts_y, *parts_m, *parts_l;
+    int parts, tiles;
+    int first;  // problem of a launch's first workgroup
+};
+
+// Rows that neighbouring heads share: row r lies at position r / group of head r % group
+struct Rows {
+    int64_t row, head;
+    int group;
+    __device__ __forceinline__ int64_t at(int r) const {
+        if (group == 1) return r * row;
+        const int t = r / group;
+        return t * row + (r - t * group) * head;
+    }
+};
+
+__device__ __forceinline__ int count_of(const Args& a, int b) { return a.counts ? max(0, min(a.counts[b], a.keys)) : a.keys; }
+
+// neighbouring workgroups, which share operands, run on the same die (every eighth one does)
+__device__ __forceinline__ int on_die(int id, int total) {
+    const int per = total >> 3;
+    return id < per * 8 ? (id & 7) * per + (id >> 3) : id;
+}
+
+// A group of values of a row, zeros past the row's end
+template <int D, typename T>
+__device__ __forceinline__ typename Vec<T>::type row_group(const T* row, int c, int width) {
+    if (width == D) return *reinterpret_cast<const typename Vec<T>::type*>(row + c);
+    T v[Vec<T>::N];
+    typename Vec<T>::type g = {};
+    if (c < width) {
+        load_group(row, c, width, T(0), v);
+#pragma unroll
+        for (int i = 0; i < Vec<T>::N; ++i) g[i] = v[i];
+    }
+    return g;
+}
+
+// What a lane holds of 16 rows as a right operand: row lane % 16, groups lane / 16 of every four
+template <typename T, int D>
+struct Fragment {
+    static constexpr int N = Vec<T>::N, C = D / (4 * N);
+    typename Vec<T>::type g[C];
+    __device__ __forceinline__ void load(const T* row, int width, T factor) {
+        const int lane = threadIdx.x & 63;
+#pragma unroll
+        for (int c = 0; c < C; ++c) g[c] = row_group<D>(row, (4 * c + (lane >> 4)) * N, width) * factor;
+    }
+};
+
+// A tile of R rows of D values in LDS, a group of padding behind each row: sixteen rows' groups at one place lie in different banks
+template <typename T, int D, int R, int THREADS = 256>
+struct Staged {
+    static constexpr int N = Vec<T>::N, PITCH = D + N, GROUPS = D / N, EACH = R * GROUPS / THREADS;
+    static constexpr int BYTES = R * PITCH * sizeof(T);
+    static_assert(R * GROUPS % THREADS == 0, "whole groups to every thread");
+    typename Vec<T>::type g[EACH];
+    // rows [first, first + R) of those below `end`, zeros elsewhere
+    __device__ __forceinline__ void fetch(const T* base, const Rows& rows, int first, int end, int width) {
+#pragma unroll
+        for (int i = 0; i < EACH; ++i) {
+            const int at = threadIdx.x + i * THREADS, r = first + at / GROUPS, c = at % GROUPS * N;
+            g[i] = r < end ? row_group<D>(base + rows.at(r), c, width) : typename Vec<T>::type{};
+        }
+    }
+    __device__ __forceinline__ void store(T* lds) const {
+#pragma unroll
+        for (int i = 0; i < EACH; ++i) {
+            const int at = threadIdx.x + i * THREADS;
+            typedef T aligned_group __attribute__((ext_vector_type(16 / sizeof(T))));
+            *reinterpret_cast<aligned_group*>(lds + at / GROUPS * PITCH + at % GROUPS * N) = g[i];
+        }
+    }
+    // the left operand along the rows: row r + lane % 16, group 4 c + lane / 16
+    static __device__ __forceinline__ typename Vec<T>::type along(const T* lds, int r, int c) {
+        typedef T aligned_group __attribute__((ext_vector_type(16 / sizeof(T))));
+        const int lane = threadIdx.x & 63;
+        return *reinterpret_cast<const aligned_group*>(lds + (r + (lane & 15)) * PITCH + (4 * c + (lane >> 4)) * N);
+    }
+};
+
+// How the D columns of a transposed result lie in accumulators: block b, tile t of it (NV tiles to a block), row i of the tile: column (16 b + i) NV + t, so
+// that a lane reads the left operand of NV tiles, and writes NV neighbours of the result, at once.
+template <typename T, int D>
+struct Columns {
+    static constexpr int NV = D % (16 * Vec<T>::N) == 0 ? Vec<T>::N : Vec<T>::N / 2, BLOCKS = D / (16 * NV);
+    static_assert(D % (16 * NV) == 0, "whole blocks");
+    typedef T values __attribute__((ext_vector_type(NV)));
+    typename Matrix<T>::acc acc[BLOCKS][NV];
+    __device__ __forceinline__ void clear() {
+#pragma unroll
+        for (int b = 0; b < BLOCKS; ++b)
+#pragma unroll
+            for (int t = 0; t < NV; ++t) acc[b][t] = typename Matrix<T>::acc{};
+    }
+    __device__ __forceinline__ void times(T f) {
+#pragma unroll
+        for (int b = 0; b < BLOCKS; ++b)
+#pragma unroll
+            for (int t = 0; t < NV; ++t) acc[b][t] *= f;
+    }
+    // the left operand across rows: row `r`, the lane's values of block b
+    static __device__ __forceinline__ values across(const T* row, int b) { return *reinterpret_cast<const values*>(row + (16 * b + (threadIdx.x & 15)) * NV); }
+    // f(column, NV values) for every run of neighbours that the lane holds
+    template <typename F>
+    __device__ __forceinline__ void each(F f) const {
+        const int g = (threadIdx.x & 63) >> 4;
+#pragma unroll
+        for (int b = 0; b < BLOCKS; ++b)
+#pragma unroll
+            for (int v = 0; v < 4; ++v) {
+                T run[NV];
+#pragma unroll
+                for (int t = 0; t < NV; ++t) run[t] = acc[b][t][v];
+                f((16 * b + Matrix<T>::row_of(v, g)) * NV, run);
+            }
+    }
+};
+
+template <int NV, typename T>
+__device__ __forceinline__ void store_run(T* row, int c, int width, const T (&run)[NV]) {
+    typedef T values __attribute__((ext_vector_type(NV), aligned(sizeof(T))));
+    if (c + NV <= width) {
+        values g;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) g[i] = run[i];
+        *reinterpret_cast<values*>(row + c) = g;
+    } else {
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+            if (c + i < width) row[c + i] = run[i];
+    }
+}
+
+// folds over the four lanes that hold a row
+template <typename T, typename Op>
+__device__ __forceinline__ T fold_row(T v, Op op) {
+    return fold_lanes<64, 16>(v, op);
+}
+
+// The running softmax of the row of a lane
+template <typename T>
+struct Running {
+    T top = Matrix<T>::lowest, sum = 0;  // (the sum of the lane's own states)
+    // takes the scores of a tile, which become weights; true where the sums so far have to be multiplied by `again`
+    template <int TILES>
+    __device__ __forceinline__ bool take(typename Matrix<T>::acc (&s)[TILES], T& again) {
+        T best = top;
+#pragma unroll
+        for (int t = 0; t < TILES; ++t)
+#pragma unroll
+            for (int v = 0; v < 4; ++v) best = Max()(best, s[t][v]);
+        best = fold_row(best, Max());
+        const bool rises = __any(best > top);
+        again = Matrix<T>::weight(top - best);
+        T here = 0;
+#pragma unroll
+        for (int t = 0; t < TILES; ++t)
+#pragma unroll
+            for (int v = 0; v < 4; ++v) {
+                s[t][v] = Matrix<T>::weight(s[t][v] - best);
+                here += s[t][v];
+            }
+        sum = sum * again + here;
+        top = best;
+        return rises;
+    }
+};
+
+template <typename T>
+__device__ __forceinline__ int64_t dense_row(const Args& a, int b, int kvh, int r) {
+    const int t = a.group == 1 ? r : r / a.group;
+    return ((int64_t)b * a.queries + t) * a.heads + (int64_t)kvh * a.group + (r - t * a.group);
+}
+
+// ------------------------------------------------------------------------------------------------ forward
+// A workgroup of four waves takes 64 RQ rows of a problem, a wave 16 RQ of them, over a part of the states, KT at a time through LDS.
+template <typename T, int D>
+struct ForwardShape {
+    static constexpr int KT = D * sizeof(T) <= 256 ? 64 : 32, RQ = D * sizeof(T) <= 512 ? 2 : 1;
+    static constexpr int LDS = 2 * Staged<T, D, KT>::BYTES;
+};
+
+template <typename T, int D>
+__global__ __launch_bounds__(256, D * sizeof(T) <= 1024 ? 2 : 1) void attention_rows(Args a) {
+    typedef Matrix<T> M;
+    typedef ForwardShape<T, D> S;
+    constexpr int KT = S::KT, RQ = S::RQ, N = Vec<T>::N, C = D / (4 * N);
+    extern __shared__ __attribute__((aligned(16))) char attention_lds[];
+    T *ks = reinterpret_cast<T*>(attention_lds), *vs = ks + KT * Staged<T, D, KT>::PITCH;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4;
+    const int id = on_die(blockIdx.x, gridDim.x);
+    const int at = id / (a.tiles * a.parts), rest = id - at * a.tiles * a.parts, part = rest / a.tiles, tile = rest - part * a.tiles, problem = a.first + at;
+    const int b = problem / a.kv_heads, kvh = problem - b * a.kv_heads;
+    const int n = count_of(a, b), slabs = (n + KT - 1) / KT;
+    const int begin = (int)((int64_t)slabs * part / a.parts), end = (int)((int64_t)slabs * (part + 1) / a.parts);
+    const T* q = (const T*)a.q.p + b * a.q.batch + (int64_t)kvh * a.group * a.q.head;
+    const T* k = (const T*)a.k.p + b * a.k.batch + kvh * a.k.head;
+    const T* v = (const T*)a.v.p + b * a.v.batch + kvh * a.v.head;
+    const Rows q_rows = {a.q.row, a.q.head, a.group}, k_rows = {a.k.row, 0, 1}, v_rows = {a.v.row, 0, 1};
+    const int r0 = tile * 64 * RQ + wave * 16 * RQ;
+    Fragment<T, D> qf[RQ];
+#pragma unroll
+    for (int i = 0; i < RQ; ++i) qf[i].load(q + q_rows.at(min(r0 + 16 * i + (lane & 15), a.rows - 1)), a.width, (T)(a.scale * M::base));
+    Columns<T, D> y[RQ];
+    Running<T> run[RQ];
+#pragma unroll
+    for (int i = 0; i < RQ; ++i) y[i].clear();
+    Staged<T, D, KT> kt, vt;
+    if (begin < end) {
+        kt.fetch(k, k_rows, begin * KT, n, a.width);
+        vt.fetch(v, v_rows, begin * KT, n, a.width);
+    }
+    for (int slab = begin; slab < end; ++slab) {
+        __syncthreads();
+        kt.store(ks);
+        vt.store(vs);
+        __syncthreads();
+        if (slab + 1 < end) {
+            kt.fetch(k, k_rows, (slab + 1) * KT, n, a.width);
+            vt.fetch(v, v_rows, (slab + 1) * KT, n, a.width);
+        }
+        typename M::acc s[RQ][KT / 16];
+#pragma unroll
+        for (int t = 0; t < KT / 16; ++t) {
+#pragma unroll
+            for (int i = 0; i < RQ; ++i) s[i][t] = typename M::acc{};
+#pragma unroll
+            for (int c = 0; c < C; ++c) {
+                const typename Vec<T>::type left = Staged<T, D, KT>::along(ks, 16 * t, c);
+#pragma unroll
+                for (int e = 0; e < N; ++e)
+#pragma unroll
+                    for (int i = 0; i < RQ; ++i) s[i][t] = M::mul(left[e], qf[i].g[c][e], s[i][t]);
+            }
+        }
+        if ((slab + 1) * KT > n) {
+#pragma unroll
+            for (int t = 0; t < KT / 16; ++t)
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (slab * KT + 16 * t + M::row_of(e, g) >= n)
+#pragma unroll
+                        for (int i = 0; i < RQ; ++i) s[i][t][e] = T(-INFINITY);
+        }
+#pragma unroll
+        for (int i = 0; i < RQ; ++i) {
+            T again;
+            if (run[i].template take<KT / 16>(s[i], again)) y[i].times(again);
+        }
+#pragma unroll
+        for (int t = 0; t < KT / 16; ++t)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const T* row = vs + (16 * t + M::row_of(e, g)) * Staged<T, D, KT>::PITCH;
+#pragma unroll
+                for (int blk = 0; blk < Columns<T, D>::BLOCKS; ++blk) {
+                    const auto left = Columns<T, D>::across(row, blk);
+#pragma unroll
+                    for (int c = 0; c < Columns<T, D>::NV; ++c)
+#pragma unroll
+                        for (int i = 0; i < RQ; ++i) y[i].acc[blk][c] = M::mul(left[c], s[i][t][e], y[i].acc[blk][c]);
+                }
+            }
+    }
+#pragma unroll
+    for (int i = 0; i < RQ; ++i) {
+        const int r = r0 + 16 * i + (lane & 15);
+        const T sum = fold_row(run[i].sum, Sum());
+        if (r >= a.rows) continue;
+        if (a.parts == 1) {
+            const int64_t to = dense_row<T>(a, b, kvh, r);
+            y[i].times(sum == T(0) ? T(0) : T(1) / sum);
+            T* out = (T*)a.y_out + to * a.width;
+            y[i].each([&](int c, const auto& values) { store_run(out, c, a.width, values); });
+            if (g == 0) ((T*)a.lse_out)[to] = sum == T(0) ? T(-INFINITY) : M::lse(run[i].top, sum);
+        } else {
+            const int64_t to = ((int64_t)part * a.batch * a.kv_heads + problem) * a.rows + r;
+            T* out = (T*)a.parts_y + to * D;
+            y[i].each([&](int c, const auto& values) { store_run(out, c, D, values); });
+            if (g == 0) ((T*)a.parts_m)[to] = run[i].top, ((T*)a.parts_l)[to] = sum;
+        }
+    }
+}
+
+// Up to 16 RQ rows: nobody shares a state with another wave, so each of the four takes states of its own, straight from memory into the operands (16 at a time,
+// 64-byte pieces of a state), and they are joined in LDS.
+template <typename T, int D, int RQ>
+__global__ __launch_bounds__(256, D * sizeof(T) <= 512 ? 2 : 1) void attention_few(Args a) {
+    typedef Matrix<T> M;
+    constexpr int N = Vec<T>::N, C = D / (4 * N);
+    extern __shared__ __attribute__((aligned(16))) char attention_lds[];
+    T* tops = reinterpret_cast<T*>(attention_lds);  // [4][16 RQ]
+    T* sums = tops + 64 * RQ;
+    T* ys = sums + 64 * RQ;  // [16 RQ][D + N]
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4;
+    const int id = on_die(blockIdx.x, gridDim.x);
+    const int at = id / a.parts, part = id - at * a.parts, problem = a.first + at;
+    const int b = problem / a.kv_heads, kvh = problem - b * a.kv_heads;
+    const int n = count_of(a, b), slabs = (n + 15) / 16, mine = part * 4 + wave;
+    const int begin = (int)((int64_t)slabs * mine / (4 * a.parts)), end = (int)((int64_t)slabs * (mine + 1) / (4 * a.parts));
+    const T* q = (const T*)a.q.p + b * a.q.batch + (int64_t)kvh * a.group * a.q.head;
+    const T* k = (const T*)a.k.p + b * a.k.batch + kvh * a.k.head;
+    const T* v = (const T*)a.v.p + b * a.v.batch + kvh * a.v.head;
+    const Rows q_rows = {a.q.row, a.q.head, a.group};
+    Fragment<T, D> qf[RQ];
+#pragma unroll
+    for (int i = 0; i < RQ; ++i) qf[i].load(q + q_rows.at(min(16 * i + (lane & 15), a.rows - 1)), a.width, (T)(a.scale * M::base));
+    Columns<T, D> y[RQ];
+    Running<T> run[RQ];
+#pragma unroll
+    for (int i = 0; i < RQ; ++i) y[i].clear();
+    for (int slab = begin; slab < end; ++slab) {
+        const int key = slab * 16 + (lane & 15);
+        typename Vec<T>::type left[C];
+        const T* k_row = k + min(key, n - 1) * a.k.row;
+#pragma unroll
+        for (int c = 0; c < C; ++c) left[c] = row_group<D>(k_row, (4 * c + g) * N, a.width);
+        // (states past the last one weigh nothing, but must not be infinite either: the last one stands in)
+        typename Columns<T, D>::values across[4][Columns<T, D>::BLOCKS];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const T* v_row = v + min(slab * 16 + M::row_of(e, g), n - 1) * a.v.row;
+#pragma unroll
+            for (int blk = 0; blk < Columns<T, D>::BLOCKS; ++blk) {
+                constexpr int NV = Columns<T, D>::NV;
+                const int c = (16 * blk + (lane & 15)) * NV;
+                typedef T loose __attribute__((ext_vector_type(NV), aligned(sizeof(T))));
+                if (c + NV <= a.width) {
+                    across[e][blk] = *reinterpret_cast<const loose*>(v_row + c);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < NV; ++i) across[e][blk][i] = c + i < a.width ? v_row[c + i] : T(0);
+                }
+            }
+        }
+        typename M::acc s[RQ][1];
+#pragma unroll
+        for (int i = 0; i < RQ; ++i) {
+            s[i][0] = typename M::acc{};
+#pragma unroll
+            for (int c = 0; c < C; ++c)
+#pragma unroll
+                for (int e = 0; e < N; ++e) s[i][0] = M::mul(left[c][e], qf[i].g[c][e], s[i][0]);
+        }
+        if (slab * 16 + 16 > n) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (slab * 16 + M::row_of(e, g) >= n)
+#pragma unroll
+                    for (int i = 0; i < RQ; ++i) s[i][0][e] = T(-INFINITY);
+        }
+#pragma unroll
+        for (int i = 0; i < RQ; ++i) {
+            T again;
+            if (run[i].template take<1>(s[i], again)) y[i].times(again);
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+#pragma unroll
+            for (int blk = 0; blk < Columns<T, D>::BLOCKS; ++blk)
+#pragma unroll
+                for (int c = 0; c < Columns<T, D>::NV; ++c)
+#pragma unroll
+                    for (int i = 0; i < RQ; ++i) y[i].acc[blk][c] = M::mul(across[e][blk][c], s[i][0][e], y[i].acc[blk][c]);
+    }
+    // the four waves' parts: maxima and sums first, then the rows, one wave after the other
+    T sum[RQ];
+#pragma unroll
+    for (int i = 0; i < RQ; ++i) {
+        sum[i] = fold_row(run[i].sum, Sum());
+        if (g == 0) {
+            tops[wave * 16 * RQ + 16 * i + lane] = run[i].top;
+            sums[wave * 16 * RQ + 16 * i + lane] = sum[i];
+        }
+    }
+    __syncthreads();
+    T best[RQ], all[RQ];
+#pragma unroll
+    for (int i = 0; i < RQ; ++i) {
+        best[i] = M::lowest, all[i] = 0;
+        for (int w = 0; w < 4; ++w) best[i] = Max()(best[i], tops[w * 16 * RQ + 16 * i + (lane & 15)]);
+        for (int w = 0; w < 4; ++w) all[i] += sums[w * 16 * RQ + 16 * i + (lane & 15)] * M::weight(tops[w * 16 * RQ + 16 * i + (lane & 15)] - best[i]);
+        y[i].times(M::weight(run[i].top - best[i]));
+    }
+    for (int w = 0; w < 4; ++w) {
+        if (wave == w)
+#pragma unroll
+            for (int i = 0; i < RQ; ++i) {
+                T* row = ys + (16 * i + (lane & 15)) * (D + N);
+                y[i].each([&](int c, const auto& values) {
+#pragma unroll
+                    for (int e = 0; e < Columns<T, D>::NV; ++e) row[c + e] = w == 0 ? values[e] : row[c + e] + values[e];
+                });
+            }
+        __syncthreads();
+    }
+    // (every wave holds the maximum and the sum of a lane's row)
+    if (wave == 0 && g == 0) {
+#pragma unroll
+        for (int i = 0; i < RQ; ++i) {
+            const int r = 16 * i + lane;
+            sums[r] = all[i];  // from here on the row's own
+            if (r >= a.rows) continue;
+            if (a.parts == 1) {
+                ((T*)a.lse_out)[dense_row<T>(a, b, kvh, r)] = all[i] == T(0) ? T(-INFINITY) : M::lse(best[i], all[i]);
+            } else {
+                const int64_t to = ((int64_t)part * a.batch * a.kv_heads + problem) * a.rows + r;
+                ((T*)a.parts_m)[to] = best[i], ((T*)a.parts_l)[to] = all[i];
+            }
+        }
+    }
+    __syncthreads();
+    for (int at = threadIdx.x; at < min(a.rows, 16 * RQ) * (D / N); at += 256) {
+        const int r = at / (D / N), c = at % (D / N) * N;
+        T values[N];
+#pragma unroll
+        for (int e = 0; e < N; ++e) values[e] = ys[r * (D + N) + c + e];
+        if (a.parts == 1) {
+            if (c >= a.width) continue;
+#pragma unroll
+            for (int e = 0; e < N; ++e) values[e] = sums[r] == T(0) ? T(0) : values[e] / sums[r];
+            store_group((T*)a.y_out + dense_row<T>(a, b, kvh, r) * a.width, c, a.width, values);
+        } else {
+            store_group((T*)a.parts_y + (((int64_t)part * a.batch * a.kv_heads + problem) * a.rows + r) * D, c, D, values);
+        }
+    }
+}
+
+// A wave joins the parts of a row.
+template <typename T, int D>
+__global__ __launch_bounds__(256) void attention_join(Args a) {
+    typedef Matrix<T> M;
+    const int64_t problems = (int64_t)a.batch * a.kv_heads, unit = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (unit >= problems * a.rows) return;
+    const int lane = threadIdx.x & 63, problem = (int)(unit / a.rows), r = (int)(unit - (int64_t)problem * a.rows);
+    const T *m = (const T*)a.parts_m + unit, *l = (const T*)a.parts_l + unit, *y = (const T*)a.parts_y + unit * D;
+    const int64_t pitch = problems * a.rows;
+    T top = M::lowest, sum = 0;
+    for (int p = 0; p < a.parts; ++p) top = Max()(top, m[p * pitch]);
+    constexpr int EACH = (D + 63) / 64;
+    T out[EACH] = {};
+    for (int p = 0; p < a.parts; ++p) {
+        const T f = M::weight(m[p * pitch] - top);
+        sum += l[p * pitch] * f;
+#pragma unroll
+        for (int i = 0; i < EACH; ++i)
+            if (i * 64 + lane < D) out[i] += y[p * pitch * D + i * 64 + lane] * f;
+    }
+    const int64_t to = dense_row<T>(a, problem / a.kv_heads, problem % a.kv_heads, r);
+#pragma unroll
+    for (int i = 0; i < EACH; ++i)
+        if (i * 64 + lane < a.width) ((T*)a.y_out)[to * a.width + i * 64 + lane] = sum == T(0) ? T(0) : out[i] / sum;
+    if (lane == 0) ((T*)a.lse_out)[to] = sum == T(0) ? T(-INFINITY) : M::lse(top, sum);
+}
+
+// ------------------------------------------------------------------------------------------------ backward
+// delta = dy.y of every row: 16 lanes to a row
+template <typename T>
+__global__ __launch_bounds__(256) void attention_delta(Args a, int64_t first) {
+    constexpr int N = Vec<T>::N;
+    const int64_t row = first + (int64_t)blockIdx.x * 16 + threadIdx.x / 16;
+    const bool there = row < (int64_t)a.batch * a.queries * a.heads;
+    T sum = 0;
+    if (there) {
+        const int64_t bt = row / a.heads;
+        const int h = (int)(row - bt * a.heads), b = (int)(bt / a.queries), t = (int)(bt - (int64_t)b * a.queries);
+        const T *dy = (const T*)a.dy.p + b * a.dy.batch + t * a.dy.row + h * a.dy.head, *y = (const T*)a.y + row * a.width;
+        for (int c = threadIdx.x % 16 * N; c < a.width; c += 16 * N) {
+            T u[N], v[N];
+            load_group(dy, c, a.width, T(0), u);
+            load_group(y, c, a.width, T(0), v);
+#pragma unroll
+            for (int e = 0; e < N; ++e) sum += u[e] * v[e];
+        }
+    }
+    sum = fold_lanes<16>(sum, Sum());
+    if (there && threadIdx.x % 16 == 0) ((T*)a.delta)[row] = sum;
+}
+
+// what weights of a row are relative to: a row without weight has none anywhere
+template <typename T>
+__device__ __forceinline__ T level_of(T lse) {
+    return lse == T(-INFINITY) ? T(INFINITY) : lse * (T)Matrix<T>::base;
+}
+
+// The gradients of the states: a workgroup takes 64 RK states, a wave 16 RK of them in its registers, and walks over the rows, RT at a time through LDS.
+// KEYS, VALUES: which of dk and dv it forms.
+template <typename T, int D>
+struct StatesShape {
+    static constexpr int RT = 32, RK = D * sizeof(T) <= 256 ? 2 : 1;
+    static constexpr bool BOTH = D * sizeof(T) <= 1024;  // both gradients' sums and both operands fit a wave's registers
+    static constexpr int LDS = 2 * Staged<T, D, RT>::BYTES + 2 * RT * (int)sizeof(T);
+};
+
+template <typename T, int D, bool KEYS, bool VALUES>
+__global__ __launch_bounds__(256, D * sizeof(T) <= 512 ? 2 : 1) void attention_states_gradient(Args a) {
+    typedef Matrix<T> M;
+    typedef StatesShape<T, D> S;
+    constexpr int RT = S::RT, RK = S::RK, N = Vec<T>::N, C = D / (4 * N), PITCH = Staged<T, D, RT>::PITCH;
+    extern __shared__ __attribute__((aligned(16))) char attention_lds[];
+    T *qs = reinterpret_cast<T*>(attention_lds), *gs = qs + RT * PITCH, *levels = gs + RT * PITCH, *deltas = levels + RT;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4;
+    const int id = on_die(blockIdx.x, gridDim.x);
+    const int at = id / a.tiles, tile = id - at * a.tiles, problem = a.first + at;
+    const int b = problem / a.kv_heads, kvh = problem - b * a.kv_heads;
+    const int n = count_of(a, b), k0 = tile * 64 * RK + wave * 16 * RK;
+    const T* q = (const T*)a.q.p + b * a.q.batch + (int64_t)kvh * a.group * a.q.head;
+    const T* dy = (const T*)a.dy.p + b * a.dy.batch + (int64_t)kvh * a.group * a.dy.head;
+    const T* k = (const T*)a.k.p + b * a.k.batch + kvh * a.k.head;
+    const T* v = (const T*)a.v.p + b * a.v.batch + kvh * a.v.head;
+    const Rows q_rows = {a.q.row, a.q.head, a.group}, dy_rows = {a.dy.row, a.dy.head, a.group};
+    Columns<T, D> dk[KEYS ? RK : 1], dv[VALUES ? RK : 1];
+    if (KEYS)
+#pragma unroll
+        for (int i = 0; i < RK; ++i) dk[i].clear();
+    if (VALUES)
+#pragma unroll
+        for (int i = 0; i < RK; ++i) dv[i].clear();
+    if (tile * 64 * RK < n) {
+        Fragment<T, D> kf[RK], vf[KEYS ? RK : 1];
+#pragma unroll
+        for (int i = 0; i < RK; ++i) {
+            const int key = min(k0 + 16 * i + (lane & 15), n - 1);
+            kf[i].load(k + key * a.k.row, a.width, (T)(a.scale * M::base));
+            if (KEYS) vf[i].load(v + key * a.v.row, a.width, T(1));
+        }
+        Staged<T, D, RT> qt, gt;
+        T level = 0, delta = 0;
+        auto fetch = [&](int r0) {
+            qt.fetch(q, q_rows, r0, a.rows, a.width);
+            gt.fetch(dy, dy_rows, r0, a.rows, a.width);
+            if (threadIdx.x < RT) {
+                const int r = r0 + threadIdx.x;
+                level = T(INFINITY), delta = 0;
+                if (r < a.rows) {
+                    const int64_t at = dense_row<T>(a, b, kvh, r);
+                    level = level_of(((const T*)a.lse)[at]);
+                    delta = ((const T*)a.delta)[at];
+                }
+            }
+        };
+        fetch(0);
+        for (int r0 = 0; r0 < a.rows; r0 += RT) {
+            __syncthreads();
+            qt.store(qs);
+            gt.store(gs);
+            if (threadIdx.x < RT) levels[threadIdx.x] = level, deltas[threadIdx.x] = delta;
+            __syncthreads();
+            if (r0 + RT < a.rows) fetch(r0 + RT);
+#pragma unroll
+            for (int t = 0; t < RT / 16; ++t) {
+                typename M::acc s[RK], dp[RK];
+#pragma unroll
+                for (int i = 0; i < RK; ++i) s[i] = dp[i] = typename M::acc{};
+#pragma unroll
+                for (int c = 0; c < C; ++c) {
+                    const typename Vec<T>::type left = Staged<T, D, RT>::along(qs, 16 * t, c);
+#pragma unroll
+                    for (int e = 0; e < N; ++e)
+#pragma unroll
+                        for (int i = 0; i < RK; ++i) s[i] = M::mul(left[e], kf[i].g[c][e], s[i]);
+                    if (KEYS) {
+                        const typename Vec<T>::type down = Staged<T, D, RT>::along(gs, 16 * t, c);
+#pragma unroll
+                        for (int e = 0; e < N; ++e)
+#pragma unroll
+                            for (int i = 0; i < RK; ++i) dp[i] = M::mul(down[e], vf[i].g[c][e], dp[i]);
+                    }
+                }
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int r = 16 * t + M::row_of(e, g);
+                    const T lev = levels[r], del = KEYS ? deltas[r] : T(0);
+#pragma unroll
+                    for (int i = 0; i < RK; ++i) {
+                        s[i][e] = lev == T(INFINITY) ? T(0) : M::weight(s[i][e] - lev);
+                        dp[i][e] = s[i][e] * (dp[i][e] - del);
+                    }
+                }
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int r = 16 * t + M::row_of(e, g);
+#pragma unroll
+                    for (int blk = 0; blk < Columns<T, D>::BLOCKS; ++blk) {
+                        if (VALUES) {
+                            const auto left = Columns<T, D>::across(gs + r * PITCH, blk);
+#pragma unroll
+                            for (int c = 0; c < Columns<T, D>::NV; ++c)
+#pragma unroll
+                                for (int i = 0; i < RK; ++i) dv[i].acc[blk][c] = M::mul(left[c], s[i][e], dv[i].acc[blk][c]);
+                        }
+                        if (KEYS) {
+                            const auto left = Columns<T, D>::across(qs + r * PITCH, blk);
+#pragma unroll
+                            for (int c = 0; c < Columns<T, D>::NV; ++c)
+#pragma unroll
+                                for (int i = 0; i < RK; ++i) dk[i].acc[blk][c] = M::mul(left[c], dp[i][e], dk[i].acc[blk][c]);
+                        }
+                    }
+                }
+            }
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < RK; ++i) {
+        const int key = k0 + 16 * i + (lane & 15);
+        if (key >= a.keys) continue;
+        const int64_t to = (((int64_t)b * a.keys + key) * a.kv_heads + kvh) * a.width;
+        // (behind the last state: what its stand-in came to is not the gradient, which is zero)
+        const bool there = key < n;
+        auto put = [&](T* out, const Columns<T, D>& sums, T factor) {
+            sums.each([&](int c, const auto& values) {
+                T run[Columns<T, D>::NV];
+#pragma unroll
+                for (int e = 0; e < Columns<T, D>::NV; ++e) run[e] = there ? values[e] * factor : T(0);
+                store_run(out + to, c, a.width, run);
+            });
+        };
+        if (KEYS) put((T*)a.dk, dk[i], (T)a.scale);
+        if (VALUES) put((T*)a.dv, dv[i], T(1));
+    }
+}
+
+// The gradient of the rows: as the forward pass, with the weights known from lse.
+template <typename T, int D>
+struct RowsShape {
+    static constexpr int KT = 32, RQ = D * sizeof(T) <= 256 ? 2 : 1;
+    static constexpr int LDS = 2 * Staged<T, D, KT>::BYTES;
+};
+
+template <typename T, int D>
+__global__ __launch_bounds__(256, D * sizeof(T) <= 512 ? 2 : 1) void attention_rows_gradient(Args a) {
+    typedef Matrix<T> M;
+    typedef RowsShape<T, D> S;
+    constexpr int KT = S::KT, RQ = S::RQ, N = Vec<T>::N, C = D / (4 * N), PITCH = Staged<T, D, KT>::PITCH;
+    extern __shared__ __attribute__((aligned(16))) char attention_lds[];
+    T *ks = reinterpret_cast<T*>(attention_lds), *vs = ks + KT * PITCH;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4;
+    const int id = on_die(blockIdx.x, gridDim.x);
+    const int at = id / a.tiles, tile = id - at * a.tiles, problem = a.first + at;
+    const int b = problem / a.kv_heads, kvh = problem - b * a.kv_heads;
+    const int n = count_of(a, b);
+    const T* q = (const T*)a.q.p + b * a.q.batch + (int64_t)kvh * a.group * a.q.head;
+    const T* dy = (const T*)a.dy.p + b * a.dy.batch + (int64_t)kvh * a.group * a.dy.head;
+    const T* k = (const T*)a.k.p + b * a.k.batch + kvh * a.k.head;
+    const T* v = (const T*)a.v.p + b * a.v.batch + kvh * a.v.head;
+    const Rows q_rows = {a.q.row, a.q.head, a.group}, dy_rows = {a.dy.row, a.dy.head, a.group}, k_rows = {a.k.row, 0, 1}, v_rows = {a.v.row, 0, 1};
+    const int r0 = tile * 64 * RQ + wave * 16 * RQ;
+    Fragment<T, D> qf[RQ], gf[RQ];
+    Columns<T, D> dq[RQ];
+    T level[RQ], delta[RQ];
+#pragma unroll
+    for (int i = 0; i < RQ; ++i) {
+        const int r = min(r0 + 16 * i + (lane & 15), a.rows - 1);
+        qf[i].load(q + q_rows.at(r), a.width, (T)(a.scale * M::base));
+        gf[i].load(dy + dy_rows.at(r), a.width, T(1));
+        const int64_t at = dense_row<T>(a, b, kvh, r);
+        level[i] = level_of(((const T*)a.lse)[at]);
+        delta[i] = ((const T*)a.delta)[at];
+        dq[i].clear();
+    }
+    Staged<T, D, KT> kt, vt;
+    if (n > 0) {
+        kt.fetch(k, k_rows, 0, n, a.width);
+        vt.fetch(v, v_rows, 0, n, a.width);
+    }
+    for (int first = 0; first < n; first += KT) {
+        __syncthreads();
+        kt.store(ks);
+        vt.store(vs);
+        __syncthreads();
+        if (first + KT < n) {
+            kt.fetch(k, k_rows, first + KT, n, a.width);
+            vt.fetch(v, v_rows, first + KT, n, a.width);
+        }
+#pragma unroll
+        for (int t = 0; t < KT / 16; ++t) {
+            typename M::acc s[RQ], dp[RQ];
+#pragma unroll
+            for (int i = 0; i < RQ; ++i) s[i] = dp[i] = typename M::acc{};
+#pragma unroll
+            for (int c = 0; c < C; ++c) {
+                const typename Vec<T>::type left = Staged<T, D, KT>::along(ks, 16 * t, c), down = Staged<T, D, KT>::along(vs, 16 * t, c);
+#pragma unroll
+                for (int e = 0; e < N; ++e)
+#pragma unroll
+                    for (int i = 0; i < RQ; ++i) {
+                        s[i] = M::mul(left[e], qf[i].g[c][e], s[i]);
+                        dp[i] = M::mul(down[e], gf[i].g[c][e], dp[i]);
+                    }
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const bool there = first + 16 * t + M::row_of(e, g) < n;
+#pragma unroll
+                for (int i = 0; i < RQ; ++i) dp[i][e] = there ? M::weight(s[i][e] - level[i]) * (dp[i][e] - delta[i]) : T(0);
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const T* row = ks + (16 * t + M::row_of(e, g)) * PITCH;
+#pragma unroll
+                for (int blk = 0; blk < Columns<T, D>::BLOCKS; ++blk) {
+                    const auto left = Columns<T, D>::across(row, blk);
+#pragma unroll
+                    for (int c = 0; c < Columns<T, D>::NV; ++c)
+#pragma unroll
+                        for (int i = 0; i < RQ; ++i) dq[i].acc[blk][c] = M::mul(left[c], dp[i][e], dq[i].acc[blk][c]);
+                }
+            }
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < RQ; ++i) {
+        const int r = r0 + 16 * i + (lane & 15);
+        if (r >= a.rows) continue;
+        T* out = (T*)a.dq + dense_row<T>(a, b, kvh, r) * a.width;
+        dq[i].times((T)a.scale);
+        dq[i].each([&](int c, const auto& values) { store_run(out, c, a.width, values); });
+    }
+}
+
+// ------------------------------------------------------------------------------------------------ launches (host)
+constexpr int kUnits = 256;  // compute units that work is cut for
+
+// Parts that the states are cut into, so that every compute unit has about `per_unit` workgroups, none with less than `least` slabs
+int parts_for(int64_t workgroups, int slabs, int per_unit, int least) {
+    if (workgroups >= kUnits * per_unit) return 1;
+    const int64_t wanted = ((int64_t)kUnits * per_unit + workgroups - 1) / workgroups;
+    return (int)std::max<int64_t>(1, std::min<int64_t>({wanted, slabs / least, 64}));
+}
+
+int padded(int width) { return width <= 32 ? 32 : width <= 64 ? 64 : width <= 128 ? 128 : 256; }
+
+// how the forward pass is cut
+struct ForwardPlan {
+    bool few;
+    int rq, tiles, parts;
+    template <typename T, int D>
+    void set(const Args& a) {
+        typedef ForwardShape<T, D> S;
+        const int64_t problems = (int64_t)a.batch * a.kv_heads;
+        few = a.rows <= 32;
+        rq = a.rows <= 16 ? 1 : 2;
+        tiles = few ? 1 : (a.rows + 64 * S::RQ - 1) / (64 * S::RQ);
+        parts = few ? parts_for(problems, (a.keys + 63) / 64, 3, 2) : parts_for(problems * tiles, (a.keys + S::KT - 1) / S::KT, 2, 4);
+    }
+};
+
+template <typename F>
+auto by_width(int dtype, int width, F f) {
+    const int d = padded(width);
+    if (dtype == DALI_HIP_FLOAT) {
+        if (d == 32) return f(float(), std::integral_constant<int, 32>());
+        if (d == 64) return f(float(), std::integral_constant<int, 64>());
+        if (d == 128) return f(float(), std::integral_constant<int, 128>());
+        return f(float(), std::integral_constant<int, 256>());
+    }
+    if (d == 32) return f(double(), std::integral_constant<int, 32>());
+    if (d == 64) return f(double(), std::integral_constant<int, 64>());
+    if (d == 128) return f(double(), std::integral_constant<int, 128>());
+    return f(double(), std::integral_constant<int, 256>());
+}
+
+size_t round256(size_t b) { return (b + 255) / 256 * 256; }
+
+// bytes of the workspace, and where its parts lie
+size_t lay_out(int dtype, Args& a, bool backward, char* space) {
+    const size_t size = dtype == DALI_HIP_FLOAT ? 4 : 8, rows = (size_t)a.batch * a.queries * a.heads;
+    if (backward) {
+        a.delta = space;
+        return round256(rows * size);
+    }
+    return by_width(dtype, a.width, [&](auto t, auto d) -> size_t {
+        ForwardPlan plan;
+        plan.set<decltype(t), decltype(d)::value>(a);
+        a.parts = plan.parts, a.tiles = plan.tiles;
+        if (plan.parts == 1) return 0;
+        const size_t y = round256(rows * plan.parts * padded(a.width) * size), one = round256(rows * plan.parts * size);
+        a.parts_y = space, a.parts_m = space + y, a.parts_l = space + y + one;
+        return y + 2 * one;
+    });
+}
+
+// `each` workgroups for each of the problems, in launches of fewer than 2^32 threads
+template <typename K>
+int launch(const char* what, K kernel, int64_t problems, int64_t each, int lds, Args a) {
+    if (lds > 65536) {
+        const hipError_t e = reserve_dynamic_lds((const void*)kernel, lds);
+        if (e != hipSuccess) return fail("%s: cannot reserve %d bytes of LDS: %s", what, lds, hipGetErrorString(e));
+    }
+    const int64_t most = std::max<int64_t>(1, (1 << 23) / each);
+    for (int64_t first = 0; first < problems; first += most) {
+        a.first = (int)first;
+        kernel<<<dim3((unsigned)(std::min(problems - first, most) * each)), dim3(256), lds, stream()>>>(a);
+        if (launched(what)) return DALI_HIP_ERROR;
+    }
+    return DALI_HIP_OK;
+}
+
+template <typename T, int D>
+int forward(const char* what, Args a) {
+    ForwardPlan plan;
+    plan.set<T, D>(a);
+    a.parts = plan.parts, a.tiles = plan.tiles;
+    const int64_t problems = (int64_t)a.batch * a.kv_heads;
+    const int few_lds = 16 * plan.rq * (D + Vec<T>::N + 8) * (int)sizeof(T);
+    const int status = plan.few ? (plan.rq == 1 ? launch(what, attention_few<T, D, 1>, problems, plan.parts, few_lds, a)
+                                                : launch(what, attention_few<T, D, 2>, problems, plan.parts, few_lds, a))
+                                : launch(what, attention_rows<T, D>, problems, plan.tiles * plan.parts, ForwardShape<T, D>::LDS, a);
+    if (status || plan.parts == 1) return status;
+    return launch(what, attention_join<T, D>, 1, (problems * a.rows + 3) / 4, 0, a);
+}
+
+template <typename T, int D>
+int backward(const char* what, Args a) {
+    const int64_t problems = (int64_t)a.batch * a.kv_heads, rows = (int64_t)a.batch * a.queries * a.heads;
+    const int64_t most = (int64_t)1 << 26;
+    for (int64_t first = 0; first < rows; first += most) {
+        attention_delta<T><<<dim3((unsigned)((std::min(rows - first, most) + 15) / 16)), dim3(256), 0, stream()>>>(a, first);
+        if (launched(what)) return DALI_HIP_ERROR;
+    }
+    if (a.keys > 0) {
+        typedef StatesShape<T, D> S;
+        a.tiles = (a.keys + 64 * S::RK - 1) / (64 * S::RK);
+        if constexpr (S::BOTH) {
+            if (launch(what, attention_states_gradient<T, D, true, true>, problems, a.tiles, S::LDS, a)) return DALI_HIP_ERROR;
+        } else {
+            if (launch(what, attention_states_gradient<T, D, true, false>, problems, a.tiles, S::LDS, a)) return DALI_HIP_ERROR;
+            if (launch(what, attention_states_gradient<T, D, false, true>, problems, a.tiles, S::LDS, a)) return DALI_HIP_ERROR;
+        }
+    }
+    if (rows > 0) {
+        typedef RowsShape<T, D> S;
+        a.tiles = (a.rows + 64 * S::RQ - 1) / (64 * S::RQ);
+        return launch(what, attention_rows_gradient<T, D>, problems, a.tiles, S::LDS, a);
+    }
+    return DALI_HIP_OK;
+}
+
+// ------------------------------------------------------------------------------------------------ arguments (host)
+int check_extents(const char* what, int dtype, int batch, int queries, int keys, int heads, int kv_heads, int width, double scale, Args& a) {
+    if (!is_real(dtype)) return fail("%s: dtype %d is neither float nor double", what, dtype);
+    if (batch < 0 || queries < 0 || keys < 0) return fail("%s: %d sequences of %d positions and %d states", what, batch, queries, keys);
+    if (heads < 1 || kv_heads < 1 || heads % kv_heads) return fail("%s: %d heads cannot share %d", what, heads, kv_heads);
+    if (width < 1 || width > DALI_HIP_MAX_HEAD_WIDTH) return fail("%s: heads are from 1 to %d wide (got %d)", what, DALI_HIP_MAX_HEAD_WIDTH, width);
+    if (!std::isfinite(scale)) return fail("%s: the scale must be finite (got %g)", what, scale);
+    const int group = heads / kv_heads;
+    if ((int64_t)queries * group > 1 << 28 || keys > 1 << 28 || (int64_t)batch * kv_heads > 2147483647LL)
+        return fail("%s: %d sequences of %d positions and %d states with %d heads are too many", what, batch, queries, keys, heads);
+    a = {};
+    a.batch = batch, a.queries = queries, a.keys = keys, a.heads = heads, a.kv_heads = kv_heads, a.width = width, a.group = group, a.rows = queries * group, a.scale = scale;
+    return DALI_HIP_OK;
+}
+
+Operand operand(const void* p, const int64_t* strides) { return {p, strides[0], strides[1], strides[2]}; }
+
+// what an operand of [batch, rows, heads, width] values covers
+Span span_of(const char* name, const Operand& o, int batch, int rows, int heads, int width, size_t size) {
+    Span s(name, nullptr, 0, size);
+    if (!o.p || batch < 1 || rows < 1) return s;
+    int64_t lo = 0, hi = width;
+    for (const int64_t reach : {(batch - 1) * o.batch, (rows - 1) * o.row, (heads - 1) * o.head}) (reach < 0 ? lo : hi) += reach;
+    s.first = (uintptr_t)o.p;
+    s.lo = (uintptr_t)o.p + (intptr_t)(lo * (int64_t)size);
+    s.hi = (uintptr_t)o.p + (intptr_t)(hi * (int64_t)size);
+    return s;
+}
+
+}  // namespace
+}  // namespace dali_hip
+
+using namespace dali_hip;
+
+extern "C" int dali_hip_cross_attention_workspace(int dtype, int batch, int queries, int keys, int heads, int kv_heads, int width, int backward, size_t* bytes) {
+    const char* what = "dali_hip_cross_attention_workspace";
+    Args a;
+    if (check_extents(what, dtype, batch, queries, keys, heads, kv_heads, width, 1.0, a)) return DALI_HIP_ERROR;
+    if (!bytes) return fail("%s: NULL argument", what);
+    *bytes = batch && queries ? lay_out(dtype, a, backward != 0, nullptr) : 0;
+    return DALI_HIP_OK;
+}
+
+extern "C" int dali_hip_cross_attention(int dtype, int batch, int queries, int keys, int heads, int kv_heads, int width, const void* q, const int64_t* q_strides, const void* k,
+                                        const int64_t* k_strides, const void* v, const int64_t* v_strides, const int32_t* counts, double scale, void* y, void* lse,
+                                        void* workspace) {
+    const char* what = "dali_hip_cross_attention";
+    Args a;
+    if (check_extents(what, dtype, batch, queries, keys, heads, kv_heads, width, scale, a)) return DALI_HIP_ERROR;
+    if (batch == 0 || queries == 0) return DALI_HIP_OK;
+    if (!q || !q_strides || !y || !lse || (keys && (!k || !k_strides || !v || !v_strides))) return fail("%s: NULL argument", what);
+    const size_t size = dtype == DALI_HIP_FLOAT ? 4 : 8;
+    a.q = operand(q, q_strides);
+    if (keys) a.k = operand(k, k_strides), a.v = operand(v, v_strides);
+    a.counts = counts, a.y_out = y, a.lse_out = lse;
+    const size_t bytes = lay_out(dtype, a, false, (char*)workspace);
+    if (bytes && !workspace) return fail("%s: NULL argument", what);
+    if (off_elements({q, k, v, y, lse}, size) || off_elements({counts}, 4)) return fail("%s: an address is off its type's size", what);
+    if (bytes && (uintptr_t)workspace % 256 != 0) return fail("%s: the workspace must lie on 256 bytes", what);
+    const int64_t rows = (int64_t)batch * queries * heads;
+    if (check_spans(what, {Span("y", y, rows * width, size), Span("lse", lse, rows, size), Span("the workspace", bytes ? workspace : nullptr, (int64_t)bytes, 1)},
+                    {span_of("q", a.q, batch, queries, heads, width, size), span_of("k", a.k, batch, keys, kv_heads, width, size),
+                     span_of("v", a.v, batch, keys, kv_heads, width, size), Span("key_counts", counts, batch, 4)}, 0))
+        return DALI_HIP_ERROR;
+    if (ensure_init()) return DALI_HIP_ERROR;
+    return by_width(dtype, width, [&](auto t, auto d) { return forward<decltype(t), decltype(d)::value>(what, a); });
+}
+
+extern "C" int dali_hip_cross_attention_backward(int dtype, int batch, int queries, int keys, int heads, int kv_heads, int width, const void* dy, const int64_t* dy_strides,
+                                                 const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides, const void* v, const int64_t* v_strides,
+                                                 const void* y, const void* lse, const int32_t* counts, double scale, void* dq, void* dk, void* dv, void* workspace) {
+    const char* what = "dali_hip_cross_attention_backward";
+    Args a;
+    if (check_extents(what, dtype, batch, queries, keys, heads, kv_heads, width, scale, a)) return DALI_HIP_ERROR;
+    if (batch == 0 || (queries == 0 && keys == 0)) return DALI_HIP_OK;
+    if ((queries && (!dy || !dy_strides || !q || !q_strides || !y || !lse || !dq || !workspace)) || (keys && (!k || !k_strides || !v || !v_strides || !dk || !dv)))
+        return fail("%s: NULL argument", what);
+    const size_t size = dtype == DALI_HIP_FLOAT ? 4 : 8;
+    if (queries) a.q = operand(q, q_strides), a.dy = operand(dy, dy_strides);
+    if (keys) a.k = operand(k, k_strides), a.v = operand(v, v_strides);
+    a.counts = counts, a.y = y, a.lse = lse, a.dq = dq, a.dk = dk, a.dv = dv;
+    const size_t bytes = queries ? lay_out(dtype, a, true, (char*)workspace) : 0;
+    if (off_elements({dy, q, k, v, y, lse, dq, dk, dv}, size) || off_elements({counts}, 4)) return fail("%s: an address is off its type's size", what);
+    if (bytes && (uintptr_t)workspace % 256 != 0) return fail("%s: the workspace must lie on 256 bytes", what);
+    const int64_t rows = (int64_t)batch * queries * heads, states = (int64_t)batch * keys * kv_heads;
+    if (check_spans(what, {Span("dq", dq, rows * width, size), Span("dk", dk, states * width, size), Span("dv", dv, states * width, size),
+                           Span("the workspace", bytes ? workspace : nullptr, (int64_t)bytes, 1)},
+                    {span_of("dy", a.dy, batch, queries, heads, width, size), span_of("q", a.q, batch, queries, heads, width, size),
+                     span_of("k", a.k, batch, keys, kv_heads, width, size), span_of("v", a.v, batch, keys, kv_heads, width, size), Span("y", y, rows * width, size),
+                     Span("lse", lse, rows, size), Span("key_counts", counts, batch, 4)}, 0))
+        return DALI_HIP_ERROR;
+    if (ensure_init()) return DALI_HIP_ERROR;
+    return by_width(dtype, width, [&](auto t, auto d) { return backward<decltype(t), decltype(d)::value>(what, a); });
+}

@@ -1,0 +1,355 @@
+// Softmax cross entropy of rows against a large vocabulary, from the hidden states and the projection, and its gradients: the logits are never kept. Beyond the reference
+// (its softmax_cross_entropy takes logits).
+//
+// l = x w + bias; lse = m + ln S with the maximum m and S = sum e^(l - m); loss = (m - l_target) + ln S. The gradient of the logits is g = d (e^(l - lse) - [target]),
+// from which dx = g w^T, dw = x^T g, dbias = sum over the rows of g.
+//
+// The vocabulary is taken in pieces, the rows in blocks, so that a piece of logits holds at most kPieceBytes and stays in the 256 MiB cache between the product that
+// writes it and the kernel that reads it. Forward, every kSegment columns of a row leave a maximum and a sum of weights relative to it, and a last launch joins a
+// row's. Backward, the piece is formed again and becomes g in its place; the products add it up in the order of pieces and blocks.
+#include <algorithm>
+#include <cmath>
+
+#include "row_math.h"
+
+namespace dali_hip {
+namespace {
+
+template <typename T>
+struct Exponent;
+template <>
+struct Exponent<float> {
+    static constexpr float lowest = -3.402823466e+38f;  // where a running maximum begins: finite, so that no difference to it is NaN
+    static __device__ __forceinline__ float weight(float d) { return __builtin_amdgcn_exp2f(d * 1.44269504088896341f); }
+    static __device__ __forceinline__ float ln(float s) { return logf(s); }
+};
+template <>
+struct Exponent<double> {
+    static constexpr double lowest = -1.7976931348623157e+308;
+    static __device__ __forceinline__ double weight(double d) { return exp(d); }
+    static __device__ __forceinline__ double ln(double s) { return log(s); }
+};
+
+constexpr int kGroupsEach = 4;  // of a lane, in a segment
+template <typename T>
+constexpr int kSegment = 64 * kGroupsEach * Vec<T>::N;  // 1024 floats, 512 doubles
+constexpr int kChunkRows = 64;                          // that a workgroup of the gradient adds up for the bias
+constexpr size_t kPieceBytes = (size_t)128 << 20;
+constexpr int kMostRows = 16384;
+
+// How a call is cut, and what it keeps beside its operands
+template <typename T>
+struct Cut {
+    int64_t rows;
+    int inputs, vocab, block, piece, segments, chunks;
+    size_t logits = 0, maxima, sums, chosen, inputs_kept, columns, bytes;
+    Cut(int64_t rows_, int inputs_, int vocab_, bool backward, bool bias) : rows(rows_), inputs(inputs_), vocab(vocab_) {
+        const auto round = [](size_t b) { return (b + 255) / 256 * 256; };
+        block = (int)std::min<int64_t>(std::max<int64_t>(rows, 1), kMostRows);
+        const int64_t fits = (int64_t)(kPieceBytes / sizeof(T)) / block / kSegment<T> * kSegment<T>;  // columns
+        piece = (int)std::min<int64_t>(vocab, std::max<int64_t>(fits, kSegment<T>));
+        segments = (int)(((int64_t)vocab + kSegment<T> - 1) / kSegment<T>);
+        chunks = (block + kChunkRows - 1) / kChunkRows;
+        maxima = round((size_t)block * piece * sizeof(T));
+        sums = maxima + (backward ? 0 : round((size_t)block * segments * sizeof(T)));
+        chosen = sums + (backward ? 0 : round((size_t)block * segments * sizeof(T)));
+        inputs_kept = chosen + (backward ? 0 : round((size_t)block * sizeof(T)));
+        columns = inputs_kept + (backward ? round((size_t)block * inputs * sizeof(T)) : 0);
+        bytes = columns + (backward && bias ? round((size_t)chunks * piece * sizeof(T)) : 0);
+    }
+};
+
+// row-major C[m, n] = op(A) op(B) + beta C
+int product(bool ta, bool tb, int m, int n, int k, const float* a, int lda, const float* b, int ldb, float beta, float* c, int ldc) {
+    return dali_hip_sgemm(tb, ta, n, m, k, 1.0f, b, ldb, a, lda, beta, c, ldc);
+}
+int product(bool ta, bool tb, int m, int n, int k, const double* a, int lda, const double* b, int ldb, double beta, double* c, int ldc) {
+    return dali_hip_dgemm(tb, ta, n, m, k, 1.0, b, ldb, a, lda, beta, c, ldc);
+}
+
+// ------------------------------------------------------------------------------------------------ forward
+// A wave takes a segment of a row of the piece of logits that begins at column v0 of `width` columns.
+template <typename T>
+__global__ __launch_bounds__(256) void entropy_segments(const T* logits, int rows, int width, int v0, int segments, const T* bias, const int32_t* targets, int all, T* maxima,
+                                                        T* sums, T* chosen) {
+    constexpr int N = Vec<T>::N;
+    typedef Exponent<T> E;
+    const int here = (width + kSegment<T> - 1) / kSegment<T>, lane = threadIdx.x & 63;
+    const int64_t unit = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    const int row = (int)(unit / here), s = (int)(unit - (int64_t)row * here);
+    if (row >= rows) return;
+    const T* x = logits + (int64_t)row * width;
+    const int first = s * kSegment<T>;
+    T v[kGroupsEach][N];
+    typename Vec<T>::type g[kGroupsEach];
+#pragma unroll
+    for (int j = 0; j < kGroupsEach; ++j) {
+        const int c = first + (j * 64 + lane) * N;
+        if (c < width) g[j] = ask_group(x, c, width);
+    }
+    T top = E::lowest;
+    const int target = targets[row] - v0;
+#pragma unroll
+    for (int j = 0; j < kGroupsEach; ++j) {
+        const int c = first + (j * 64 + lane) * N;
+        if (c < width) {
+            take_group(g[j], c, width, T(-INFINITY), v[j]);
+            if (bias) {
+                T b[N];
+                load_group(bias, c, width, T(0), b);
+#pragma unroll
+                for (int e = 0; e < N; ++e) v[j][e] += b[e];
+            }
+            if (target >= c && target < c + N && target < width) {
+#pragma unroll
+                for (int e = 0; e < N; ++e)
+                    if (target == c + e) chosen[row] = v[j][e];
+            }
+        } else {
+#pragma unroll
+            for (int e = 0; e < N; ++e) v[j][e] = T(-INFINITY);
+        }
+#pragma unroll
+        for (int e = 0; e < N; ++e) top = Max()(top, v[j][e]);
+    }
+    top = fold_lanes<64>(top, Max());
+    T sum = 0;
+#pragma unroll
+    for (int j = 0; j < kGroupsEach; ++j)
+#pragma unroll
+        for (int e = 0; e < N; ++e) sum += E::weight(v[j][e] - top);
+    sum = fold_lanes<64>(sum, Sum());
+    if (lane == 0) {
+        const int64_t at = (int64_t)row * all + segments + s;
+        maxima[at] = top;
+        sums[at] = sum;
+    }
+}
+
+// A wave joins the segments of a row.
+template <typename T>
+__global__ __launch_bounds__(256) void entropy_join(const T* maxima, const T* sums, const T* chosen, const int32_t* targets, int rows, int segments, int vocab, T* losses, T* lse) {
+    typedef Exponent<T> E;
+    const int row = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
+    if (row >= rows) return;
+    const T *m = maxima + (int64_t)row * segments, *s = sums + (int64_t)row * segments;
+    T top = E::lowest, sum = 0;
+    for (int i = lane; i < segments; i += 64) {
+        const T next = Max()(top, m[i]);
+        sum = sum * E::weight(top - next) + s[i] * E::weight(m[i] - next);
+        top = next;
+    }
+    const T best = fold_lanes<64>(top, Max());
+    sum = fold_lanes<64>(sum * E::weight(top - best), Sum());
+    if (lane == 0) {
+        const T logarithm = E::ln(sum);
+        lse[row] = best + logarithm;
+        const int target = targets[row];
+        // (a row without weight leaves no probability for its target)
+        losses[row] = target < 0 || target >= vocab ? T(0) : sum == T(0) ? T(INFINITY) : (best - chosen[row]) + logarithm;
+    }
+}
+
+template <typename T>
+int cross_entropy(int64_t rows, int inputs, int vocab, const T* x, int64_t x_stride, const T* w, int64_t w_stride, bool w_by_columns, const T* bias, const int32_t* targets,
+                  T* losses, T* lse, char* space) {
+    const char* what = "dali_hip_projected_cross_entropy";
+    const Cut<T> cut(rows, inputs, vocab, false, bias != nullptr);
+    T *logits = (T*)(space + cut.logits), *maxima = (T*)(space + cut.maxima), *sums = (T*)(space + cut.sums), *chosen = (T*)(space + cut.chosen);
+    for (int64_t r = 0; r < rows; r += cut.block) {
+        const int n = (int)std::min<int64_t>(cut.block, rows - r);
+        for (int64_t v = 0; v < vocab; v += cut.piece) {
+            const int width = (int)std::min<int64_t>(cut.piece, vocab - v), here = (width + kSegment<T> - 1) / kSegment<T>;
+            if (product(false, w_by_columns, n, width, inputs, x + r * x_stride, (int)x_stride, w_by_columns ? w + v * w_stride : w + v, (int)w_stride, T(0), logits, width))
+                return DALI_HIP_ERROR;
+            entropy_segments<T><<<dim3((unsigned)(((int64_t)n * here + 3) / 4)), dim3(256), 0, stream()>>>(
+                logits, n, width, (int)v, (int)(v / kSegment<T>), bias ? bias + v : nullptr, targets + r, cut.segments, maxima, sums, chosen);
+            if (launched(what)) return DALI_HIP_ERROR;
+        }
+        entropy_join<T><<<dim3((unsigned)((n + 3) / 4)), dim3(256), 0, stream()>>>(maxima, sums, chosen, targets + r, n, cut.segments, vocab, losses + r, lse + r);
+        if (launched(what)) return DALI_HIP_ERROR;
+    }
+    return DALI_HIP_OK;
+}
+
+// ------------------------------------------------------------------------------------------------ backward
+// x with zeros in the rows that have no target, whatever those hold: they have no part in dw
+template <typename T>
+__global__ __launch_bounds__(256) void entropy_inputs(const T* x, int64_t x_stride, int inputs, const int32_t* targets, int vocab, T* kept) {
+    constexpr int N = Vec<T>::N;
+    const int row = blockIdx.x, target = targets[row];
+    const bool there = target >= 0 && target < vocab;
+    for (int c = threadIdx.x * N; c < inputs; c += 256 * N) {
+        T v[N] = {};
+        if (there) load_group(x + row * x_stride, c, inputs, T(0), v);
+        store_group(kept + (int64_t)row * inputs, c, inputs, v);
+    }
+}
+
+// A thread turns its group of columns of up to kChunkRows rows of logits into their gradient and adds up what that comes to.
+template <typename T>
+__global__ __launch_bounds__(256) void entropy_gradient(T* logits, int rows, int width, int v0, int vocab, const T* bias, const int32_t* targets, const T* lse, const T* d_losses,
+                                                        T* columns) {
+    constexpr int N = Vec<T>::N;
+    typedef Exponent<T> E;
+    const int c = (blockIdx.x * 256 + threadIdx.x) * N, r0 = blockIdx.y * kChunkRows, r1 = min(rows, r0 + kChunkRows);
+    if (c >= width) return;
+    T b[N] = {}, sum[N] = {};
+    if (bias) load_group(bias, c, width, T(0), b);
+    // (rows of a piece that end inside a group: a thread's group holds its own columns only, so that no other thread writes what it reads)
+    const bool whole = c + N <= width;
+    for (int r = r0; r < r1; ++r) {
+        T* x = logits + (int64_t)r * width;
+        T v[N];
+        if (whole) {
+            const typename Vec<T>::type g = *reinterpret_cast<const typename Vec<T>::type*>(x + c);
+#pragma unroll
+            for (int e = 0; e < N; ++e) v[e] = g[e];
+        } else {
+#pragma unroll
+            for (int e = 0; e < N; ++e) v[e] = c + e < width ? x[c + e] : T(0);
+        }
+        const int target = targets[r];
+        const T total = lse[r];
+        const T d = target >= 0 && target < vocab ? d_losses[r] : T(0);
+        // a row without a target has no gradient, nor one without weight
+        const bool none = target < 0 || target >= vocab || total == T(-INFINITY);
+#pragma unroll
+        for (int e = 0; e < N; ++e) {
+            const T p = E::weight(v[e] + b[e] - total) - (target == v0 + c + e ? T(1) : T(0));
+            v[e] = none ? T(0) : d * p;
+            sum[e] += v[e];
+        }
+        store_group(x, c, width, v);
+    }
+    if (columns) store_group(columns + (int64_t)blockIdx.y * width, c, width, sum);
+}
+
+template <typename T>
+__global__ __launch_bounds__(256) void entropy_bias(const T* columns, int chunks, int width, bool more, T* dbias) {
+    const int c = blockIdx.x * 256 + threadIdx.x;
+    if (c >= width) return;
+    T sum = more ? dbias[c] : T(0);
+    for (int i = 0; i < chunks; ++i) sum += columns[(int64_t)i * width + c];
+    dbias[c] = sum;
+}
+
+template <typename T>
+__global__ __launch_bounds__(256) void entropy_zeros(T* out, int64_t n) {
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) out[i] = T(0);
+}
+
+template <typename T>
+int cross_entropy_backward(int64_t rows, int inputs, int vocab, const T* d_losses, const T* x, int64_t x_stride, const T* w, int64_t w_stride, bool w_by_columns, const T* bias,
+                           const int32_t* targets, const T* lse, T* dx, T* dw, bool dw_by_columns, T* dbias, char* space) {
+    const char* what = "dali_hip_projected_cross_entropy_backward";
+    const Cut<T> cut(rows, inputs, vocab, true, dbias != nullptr);
+    T *g = (T*)(space + cut.logits), *kept = (T*)(space + cut.inputs_kept), *columns = dbias ? (T*)(space + cut.columns) : nullptr;
+    if (rows == 0) {  // (nothing is added up)
+        entropy_zeros<T><<<dim3(1024), dim3(256), 0, stream()>>>(dw, (int64_t)inputs * vocab);
+        if (!launched(what) && dbias) entropy_zeros<T><<<dim3(1024), dim3(256), 0, stream()>>>(dbias, (int64_t)vocab);
+        return launched(what);
+    }
+    for (int64_t r = 0; r < rows; r += cut.block) {
+        const int n = (int)std::min<int64_t>(cut.block, rows - r), chunks = (n + kChunkRows - 1) / kChunkRows;
+        entropy_inputs<T><<<dim3((unsigned)n), dim3(256), 0, stream()>>>(x + r * x_stride, x_stride, inputs, targets + r, vocab, kept);
+        if (launched(what)) return DALI_HIP_ERROR;
+        for (int64_t v = 0; v < vocab; v += cut.piece) {
+            const int width = (int)std::min<int64_t>(cut.piece, vocab - v);
+            const T* wp = w_by_columns ? w + v * w_stride : w + v;
+            if (product(false, w_by_columns, n, width, inputs, x + r * x_stride, (int)x_stride, wp, (int)w_stride, T(0), g, width)) return DALI_HIP_ERROR;
+            entropy_gradient<T><<<dim3((unsigned)((width + 256 * Vec<T>::N - 1) / (256 * Vec<T>::N)), (unsigned)chunks), dim3(256), 0, stream()>>>(
+                g, n, width, (int)v, vocab, bias ? bias + v : nullptr, targets + r, lse + r, d_losses + r, columns);
+            if (launched(what)) return DALI_HIP_ERROR;
+            if (product(false, !w_by_columns, n, inputs, width, g, width, wp, (int)w_stride, T(v > 0), dx + r * inputs, inputs)) return DALI_HIP_ERROR;
+            const T more = T(r > 0);
+            if (dw_by_columns ? product(true, false, width, inputs, n, g, width, kept, inputs, more, dw + v * inputs, inputs)
+                              : product(true, false, inputs, width, n, kept, inputs, g, width, more, dw + v, vocab))
+                return DALI_HIP_ERROR;
+            if (dbias) {
+                entropy_bias<T><<<dim3((unsigned)((width + 255) / 256)), dim3(256), 0, stream()>>>(columns, chunks, width, r > 0, dbias + v);
+                if (launched(what)) return DALI_HIP_ERROR;
+            }
+        }
+    }
+    return DALI_HIP_OK;
+}
+
+int check_extents(const char* what, int dtype, int64_t rows, int inputs, int vocab) {
+    if (!is_real(dtype)) return fail("%s: dtype %d is neither float nor double", what, dtype);
+    if (rows < 0 || rows > 2147483647LL) return fail("%s: %lld rows", what, (long long)rows);
+    if (inputs < 1) return fail("%s: rows of %d values", what, inputs);
+    if (vocab < 1 || vocab > 2147483647 - 4096) return fail("%s: a vocabulary of %d", what, vocab);
+    return DALI_HIP_OK;
+}
+
+int check_strides(const char* what, int64_t rows, int inputs, int vocab, int64_t& x_stride, int64_t w_stride, bool w_by_columns) {
+    if (rows <= 1) x_stride = inputs;
+    if (x_stride < inputs || x_stride > 2147483647LL) return fail("%s: rows of x are %lld values apart and %d long", what, (long long)x_stride, inputs);
+    if (w_stride < (w_by_columns ? inputs : vocab) || w_stride > 2147483647LL) return fail("%s: w's stride is %lld", what, (long long)w_stride);
+    return DALI_HIP_OK;
+}
+
+size_t space_of(int dtype, int64_t rows, int inputs, int vocab, bool backward, bool bias) {
+    return dtype == DALI_HIP_FLOAT ? Cut<float>(rows, inputs, vocab, backward, bias).bytes : Cut<double>(rows, inputs, vocab, backward, bias).bytes;
+}
+
+}  // namespace
+}  // namespace dali_hip
+
+using namespace dali_hip;
+
+extern "C" int dali_hip_projected_cross_entropy_workspace(int dtype, int64_t rows, int inputs, int vocab, int backward, int with_bias, size_t* bytes) {
+    const char* what = "dali_hip_projected_cross_entropy_workspace";
+    if (check_extents(what, dtype, rows, inputs, vocab)) return DALI_HIP_ERROR;
+    if (!bytes) return fail("%s: NULL argument", what);
+    *bytes = rows ? space_of(dtype, rows, inputs, vocab, backward != 0, with_bias != 0) : 0;
+    return DALI_HIP_OK;
+}
+
+extern "C" int dali_hip_projected_cross_entropy(int dtype, int64_t rows, int inputs, int vocab, const void* x, int64_t x_stride, const void* w, int64_t w_stride, int w_by_columns,
+                                                const void* bias, const int32_t* targets, void* losses, void* lse, void* workspace) {
+    const char* what = "dali_hip_projected_cross_entropy";
+    if (check_extents(what, dtype, rows, inputs, vocab)) return DALI_HIP_ERROR;
+    if (rows == 0) return DALI_HIP_OK;
+    if (!x || !w || !targets || !losses || !lse || !workspace) return fail("%s: NULL argument", what);
+    if (check_strides(what, rows, inputs, vocab, x_stride, w_stride, w_by_columns != 0)) return DALI_HIP_ERROR;
+    const size_t size = dtype == DALI_HIP_FLOAT ? 4 : 8;
+    if (off_elements({x, w, bias, losses, lse}, size) || off_elements({targets}, 4)) return fail("%s: an address is off its type's size", what);
+    if ((uintptr_t)workspace % 256 != 0) return fail("%s: the workspace must lie on 256 bytes", what);
+    if (check_spans(what, {Span("losses", losses, rows, size), Span("lse", lse, rows, size),
+                           Span("the workspace", workspace, (int64_t)space_of(dtype, rows, inputs, vocab, false, bias != nullptr), 1)},
+                    {Span("x", x, rows, inputs, x_stride, size), Span("w", w, w_by_columns ? vocab : inputs, w_by_columns ? inputs : vocab, w_stride, size),
+                     Span("bias", bias, vocab, size), Span("targets", targets, rows, 4)}, 0))
+        return DALI_HIP_ERROR;
+    if (ensure_init()) return DALI_HIP_ERROR;
+    return dtype == DALI_HIP_FLOAT ? cross_entropy(rows, inputs, vocab, (const float*)x, x_stride, (const float*)w, w_stride, w_by_columns != 0, (const float*)bias, targets,
+                                                   (float*)losses, (float*)lse, (char*)workspace)
+                                   : cross_entropy(rows, inputs, vocab, (const double*)x, x_stride, (const double*)w, w_stride, w_by_columns != 0, (const double*)bias, targets,
+                                                   (double*)losses, (double*)lse, (char*)workspace);
+}
+
+extern "C" int dali_hip_projected_cross_entropy_backward(int dtype, int64_t rows, int inputs, int vocab, const void* d_losses, const void* x, int64_t x_stride, const void* w,
+                                                         int64_t w_stride, int w_by_columns, const void* bias, const int32_t* targets, const void* lse, void* dx, void* dw,
+                                                         int dw_by_columns, void* dbias, void* workspace) {
+    const char* what = "dali_hip_projected_cross_entropy_backward";
+    if (check_extents(what, dtype, rows, inputs, vocab)) return DALI_HIP_ERROR;
+    if (!w || !dw || (rows && (!d_losses || !x || !targets || !lse || !dx || !workspace))) return fail("%s: NULL argument", what);
+    if (!bias != !dbias) return fail("%s: bias and dbias come together", what);
+    if (check_strides(what, rows, inputs, vocab, x_stride, w_stride, w_by_columns != 0)) return DALI_HIP_ERROR;
+    const size_t size = dtype == DALI_HIP_FLOAT ? 4 : 8;
+    if (off_elements({d_losses, x, w, bias, lse, dx, dw, dbias}, size) || off_elements({targets}, 4)) return fail("%s: an address is off its type's size", what);
+    if (rows && (uintptr_t)workspace % 256 != 0) return fail("%s: the workspace must lie on 256 bytes", what);
+    if (check_spans(what, {Span("dx", dx, rows * inputs, size), Span("dw", dw, (int64_t)inputs * vocab, size), Span("dbias", dbias, vocab, size),
+                           Span("the workspace", rows ? workspace : nullptr, (int64_t)space_of(dtype, rows, inputs, vocab, true, bias != nullptr), 1)},
+                    {Span("d_losses", d_losses, rows, size), Span("x", x, rows, inputs, x_stride, size),
+                     Span("w", w, w_by_columns ? vocab : inputs, w_by_columns ? inputs : vocab, w_stride, size), Span("bias", bias, vocab, size), Span("targets", targets, rows, 4),
+                     Span("lse", lse, rows, size)}, 0))
+        return DALI_HIP_ERROR;
+    if (ensure_init()) return DALI_HIP_ERROR;
+    return dtype == DALI_HIP_FLOAT
+               ? cross_entropy_backward(rows, inputs, vocab, (const float*)d_losses, (const float*)x, x_stride, (const float*)w, w_stride, w_by_columns != 0, (const float*)bias,
+                                        targets, (const float*)lse, (float*)dx, (float*)dw, dw_by_columns != 0, (float*)dbias, (char*)workspace)
+               : cross_entropy_backward(rows, inputs, vocab, (const double*)d_losses, (const double*)x, x_stride, (const double*)w, w_stride, w_by_columns != 0,
+                                        (const double*)bias, targets, (const double*)lse, (double*)dx, (double*)dw, dw_by_columns != 0, (double*)dbias, (char*)workspace);
+}

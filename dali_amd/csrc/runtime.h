@@ -46,6 +46,10 @@ class Carried {
 int bound_device();
 // sort.hip: looks up the device address of its built-in scratch array; called by dali_hip_init with `device` current
 int sort_scratch_init(int device);
+// sort.hip: dali_hip_argsort_i32 (n > 0, arguments checked) with a block of argsort_scratch_bytes(n) that the caller holds, so that nothing is allocated; nullptr: one
+// from the bank. Up to 16384 keys it uses the library workspace, within one launch.
+size_t argsort_scratch_bytes(int64_t n);
+int argsort_with(const int32_t* keys, int64_t n, int32_t key_limit, int32_t* sorted_keys, int32_t* perm, void* scratch);
 // sgemm_skinny.hip: row-major C[M, N] = alpha * A[M, K] . B[K, N] + beta * C for M <= 64 by streaming B once
 // (tb: B stored as [N][K]). 1: launched; 0: not a case for it (take the tiled kernels); -1: failure (message set)
 int sgemm_skinny(bool tb, int M, int N, int K, float alpha, const float* A, int lda, const float* B, int ldb, float beta, float* C, int ldc);

@@ -690,13 +690,14 @@ static bool argsort_arrays_overlap(const int32_t* keys, int64_t n, const int32_t
     return meet(keys, sorted_keys) || meet(keys, perm) || meet(sorted_keys, perm);
 }
 
-extern "C" int dali_hip_argsort_i32(const int32_t* keys, int64_t n, int32_t key_limit, int32_t* sorted_keys, int32_t* perm) {
-    if (ensure_init()) return DALI_HIP_ERROR;
-    if (n < 0) return fail("dali_hip_argsort_i32: negative length %lld", (long long)n);
-    if (n == 0) return DALI_HIP_OK;
-    if (n > 2147483647LL) return fail("dali_hip_argsort_i32: %lld keys exceed the int32 position range", (long long)n);
-    if (!keys || !sorted_keys || !perm) return fail("dali_hip_argsort_i32: NULL argument");
-    if (argsort_arrays_overlap(keys, n, sorted_keys, perm)) return fail("dali_hip_argsort_i32: keys, sorted_keys and perm must not overlap");
+namespace dali_hip {
+
+size_t argsort_scratch_bytes(int64_t n) {
+    const int rounds = radix_rounds(n), tiles = (int)((n + 256 * rounds - 1) / (256 * rounds));
+    return ((size_t)2 * (size_t)n + (size_t)256 * (size_t)tiles + 256) * sizeof(int32_t);
+}
+
+int argsort_with(const int32_t* keys, int64_t n, int32_t key_limit, int32_t* sorted_keys, int32_t* perm, void* scratch_block) {
     hipStream_t st = stream();
     // keys known to lie in [0, key_limit) need only their low bits sorted
     int end_bit = 32;
@@ -716,9 +717,8 @@ extern "C" int dali_hip_argsort_i32(const int32_t* keys, int64_t n, int32_t key_
     const int rounds = radix_rounds(n);
     const int passes = (end_bit + 7) / 8, tiles = (int)((n + 256 * rounds - 1) / (256 * rounds));
     const unsigned int flip = key_limit > 0 ? 0u : 0x80000000u, limit = key_limit > 0 ? (unsigned int)key_limit : 0u;
-    const size_t temp_bytes = ((size_t)2 * (size_t)n + (size_t)256 * (size_t)tiles + 256) * sizeof(int32_t);
-    void* temp = nullptr;
-    if (dali_hip_bank_allocate(&temp, temp_bytes)) return DALI_HIP_ERROR;
+    void* temp = scratch_block;
+    if (!temp && dali_hip_bank_allocate(&temp, argsort_scratch_bytes(n))) return DALI_HIP_ERROR;
     int32_t* tkeys = (int32_t*)temp;
     int32_t* tpos = tkeys + n;
     unsigned int* hist = (unsigned int*)(tpos + n);
@@ -737,8 +737,20 @@ extern "C" int dali_hip_argsort_i32(const int32_t* keys, int64_t n, int32_t key_
     hipError_t le = hipGetLastError();
     if (le != hipSuccess) status = fail("radix sort launch failed: %s", hipGetErrorString(le));
     // the block goes back to the bank at once: the next user of it is ordered behind the sort on the stream
-    dali_hip_bank_deposit(temp, temp_bytes);
+    if (!scratch_block) dali_hip_bank_deposit(temp, argsort_scratch_bytes(n));
     return status;
+}
+
+}  // namespace dali_hip
+
+extern "C" int dali_hip_argsort_i32(const int32_t* keys, int64_t n, int32_t key_limit, int32_t* sorted_keys, int32_t* perm) {
+    if (ensure_init()) return DALI_HIP_ERROR;
+    if (n < 0) return fail("dali_hip_argsort_i32: negative length %lld", (long long)n);
+    if (n == 0) return DALI_HIP_OK;
+    if (n > 2147483647LL) return fail("dali_hip_argsort_i32: %lld keys exceed the int32 position range", (long long)n);
+    if (!keys || !sorted_keys || !perm) return fail("dali_hip_argsort_i32: NULL argument");
+    if (argsort_arrays_overlap(keys, n, sorted_keys, perm)) return fail("dali_hip_argsort_i32: keys, sorted_keys and perm must not overlap");
+    return argsort_with(keys, n, key_limit, sorted_keys, perm, nullptr);
 }
 
 extern "C" int dali_hip_argsort_i32_noalloc(const int32_t* keys, int64_t n, int32_t key_limit, int32_t* sorted_keys, int32_t* perm) {

@@ -292,6 +292,33 @@ int dali_fe_token_log_probs_backward(dali_array_t d_log_probs, dali_array_t d_en
                                      dali_array_t* d_logits) {
     FE_TRY(deliver(d_logits, dali::op::token_log_probs_backward(A(d_log_probs), maybe(d_entropy), A(logits), A(tokens), A(lse), maybe(entropy), given(d_logits))); return 0;, 1)
 }
+int dali_fe_embedding(dali_array_t table, dali_array_t tokens, double scale, dali_array_t* y) {
+    FE_TRY(deliver(y, dali::op::embedding(A(table), A(tokens), scale, given(y))); return 0;, 1)
+}
+int dali_fe_embedding_backward(dali_array_t dy, dali_array_t tokens, int rows, double scale, dali_array_t* dtable) {
+    FE_TRY(deliver(dtable, dali::op::embedding_backward(A(dy), A(tokens), rows, scale, given(dtable))); return 0;, 1)
+}
+int dali_fe_cross_attention(dali_array_t queries, dali_array_t keys, dali_array_t values, dali_array_t key_counts, double scale, dali_array_t* y, dali_array_t* lse) {
+    FE_TRY(auto r = dali::op::cross_attention(A(queries), A(keys), A(values), maybe(key_counts), scale, {given(y), given(lse)}); deliver(y, r.y); deliver(lse, r.lse); return 0;
+           , 1)
+}
+int dali_fe_cross_attention_backward(dali_array_t dy, dali_array_t queries, dali_array_t keys, dali_array_t values, dali_array_t y, dali_array_t lse,
+                                     dali_array_t key_counts, double scale, dali_array_t* d_queries, dali_array_t* d_keys, dali_array_t* d_values) {
+    FE_TRY(auto r = dali::op::cross_attention_backward(A(dy), A(queries), A(keys), A(values), A(y), A(lse), maybe(key_counts), scale,
+                                                       {given(d_queries), given(d_keys), given(d_values)});
+           deliver(d_queries, r.queries); deliver(d_keys, r.keys); deliver(d_values, r.values); return 0;
+           , 1)
+}
+int dali_fe_projected_cross_entropy(dali_array_t x, dali_array_t w, dali_array_t targets, dali_array_t bias, dali_array_t* losses, dali_array_t* lse) {
+    FE_TRY(auto r = dali::op::projected_cross_entropy(A(x), A(w), A(targets), maybe(bias), {given(losses), given(lse)}); deliver(losses, r.losses); deliver(lse, r.lse); return 0;
+           , 1)
+}
+int dali_fe_projected_cross_entropy_backward(dali_array_t d_losses, dali_array_t x, dali_array_t w, dali_array_t targets, dali_array_t lse, dali_array_t bias,
+                                             dali_array_t* dx, dali_array_t* dw, dali_array_t* dbias) {
+    FE_TRY(auto r = dali::op::projected_cross_entropy_backward(A(d_losses), A(x), A(w), A(targets), A(lse), maybe(bias), {given(dx), given(dw), given(dbias)});
+           deliver(dx, r.x); deliver(dw, r.w); deliver(dbias, r.bias); return 0;
+           , 1)
+}
 int dali_fe_clip_by_global_norm(const dali_array_t* arrays, int count, double max_norm, dali_array_t* clipped, dali_array_t* norm) {
     FE_TRY(std::vector<Array> in; for (int i = 0; i < count; ++i) in.push_back(A(arrays[i]));
            if (!clipped) { deliver(norm, dali::op::global_norm(in, given(norm))); return 0; }

@@ -421,6 +421,36 @@ struct ClippedArrays {
     Array norm;
 };
 ClippedArrays clip_by_global_norm(const std::vector<Array>& arrays, double max_norm, const ClippedArrays& out = ClippedArrays());
+
+// scale * table[token] for every token, [tokens' shape, width]; a token outside the table gives zeros
+Array embedding(const Array& table, const Array& tokens, double scale = 1.0, const Array& out = Array());
+// the gradient of a table of `rows` rows, written whole
+Array embedding_backward(const Array& dy, const Array& tokens, int rows, double scale = 1.0, const Array& out = Array());
+// Attention of queries [batch, positions, heads, width] to keys and values [batch, states, shared heads, width] of another length, of which sequence b has key_counts[b] (int32
+// [batch]; stateless: all). Heads are shared by neighbours. y has the queries' shape, lse [batch, positions, heads]; a row without states has y = 0, lse = -inf.
+struct Attention {
+    Array y, lse;
+};
+Attention cross_attention(const Array& queries, const Array& keys, const Array& values, const Array& key_counts, double scale, const Attention& out = Attention());
+// the gradients from dy, that of y, dense in the shapes of their operands; zeros for states behind a sequence's last
+struct AttentionGradient {
+    Array queries, keys, values;
+};
+AttentionGradient cross_attention_backward(const Array& dy, const Array& queries, const Array& keys, const Array& values, const Array& y, const Array& lse,
+                                           const Array& key_counts, double scale, const AttentionGradient& out = AttentionGradient());
+// Softmax cross entropy of x [..., inputs] against logits x w + bias (w [inputs, vocab], or a transposed view of [vocab, inputs]; bias [vocab] or stateless) that are not kept:
+// losses and lse in the shape of the targets. A target outside [0, vocab) stands for none: loss 0, no gradient.
+struct ProjectedCrossEntropy {
+    Array losses, lse;
+};
+ProjectedCrossEntropy projected_cross_entropy(const Array& x, const Array& w, const Array& targets, const Array& bias = Array(),
+                                              const ProjectedCrossEntropy& out = ProjectedCrossEntropy());
+// the gradients from d_losses and lse; w's lies in memory as w does (a destination: a dense buffer or the transposition of one), a stateless bias has none
+struct ProjectedCrossEntropyGradient {
+    Array x, w, bias;
+};
+ProjectedCrossEntropyGradient projected_cross_entropy_backward(const Array& d_losses, const Array& x, const Array& w, const Array& targets, const Array& lse,
+                                                               const Array& bias = Array(), const ProjectedCrossEntropyGradient& out = ProjectedCrossEntropyGradient());
 }  // namespace op
 
 // Named scopes (dali/utils/scope.h:11-34): DALI_SCOPE(name) opens a scope that lasts to the end of the block when

@@ -1,6 +1,9 @@
 // Operators that language models are trained, scored and answered with, over the library's own kernels: layer normalisation, log probabilities of
-// tokens, clipping by the global norm. They are evaluated when called, as the composites of array.cpp are, write into new arrays or into
+// tokens, clipping by the global norm, embedding rows, attention to an encoder's states, cross entropy of a projection. They are evaluated when called, as the composites of array.cpp are, write into new arrays or into
 // destinations that the caller keeps, and record themselves like any other launch.
+#include <array>
+#include <cmath>
+
 #include "../../include/dali_hip.h"
 #include "jit_internal.h"
 
@@ -61,6 +64,65 @@ Array destination(const char* what, const char* name, const Array& given, const 
     check_shape(what, name, given, shape, dtype);
     DALI_ASSERT(given.is_buffer() && given.contiguous_memory(), make_message(what, ": the destination of ", name, " must be a dense buffer"));
     return given;
+}
+
+// what an entry of the library keeps beside its operands for the time of a call (or as long as a recording holds it)
+template <typename Bytes>
+Array workspace(const char* what, const Bytes& bytes) {
+    size_t n = 0;
+    check_hip(bytes(&n), what);
+    if (n == 0) return Array();
+    DALI_ASSERT(n / 8 < 2147483647u, make_message(what, ": a workspace of ", n, " bytes"));
+    return Array({(int)(n / 8) + 1}, DTYPE_DOUBLE);
+}
+
+// the operand [batch, rows, heads, width] with the strides of its first three axes: a view whose last axis is dense is read where it lies
+struct Heads {
+    Array array;
+    std::array<int64_t, 3> strides;
+};
+
+Heads as_heads(const Array& a) {
+    a.eval();
+    Heads h;
+    h.array = a;
+    const std::vector<int>& shape = a.shape();
+    if (!a.contiguous_memory()) {
+        const std::vector<int> st = a.normalized_strides();
+        if (shape[3] == 1 || st[3] == 1) {
+            h.strides = {st[0], st[1], st[2]};
+            return h;
+        }
+        h.array = a.ascontiguousarray();
+    }
+    h.strides = {(int64_t)shape[1] * shape[2] * shape[3], (int64_t)shape[2] * shape[3], shape[3]};
+    return h;
+}
+
+// a matrix as the products take it: rows `stride` apart, or (by_columns) its transposition's
+struct Projection {
+    Array array;
+    int64_t stride = 0;
+    bool by_columns = false;
+};
+
+Projection as_projection(const Array& w) {
+    w.eval();
+    Projection p;
+    p.array = w;
+    const int rows = w.shape()[0], cols = w.shape()[1];
+    p.stride = cols;
+    if (w.contiguous_memory()) return p;
+    const std::vector<int> st = w.normalized_strides();
+    if (st[1] == 1 && st[0] >= cols) {
+        p.stride = st[0];
+    } else if (st[0] == 1 && st[1] >= rows) {
+        p.by_columns = true;
+        p.stride = st[1];
+    } else {
+        p.array = w.ascontiguousarray();
+    }
+    return p;
 }
 
 const void* read(const Array& a) { return a.is_stateless() ? nullptr : a.device_ptr(); }
@@ -198,6 +260,204 @@ Array token_log_probs_backward(const Array& d_log_probs, const Array& d_entropy,
     issue(
         what, [=]() { return dali_hip_token_log_probs_backward(dtype, rows, vocab, gp, hp, xp, stride, (const int32_t*)tp, lp, ep, rp); },
         [&](std::vector<Array>& reads, std::vector<Array>& writes) { reads = {in.array, g, t, l, h, e}, writes = {r}; });
+    return r;
+}
+
+Array embedding(const Array& table, const Array& tokens, double scale, const Array& out) {
+    const char* what = "embedding";
+    DALI_ASSERT(table.ndim() == 2 && is_real(table) && table.shape()[0] >= 1 && table.shape()[1] >= 1,
+                make_message(what, ": the table must be a float or double matrix that is not empty"));
+    DALI_ASSERT(tokens.dtype() == DTYPE_INT32, make_message(what, ": tokens must be int"));
+    DALI_ASSERT(std::isfinite(scale), make_message(what, ": the scale must be finite (got ", scale, ")"));
+    const DType dtype = table.dtype();
+    std::vector<int> shape = tokens.shape();
+    shape.push_back(table.shape()[1]);
+    const Array y = destination(what, "y", out, shape, dtype);
+    const Rows in = as_rows(table);
+    const Array t = dense(tokens);
+    if (g_dry_run) return y;
+    const void *xp = read(in.array), *tp = read(t);
+    void* yp = write(y);
+    const int64_t count = t.number_of_elements(), stride = in.stride;
+    const int rows = table.shape()[0], width = in.width;
+    issue(
+        what, [=]() { return dali_hip_embedding(dtype, count, rows, width, xp, stride, (const int32_t*)tp, scale, yp); },
+        [&](std::vector<Array>& reads, std::vector<Array>& writes) { reads = {in.array, t}, writes = {y}; });
+    return y;
+}
+
+Array embedding_backward(const Array& dy, const Array& tokens, int rows, double scale, const Array& out) {
+    const char* what = "embedding_backward";
+    DALI_ASSERT(dy.ndim() >= 1 && is_real(dy) && dy.shape().back() >= 1, make_message(what, ": dy must be float or double and have a last axis that is not empty"));
+    check_shape(what, "tokens", tokens, leading(dy), DTYPE_INT32);
+    DALI_ASSERT(rows >= 1, make_message(what, ": a table has at least one row (got ", rows, ")"));
+    DALI_ASSERT(std::isfinite(scale), make_message(what, ": the scale must be finite (got ", scale, ")"));
+    const DType dtype = dy.dtype();
+    const int width = dy.shape().back();
+    const Array r = destination(what, "dtable", out, {rows, width}, dtype);
+    const Rows in = as_rows(dy);
+    const Array t = dense(tokens);
+    const int64_t count = t.number_of_elements(), stride = in.stride;
+    const Array space = workspace(what, [&](size_t* n) { return dali_hip_embedding_backward_workspace(dtype, count, rows, width, n); });
+    if (g_dry_run) return r;
+    const void *xp = count ? read(in.array) : nullptr, *tp = count ? read(t) : nullptr;
+    void *rp = write(r), *sp = write(space);
+    issue(
+        what, [=]() { return dali_hip_embedding_backward(dtype, count, rows, width, xp, stride, (const int32_t*)tp, scale, rp, sp); },
+        [&](std::vector<Array>& reads, std::vector<Array>& writes) { reads = {in.array, t}, writes = {r, space}; });
+    return r;
+}
+
+// what both directions of attention ask of their operands; the sizes that the entries take
+struct AttentionSizes {
+    DType dtype;
+    int batch, queries, keys, heads, kv_heads, width;
+    AttentionSizes(const char* what, const Array& q, const Array& k, const Array& v, const Array& counts, double scale) {
+        DALI_ASSERT(q.ndim() == 4 && is_real(q), make_message(what, ": queries must be float or double of shape [batch, positions, heads, width]"));
+        dtype = q.dtype();
+        batch = q.shape()[0], queries = q.shape()[1], heads = q.shape()[2], width = q.shape()[3];
+        DALI_ASSERT(width >= 1 && width <= DALI_HIP_MAX_HEAD_WIDTH, make_message(what, ": heads are from 1 to ", DALI_HIP_MAX_HEAD_WIDTH, " wide (got ", width, ")"));
+        DALI_ASSERT(k.ndim() == 4 && k.dtype() == dtype && k.shape()[0] == batch && k.shape()[3] == width,
+                    make_message(what, ": keys must be ", dtype_to_cpp_name(dtype), " of shape [", batch, ", states, shared heads, ", width, "], got ", dtype_to_cpp_name(k.dtype()), " of shape ",
+                                 shape_str(k.shape())));
+        keys = k.shape()[1], kv_heads = k.shape()[2];
+        check_shape(what, "values", v, k.shape(), dtype);
+        DALI_ASSERT(heads >= 1 && kv_heads >= 1 && heads % kv_heads == 0, make_message(what, ": ", heads, " heads cannot share ", kv_heads));
+        if (!counts.is_stateless()) check_shape(what, "key_counts", counts, {batch}, DTYPE_INT32);
+        DALI_ASSERT(std::isfinite(scale), make_message(what, ": the scale must be finite (got ", scale, ")"));
+    }
+};
+
+Attention cross_attention(const Array& queries, const Array& keys, const Array& values, const Array& key_counts, double scale, const Attention& out) {
+    const char* what = "cross_attention";
+    const AttentionSizes z(what, queries, keys, values, key_counts, scale);
+    const std::vector<int> rows = leading(queries);
+    Attention r = {destination(what, "y", out.y, queries.shape(), z.dtype), destination(what, "lse", out.lse, rows, z.dtype)};
+    const Heads q = as_heads(queries), k = as_heads(keys), v = as_heads(values);
+    const Array n = key_counts.is_stateless() ? key_counts : dense(key_counts);
+    const Array space = workspace(
+        what, [&](size_t* bytes) { return dali_hip_cross_attention_workspace(z.dtype, z.batch, z.queries, z.keys, z.heads, z.kv_heads, z.width, 0, bytes); });
+    if (g_dry_run) return r;
+    const void *qp = read(q.array), *kp = read(k.array), *vp = read(v.array), *np = read(n);
+    void *yp = write(r.y), *lp = write(r.lse), *sp = write(space);
+    const auto qs = q.strides, ks = k.strides, vs = v.strides;
+    issue(
+        what,
+        [=]() {
+            return dali_hip_cross_attention(z.dtype, z.batch, z.queries, z.keys, z.heads, z.kv_heads, z.width, qp, qs.data(), kp, ks.data(), vp, vs.data(),
+                                            (const int32_t*)np, scale, yp, lp, sp);
+        },
+        [&](std::vector<Array>& reads, std::vector<Array>& writes) { reads = {q.array, k.array, v.array, n}, writes = {r.y, r.lse, space}; });
+    return r;
+}
+
+AttentionGradient cross_attention_backward(const Array& dy, const Array& queries, const Array& keys, const Array& values, const Array& y, const Array& lse,
+                                           const Array& key_counts, double scale, const AttentionGradient& out) {
+    const char* what = "cross_attention_backward";
+    const AttentionSizes z(what, queries, keys, values, key_counts, scale);
+    check_shape(what, "dy", dy, queries.shape(), z.dtype);
+    check_shape(what, "y", y, queries.shape(), z.dtype);
+    check_shape(what, "lse", lse, leading(queries), z.dtype);
+    AttentionGradient r = {destination(what, "d_queries", out.queries, queries.shape(), z.dtype), destination(what, "d_keys", out.keys, keys.shape(), z.dtype),
+                           destination(what, "d_values", out.values, keys.shape(), z.dtype)};
+    const Heads g = as_heads(dy), q = as_heads(queries), k = as_heads(keys), v = as_heads(values);
+    const Array yd = dense(y), l = dense(lse), n = key_counts.is_stateless() ? key_counts : dense(key_counts);
+    const Array space = workspace(
+        what, [&](size_t* bytes) { return dali_hip_cross_attention_workspace(z.dtype, z.batch, z.queries, z.keys, z.heads, z.kv_heads, z.width, 1, bytes); });
+    if (g_dry_run) return r;
+    const void *gp = read(g.array), *qp = read(q.array), *kp = read(k.array), *vp = read(v.array), *yp = read(yd), *lp = read(l), *np = read(n);
+    void *dqp = write(r.queries), *dkp = write(r.keys), *dvp = write(r.values), *sp = write(space);
+    const auto gs = g.strides, qs = q.strides, ks = k.strides, vs = v.strides;
+    issue(
+        what,
+        [=]() {
+            return dali_hip_cross_attention_backward(z.dtype, z.batch, z.queries, z.keys, z.heads, z.kv_heads, z.width, gp, gs.data(), qp, qs.data(), kp, ks.data(), vp,
+                                                     vs.data(), yp, lp, (const int32_t*)np, scale, dqp, dkp, dvp, sp);
+        },
+        [&](std::vector<Array>& reads, std::vector<Array>& writes) {
+            reads = {g.array, q.array, k.array, v.array, yd, l, n}, writes = {r.queries, r.keys, r.values, space};
+        });
+    return r;
+}
+
+// rows of x as a product takes them: whole rows one after the other
+static Rows as_whole_rows(const Array& x) {
+    Rows r = as_rows(x);
+    if (r.rows > 1 && r.stride < r.width) {
+        r.array = x.ascontiguousarray();
+        r.stride = r.width;
+    }
+    return r;
+}
+
+static void check_projection(const char* what, const Array& x, const Array& w, const Array& targets, const Array& bias) {
+    DALI_ASSERT(x.ndim() >= 1 && is_real(x) && x.shape().back() >= 1, make_message(what, ": x must be float or double and have a last axis that is not empty"));
+    const int inputs = x.shape().back();
+    DALI_ASSERT(w.ndim() == 2 && w.dtype() == x.dtype() && w.shape()[0] == inputs && w.shape()[1] >= 1,
+                make_message(what, ": w must be ", dtype_to_cpp_name(x.dtype()), " of shape [", inputs, ", vocabulary], got ", dtype_to_cpp_name(w.dtype()), " of shape ",
+                             shape_str(w.shape())));
+    check_shape(what, "targets", targets, leading(x), DTYPE_INT32);
+    if (!bias.is_stateless()) check_shape(what, "bias", bias, {w.shape()[1]}, x.dtype());
+}
+
+ProjectedCrossEntropy projected_cross_entropy(const Array& x, const Array& w, const Array& targets, const Array& bias, const ProjectedCrossEntropy& out) {
+    const char* what = "projected_cross_entropy";
+    check_projection(what, x, w, targets, bias);
+    const DType dtype = x.dtype();
+    ProjectedCrossEntropy r = {destination(what, "losses", out.losses, leading(x), dtype), destination(what, "lse", out.lse, leading(x), dtype)};
+    const Rows in = as_whole_rows(x);
+    const Projection p = as_projection(w);
+    const Array t = dense(targets), b = bias.is_stateless() ? bias : dense(bias);
+    const int64_t rows = in.rows, stride = in.stride, w_stride = p.stride;
+    const int inputs = in.width, vocab = w.shape()[1], by_columns = p.by_columns;
+    const Array space =
+        workspace(what, [&](size_t* n) { return dali_hip_projected_cross_entropy_workspace(dtype, rows, inputs, vocab, 0, !b.is_stateless(), n); });
+    if (g_dry_run) return r;
+    const void *xp = read(in.array), *wp = read(p.array), *tp = read(t), *bp = read(b);
+    void *op = write(r.losses), *lp = write(r.lse), *sp = write(space);
+    issue(
+        what,
+        [=]() { return dali_hip_projected_cross_entropy(dtype, rows, inputs, vocab, xp, stride, wp, w_stride, by_columns, bp, (const int32_t*)tp, op, lp, sp); },
+        [&](std::vector<Array>& reads, std::vector<Array>& writes) { reads = {in.array, p.array, t, b}, writes = {r.losses, r.lse, space}; });
+    return r;
+}
+
+ProjectedCrossEntropyGradient projected_cross_entropy_backward(const Array& d_losses, const Array& x, const Array& w, const Array& targets, const Array& lse,
+                                                               const Array& bias, const ProjectedCrossEntropyGradient& out) {
+    const char* what = "projected_cross_entropy_backward";
+    check_projection(what, x, w, targets, bias);
+    const DType dtype = x.dtype();
+    check_shape(what, "d_losses", d_losses, leading(x), dtype);
+    check_shape(what, "lse", lse, leading(x), dtype);
+    DALI_ASSERT(!bias.is_stateless() || out.bias.is_stateless(), make_message(what, ": without bias there is no gradient of it to write"));
+    const Projection p = as_projection(w);
+    ProjectedCrossEntropyGradient r;
+    r.x = destination(what, "dx", out.x, x.shape(), dtype);
+    bool dw_by_columns = p.by_columns;
+    if (out.w.is_stateless()) {
+        r.w = p.by_columns ? Array({w.shape()[1], w.shape()[0]}, dtype).transpose() : Array(w.shape(), dtype);
+    } else {
+        check_shape(what, "dw", out.w, w.shape(), dtype);
+        dw_by_columns = out.w.is_buffer() && !out.w.contiguous_memory() && out.w.transpose().contiguous_memory();
+        r.w = dw_by_columns ? out.w : destination(what, "dw", out.w, w.shape(), dtype);
+    }
+    if (!bias.is_stateless()) r.bias = destination(what, "dbias", out.bias, {w.shape()[1]}, dtype);
+    const Rows in = as_whole_rows(x);
+    const Array g = dense(d_losses), t = dense(targets), l = dense(lse), b = bias.is_stateless() ? bias : dense(bias);
+    const int64_t rows = in.rows, stride = in.stride, w_stride = p.stride;
+    const int inputs = in.width, vocab = w.shape()[1], by_columns = p.by_columns, dw_columns = dw_by_columns;
+    const Array space =
+        workspace(what, [&](size_t* n) { return dali_hip_projected_cross_entropy_workspace(dtype, rows, inputs, vocab, 1, !b.is_stateless(), n); });
+    if (g_dry_run) return r;
+    const void *gp = read(g), *xp = read(in.array), *wp = read(p.array), *tp = read(t), *lp = read(l), *bp = read(b);
+    void *dxp = write(r.x), *dwp = write(r.w), *dbp = write(r.bias), *sp = write(space);
+    issue(
+        what,
+        [=]() {
+            return dali_hip_projected_cross_entropy_backward(dtype, rows, inputs, vocab, gp, xp, stride, wp, w_stride, by_columns, bp, (const int32_t*)tp, lp, dxp, dwp,
+                                                             dw_columns, dbp, sp);
+        },
+        [&](std::vector<Array>& reads, std::vector<Array>& writes) { reads = {g, in.array, p.array, t, l, b}, writes = {r.x, r.w, r.bias, space}; });
     return r;
 }
 

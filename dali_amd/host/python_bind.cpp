@@ -496,6 +496,100 @@ PyObject* f_token_log_probs_backward(PyObject*, PyObject* const* args, Py_ssize_
     return d;
 }
 
+// a call whose one result may have a destination (an array or None)
+template <typename Call>
+PyObject* one_result(const char* what, PyObject* given, const Call& call) {
+    Destinations out;
+    PyObject* one = PyTuple_Pack(1, given);
+    const bool ok = one && out.set(one, 1, what);
+    Py_XDECREF(one);
+    if (!ok) return nullptr;
+    const int status = unlocked([&] { return call(&out.handles[0]); });
+    PyObject* t = status != 0 ? fail(what) : out.results(what);
+    if (!t) return nullptr;
+    PyObject* d = PyTuple_GET_ITEM(t, 0);
+    Py_INCREF(d);
+    Py_DECREF(t);
+    return d;
+}
+
+// table, tokens, scale, out (one array or None)
+PyObject* f_embedding(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    Operand table, tokens;
+    double scale;
+    if (!count_is(n, 4, "embedding") || !table.set(args[0]) || !tokens.set(args[1]) || !number(args[2], &scale)) return nullptr;
+    return one_result("embedding", args[3], [&](dali_array_t* r) { return dali_fe_embedding(table.handle, tokens.handle, scale, r); });
+}
+
+// dy, tokens, rows, scale, out (one array or None)
+PyObject* f_embedding_backward(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    Operand dy, tokens;
+    double scale;
+    if (!count_is(n, 5, "embedding_backward") || !dy.set(args[0]) || !tokens.set(args[1]) || !number(args[3], &scale)) return nullptr;
+    int too_large = 0;
+    const long asked = PyLong_AsLongAndOverflow(args[2], &too_large);  // (a count that is not one of an int is refused, not cut)
+    if (asked == -1 && PyErr_Occurred()) return nullptr;
+    const int rows = too_large || asked != (int)asked ? -1 : (int)asked;
+    return one_result("embedding_backward", args[4], [&](dali_array_t* r) { return dali_fe_embedding_backward(dy.handle, tokens.handle, rows, scale, r); });
+}
+
+// queries, keys, values, key_counts, scale, out
+PyObject* f_cross_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    const char* what = "cross_attention";
+    Operand q, k, v, counts;
+    Destinations out;
+    double scale;
+    if (!count_is(n, 6, what) || !q.set(args[0]) || !k.set(args[1]) || !v.set(args[2]) || !optional(counts, args[3]) || !number(args[4], &scale) || !out.set(args[5], 2, what))
+        return nullptr;
+    dali_array_t* r = out.handles.data();
+    const int status = unlocked([&] { return dali_fe_cross_attention(q.handle, k.handle, v.handle, counts.handle, scale, &r[0], &r[1]); });
+    return status != 0 ? fail(what) : out.results(what);
+}
+
+// dy, queries, keys, values, y, lse, key_counts, scale, out
+PyObject* f_cross_attention_backward(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    const char* what = "cross_attention_backward";
+    Operand a[6], counts;
+    Destinations out;
+    double scale;
+    if (!count_is(n, 9, what)) return nullptr;
+    for (int i = 0; i < 6; ++i)
+        if (!a[i].set(args[i])) return nullptr;
+    if (!optional(counts, args[6]) || !number(args[7], &scale) || !out.set(args[8], 3, what)) return nullptr;
+    dali_array_t* r = out.handles.data();
+    const int status = unlocked([&] {
+        return dali_fe_cross_attention_backward(a[0].handle, a[1].handle, a[2].handle, a[3].handle, a[4].handle, a[5].handle, counts.handle, scale, &r[0], &r[1], &r[2]);
+    });
+    return status != 0 ? fail(what) : out.results(what);
+}
+
+// x, w, targets, bias, out
+PyObject* f_projected_cross_entropy(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    const char* what = "projected_cross_entropy";
+    Operand x, w, targets, bias;
+    Destinations out;
+    if (!count_is(n, 5, what) || !x.set(args[0]) || !w.set(args[1]) || !targets.set(args[2]) || !optional(bias, args[3]) || !out.set(args[4], 2, what)) return nullptr;
+    dali_array_t* r = out.handles.data();
+    const int status = unlocked([&] { return dali_fe_projected_cross_entropy(x.handle, w.handle, targets.handle, bias.handle, &r[0], &r[1]); });
+    return status != 0 ? fail(what) : out.results(what);
+}
+
+// d_losses, x, w, targets, lse, bias, out
+PyObject* f_projected_cross_entropy_backward(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    const char* what = "projected_cross_entropy_backward";
+    Operand a[5], bias;
+    Destinations out;
+    if (!count_is(n, 7, what)) return nullptr;
+    for (int i = 0; i < 5; ++i)
+        if (!a[i].set(args[i])) return nullptr;
+    if (!optional(bias, args[5]) || !out.set(args[6], 3, what)) return nullptr;
+    dali_array_t* r = out.handles.data();
+    const int status = unlocked([&] {
+        return dali_fe_projected_cross_entropy_backward(a[0].handle, a[1].handle, a[2].handle, a[3].handle, a[4].handle, bias.handle, &r[0], &r[1], &r[2]);
+    });
+    return status != 0 ? fail(what) : out.results(what);
+}
+
 // arrays, max_norm (None: the norm alone), destinations of the arrays, destination of the norm -> (tuple of arrays, norm), or the norm
 PyObject* f_clip_by_global_norm(PyObject*, PyObject* const* args, Py_ssize_t n) {
     const char* what = "clip_by_global_norm";
@@ -540,6 +634,8 @@ PyMethodDef functions[] = {FUNCTION(register),        FUNCTION(unary),     FUNCT
                            FUNCTION(transpose),       FUNCTION(assign),    FUNCTION(softmax_cross_entropy),         FUNCTION(lstm_step),
                            FUNCTION(layer_norm),      FUNCTION(layer_norm_backward),   FUNCTION(token_log_probs),    FUNCTION(token_log_probs_backward),
                            FUNCTION(clip_by_global_norm),
+                           FUNCTION(embedding),       FUNCTION(embedding_backward),    FUNCTION(cross_attention),    FUNCTION(cross_attention_backward),
+                           FUNCTION(projected_cross_entropy),                          FUNCTION(projected_cross_entropy_backward),
                            {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_bind", nullptr, -1, functions, nullptr, nullptr, nullptr, nullptr};
 

@@ -258,6 +258,51 @@ def clip_by_global_norm(arrays, max_norm, out=None):
     return _bind.clip_by_global_norm(arrays, float(max_norm), destinations, norm)
 
 
+def embedding(table, tokens, scale=1.0, out=None):
+    """scale * table[token] for int32 tokens of any shape: [tokens' shape, width]. A token outside the table (-1, say, for padding) gives a row of zeros."""
+    return _bind.embedding(table, tokens, float(scale), out)
+
+
+def embedding_backward(dy, tokens, rows, scale=1.0, out=None):
+    """The gradient [rows, width] of a table from dy, that of ``embedding``: scale times the sum of the rows of dy whose token names a row, in their order, zeros where none
+    does. It is written whole; tokens outside the table have no part in it."""
+    return _bind.embedding_backward(dy, tokens, rows, float(scale), out)
+
+
+def _attention_scale(queries, scale):
+    return 1.0 / queries.shape[-1] ** 0.5 if scale is None and queries.shape and queries.shape[-1] else 1.0 if scale is None else float(scale)
+
+
+def cross_attention(queries, keys, values, key_counts=None, scale=None, out=None):
+    """(y, lse) of the attention of queries [batch, positions, heads, width] to the keys and values [batch, states, shared heads, width] of an encoder, of another length:
+    y = softmax(scale * q.k) v in the shape of the queries, lse [batch, positions, heads] the logarithm of the sum of the exponentials, which the gradient needs. Neighbouring
+    heads share keys and values where there are fewer of them. key_counts (int32 [batch], None: all) says how many states each sequence has (held inside
+    [0, states]); what lies behind them is not read. A row without states has y = 0 and lse = -inf. scale None: 1 / sqrt(width). Heads are at most 256 wide. Views whose
+    last axis is dense are read where they lie, [batch, heads, positions, width] as its transposition (0, 2, 1, 3)."""
+    queries = as_array(queries)
+    return _bind.cross_attention(queries, keys, values, key_counts, _attention_scale(queries, scale), out)
+
+
+def cross_attention_backward(dy, queries, keys, values, y, lse, key_counts=None, scale=None, out=None):
+    """(d_queries, d_keys, d_values) from dy, the gradient of y, and the y and lse that ``cross_attention`` left. States behind a sequence's last get zeros. Sums are formed in
+    an order that depends on the shapes and counts alone."""
+    queries = as_array(queries)
+    return _bind.cross_attention_backward(dy, queries, keys, values, y, lse, key_counts, _attention_scale(queries, scale), out)
+
+
+def projected_cross_entropy(x, w, targets, bias=None, out=None):
+    """(losses, lse) of the softmax cross entropy of x [..., inputs] against the logits x w + bias over a large vocabulary, whose logits are formed in pieces and not kept:
+    losses = lse - logit[target], in the shape of the targets (int32). w is [inputs, vocab] or a transposed view of a [vocab, inputs] table, which is read where it lies.
+    A target outside the vocabulary (-1, say) stands for none: loss 0. A logit of -inf has probability 0; a row of nothing else has lse = -inf and loss +inf."""
+    return _bind.projected_cross_entropy(x, w, targets, bias, out)
+
+
+def projected_cross_entropy_backward(d_losses, x, w, targets, lse, bias=None, out=None):
+    """(dx, dw, dbias) from d_losses and the lse that ``projected_cross_entropy`` left; without bias, dbias is None. A row without a target has no part in them, whatever it
+    holds, nor has a row whose logits are all -inf. dw lies in memory as w does: where w is a transposed view, its destination may be one too."""
+    return _bind.projected_cross_entropy_backward(d_losses, x, w, targets, lse, bias, out)
+
+
 def lstm_step(x, h, c, W, U, b):
     """One LSTM cell step; returns (c', h') already evaluated."""
     return _bind.lstm_step(x, h, c, W, U, b)

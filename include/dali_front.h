@@ -167,6 +167,17 @@ int dali_fe_token_log_probs_backward(dali_array_t d_log_probs, dali_array_t d_en
 /* clipped: `count` handles, or NULL for the norm alone */
 int dali_fe_clip_by_global_norm(const dali_array_t* arrays, int count, double max_norm, dali_array_t* clipped, dali_array_t* norm);
 
+/* Embedding rows, attention to an encoder's states and the cross entropy of a projection, with their gradients; see op.embedding and what follows it in dali_amd/op.py.
+ * Results are passed as above. key_counts and bias may be NULL; without bias the handle of dbias is left alone. */
+int dali_fe_embedding(dali_array_t table, dali_array_t tokens, double scale, dali_array_t* y);
+int dali_fe_embedding_backward(dali_array_t dy, dali_array_t tokens, int rows, double scale, dali_array_t* dtable);
+int dali_fe_cross_attention(dali_array_t queries, dali_array_t keys, dali_array_t values, dali_array_t key_counts, double scale, dali_array_t* y, dali_array_t* lse);
+int dali_fe_cross_attention_backward(dali_array_t dy, dali_array_t queries, dali_array_t keys, dali_array_t values, dali_array_t y, dali_array_t lse,
+                                     dali_array_t key_counts, double scale, dali_array_t* d_queries, dali_array_t* d_keys, dali_array_t* d_values);
+int dali_fe_projected_cross_entropy(dali_array_t x, dali_array_t w, dali_array_t targets, dali_array_t bias, dali_array_t* losses, dali_array_t* lse);
+int dali_fe_projected_cross_entropy_backward(dali_array_t d_losses, dali_array_t x, dali_array_t w, dali_array_t targets, dali_array_t lse, dali_array_t bias,
+                                             dali_array_t* dx, dali_array_t* dw, dali_array_t* dbias);
+
 /* evaluation, assignment, host access */
 int dali_fe_eval(dali_array_t a);
 int dali_fe_eval_together(dali_array_t* roots, int n);

@@ -383,6 +383,60 @@ int dali_hip_token_log_probs(int dtype, int64_t rows, int vocab, const void* log
 int dali_hip_token_log_probs_backward(int dtype, int64_t rows, int vocab, const void* d_log_probs, const void* d_entropy, const void* logits, int64_t stride,
                                       const int32_t* tokens, const void* lse, const void* entropy, void* d_logits);
 
+/* ------------------------------------------------------------- embedding rows, cross attention, cross entropy of a projection */
+/*
+ * Operators of an encoder-decoder language model; the reference has none of them. dtype: DALI_HIP_FLOAT or DALI_HIP_DOUBLE, of every operand that is not int32. They allocate
+ * nothing: where a function ..._workspace is declared, `workspace` is device memory of the bytes that it answers for the same extents, on 256 bytes, which must not
+ * overlap anything and holds nothing before or after the call. Destinations must not overlap operands or each other. Results do not depend on the order of arrivals.
+ */
+
+/*
+ * y[i] = scale * table[tokens[i]] for `count` tokens; a token outside [0, rows) gives a row of zeros. Rows of the table are `stride` values apart, y [count, width] is dense.
+ */
+int dali_hip_embedding(int dtype, int64_t count, int rows, int width, const void* table, int64_t stride, const int32_t* tokens, double scale, void* y);
+/*
+ * Its gradient, written whole: dtable[r] = scale * sum of dy[i] over the i with tokens[i] = r, in the order of i up to blocks of 64 ordered tokens that are summed first; zeros
+ * where there is none. Rows of dy are `stride` values apart, dtable [rows, width] is dense. count may be 0.
+ */
+int dali_hip_embedding_backward_workspace(int dtype, int64_t count, int rows, int width, size_t* bytes);
+int dali_hip_embedding_backward(int dtype, int64_t count, int rows, int width, const void* dy, int64_t stride, const int32_t* tokens, double scale, void* dtable,
+                                void* workspace);
+
+#define DALI_HIP_MAX_HEAD_WIDTH 256
+/*
+ * Attention of positions q [batch, queries, heads, width] to states k, v [batch, keys, kv_heads, width] of another length: head h looks at kv head h / (heads / kv_heads), and
+ * sequence b has counts[b] states (held inside [0, keys]; counts NULL: all of them), what lies behind them is not read. With s = scale * q.k: lse = ln sum e^s
+ * [batch, queries, heads], y = sum e^(s - lse) v [batch, queries, heads, width], both dense. A row without states, or with scores of -inf alone, has y = 0 and lse = -inf; a
+ * score of +inf or NaN makes its row NaN. Strides are in values, of the first three axes; the last one is dense. width is at most DALI_HIP_MAX_HEAD_WIDTH.
+ */
+int dali_hip_cross_attention_workspace(int dtype, int batch, int queries, int keys, int heads, int kv_heads, int width, int backward, size_t* bytes);
+int dali_hip_cross_attention(int dtype, int batch, int queries, int keys, int heads, int kv_heads, int width, const void* q, const int64_t* q_strides, const void* k,
+                             const int64_t* k_strides, const void* v, const int64_t* v_strides, const int32_t* counts, double scale, void* y, void* lse, void* workspace);
+/*
+ * Its gradients from dy, that of y, and the y and lse (dense) of the forward pass: with p = e^(s - lse) and ds = p (dy.v - dy.y), dq = scale sum ds k, dk = scale sum ds q,
+ * dv = sum p dy, dense in the shapes of q, k and v; zeros for the states behind a sequence's last. Nothing flows through lse.
+ */
+int dali_hip_cross_attention_backward(int dtype, int batch, int queries, int keys, int heads, int kv_heads, int width, const void* dy, const int64_t* dy_strides, const void* q,
+                                      const int64_t* q_strides, const void* k, const int64_t* k_strides, const void* v, const int64_t* v_strides, const void* y,
+                                      const void* lse, const int32_t* counts, double scale, void* dq, void* dk, void* dv, void* workspace);
+
+/*
+ * Softmax cross entropy of rows x [rows, inputs] (x_stride values apart) against the logits x w + bias, which are formed in pieces and not kept: lse = ln sum e^logit,
+ * losses = lse - logit[target], both [rows]. w holds rows of the vocabulary's logits [inputs, vocab] w_stride values apart, or (w_by_columns) [vocab, inputs]; bias [vocab]
+ * may be NULL. A target outside [0, vocab) stands for none: loss 0. A logit of -inf has probability 0; a row of -inf alone has lse -inf and loss +inf.
+ */
+int dali_hip_projected_cross_entropy_workspace(int dtype, int64_t rows, int inputs, int vocab, int backward, int with_bias, size_t* bytes);
+int dali_hip_projected_cross_entropy(int dtype, int64_t rows, int inputs, int vocab, const void* x, int64_t x_stride, const void* w, int64_t w_stride, int w_by_columns,
+                                     const void* bias, const int32_t* targets, void* losses, void* lse, void* workspace);
+/*
+ * Its gradients from d_losses and the lse of the forward pass: with g = d_losses (e^(logit - lse) - [target]), dx = g w^T [rows, inputs], dw = x^T g [inputs, vocab] or (dw_by_columns)
+ * [vocab, inputs], dbias = sum of g over the rows; all dense; bias and dbias come together. A row without a target has no part in them whatever it holds (its dx is 0), nor has
+ * one of logits of -inf alone.
+ */
+int dali_hip_projected_cross_entropy_backward(int dtype, int64_t rows, int inputs, int vocab, const void* d_losses, const void* x, int64_t x_stride, const void* w,
+                                              int64_t w_stride, int w_by_columns, const void* bias, const int32_t* targets, const void* lse, void* dx, void* dw,
+                                              int dw_by_columns, void* dbias, void* workspace);
+
 /* ------------------------------------------------------------- the norm of many arrays */
 /*
  * *norm = sqrt(sum of the squares of all values of `count` arrays of sizes[i] values each), summed in double whatever the type, also where the squares of doubles are no
