@@ -62,6 +62,8 @@ struct Args {
     // results of parts of the states (or rows): [part][problem][row][D], and maxima and sums [part][problem][row]
     void *parts_y, *parts_m, *parts_l;
     int parts, tiles;
+    unsigned* counters;  // of arrivals, counter_step words apart
+    int counter_step;
     int first;  // problem of a launch's first workgroup
 };
 
@@ -372,14 +374,15 @@ __global__ __launch_bounds__(256, D * sizeof(T) <= 512 ? 2 : 1) void attention_f
     Running<T> run[RQ];
 #pragma unroll
     for (int i = 0; i < RQ; ++i) y[i].clear();
-    for (int slab = begin; slab < end; ++slab) {
-        const int key = slab * 16 + (lane & 15);
+    // 16 states as left operands, along them and across them (states past the last one weigh nothing, but must not be infinite either: the last one stands in)
+    struct Slab {
         typename Vec<T>::type left[C];
-        const T* k_row = k + min(key, n - 1) * a.k.row;
-#pragma unroll
-        for (int c = 0; c < C; ++c) left[c] = row_group<D>(k_row, (4 * c + g) * N, a.width);
-        // (states past the last one weigh nothing, but must not be infinite either: the last one stands in)
         typename Columns<T, D>::values across[4][Columns<T, D>::BLOCKS];
+    };
+    auto fetch = [&](Slab& to, int slab) {
+        const T* k_row = k + min(slab * 16 + (lane & 15), n - 1) * a.k.row;
+#pragma unroll
+        for (int c = 0; c < C; ++c) to.left[c] = row_group<D>(k_row, (4 * c + g) * N, a.width);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
             const T* v_row = v + min(slab * 16 + M::row_of(e, g), n - 1) * a.v.row;
@@ -389,13 +392,15 @@ __global__ __launch_bounds__(256, D * sizeof(T) <= 512 ? 2 : 1) void attention_f
                 const int c = (16 * blk + (lane & 15)) * NV;
                 typedef T loose __attribute__((ext_vector_type(NV), aligned(sizeof(T))));
                 if (c + NV <= a.width) {
-                    across[e][blk] = *reinterpret_cast<const loose*>(v_row + c);
+                    to.across[e][blk] = *reinterpret_cast<const loose*>(v_row + c);
                 } else {
 #pragma unroll
-                    for (int i = 0; i < NV; ++i) across[e][blk][i] = c + i < a.width ? v_row[c + i] : T(0);
+                    for (int i = 0; i < NV; ++i) to.across[e][blk][i] = c + i < a.width ? v_row[c + i] : T(0);
                 }
             }
         }
+    };
+    auto take = [&](const Slab& from, int slab) {
         typename M::acc s[RQ][1];
 #pragma unroll
         for (int i = 0; i < RQ; ++i) {
@@ -403,7 +408,7 @@ __global__ __launch_bounds__(256, D * sizeof(T) <= 512 ? 2 : 1) void attention_f
 #pragma unroll
             for (int c = 0; c < C; ++c)
 #pragma unroll
-                for (int e = 0; e < N; ++e) s[i][0] = M::mul(left[c][e], qf[i].g[c][e], s[i][0]);
+                for (int e = 0; e < N; ++e) s[i][0] = M::mul(from.left[c][e], qf[i].g[c][e], s[i][0]);
         }
         if (slab * 16 + 16 > n) {
 #pragma unroll
@@ -424,7 +429,24 @@ __global__ __launch_bounds__(256, D * sizeof(T) <= 512 ? 2 : 1) void attention_f
 #pragma unroll
                 for (int c = 0; c < Columns<T, D>::NV; ++c)
 #pragma unroll
-                    for (int i = 0; i < RQ; ++i) y[i].acc[blk][c] = M::mul(across[e][blk][c], s[i][0][e], y[i].acc[blk][c]);
+                    for (int i = 0; i < RQ; ++i) y[i].acc[blk][c] = M::mul(from.across[e][blk][c], s[i][0][e], y[i].acc[blk][c]);
+    };
+    if constexpr (D * sizeof(T) <= 512) {  // the next slab is under way while one is worked on
+        Slab even, odd;
+        if (begin < end) fetch(even, begin);
+        for (int slab = begin; slab < end; slab += 2) {
+            if (slab + 1 < end) fetch(odd, slab + 1);
+            take(even, slab);
+            if (slab + 1 >= end) break;
+            if (slab + 2 < end) fetch(even, slab + 2);
+            take(odd, slab + 1);
+        }
+    } else {
+        for (int slab = begin; slab < end; ++slab) {
+            Slab one;
+            fetch(one, slab);
+            take(one, slab);
+        }
     }
     // the four waves' parts: maxima and sums first, then the rows, one wave after the other
     T sum[RQ];
@@ -458,6 +480,7 @@ __global__ __launch_bounds__(256, D * sizeof(T) <= 512 ? 2 : 1) void attention_f
         __syncthreads();
     }
     // (every wave holds the maximum and the sum of a lane's row)
+    const int64_t pitch = (int64_t)a.batch * a.kv_heads * a.rows, own = (int64_t)problem * a.rows;  // of a part; this problem's rows in it
     if (wave == 0 && g == 0) {
 #pragma unroll
         for (int i = 0; i < RQ; ++i) {
@@ -467,25 +490,51 @@ __global__ __launch_bounds__(256, D * sizeof(T) <= 512 ? 2 : 1) void attention_f
             if (a.parts == 1) {
                 ((T*)a.lse_out)[dense_row<T>(a, b, kvh, r)] = all[i] == T(0) ? T(-INFINITY) : M::lse(best[i], all[i]);
             } else {
-                const int64_t to = ((int64_t)part * a.batch * a.kv_heads + problem) * a.rows + r;
-                ((T*)a.parts_m)[to] = best[i], ((T*)a.parts_l)[to] = all[i];
+                publish((T*)a.parts_m + part * pitch + own + r, best[i]);
+                publish((T*)a.parts_l + part * pitch + own + r, all[i]);
             }
         }
     }
     __syncthreads();
-    for (int at = threadIdx.x; at < min(a.rows, 16 * RQ) * (D / N); at += 256) {
-        const int r = at / (D / N), c = at % (D / N) * N;
-        T values[N];
-#pragma unroll
-        for (int e = 0; e < N; ++e) values[e] = ys[r * (D + N) + c + e];
-        if (a.parts == 1) {
+    const int groups = a.rows * (D / N);
+    if (a.parts == 1) {
+        for (int at = threadIdx.x; at < groups; at += 256) {
+            const int r = at / (D / N), c = at % (D / N) * N;
             if (c >= a.width) continue;
+            T values[N];
 #pragma unroll
-            for (int e = 0; e < N; ++e) values[e] = sums[r] == T(0) ? T(0) : values[e] / sums[r];
+            for (int e = 0; e < N; ++e) values[e] = sums[r] == T(0) ? T(0) : ys[r * (D + N) + c + e] / sums[r];
             store_group((T*)a.y_out + dense_row<T>(a, b, kvh, r) * a.width, c, a.width, values);
-        } else {
-            store_group((T*)a.parts_y + (((int64_t)part * a.batch * a.kv_heads + problem) * a.rows + r) * D, c, D, values);
         }
+        return;
+    }
+    // The parts of a problem meet in the workspace; the last workgroup to arrive joins them, in their order.
+    for (int at = threadIdx.x; at < groups; at += 256) {
+        const int r = at / (D / N), c = at % (D / N) * N;
+#pragma unroll
+        for (int e = 0; e < N; ++e) publish((T*)a.parts_y + (part * pitch + own + r) * D + c + e, ys[r * (D + N) + c + e]);
+    }
+    __shared__ unsigned ticket;
+    if (!last_to_arrive(a.counters + at * a.counter_step, a.parts, &ticket)) return;
+    const T *pm = (const T*)a.parts_m + own, *pl = (const T*)a.parts_l + own, *py = (const T*)a.parts_y + own * D;
+    for (int at = threadIdx.x; at < groups; at += 256) {
+        const int r = at / (D / N), c = at % (D / N) * N;
+        T top = M::lowest, sum = 0, values[N] = {};
+#pragma unroll 4
+        for (int p = 0; p < a.parts; ++p) top = Max()(top, observe(pm + p * pitch + r));
+#pragma unroll 4
+        for (int p = 0; p < a.parts; ++p) {
+            const T f = M::weight(observe(pm + p * pitch + r) - top);
+            sum += observe(pl + p * pitch + r) * f;
+#pragma unroll
+            for (int e = 0; e < N; ++e) values[e] += observe(py + (p * pitch + r) * D + c + e) * f;
+        }
+        const int64_t to = dense_row<T>(a, b, kvh, r);
+        if (c == 0) ((T*)a.lse_out)[to] = sum == T(0) ? T(-INFINITY) : M::lse(top, sum);
+        if (c >= a.width) continue;
+#pragma unroll
+        for (int e = 0; e < N; ++e) values[e] = sum == T(0) ? T(0) : values[e] / sum;
+        store_group((T*)a.y_out + to * a.width, c, a.width, values);
     }
 }
 
@@ -802,7 +851,7 @@ struct ForwardPlan {
     void set(const Args& a) {
         typedef ForwardShape<T, D> S;
         const int64_t problems = (int64_t)a.batch * a.kv_heads;
-        few = a.rows <= 32;
+        few = a.rows <= (D * sizeof(T) <= 512 ? 32 : 16);  // (wider rows: 32 would not fit a wave's registers)
         rq = a.rows <= 16 ? 1 : 2;
         tiles = few ? 1 : (a.rows + 64 * S::RQ - 1) / (64 * S::RQ);
         parts = few ? parts_for(problems, (a.keys + 63) / 64, 3, 2) : parts_for(problems * tiles, (a.keys + S::KT - 1) / S::KT, 2, 4);
@@ -866,11 +915,15 @@ int forward(const char* what, Args a) {
     plan.set<T, D>(a);
     a.parts = plan.parts, a.tiles = plan.tiles;
     const int64_t problems = (int64_t)a.batch * a.kv_heads;
+    if (plan.few && plan.parts > 1) {  // (so few problems that one launch takes them all)
+        a.counters = (unsigned*)workspace();
+        a.counter_step = counter_step(problems);
+    }
     const int few_lds = 16 * plan.rq * (D + Vec<T>::N + 8) * (int)sizeof(T);
     const int status = plan.few ? (plan.rq == 1 ? launch(what, attention_few<T, D, 1>, problems, plan.parts, few_lds, a)
                                                 : launch(what, attention_few<T, D, 2>, problems, plan.parts, few_lds, a))
                                 : launch(what, attention_rows<T, D>, problems, plan.tiles * plan.parts, ForwardShape<T, D>::LDS, a);
-    if (status || plan.parts == 1) return status;
+    if (status || plan.parts == 1 || plan.few) return status;
     return launch(what, attention_join<T, D>, 1, (problems * a.rows + 3) / 4, 0, a);
 }
 

@@ -9,6 +9,7 @@
 // address arithmetic of a slab hide behind the sixteen to sixty-four instructions each wave issues for it. Operands are
 // addressed through (row stride, k stride) pairs, which covers the four transposition cases; the lane-to-element map of
 // the global loads follows whichever stride is 1.
+#include <algorithm>
 #include <cstdint>
 
 #include "runtime.h"
@@ -29,6 +30,8 @@ struct DgemmArgs {
     double* C;
     long ldc;
     double alpha, beta;
+    int share;      // values of k that a share of the inner extent has (a multiple of BK), 0: there is one
+    long share_c;   // elements from a share's C to the next one's
 };
 
 // T: 16 x 16 accumulators per wave and dimension. T = 2: the workgroup's tile of C is 64 x 64 (many workgroups for a small
@@ -137,6 +140,13 @@ template <int T>
 __global__ __launch_bounds__(256, T == 4 ? 2 : 4) void dgemm_kernel(DgemmArgs a, int offsets_fit) {
     extern __shared__ double dgemm_lds[];  // [A, B][2 buffers][BK][32 T + 2]
     constexpr int BM = 32 * T, BN = 32 * T;
+    if (a.share) {
+        const int k0 = blockIdx.y * a.share;
+        a.A += (long)k0 * a.ak;
+        a.B += (long)k0 * a.bk;
+        a.C += blockIdx.y * a.share_c;
+        a.K = min(a.K - k0, a.share);
+    }
     const int tiles_n = (a.N + BN - 1) / BN;
     const int tm = blockIdx.x / tiles_n, tn = blockIdx.x % tiles_n;
     const int m0 = tm * BM, n0 = tn * BN;
@@ -145,7 +155,57 @@ __global__ __launch_bounds__(256, T == 4 ? 2 : 4) void dgemm_kernel(DgemmArgs a,
     else dgemm_tile<true, T>(a, dgemm_lds, m0, n0);
 }
 
+// c[i, j] = beta c[i, j] + the shares' products in their order
+__global__ __launch_bounds__(256) void dgemm_fold(const double* parts, int shares, long size, int cols, double beta, double* c, long ldc) {
+    const long at = (long)blockIdx.x * 256 + threadIdx.x;
+    if (at >= size) return;
+    double* p = c + at / cols * ldc + at % cols;
+    double sum = parts[at];
+    for (int s = 1; s < shares; ++s) sum += parts[s * size + at];
+    *p = beta == 0.0 ? sum : sum + beta * *p;
+}
+
+constexpr int kShareTiles = 512;  // workgroups that a product is cut for
+
+int share_of(int M, int N, int K, int* shares) {
+    const long tiles = (long)((M + 63) / 64) * ((N + 63) / 64);
+    *shares = (int)std::max(1L, std::min({(long)kShareTiles / tiles, (long)K / 256, 64L}));
+    const int share = ((K + *shares - 1) / *shares + BK - 1) / BK * BK;
+    *shares = (K + share - 1) / share;
+    return share;
+}
+
 }  // namespace
+
+size_t dgemm_shares_bytes(int M, int N, int K) {
+    int shares;
+    share_of(M, N, K, &shares);
+    return shares == 1 ? 0 : (size_t)shares * M * N * sizeof(double);
+}
+
+int dgemm_shares(bool ta, bool tb, int M, int N, int K, const double* A, int lda, const double* B, int ldb, double beta, double* C, int ldc, void* parts) {
+    int shares;
+    const int share = share_of(M, N, K, &shares);
+    if (shares == 1) return dali_hip_dgemm(tb, ta, N, M, K, 1.0, B, ldb, A, lda, beta, C, ldc);
+    DgemmArgs a = {};
+    a.M = M; a.N = N; a.K = K;
+    a.A = A; a.ai = ta ? 1 : lda; a.ak = ta ? lda : 1;
+    a.B = B; a.bk = tb ? 1 : ldb; a.bj = tb ? ldb : 1;
+    a.C = (double*)parts; a.ldc = N; a.alpha = 1.0;
+    a.share = share; a.share_c = (long)M * N;
+    const long span_a = 63 * (ta ? 1L : (long)lda) + 15 * (ta ? (long)lda : 1L), span_b = 15 * (tb ? 1L : (long)ldb) + 63 * (tb ? (long)ldb : 1L);
+    const unsigned tiles = (unsigned)(((M + 63) / 64) * ((N + 63) / 64));
+    hipLaunchKernelGGL(dgemm_kernel<2>, dim3(tiles, (unsigned)shares), dim3(256), (size_t)2 * 2 * BK * 66 * sizeof(double), stream(), a,
+                       span_a < (1L << 28) && span_b < (1L << 28));
+    hipError_t e = hipGetLastError();
+    if (e == hipSuccess) {
+        const long size = (long)M * N;
+        hipLaunchKernelGGL(dgemm_fold, dim3((unsigned)((size + 255) / 256)), dim3(256), 0, stream(), (const double*)parts, shares, size, N, beta, C, (long)ldc);
+        e = hipGetLastError();
+    }
+    return e == hipSuccess ? DALI_HIP_OK : fail("dgemm launch failed: %s", hipGetErrorString(e));
+}
+
 }  // namespace dali_hip
 
 using namespace dali_hip;
@@ -163,7 +223,7 @@ extern "C" int dali_hip_dgemm(int transB, int transA, int m, int n, int k, doubl
         if (lda < (transA ? rows : k)) return fail("dali_hip_dgemm: lda %d is too small", lda);
         if (ldb < (transB ? k : cols)) return fail("dali_hip_dgemm: ldb %d is too small", ldb);
     }
-    DgemmArgs a;
+    DgemmArgs a = {};
     a.M = rows; a.N = cols; a.K = k;
     a.A = A; a.ai = transA ? 1 : lda; a.ak = transA ? lda : 1;
     a.B = B; a.bk = transB ? 1 : ldb; a.bj = transB ? ldb : 1;

@@ -1,11 +1,11 @@
 // Rows of an embedding table for tokens, scaled, and the gradient of the table. Beyond the reference (its gather has neither scale nor padding).
 //
-// y[i] = scale table[t_i], zeros where t_i lies outside the table. The gradient is written whole: dtable[r] = scale sum over i with t_i = r of dy[i], in the order
-// of i, zeros for rows that no token names. The tokens are ordered first (stable, so a row's positions stay in their order), and a workgroup that owns
-// neighbouring rows of the table finds where their runs begin by looking at 64 places of the ordered tokens at a time.
+// y[i] = scale table[t_i], zeros where t_i lies outside the table. The gradient is written whole: dtable[r] = scale sum over i with t_i = r of dy[i], in the order of i, zeros
+// for rows that no token names.
 //
-// Texts name a few tokens very often: positions that lie in a block of kChunk ordered tokens that are all the same are summed by a launch of their own before, so that a
-// row's owner adds at most 2 (kChunk - 1) positions and the sums of whole blocks. What is summed in which order depends on the tokens alone, never on arrival.
+// The tokens are ordered first (stable, so a row's positions stay in their order). Texts name a few tokens very often and most words never, so the work is cut by places of the
+// order, not by rows: a wave adds up the rows of dy at 16 to 128 neighbouring places, eight loads under way, and writes the runs that lie within them. A second launch
+// joins the parts of longer runs and writes the rows that no token names. What is summed in which order depends on the tokens alone, never on arrival.
 #include <algorithm>
 #include <cmath>
 
@@ -69,9 +69,7 @@ int embedding(int64_t count, int rows, int width, const T* table, int64_t stride
 }
 
 // ------------------------------------------------------------------------------------------------ the gradient of the table
-constexpr int kChunk = 64;
-
-// The first of `n` ordered tokens that is not below `key`; all lanes of the wave take part. (Tokens outside the table come out behind the others, negative ones
+// the first of `n` ordered tokens that is not below `key`; all lanes of the wave take part. (Tokens outside the table come out behind the others, negative ones
 // among them: read without a sign they are above any row's number.)
 __device__ __forceinline__ int lower_bound(const int32_t* keys, int n, unsigned key) {
     const int lane = threadIdx.x & 63;
@@ -87,53 +85,66 @@ __device__ __forceinline__ int lower_bound(const int32_t* keys, int n, unsigned 
     return lo;
 }
 
-// adds rows of dy to N sums of a lane, eight loads at a time; `place(p)` is the row at position p
-template <bool LONG, typename T, typename Place>
-__device__ __forceinline__ void add_rows(T (&sum)[Vec<T>::N], const T* from, int64_t stride, int c, int width, int begin, int end, Place place) {
-    constexpr int N = Vec<T>::N;
-    constexpr int DEEP = 8;
-    int p = begin;
-    for (; p + DEEP <= end; p += DEEP) {
-        typename Vec<T>::type g[DEEP];
-#pragma unroll
-        for (int j = 0; j < DEEP; ++j) g[j] = ask_group<LONG>(from + place(p + j) * stride, c, width);
-#pragma unroll
-        for (int j = 0; j < DEEP; ++j) {
+// A wave takes 64 groups of columns of the rows at `chunk` neighbouring places of the order. A run of one token that lies within them is written to its row; what a run that
+// goes on before or behind them comes to here is left in partials[chunk][0] (a run that the chunk begins with) or [1].
+template <typename T>
+__global__ __launch_bounds__(64) void embedding_chunks(const T* dy, int64_t stride, int width, const int32_t* keys, const int32_t* positions, int count, int rows, int chunk,
+                                                       int first_chunk, T scale, T* dtable, T* partials) {
+    constexpr int N = Vec<T>::N, DEEP = 8;
+    const int lane = threadIdx.x, at = first_chunk + blockIdx.x, begin = at * chunk, end = min(begin + chunk, count);
+    const int c = (blockIdx.y * 64 + lane) * N;
+    T sum[N] = {};
+    int run = begin;  // where the run at hand begins
+    int token = __builtin_amdgcn_readfirstlane(keys[begin]);
+    const bool goes_back = begin > 0 && keys[begin - 1] == token;
+    // what the run at hand has come to, up to `to`; it goes on behind the chunk: `on`
+    auto leave = [&](int to, bool on) {
+        if ((unsigned)token < (unsigned)rows && c < width) {
+            const bool part = on || (run == begin && goes_back);
+            T* out = part ? partials + ((int64_t)at * 2 + (run == begin ? 0 : 1)) * width : dtable + (int64_t)token * width;
             T v[N];
-            take_group<LONG>(g[j], c, width, T(0), v);
 #pragma unroll
-            for (int e = 0; e < N; ++e) sum[e] += v[e];
+            for (int e = 0; e < N; ++e) v[e] = part ? sum[e] : sum[e] * scale;
+            store_group(out, c, width, v);
+        }
+        run = to;
+#pragma unroll
+        for (int e = 0; e < N; ++e) sum[e] = 0;
+    };
+    for (int p0 = begin; p0 < end; p0 += 64) {
+        const int p = min(p0 + lane, end - 1), key = keys[p], place = positions[p], here = min(64, end - p0);
+        // (the runs that begin here: the chunk's first is at hand already)
+        const unsigned long long heads = __ballot(p0 + lane < end && p > begin && keys[max(p - 1, 0)] != key);
+        for (int i = 0; i < here; i += DEEP) {
+            typename Vec<T>::type g[DEEP];
+#pragma unroll
+            for (int j = 0; j < DEEP; ++j) {
+                const int64_t row = __builtin_amdgcn_readlane(place, min(i + j, here - 1));
+                if (c < width) g[j] = ask_group(dy + row * stride, c, width);
+            }
+#pragma unroll
+            for (int j = 0; j < DEEP; ++j) {
+                if (i + j >= here) break;
+                if (heads >> (i + j) & 1) {
+                    leave(p0 + i + j, false);
+                    token = __builtin_amdgcn_readlane(key, i + j);
+                }
+                T v[N];
+                take_group(g[j], c, width, T(0), v);
+#pragma unroll
+                for (int e = 0; e < N; ++e) sum[e] += v[e];
+            }
         }
     }
-    for (; p < end; ++p) {
-        T v[N];
-        load_group(from + place(p) * stride, c, width, T(0), v);
-#pragma unroll
-        for (int e = 0; e < N; ++e) sum[e] += v[e];
-    }
+    leave(end, end < count && keys[end] == token);
 }
 
-// The sums of blocks of kChunk ordered tokens that are all the same: a wave takes 64 groups of columns of one.
-template <typename T>
-__global__ __launch_bounds__(256) void embedding_chunks(const T* dy, int64_t stride, int width, const int32_t* keys, const int32_t* positions, int rows, int first_chunk, T* partials) {
-    constexpr int N = Vec<T>::N;
-    const int chunk = first_chunk + blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int32_t* k = keys + (int64_t)chunk * kChunk;
-    const int first = k[0];
-    if (first != k[kChunk - 1] || first < 0 || first >= rows) return;
-    const int32_t* at = positions + (int64_t)chunk * kChunk;
-    for (int c = (wave * 64 + lane) * N; c < width; c += 256 * N) {
-        T sum[N] = {};
-        add_rows<false>(sum, dy, stride, c, width, 0, kChunk, [&](int p) { return (int64_t)at[p]; });
-        store_group(partials + (int64_t)chunk * width, c, width, sum);
-    }
-}
-
-// A workgroup writes `per` neighbouring rows of the table (at most 16), its waves each a quarter of the columns.
+// A workgroup sees to `per` neighbouring rows of the table (at most 16): zeros where no token names one, and the parts of a run that lies in several chunks, in their order.
+// A wave takes every fourth 64 groups of columns.
 template <typename T, bool PAST>
-__global__ __launch_bounds__(256) void embedding_gradient(const T* dy, int64_t stride, int width, const int32_t* keys, const int32_t* positions, int count, int rows, int first_row,
-                                                          int per, const T* partials, T scale, T* dtable) {
-    constexpr int N = Vec<T>::N;
+__global__ __launch_bounds__(256) void embedding_gradient(int width, const int32_t* keys, int count, int rows, int chunk, int first_row, int per, const T* partials, T scale,
+                                                          T* dtable) {
+    constexpr int N = Vec<T>::N, DEEP = 8;
     __shared__ int begin[17];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int r0 = first_row + blockIdx.x * per, here = min(per, rows - r0);
@@ -144,18 +155,26 @@ __global__ __launch_bounds__(256) void embedding_gradient(const T* dy, int64_t s
     __syncthreads();
     for (int r = 0; r < here; ++r) {
         const int from = begin[r], to = begin[r + 1];
-        // whole blocks of this row's positions: [whole, whole_end) kChunk
-        const int whole = (from + kChunk - 1) / kChunk, whole_end = to / kChunk;
+        const int first = from / chunk, last = (to - 1) / chunk;
+        if (from < to && first == last) continue;  // written already
         T* out = dtable + (int64_t)(r0 + r) * width;
         for (int c = (wave * 64 + lane) * N; c < width; c += 256 * N) {
             T sum[N] = {};
-            const auto place = [&](int p) { return (int64_t)positions[p]; };
-            if (whole < whole_end) {
-                add_rows<false>(sum, dy, stride, c, width, from, whole * kChunk, place);
-                add_rows<false>(sum, partials, (int64_t)width, c, width, whole, whole_end, [](int p) { return (int64_t)p; });
-                add_rows<false>(sum, dy, stride, c, width, whole_end * kChunk, to, place);
-            } else {
-                add_rows<false>(sum, dy, stride, c, width, from, to, place);
+            if (from < to) {
+                load_group(partials + ((int64_t)first * 2 + (from % chunk ? 1 : 0)) * width, c, width, T(0), sum);
+                for (int p = first + 1; p <= last; p += DEEP) {
+                    typename Vec<T>::type g[DEEP];
+#pragma unroll
+                    for (int j = 0; j < DEEP; ++j) g[j] = ask_group(partials + (int64_t)min(p + j, last) * 2 * width, c, width);
+#pragma unroll
+                    for (int j = 0; j < DEEP; ++j) {
+                        if (p + j > last) break;
+                        T v[N];
+                        take_group(g[j], c, width, T(0), v);
+#pragma unroll
+                        for (int e = 0; e < N; ++e) sum[e] += v[e];
+                    }
+                }
             }
 #pragma unroll
             for (int e = 0; e < N; ++e) sum[e] *= scale;
@@ -164,7 +183,14 @@ __global__ __launch_bounds__(256) void embedding_gradient(const T* dy, int64_t s
     }
 }
 
-// what the gradient keeps beside its operands: ordered tokens, their positions, room for ordering them, and the sums of whole blocks
+// Places of the order that a wave of the first launch takes: enough chunks to fill the chip, few enough parts of a frequent token
+int chunk_of(int64_t count) {
+    int chunk = 16;
+    while (chunk < 128 && count / chunk > 1024) chunk *= 2;
+    return chunk;
+}
+
+// what the gradient keeps beside its operands: ordered tokens, their positions, room for ordering them, and the parts of runs
 struct GradientSpace {
     size_t keys, positions, order, partials, bytes;
     GradientSpace(int64_t count, int width, size_t size) {
@@ -173,7 +199,8 @@ struct GradientSpace {
         positions = round((size_t)count * 4);
         order = 2 * positions;
         partials = order + round(argsort_scratch_bytes(count));
-        bytes = partials + (size_t)(count / kChunk) * width * size;
+        const int chunk = chunk_of(count);
+        bytes = partials + 2 * (size_t)((count + chunk - 1) / chunk) * width * size;
     }
 };
 
@@ -184,9 +211,12 @@ int embedding_backward(int64_t count, int rows, int width, const T* dy, int64_t 
     int32_t *keys = (int32_t*)(space + s.keys), *positions = (int32_t*)(space + s.positions);
     T* partials = (T*)(space + s.partials);
     if (count && argsort_with(tokens, count, rows, keys, positions, space + s.order)) return DALI_HIP_ERROR;
-    const int chunks = (int)(count / kChunk), most = 1 << 23;  // workgroups of one launch, which has fewer than 2^32 threads
+    const int chunk = chunk_of(count), chunks = (int)((count + chunk - 1) / chunk), most = 1 << 23;  // workgroups along an axis of a launch, which has fewer than 2^32 threads
+    const int across = (groups_of<T>(width) + 63) / 64;
+    if (across > 65535) return fail("%s: rows of %d values are too wide", what, width);
     for (int first = 0; first < chunks; first += most) {
-        embedding_chunks<T><<<dim3((unsigned)std::min(chunks - first, most)), dim3(256), 0, stream()>>>(dy, stride, width, keys, positions, rows, first, partials);
+        embedding_chunks<T><<<dim3((unsigned)std::min(chunks - first, most), (unsigned)across), dim3(64), 0, stream()>>>(dy, stride, width, keys, positions, (int)count, rows, chunk,
+                                                                                                                 first, (T)scale, dtable, partials);
         if (launched(what)) return DALI_HIP_ERROR;
     }
     const int per = std::max(1, std::min(16, rows / 2048));
@@ -195,7 +225,7 @@ int embedding_backward(int64_t count, int rows, int width, const T* dy, int64_t 
         const int64_t blocks = std::min((rows - first + per - 1) / per, (int64_t)most);
         either_way(past, [&](auto p) {
             embedding_gradient<T, decltype(p)::value>
-                <<<dim3((unsigned)blocks), dim3(256), 0, stream()>>>(dy, stride, width, keys, positions, (int)count, rows, (int)first, per, partials, (T)scale, dtable);
+                <<<dim3((unsigned)blocks), dim3(256), 0, stream()>>>(width, keys, (int)count, rows, chunk, (int)first, per, partials, (T)scale, dtable);
         });
         if (launched(what)) return DALI_HIP_ERROR;
     }

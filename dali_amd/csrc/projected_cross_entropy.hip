@@ -37,12 +37,30 @@ constexpr int kChunkRows = 64;                          // that a workgroup of t
 constexpr size_t kPieceBytes = (size_t)128 << 20;
 constexpr int kMostRows = 16384;
 
+// row-major C[m, n] = op(A) op(B) + beta C
+int product(bool ta, bool tb, int m, int n, int k, const float* a, int lda, const float* b, int ldb, float beta, float* c, int ldc) {
+    return dali_hip_sgemm(tb, ta, n, m, k, 1.0f, b, ldb, a, lda, beta, c, ldc);
+}
+int product(bool ta, bool tb, int m, int n, int k, const double* a, int lda, const double* b, int ldb, double beta, double* c, int ldc) {
+    return dali_hip_dgemm(tb, ta, n, m, k, 1.0, b, ldb, a, lda, beta, c, ldc);
+}
+// The same where C may have few tiles and a long inner extent: the fp32 kernels cut that by themselves, the fp64 kernel into parts that lie in `parts` ([301, 10007] .
+// [10007, 515] 600 us uncut)
+size_t cut_bytes(float, int, int, int) { return 0; }
+size_t cut_bytes(double, int m, int n, int k) { return dgemm_shares_bytes(m, n, k); }
+int cut_product(bool ta, bool tb, int m, int n, int k, const float* a, int lda, const float* b, int ldb, float beta, float* c, int ldc, void*) {
+    return product(ta, tb, m, n, k, a, lda, b, ldb, beta, c, ldc);
+}
+int cut_product(bool ta, bool tb, int m, int n, int k, const double* a, int lda, const double* b, int ldb, double beta, double* c, int ldc, void* parts) {
+    return dgemm_shares(ta, tb, m, n, k, a, lda, b, ldb, beta, c, ldc, parts);
+}
+
 // How a call is cut, and what it keeps beside its operands
 template <typename T>
 struct Cut {
     int64_t rows;
     int inputs, vocab, block, piece, segments, chunks;
-    size_t logits = 0, maxima, sums, chosen, inputs_kept, columns, bytes;
+    size_t logits = 0, maxima, sums, chosen, inputs_kept, columns, parts, bytes;
     Cut(int64_t rows_, int inputs_, int vocab_, bool backward, bool bias) : rows(rows_), inputs(inputs_), vocab(vocab_) {
         const auto round = [](size_t b) { return (b + 255) / 256 * 256; };
         block = (int)std::min<int64_t>(std::max<int64_t>(rows, 1), kMostRows);
@@ -55,17 +73,17 @@ struct Cut {
         chosen = sums + (backward ? 0 : round((size_t)block * segments * sizeof(T)));
         inputs_kept = chosen + (backward ? 0 : round((size_t)block * sizeof(T)));
         columns = inputs_kept + (backward ? round((size_t)block * inputs * sizeof(T)) : 0);
-        bytes = columns + (backward && bias ? round((size_t)chunks * piece * sizeof(T)) : 0);
+        parts = columns + (backward && bias ? round((size_t)chunks * piece * sizeof(T)) : 0);
+        bytes = parts;
+        // (the last block and piece may be smaller, and cut more finely)
+        const int b = (int)((std::max<int64_t>(rows, 1) - 1) % block) + 1, p = (vocab - 1) % piece + 1;
+        for (const int m : {block, b})
+            for (const int v : {piece, p}) {
+                bytes = std::max(bytes, parts + cut_bytes(T(), m, v, inputs));
+                if (backward) bytes = std::max({bytes, parts + cut_bytes(T(), m, inputs, v), parts + cut_bytes(T(), inputs, v, m), parts + cut_bytes(T(), v, inputs, m)});
+            }
     }
 };
-
-// row-major C[m, n] = op(A) op(B) + beta C
-int product(bool ta, bool tb, int m, int n, int k, const float* a, int lda, const float* b, int ldb, float beta, float* c, int ldc) {
-    return dali_hip_sgemm(tb, ta, n, m, k, 1.0f, b, ldb, a, lda, beta, c, ldc);
-}
-int product(bool ta, bool tb, int m, int n, int k, const double* a, int lda, const double* b, int ldb, double beta, double* c, int ldc) {
-    return dali_hip_dgemm(tb, ta, n, m, k, 1.0, b, ldb, a, lda, beta, c, ldc);
-}
 
 // ------------------------------------------------------------------------------------------------ forward
 // A wave takes a segment of a row of the piece of logits that begins at column v0 of `width` columns.
@@ -160,7 +178,7 @@ int cross_entropy(int64_t rows, int inputs, int vocab, const T* x, int64_t x_str
         const int n = (int)std::min<int64_t>(cut.block, rows - r);
         for (int64_t v = 0; v < vocab; v += cut.piece) {
             const int width = (int)std::min<int64_t>(cut.piece, vocab - v), here = (width + kSegment<T> - 1) / kSegment<T>;
-            if (product(false, w_by_columns, n, width, inputs, x + r * x_stride, (int)x_stride, w_by_columns ? w + v * w_stride : w + v, (int)w_stride, T(0), logits, width))
+            if (cut_product(false, w_by_columns, n, width, inputs, x + r * x_stride, (int)x_stride, w_by_columns ? w + v * w_stride : w + v, (int)w_stride, T(0), logits, width, space + cut.parts))
                 return DALI_HIP_ERROR;
             entropy_segments<T><<<dim3((unsigned)(((int64_t)n * here + 3) / 4)), dim3(256), 0, stream()>>>(
                 logits, n, width, (int)v, (int)(v / kSegment<T>), bias ? bias + v : nullptr, targets + r, cut.segments, maxima, sums, chosen);
@@ -245,6 +263,7 @@ int cross_entropy_backward(int64_t rows, int inputs, int vocab, const T* d_losse
     const char* what = "dali_hip_projected_cross_entropy_backward";
     const Cut<T> cut(rows, inputs, vocab, true, dbias != nullptr);
     T *g = (T*)(space + cut.logits), *kept = (T*)(space + cut.inputs_kept), *columns = dbias ? (T*)(space + cut.columns) : nullptr;
+    void* parts = space + cut.parts;
     if (rows == 0) {  // (nothing is added up)
         entropy_zeros<T><<<dim3(1024), dim3(256), 0, stream()>>>(dw, (int64_t)inputs * vocab);
         if (!launched(what) && dbias) entropy_zeros<T><<<dim3(1024), dim3(256), 0, stream()>>>(dbias, (int64_t)vocab);
@@ -257,14 +276,14 @@ int cross_entropy_backward(int64_t rows, int inputs, int vocab, const T* d_losse
         for (int64_t v = 0; v < vocab; v += cut.piece) {
             const int width = (int)std::min<int64_t>(cut.piece, vocab - v);
             const T* wp = w_by_columns ? w + v * w_stride : w + v;
-            if (product(false, w_by_columns, n, width, inputs, x + r * x_stride, (int)x_stride, wp, (int)w_stride, T(0), g, width)) return DALI_HIP_ERROR;
+            if (cut_product(false, w_by_columns, n, width, inputs, x + r * x_stride, (int)x_stride, wp, (int)w_stride, T(0), g, width, parts)) return DALI_HIP_ERROR;
             entropy_gradient<T><<<dim3((unsigned)((width + 256 * Vec<T>::N - 1) / (256 * Vec<T>::N)), (unsigned)chunks), dim3(256), 0, stream()>>>(
                 g, n, width, (int)v, vocab, bias ? bias + v : nullptr, targets + r, lse + r, d_losses + r, columns);
             if (launched(what)) return DALI_HIP_ERROR;
-            if (product(false, !w_by_columns, n, inputs, width, g, width, wp, (int)w_stride, T(v > 0), dx + r * inputs, inputs)) return DALI_HIP_ERROR;
+            if (cut_product(false, !w_by_columns, n, inputs, width, g, width, wp, (int)w_stride, T(v > 0), dx + r * inputs, inputs, parts)) return DALI_HIP_ERROR;
             const T more = T(r > 0);
-            if (dw_by_columns ? product(true, false, width, inputs, n, g, width, kept, inputs, more, dw + v * inputs, inputs)
-                              : product(true, false, inputs, width, n, kept, inputs, g, width, more, dw + v, vocab))
+            if (dw_by_columns ? cut_product(true, false, width, inputs, n, g, width, kept, inputs, more, dw + v * inputs, inputs, parts)
+                              : cut_product(true, false, inputs, width, n, kept, inputs, g, width, more, dw + v, vocab, parts))
                 return DALI_HIP_ERROR;
             if (dbias) {
                 entropy_bias<T><<<dim3((unsigned)((width + 255) / 256)), dim3(256), 0, stream()>>>(columns, chunks, width, r > 0, dbias + v);

@@ -90,6 +90,10 @@ int sgemm_split(bool ta, bool tb, int M, int N, int nseg, const int* K, const fl
 int split_conv_nhwc(bool filters_gradient, int n, int h, int w, int c, int f, int fh, int fw, int stride_h, int stride_w, const float* image, const float* other,
                     float* result, int cus);
 bool split_conv_nhwc_takes(bool filters_gradient, int n, int h, int w, int c, int f, int fh, int fw, int stride_h, int stride_w, int cus);
+// dgemm.hip: row-major C[M, N] = op(A) . op(B) + beta * C in double for a C of few tiles and a long inner extent, which is cut into shares of their own workgroups; `parts`
+// holds dgemm_shares_bytes of what they come to (0: not cut, the product of dali_hip_dgemm)
+size_t dgemm_shares_bytes(int M, int N, int K);
+int dgemm_shares(bool ta, bool tb, int M, int N, int K, const double* A, int lda, const double* B, int ldb, double beta, double* C, int ldc, void* parts);
 // hipFuncSetAttribute(MaxDynamicSharedMemorySize) once per kernel: later launches of that kernel, which may be recorded into a
 // graph, are launches only. Keyed on the kernel's address (kernels of one signature share a function type, so a flag inside a
 // generic lambda or template would be shared among them).
