@@ -1,0 +1,480 @@
+// Attention in fp32 on the bf16 matrix cores: every value is cut into three bf16 pieces that add up to it (as sgemm_split.hip does, after Henry, Tang and Heinecke, "Leveraging the
+// bfloat16 Artificial Intelligence Datatype For Higher-Precision Computations", 2019), and the six products of pieces of weight 2^-16 and more are summed in fp32. What
+// is left out comes to at most 2^-24 of a product, as much as rounding it once costs. A bf16 instruction does sixteen times the work of an fp32 one in the
+// same time, so six of them take 3/8 of its time.
+//
+// Operands are multiplied by 2^16 as they are cut and sums by a power of two afterwards, so that no value is too small for its pieces. Values from 2^112 on, sums from 2^96 on,
+// infinities and NaN leave something that is not finite behind: such a tile is taken again with the fp32 instructions on the values as they are, whatever that comes to.
+//
+// The arrangement is that of attention_tiles.h with instructions of 32x32x16: states by rows, a row of the problem (or a state, for the gradients of states) to a lane
+// (lane % 32), whose scores leave the instruction in the order in which the next product takes them as its right operand. Left operands lie in LDS as three planes of rows,
+// 16 bytes of padding behind each row: along a row they are read 16 bytes at a time, across rows by the transposing read, four rows of a column to a lane.
+#ifndef DALI_HIP_ATTENTION_SPLIT_H
+#define DALI_HIP_ATTENTION_SPLIT_H
+
+#include "attention_tiles.h"
+
+namespace dali_hip {
+namespace {
+
+typedef float floatx16 __attribute__((ext_vector_type(16)));
+typedef float floatx2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef unsigned int uintx4 __attribute__((ext_vector_type(4)));
+typedef short shortx4 __attribute__((ext_vector_type(4)));
+typedef short shortx8 __attribute__((ext_vector_type(8)));
+
+constexpr float kUp = 0x1p16f, kDown = 0x1p-16f, kDownTwice = 0x1p-32f;
+
+// two values' pieces, packed
+__device__ __forceinline__ void cut_pair(float a, float b, unsigned& h, unsigned& m, unsigned& l) {
+    const auto pack = [](float x, float y) { return __builtin_bit_cast(unsigned, __builtin_convertvector((floatx2{x, y}), bf16x2)); };
+    h = pack(a, b);
+    const float a1 = a - __uint_as_float(h << 16), b1 = b - __uint_as_float(h & 0xffff0000u);
+    m = pack(a1, b1);
+    const float a2 = a1 - __uint_as_float(m << 16), b2 = b1 - __uint_as_float(m & 0xffff0000u);
+    l = pack(a2, b2);
+}
+
+// eight neighbours along the inner extent, in pieces
+struct Pieces {
+    bf16x8 p[3];
+    __device__ __forceinline__ void cut(const float (&v)[8], float factor = 1.0f) {
+        uintx4 h, m, l;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            unsigned x, y, z;
+            cut_pair(v[2 * i] * factor, v[2 * i + 1] * factor, x, y, z);
+            h[i] = x, m[i] = y, l[i] = z;
+        }
+        p[0] = __builtin_bit_cast(bf16x8, h), p[1] = __builtin_bit_cast(bf16x8, m), p[2] = __builtin_bit_cast(bf16x8, l);
+    }
+};
+
+// the sum of products of pieces, the small ones first
+__device__ __forceinline__ floatx16 multiply(const Pieces& a, const Pieces& b, floatx16 c) {
+    c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.p[2], b.p[0], c, 0, 0, 0);
+    c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.p[0], b.p[2], c, 0, 0, 0);
+    c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.p[1], b.p[1], c, 0, 0, 0);
+    c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.p[1], b.p[0], c, 0, 0, 0);
+    c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.p[0], b.p[1], c, 0, 0, 0);
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.p[0], b.p[0], c, 0, 0, 0);
+}
+
+// eight values of a row, zeros past its end
+template <int D>
+__device__ __forceinline__ void row_eight(const float* row, int c, int width, float (&v)[8]) {
+    const auto a = row_group<D>(row, c, width), b = row_group<D>(row, c + 4, width);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = a[i], v[4 + i] = b[i];
+}
+
+// what a lane holds of 32 rows as a right operand: of row lane % 32, eight values of every sixteen
+template <int D>
+struct SplitFragment {
+    Pieces step[D / 16];
+    __device__ __forceinline__ void load(const float* row, int width, float factor) {
+        const int lane = threadIdx.x & 63;
+#pragma unroll
+        for (int s = 0; s < D / 16; ++s) {
+            float v[8];
+            row_eight<D>(row, 16 * s + 8 * (lane >> 5), width, v);
+            step[s].cut(v, factor);
+        }
+    }
+};
+
+// R rows of D values in LDS as three planes, brought there by 256 threads
+template <int D, int R>
+struct SplitStaged {
+    static constexpr int PITCH = 2 * D + 16, PLANE = R * PITCH, BYTES = 3 * PLANE, EIGHTS = D / 8, ALL = R * EIGHTS, EACH = (ALL + 255) / 256;
+    float v[EACH][8];
+    __device__ __forceinline__ void fetch(const float* base, const Rows& rows, int first, int end, int width) {
+#pragma unroll
+        for (int i = 0; i < EACH; ++i) {
+            const int at = threadIdx.x + i * 256, r = first + at / EIGHTS;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[i][j] = 0.0f;
+            if ((ALL % 256 == 0 || at < ALL) && r < end) row_eight<D>(base + rows.at(r), at % EIGHTS * 8, width, v[i]);
+        }
+    }
+    __device__ __forceinline__ void store(char* lds) const {
+#pragma unroll
+        for (int i = 0; i < EACH; ++i) {
+            const int at = threadIdx.x + i * 256;
+            if (ALL % 256 && at >= ALL) break;
+            char* to = lds + at / EIGHTS * PITCH + at % EIGHTS * 16;
+            Pieces p;
+            p.cut(v[i], kUp);
+#pragma unroll
+            for (int q = 0; q < 3; ++q) *reinterpret_cast<bf16x8*>(to + q * PLANE) = p.p[q];
+        }
+    }
+    // left operand along the rows: row r + lane % 32, values 16 s + 8 (lane / 32) ...
+    static __device__ __forceinline__ Pieces along(const char* lds, int r, int s) {
+        const int lane = threadIdx.x & 63;
+        const char* from = lds + (r + (lane & 31)) * PITCH + 32 * s + 16 * (lane >> 5);
+        Pieces p;
+#pragma unroll
+        for (int q = 0; q < 3; ++q) p.p[q] = *reinterpret_cast<const bf16x8*>(from + q * PLANE);
+        return p;
+    }
+    // Left operand across the rows: column c + lane % 32, of the 16 rows from r on those that a lane's scores are of: 4 (lane / 32) + (0..3) and 8 further. (Of 16 lanes that
+    // take part in one transposing read, lane i brings 8 bytes of row i / 4, and gets column i of the four rows.)
+    static __device__ __forceinline__ Pieces across(const char* lds, int r, int c) {
+        const int lane = threadIdx.x & 63;
+        const char* from = lds + (r + 4 * (lane >> 5) + ((lane & 15) >> 2)) * PITCH + 2 * (c + 16 * ((lane >> 4) & 1) + 4 * (lane & 3));
+        Pieces p;
+#pragma unroll
+        for (int q = 0; q < 3; ++q) {
+            typedef __attribute__((address_space(3))) shortx4 lds_four;
+            const shortx4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_four*)(from + q * PLANE));
+            const shortx4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_four*)(from + q * PLANE + 8 * PITCH));
+            p.p[q] = __builtin_bit_cast(bf16x8, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
+        }
+        return p;
+    }
+};
+
+// the weights of 16 states (or rows) as a right operand: the half `half` of what a lane holds of 32
+__device__ __forceinline__ Pieces weights_of(const floatx16& s, int half) {
+    float v[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = s[8 * half + i];
+    Pieces p;
+    p.cut(v);
+    return p;
+}
+
+// row of a tile's accumulator that a lane of half h holds in register v
+__device__ __forceinline__ int split_row(int v, int h) { return 8 * (v >> 2) + 4 * h + (v & 3); }
+
+// D columns of a transposed result
+template <int D>
+struct SplitColumns {
+    floatx16 acc[D / 32];
+    __device__ __forceinline__ void clear() {
+#pragma unroll
+        for (int b = 0; b < D / 32; ++b) acc[b] = floatx16{};
+    }
+    __device__ __forceinline__ void times(float f) {
+#pragma unroll
+        for (int b = 0; b < D / 32; ++b) acc[b] *= f;
+    }
+    __device__ __forceinline__ bool finite() const {
+        float probe = 0.0f;  // (0 * x is 0 for finite x and NaN else)
+#pragma unroll
+        for (int b = 0; b < D / 32; ++b)
+#pragma unroll
+            for (int v = 0; v < 16; ++v) probe = fmaf(acc[b][v], 0.0f, probe);
+        return probe == 0.0f;
+    }
+    template <typename F>
+    __device__ __forceinline__ void each(F f) const {
+        const int h = (threadIdx.x & 63) >> 5;
+#pragma unroll
+        for (int b = 0; b < D / 32; ++b)
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const float run[4] = {acc[b][4 * q], acc[b][4 * q + 1], acc[b][4 * q + 2], acc[b][4 * q + 3]};
+                f(32 * b + 8 * q + 4 * h, run);
+            }
+    }
+};
+
+// ------------------------------------------------------------------------------------------------ forward
+template <int D>
+struct SplitForward {
+    static constexpr int KT = ForwardShape<float, D>::KT;  // (the same: a tile that is taken again belongs to a part whose others are not)
+    static constexpr int LDS = 2 * SplitStaged<D, KT>::BYTES > ForwardShape<float, D>::LDS ? 2 * SplitStaged<D, KT>::BYTES : ForwardShape<float, D>::LDS;
+};
+
+// A workgroup of four waves takes 128 rows of a problem over a part of the states, a wave 32 of them.
+template <int D>
+__global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void attention_rows_split(Args a) {
+    constexpr int KT = SplitForward<D>::KT;
+    typedef SplitStaged<D, KT> Tile;
+    extern __shared__ __attribute__((aligned(16))) char attention_lds[];
+    char *ks = attention_lds, *vs = ks + Tile::BYTES;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5;
+    const int id = on_die(blockIdx.x, gridDim.x), at = id / (a.tiles * a.parts), rest = id - at * a.tiles * a.parts, part = rest / a.tiles, tile = rest - part * a.tiles;
+    const int problem = a.first + at, b = problem / a.kv_heads, kvh = problem - b * a.kv_heads;
+    const int n = count_of(a, b), slabs = (n + KT - 1) / KT;
+    const int begin = (int)((int64_t)slabs * part / a.parts), end = (int)((int64_t)slabs * (part + 1) / a.parts);
+    const float* q = (const float*)a.q.p + b * a.q.batch + (int64_t)kvh * a.group * a.q.head;
+    const float* k = (const float*)a.k.p + b * a.k.batch + kvh * a.k.head;
+    const float* v = (const float*)a.v.p + b * a.v.batch + kvh * a.v.head;
+    const Rows q_rows = {a.q.row, a.q.head, a.group}, k_rows = {a.k.row, 0, 1}, v_rows = {a.v.row, 0, 1};
+    const int row = tile * 128 + wave * 32 + (lane & 31);
+    SplitFragment<D> qf;
+    qf.load(q + q_rows.at(min(row, a.rows - 1)), a.width, (float)(a.scale * Matrix<float>::base * kUp));
+    SplitColumns<D> y;
+    y.clear();
+    float top = Matrix<float>::lowest, sum = 0;  // (of the scores as they are; of the lane's own states)
+    Tile kt, vt;
+    if (begin < end) {
+        kt.fetch(k, k_rows, begin * KT, n, a.width);
+        vt.fetch(v, v_rows, begin * KT, n, a.width);
+    }
+    for (int slab = begin; slab < end; ++slab) {
+        __syncthreads();
+        kt.store(ks);
+        vt.store(vs);
+        __syncthreads();
+        if (slab + 1 < end) {
+            kt.fetch(k, k_rows, (slab + 1) * KT, n, a.width);
+            vt.fetch(v, v_rows, (slab + 1) * KT, n, a.width);
+        }
+        floatx16 s[KT / 32];
+#pragma unroll
+        for (int t = 0; t < KT / 32; ++t) s[t] = floatx16{};
+#pragma unroll
+        for (int step = 0; step < D / 16; ++step)
+#pragma unroll
+            for (int t = 0; t < KT / 32; ++t) s[t] = multiply(Tile::along(ks, 32 * t, step), qf.step[step], s[t]);
+        if ((slab + 1) * KT > n) {
+#pragma unroll
+            for (int t = 0; t < KT / 32; ++t)
+#pragma unroll
+                for (int e = 0; e < 16; ++e)
+                    if (slab * KT + 32 * t + split_row(e, h) >= n) s[t][e] = -INFINITY;
+        }
+        float best = -INFINITY;
+#pragma unroll
+        for (int t = 0; t < KT / 32; ++t)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) best = fmaxf(best, s[t][e]);
+        best = fmaxf(top, fold_lanes<64, 32>(best, Max()) * kDownTwice);
+        if (__any(best > top)) {
+            const float again = Matrix<float>::weight(top - best);
+            sum *= again;
+            y.times(again);
+            top = best;
+        }
+#pragma unroll
+        for (int t = 0; t < KT / 32; ++t) {
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                s[t][e] = Matrix<float>::weight(fmaf(s[t][e], kDownTwice, -top));
+                sum += s[t][e];
+            }
+        }
+#pragma unroll
+        for (int t = 0; t < KT / 32; ++t)
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                const Pieces p = weights_of(s[t], half);
+#pragma unroll
+                for (int c = 0; c < D / 32; ++c) y.acc[c] = multiply(Tile::across(vs, 32 * t + 16 * half, 32 * c), p, y.acc[c]);
+            }
+    }
+    sum = fold_lanes<64, 32>(sum, Sum());
+    // (a sum of 0: scores that are all -inf, or below what their pieces hold)
+    const bool bad = begin < end && (!(sum > 0.0f && sum < INFINITY) || !y.finite());
+    if (__syncthreads_or(bad)) {
+        constexpr int STEP = 64 * ForwardShape<float, D>::RQ;
+        for (int r = 0; r < 128 && tile * 128 + r < a.rows; r += STEP) {
+            __syncthreads();
+            rows_tile<float, D>(a, attention_lds, problem, part, tile * 128 + r);
+        }
+        return;
+    }
+    if (row >= a.rows) return;
+    if (a.parts == 1) {
+        const int64_t to = dense_row<float>(a, b, kvh, row);
+        y.times(sum == 0.0f ? 0.0f : kDown / sum);
+        float* out = (float*)a.y_out + to * a.width;
+        y.each([&](int c, const auto& values) { store_run(out, c, a.width, values); });
+        if (h == 0) ((float*)a.lse_out)[to] = sum == 0.0f ? -INFINITY : Matrix<float>::lse(top, sum);
+    } else {
+        const int64_t to = ((int64_t)part * a.batch * a.kv_heads + problem) * a.rows + row;
+        float* out = (float*)a.parts_y + to * D;
+        y.times(kDown);
+        y.each([&](int c, const auto& values) { store_run(out, c, D, values); });
+        if (h == 0) ((float*)a.parts_m)[to] = top, ((float*)a.parts_l)[to] = sum;
+    }
+}
+
+// ------------------------------------------------------------------------------------------------ backward
+// The gradients of the states: a workgroup takes 128 states, a wave 32 of them in its registers, and walks over the rows, 32 at a time through LDS.
+template <int D>
+struct SplitStates {
+    static constexpr int RT = 32;
+    static constexpr int MINE = 2 * SplitStaged<D, RT>::BYTES + 2 * RT * 4, LDS = MINE > StatesShape<float, D>::LDS ? MINE : StatesShape<float, D>::LDS;
+};
+
+template <int D>
+__global__ __launch_bounds__(256, D <= 64 ? 2 : 1) void attention_states_gradient_split(Args a) {
+    constexpr int RT = SplitStates<D>::RT;
+    typedef SplitStaged<D, RT> Tile;
+    extern __shared__ __attribute__((aligned(16))) char attention_lds[];
+    char *qs = attention_lds, *gs = qs + Tile::BYTES;
+    float *levels = reinterpret_cast<float*>(gs + Tile::BYTES), *deltas = levels + RT;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5;
+    const int id = on_die(blockIdx.x, gridDim.x), at = id / a.tiles, tile = id - at * a.tiles;
+    const int problem = a.first + at, b = problem / a.kv_heads, kvh = problem - b * a.kv_heads;
+    const int n = count_of(a, b), key = tile * 128 + wave * 32 + (lane & 31);
+    const float* q = (const float*)a.q.p + b * a.q.batch + (int64_t)kvh * a.group * a.q.head;
+    const float* dy = (const float*)a.dy.p + b * a.dy.batch + (int64_t)kvh * a.group * a.dy.head;
+    const float* k = (const float*)a.k.p + b * a.k.batch + kvh * a.k.head;
+    const float* v = (const float*)a.v.p + b * a.v.batch + kvh * a.v.head;
+    const Rows q_rows = {a.q.row, a.q.head, a.group}, dy_rows = {a.dy.row, a.dy.head, a.group};
+    SplitColumns<D> dk, dv;
+    dk.clear();
+    dv.clear();
+    float extreme = 0.0f;
+    if (tile * 128 < n) {
+        SplitFragment<D> kf, vf;
+        kf.load(k + min(key, n - 1) * a.k.row, a.width, (float)(a.scale * Matrix<float>::base * kUp));
+        vf.load(v + min(key, n - 1) * a.v.row, a.width, kUp);
+        Tile qt, gt;
+        float level = 0, delta = 0;
+        auto fetch = [&](int r0) {
+            qt.fetch(q, q_rows, r0, a.rows, a.width);
+            gt.fetch(dy, dy_rows, r0, a.rows, a.width);
+            if (threadIdx.x < RT) {
+                const int r = r0 + threadIdx.x;
+                level = INFINITY, delta = 0;
+                if (r < a.rows) {
+                    const int64_t from = dense_row<float>(a, b, kvh, r);
+                    level = level_of(((const float*)a.lse)[from]);
+                    delta = ((const float*)a.delta)[from];
+                }
+            }
+        };
+        fetch(0);
+        for (int r0 = 0; r0 < a.rows; r0 += RT) {
+            __syncthreads();
+            qt.store(qs);
+            gt.store(gs);
+            if (threadIdx.x < RT) levels[threadIdx.x] = level, deltas[threadIdx.x] = delta;
+            __syncthreads();
+            if (r0 + RT < a.rows) fetch(r0 + RT);
+            floatx16 s = floatx16{}, dp = floatx16{};
+#pragma unroll
+            for (int step = 0; step < D / 16; ++step) {
+                s = multiply(Tile::along(qs, 0, step), kf.step[step], s);
+                dp = multiply(Tile::along(gs, 0, step), vf.step[step], dp);
+            }
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                const float lev = levels[split_row(e, h)], del = deltas[split_row(e, h)];
+                extreme = fmaxf(extreme, fabsf(s[e]));
+                s[e] = lev == INFINITY ? 0.0f : Matrix<float>::weight(fmaf(s[e], kDownTwice, 16.0f - lev));  // (times 2^16, as the pieces want it)
+                dp[e] = s[e] * fmaf(dp[e], kDownTwice, -del);
+            }
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                const Pieces p = weights_of(s, half), ds = weights_of(dp, half);
+#pragma unroll
+                for (int c = 0; c < D / 32; ++c) {
+                    dv.acc[c] = multiply(Tile::across(gs, 16 * half, 32 * c), p, dv.acc[c]);
+                    dk.acc[c] = multiply(Tile::across(qs, 16 * half, 32 * c), ds, dk.acc[c]);
+                }
+            }
+        }
+    }
+    if (__syncthreads_or(extreme == INFINITY || !dk.finite() || !dv.finite())) {
+        constexpr int STEP = 64 * StatesShape<float, D>::RK;
+        for (int r = 0; r < 128; r += STEP) {
+            __syncthreads();
+            states_gradient_tile<float, D, true, true>(a, attention_lds, problem, tile * 128 + r);
+        }
+        return;
+    }
+    if (key >= a.keys) return;
+    const int64_t to = (((int64_t)b * a.keys + key) * a.kv_heads + kvh) * a.width;
+    // (behind the last state: what its stand-in came to is not the gradient, which is zero)
+    dk.times(key < n ? (float)a.scale * kDownTwice : 0.0f);
+    dv.times(key < n ? kDownTwice : 0.0f);
+    dk.each([&](int c, const auto& values) { store_run((float*)a.dk + to, c, a.width, values); });
+    dv.each([&](int c, const auto& values) { store_run((float*)a.dv + to, c, a.width, values); });
+}
+
+// The gradient of the rows: as the forward pass, with the weights known from lse.
+template <int D>
+struct SplitRows {
+    static constexpr int KT = 32;
+    static constexpr int LDS = 2 * SplitStaged<D, KT>::BYTES > RowsShape<float, D>::LDS ? 2 * SplitStaged<D, KT>::BYTES : RowsShape<float, D>::LDS;
+};
+
+template <int D>
+__global__ __launch_bounds__(256, D <= 64 ? 2 : 1) void attention_rows_gradient_split(Args a) {
+    constexpr int KT = SplitRows<D>::KT;
+    typedef SplitStaged<D, KT> Tile;
+    extern __shared__ __attribute__((aligned(16))) char attention_lds[];
+    char *ks = attention_lds, *vs = ks + Tile::BYTES;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5;
+    const int id = on_die(blockIdx.x, gridDim.x), at = id / a.tiles, tile = id - at * a.tiles;
+    const int problem = a.first + at, b = problem / a.kv_heads, kvh = problem - b * a.kv_heads;
+    const int n = count_of(a, b), row = tile * 128 + wave * 32 + (lane & 31), mine = min(row, a.rows - 1);
+    const float* q = (const float*)a.q.p + b * a.q.batch + (int64_t)kvh * a.group * a.q.head;
+    const float* dy = (const float*)a.dy.p + b * a.dy.batch + (int64_t)kvh * a.group * a.dy.head;
+    const float* k = (const float*)a.k.p + b * a.k.batch + kvh * a.k.head;
+    const float* v = (const float*)a.v.p + b * a.v.batch + kvh * a.v.head;
+    const Rows q_rows = {a.q.row, a.q.head, a.group}, dy_rows = {a.dy.row, a.dy.head, a.group}, k_rows = {a.k.row, 0, 1}, v_rows = {a.v.row, 0, 1};
+    SplitFragment<D> qf, gf;
+    qf.load(q + q_rows.at(mine), a.width, (float)(a.scale * Matrix<float>::base * kUp));
+    gf.load(dy + dy_rows.at(mine), a.width, kUp);
+    const int64_t own = dense_row<float>(a, b, kvh, mine);
+    const float level = level_of(((const float*)a.lse)[own]), delta = ((const float*)a.delta)[own];
+    SplitColumns<D> dq;
+    dq.clear();
+    float extreme = 0.0f;
+    Tile kt, vt;
+    if (n > 0) {
+        kt.fetch(k, k_rows, 0, n, a.width);
+        vt.fetch(v, v_rows, 0, n, a.width);
+    }
+    for (int first = 0; first < n; first += KT) {
+        __syncthreads();
+        kt.store(ks);
+        vt.store(vs);
+        __syncthreads();
+        if (first + KT < n) {
+            kt.fetch(k, k_rows, first + KT, n, a.width);
+            vt.fetch(v, v_rows, first + KT, n, a.width);
+        }
+        floatx16 s = floatx16{}, dp = floatx16{};
+#pragma unroll
+        for (int step = 0; step < D / 16; ++step) {
+            s = multiply(Tile::along(ks, 0, step), qf.step[step], s);
+            dp = multiply(Tile::along(vs, 0, step), gf.step[step], dp);
+        }
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+            extreme = fmaxf(extreme, fabsf(s[e]));
+            const float p = Matrix<float>::weight(fmaf(s[e], kDownTwice, 16.0f - level));  // (times 2^16, as the pieces want it)
+            dp[e] = p * fmaf(dp[e], kDownTwice, -delta);
+        }
+        if (first + KT > n) {
+#pragma unroll
+            for (int e = 0; e < 16; ++e)
+                if (first + split_row(e, h) >= n) dp[e] = 0.0f;
+        }
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+            const Pieces ds = weights_of(dp, half);
+#pragma unroll
+            for (int c = 0; c < D / 32; ++c) dq.acc[c] = multiply(Tile::across(ks, 16 * half, 32 * c), ds, dq.acc[c]);
+        }
+    }
+    if (__syncthreads_or(extreme == INFINITY || !dq.finite())) {
+        constexpr int STEP = 64 * RowsShape<float, D>::RQ;
+        for (int r = 0; r < 128 && tile * 128 + r < a.rows; r += STEP) {
+            __syncthreads();
+            rows_gradient_tile<float, D>(a, attention_lds, problem, tile * 128 + r);
+        }
+        return;
+    }
+    if (row >= a.rows) return;
+    float* out = (float*)a.dq + own * a.width;
+    dq.times((float)a.scale * kDownTwice);
+    dq.each([&](int c, const auto& values) { store_run(out, c, a.width, values); });
+}
+
+}  // namespace
+}  // namespace dali_hip
+
+#endif

@@ -13,340 +13,35 @@
 #include <algorithm>
 #include <cmath>
 
-#include "row_math.h"
+#include "attention_split.h"
+#include "attention_tiles.h"
 
 namespace dali_hip {
 namespace {
 
-typedef float floatx4 __attribute__((ext_vector_type(4)));
-typedef double doublex4 __attribute__((ext_vector_type(4)));
-
-// The 16x16x4 matrix instruction: lane l holds a[l % 16][l / 16] and b[l / 16][l % 16], and of the result column l % 16, rows row_of(0..3, l / 16).
-// Exponents are those of 2 in fp32 (the instruction's base) and of e in fp64.
-template <typename T>
-struct Matrix;
-template <>
-struct Matrix<float> {
-    typedef floatx4 acc;
-    static constexpr float lowest = -3.402823466e+38f;
-    static constexpr double base = 1.4426950408889634074;  // exponents are counted in powers of 2
-    static __device__ __forceinline__ int row_of(int v, int g) { return 4 * g + v; }
-    static __device__ __forceinline__ acc mul(float a, float b, acc c) { return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0); }
-    static __device__ __forceinline__ float weight(float d) { return __builtin_amdgcn_exp2f(d); }
-    static __device__ __forceinline__ float lse(float top, float sum) { return (top + log2f(sum)) * 0.693147180559945309f; }
-};
-template <>
-struct Matrix<double> {
-    typedef doublex4 acc;
-    static constexpr double lowest = -1.7976931348623157e+308;
-    static constexpr double base = 1.0;
-    static __device__ __forceinline__ int row_of(int v, int g) { return 4 * v + g; }
-    static __device__ __forceinline__ acc mul(double a, double b, acc c) { return __builtin_amdgcn_mfma_f64_16x16x4f64(a, b, c, 0, 0, 0); }
-    static __device__ __forceinline__ double weight(double d) { return exp(d); }
-    static __device__ __forceinline__ double lse(double top, double sum) { return top + log(sum); }
-};
-
-struct Operand {
-    const void* p;
-    int64_t batch, row, head;  // strides in values
-};
-
-struct Args {
-    int batch, queries, keys, heads, kv_heads, width, group, rows;  // group: heads that share a kv head; rows: queries * group
-    Operand q, k, v, dy;
-    const int32_t* counts;
-    const void *y, *lse;  // dense
-    double scale;
-    void *y_out, *lse_out, *dq, *dk, *dv;  // dense
-    void* delta;                            // [batch, queries, heads]
-    // results of parts of the states (or rows): [part][problem][row][D], and maxima and sums [part][problem][row]
-    void *parts_y, *parts_m, *parts_l;
-    int parts, tiles;
-    unsigned* counters;  // of arrivals, counter_step words apart
-    int counter_step;
-    int first;  // problem of a launch's first workgroup
-};
-
-// Rows that neighbouring heads share: row r lies at position r / group of head r % group
-struct Rows {
-    int64_t row, head;
-    int group;
-    __device__ __forceinline__ int64_t at(int r) const {
-        if (group == 1) return r * row;
-        const int t = r / group;
-        return t * row + (r - t * group) * head;
-    }
-};
-
-__device__ __forceinline__ int count_of(const Args& a, int b) { return a.counts ? max(0, min(a.counts[b], a.keys)) : a.keys; }
-
-// neighbouring workgroups, which share operands, run on the same die (every eighth one does)
-__device__ __forceinline__ int on_die(int id, int total) {
-    const int per = total >> 3;
-    return id < per * 8 ? (id & 7) * per + (id >> 3) : id;
-}
-
-// A group of values of a row, zeros past the row's end
-template <int D, typename T>
-__device__ __forceinline__ typename Vec<T>::type row_group(const T* row, int c, int width) {
-    if (width == D) return *reinterpret_cast<const typename Vec<T>::type*>(row + c);
-    T v[Vec<T>::N];
-    typename Vec<T>::type g = {};
-    if (c < width) {
-        load_group(row, c, width, T(0), v);
-#pragma unroll
-        for (int i = 0; i < Vec<T>::N; ++i) g[i] = v[i];
-    }
-    return g;
-}
-
-// What a lane holds of 16 rows as a right operand: row lane % 16, groups lane / 16 of every four
-template <typename T, int D>
-struct Fragment {
-    static constexpr int N = Vec<T>::N, C = D / (4 * N);
-    typename Vec<T>::type g[C];
-    __device__ __forceinline__ void load(const T* row, int width, T factor) {
-        const int lane = threadIdx.x & 63;
-#pragma unroll
-        for (int c = 0; c < C; ++c) g[c] = row_group<D>(row, (4 * c + (lane >> 4)) * N, width) * factor;
-    }
-};
-
-// A tile of R rows of D values in LDS, a group of padding behind each row: sixteen rows' groups at one place lie in different banks
-template <typename T, int D, int R, int THREADS = 256>
-struct Staged {
-    static constexpr int N = Vec<T>::N, PITCH = D + N, GROUPS = D / N, EACH = R * GROUPS / THREADS;
-    static constexpr int BYTES = R * PITCH * sizeof(T);
-    static_assert(R * GROUPS % THREADS == 0, "whole groups to every thread");
-    typename Vec<T>::type g[EACH];
-    // rows [first, first + R) of those below `end`, zeros elsewhere
-    __device__ __forceinline__ void fetch(const T* base, const Rows& rows, int first, int end, int width) {
-#pragma unroll
-        for (int i = 0; i < EACH; ++i) {
-            const int at = threadIdx.x + i * THREADS, r = first + at / GROUPS, c = at % GROUPS * N;
-            g[i] = r < end ? row_group<D>(base + rows.at(r), c, width) : typename Vec<T>::type{};
-        }
-    }
-    __device__ __forceinline__ void store(T* lds) const {
-#pragma unroll
-        for (int i = 0; i < EACH; ++i) {
-            const int at = threadIdx.x + i * THREADS;
-            typedef T aligned_group __attribute__((ext_vector_type(16 / sizeof(T))));
-            *reinterpret_cast<aligned_group*>(lds + at / GROUPS * PITCH + at % GROUPS * N) = g[i];
-        }
-    }
-    // the left operand along the rows: row r + lane % 16, group 4 c + lane / 16
-    static __device__ __forceinline__ typename Vec<T>::type along(const T* lds, int r, int c) {
-        typedef T aligned_group __attribute__((ext_vector_type(16 / sizeof(T))));
-        const int lane = threadIdx.x & 63;
-        return *reinterpret_cast<const aligned_group*>(lds + (r + (lane & 15)) * PITCH + (4 * c + (lane >> 4)) * N);
-    }
-};
-
-// How the D columns of a transposed result lie in accumulators: block b, tile t of it (NV tiles to a block), row i of the tile: column (16 b + i) NV + t, so
-// that a lane reads the left operand of NV tiles, and writes NV neighbours of the result, at once.
-template <typename T, int D>
-struct Columns {
-    static constexpr int NV = D % (16 * Vec<T>::N) == 0 ? Vec<T>::N : Vec<T>::N / 2, BLOCKS = D / (16 * NV);
-    static_assert(D % (16 * NV) == 0, "whole blocks");
-    typedef T values __attribute__((ext_vector_type(NV)));
-    typename Matrix<T>::acc acc[BLOCKS][NV];
-    __device__ __forceinline__ void clear() {
-#pragma unroll
-        for (int b = 0; b < BLOCKS; ++b)
-#pragma unroll
-            for (int t = 0; t < NV; ++t) acc[b][t] = typename Matrix<T>::acc{};
-    }
-    __device__ __forceinline__ void times(T f) {
-#pragma unroll
-        for (int b = 0; b < BLOCKS; ++b)
-#pragma unroll
-            for (int t = 0; t < NV; ++t) acc[b][t] *= f;
-    }
-    // the left operand across rows: row `r`, the lane's values of block b
-    static __device__ __forceinline__ values across(const T* row, int b) { return *reinterpret_cast<const values*>(row + (16 * b + (threadIdx.x & 15)) * NV); }
-    // f(column, NV values) for every run of neighbours that the lane holds
-    template <typename F>
-    __device__ __forceinline__ void each(F f) const {
-        const int g = (threadIdx.x & 63) >> 4;
-#pragma unroll
-        for (int b = 0; b < BLOCKS; ++b)
-#pragma unroll
-            for (int v = 0; v < 4; ++v) {
-                T run[NV];
-#pragma unroll
-                for (int t = 0; t < NV; ++t) run[t] = acc[b][t][v];
-                f((16 * b + Matrix<T>::row_of(v, g)) * NV, run);
-            }
-    }
-};
-
-template <int NV, typename T>
-__device__ __forceinline__ void store_run(T* row, int c, int width, const T (&run)[NV]) {
-    typedef T values __attribute__((ext_vector_type(NV), aligned(sizeof(T))));
-    if (c + NV <= width) {
-        values g;
-#pragma unroll
-        for (int i = 0; i < NV; ++i) g[i] = run[i];
-        *reinterpret_cast<values*>(row + c) = g;
-    } else {
-#pragma unroll
-        for (int i = 0; i < NV; ++i)
-            if (c + i < width) row[c + i] = run[i];
-    }
-}
-
-// folds over the four lanes that hold a row
-template <typename T, typename Op>
-__device__ __forceinline__ T fold_row(T v, Op op) {
-    return fold_lanes<64, 16>(v, op);
-}
-
-// The running softmax of the row of a lane
-template <typename T>
-struct Running {
-    T top = Matrix<T>::lowest, sum = 0;  // (the sum of the lane's own states)
-    // takes the scores of a tile, which become weights; true where the sums so far have to be multiplied by `again`
-    template <int TILES>
-    __device__ __forceinline__ bool take(typename Matrix<T>::acc (&s)[TILES], T& again) {
-        T best = top;
-#pragma unroll
-        for (int t = 0; t < TILES; ++t)
-#pragma unroll
-            for (int v = 0; v < 4; ++v) best = Max()(best, s[t][v]);
-        best = fold_row(best, Max());
-        const bool rises = __any(best > top);
-        again = Matrix<T>::weight(top - best);
-        T here = 0;
-#pragma unroll
-        for (int t = 0; t < TILES; ++t)
-#pragma unroll
-            for (int v = 0; v < 4; ++v) {
-                s[t][v] = Matrix<T>::weight(s[t][v] - best);
-                here += s[t][v];
-            }
-        sum = sum * again + here;
-        top = best;
-        return rises;
-    }
-};
-
-template <typename T>
-__device__ __forceinline__ int64_t dense_row(const Args& a, int b, int kvh, int r) {
-    const int t = a.group == 1 ? r : r / a.group;
-    return ((int64_t)b * a.queries + t) * a.heads + (int64_t)kvh * a.group + (r - t * a.group);
-}
-
-// ------------------------------------------------------------------------------------------------ forward
-// A workgroup of four waves takes 64 RQ rows of a problem, a wave 16 RQ of them, over a part of the states, KT at a time through LDS.
-template <typename T, int D>
-struct ForwardShape {
-    static constexpr int KT = D * sizeof(T) <= 256 ? 64 : 32, RQ = D * sizeof(T) <= 512 ? 2 : 1;
-    static constexpr int LDS = 2 * Staged<T, D, KT>::BYTES;
-};
-
+// ------------------------------------------------------------------------------------------------ many rows
 template <typename T, int D>
 __global__ __launch_bounds__(256, D * sizeof(T) <= 1024 ? 2 : 1) void attention_rows(Args a) {
-    typedef Matrix<T> M;
-    typedef ForwardShape<T, D> S;
-    constexpr int KT = S::KT, RQ = S::RQ, N = Vec<T>::N, C = D / (4 * N);
     extern __shared__ __attribute__((aligned(16))) char attention_lds[];
-    T *ks = reinterpret_cast<T*>(attention_lds), *vs = ks + KT * Staged<T, D, KT>::PITCH;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4;
-    const int id = on_die(blockIdx.x, gridDim.x);
-    const int at = id / (a.tiles * a.parts), rest = id - at * a.tiles * a.parts, part = rest / a.tiles, tile = rest - part * a.tiles, problem = a.first + at;
-    const int b = problem / a.kv_heads, kvh = problem - b * a.kv_heads;
-    const int n = count_of(a, b), slabs = (n + KT - 1) / KT;
-    const int begin = (int)((int64_t)slabs * part / a.parts), end = (int)((int64_t)slabs * (part + 1) / a.parts);
-    const T* q = (const T*)a.q.p + b * a.q.batch + (int64_t)kvh * a.group * a.q.head;
-    const T* k = (const T*)a.k.p + b * a.k.batch + kvh * a.k.head;
-    const T* v = (const T*)a.v.p + b * a.v.batch + kvh * a.v.head;
-    const Rows q_rows = {a.q.row, a.q.head, a.group}, k_rows = {a.k.row, 0, 1}, v_rows = {a.v.row, 0, 1};
-    const int r0 = tile * 64 * RQ + wave * 16 * RQ;
-    Fragment<T, D> qf[RQ];
-#pragma unroll
-    for (int i = 0; i < RQ; ++i) qf[i].load(q + q_rows.at(min(r0 + 16 * i + (lane & 15), a.rows - 1)), a.width, (T)(a.scale * M::base));
-    Columns<T, D> y[RQ];
-    Running<T> run[RQ];
-#pragma unroll
-    for (int i = 0; i < RQ; ++i) y[i].clear();
-    Staged<T, D, KT> kt, vt;
-    if (begin < end) {
-        kt.fetch(k, k_rows, begin * KT, n, a.width);
-        vt.fetch(v, v_rows, begin * KT, n, a.width);
-    }
-    for (int slab = begin; slab < end; ++slab) {
-        __syncthreads();
-        kt.store(ks);
-        vt.store(vs);
-        __syncthreads();
-        if (slab + 1 < end) {
-            kt.fetch(k, k_rows, (slab + 1) * KT, n, a.width);
-            vt.fetch(v, v_rows, (slab + 1) * KT, n, a.width);
-        }
-        typename M::acc s[RQ][KT / 16];
-#pragma unroll
-        for (int t = 0; t < KT / 16; ++t) {
-#pragma unroll
-            for (int i = 0; i < RQ; ++i) s[i][t] = typename M::acc{};
-#pragma unroll
-            for (int c = 0; c < C; ++c) {
-                const typename Vec<T>::type left = Staged<T, D, KT>::along(ks, 16 * t, c);
-#pragma unroll
-                for (int e = 0; e < N; ++e)
-#pragma unroll
-                    for (int i = 0; i < RQ; ++i) s[i][t] = M::mul(left[e], qf[i].g[c][e], s[i][t]);
-            }
-        }
-        if ((slab + 1) * KT > n) {
-#pragma unroll
-            for (int t = 0; t < KT / 16; ++t)
-#pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    if (slab * KT + 16 * t + M::row_of(e, g) >= n)
-#pragma unroll
-                        for (int i = 0; i < RQ; ++i) s[i][t][e] = T(-INFINITY);
-        }
-#pragma unroll
-        for (int i = 0; i < RQ; ++i) {
-            T again;
-            if (run[i].template take<KT / 16>(s[i], again)) y[i].times(again);
-        }
-#pragma unroll
-        for (int t = 0; t < KT / 16; ++t)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const T* row = vs + (16 * t + M::row_of(e, g)) * Staged<T, D, KT>::PITCH;
-#pragma unroll
-                for (int blk = 0; blk < Columns<T, D>::BLOCKS; ++blk) {
-                    const auto left = Columns<T, D>::across(row, blk);
-#pragma unroll
-                    for (int c = 0; c < Columns<T, D>::NV; ++c)
-#pragma unroll
-                        for (int i = 0; i < RQ; ++i) y[i].acc[blk][c] = M::mul(left[c], s[i][t][e], y[i].acc[blk][c]);
-                }
-            }
-    }
-#pragma unroll
-    for (int i = 0; i < RQ; ++i) {
-        const int r = r0 + 16 * i + (lane & 15);
-        const T sum = fold_row(run[i].sum, Sum());
-        if (r >= a.rows) continue;
-        if (a.parts == 1) {
-            const int64_t to = dense_row<T>(a, b, kvh, r);
-            y[i].times(sum == T(0) ? T(0) : T(1) / sum);
-            T* out = (T*)a.y_out + to * a.width;
-            y[i].each([&](int c, const auto& values) { store_run(out, c, a.width, values); });
-            if (g == 0) ((T*)a.lse_out)[to] = sum == T(0) ? T(-INFINITY) : M::lse(run[i].top, sum);
-        } else {
-            const int64_t to = ((int64_t)part * a.batch * a.kv_heads + problem) * a.rows + r;
-            T* out = (T*)a.parts_y + to * D;
-            y[i].each([&](int c, const auto& values) { store_run(out, c, D, values); });
-            if (g == 0) ((T*)a.parts_m)[to] = run[i].top, ((T*)a.parts_l)[to] = sum;
-        }
-    }
+    const int id = on_die(blockIdx.x, gridDim.x), at = id / (a.tiles * a.parts), rest = id - at * a.tiles * a.parts, part = rest / a.tiles, tile = rest - part * a.tiles;
+    rows_tile<T, D>(a, attention_lds, a.first + at, part, tile * 64 * ForwardShape<T, D>::RQ);
 }
 
+template <typename T, int D, bool KEYS, bool VALUES>
+__global__ __launch_bounds__(256, D * sizeof(T) <= 512 ? 2 : 1) void attention_states_gradient(Args a) {
+    extern __shared__ __attribute__((aligned(16))) char attention_lds[];
+    const int id = on_die(blockIdx.x, gridDim.x), at = id / a.tiles, tile = id - at * a.tiles;
+    states_gradient_tile<T, D, KEYS, VALUES>(a, attention_lds, a.first + at, tile * 64 * StatesShape<T, D>::RK);
+}
+
+template <typename T, int D>
+__global__ __launch_bounds__(256, D * sizeof(T) <= 512 ? 2 : 1) void attention_rows_gradient(Args a) {
+    extern __shared__ __attribute__((aligned(16))) char attention_lds[];
+    const int id = on_die(blockIdx.x, gridDim.x), at = id / a.tiles, tile = id - at * a.tiles;
+    rows_gradient_tile<T, D>(a, attention_lds, a.first + at, tile * 64 * RowsShape<T, D>::RQ);
+}
+
+// ------------------------------------------------------------------------------------------------ few rows
 // Up to 16 RQ rows: nobody shares a state with another wave, so each of the four takes states of its own, straight from memory into the operands (16 at a time,
 // 64-byte pieces of a state), and they are joined in LDS.
 template <typename T, int D, int RQ>
@@ -565,7 +260,6 @@ __global__ __launch_bounds__(256) void attention_join(Args a) {
     if (lane == 0) ((T*)a.lse_out)[to] = sum == T(0) ? T(-INFINITY) : M::lse(top, sum);
 }
 
-// ------------------------------------------------------------------------------------------------ backward
 // delta = dy.y of every row: 16 lanes to a row
 template <typename T>
 __global__ __launch_bounds__(256) void attention_delta(Args a, int64_t first) {
@@ -587,248 +281,6 @@ __global__ __launch_bounds__(256) void attention_delta(Args a, int64_t first) {
     }
     sum = fold_lanes<16>(sum, Sum());
     if (there && threadIdx.x % 16 == 0) ((T*)a.delta)[row] = sum;
-}
-
-// what weights of a row are relative to: a row without weight has none anywhere
-template <typename T>
-__device__ __forceinline__ T level_of(T lse) {
-    return lse == T(-INFINITY) ? T(INFINITY) : lse * (T)Matrix<T>::base;
-}
-
-// The gradients of the states: a workgroup takes 64 RK states, a wave 16 RK of them in its registers, and walks over the rows, RT at a time through LDS.
-// KEYS, VALUES: which of dk and dv it forms.
-template <typename T, int D>
-struct StatesShape {
-    static constexpr int RT = 32, RK = D * sizeof(T) <= 256 ? 2 : 1;
-    static constexpr bool BOTH = D * sizeof(T) <= 1024;  // both gradients' sums and both operands fit a wave's registers
-    static constexpr int LDS = 2 * Staged<T, D, RT>::BYTES + 2 * RT * (int)sizeof(T);
-};
-
-template <typename T, int D, bool KEYS, bool VALUES>
-__global__ __launch_bounds__(256, D * sizeof(T) <= 512 ? 2 : 1) void attention_states_gradient(Args a) {
-    typedef Matrix<T> M;
-    typedef StatesShape<T, D> S;
-    constexpr int RT = S::RT, RK = S::RK, N = Vec<T>::N, C = D / (4 * N), PITCH = Staged<T, D, RT>::PITCH;
-    extern __shared__ __attribute__((aligned(16))) char attention_lds[];
-    T *qs = reinterpret_cast<T*>(attention_lds), *gs = qs + RT * PITCH, *levels = gs + RT * PITCH, *deltas = levels + RT;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4;
-    const int id = on_die(blockIdx.x, gridDim.x);
-    const int at = id / a.tiles, tile = id - at * a.tiles, problem = a.first + at;
-    const int b = problem / a.kv_heads, kvh = problem - b * a.kv_heads;
-    const int n = count_of(a, b), k0 = tile * 64 * RK + wave * 16 * RK;
-    const T* q = (const T*)a.q.p + b * a.q.batch + (int64_t)kvh * a.group * a.q.head;
-    const T* dy = (const T*)a.dy.p + b * a.dy.batch + (int64_t)kvh * a.group * a.dy.head;
-    const T* k = (const T*)a.k.p + b * a.k.batch + kvh * a.k.head;
-    const T* v = (const T*)a.v.p + b * a.v.batch + kvh * a.v.head;
-    const Rows q_rows = {a.q.row, a.q.head, a.group}, dy_rows = {a.dy.row, a.dy.head, a.group};
-    Columns<T, D> dk[KEYS ? RK : 1], dv[VALUES ? RK : 1];
-    if (KEYS)
-#pragma unroll
-        for (int i = 0; i < RK; ++i) dk[i].clear();
-    if (VALUES)
-#pragma unroll
-        for (int i = 0; i < RK; ++i) dv[i].clear();
-    if (tile * 64 * RK < n) {
-        Fragment<T, D> kf[RK], vf[KEYS ? RK : 1];
-#pragma unroll
-        for (int i = 0; i < RK; ++i) {
-            const int key = min(k0 + 16 * i + (lane & 15), n - 1);
-            kf[i].load(k + key * a.k.row, a.width, (T)(a.scale * M::base));
-            if (KEYS) vf[i].load(v + key * a.v.row, a.width, T(1));
-        }
-        Staged<T, D, RT> qt, gt;
-        T level = 0, delta = 0;
-        auto fetch = [&](int r0) {
-            qt.fetch(q, q_rows, r0, a.rows, a.width);
-            gt.fetch(dy, dy_rows, r0, a.rows, a.width);
-            if (threadIdx.x < RT) {
-                const int r = r0 + threadIdx.x;
-                level = T(INFINITY), delta = 0;
-                if (r < a.rows) {
-                    const int64_t at = dense_row<T>(a, b, kvh, r);
-                    level = level_of(((const T*)a.lse)[at]);
-                    delta = ((const T*)a.delta)[at];
-                }
-            }
-        };
-        fetch(0);
-        for (int r0 = 0; r0 < a.rows; r0 += RT) {
-            __syncthreads();
-            qt.store(qs);
-            gt.store(gs);
-            if (threadIdx.x < RT) levels[threadIdx.x] = level, deltas[threadIdx.x] = delta;
-            __syncthreads();
-            if (r0 + RT < a.rows) fetch(r0 + RT);
-#pragma unroll
-            for (int t = 0; t < RT / 16; ++t) {
-                typename M::acc s[RK], dp[RK];
-#pragma unroll
-                for (int i = 0; i < RK; ++i) s[i] = dp[i] = typename M::acc{};
-#pragma unroll
-                for (int c = 0; c < C; ++c) {
-                    const typename Vec<T>::type left = Staged<T, D, RT>::along(qs, 16 * t, c);
-#pragma unroll
-                    for (int e = 0; e < N; ++e)
-#pragma unroll
-                        for (int i = 0; i < RK; ++i) s[i] = M::mul(left[e], kf[i].g[c][e], s[i]);
-                    if (KEYS) {
-                        const typename Vec<T>::type down = Staged<T, D, RT>::along(gs, 16 * t, c);
-#pragma unroll
-                        for (int e = 0; e < N; ++e)
-#pragma unroll
-                            for (int i = 0; i < RK; ++i) dp[i] = M::mul(down[e], vf[i].g[c][e], dp[i]);
-                    }
-                }
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const int r = 16 * t + M::row_of(e, g);
-                    const T lev = levels[r], del = KEYS ? deltas[r] : T(0);
-#pragma unroll
-                    for (int i = 0; i < RK; ++i) {
-                        s[i][e] = lev == T(INFINITY) ? T(0) : M::weight(s[i][e] - lev);
-                        dp[i][e] = s[i][e] * (dp[i][e] - del);
-                    }
-                }
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const int r = 16 * t + M::row_of(e, g);
-#pragma unroll
-                    for (int blk = 0; blk < Columns<T, D>::BLOCKS; ++blk) {
-                        if (VALUES) {
-                            const auto left = Columns<T, D>::across(gs + r * PITCH, blk);
-#pragma unroll
-                            for (int c = 0; c < Columns<T, D>::NV; ++c)
-#pragma unroll
-                                for (int i = 0; i < RK; ++i) dv[i].acc[blk][c] = M::mul(left[c], s[i][e], dv[i].acc[blk][c]);
-                        }
-                        if (KEYS) {
-                            const auto left = Columns<T, D>::across(qs + r * PITCH, blk);
-#pragma unroll
-                            for (int c = 0; c < Columns<T, D>::NV; ++c)
-#pragma unroll
-                                for (int i = 0; i < RK; ++i) dk[i].acc[blk][c] = M::mul(left[c], dp[i][e], dk[i].acc[blk][c]);
-                        }
-                    }
-                }
-            }
-        }
-    }
-#pragma unroll
-    for (int i = 0; i < RK; ++i) {
-        const int key = k0 + 16 * i + (lane & 15);
-        if (key >= a.keys) continue;
-        const int64_t to = (((int64_t)b * a.keys + key) * a.kv_heads + kvh) * a.width;
-        // (behind the last state: what its stand-in came to is not the gradient, which is zero)
-        const bool there = key < n;
-        auto put = [&](T* out, const Columns<T, D>& sums, T factor) {
-            sums.each([&](int c, const auto& values) {
-                T run[Columns<T, D>::NV];
-#pragma unroll
-                for (int e = 0; e < Columns<T, D>::NV; ++e) run[e] = there ? values[e] * factor : T(0);
-                store_run(out + to, c, a.width, run);
-            });
-        };
-        if (KEYS) put((T*)a.dk, dk[i], (T)a.scale);
-        if (VALUES) put((T*)a.dv, dv[i], T(1));
-    }
-}
-
-// The gradient of the rows: as the forward pass, with the weights known from lse.
-template <typename T, int D>
-struct RowsShape {
-    static constexpr int KT = 32, RQ = D * sizeof(T) <= 256 ? 2 : 1;
-    static constexpr int LDS = 2 * Staged<T, D, KT>::BYTES;
-};
-
-template <typename T, int D>
-__global__ __launch_bounds__(256, D * sizeof(T) <= 512 ? 2 : 1) void attention_rows_gradient(Args a) {
-    typedef Matrix<T> M;
-    typedef RowsShape<T, D> S;
-    constexpr int KT = S::KT, RQ = S::RQ, N = Vec<T>::N, C = D / (4 * N), PITCH = Staged<T, D, KT>::PITCH;
-    extern __shared__ __attribute__((aligned(16))) char attention_lds[];
-    T *ks = reinterpret_cast<T*>(attention_lds), *vs = ks + KT * PITCH;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4;
-    const int id = on_die(blockIdx.x, gridDim.x);
-    const int at = id / a.tiles, tile = id - at * a.tiles, problem = a.first + at;
-    const int b = problem / a.kv_heads, kvh = problem - b * a.kv_heads;
-    const int n = count_of(a, b);
-    const T* q = (const T*)a.q.p + b * a.q.batch + (int64_t)kvh * a.group * a.q.head;
-    const T* dy = (const T*)a.dy.p + b * a.dy.batch + (int64_t)kvh * a.group * a.dy.head;
-    const T* k = (const T*)a.k.p + b * a.k.batch + kvh * a.k.head;
-    const T* v = (const T*)a.v.p + b * a.v.batch + kvh * a.v.head;
-    const Rows q_rows = {a.q.row, a.q.head, a.group}, dy_rows = {a.dy.row, a.dy.head, a.group}, k_rows = {a.k.row, 0, 1}, v_rows = {a.v.row, 0, 1};
-    const int r0 = tile * 64 * RQ + wave * 16 * RQ;
-    Fragment<T, D> qf[RQ], gf[RQ];
-    Columns<T, D> dq[RQ];
-    T level[RQ], delta[RQ];
-#pragma unroll
-    for (int i = 0; i < RQ; ++i) {
-        const int r = min(r0 + 16 * i + (lane & 15), a.rows - 1);
-        qf[i].load(q + q_rows.at(r), a.width, (T)(a.scale * M::base));
-        gf[i].load(dy + dy_rows.at(r), a.width, T(1));
-        const int64_t at = dense_row<T>(a, b, kvh, r);
-        level[i] = level_of(((const T*)a.lse)[at]);
-        delta[i] = ((const T*)a.delta)[at];
-        dq[i].clear();
-    }
-    Staged<T, D, KT> kt, vt;
-    if (n > 0) {
-        kt.fetch(k, k_rows, 0, n, a.width);
-        vt.fetch(v, v_rows, 0, n, a.width);
-    }
-    for (int first = 0; first < n; first += KT) {
-        __syncthreads();
-        kt.store(ks);
-        vt.store(vs);
-        __syncthreads();
-        if (first + KT < n) {
-            kt.fetch(k, k_rows, first + KT, n, a.width);
-            vt.fetch(v, v_rows, first + KT, n, a.width);
-        }
-#pragma unroll
-        for (int t = 0; t < KT / 16; ++t) {
-            typename M::acc s[RQ], dp[RQ];
-#pragma unroll
-            for (int i = 0; i < RQ; ++i) s[i] = dp[i] = typename M::acc{};
-#pragma unroll
-            for (int c = 0; c < C; ++c) {
-                const typename Vec<T>::type left = Staged<T, D, KT>::along(ks, 16 * t, c), down = Staged<T, D, KT>::along(vs, 16 * t, c);
-#pragma unroll
-                for (int e = 0; e < N; ++e)
-#pragma unroll
-                    for (int i = 0; i < RQ; ++i) {
-                        s[i] = M::mul(left[e], qf[i].g[c][e], s[i]);
-                        dp[i] = M::mul(down[e], gf[i].g[c][e], dp[i]);
-                    }
-            }
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const bool there = first + 16 * t + M::row_of(e, g) < n;
-#pragma unroll
-                for (int i = 0; i < RQ; ++i) dp[i][e] = there ? M::weight(s[i][e] - level[i]) * (dp[i][e] - delta[i]) : T(0);
-            }
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const T* row = ks + (16 * t + M::row_of(e, g)) * PITCH;
-#pragma unroll
-                for (int blk = 0; blk < Columns<T, D>::BLOCKS; ++blk) {
-                    const auto left = Columns<T, D>::across(row, blk);
-#pragma unroll
-                    for (int c = 0; c < Columns<T, D>::NV; ++c)
-#pragma unroll
-                        for (int i = 0; i < RQ; ++i) dq[i].acc[blk][c] = M::mul(left[c], dp[i][e], dq[i].acc[blk][c]);
-                }
-            }
-        }
-    }
-#pragma unroll
-    for (int i = 0; i < RQ; ++i) {
-        const int r = r0 + 16 * i + (lane & 15);
-        if (r >= a.rows) continue;
-        T* out = (T*)a.dq + dense_row<T>(a, b, kvh, r) * a.width;
-        dq[i].times((T)a.scale);
-        dq[i].each([&](int c, const auto& values) { store_run(out, c, a.width, values); });
-    }
 }
 
 // ------------------------------------------------------------------------------------------------ launches (host)
@@ -853,7 +305,8 @@ struct ForwardPlan {
         const int64_t problems = (int64_t)a.batch * a.kv_heads;
         few = a.rows <= (D * sizeof(T) <= 512 ? 32 : 16);  // (wider rows: 32 would not fit a wave's registers)
         rq = a.rows <= 16 ? 1 : 2;
-        tiles = few ? 1 : (a.rows + 64 * S::RQ - 1) / (64 * S::RQ);
+        const int rows = std::is_same_v<T, float> ? 128 : 64 * S::RQ;
+        tiles = few ? 1 : (a.rows + rows - 1) / rows;
         parts = few ? parts_for(problems, (a.keys + 63) / 64, 3, 2) : parts_for(problems * tiles, (a.keys + S::KT - 1) / S::KT, 2, 4);
     }
 };
@@ -920,9 +373,13 @@ int forward(const char* what, Args a) {
         a.counter_step = counter_step(problems);
     }
     const int few_lds = 16 * plan.rq * (D + Vec<T>::N + 8) * (int)sizeof(T);
-    const int status = plan.few ? (plan.rq == 1 ? launch(what, attention_few<T, D, 1>, problems, plan.parts, few_lds, a)
-                                                : launch(what, attention_few<T, D, 2>, problems, plan.parts, few_lds, a))
-                                : launch(what, attention_rows<T, D>, problems, plan.tiles * plan.parts, ForwardShape<T, D>::LDS, a);
+    int status;
+    if (plan.few)
+        status = plan.rq == 1 ? launch(what, attention_few<T, D, 1>, problems, plan.parts, few_lds, a) : launch(what, attention_few<T, D, 2>, problems, plan.parts, few_lds, a);
+    else if constexpr (std::is_same_v<T, float>)
+        status = launch(what, attention_rows_split<D>, problems, plan.tiles * plan.parts, SplitForward<D>::LDS, a);
+    else
+        status = launch(what, attention_rows<T, D>, problems, plan.tiles * plan.parts, ForwardShape<T, D>::LDS, a);
     if (status || plan.parts == 1 || plan.few) return status;
     return launch(what, attention_join<T, D>, 1, (problems * a.rows + 3) / 4, 0, a);
 }
@@ -934,6 +391,14 @@ int backward(const char* what, Args a) {
     for (int64_t first = 0; first < rows; first += most) {
         attention_delta<T><<<dim3((unsigned)((std::min(rows - first, most) + 15) / 16)), dim3(256), 0, stream()>>>(a, first);
         if (launched(what)) return DALI_HIP_ERROR;
+    }
+    if constexpr (std::is_same_v<T, float> && D <= 128) {
+        if (a.keys > 0) {
+            a.tiles = (a.keys + 127) / 128;
+            if (launch(what, attention_states_gradient_split<D>, problems, a.tiles, SplitStates<D>::LDS, a)) return DALI_HIP_ERROR;
+        }
+        a.tiles = (a.rows + 127) / 128;
+        return rows == 0 ? DALI_HIP_OK : launch(what, attention_rows_gradient_split<D>, problems, a.tiles, SplitRows<D>::LDS, a);
     }
     if (a.keys > 0) {
         typedef StatesShape<T, D> S;
