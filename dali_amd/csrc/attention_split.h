@@ -297,7 +297,7 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void attention_rows_split(Ar
 }
 
 // ------------------------------------------------------------------------------------------------ backward
-// The gradients of the states: a workgroup takes 128 states, a wave 32 of them in its registers, and walks over the rows, 32 at a time through LDS.
+// The gradients of the states: a workgroup takes 128 states, a wave 32 of them in its registers, and walks over the rows of a part, 32 at a time through LDS.
 template <int D>
 struct SplitStates {
     static constexpr int RT = 32;
@@ -312,9 +312,10 @@ __global__ __launch_bounds__(256, D <= 64 ? 2 : 1) void attention_states_gradien
     char *qs = attention_lds, *gs = qs + Tile::BYTES;
     float *levels = reinterpret_cast<float*>(gs + Tile::BYTES), *deltas = levels + RT;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5;
-    const int id = on_die(blockIdx.x, gridDim.x), at = id / a.tiles, tile = id - at * a.tiles;
+    const int id = on_die(blockIdx.x, gridDim.x), at = id / (a.tiles * a.parts), rest = id - at * a.tiles * a.parts, part = rest / a.tiles, tile = rest - part * a.tiles;
     const int problem = a.first + at, b = problem / a.kv_heads, kvh = problem - b * a.kv_heads;
     const int n = count_of(a, b), key = tile * 128 + wave * 32 + (lane & 31);
+    const int begin = part_of(a, part, a.rows, RT), end = part_of(a, part + 1, a.rows, RT);
     const float* q = (const float*)a.q.p + b * a.q.batch + (int64_t)kvh * a.group * a.q.head;
     const float* dy = (const float*)a.dy.p + b * a.dy.batch + (int64_t)kvh * a.group * a.dy.head;
     const float* k = (const float*)a.k.p + b * a.k.batch + kvh * a.k.head;
@@ -324,38 +325,39 @@ __global__ __launch_bounds__(256, D <= 64 ? 2 : 1) void attention_states_gradien
     dk.clear();
     dv.clear();
     float extreme = 0.0f;
-    if (tile * 128 < n) {
+    if (tile * 128 < n && begin < end) {
         SplitFragment<D> kf, vf;
         kf.load(k + min(key, n - 1) * a.k.row, a.width, (float)(a.scale * Matrix<float>::base * kUp));
         vf.load(v + min(key, n - 1) * a.v.row, a.width, kUp);
         Tile qt, gt;
         float level = 0, delta = 0;
         auto fetch = [&](int r0) {
-            qt.fetch(q, q_rows, r0, a.rows, a.width);
-            gt.fetch(dy, dy_rows, r0, a.rows, a.width);
+            qt.fetch(q, q_rows, r0, end, a.width);
+            gt.fetch(dy, dy_rows, r0, end, a.width);
             if (threadIdx.x < RT) {
                 const int r = r0 + threadIdx.x;
                 level = INFINITY, delta = 0;
-                if (r < a.rows) {
+                if (r < end) {
                     const int64_t from = dense_row<float>(a, b, kvh, r);
                     level = level_of(((const float*)a.lse)[from]);
                     delta = ((const float*)a.delta)[from];
                 }
             }
         };
-        fetch(0);
-        for (int r0 = 0; r0 < a.rows; r0 += RT) {
+        fetch(begin);
+        for (int r0 = begin; r0 < end; r0 += RT) {
             __syncthreads();
             qt.store(qs);
             gt.store(gs);
             if (threadIdx.x < RT) levels[threadIdx.x] = level, deltas[threadIdx.x] = delta;
             __syncthreads();
-            if (r0 + RT < a.rows) fetch(r0 + RT);
+            if (r0 + RT < end) fetch(r0 + RT);
             floatx16 s = floatx16{}, dp = floatx16{};
 #pragma unroll
             for (int step = 0; step < D / 16; ++step) {
                 s = multiply(Tile::along(qs, 0, step), kf.step[step], s);
                 dp = multiply(Tile::along(gs, 0, step), vf.step[step], dp);
+                __builtin_amdgcn_sched_barrier(0);  // (operands of one step at a time: there are no registers for more)
             }
 #pragma unroll
             for (int e = 0; e < 16; ++e) {
@@ -364,6 +366,7 @@ __global__ __launch_bounds__(256, D <= 64 ? 2 : 1) void attention_states_gradien
                 s[e] = lev == INFINITY ? 0.0f : Matrix<float>::weight(fmaf(s[e], kDownTwice, 16.0f - lev));  // (times 2^16, as the pieces want it)
                 dp[e] = s[e] * fmaf(dp[e], kDownTwice, -del);
             }
+            __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
             for (int half = 0; half < 2; ++half) {
                 const Pieces p = weights_of(s, half), ds = weights_of(dp, half);
@@ -371,6 +374,7 @@ __global__ __launch_bounds__(256, D <= 64 ? 2 : 1) void attention_states_gradien
                 for (int c = 0; c < D / 32; ++c) {
                     dv.acc[c] = multiply(Tile::across(gs, 16 * half, 32 * c), p, dv.acc[c]);
                     dk.acc[c] = multiply(Tile::across(qs, 16 * half, 32 * c), ds, dk.acc[c]);
+                    __builtin_amdgcn_sched_barrier(0);
                 }
             }
         }
@@ -379,12 +383,12 @@ __global__ __launch_bounds__(256, D <= 64 ? 2 : 1) void attention_states_gradien
         constexpr int STEP = 64 * StatesShape<float, D>::RK;
         for (int r = 0; r < 128; r += STEP) {
             __syncthreads();
-            states_gradient_tile<float, D, true, true>(a, attention_lds, problem, tile * 128 + r);
+            states_gradient_tile<float, D, true, true>(a, attention_lds, problem, part, tile * 128 + r);
         }
         return;
     }
     if (key >= a.keys) return;
-    const int64_t to = (((int64_t)b * a.keys + key) * a.kv_heads + kvh) * a.width;
+    const int64_t to = part * a.part_size + (((int64_t)b * a.keys + key) * a.kv_heads + kvh) * a.width;
     // (behind the last state: what its stand-in came to is not the gradient, which is zero)
     dk.times(key < n ? (float)a.scale * kDownTwice : 0.0f);
     dv.times(key < n ? kDownTwice : 0.0f);
@@ -406,9 +410,10 @@ __global__ __launch_bounds__(256, D <= 64 ? 2 : 1) void attention_rows_gradient_
     extern __shared__ __attribute__((aligned(16))) char attention_lds[];
     char *ks = attention_lds, *vs = ks + Tile::BYTES;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5;
-    const int id = on_die(blockIdx.x, gridDim.x), at = id / a.tiles, tile = id - at * a.tiles;
+    const int id = on_die(blockIdx.x, gridDim.x), at = id / (a.tiles * a.parts), rest = id - at * a.tiles * a.parts, part = rest / a.tiles, tile = rest - part * a.tiles;
     const int problem = a.first + at, b = problem / a.kv_heads, kvh = problem - b * a.kv_heads;
     const int n = count_of(a, b), row = tile * 128 + wave * 32 + (lane & 31), mine = min(row, a.rows - 1);
+    const int begin = part_of(a, part, n, KT), end = part_of(a, part + 1, n, KT);
     const float* q = (const float*)a.q.p + b * a.q.batch + (int64_t)kvh * a.group * a.q.head;
     const float* dy = (const float*)a.dy.p + b * a.dy.batch + (int64_t)kvh * a.group * a.dy.head;
     const float* k = (const float*)a.k.p + b * a.k.batch + kvh * a.k.head;
@@ -423,18 +428,18 @@ __global__ __launch_bounds__(256, D <= 64 ? 2 : 1) void attention_rows_gradient_
     dq.clear();
     float extreme = 0.0f;
     Tile kt, vt;
-    if (n > 0) {
-        kt.fetch(k, k_rows, 0, n, a.width);
-        vt.fetch(v, v_rows, 0, n, a.width);
+    if (begin < end) {
+        kt.fetch(k, k_rows, begin, end, a.width);
+        vt.fetch(v, v_rows, begin, end, a.width);
     }
-    for (int first = 0; first < n; first += KT) {
+    for (int first = begin; first < end; first += KT) {
         __syncthreads();
         kt.store(ks);
         vt.store(vs);
         __syncthreads();
-        if (first + KT < n) {
-            kt.fetch(k, k_rows, first + KT, n, a.width);
-            vt.fetch(v, v_rows, first + KT, n, a.width);
+        if (first + KT < end) {
+            kt.fetch(k, k_rows, first + KT, end, a.width);
+            vt.fetch(v, v_rows, first + KT, end, a.width);
         }
         floatx16 s = floatx16{}, dp = floatx16{};
 #pragma unroll
@@ -448,10 +453,10 @@ __global__ __launch_bounds__(256, D <= 64 ? 2 : 1) void attention_rows_gradient_
             const float p = Matrix<float>::weight(fmaf(s[e], kDownTwice, 16.0f - level));  // (times 2^16, as the pieces want it)
             dp[e] = p * fmaf(dp[e], kDownTwice, -delta);
         }
-        if (first + KT > n) {
+        if (first + KT > end) {
 #pragma unroll
             for (int e = 0; e < 16; ++e)
-                if (first + split_row(e, h) >= n) dp[e] = 0.0f;
+                if (first + split_row(e, h) >= end) dp[e] = 0.0f;
         }
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
@@ -464,12 +469,12 @@ __global__ __launch_bounds__(256, D <= 64 ? 2 : 1) void attention_rows_gradient_
         constexpr int STEP = 64 * RowsShape<float, D>::RQ;
         for (int r = 0; r < 128 && tile * 128 + r < a.rows; r += STEP) {
             __syncthreads();
-            rows_gradient_tile<float, D>(a, attention_lds, problem, tile * 128 + r);
+            rows_gradient_tile<float, D>(a, attention_lds, problem, part, tile * 128 + r);
         }
         return;
     }
     if (row >= a.rows) return;
-    float* out = (float*)a.dq + own * a.width;
+    float* out = (float*)a.dq + part * a.part_size + own * a.width;
     dq.times((float)a.scale * kDownTwice);
     dq.each([&](int c, const auto& values) { store_run(out, c, a.width, values); });
 }

@@ -1,5 +1,5 @@
 // What the kernels of attention share: the operands of a call, tiles of them in registers and LDS, the running softmax, and what a workgroup does for a tile of rows or of
-// states in the type's own arithmetic (cross_attention.hip; cross_attention_split.hip, where its own does not serve).
+// states in the type's own arithmetic (cross_attention.hip; attention_split.h, where its own does not serve).
 #ifndef DALI_HIP_ATTENTION_TILES_H
 #define DALI_HIP_ATTENTION_TILES_H
 
@@ -51,6 +51,7 @@ struct Args {
     void* delta;                            // [batch, queries, heads]
     // results of parts of the states (or rows): [part][problem][row][D], and maxima and sums [part][problem][row]
     void *parts_y, *parts_m, *parts_l;
+    int64_t part_size;  // of the gradients: values from one part's to the next one's, which lie as the gradients do
     int parts, tiles;
     unsigned* counters;  // of arrivals, counter_step words apart
     int counter_step;
@@ -335,13 +336,16 @@ __device__ __forceinline__ void rows_tile(const Args& a, char* lds, int problem,
 }
 
 // ------------------------------------------------------------------------------------------------ backward
+// where part `part` of `n` rows or states begins: on whole slabs
+__device__ __forceinline__ int part_of(const Args& a, int part, int n, int slab) { return min(n, (int)((int64_t)((n + slab - 1) / slab) * part / a.parts) * slab); }
+
 // what weights of a row are relative to: a row without weight has none anywhere
 template <typename T>
 __device__ __forceinline__ T level_of(T lse) {
     return lse == T(-INFINITY) ? T(INFINITY) : lse * (T)Matrix<T>::base;
 }
 
-// The gradients of the states: a workgroup takes 64 RK states, a wave 16 RK of them in its registers, and walks over the rows, RT at a time through LDS.
+// The gradients of the states: a workgroup takes 64 RK states, a wave 16 RK of them in its registers, and walks over the rows of a part of them, RT at a time through LDS.
 // KEYS, VALUES: which of dk and dv it forms.
 template <typename T, int D>
 struct StatesShape {
@@ -351,7 +355,7 @@ struct StatesShape {
 };
 
 template <typename T, int D, bool KEYS, bool VALUES>
-__device__ __forceinline__ void states_gradient_tile(const Args& a, char* lds, int problem, int first_state) {
+__device__ __forceinline__ void states_gradient_tile(const Args& a, char* lds, int problem, int part, int first_state) {
     typedef Matrix<T> M;
     typedef StatesShape<T, D> S;
     constexpr int RT = S::RT, RK = S::RK, N = Vec<T>::N, C = D / (4 * N), PITCH = Staged<T, D, RT>::PITCH;
@@ -359,6 +363,7 @@ __device__ __forceinline__ void states_gradient_tile(const Args& a, char* lds, i
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4;
     const int b = problem / a.kv_heads, kvh = problem - b * a.kv_heads;
     const int n = count_of(a, b), k0 = first_state + wave * 16 * RK;
+    const int begin = part_of(a, part, a.rows, RT), end = part_of(a, part + 1, a.rows, RT);
     const T* q = (const T*)a.q.p + b * a.q.batch + (int64_t)kvh * a.group * a.q.head;
     const T* dy = (const T*)a.dy.p + b * a.dy.batch + (int64_t)kvh * a.group * a.dy.head;
     const T* k = (const T*)a.k.p + b * a.k.batch + kvh * a.k.head;
@@ -382,26 +387,26 @@ __device__ __forceinline__ void states_gradient_tile(const Args& a, char* lds, i
         Staged<T, D, RT> qt, gt;
         T level = 0, delta = 0;
         auto fetch = [&](int r0) {
-            qt.fetch(q, q_rows, r0, a.rows, a.width);
-            gt.fetch(dy, dy_rows, r0, a.rows, a.width);
+            qt.fetch(q, q_rows, r0, end, a.width);
+            gt.fetch(dy, dy_rows, r0, end, a.width);
             if (threadIdx.x < RT) {
                 const int r = r0 + threadIdx.x;
                 level = T(INFINITY), delta = 0;
-                if (r < a.rows) {
+                if (r < end) {
                     const int64_t at = dense_row<T>(a, b, kvh, r);
                     level = level_of(((const T*)a.lse)[at]);
                     delta = ((const T*)a.delta)[at];
                 }
             }
         };
-        fetch(0);
-        for (int r0 = 0; r0 < a.rows; r0 += RT) {
+        fetch(begin);
+        for (int r0 = begin; r0 < end; r0 += RT) {
             __syncthreads();
             qt.store(qs);
             gt.store(gs);
             if (threadIdx.x < RT) levels[threadIdx.x] = level, deltas[threadIdx.x] = delta;
             __syncthreads();
-            if (r0 + RT < a.rows) fetch(r0 + RT);
+            if (r0 + RT < end) fetch(r0 + RT);
 #pragma unroll
             for (int t = 0; t < RT / 16; ++t) {
                 typename M::acc s[RK], dp[RK];
@@ -460,7 +465,7 @@ __device__ __forceinline__ void states_gradient_tile(const Args& a, char* lds, i
     for (int i = 0; i < RK; ++i) {
         const int key = k0 + 16 * i + (lane & 15);
         if (key >= a.keys) continue;
-        const int64_t to = (((int64_t)b * a.keys + key) * a.kv_heads + kvh) * a.width;
+        const int64_t to = part * a.part_size + (((int64_t)b * a.keys + key) * a.kv_heads + kvh) * a.width;
         // (behind the last state: what its stand-in came to is not the gradient, which is zero)
         const bool there = key < n;
         auto put = [&](T* out, const Columns<T, D>& sums, T factor) {
@@ -484,14 +489,14 @@ struct RowsShape {
 };
 
 template <typename T, int D>
-__device__ __forceinline__ void rows_gradient_tile(const Args& a, char* lds, int problem, int first_row) {
+__device__ __forceinline__ void rows_gradient_tile(const Args& a, char* lds, int problem, int part, int first_row) {
     typedef Matrix<T> M;
     typedef RowsShape<T, D> S;
     constexpr int KT = S::KT, RQ = S::RQ, N = Vec<T>::N, C = D / (4 * N), PITCH = Staged<T, D, KT>::PITCH;
     T *ks = reinterpret_cast<T*>(lds), *vs = ks + KT * PITCH;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4;
     const int b = problem / a.kv_heads, kvh = problem - b * a.kv_heads;
-    const int n = count_of(a, b);
+    const int n = count_of(a, b), begin = part_of(a, part, n, KT), end = part_of(a, part + 1, n, KT);
     const T* q = (const T*)a.q.p + b * a.q.batch + (int64_t)kvh * a.group * a.q.head;
     const T* dy = (const T*)a.dy.p + b * a.dy.batch + (int64_t)kvh * a.group * a.dy.head;
     const T* k = (const T*)a.k.p + b * a.k.batch + kvh * a.k.head;
@@ -512,18 +517,18 @@ __device__ __forceinline__ void rows_gradient_tile(const Args& a, char* lds, int
         dq[i].clear();
     }
     Staged<T, D, KT> kt, vt;
-    if (n > 0) {
-        kt.fetch(k, k_rows, 0, n, a.width);
-        vt.fetch(v, v_rows, 0, n, a.width);
+    if (begin < end) {
+        kt.fetch(k, k_rows, begin, end, a.width);
+        vt.fetch(v, v_rows, begin, end, a.width);
     }
-    for (int first = 0; first < n; first += KT) {
+    for (int first = begin; first < end; first += KT) {
         __syncthreads();
         kt.store(ks);
         vt.store(vs);
         __syncthreads();
-        if (first + KT < n) {
-            kt.fetch(k, k_rows, first + KT, n, a.width);
-            vt.fetch(v, v_rows, first + KT, n, a.width);
+        if (first + KT < end) {
+            kt.fetch(k, k_rows, first + KT, end, a.width);
+            vt.fetch(v, v_rows, first + KT, end, a.width);
         }
 #pragma unroll
         for (int t = 0; t < KT / 16; ++t) {
@@ -543,7 +548,7 @@ __device__ __forceinline__ void rows_gradient_tile(const Args& a, char* lds, int
             }
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                const bool there = first + 16 * t + M::row_of(e, g) < n;
+                const bool there = first + 16 * t + M::row_of(e, g) < end;
 #pragma unroll
                 for (int i = 0; i < RQ; ++i) dp[i][e] = there ? M::weight(s[i][e] - level[i]) * (dp[i][e] - delta[i]) : T(0);
             }
@@ -565,7 +570,7 @@ __device__ __forceinline__ void rows_gradient_tile(const Args& a, char* lds, int
     for (int i = 0; i < RQ; ++i) {
         const int r = r0 + 16 * i + (lane & 15);
         if (r >= a.rows) continue;
-        T* out = (T*)a.dq + dense_row<T>(a, b, kvh, r) * a.width;
+        T* out = (T*)a.dq + part * a.part_size + dense_row<T>(a, b, kvh, r) * a.width;
         dq[i].times((T)a.scale);
         dq[i].each([&](int c, const auto& values) { store_run(out, c, a.width, values); });
     }

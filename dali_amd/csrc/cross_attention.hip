@@ -30,15 +30,15 @@ __global__ __launch_bounds__(256, D * sizeof(T) <= 1024 ? 2 : 1) void attention_
 template <typename T, int D, bool KEYS, bool VALUES>
 __global__ __launch_bounds__(256, D * sizeof(T) <= 512 ? 2 : 1) void attention_states_gradient(Args a) {
     extern __shared__ __attribute__((aligned(16))) char attention_lds[];
-    const int id = on_die(blockIdx.x, gridDim.x), at = id / a.tiles, tile = id - at * a.tiles;
-    states_gradient_tile<T, D, KEYS, VALUES>(a, attention_lds, a.first + at, tile * 64 * StatesShape<T, D>::RK);
+    const int id = on_die(blockIdx.x, gridDim.x), at = id / (a.tiles * a.parts), rest = id - at * a.tiles * a.parts, part = rest / a.tiles, tile = rest - part * a.tiles;
+    states_gradient_tile<T, D, KEYS, VALUES>(a, attention_lds, a.first + at, part, tile * 64 * StatesShape<T, D>::RK);
 }
 
 template <typename T, int D>
 __global__ __launch_bounds__(256, D * sizeof(T) <= 512 ? 2 : 1) void attention_rows_gradient(Args a) {
     extern __shared__ __attribute__((aligned(16))) char attention_lds[];
-    const int id = on_die(blockIdx.x, gridDim.x), at = id / a.tiles, tile = id - at * a.tiles;
-    rows_gradient_tile<T, D>(a, attention_lds, a.first + at, tile * 64 * RowsShape<T, D>::RQ);
+    const int id = on_die(blockIdx.x, gridDim.x), at = id / (a.tiles * a.parts), rest = id - at * a.tiles * a.parts, part = rest / a.tiles, tile = rest - part * a.tiles;
+    rows_gradient_tile<T, D>(a, attention_lds, a.first + at, part, tile * 64 * RowsShape<T, D>::RQ);
 }
 
 // ------------------------------------------------------------------------------------------------ few rows
@@ -283,6 +283,23 @@ __global__ __launch_bounds__(256) void attention_delta(Args a, int64_t first) {
     if (there && threadIdx.x % 16 == 0) ((T*)a.delta)[row] = sum;
 }
 
+// A gradient from what parts of the rows or states came to, in their order
+template <typename T>
+__global__ __launch_bounds__(256) void attention_gradient_join(const T* parts, int64_t part_size, int count, int64_t size, T* out) {
+    constexpr int N = Vec<T>::N;
+    for (int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * N; i < size; i += (int64_t)gridDim.x * 256 * N) {
+        const int here = (int)min((int64_t)N, size - i);
+        T sum[N] = {};
+        for (int p = 0; p < count; ++p) {
+            T v[N];
+            load_group(parts + p * part_size + i, 0, here, T(0), v);
+#pragma unroll
+            for (int e = 0; e < N; ++e) sum[e] += v[e];
+        }
+        store_group(out + i, 0, here, sum);
+    }
+}
+
 // ------------------------------------------------------------------------------------------------ launches (host)
 constexpr int kUnits = 256;  // compute units that work is cut for
 
@@ -311,6 +328,25 @@ struct ForwardPlan {
     }
 };
 
+// how the gradients are cut: tiles of the states over parts of the rows, tiles of the rows over parts of the states
+struct BackwardPlan {
+    int state_tiles, state_parts, row_tiles, row_parts;
+    int64_t state_size, row_size;  // values of a gradient
+    template <typename T, int D>
+    void set(const Args& a) {
+        const int64_t problems = (int64_t)a.batch * a.kv_heads;
+        constexpr bool split = std::is_same_v<T, float> && D <= 128;
+        constexpr int states = split ? 128 : 64 * StatesShape<T, D>::RK, rows = split ? 128 : 64 * RowsShape<T, D>::RQ;
+        state_tiles = (a.keys + states - 1) / states, row_tiles = (a.rows + rows - 1) / rows;
+        state_parts = a.keys && a.rows ? parts_for(problems * state_tiles, (a.rows + 31) / 32, 3, 8) : 1;
+        row_parts = a.keys && a.rows ? parts_for(problems * row_tiles, (a.keys + 31) / 32, 3, 8) : 1;
+        const auto round = [](int64_t n) { return (n + 63) / 64 * 64; };
+        state_size = round((int64_t)a.batch * a.keys * a.kv_heads * a.width), row_size = round((int64_t)a.batch * a.queries * a.heads * a.width);
+    }
+    // of what the parts came to, in values
+    int64_t space() const { return std::max(state_parts > 1 ? 2 * state_parts * state_size : 0, row_parts > 1 ? row_parts * row_size : 0); }
+};
+
 template <typename F>
 auto by_width(int dtype, int width, F f) {
     const int d = padded(width);
@@ -331,10 +367,13 @@ size_t round256(size_t b) { return (b + 255) / 256 * 256; }
 // bytes of the workspace, and where its parts lie
 size_t lay_out(int dtype, Args& a, bool backward, char* space) {
     const size_t size = dtype == DALI_HIP_FLOAT ? 4 : 8, rows = (size_t)a.batch * a.queries * a.heads;
-    if (backward) {
-        a.delta = space;
-        return round256(rows * size);
-    }
+    if (backward)
+        return by_width(dtype, a.width, [&](auto t, auto d) -> size_t {
+            BackwardPlan plan;
+            plan.set<decltype(t), decltype(d)::value>(a);
+            a.delta = space, a.parts_y = space + round256(rows * size);
+            return round256(rows * size) + (size_t)plan.space() * size;
+        });
     return by_width(dtype, a.width, [&](auto t, auto d) -> size_t {
         ForwardPlan plan;
         plan.set<decltype(t), decltype(d)::value>(a);
@@ -384,6 +423,13 @@ int forward(const char* what, Args a) {
     return launch(what, attention_join<T, D>, 1, (problems * a.rows + 3) / 4, 0, a);
 }
 
+template <typename T>
+int join(const char* what, const T* parts, int64_t part_size, int count, int64_t size, void* out) {
+    const int64_t groups = (size + Vec<T>::N - 1) / Vec<T>::N;
+    attention_gradient_join<T><<<dim3((unsigned)std::min<int64_t>((groups + 255) / 256, 8 * kUnits)), dim3(256), 0, stream()>>>(parts, part_size, count, size, (T*)out);
+    return launched(what);
+}
+
 template <typename T, int D>
 int backward(const char* what, Args a) {
     const int64_t problems = (int64_t)a.batch * a.kv_heads, rows = (int64_t)a.batch * a.queries * a.heads;
@@ -392,30 +438,38 @@ int backward(const char* what, Args a) {
         attention_delta<T><<<dim3((unsigned)((std::min(rows - first, most) + 15) / 16)), dim3(256), 0, stream()>>>(a, first);
         if (launched(what)) return DALI_HIP_ERROR;
     }
-    if constexpr (std::is_same_v<T, float> && D <= 128) {
-        if (a.keys > 0) {
-            a.tiles = (a.keys + 127) / 128;
-            if (launch(what, attention_states_gradient_split<D>, problems, a.tiles, SplitStates<D>::LDS, a)) return DALI_HIP_ERROR;
-        }
-        a.tiles = (a.rows + 127) / 128;
-        return rows == 0 ? DALI_HIP_OK : launch(what, attention_rows_gradient_split<D>, problems, a.tiles, SplitRows<D>::LDS, a);
-    }
+    BackwardPlan plan;
+    plan.set<T, D>(a);
+    constexpr bool split = std::is_same_v<T, float> && D <= 128;
+    T* parts = (T*)a.parts_y;
     if (a.keys > 0) {
         typedef StatesShape<T, D> S;
-        a.tiles = (a.keys + 64 * S::RK - 1) / (64 * S::RK);
-        if constexpr (S::BOTH) {
-            if (launch(what, attention_states_gradient<T, D, true, true>, problems, a.tiles, S::LDS, a)) return DALI_HIP_ERROR;
+        Args b = a;
+        b.tiles = plan.state_tiles, b.parts = plan.state_parts;
+        if (b.parts > 1) b.part_size = plan.state_size, b.dk = parts, b.dv = parts + b.parts * plan.state_size;
+        const int64_t each = (int64_t)b.tiles * b.parts;
+        if constexpr (split) {
+            if (launch(what, attention_states_gradient_split<D>, problems, each, SplitStates<D>::LDS, b)) return DALI_HIP_ERROR;
+        } else if constexpr (S::BOTH) {
+            if (launch(what, attention_states_gradient<T, D, true, true>, problems, each, S::LDS, b)) return DALI_HIP_ERROR;
         } else {
-            if (launch(what, attention_states_gradient<T, D, true, false>, problems, a.tiles, S::LDS, a)) return DALI_HIP_ERROR;
-            if (launch(what, attention_states_gradient<T, D, false, true>, problems, a.tiles, S::LDS, a)) return DALI_HIP_ERROR;
+            if (launch(what, attention_states_gradient<T, D, true, false>, problems, each, S::LDS, b)) return DALI_HIP_ERROR;
+            if (launch(what, attention_states_gradient<T, D, false, true>, problems, each, S::LDS, b)) return DALI_HIP_ERROR;
+        }
+        if (b.parts > 1) {
+            const int64_t size = (int64_t)a.batch * a.keys * a.kv_heads * a.width;
+            if (join(what, (const T*)b.dk, b.part_size, b.parts, size, a.dk) || join(what, (const T*)b.dv, b.part_size, b.parts, size, a.dv)) return DALI_HIP_ERROR;
         }
     }
-    if (rows > 0) {
-        typedef RowsShape<T, D> S;
-        a.tiles = (a.rows + 64 * S::RQ - 1) / (64 * S::RQ);
-        return launch(what, attention_rows_gradient<T, D>, problems, a.tiles, S::LDS, a);
-    }
-    return DALI_HIP_OK;
+    if (rows == 0) return DALI_HIP_OK;
+    Args b = a;
+    b.tiles = plan.row_tiles, b.parts = plan.row_parts;
+    if (b.parts > 1) b.part_size = plan.row_size, b.dq = parts;
+    const int64_t each = (int64_t)b.tiles * b.parts;
+    int status;
+    if constexpr (split) status = launch(what, attention_rows_gradient_split<D>, problems, each, SplitRows<D>::LDS, b);
+    else status = launch(what, attention_rows_gradient<T, D>, problems, each, RowsShape<T, D>::LDS, b);
+    return status || b.parts == 1 ? status : join(what, (const T*)parts, b.part_size, b.parts, rows * a.width, a.dq);
 }
 
 // ------------------------------------------------------------------------------------------------ arguments (host)
