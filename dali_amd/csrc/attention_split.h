@@ -62,6 +62,16 @@ __device__ __forceinline__ floatx16 multiply(const Pieces& a, const Pieces& b, f
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.p[0], b.p[0], c, 0, 0, 0);
 }
 
+// two of them in turn: neither waits for the result it has just asked for
+__device__ __forceinline__ void multiply_both(const Pieces& a, const Pieces& b, floatx16& c, const Pieces& d, const Pieces& e, floatx16& f) {
+    constexpr int left[6] = {2, 0, 1, 1, 0, 0}, right[6] = {0, 2, 1, 0, 1, 0};
+#pragma unroll
+    for (int i = 0; i < 6; ++i) {
+        c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.p[left[i]], b.p[right[i]], c, 0, 0, 0);
+        f = __builtin_amdgcn_mfma_f32_32x32x16_bf16(d.p[left[i]], e.p[right[i]], f, 0, 0, 0);
+    }
+}
+
 // eight values of a row, zeros past its end
 template <int D>
 __device__ __forceinline__ void row_eight(const float* row, int c, int width, float (&v)[8]) {
@@ -205,27 +215,28 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void attention_rows_split(Ar
     const float* q = (const float*)a.q.p + b * a.q.batch + (int64_t)kvh * a.group * a.q.head;
     const float* k = (const float*)a.k.p + b * a.k.batch + kvh * a.k.head;
     const float* v = (const float*)a.v.p + b * a.v.batch + kvh * a.v.head;
-    const Rows q_rows = {a.q.row, a.q.head, a.group}, k_rows = {a.k.row, 0, 1}, v_rows = {a.v.row, 0, 1};
+    const Rows q_rows(a, a.q), k_rows(a.k), v_rows(a.v);
     const int row = tile * 128 + wave * 32 + (lane & 31);
     SplitFragment<D> qf;
     qf.load(q + q_rows.at(min(row, a.rows - 1)), a.width, (float)(a.scale * Matrix<float>::base * kUp));
     SplitColumns<D> y;
     y.clear();
     float top = Matrix<float>::lowest, sum = 0;  // (of the scores as they are; of the lane's own states)
-    Tile kt, vt;
-    if (begin < end) {
-        kt.fetch(k, k_rows, begin * KT, n, a.width);
-        vt.fetch(v, v_rows, begin * KT, n, a.width);
-    }
-    for (int slab = begin; slab < end; ++slab) {
-        __syncthreads();
-        kt.store(ks);
-        vt.store(vs);
-        __syncthreads();
-        if (slab + 1 < end) {
-            kt.fetch(k, k_rows, (slab + 1) * KT, n, a.width);
-            vt.fetch(v, v_rows, (slab + 1) * KT, n, a.width);
+    // K is read for the scores only and V for the sums only: while one is worked with, the other's next states are cut and written
+    auto fetch = [&](Tile& to, const float* from, const Rows& rows, int slab) { to.fetch(from, rows, slab * KT, n, a.width); };
+    {
+        Tile kt, vt;
+        if (begin < end) {
+            fetch(kt, k, k_rows, begin);
+            fetch(vt, v, v_rows, begin);
+            kt.store(ks);
+            vt.store(vs);
         }
+    }
+    __syncthreads();
+    for (int slab = begin; slab < end; ++slab) {
+        Tile next;
+        if (slab + 1 < end) fetch(next, k, k_rows, slab + 1);
         floatx16 s[KT / 32];
 #pragma unroll
         for (int t = 0; t < KT / 32; ++t) s[t] = floatx16{};
@@ -233,6 +244,11 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void attention_rows_split(Ar
         for (int step = 0; step < D / 16; ++step)
 #pragma unroll
             for (int t = 0; t < KT / 32; ++t) s[t] = multiply(Tile::along(ks, 32 * t, step), qf.step[step], s[t]);
+        __syncthreads();
+        if (slab + 1 < end) {
+            next.store(ks);
+            fetch(next, v, v_rows, slab + 1);
+        }
         if ((slab + 1) * KT > n) {
 #pragma unroll
             for (int t = 0; t < KT / 32; ++t)
@@ -268,6 +284,8 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void attention_rows_split(Ar
 #pragma unroll
                 for (int c = 0; c < D / 32; ++c) y.acc[c] = multiply(Tile::across(vs, 32 * t + 16 * half, 32 * c), p, y.acc[c]);
             }
+        __syncthreads();
+        if (slab + 1 < end) next.store(vs);
     }
     sum = fold_lanes<64, 32>(sum, Sum());
     // (a sum of 0: scores that are all -inf, or below what their pieces hold)
@@ -301,7 +319,7 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void attention_rows_split(Ar
 template <int D>
 struct SplitStates {
     static constexpr int RT = 32;
-    static constexpr int MINE = 2 * SplitStaged<D, RT>::BYTES + 2 * RT * 4, LDS = MINE > StatesShape<float, D>::LDS ? MINE : StatesShape<float, D>::LDS;
+    static constexpr int STAGE = 2 * SplitStaged<D, RT>::BYTES + 2 * RT * 4, MINE = 2 * STAGE, LDS = MINE > StatesShape<float, D>::LDS ? MINE : StatesShape<float, D>::LDS;
 };
 
 template <int D>
@@ -309,8 +327,6 @@ __global__ __launch_bounds__(256, D <= 64 ? 2 : 1) void attention_states_gradien
     constexpr int RT = SplitStates<D>::RT;
     typedef SplitStaged<D, RT> Tile;
     extern __shared__ __attribute__((aligned(16))) char attention_lds[];
-    char *qs = attention_lds, *gs = qs + Tile::BYTES;
-    float *levels = reinterpret_cast<float*>(gs + Tile::BYTES), *deltas = levels + RT;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5;
     const int id = on_die(blockIdx.x, gridDim.x), at = id / (a.tiles * a.parts), rest = id - at * a.tiles * a.parts, part = rest / a.tiles, tile = rest - part * a.tiles;
     const int problem = a.first + at, b = problem / a.kv_heads, kvh = problem - b * a.kv_heads;
@@ -320,7 +336,7 @@ __global__ __launch_bounds__(256, D <= 64 ? 2 : 1) void attention_states_gradien
     const float* dy = (const float*)a.dy.p + b * a.dy.batch + (int64_t)kvh * a.group * a.dy.head;
     const float* k = (const float*)a.k.p + b * a.k.batch + kvh * a.k.head;
     const float* v = (const float*)a.v.p + b * a.v.batch + kvh * a.v.head;
-    const Rows q_rows = {a.q.row, a.q.head, a.group}, dy_rows = {a.dy.row, a.dy.head, a.group};
+    const Rows q_rows(a, a.q), dy_rows(a, a.dy);
     SplitColumns<D> dk, dv;
     dk.clear();
     dv.clear();
@@ -329,11 +345,10 @@ __global__ __launch_bounds__(256, D <= 64 ? 2 : 1) void attention_states_gradien
         SplitFragment<D> kf, vf;
         kf.load(k + min(key, n - 1) * a.k.row, a.width, (float)(a.scale * Matrix<float>::base * kUp));
         vf.load(v + min(key, n - 1) * a.v.row, a.width, kUp);
-        Tile qt, gt;
+        Tile next;
         float level = 0, delta = 0;
-        auto fetch = [&](int r0) {
-            qt.fetch(q, q_rows, r0, end, a.width);
-            gt.fetch(dy, dy_rows, r0, end, a.width);
+        // what a thread holds of the rows' levels goes along with dy
+        auto fetch_levels = [&](int r0) {
             if (threadIdx.x < RT) {
                 const int r = r0 + threadIdx.x;
                 level = INFINITY, delta = 0;
@@ -344,21 +359,45 @@ __global__ __launch_bounds__(256, D <= 64 ? 2 : 1) void attention_states_gradien
                 }
             }
         };
-        fetch(begin);
-        for (int r0 = begin; r0 < end; r0 += RT) {
-            __syncthreads();
-            qt.store(qs);
-            gt.store(gs);
-            if (threadIdx.x < RT) levels[threadIdx.x] = level, deltas[threadIdx.x] = delta;
-            __syncthreads();
-            if (r0 + RT < end) fetch(r0 + RT);
+        auto store_levels = [&](char* stage) {
+            float* levels = reinterpret_cast<float*>(stage + 2 * Tile::BYTES);
+            if (threadIdx.x < RT) levels[threadIdx.x] = level, levels[RT + threadIdx.x] = delta;
+        };
+        next.fetch(q, q_rows, begin, end, a.width);
+        next.store(attention_lds);
+        next.fetch(dy, dy_rows, begin, end, a.width);
+        fetch_levels(begin);
+        next.store(attention_lds + Tile::BYTES);
+        store_levels(attention_lds);
+        __syncthreads();
+        int stage = 0;
+        for (int r0 = begin; r0 < end; r0 += RT, stage ^= 1) {
+            // (two stages: the next rows are cut and written while these are worked with)
+            const char *qs = attention_lds + stage * SplitStates<D>::STAGE, *gs = qs + Tile::BYTES;
+            const float *levels = reinterpret_cast<const float*>(gs + Tile::BYTES), *deltas = levels + RT;
+            char* to = attention_lds + (stage ^ 1) * SplitStates<D>::STAGE;
+            const bool more = r0 + RT < end;
+            if (more) next.fetch(q, q_rows, r0 + RT, end, a.width);
             floatx16 s = floatx16{}, dp = floatx16{};
+            // where a wave has its vector unit to itself, operands are asked for a step ahead of their products; no further, there are no registers for more
+            constexpr bool AHEAD = D > 64;
+            Pieces left, down;
+            if (AHEAD) left = Tile::along(qs, 0, 0), down = Tile::along(gs, 0, 0);
 #pragma unroll
             for (int step = 0; step < D / 16; ++step) {
-                s = multiply(Tile::along(qs, 0, step), kf.step[step], s);
-                dp = multiply(Tile::along(gs, 0, step), vf.step[step], dp);
-                __builtin_amdgcn_sched_barrier(0);  // (operands of one step at a time: there are no registers for more)
+                if (!AHEAD) left = Tile::along(qs, 0, step), down = Tile::along(gs, 0, step);
+                Pieces left1 = left, down1 = down;
+                if (AHEAD && step + 1 < D / 16) left1 = Tile::along(qs, 0, step + 1), down1 = Tile::along(gs, 0, step + 1);
+                multiply_both(left, kf.step[step], s, down, vf.step[step], dp);
+                __builtin_amdgcn_sched_barrier(0);
+                left = left1, down = down1;
             }
+            if (more) {
+                next.store(to);
+                next.fetch(dy, dy_rows, r0 + RT, end, a.width);
+                fetch_levels(r0 + RT);
+            }
+            if (AHEAD) left = Tile::across(gs, 0, 0), down = Tile::across(qs, 0, 0);
 #pragma unroll
             for (int e = 0; e < 16; ++e) {
                 const float lev = levels[split_row(e, h)], del = deltas[split_row(e, h)];
@@ -372,11 +411,20 @@ __global__ __launch_bounds__(256, D <= 64 ? 2 : 1) void attention_states_gradien
                 const Pieces p = weights_of(s, half), ds = weights_of(dp, half);
 #pragma unroll
                 for (int c = 0; c < D / 32; ++c) {
-                    dv.acc[c] = multiply(Tile::across(gs, 16 * half, 32 * c), p, dv.acc[c]);
-                    dk.acc[c] = multiply(Tile::across(qs, 16 * half, 32 * c), ds, dk.acc[c]);
+                    if (!AHEAD) left = Tile::across(gs, 16 * half, 32 * c), down = Tile::across(qs, 16 * half, 32 * c);
+                    Pieces left1 = left, down1 = down;
+                    const int then = half * (D / 32) + c + 1;
+                    if (AHEAD && then < D / 16) left1 = Tile::across(gs, then / (D / 32) * 16, then % (D / 32) * 32), down1 = Tile::across(qs, then / (D / 32) * 16, then % (D / 32) * 32);
+                    multiply_both(left, p, dv.acc[c], down, ds, dk.acc[c]);
                     __builtin_amdgcn_sched_barrier(0);
+                    left = left1, down = down1;
                 }
             }
+            if (more) {
+                next.store(to + Tile::BYTES);
+                store_levels(to);
+            }
+            __syncthreads();
         }
     }
     if (__syncthreads_or(extreme == INFINITY || !dk.finite() || !dv.finite())) {
@@ -400,7 +448,7 @@ __global__ __launch_bounds__(256, D <= 64 ? 2 : 1) void attention_states_gradien
 template <int D>
 struct SplitRows {
     static constexpr int KT = 32;
-    static constexpr int LDS = 2 * SplitStaged<D, KT>::BYTES > RowsShape<float, D>::LDS ? 2 * SplitStaged<D, KT>::BYTES : RowsShape<float, D>::LDS;
+    static constexpr int STAGE = 2 * SplitStaged<D, KT>::BYTES, LDS = 2 * STAGE > RowsShape<float, D>::LDS ? 2 * STAGE : RowsShape<float, D>::LDS;
 };
 
 template <int D>
@@ -408,7 +456,6 @@ __global__ __launch_bounds__(256, D <= 64 ? 2 : 1) void attention_rows_gradient_
     constexpr int KT = SplitRows<D>::KT;
     typedef SplitStaged<D, KT> Tile;
     extern __shared__ __attribute__((aligned(16))) char attention_lds[];
-    char *ks = attention_lds, *vs = ks + Tile::BYTES;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5;
     const int id = on_die(blockIdx.x, gridDim.x), at = id / (a.tiles * a.parts), rest = id - at * a.tiles * a.parts, part = rest / a.tiles, tile = rest - part * a.tiles;
     const int problem = a.first + at, b = problem / a.kv_heads, kvh = problem - b * a.kv_heads;
@@ -418,7 +465,7 @@ __global__ __launch_bounds__(256, D <= 64 ? 2 : 1) void attention_rows_gradient_
     const float* dy = (const float*)a.dy.p + b * a.dy.batch + (int64_t)kvh * a.group * a.dy.head;
     const float* k = (const float*)a.k.p + b * a.k.batch + kvh * a.k.head;
     const float* v = (const float*)a.v.p + b * a.v.batch + kvh * a.v.head;
-    const Rows q_rows = {a.q.row, a.q.head, a.group}, dy_rows = {a.dy.row, a.dy.head, a.group}, k_rows = {a.k.row, 0, 1}, v_rows = {a.v.row, 0, 1};
+    const Rows q_rows(a, a.q), dy_rows(a, a.dy), k_rows(a.k), v_rows(a.v);
     SplitFragment<D> qf, gf;
     qf.load(q + q_rows.at(mine), a.width, (float)(a.scale * Matrix<float>::base * kUp));
     gf.load(dy + dy_rows.at(mine), a.width, kUp);
@@ -427,25 +474,33 @@ __global__ __launch_bounds__(256, D <= 64 ? 2 : 1) void attention_rows_gradient_
     SplitColumns<D> dq;
     dq.clear();
     float extreme = 0.0f;
-    Tile kt, vt;
+    Tile next;
     if (begin < end) {
-        kt.fetch(k, k_rows, begin, end, a.width);
-        vt.fetch(v, v_rows, begin, end, a.width);
+        next.fetch(k, k_rows, begin, end, a.width);
+        next.store(attention_lds);
+        next.fetch(v, v_rows, begin, end, a.width);
+        next.store(attention_lds + Tile::BYTES);
     }
-    for (int first = begin; first < end; first += KT) {
-        __syncthreads();
-        kt.store(ks);
-        vt.store(vs);
-        __syncthreads();
-        if (first + KT < end) {
-            kt.fetch(k, k_rows, first + KT, end, a.width);
-            vt.fetch(v, v_rows, first + KT, end, a.width);
-        }
+    __syncthreads();
+    int stage = 0;
+    for (int first = begin; first < end; first += KT, stage ^= 1) {
+        const char *ks = attention_lds + stage * SplitRows<D>::STAGE, *vs = ks + Tile::BYTES;
+        char* to = attention_lds + (stage ^ 1) * SplitRows<D>::STAGE;
+        const bool more = first + KT < end;
+        if (more) next.fetch(k, k_rows, first + KT, end, a.width);
         floatx16 s = floatx16{}, dp = floatx16{};
+        Pieces left = Tile::along(ks, 0, 0), down = Tile::along(vs, 0, 0);
 #pragma unroll
         for (int step = 0; step < D / 16; ++step) {
-            s = multiply(Tile::along(ks, 0, step), qf.step[step], s);
-            dp = multiply(Tile::along(vs, 0, step), gf.step[step], dp);
+            Pieces left1 = left, down1 = down;
+            if (step + 1 < D / 16) left1 = Tile::along(ks, 0, step + 1), down1 = Tile::along(vs, 0, step + 1);
+            multiply_both(left, qf.step[step], s, down, gf.step[step], dp);
+            __builtin_amdgcn_sched_barrier(0);
+            left = left1, down = down1;
+        }
+        if (more) {
+            next.store(to);
+            next.fetch(v, v_rows, first + KT, end, a.width);
         }
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
@@ -464,6 +519,8 @@ __global__ __launch_bounds__(256, D <= 64 ? 2 : 1) void attention_rows_gradient_
 #pragma unroll
             for (int c = 0; c < D / 32; ++c) dq.acc[c] = multiply(Tile::across(ks, 16 * half, 32 * c), ds, dq.acc[c]);
         }
+        if (more) next.store(to + Tile::BYTES);
+        __syncthreads();
     }
     if (__syncthreads_or(extreme == INFINITY || !dq.finite())) {
         constexpr int STEP = 64 * RowsShape<float, D>::RQ;

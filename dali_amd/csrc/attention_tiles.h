@@ -4,6 +4,7 @@
 #define DALI_HIP_ATTENTION_TILES_H
 
 #include "row_math.h"
+#include "runtime.h"
 
 namespace dali_hip {
 namespace {
@@ -56,15 +57,23 @@ struct Args {
     unsigned* counters;  // of arrivals, counter_step words apart
     int counter_step;
     int first;  // problem of a launch's first workgroup
+    // r / group for rows r: an exact division by a product (sgemm_row_map_div)
+    unsigned group_m;
+    int group_s;
+    __device__ __forceinline__ int position_of(int r) const { return group == 1 ? r : (int)sgemm_row_map_div((unsigned)r, group_m, group_s); }
 };
 
 // Rows that neighbouring heads share: row r lies at position r / group of head r % group
 struct Rows {
     int64_t row, head;
     int group;
+    unsigned group_m;
+    int group_s;
+    __device__ __forceinline__ Rows(const Args& a, const Operand& o) : row(o.row), head(o.head), group(a.group), group_m(a.group_m), group_s(a.group_s) {}
+    __device__ __forceinline__ explicit Rows(const Operand& o) : row(o.row), head(0), group(1), group_m(0), group_s(0) {}
     __device__ __forceinline__ int64_t at(int r) const {
         if (group == 1) return r * row;
-        const int t = r / group;
+        const int t = (int)sgemm_row_map_div((unsigned)r, group_m, group_s);
         return t * row + (r - t * group) * head;
     }
 };
@@ -224,7 +233,7 @@ struct Running {
 
 template <typename T>
 __device__ __forceinline__ int64_t dense_row(const Args& a, int b, int kvh, int r) {
-    const int t = a.group == 1 ? r : r / a.group;
+    const int t = a.position_of(r);
     return ((int64_t)b * a.queries + t) * a.heads + (int64_t)kvh * a.group + (r - t * a.group);
 }
 
@@ -249,7 +258,7 @@ __device__ __forceinline__ void rows_tile(const Args& a, char* lds, int problem,
     const T* q = (const T*)a.q.p + b * a.q.batch + (int64_t)kvh * a.group * a.q.head;
     const T* k = (const T*)a.k.p + b * a.k.batch + kvh * a.k.head;
     const T* v = (const T*)a.v.p + b * a.v.batch + kvh * a.v.head;
-    const Rows q_rows = {a.q.row, a.q.head, a.group}, k_rows = {a.k.row, 0, 1}, v_rows = {a.v.row, 0, 1};
+    const Rows q_rows(a, a.q), k_rows(a.k), v_rows(a.v);
     const int r0 = first_row + wave * 16 * RQ;
     Fragment<T, D> qf[RQ];
 #pragma unroll
@@ -368,7 +377,7 @@ __device__ __forceinline__ void states_gradient_tile(const Args& a, char* lds, i
     const T* dy = (const T*)a.dy.p + b * a.dy.batch + (int64_t)kvh * a.group * a.dy.head;
     const T* k = (const T*)a.k.p + b * a.k.batch + kvh * a.k.head;
     const T* v = (const T*)a.v.p + b * a.v.batch + kvh * a.v.head;
-    const Rows q_rows = {a.q.row, a.q.head, a.group}, dy_rows = {a.dy.row, a.dy.head, a.group};
+    const Rows q_rows(a, a.q), dy_rows(a, a.dy);
     Columns<T, D> dk[KEYS ? RK : 1], dv[VALUES ? RK : 1];
     if (KEYS)
 #pragma unroll
@@ -501,7 +510,7 @@ __device__ __forceinline__ void rows_gradient_tile(const Args& a, char* lds, int
     const T* dy = (const T*)a.dy.p + b * a.dy.batch + (int64_t)kvh * a.group * a.dy.head;
     const T* k = (const T*)a.k.p + b * a.k.batch + kvh * a.k.head;
     const T* v = (const T*)a.v.p + b * a.v.batch + kvh * a.v.head;
-    const Rows q_rows = {a.q.row, a.q.head, a.group}, dy_rows = {a.dy.row, a.dy.head, a.group}, k_rows = {a.k.row, 0, 1}, v_rows = {a.v.row, 0, 1};
+    const Rows q_rows(a, a.q), dy_rows(a, a.dy), k_rows(a.k), v_rows(a.v);
     const int r0 = first_row + wave * 16 * RQ;
     Fragment<T, D> qf[RQ], gf[RQ];
     Columns<T, D> dq[RQ];

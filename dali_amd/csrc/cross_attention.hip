@@ -61,7 +61,7 @@ __global__ __launch_bounds__(256, D * sizeof(T) <= 512 ? 2 : 1) void attention_f
     const T* q = (const T*)a.q.p + b * a.q.batch + (int64_t)kvh * a.group * a.q.head;
     const T* k = (const T*)a.k.p + b * a.k.batch + kvh * a.k.head;
     const T* v = (const T*)a.v.p + b * a.v.batch + kvh * a.v.head;
-    const Rows q_rows = {a.q.row, a.q.head, a.group};
+    const Rows q_rows(a, a.q);
     Fragment<T, D> qf[RQ];
 #pragma unroll
     for (int i = 0; i < RQ; ++i) qf[i].load(q + q_rows.at(min(16 * i + (lane & 15), a.rows - 1)), a.width, (T)(a.scale * M::base));
@@ -413,9 +413,12 @@ int forward(const char* what, Args a) {
     }
     const int few_lds = 16 * plan.rq * (D + Vec<T>::N + 8) * (int)sizeof(T);
     int status;
-    if (plan.few)
-        status = plan.rq == 1 ? launch(what, attention_few<T, D, 1>, problems, plan.parts, few_lds, a) : launch(what, attention_few<T, D, 2>, problems, plan.parts, few_lds, a);
-    else if constexpr (std::is_same_v<T, float>)
+    if (plan.few && plan.rq == 1)
+        status = launch(what, attention_few<T, D, 1>, problems, plan.parts, few_lds, a);
+    else if (plan.few) {
+        if constexpr (D * sizeof(T) <= 512) status = launch(what, attention_few<T, D, 2>, problems, plan.parts, few_lds, a);
+        else status = fail("%s: no kernel for %d rows", what, a.rows);  // (a plan makes none)
+    } else if constexpr (std::is_same_v<T, float>)
         status = launch(what, attention_rows_split<D>, problems, plan.tiles * plan.parts, SplitForward<D>::LDS, a);
     else
         status = launch(what, attention_rows<T, D>, problems, plan.tiles * plan.parts, ForwardShape<T, D>::LDS, a);
@@ -484,6 +487,8 @@ int check_extents(const char* what, int dtype, int batch, int queries, int keys,
         return fail("%s: %d sequences of %d positions and %d states with %d heads are too many", what, batch, queries, keys, heads);
     a = {};
     a.batch = batch, a.queries = queries, a.keys = keys, a.heads = heads, a.kv_heads = kv_heads, a.width = width, a.group = group, a.rows = queries * group, a.scale = scale;
+    while ((1 << a.group_s) < group) ++a.group_s;
+    a.group_m = (unsigned)((((uint64_t)1 << (31 + a.group_s)) + group - 1) / group);
     return DALI_HIP_OK;
 }
 
