@@ -8,7 +8,7 @@
 //
 // The arrangement is that of attention_tiles.h with instructions of 32x32x16: states by rows, a row of the problem (or a state, for the gradients of states) to a lane
 // (lane % 32), whose scores leave the instruction in the order in which the next product takes them as its right operand. Left operands lie in LDS as three planes of rows,
-// 16 bytes of padding behind each row: along a row they are read 16 bytes at a time, across rows by the transposing read, four rows of a column to a lane.
+// padded: along a row they are read 16 bytes at a time, across rows by the transposing read, four rows of a column to a lane.
 #ifndef DALI_HIP_ATTENTION_SPLIT_H
 #define DALI_HIP_ATTENTION_SPLIT_H
 
@@ -95,25 +95,26 @@ struct SplitFragment {
     }
 };
 
-// R rows of D values in LDS as three planes, brought there by 256 threads
-template <int D, int R>
+// R rows of D values in LDS as three planes, brought there by THREADS threads. Behind each row lie 32 bytes of padding: neither eight rows' sixteen bytes at one place nor four
+// rows' 32 share banks.
+template <int D, int R, int THREADS = 256>
 struct SplitStaged {
-    static constexpr int PITCH = 2 * D + 16, PLANE = R * PITCH, BYTES = 3 * PLANE, EIGHTS = D / 8, ALL = R * EIGHTS, EACH = (ALL + 255) / 256;
+    static constexpr int PITCH = 2 * D + 32, PLANE = R * PITCH, BYTES = 3 * PLANE, EIGHTS = D / 8, ALL = R * EIGHTS, EACH = (ALL + THREADS - 1) / THREADS;
     float v[EACH][8];
     __device__ __forceinline__ void fetch(const float* base, const Rows& rows, int first, int end, int width) {
 #pragma unroll
         for (int i = 0; i < EACH; ++i) {
-            const int at = threadIdx.x + i * 256, r = first + at / EIGHTS;
+            const int at = threadIdx.x + i * THREADS, r = first + at / EIGHTS;
 #pragma unroll
             for (int j = 0; j < 8; ++j) v[i][j] = 0.0f;
-            if ((ALL % 256 == 0 || at < ALL) && r < end) row_eight<D>(base + rows.at(r), at % EIGHTS * 8, width, v[i]);
+            if ((ALL % THREADS == 0 || at < ALL) && r < end) row_eight<D>(base + rows.at(r), at % EIGHTS * 8, width, v[i]);
         }
     }
     __device__ __forceinline__ void store(char* lds) const {
 #pragma unroll
         for (int i = 0; i < EACH; ++i) {
-            const int at = threadIdx.x + i * 256;
-            if (ALL % 256 && at >= ALL) break;
+            const int at = threadIdx.x + i * THREADS;
+            if (ALL % THREADS && at >= ALL) break;
             char* to = lds + at / EIGHTS * PITCH + at % EIGHTS * 16;
             Pieces p;
             p.cut(v[i], kUp);
@@ -250,6 +251,7 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void attention_rows_split(Ar
             fetch(next, v, v_rows, slab + 1);
         }
         if ((slab + 1) * KT > n) {
+            asm volatile("");  // (a branch that the other slabs jump over, no selection that they all make)
 #pragma unroll
             for (int t = 0; t < KT / 32; ++t)
 #pragma unroll
@@ -509,6 +511,7 @@ __global__ __launch_bounds__(256, D <= 64 ? 2 : 1) void attention_rows_gradient_
             dp[e] = p * fmaf(dp[e], kDownTwice, -delta);
         }
         if (first + KT > end) {
+            asm volatile("");
 #pragma unroll
             for (int e = 0; e < 16; ++e)
                 if (first + split_row(e, h) >= end) dp[e] = 0.0f;
@@ -534,6 +537,311 @@ __global__ __launch_bounds__(256, D <= 64 ? 2 : 1) void attention_rows_gradient_
     float* out = (float*)a.dq + part * a.part_size + own * a.width;
     dq.times((float)a.scale * kDownTwice);
     dq.each([&](int c, const auto& values) { store_run(out, c, a.width, values); });
+}
+
+// ------------------------------------------------------------------------------------------------ backward, wide heads
+// Heads of more than 64: 32 columns of two operands and their sums would leave a wave's vector unit to itself, with nobody to work while it waits (heads of 128: 802 and 628 us at
+// 2x1999x4001). So a wave takes 16 with instructions of 16x16x32: half the registers, and two waves to a unit where heads have 128; each value read from LDS is used half as often.
+// Lane l holds eight values of every 32 of its column l % 16, and of the results the rows 4 (l / 16) + (0..3).
+__device__ __forceinline__ floatx4 narrow_mul(const Pieces& a, const Pieces& b, floatx4 c) {
+    constexpr int left[6] = {2, 0, 1, 1, 0, 0}, right[6] = {0, 2, 1, 0, 1, 0};
+#pragma unroll
+    for (int i = 0; i < 6; ++i) c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.p[left[i]], b.p[right[i]], c, 0, 0, 0);
+    return c;
+}
+__device__ __forceinline__ void narrow_both(const Pieces& a, const Pieces& b, floatx4& c, const Pieces& d, const Pieces& e, floatx4& f) {
+    constexpr int left[6] = {2, 0, 1, 1, 0, 0}, right[6] = {0, 2, 1, 0, 1, 0};
+#pragma unroll
+    for (int i = 0; i < 6; ++i) {
+        c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.p[left[i]], b.p[right[i]], c, 0, 0, 0);
+        f = __builtin_amdgcn_mfma_f32_16x16x32_bf16(d.p[left[i]], e.p[right[i]], f, 0, 0, 0);
+    }
+}
+
+template <int D>
+struct NarrowFragment {
+    Pieces step[D / 32];
+    __device__ __forceinline__ void load(const float* row, int width, float factor) {
+        const int lane = threadIdx.x & 63;
+#pragma unroll
+        for (int s = 0; s < D / 32; ++s) {
+            float v[8];
+            row_eight<D>(row, 32 * s + 8 * (lane >> 4), width, v);
+            step[s].cut(v, factor);
+        }
+    }
+};
+
+// the tiles of SplitStaged as left operands: along row r + lane % 16, values 32 s + 8 (lane / 16) ...
+template <typename Tile>
+__device__ __forceinline__ Pieces narrow_along(const char* lds, int r, int s) {
+    const int lane = threadIdx.x & 63;
+    const char* from = lds + (r + (lane & 15)) * Tile::PITCH + 64 * s + 16 * (lane >> 4);
+    Pieces p;
+#pragma unroll
+    for (int q = 0; q < 3; ++q) p.p[q] = *reinterpret_cast<const bf16x8*>(from + q * Tile::PLANE);
+    return p;
+}
+// across all 32 rows: column c + lane % 16, rows 4 (lane / 16) + (0..3) and 16 further: those that a lane's scores of two tiles are of
+template <typename Tile>
+__device__ __forceinline__ Pieces narrow_across(const char* lds, int c) {
+    const int lane = threadIdx.x & 63;
+    const char* from = lds + (4 * (lane >> 4) + ((lane & 15) >> 2)) * Tile::PITCH + 2 * (c + 4 * (lane & 3));
+    Pieces p;
+#pragma unroll
+    for (int q = 0; q < 3; ++q) {
+        typedef __attribute__((address_space(3))) shortx4 lds_four;
+        const shortx4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_four*)(from + q * Tile::PLANE));
+        const shortx4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_four*)(from + q * Tile::PLANE + 16 * Tile::PITCH));
+        p.p[q] = __builtin_bit_cast(bf16x8, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
+    }
+    return p;
+}
+__device__ __forceinline__ Pieces narrow_weights(const floatx4 (&s)[2]) {
+    float v[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = s[i >> 2][i & 3];
+    Pieces p;
+    p.cut(v);
+    return p;
+}
+
+template <int D>
+struct NarrowColumns {
+    floatx4 acc[D / 16];
+    __device__ __forceinline__ void clear() {
+#pragma unroll
+        for (int b = 0; b < D / 16; ++b) acc[b] = floatx4{};
+    }
+    __device__ __forceinline__ bool finite() const {
+        float probe = 0.0f;
+#pragma unroll
+        for (int b = 0; b < D / 16; ++b)
+#pragma unroll
+            for (int v = 0; v < 4; ++v) probe = fmaf(acc[b][v], 0.0f, probe);
+        return probe == 0.0f;
+    }
+    __device__ __forceinline__ void put(float* row, int width, float factor) const {
+        const int g = (threadIdx.x & 63) >> 4;
+#pragma unroll
+        for (int b = 0; b < D / 16; ++b) {
+            const float run[4] = {acc[b][0] * factor, acc[b][1] * factor, acc[b][2] * factor, acc[b][3] * factor};
+            store_run(row, 16 * b + 4 * g, width, run);
+        }
+    }
+};
+
+// Threads, and stages of 32 rows of two operands in LDS
+template <int D>
+struct Narrow {
+    static constexpr int THREADS = D <= 128 ? 512 : 256, MINE = 16 * THREADS / 64, STAGES = D <= 128 ? 2 : 1;
+    typedef SplitStaged<D, 32, THREADS> Tile;
+    static constexpr int STAGE = 2 * Tile::BYTES + 64 * 4, OWN = STAGES * STAGE;
+    static constexpr int STATES_LDS = OWN > StatesShape<float, D>::LDS ? OWN : StatesShape<float, D>::LDS, ROWS_LDS = OWN > RowsShape<float, D>::LDS ? OWN : RowsShape<float, D>::LDS;
+    static_assert(StatesShape<float, D>::RK == 1 && RowsShape<float, D>::RQ == 1, "a tile that is taken again is of the same states and rows");
+};
+
+template <int D>
+__global__ __launch_bounds__(Narrow<D>::THREADS, D <= 128 ? 2 : 1) void attention_states_gradient_narrow(Args a) {
+    typedef Narrow<D> Z;
+    typedef typename Z::Tile Tile;
+    extern __shared__ __attribute__((aligned(16))) char attention_lds[];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4;
+    const int id = on_die(blockIdx.x, gridDim.x), at = id / (a.tiles * a.parts), rest = id - at * a.tiles * a.parts, part = rest / a.tiles, tile = rest - part * a.tiles;
+    const int problem = a.first + at, b = problem / a.kv_heads, kvh = problem - b * a.kv_heads;
+    const int n = count_of(a, b), key = tile * Z::MINE + wave * 16 + (lane & 15);
+    const int begin = part_of(a, part, a.rows, 32), end = part_of(a, part + 1, a.rows, 32);
+    const float* q = (const float*)a.q.p + b * a.q.batch + (int64_t)kvh * a.group * a.q.head;
+    const float* dy = (const float*)a.dy.p + b * a.dy.batch + (int64_t)kvh * a.group * a.dy.head;
+    const float* k = (const float*)a.k.p + b * a.k.batch + kvh * a.k.head;
+    const float* v = (const float*)a.v.p + b * a.v.batch + kvh * a.v.head;
+    const Rows q_rows(a, a.q), dy_rows(a, a.dy);
+    NarrowColumns<D> dk, dv;
+    dk.clear();
+    dv.clear();
+    float extreme = 0.0f;
+    if (tile * Z::MINE < n && begin < end) {
+        NarrowFragment<D> kf, vf;
+        kf.load(k + min(key, n - 1) * a.k.row, a.width, (float)(a.scale * Matrix<float>::base * kUp));
+        vf.load(v + min(key, n - 1) * a.v.row, a.width, kUp);
+        Tile next;
+        float level = 0, delta = 0;
+        auto fetch_levels = [&](int r0) {
+            if (threadIdx.x < 32) {
+                const int r = r0 + threadIdx.x;
+                level = INFINITY, delta = 0;
+                if (r < end) {
+                    const int64_t from = dense_row<float>(a, b, kvh, r);
+                    level = level_of(((const float*)a.lse)[from]);
+                    delta = ((const float*)a.delta)[from];
+                }
+            }
+        };
+        auto store_levels = [&](char* stage) {
+            float* levels = reinterpret_cast<float*>(stage + 2 * Tile::BYTES);
+            if (threadIdx.x < 32) levels[threadIdx.x] = level, levels[32 + threadIdx.x] = delta;
+        };
+        next.fetch(q, q_rows, begin, end, a.width);
+        next.store(attention_lds);
+        next.fetch(dy, dy_rows, begin, end, a.width);
+        fetch_levels(begin);
+        next.store(attention_lds + Tile::BYTES);
+        store_levels(attention_lds);
+        __syncthreads();
+        int stage = 0;
+        for (int r0 = begin; r0 < end; r0 += 32, stage ^= Z::STAGES - 1) {
+            const char *qs = attention_lds + stage * Z::STAGE, *gs = qs + Tile::BYTES;
+            const float *levels = reinterpret_cast<const float*>(gs + Tile::BYTES), *deltas = levels + 32;
+            char* to = attention_lds + (stage ^ (Z::STAGES - 1)) * Z::STAGE;
+            const bool more = r0 + 32 < end;
+            if (more) next.fetch(q, q_rows, r0 + 32, end, a.width);
+            floatx4 s[2] = {floatx4{}, floatx4{}}, dp[2] = {floatx4{}, floatx4{}};
+#pragma unroll
+            for (int step = 0; step < D / 32; ++step)
+#pragma unroll
+                for (int t = 0; t < 2; ++t) {
+                    narrow_both(narrow_along<Tile>(qs, 16 * t, step), kf.step[step], s[t], narrow_along<Tile>(gs, 16 * t, step), vf.step[step], dp[t]);
+                    __builtin_amdgcn_sched_barrier(0);  // (operands of one step at a time: there are no registers for more)
+                }
+            if (Z::STAGES == 2 && more) {
+                next.store(to);
+                next.fetch(dy, dy_rows, r0 + 32, end, a.width);
+                fetch_levels(r0 + 32);
+            }
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                const floatx4 lev = *reinterpret_cast<const floatx4*>(levels + 16 * t + 4 * g), del = *reinterpret_cast<const floatx4*>(deltas + 16 * t + 4 * g);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    extreme = fmaxf(extreme, fabsf(s[t][e]));
+                    s[t][e] = lev[e] == INFINITY ? 0.0f : Matrix<float>::weight(fmaf(s[t][e], kDownTwice, 16.0f - lev[e]));  // (times 2^16, as the pieces want it)
+                    dp[t][e] = s[t][e] * fmaf(dp[t][e], kDownTwice, -del[e]);
+                }
+            }
+            const Pieces p = narrow_weights(s), ds = narrow_weights(dp);
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int c = 0; c < D / 16; ++c) {
+                narrow_both(narrow_across<Tile>(gs, 16 * c), p, dv.acc[c], narrow_across<Tile>(qs, 16 * c), ds, dk.acc[c]);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            if (Z::STAGES == 2) {
+                if (more) {
+                    next.store(to + Tile::BYTES);
+                    store_levels(to);
+                }
+                __syncthreads();
+            } else {
+                __syncthreads();
+                if (more) {
+                    next.store(to);
+                    next.fetch(dy, dy_rows, r0 + 32, end, a.width);
+                    fetch_levels(r0 + 32);
+                    next.store(to + Tile::BYTES);
+                    store_levels(to);
+                }
+                __syncthreads();
+            }
+        }
+    }
+    if (__syncthreads_or(extreme == INFINITY || !dk.finite() || !dv.finite())) {
+        states_gradient_tile<float, D, true, true, Z::THREADS>(a, attention_lds, problem, part, tile * Z::MINE);
+        return;
+    }
+    if (key >= a.keys) return;
+    const int64_t to = part * a.part_size + (((int64_t)b * a.keys + key) * a.kv_heads + kvh) * a.width;
+    // (behind the last state: what its stand-in came to is not the gradient, which is zero)
+    dk.put((float*)a.dk + to, a.width, key < n ? (float)a.scale * kDownTwice : 0.0f);
+    dv.put((float*)a.dv + to, a.width, key < n ? kDownTwice : 0.0f);
+}
+
+template <int D>
+__global__ __launch_bounds__(Narrow<D>::THREADS, D <= 128 ? 2 : 1) void attention_rows_gradient_narrow(Args a) {
+    typedef Narrow<D> Z;
+    typedef typename Z::Tile Tile;
+    extern __shared__ __attribute__((aligned(16))) char attention_lds[];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4;
+    const int id = on_die(blockIdx.x, gridDim.x), at = id / (a.tiles * a.parts), rest = id - at * a.tiles * a.parts, part = rest / a.tiles, tile = rest - part * a.tiles;
+    const int problem = a.first + at, b = problem / a.kv_heads, kvh = problem - b * a.kv_heads;
+    const int n = count_of(a, b), row = tile * Z::MINE + wave * 16 + (lane & 15), mine = min(row, a.rows - 1);
+    const int begin = part_of(a, part, n, 32), end = part_of(a, part + 1, n, 32);
+    const float* q = (const float*)a.q.p + b * a.q.batch + (int64_t)kvh * a.group * a.q.head;
+    const float* dy = (const float*)a.dy.p + b * a.dy.batch + (int64_t)kvh * a.group * a.dy.head;
+    const float* k = (const float*)a.k.p + b * a.k.batch + kvh * a.k.head;
+    const float* v = (const float*)a.v.p + b * a.v.batch + kvh * a.v.head;
+    const Rows q_rows(a, a.q), dy_rows(a, a.dy), k_rows(a.k), v_rows(a.v);
+    NarrowFragment<D> qf, gf;
+    qf.load(q + q_rows.at(mine), a.width, (float)(a.scale * Matrix<float>::base * kUp));
+    gf.load(dy + dy_rows.at(mine), a.width, kUp);
+    const int64_t own = dense_row<float>(a, b, kvh, mine);
+    const float level = level_of(((const float*)a.lse)[own]), delta = ((const float*)a.delta)[own];
+    NarrowColumns<D> dq;
+    dq.clear();
+    float extreme = 0.0f;
+    Tile next;
+    if (begin < end) {
+        next.fetch(k, k_rows, begin, end, a.width);
+        next.store(attention_lds);
+        next.fetch(v, v_rows, begin, end, a.width);
+        next.store(attention_lds + Tile::BYTES);
+    }
+    __syncthreads();
+    int stage = 0;
+    for (int first = begin; first < end; first += 32, stage ^= Z::STAGES - 1) {
+        const char *ks = attention_lds + stage * Z::STAGE, *vs = ks + Tile::BYTES;
+        char* to = attention_lds + (stage ^ (Z::STAGES - 1)) * Z::STAGE;
+        const bool more = first + 32 < end;
+        if (more) next.fetch(k, k_rows, first + 32, end, a.width);
+        floatx4 s[2] = {floatx4{}, floatx4{}}, dp[2] = {floatx4{}, floatx4{}};
+#pragma unroll
+        for (int step = 0; step < D / 32; ++step)
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                narrow_both(narrow_along<Tile>(ks, 16 * t, step), qf.step[step], s[t], narrow_along<Tile>(vs, 16 * t, step), gf.step[step], dp[t]);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        if (Z::STAGES == 2 && more) {
+            next.store(to);
+            next.fetch(v, v_rows, first + 32, end, a.width);
+        }
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                extreme = fmaxf(extreme, fabsf(s[t][e]));
+                const float p = Matrix<float>::weight(fmaf(s[t][e], kDownTwice, 16.0f - level));  // (times 2^16, as the pieces want it)
+                dp[t][e] = p * fmaf(dp[t][e], kDownTwice, -delta);
+            }
+        if (first + 32 > end) {
+            asm volatile("");
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (first + 16 * t + 4 * g + e >= end) dp[t][e] = 0.0f;
+        }
+        const Pieces ds = narrow_weights(dp);
+#pragma unroll
+        for (int c = 0; c < D / 16; ++c) dq.acc[c] = narrow_mul(narrow_across<Tile>(ks, 16 * c), ds, dq.acc[c]);
+        if (Z::STAGES == 2) {
+            if (more) next.store(to + Tile::BYTES);
+            __syncthreads();
+        } else {
+            __syncthreads();
+            if (more) {
+                next.store(to);
+                next.fetch(v, v_rows, first + 32, end, a.width);
+                next.store(to + Tile::BYTES);
+            }
+            __syncthreads();
+        }
+    }
+    if (__syncthreads_or(extreme == INFINITY || !dq.finite())) {
+        rows_gradient_tile<float, D, Z::THREADS>(a, attention_lds, problem, part, tile * Z::MINE);
+        return;
+    }
+    if (row >= a.rows) return;
+    dq.put((float*)a.dq + part * a.part_size + own * a.width, a.width, (float)a.scale * kDownTwice);
 }
 
 }  // namespace

@@ -354,7 +354,7 @@ __device__ __forceinline__ T level_of(T lse) {
     return lse == T(-INFINITY) ? T(INFINITY) : lse * (T)Matrix<T>::base;
 }
 
-// The gradients of the states: a workgroup takes 64 RK states, a wave 16 RK of them in its registers, and walks over the rows of a part of them, RT at a time through LDS.
+// The gradients of the states: a workgroup takes 64 RK states (of four waves), a wave 16 RK of them in its registers, and walks over the rows of a part of them, RT at a time through LDS.
 // KEYS, VALUES: which of dk and dv it forms.
 template <typename T, int D>
 struct StatesShape {
@@ -363,11 +363,11 @@ struct StatesShape {
     static constexpr int LDS = 2 * Staged<T, D, RT>::BYTES + 2 * RT * (int)sizeof(T);
 };
 
-template <typename T, int D, bool KEYS, bool VALUES>
+template <typename T, int D, bool KEYS, bool VALUES, int THREADS = 256>
 __device__ __forceinline__ void states_gradient_tile(const Args& a, char* lds, int problem, int part, int first_state) {
     typedef Matrix<T> M;
     typedef StatesShape<T, D> S;
-    constexpr int RT = S::RT, RK = S::RK, N = Vec<T>::N, C = D / (4 * N), PITCH = Staged<T, D, RT>::PITCH;
+    constexpr int RT = S::RT, RK = S::RK, N = Vec<T>::N, C = D / (4 * N), PITCH = Staged<T, D, RT, THREADS>::PITCH;
     T *qs = reinterpret_cast<T*>(lds), *gs = qs + RT * PITCH, *levels = gs + RT * PITCH, *deltas = levels + RT;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4;
     const int b = problem / a.kv_heads, kvh = problem - b * a.kv_heads;
@@ -393,7 +393,7 @@ __device__ __forceinline__ void states_gradient_tile(const Args& a, char* lds, i
             kf[i].load(k + key * a.k.row, a.width, (T)(a.scale * M::base));
             if (KEYS) vf[i].load(v + key * a.v.row, a.width, T(1));
         }
-        Staged<T, D, RT> qt, gt;
+        Staged<T, D, RT, THREADS> qt, gt;
         T level = 0, delta = 0;
         auto fetch = [&](int r0) {
             qt.fetch(q, q_rows, r0, end, a.width);
@@ -423,13 +423,13 @@ __device__ __forceinline__ void states_gradient_tile(const Args& a, char* lds, i
                 for (int i = 0; i < RK; ++i) s[i] = dp[i] = typename M::acc{};
 #pragma unroll
                 for (int c = 0; c < C; ++c) {
-                    const typename Vec<T>::type left = Staged<T, D, RT>::along(qs, 16 * t, c);
+                    const typename Vec<T>::type left = Staged<T, D, RT, THREADS>::along(qs, 16 * t, c);
 #pragma unroll
                     for (int e = 0; e < N; ++e)
 #pragma unroll
                         for (int i = 0; i < RK; ++i) s[i] = M::mul(left[e], kf[i].g[c][e], s[i]);
                     if (KEYS) {
-                        const typename Vec<T>::type down = Staged<T, D, RT>::along(gs, 16 * t, c);
+                        const typename Vec<T>::type down = Staged<T, D, RT, THREADS>::along(gs, 16 * t, c);
 #pragma unroll
                         for (int e = 0; e < N; ++e)
 #pragma unroll
@@ -497,11 +497,11 @@ struct RowsShape {
     static constexpr int LDS = 2 * Staged<T, D, KT>::BYTES;
 };
 
-template <typename T, int D>
+template <typename T, int D, int THREADS = 256>
 __device__ __forceinline__ void rows_gradient_tile(const Args& a, char* lds, int problem, int part, int first_row) {
     typedef Matrix<T> M;
     typedef RowsShape<T, D> S;
-    constexpr int KT = S::KT, RQ = S::RQ, N = Vec<T>::N, C = D / (4 * N), PITCH = Staged<T, D, KT>::PITCH;
+    constexpr int KT = S::KT, RQ = S::RQ, N = Vec<T>::N, C = D / (4 * N), PITCH = Staged<T, D, KT, THREADS>::PITCH;
     T *ks = reinterpret_cast<T*>(lds), *vs = ks + KT * PITCH;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4;
     const int b = problem / a.kv_heads, kvh = problem - b * a.kv_heads;
@@ -525,7 +525,7 @@ __device__ __forceinline__ void rows_gradient_tile(const Args& a, char* lds, int
         delta[i] = ((const T*)a.delta)[at];
         dq[i].clear();
     }
-    Staged<T, D, KT> kt, vt;
+    Staged<T, D, KT, THREADS> kt, vt;
     if (begin < end) {
         kt.fetch(k, k_rows, begin, end, a.width);
         vt.fetch(v, v_rows, begin, end, a.width);
@@ -546,7 +546,7 @@ __device__ __forceinline__ void rows_gradient_tile(const Args& a, char* lds, int
             for (int i = 0; i < RQ; ++i) s[i] = dp[i] = typename M::acc{};
 #pragma unroll
             for (int c = 0; c < C; ++c) {
-                const typename Vec<T>::type left = Staged<T, D, KT>::along(ks, 16 * t, c), down = Staged<T, D, KT>::along(vs, 16 * t, c);
+                const typename Vec<T>::type left = Staged<T, D, KT, THREADS>::along(ks, 16 * t, c), down = Staged<T, D, KT, THREADS>::along(vs, 16 * t, c);
 #pragma unroll
                 for (int e = 0; e < N; ++e)
 #pragma unroll

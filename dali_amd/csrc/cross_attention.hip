@@ -335,8 +335,8 @@ struct BackwardPlan {
     template <typename T, int D>
     void set(const Args& a) {
         const int64_t problems = (int64_t)a.batch * a.kv_heads;
-        constexpr bool split = std::is_same_v<T, float> && D <= 128;
-        constexpr int states = split ? 128 : 64 * StatesShape<T, D>::RK, rows = split ? 128 : 64 * RowsShape<T, D>::RQ;
+        // (float: rows and states of a tile by the kernels of attention_split.h)
+        constexpr int states = !std::is_same_v<T, float> ? 64 * StatesShape<T, D>::RK : D <= 128 ? 128 : 64, rows = !std::is_same_v<T, float> ? 64 * RowsShape<T, D>::RQ : states;
         state_tiles = (a.keys + states - 1) / states, row_tiles = (a.rows + rows - 1) / rows;
         state_parts = a.keys && a.rows ? parts_for(problems * state_tiles, (a.rows + 31) / 32, 3, 8) : 1;
         row_parts = a.keys && a.rows ? parts_for(problems * row_tiles, (a.keys + 31) / 32, 3, 8) : 1;
@@ -387,15 +387,15 @@ size_t lay_out(int dtype, Args& a, bool backward, char* space) {
 
 // `each` workgroups for each of the problems, in launches of fewer than 2^32 threads
 template <typename K>
-int launch(const char* what, K kernel, int64_t problems, int64_t each, int lds, Args a) {
+int launch(const char* what, K kernel, int64_t problems, int64_t each, int lds, Args a, int threads = 256) {
     if (lds > 65536) {
         const hipError_t e = reserve_dynamic_lds((const void*)kernel, lds);
         if (e != hipSuccess) return fail("%s: cannot reserve %d bytes of LDS: %s", what, lds, hipGetErrorString(e));
     }
-    const int64_t most = std::max<int64_t>(1, (1 << 23) / each);
+    const int64_t most = std::max<int64_t>(1, (1 << 22) / each);
     for (int64_t first = 0; first < problems; first += most) {
         a.first = (int)first;
-        kernel<<<dim3((unsigned)(std::min(problems - first, most) * each)), dim3(256), lds, stream()>>>(a);
+        kernel<<<dim3((unsigned)(std::min(problems - first, most) * each)), dim3(threads), lds, stream()>>>(a);
         if (launched(what)) return DALI_HIP_ERROR;
     }
     return DALI_HIP_OK;
@@ -443,7 +443,7 @@ int backward(const char* what, Args a) {
     }
     BackwardPlan plan;
     plan.set<T, D>(a);
-    constexpr bool split = std::is_same_v<T, float> && D <= 128;
+    constexpr bool split = std::is_same_v<T, float>;
     T* parts = (T*)a.parts_y;
     if (a.keys > 0) {
         typedef StatesShape<T, D> S;
@@ -451,7 +451,9 @@ int backward(const char* what, Args a) {
         b.tiles = plan.state_tiles, b.parts = plan.state_parts;
         if (b.parts > 1) b.part_size = plan.state_size, b.dk = parts, b.dv = parts + b.parts * plan.state_size;
         const int64_t each = (int64_t)b.tiles * b.parts;
-        if constexpr (split) {
+        if constexpr (split && D > 64) {
+            if (launch(what, attention_states_gradient_narrow<D>, problems, each, Narrow<D>::STATES_LDS, b, Narrow<D>::THREADS)) return DALI_HIP_ERROR;
+        } else if constexpr (split) {
             if (launch(what, attention_states_gradient_split<D>, problems, each, SplitStates<D>::LDS, b)) return DALI_HIP_ERROR;
         } else if constexpr (S::BOTH) {
             if (launch(what, attention_states_gradient<T, D, true, true>, problems, each, S::LDS, b)) return DALI_HIP_ERROR;
@@ -470,7 +472,8 @@ int backward(const char* what, Args a) {
     if (b.parts > 1) b.part_size = plan.row_size, b.dq = parts;
     const int64_t each = (int64_t)b.tiles * b.parts;
     int status;
-    if constexpr (split) status = launch(what, attention_rows_gradient_split<D>, problems, each, SplitRows<D>::LDS, b);
+    if constexpr (split && D > 64) status = launch(what, attention_rows_gradient_narrow<D>, problems, each, Narrow<D>::ROWS_LDS, b, Narrow<D>::THREADS);
+    else if constexpr (split) status = launch(what, attention_rows_gradient_split<D>, problems, each, SplitRows<D>::LDS, b);
     else status = launch(what, attention_rows_gradient<T, D>, problems, each, RowsShape<T, D>::LDS, b);
     return status || b.parts == 1 ? status : join(what, (const T*)parts, b.part_size, b.parts, rows * a.width, a.dq);
 }
