@@ -338,8 +338,8 @@ struct BackwardPlan {
         // (float: rows and states of a tile by the kernels of attention_split.h)
         constexpr int states = !std::is_same_v<T, float> ? 64 * StatesShape<T, D>::RK : D <= 128 ? 128 : 64, rows = !std::is_same_v<T, float> ? 64 * RowsShape<T, D>::RQ : states;
         state_tiles = (a.keys + states - 1) / states, row_tiles = (a.rows + rows - 1) / rows;
-        state_parts = a.keys && a.rows ? parts_for(problems * state_tiles, (a.rows + 31) / 32, 3, 8) : 1;
-        row_parts = a.keys && a.rows ? parts_for(problems * row_tiles, (a.keys + 31) / 32, 3, 8) : 1;
+        state_parts = a.keys && a.rows ? parts_for(problems * state_tiles, (a.rows + 31) / 32, D <= 64 ? 3 : 4, 8) : 1;
+        row_parts = a.keys && a.rows ? parts_for(problems * row_tiles, (a.keys + 31) / 32, D <= 64 ? 3 : 4, 8) : 1;
         const auto round = [](int64_t n) { return (n + 63) / 64 * 64; };
         state_size = round((int64_t)a.batch * a.keys * a.kv_heads * a.width), row_size = round((int64_t)a.batch * a.queries * a.heads * a.width);
     }

@@ -4,12 +4,14 @@
 // l = x w + bias; lse = m + ln S with the maximum m and S = sum e^(l - m); loss = (m - l_target) + ln S. The gradient of the logits is g = d (e^(l - lse) - [target]),
 // from which dx = g w^T, dw = x^T g, dbias = sum over the rows of g.
 //
-// The vocabulary is taken in pieces, the rows in blocks, so that a piece of logits holds at most kPieceBytes and stays in the 256 MiB cache between the product that
+// Many rows in fp32 go by products of matrices that are cut beforehand, with the softmax at their ends (further below). Else the vocabulary is taken in pieces, the rows in
+// blocks, so that a piece of logits holds at most kPieceBytes and stays in the 256 MiB cache between the product that
 // writes it and the kernel that reads it. Forward, every kSegment columns of a row leave a maximum and a sum of weights relative to it, and a last launch joins a
 // row's. Backward, the piece is formed again and becomes g in its place; the products add it up in the order of pieces and blocks.
 #include <algorithm>
 #include <cmath>
 
+#include "product_of_pieces.h"
 #include "row_math.h"
 
 namespace dali_hip {
@@ -243,12 +245,20 @@ __global__ __launch_bounds__(256) void entropy_gradient(T* logits, int rows, int
     if (columns) store_group(columns + (int64_t)blockIdx.y * width, c, width, sum);
 }
 
+// Sixteen waves add up the chunks of 64 columns, a lane a column, and are joined in their order.
 template <typename T>
-__global__ __launch_bounds__(256) void entropy_bias(const T* columns, int chunks, int width, bool more, T* dbias) {
-    const int c = blockIdx.x * 256 + threadIdx.x;
-    if (c >= width) return;
-    T sum = more ? dbias[c] : T(0);
-    for (int i = 0; i < chunks; ++i) sum += columns[(int64_t)i * width + c];
+__global__ __launch_bounds__(1024) void entropy_bias(const T* columns, int chunks, int width, bool more, T* dbias) {
+    __shared__ T parts[16][64];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = blockIdx.x * 64 + lane;
+    T sum = 0;
+    if (c < width)
+#pragma unroll 4
+        for (int i = wave; i < chunks; i += 16) sum += columns[(int64_t)i * width + c];
+    parts[wave][lane] = sum;
+    __syncthreads();
+    if (wave != 0 || c >= width) return;
+    sum = more ? dbias[c] : T(0);
+    for (int w = 0; w < 16; ++w) sum += parts[w][lane];
     dbias[c] = sum;
 }
 
@@ -286,12 +296,262 @@ int cross_entropy_backward(int64_t rows, int inputs, int vocab, const T* d_losse
                               : cut_product(true, false, inputs, width, n, kept, inputs, g, width, more, dw + v, vocab, parts))
                 return DALI_HIP_ERROR;
             if (dbias) {
-                entropy_bias<T><<<dim3((unsigned)((width + 255) / 256)), dim3(256), 0, stream()>>>(columns, chunks, width, r > 0, dbias + v);
+                entropy_bias<T><<<dim3((unsigned)((width + 63) / 64)), dim3(1024), 0, stream()>>>(columns, chunks, width, r > 0, dbias + v);
                 if (launched(what)) return DALI_HIP_ERROR;
             }
         }
     }
     return DALI_HIP_OK;
+}
+
+// ------------------------------------------------------------------------------------------------ many rows in fp32
+// Products of images (product_of_pieces.h): x is cut once for all pieces of the vocabulary, a piece of w once for all products with it. The logits come out transposed, a
+// row of them to a lane. Forward they are folded where they are and never leave the registers: every 64 columns leave a maximum and a sum. Backward they become g, which is
+// written as an image at once for both products with it.
+constexpr size_t kWeightImageBytes = (size_t)256 << 20, kSlopeImageBytes = (size_t)512 << 20;
+
+struct ImageCut {
+    int block, piece, segments, chunks;
+    size_t x, w, slopes, columns, parts, maxima, sums, chosen, bytes;
+    ImageCut(int64_t rows, int inputs, int vocab, bool backward, bool bias) {
+        using namespace pieces;
+        const auto round = [](size_t b) { return (b + 255) / 256 * 256; };
+        block = (int)std::min<int64_t>(rows, kMostRows);
+        size_t wide = kWeightImageBytes / ((size_t)blocks_of(inputs) * kBlock);
+        if (backward) wide = std::min(wide, kSlopeImageBytes / ((size_t)blocks_of(block) * kBlock));
+        // (pieces of like size, of whole rounds of tiles: 1024 columns are eight)
+        const int64_t most = std::max<int64_t>(1024, (int64_t)wide * 16 / 1024 * 1024), count = (vocab + most - 1) / most;
+        piece = (int)std::min<int64_t>(vocab, (vocab + count * 1024 - 1) / (count * 1024) * 1024);
+        segments = (vocab + 63) / 64;
+        chunks = (block + 63) / 64;
+        x = 0;
+        w = x + round(image_bytes(block, inputs));
+        size_t at = w + round(image_bytes(inputs, piece));
+        if (!backward) {
+            maxima = at;
+            sums = maxima + round((size_t)segments * block * sizeof(float));
+            chosen = sums + round((size_t)segments * block * sizeof(float));
+            bytes = chosen + round((size_t)block * sizeof(float));
+            return;
+        }
+        slopes = at;
+        columns = slopes + round(image_bytes(block, piece));
+        parts = columns + (bias ? round((size_t)chunks * piece * sizeof(float)) : 0);
+        bytes = parts;
+        const int b = (int)((rows - 1) % block) + 1, p = (vocab - 1) % piece + 1;  // the last ones
+        for (const int m : {block, b})
+            for (const int v : {piece, p}) bytes = std::max({bytes, parts + shares_bytes(m, inputs, v), parts + shares_bytes(inputs, v, m), parts + shares_bytes(v, inputs, m)});
+    }
+};
+
+// A wave's logits, transposed: f(row, of that row's 64 columns the first, the sums [32-column block][register])
+template <typename F>
+__device__ __forceinline__ void each_row(const pieces::floatx16 (&sum)[2][2], int n0, F f) {
+#pragma unroll
+    for (int j = 0; j < 2; ++j) f(j, n0 + 32 * j + (threadIdx.x & 31));
+}
+// bias of a lane's columns, zeros without and past the end
+__device__ __forceinline__ void columns_bias(const float* bias, int c0, int width, float (&b)[2][16]) {
+    const int h = (threadIdx.x & 63) >> 5;
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int v = 0; v < 16; ++v) {
+            const int c = c0 + 32 * i + pieces::row_of(v, h);
+            b[i][v] = bias && c < width ? bias[c] : 0.0f;
+        }
+}
+
+__global__ __launch_bounds__(256, 3) void entropy_scores(pieces::Product g, int v0, const float* bias, const int32_t* targets, float* maxima, float* sums, float* chosen) {
+    extern __shared__ __attribute__((aligned(16))) char pieces_lds[];
+    pieces::product<true, false>(g, pieces_lds, [&](const pieces::floatx16 (&sum)[2][2], int c0, int n0, int) {
+        typedef Exponent<float> E;
+        if (c0 >= g.m) return;
+        const int h = (threadIdx.x & 63) >> 5;
+        float b[2][16];
+        columns_bias(bias, c0, g.m, b);
+        each_row(sum, n0, [&](int j, int row) {
+            const int target = (row < g.n ? targets[row] : -1) - v0 - c0;
+            float top = E::lowest, l[2][16];
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int v = 0; v < 16; ++v) {
+                    const int c = 32 * i + pieces::row_of(v, h);
+                    l[i][v] = c0 + c < g.m ? sum[i][j][v] + b[i][v] : -INFINITY;
+                    top = fmaxf(top, l[i][v]);
+                    if (c == target && c0 + c < g.m) chosen[row] = l[i][v];
+                }
+            top = fold_lanes<64, 32>(top, Max());
+            float all = 0;
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int v = 0; v < 16; ++v) all += E::weight(l[i][v] - top);
+            all = fold_lanes<64, 32>(all, Sum());
+            if (row < g.n && h == 0) {
+                const int64_t at = (int64_t)((v0 + c0) / 64) * g.n + row;
+                maxima[at] = top;
+                sums[at] = all;
+            }
+        });
+    });
+}
+
+// Sixteen waves join the segments of 64 rows, a lane a row.
+__global__ __launch_bounds__(1024) void entropy_join_columns(const float* maxima, const float* sums, const float* chosen, const int32_t* targets, int rows, int segments, int vocab,
+                                                             float* losses, float* lse) {
+    typedef Exponent<float> E;
+    __shared__ float tops[16][64], alls[16][64];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, row = blockIdx.x * 64 + lane;
+    float top = E::lowest, sum = 0;
+    if (row < rows)
+#pragma unroll 4
+        for (int i = wave; i < segments; i += 16) {
+            const float m = maxima[(int64_t)i * rows + row], s = sums[(int64_t)i * rows + row], next = fmaxf(top, m);
+            sum = sum * E::weight(top - next) + s * E::weight(m - next);
+            top = next;
+        }
+    tops[wave][lane] = top;
+    alls[wave][lane] = sum;
+    __syncthreads();
+    if (wave != 0 || row >= rows) return;
+    for (int w = 1; w < 16; ++w) top = fmaxf(top, tops[w][lane]);
+    sum = 0;
+    for (int w = 0; w < 16; ++w) sum += alls[w][lane] * E::weight(tops[w][lane] - top);
+    const float logarithm = E::ln(sum);
+    lse[row] = top + logarithm;
+    const int target = targets[row];
+    losses[row] = target < 0 || target >= vocab ? 0.0f : sum == 0.0f ? INFINITY : (top - chosen[row]) + logarithm;
+}
+
+__global__ __launch_bounds__(256, 3) void entropy_slopes(pieces::Product g, int v0, int vocab, const float* bias, const int32_t* targets, const float* lse, const float* d_losses,
+                                                         char* slopes, int row_blocks, int col_blocks, float* columns) {
+    extern __shared__ __attribute__((aligned(16))) char pieces_lds[];
+    pieces::product<true, false>(g, pieces_lds, [&](const pieces::floatx16 (&sum)[2][2], int c0, int n0, int) {
+        typedef Exponent<float> E;
+        const int lane = threadIdx.x & 63, h = lane >> 5;
+        float b[2][16], total[2][16];
+        columns_bias(bias, c0, g.m, b);
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int v = 0; v < 16; ++v) total[i][v] = 0;
+        each_row(sum, n0, [&](int j, int row) {
+            const bool there = row < g.n;
+            const int target = there ? targets[row] : -1;
+            const float level = there ? lse[row] : 0.0f;
+            // a row without a target has no gradient, nor one without weight
+            const bool none = target < 0 || target >= vocab || level == -INFINITY;
+            const float d = none ? 0.0f : d_losses[row];
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    float v[4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const int c = c0 + 32 * i + 8 * q + 4 * h + e;
+                        const float p = E::weight(sum[i][j][4 * q + e] + b[i][4 * q + e] - level) - (target == v0 + c ? 1.0f : 0.0f);
+                        v[e] = none || c >= g.m ? 0.0f : d * p;
+                        total[i][4 * q + e] += v[e];
+                    }
+                    const int block_row = row >> 4, block_col = (c0 + 32 * i + 8 * q) >> 4;
+                    if (block_row >= row_blocks || block_col >= col_blocks) continue;
+                    pieces::uintx2 hi, mid, low;
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        unsigned x, y, z;
+                        pieces::cut(v[2 * e], v[2 * e + 1], x, y, z);
+                        hi[e] = x, mid[e] = y, low[e] = z;
+                    }
+                    char* to = slopes + ((int64_t)block_row * col_blocks + block_col) * pieces::kBlock + (row & 15) * 32 + pieces::half_at(row, q & 1) + 8 * h;
+                    *reinterpret_cast<pieces::uintx2*>(to) = hi;
+                    *reinterpret_cast<pieces::uintx2*>(to + pieces::kPlane) = mid;
+                    *reinterpret_cast<pieces::uintx2*>(to + 2 * pieces::kPlane) = low;
+                }
+        });
+        if (!columns || n0 >= g.n) return;
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int v = 0; v < 16; ++v) {
+                const float s = fold_lanes<32>(total[i][v], Sum());
+                const int c = c0 + 32 * i + pieces::row_of(v, h);
+                if ((lane & 31) == 0 && c < g.m) columns[(int64_t)(n0 / 64) * g.m + c] = s;
+            }
+    });
+}
+
+int weight_image(const char* what, const float* w, int64_t w_stride, bool w_by_columns, int inputs, int width, char* image) {
+    return w_by_columns ? pieces::image_of<true>(what, w, w_stride, inputs, width, nullptr, 0, image) : pieces::image_of<false>(what, w, w_stride, inputs, width, nullptr, 0, image);
+}
+
+int cross_entropy_by_images(int64_t rows, int inputs, int vocab, const float* x, int64_t x_stride, const float* w, int64_t w_stride, bool w_by_columns, const float* bias,
+                            const int32_t* targets, float* losses, float* lse, char* space) {
+    using namespace pieces;
+    const char* what = "dali_hip_projected_cross_entropy";
+    const ImageCut cut(rows, inputs, vocab, false, bias != nullptr);
+    float *maxima = (float*)(space + cut.maxima), *sums = (float*)(space + cut.sums), *chosen = (float*)(space + cut.chosen);
+    if (reserve(what, (const void*)entropy_scores)) return DALI_HIP_ERROR;
+    for (int64_t r = 0; r < rows; r += cut.block) {
+        const int n = (int)std::min<int64_t>(cut.block, rows - r);
+        const Image xs = {space + cut.x, blocks_of(n), blocks_of(inputs)};
+        if (image_of<false>(what, x + r * x_stride, x_stride, n, inputs, nullptr, 0, space + cut.x)) return DALI_HIP_ERROR;
+        for (int64_t v = 0; v < vocab; v += cut.piece) {
+            const int width = (int)std::min<int64_t>(cut.piece, vocab - v);
+            const Image ws = {space + cut.w, blocks_of(inputs), blocks_of(width)};
+            if (weight_image(what, w_by_columns ? w + v * w_stride : w + v, w_stride, w_by_columns, inputs, width, space + cut.w)) return DALI_HIP_ERROR;
+            const Product g = product_for(ws, xs, width, n, xs.cols, 1);
+            entropy_scores<<<dim3((unsigned)(g.tiles_m * g.tiles_n)), dim3(256), kLds, stream()>>>(g, (int)v, bias ? bias + v : nullptr, targets + r, maxima, sums, chosen);
+            if (launched(what)) return DALI_HIP_ERROR;
+        }
+        entropy_join_columns<<<dim3((unsigned)((n + 63) / 64)), dim3(1024), 0, stream()>>>(maxima, sums, chosen, targets + r, n, cut.segments, vocab, losses + r, lse + r);
+        if (launched(what)) return DALI_HIP_ERROR;
+    }
+    return DALI_HIP_OK;
+}
+
+int cross_entropy_backward_by_images(int64_t rows, int inputs, int vocab, const float* d_losses, const float* x, int64_t x_stride, const float* w, int64_t w_stride,
+                                     bool w_by_columns, const float* bias, const int32_t* targets, const float* lse, float* dx, float* dw, bool dw_by_columns, float* dbias,
+                                     char* space) {
+    using namespace pieces;
+    const char* what = "dali_hip_projected_cross_entropy_backward";
+    const ImageCut cut(rows, inputs, vocab, true, dbias != nullptr);
+    float *parts = (float*)(space + cut.parts), *columns = dbias ? (float*)(space + cut.columns) : nullptr;
+    if (reserve(what, (const void*)entropy_slopes)) return DALI_HIP_ERROR;
+    for (int64_t r = 0; r < rows; r += cut.block) {
+        const int n = (int)std::min<int64_t>(cut.block, rows - r), chunks = (n + 63) / 64;
+        const Image xs = {space + cut.x, blocks_of(n), blocks_of(inputs)};
+        if (image_of<false>(what, x + r * x_stride, x_stride, n, inputs, targets + r, vocab, space + cut.x)) return DALI_HIP_ERROR;
+        for (int64_t v = 0; v < vocab; v += cut.piece) {
+            const int width = (int)std::min<int64_t>(cut.piece, vocab - v);
+            const Image ws = {space + cut.w, blocks_of(inputs), blocks_of(width)}, gs = {space + cut.slopes, blocks_of(n), blocks_of(width)};
+            if (weight_image(what, w_by_columns ? w + v * w_stride : w + v, w_stride, w_by_columns, inputs, width, space + cut.w)) return DALI_HIP_ERROR;
+            const Product g = product_for(ws, xs, width, n, xs.cols, 1);
+            entropy_slopes<<<dim3((unsigned)(g.tiles_m * g.tiles_n)), dim3(256), kLds, stream()>>>(g, (int)v, vocab, bias ? bias + v : nullptr, targets + r, lse + r, d_losses + r,
+                                                                                                 space + cut.slopes, gs.rows, gs.cols, columns);
+            if (launched(what)) return DALI_HIP_ERROR;
+            if (kept_product<false, false>(what, gs, ws, n, inputs, {dx + r * inputs, inputs, 0, v > 0}, parts)) return DALI_HIP_ERROR;
+            if (dw_by_columns ? kept_product<true, true>(what, gs, xs, width, inputs, {dw + v * inputs, inputs, 0, r > 0}, parts)
+                              : kept_product<true, true>(what, xs, gs, inputs, width, {dw + v, vocab, 0, r > 0}, parts))
+                return DALI_HIP_ERROR;
+            if (dbias) {
+                entropy_bias<float><<<dim3((unsigned)((width + 63) / 64)), dim3(1024), 0, stream()>>>(columns, chunks, width, r > 0, dbias + v);
+                if (launched(what)) return DALI_HIP_ERROR;
+            }
+        }
+    }
+    return DALI_HIP_OK;
+}
+
+// Whether a call goes by images: where tiles fill the chip and the cutting of w, which takes as long for a few rows as for many, is a small part. us, by images and by fp32 products,
+// inner extents of 32 to 1024. Taken: [512, 10000] forward 21 to 99 and 28 to 103, backward 85 to 225 and 98 to 296; [2048, 2048] 18 to 69 and 23 to 75, 86 to 184 and 81 to 234;
+// [1024, 40000] 54 to 453 and 94 to 564, 247 to 1296 and 285 to 1655. Not taken: [256, 40000] 30 to 193 and 38 to 171, 152 to 467 and 130 to 499; [1024, 2048] 18 to 63 and 18
+// to 44, 81 to 134 and 71 to 142; [128, 10000] 19 to 71 and 17 to 44, 67 to 132 and 80 to 146.
+bool by_images(int dtype, int64_t rows, int vocab) {
+    const int64_t tiles = ((rows + pieces::kTile - 1) / pieces::kTile) * (((int64_t)vocab + pieces::kTile - 1) / pieces::kTile);
+    return dtype == DALI_HIP_FLOAT && rows >= 512 && tiles >= 256;
 }
 
 int check_extents(const char* what, int dtype, int64_t rows, int inputs, int vocab) {
@@ -310,6 +570,7 @@ int check_strides(const char* what, int64_t rows, int inputs, int vocab, int64_t
 }
 
 size_t space_of(int dtype, int64_t rows, int inputs, int vocab, bool backward, bool bias) {
+    if (by_images(dtype, rows, vocab)) return ImageCut(rows, inputs, vocab, backward, bias).bytes;
     return dtype == DALI_HIP_FLOAT ? Cut<float>(rows, inputs, vocab, backward, bias).bytes : Cut<double>(rows, inputs, vocab, backward, bias).bytes;
 }
 
@@ -342,6 +603,9 @@ extern "C" int dali_hip_projected_cross_entropy(int dtype, int64_t rows, int inp
                      Span("bias", bias, vocab, size), Span("targets", targets, rows, 4)}, 0))
         return DALI_HIP_ERROR;
     if (ensure_init()) return DALI_HIP_ERROR;
+    if (by_images(dtype, rows, vocab))
+        return cross_entropy_by_images(rows, inputs, vocab, (const float*)x, x_stride, (const float*)w, w_stride, w_by_columns != 0, (const float*)bias, targets, (float*)losses,
+                                       (float*)lse, (char*)workspace);
     return dtype == DALI_HIP_FLOAT ? cross_entropy(rows, inputs, vocab, (const float*)x, x_stride, (const float*)w, w_stride, w_by_columns != 0, (const float*)bias, targets,
                                                    (float*)losses, (float*)lse, (char*)workspace)
                                    : cross_entropy(rows, inputs, vocab, (const double*)x, x_stride, (const double*)w, w_stride, w_by_columns != 0, (const double*)bias, targets,
@@ -366,6 +630,9 @@ extern "C" int dali_hip_projected_cross_entropy_backward(int dtype, int64_t rows
                      Span("lse", lse, rows, size)}, 0))
         return DALI_HIP_ERROR;
     if (ensure_init()) return DALI_HIP_ERROR;
+    if (by_images(dtype, rows, vocab))
+        return cross_entropy_backward_by_images(rows, inputs, vocab, (const float*)d_losses, (const float*)x, x_stride, (const float*)w, w_stride, w_by_columns != 0,
+                                                (const float*)bias, targets, (const float*)lse, (float*)dx, (float*)dw, dw_by_columns != 0, (float*)dbias, (char*)workspace);
     return dtype == DALI_HIP_FLOAT
                ? cross_entropy_backward(rows, inputs, vocab, (const float*)d_losses, (const float*)x, x_stride, (const float*)w, w_stride, w_by_columns != 0, (const float*)bias,
                                         targets, (const float*)lse, (float*)dx, (float*)dw, dw_by_columns != 0, (float*)dbias, (char*)workspace)
