@@ -69,18 +69,20 @@ int embedding(int64_t count, int rows, int width, const T* table, int64_t stride
 }
 
 // ------------------------------------------------------------------------------------------------ the gradient of the table
-// the first of `n` ordered tokens that is not below `key`; all lanes of the wave take part. (Tokens outside the table come out behind the others, negative ones
-// among them: read without a sign they are above any row's number.)
+// the first of `n` ordered tokens that is not below `key`, sixteen lanes to a key. (Tokens outside the table come out behind the others, negative ones among
+// them: read without a sign they are above any row's number.)
 __device__ __forceinline__ int lower_bound(const int32_t* keys, int n, unsigned key) {
-    const int lane = threadIdx.x & 63;
+    const int lane = threadIdx.x & 15, shift = threadIdx.x & 48;
     int lo = 0, hi = n;  // it lies in [lo, hi]
-    while (lo < hi) {
-        const int step = (hi - lo + 63) / 64;  // (at least one)
+    while (__any(lo < hi)) {
+        const int step = (hi - lo + 15) / 16;
         const int at = lo + (lane + 1) * step - 1;
-        const unsigned long long below = __ballot(at < hi && (unsigned)keys[min(at, n - 1)] < key);
-        const int passed = __popcll(below);  // so many of the 64 places are below, the first ones
-        hi = min(hi, lo + (passed + 1) * step - 1);
-        lo = min(lo + passed * step, hi);
+        const unsigned long long below = __ballot(step > 0 && at < hi && (unsigned)keys[min(max(at, 0), n - 1)] < key);
+        const int passed = __popcll(below >> shift & 0xffffu);  // so many of the sixteen places are below, the first ones
+        if (step > 0) {
+            hi = min(hi, lo + (passed + 1) * step - 1);
+            lo = min(lo + passed * step, hi);
+        }
     }
     return lo;
 }
@@ -139,18 +141,18 @@ __global__ __launch_bounds__(64) void embedding_chunks(const T* dy, int64_t stri
     leave(end, end < count && keys[end] == token);
 }
 
-// A workgroup sees to `per` neighbouring rows of the table (at most 16): zeros where no token names one, and the parts of a run that lies in several chunks, in their order.
+// A workgroup sees to `per` neighbouring rows of the table (at most 15): zeros where no token names one, and the parts of a run that lies in several chunks, in their order.
 // A wave takes every fourth 64 groups of columns.
 template <typename T, bool PAST>
 __global__ __launch_bounds__(256) void embedding_gradient(int width, const int32_t* keys, int count, int rows, int chunk, int first_row, int per, const T* partials, T scale,
                                                           T* dtable) {
     constexpr int N = Vec<T>::N, DEEP = 8;
-    __shared__ int begin[17];
+    __shared__ int begin[16];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int r0 = first_row + blockIdx.x * per, here = min(per, rows - r0);
-    for (int i = wave; i <= here; i += 4) {
-        const int at = lower_bound(keys, count, (unsigned)(r0 + i));
-        if (lane == 0) begin[i] = at;
+    {
+        const int i = threadIdx.x / 16, at = lower_bound(keys, count, (unsigned)(r0 + min(i, here)));
+        if (threadIdx.x % 16 == 0) begin[i] = at;
     }
     __syncthreads();
     for (int r = 0; r < here; ++r) {
@@ -219,7 +221,7 @@ int embedding_backward(int64_t count, int rows, int width, const T* dy, int64_t 
                                                                                                                  first, (T)scale, dtable, partials);
         if (launched(what)) return DALI_HIP_ERROR;
     }
-    const int per = std::max(1, std::min(16, rows / 2048));
+    const int per = std::max(1, std::min(15, rows / 2048));
     const bool past = past_caches((double)rows * width * sizeof(T));
     for (int64_t first = 0; first < rows; first += (int64_t)most * per) {
         const int64_t blocks = std::min((rows - first + per - 1) / per, (int64_t)most);

@@ -38,6 +38,7 @@ constexpr int kSegment = 64 * kGroupsEach * Vec<T>::N;  // 1024 floats, 512 doub
 constexpr int kChunkRows = 64;                          // that a workgroup of the gradient adds up for the bias
 constexpr size_t kPieceBytes = (size_t)128 << 20;
 constexpr int kMostRows = 16384;
+constexpr int kJoinRows = 1024;                         // up to which a row's segments are joined by the launch that forms them (with more that launch fills the chip)
 
 // row-major C[m, n] = op(A) op(B) + beta C
 int product(bool ta, bool tb, int m, int n, int k, const float* a, int lda, const float* b, int ldb, float beta, float* c, int ldc) {
@@ -88,16 +89,40 @@ struct Cut {
 };
 
 // ------------------------------------------------------------------------------------------------ forward
-// A wave takes a segment of a row of the piece of logits that begins at column v0 of `width` columns.
-template <typename T>
+// What the segments of a row come to, by `threads` neighbouring threads of which this is number `at`; all of them return it
+template <typename T, int THREADS, typename Get>
+__device__ __forceinline__ void entropy_row(int segments, int vocab, int target, int row, const Get& get, T* scratch, T* losses, T* lse) {
+    typedef Exponent<T> E;
+    T top = E::lowest, sum = 0;
+    for (int i = threadIdx.x % THREADS; i < segments; i += THREADS) {
+        T m, s, chosen;
+        get(i, m, s, chosen);
+        const T next = Max()(top, m);
+        sum = sum * E::weight(top - next) + s * E::weight(m - next);
+        top = next;
+    }
+    const T best = THREADS == 64 ? fold_lanes<64>(top, Max()) : fold_block<THREADS>(top, scratch, Max());
+    sum *= E::weight(top - best);
+    sum = THREADS == 64 ? fold_lanes<64>(sum, Sum()) : fold_block<THREADS>(sum, scratch, Sum());
+    if (threadIdx.x % THREADS) return;
+    T m, s, chosen;
+    get(0, m, s, chosen);
+    const T logarithm = E::ln(sum);
+    lse[row] = best + logarithm;
+    // (a row without weight leaves no probability for its target)
+    losses[row] = target < 0 || target >= vocab ? T(0) : sum == T(0) ? T(INFINITY) : (best - chosen) + logarithm;
+}
+
+// A wave takes a segment of a row of the piece of logits that begins at column v0 of `width` columns, a workgroup up to four of one row. JOIN: the piece is all there is, and the last
+// workgroup of a row to arrive joins its segments.
+template <typename T, bool JOIN>
 __global__ __launch_bounds__(256) void entropy_segments(const T* logits, int rows, int width, int v0, int segments, const T* bias, const int32_t* targets, int all, T* maxima,
-                                                        T* sums, T* chosen) {
+                                                        T* sums, T* chosen, unsigned* counters, int counter_step, T* losses, T* lse) {
     constexpr int N = Vec<T>::N;
     typedef Exponent<T> E;
-    const int here = (width + kSegment<T> - 1) / kSegment<T>, lane = threadIdx.x & 63;
-    const int64_t unit = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    const int row = (int)(unit / here), s = (int)(unit - (int64_t)row * here);
-    if (row >= rows) return;
+    const int here = (width + kSegment<T> - 1) / kSegment<T>, lane = threadIdx.x & 63, each = (here + 3) / 4;
+    const int row = blockIdx.x / each, s = (blockIdx.x - row * each) * 4 + (threadIdx.x >> 6);
+    if (!JOIN && s >= here) return;
     const T* x = logits + (int64_t)row * width;
     const int first = s * kSegment<T>;
     T v[kGroupsEach][N];
@@ -123,7 +148,7 @@ __global__ __launch_bounds__(256) void entropy_segments(const T* logits, int row
             if (target >= c && target < c + N && target < width) {
 #pragma unroll
                 for (int e = 0; e < N; ++e)
-                    if (target == c + e) chosen[row] = v[j][e];
+                    if (target == c + e) publish(chosen + row, v[j][e]);
             }
         } else {
 #pragma unroll
@@ -139,35 +164,35 @@ __global__ __launch_bounds__(256) void entropy_segments(const T* logits, int row
 #pragma unroll
         for (int e = 0; e < N; ++e) sum += E::weight(v[j][e] - top);
     sum = fold_lanes<64>(sum, Sum());
-    if (lane == 0) {
+    if (lane == 0 && s < here) {
         const int64_t at = (int64_t)row * all + segments + s;
-        maxima[at] = top;
-        sums[at] = sum;
+        publish(maxima + at, top);
+        publish(sums + at, sum);
+    }
+    if constexpr (JOIN) {
+        __shared__ unsigned ticket;
+        __shared__ T scratch[4];
+        if (each > 1) {
+            if (!last_to_arrive(counters + row * counter_step, each, &ticket)) return;
+        } else {  // nobody else to wait for
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            __syncthreads();
+        }
+        entropy_row<T, 256>(
+            here, width, target, row,
+            [&](int i, T& m, T& sum_of, T& c) { m = observe(maxima + (int64_t)row * all + i), sum_of = observe(sums + (int64_t)row * all + i), c = observe(chosen + row); }, scratch,
+            losses, lse);
     }
 }
 
 // A wave joins the segments of a row.
 template <typename T>
 __global__ __launch_bounds__(256) void entropy_join(const T* maxima, const T* sums, const T* chosen, const int32_t* targets, int rows, int segments, int vocab, T* losses, T* lse) {
-    typedef Exponent<T> E;
-    const int row = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
+    const int row = blockIdx.x * 4 + (threadIdx.x >> 6);
     if (row >= rows) return;
-    const T *m = maxima + (int64_t)row * segments, *s = sums + (int64_t)row * segments;
-    T top = E::lowest, sum = 0;
-    for (int i = lane; i < segments; i += 64) {
-        const T next = Max()(top, m[i]);
-        sum = sum * E::weight(top - next) + s[i] * E::weight(m[i] - next);
-        top = next;
-    }
-    const T best = fold_lanes<64>(top, Max());
-    sum = fold_lanes<64>(sum * E::weight(top - best), Sum());
-    if (lane == 0) {
-        const T logarithm = E::ln(sum);
-        lse[row] = best + logarithm;
-        const int target = targets[row];
-        // (a row without weight leaves no probability for its target)
-        losses[row] = target < 0 || target >= vocab ? T(0) : sum == T(0) ? T(INFINITY) : (best - chosen[row]) + logarithm;
-    }
+    entropy_row<T, 64>(
+        segments, vocab, targets[row], row,
+        [&](int i, T& m, T& sum_of, T& c) { m = maxima[(int64_t)row * segments + i], sum_of = sums[(int64_t)row * segments + i], c = chosen[row]; }, (T*)nullptr, losses, lse);
 }
 
 template <typename T>
@@ -176,16 +201,25 @@ int cross_entropy(int64_t rows, int inputs, int vocab, const T* x, int64_t x_str
     const char* what = "dali_hip_projected_cross_entropy";
     const Cut<T> cut(rows, inputs, vocab, false, bias != nullptr);
     T *logits = (T*)(space + cut.logits), *maxima = (T*)(space + cut.maxima), *sums = (T*)(space + cut.sums), *chosen = (T*)(space + cut.chosen);
+    const bool joins = cut.piece == vocab && cut.block <= kJoinRows;
     for (int64_t r = 0; r < rows; r += cut.block) {
         const int n = (int)std::min<int64_t>(cut.block, rows - r);
         for (int64_t v = 0; v < vocab; v += cut.piece) {
             const int width = (int)std::min<int64_t>(cut.piece, vocab - v), here = (width + kSegment<T> - 1) / kSegment<T>;
             if (cut_product(false, w_by_columns, n, width, inputs, x + r * x_stride, (int)x_stride, w_by_columns ? w + v * w_stride : w + v, (int)w_stride, T(0), logits, width, space + cut.parts))
                 return DALI_HIP_ERROR;
-            entropy_segments<T><<<dim3((unsigned)(((int64_t)n * here + 3) / 4)), dim3(256), 0, stream()>>>(
-                logits, n, width, (int)v, (int)(v / kSegment<T>), bias ? bias + v : nullptr, targets + r, cut.segments, maxima, sums, chosen);
+            const dim3 grid((unsigned)(n * ((here + 3) / 4)));
+            const T* b = bias ? bias + v : nullptr;
+            const int segment = (int)(v / kSegment<T>);
+            if (joins)
+                entropy_segments<T, true><<<grid, dim3(256), 0, stream()>>>(logits, n, width, (int)v, segment, b, targets + r, cut.segments, maxima, sums, chosen,
+                                                                           (unsigned*)workspace(), counter_step(n), losses + r, lse + r);
+            else
+                entropy_segments<T, false><<<grid, dim3(256), 0, stream()>>>(logits, n, width, (int)v, segment, b, targets + r, cut.segments, maxima, sums, chosen, nullptr, 0,
+                                                                            nullptr, nullptr);
             if (launched(what)) return DALI_HIP_ERROR;
         }
+        if (joins) continue;
         entropy_join<T><<<dim3((unsigned)((n + 3) / 4)), dim3(256), 0, stream()>>>(maxima, sums, chosen, targets + r, n, cut.segments, vocab, losses + r, lse + r);
         if (launched(what)) return DALI_HIP_ERROR;
     }
