@@ -303,7 +303,9 @@ __global__ __launch_bounds__(256) void attention_gradient_join(const T* parts, i
 // ------------------------------------------------------------------------------------------------ launches (host)
 constexpr int kUnits = 256;  // compute units that work is cut for
 
-// Parts that the states are cut into, so that every compute unit has about `per_unit` workgroups, none with less than `least` slabs
+// Parts that the states (or rows) are cut into, so that every compute unit has about `per_unit` workgroups, none with less than `least` slabs. As many to a unit as it holds at once
+// does best: gradients with heads of up to 64 two (4x1000x2000, heads of 64: 801 us with one, 686 with two, 738 with three), of more than 64 one (4x512x1024, heads of 256:
+// 501, 536, 565); single positions two (32x1x2048: 33.8, 25.9, 26.8).
 int parts_for(int64_t workgroups, int slabs, int per_unit, int least) {
     if (workgroups >= kUnits * per_unit) return 1;
     const int64_t wanted = ((int64_t)kUnits * per_unit + workgroups - 1) / workgroups;
@@ -324,7 +326,7 @@ struct ForwardPlan {
         rq = a.rows <= 16 ? 1 : 2;
         const int rows = std::is_same_v<T, float> ? 128 : 64 * S::RQ;
         tiles = few ? 1 : (a.rows + rows - 1) / rows;
-        parts = few ? parts_for(problems, (a.keys + 63) / 64, 3, 2) : parts_for(problems * tiles, (a.keys + S::KT - 1) / S::KT, 2, 4);
+        parts = few ? parts_for(problems, (a.keys + 63) / 64, 2, 2) : parts_for(problems * tiles, (a.keys + S::KT - 1) / S::KT, 2, 4);
     }
 };
 
@@ -338,8 +340,8 @@ struct BackwardPlan {
         // (float: rows and states of a tile by the kernels of attention_split.h)
         constexpr int states = !std::is_same_v<T, float> ? 64 * StatesShape<T, D>::RK : D <= 128 ? 128 : 64, rows = !std::is_same_v<T, float> ? 64 * RowsShape<T, D>::RQ : states;
         state_tiles = (a.keys + states - 1) / states, row_tiles = (a.rows + rows - 1) / rows;
-        state_parts = a.keys && a.rows ? parts_for(problems * state_tiles, (a.rows + 31) / 32, D <= 64 ? 3 : 4, 8) : 1;
-        row_parts = a.keys && a.rows ? parts_for(problems * row_tiles, (a.keys + 31) / 32, D <= 64 ? 3 : 4, 8) : 1;
+        state_parts = a.keys && a.rows ? parts_for(problems * state_tiles, (a.rows + 31) / 32, D <= 64 ? 2 : 1, 8) : 1;
+        row_parts = a.keys && a.rows ? parts_for(problems * row_tiles, (a.keys + 31) / 32, D <= 64 ? 2 : 1, 8) : 1;
         const auto round = [](int64_t n) { return (n + 63) / 64 * 64; };
         state_size = round((int64_t)a.batch * a.keys * a.kv_heads * a.width), row_size = round((int64_t)a.batch * a.queries * a.heads * a.width);
     }
