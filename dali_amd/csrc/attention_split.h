@@ -223,21 +223,20 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void attention_rows_split(Ar
     SplitColumns<D> y;
     y.clear();
     float top = Matrix<float>::lowest, sum = 0;  // (of the scores as they are; of the lane's own states)
-    // K is read for the scores only and V for the sums only: while one is worked with, the other's next states are cut and written
-    auto fetch = [&](Tile& to, const float* from, const Rows& rows, int slab) { to.fetch(from, rows, slab * KT, n, a.width); };
-    {
-        Tile kt, vt;
-        if (begin < end) {
-            fetch(kt, k, k_rows, begin);
-            fetch(vt, v, v_rows, begin);
-            kt.store(ks);
-            vt.store(vs);
-        }
+    Tile kt, vt;
+    if (begin < end) {
+        kt.fetch(k, k_rows, begin * KT, n, a.width);
+        vt.fetch(v, v_rows, begin * KT, n, a.width);
     }
-    __syncthreads();
     for (int slab = begin; slab < end; ++slab) {
-        Tile next;
-        if (slab + 1 < end) fetch(next, k, k_rows, slab + 1);
+        __syncthreads();
+        kt.store(ks);
+        vt.store(vs);
+        __syncthreads();
+        if (slab + 1 < end) {
+            kt.fetch(k, k_rows, (slab + 1) * KT, n, a.width);
+            vt.fetch(v, v_rows, (slab + 1) * KT, n, a.width);
+        }
         floatx16 s[KT / 32];
 #pragma unroll
         for (int t = 0; t < KT / 32; ++t) s[t] = floatx16{};
@@ -245,11 +244,6 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void attention_rows_split(Ar
         for (int step = 0; step < D / 16; ++step)
 #pragma unroll
             for (int t = 0; t < KT / 32; ++t) s[t] = multiply(Tile::along(ks, 32 * t, step), qf.step[step], s[t]);
-        __syncthreads();
-        if (slab + 1 < end) {
-            next.store(ks);
-            fetch(next, v, v_rows, slab + 1);
-        }
         if ((slab + 1) * KT > n) {
             asm volatile("");  // (a branch that the other slabs jump over, no selection that they all make)
 #pragma unroll
@@ -286,8 +280,6 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void attention_rows_split(Ar
 #pragma unroll
                 for (int c = 0; c < D / 32; ++c) y.acc[c] = multiply(Tile::across(vs, 32 * t + 16 * half, 32 * c), p, y.acc[c]);
             }
-        __syncthreads();
-        if (slab + 1 < end) next.store(vs);
     }
     sum = fold_lanes<64, 32>(sum, Sum());
     // (a sum of 0: scores that are all -inf, or below what their pieces hold)

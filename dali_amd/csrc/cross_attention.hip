@@ -305,7 +305,8 @@ constexpr int kUnits = 256;  // compute units that work is cut for
 
 // Parts that the states (or rows) are cut into, so that every compute unit has about `per_unit` workgroups, none with less than `least` slabs. As many to a unit as it holds at once
 // does best: gradients with heads of up to 64 two (4x1000x2000, heads of 64: 801 us with one, 686 with two, 738 with three), of more than 64 one (4x512x1024, heads of 256:
-// 501, 536, 565); single positions two (32x1x2048: 33.8, 25.9, 26.8).
+// 501, 536, 565); single positions three,
+// whose states come from memory (32x1x2048: 30.3 us with two, 28.6 with three).
 int parts_for(int64_t workgroups, int slabs, int per_unit, int least) {
     if (workgroups >= kUnits * per_unit) return 1;
     const int64_t wanted = ((int64_t)kUnits * per_unit + workgroups - 1) / workgroups;
@@ -326,7 +327,7 @@ struct ForwardPlan {
         rq = a.rows <= 16 ? 1 : 2;
         const int rows = std::is_same_v<T, float> ? 128 : 64 * S::RQ;
         tiles = few ? 1 : (a.rows + rows - 1) / rows;
-        parts = few ? parts_for(problems, (a.keys + 63) / 64, 2, 2) : parts_for(problems * tiles, (a.keys + S::KT - 1) / S::KT, 2, 4);
+        parts = few ? parts_for(problems, (a.keys + 63) / 64, 3, 2) : parts_for(problems * tiles, (a.keys + S::KT - 1) / S::KT, 2, 4);
     }
 };
 
