@@ -36,6 +36,8 @@ typedef short shortx4 __attribute__((ext_vector_type(4)));
 constexpr int kBlock = 1536, kPlane = 512;             // bytes
 constexpr int kTile = 128, kOperand = 8 * kBlock;      // an operand's slab: eight blocks
 constexpr int kStage = 2 * kOperand, kLds = 2 * kStage;
+constexpr int kMostInner = 1 << 20;                    // of an image, so that eight blocks' distance fits 32 bits
+static_assert(kLds <= 65536, "needs no reserving");
 
 inline int blocks_of(int64_t n) { return (int)((n + 15) / 16); }
 inline size_t image_bytes(int64_t rows, int64_t cols) { return (size_t)blocks_of(rows) * blocks_of(cols) * kBlock; }
@@ -347,17 +349,11 @@ inline size_t shares_bytes(int64_t m, int64_t n, int64_t k) {
 inline Product product_for(const Image& a, const Image& b, int m, int n, int k, int shares) {
     return {a, b, m, n, k, (m + kTile - 1) / kTile, (n + kTile - 1) / kTile, shares};
 }
-inline int reserve(const char* what, const void* kernel) {
-    const hipError_t e = reserve_dynamic_lds(kernel, kLds);
-    return e == hipSuccess ? DALI_HIP_OK : fail("%s: cannot reserve %d bytes of LDS: %s", what, kLds, hipGetErrorString(e));
-}
-
 // c [m, n] from two images whose inner extents agree; `parts` holds shares_bytes
 template <bool A_ACROSS, bool B_ACROSS>
 int kept_product(const char* what, const Image& a, const Image& b, int m, int n, Kept to, float* parts) {
     const int k = A_ACROSS ? a.rows : a.cols, shares = shares_for(m, n, k);
     const Product g = product_for(a, b, m, n, k, shares);
-    if (reserve(what, (const void*)product_kept<A_ACROSS, B_ACROSS>)) return DALI_HIP_ERROR;
     const Kept part = {parts, n, (int64_t)m * n, false};
     product_kept<A_ACROSS, B_ACROSS><<<dim3((unsigned)(g.tiles_m * g.tiles_n * shares)), dim3(256), kLds, stream()>>>(g, shares > 1 ? part : to);
     if (launched(what)) return DALI_HIP_ERROR;

@@ -351,7 +351,7 @@ struct ImageCut {
         using namespace pieces;
         const auto round = [](size_t b) { return (b + 255) / 256 * 256; };
         block = (int)std::min<int64_t>(rows, kMostRows);
-        size_t wide = kWeightImageBytes / ((size_t)blocks_of(inputs) * kBlock);
+        size_t wide = std::min(kWeightImageBytes / ((size_t)blocks_of(inputs) * kBlock), (size_t)kMostInner / 16);
         if (backward) wide = std::min(wide, kSlopeImageBytes / ((size_t)blocks_of(block) * kBlock));
         // (pieces of like size, of whole rounds of tiles: 1024 columns are eight)
         const int64_t most = std::max<int64_t>(1024, (int64_t)wide * 16 / 1024 * 1024), count = (vocab + most - 1) / most;
@@ -527,7 +527,6 @@ int cross_entropy_by_images(int64_t rows, int inputs, int vocab, const float* x,
     const char* what = "dali_hip_projected_cross_entropy";
     const ImageCut cut(rows, inputs, vocab, false, bias != nullptr);
     float *maxima = (float*)(space + cut.maxima), *sums = (float*)(space + cut.sums), *chosen = (float*)(space + cut.chosen);
-    if (reserve(what, (const void*)entropy_scores)) return DALI_HIP_ERROR;
     for (int64_t r = 0; r < rows; r += cut.block) {
         const int n = (int)std::min<int64_t>(cut.block, rows - r);
         const Image xs = {space + cut.x, blocks_of(n), blocks_of(inputs)};
@@ -553,7 +552,6 @@ int cross_entropy_backward_by_images(int64_t rows, int inputs, int vocab, const 
     const char* what = "dali_hip_projected_cross_entropy_backward";
     const ImageCut cut(rows, inputs, vocab, true, dbias != nullptr);
     float *parts = (float*)(space + cut.parts), *columns = dbias ? (float*)(space + cut.columns) : nullptr;
-    if (reserve(what, (const void*)entropy_slopes)) return DALI_HIP_ERROR;
     for (int64_t r = 0; r < rows; r += cut.block) {
         const int n = (int)std::min<int64_t>(cut.block, rows - r), chunks = (n + 63) / 64;
         const Image xs = {space + cut.x, blocks_of(n), blocks_of(inputs)};
@@ -583,9 +581,9 @@ int cross_entropy_backward_by_images(int64_t rows, int inputs, int vocab, const 
 // inner extents of 32 to 1024. Taken: [512, 10000] forward 21 to 99 and 28 to 103, backward 85 to 225 and 98 to 296; [2048, 2048] 18 to 69 and 23 to 75, 86 to 184 and 81 to 234;
 // [1024, 40000] 54 to 453 and 94 to 564, 247 to 1296 and 285 to 1655. Not taken: [256, 40000] 30 to 193 and 38 to 171, 152 to 467 and 130 to 499; [1024, 2048] 18 to 63 and 18
 // to 44, 81 to 134 and 71 to 142; [128, 10000] 19 to 71 and 17 to 44, 67 to 132 and 80 to 146.
-bool by_images(int dtype, int64_t rows, int vocab) {
+bool by_images(int dtype, int64_t rows, int inputs, int vocab) {
     const int64_t tiles = ((rows + pieces::kTile - 1) / pieces::kTile) * (((int64_t)vocab + pieces::kTile - 1) / pieces::kTile);
-    return dtype == DALI_HIP_FLOAT && rows >= 512 && tiles >= 256;
+    return dtype == DALI_HIP_FLOAT && rows >= 512 && tiles >= 256 && inputs <= pieces::kMostInner;
 }
 
 int check_extents(const char* what, int dtype, int64_t rows, int inputs, int vocab) {
@@ -604,7 +602,7 @@ int check_strides(const char* what, int64_t rows, int inputs, int vocab, int64_t
 }
 
 size_t space_of(int dtype, int64_t rows, int inputs, int vocab, bool backward, bool bias) {
-    if (by_images(dtype, rows, vocab)) return ImageCut(rows, inputs, vocab, backward, bias).bytes;
+    if (by_images(dtype, rows, inputs, vocab)) return ImageCut(rows, inputs, vocab, backward, bias).bytes;
     return dtype == DALI_HIP_FLOAT ? Cut<float>(rows, inputs, vocab, backward, bias).bytes : Cut<double>(rows, inputs, vocab, backward, bias).bytes;
 }
 
@@ -637,7 +635,7 @@ extern "C" int dali_hip_projected_cross_entropy(int dtype, int64_t rows, int inp
                      Span("bias", bias, vocab, size), Span("targets", targets, rows, 4)}, 0))
         return DALI_HIP_ERROR;
     if (ensure_init()) return DALI_HIP_ERROR;
-    if (by_images(dtype, rows, vocab))
+    if (by_images(dtype, rows, inputs, vocab))
         return cross_entropy_by_images(rows, inputs, vocab, (const float*)x, x_stride, (const float*)w, w_stride, w_by_columns != 0, (const float*)bias, targets, (float*)losses,
                                        (float*)lse, (char*)workspace);
     return dtype == DALI_HIP_FLOAT ? cross_entropy(rows, inputs, vocab, (const float*)x, x_stride, (const float*)w, w_stride, w_by_columns != 0, (const float*)bias, targets,
@@ -664,7 +662,7 @@ extern "C" int dali_hip_projected_cross_entropy_backward(int dtype, int64_t rows
                      Span("lse", lse, rows, size)}, 0))
         return DALI_HIP_ERROR;
     if (ensure_init()) return DALI_HIP_ERROR;
-    if (by_images(dtype, rows, vocab))
+    if (by_images(dtype, rows, inputs, vocab))
         return cross_entropy_backward_by_images(rows, inputs, vocab, (const float*)d_losses, (const float*)x, x_stride, (const float*)w, w_stride, w_by_columns != 0,
                                                 (const float*)bias, targets, (const float*)lse, (float*)dx, (float*)dw, dw_by_columns != 0, (float*)dbias, (char*)workspace);
     return dtype == DALI_HIP_FLOAT
