@@ -395,7 +395,7 @@ int dali_hip_token_log_probs_backward(int dtype, int64_t rows, int vocab, const 
  */
 int dali_hip_embedding(int dtype, int64_t count, int rows, int width, const void* table, int64_t stride, const int32_t* tokens, double scale, void* y);
 /*
- * Its gradient, written whole: dtable[r] = scale * sum of dy[i] over the i with tokens[i] = r, in the order of i up to blocks of 64 ordered tokens that are summed first; zeros
+ * Its gradient, written whole: dtable[r] = scale * sum of dy[i] over the i with tokens[i] = r, in the order of i, by runs of 16 to 128 neighbours of the ordered tokens; zeros
  * where there is none. Rows of dy are `stride` values apart, dtable [rows, width] is dense. count may be 0.
  */
 int dali_hip_embedding_backward_workspace(int dtype, int64_t count, int rows, int width, size_t* bytes);
