@@ -373,25 +373,16 @@ __global__ __launch_bounds__(256, D <= 64 ? 2 : 1) void attention_states_gradien
             const bool more = r0 + RT < end;
             if (more) next.fetch(q, q_rows, r0 + RT, end, a.width);
             floatx16 s = floatx16{}, dp = floatx16{};
-            // where a wave has its vector unit to itself, operands are asked for a step ahead of their products; no further, there are no registers for more
-            constexpr bool AHEAD = D > 64;
-            Pieces left, down;
-            if (AHEAD) left = Tile::along(qs, 0, 0), down = Tile::along(gs, 0, 0);
 #pragma unroll
             for (int step = 0; step < D / 16; ++step) {
-                if (!AHEAD) left = Tile::along(qs, 0, step), down = Tile::along(gs, 0, step);
-                Pieces left1 = left, down1 = down;
-                if (AHEAD && step + 1 < D / 16) left1 = Tile::along(qs, 0, step + 1), down1 = Tile::along(gs, 0, step + 1);
-                multiply_both(left, kf.step[step], s, down, vf.step[step], dp);
-                __builtin_amdgcn_sched_barrier(0);
-                left = left1, down = down1;
+                multiply_both(Tile::along(qs, 0, step), kf.step[step], s, Tile::along(gs, 0, step), vf.step[step], dp);
+                __builtin_amdgcn_sched_barrier(0);  // (operands of one step at a time: there are no registers for more)
             }
             if (more) {
                 next.store(to);
                 next.fetch(dy, dy_rows, r0 + RT, end, a.width);
                 fetch_levels(r0 + RT);
             }
-            if (AHEAD) left = Tile::across(gs, 0, 0), down = Tile::across(qs, 0, 0);
 #pragma unroll
             for (int e = 0; e < 16; ++e) {
                 const float lev = levels[split_row(e, h)], del = deltas[split_row(e, h)];
@@ -402,17 +393,16 @@ __global__ __launch_bounds__(256, D <= 64 ? 2 : 1) void attention_states_gradien
             __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
             for (int half = 0; half < 2; ++half) {
-                const Pieces p = weights_of(s, half), ds = weights_of(dp, half);
-#pragma unroll
-                for (int c = 0; c < D / 32; ++c) {
-                    if (!AHEAD) left = Tile::across(gs, 16 * half, 32 * c), down = Tile::across(qs, 16 * half, 32 * c);
-                    Pieces left1 = left, down1 = down;
-                    const int then = half * (D / 32) + c + 1;
-                    if (AHEAD && then < D / 16) left1 = Tile::across(gs, then / (D / 32) * 16, then % (D / 32) * 32), down1 = Tile::across(qs, then / (D / 32) * 16, then % (D / 32) * 32);
-                    multiply_both(left, p, dv.acc[c], down, ds, dk.acc[c]);
+                if constexpr (D == 32) {
+                    multiply_both(Tile::across(gs, 16 * half, 0), weights_of(s, half), dv.acc[0], Tile::across(qs, 16 * half, 0), weights_of(dp, half), dk.acc[0]);
+                } else {
+                    const Pieces p = weights_of(s, half);
+                    multiply_both(Tile::across(gs, 16 * half, 0), p, dv.acc[0], Tile::across(gs, 16 * half, 32), p, dv.acc[1]);
                     __builtin_amdgcn_sched_barrier(0);
-                    left = left1, down = down1;
+                    const Pieces ds = weights_of(dp, half);
+                    multiply_both(Tile::across(qs, 16 * half, 0), ds, dk.acc[0], Tile::across(qs, 16 * half, 32), ds, dk.acc[1]);
                 }
+                __builtin_amdgcn_sched_barrier(0);
             }
             if (more) {
                 next.store(to + Tile::BYTES);
@@ -446,7 +436,7 @@ struct SplitRows {
 };
 
 template <int D>
-__global__ __launch_bounds__(256, D <= 64 ? 2 : 1) void attention_rows_gradient_split(Args a) {
+__global__ __launch_bounds__(256, 2) void attention_rows_gradient_split(Args a) {
     constexpr int KT = SplitRows<D>::KT;
     typedef SplitStaged<D, KT> Tile;
     extern __shared__ __attribute__((aligned(16))) char attention_lds[];
@@ -511,8 +501,13 @@ __global__ __launch_bounds__(256, D <= 64 ? 2 : 1) void attention_rows_gradient_
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
             const Pieces ds = weights_of(dp, half);
+            if constexpr (D == 32) {
+                dq.acc[0] = multiply(Tile::across(ks, 16 * half, 0), ds, dq.acc[0]);
+            } else {
 #pragma unroll
-            for (int c = 0; c < D / 32; ++c) dq.acc[c] = multiply(Tile::across(ks, 16 * half, 32 * c), ds, dq.acc[c]);
+                for (int c = 0; c < D / 32; c += 2)
+                    multiply_both(Tile::across(ks, 16 * half, 32 * c), ds, dq.acc[c], Tile::across(ks, 16 * half, 32 * c + 32), ds, dq.acc[c + 1]);
+            }
         }
         if (more) next.store(to + Tile::BYTES);
         __syncthreads();
@@ -688,13 +683,16 @@ __global__ __launch_bounds__(Narrow<D>::THREADS, D <= 128 ? 2 : 1) void attentio
             const bool more = r0 + 32 < end;
             if (more) next.fetch(q, q_rows, r0 + 32, end, a.width);
             floatx4 s[2] = {floatx4{}, floatx4{}}, dp[2] = {floatx4{}, floatx4{}};
+            // (operands a step ahead of their products)
+            Pieces left = narrow_along<Tile>(qs, 0, 0), down = narrow_along<Tile>(gs, 0, 0);
 #pragma unroll
-            for (int step = 0; step < D / 32; ++step)
-#pragma unroll
-                for (int t = 0; t < 2; ++t) {
-                    narrow_both(narrow_along<Tile>(qs, 16 * t, step), kf.step[step], s[t], narrow_along<Tile>(gs, 16 * t, step), vf.step[step], dp[t]);
-                    __builtin_amdgcn_sched_barrier(0);  // (operands of one step at a time: there are no registers for more)
-                }
+            for (int i = 0; i < D / 16; ++i) {
+                Pieces left1 = left, down1 = down;
+                if (i + 1 < D / 16) left1 = narrow_along<Tile>(qs, 16 * ((i + 1) & 1), (i + 1) / 2), down1 = narrow_along<Tile>(gs, 16 * ((i + 1) & 1), (i + 1) / 2);
+                narrow_both(left, kf.step[i / 2], s[i & 1], down, vf.step[i / 2], dp[i & 1]);
+                __builtin_amdgcn_sched_barrier(0);
+                left = left1, down = down1;
+            }
             if (Z::STAGES == 2 && more) {
                 next.store(to);
                 next.fetch(dy, dy_rows, r0 + 32, end, a.width);
@@ -710,12 +708,22 @@ __global__ __launch_bounds__(Narrow<D>::THREADS, D <= 128 ? 2 : 1) void attentio
                     dp[t][e] = s[t][e] * fmaf(dp[t][e], kDownTwice, -del[e]);
                 }
             }
-            const Pieces p = narrow_weights(s), ds = narrow_weights(dp);
+            left = narrow_across<Tile>(gs, 0), down = narrow_across<Tile>(gs, 16);
+            Pieces weights = narrow_weights(s);
             __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-            for (int c = 0; c < D / 16; ++c) {
-                narrow_both(narrow_across<Tile>(gs, 16 * c), p, dv.acc[c], narrow_across<Tile>(qs, 16 * c), ds, dk.acc[c]);
+            for (int c = 0; c < 2 * D / 16; c += 2) {  // dv first, then dk
+                Pieces left1 = left, down1 = down;
+                const int then = c + 2;
+                if (then < 2 * D / 16) {
+                    const char* from = then < D / 16 ? gs : qs;
+                    left1 = narrow_across<Tile>(from, 16 * (then % (D / 16))), down1 = narrow_across<Tile>(from, 16 * (then % (D / 16)) + 16);
+                }
+                if (c < D / 16) narrow_both(left, weights, dv.acc[c], down, weights, dv.acc[c + 1]);
+                else narrow_both(left, weights, dk.acc[c - D / 16], down, weights, dk.acc[c - D / 16 + 1]);
+                if (then == D / 16) weights = narrow_weights(dp);
                 __builtin_amdgcn_sched_barrier(0);
+                left = left1, down = down1;
             }
             if (Z::STAGES == 2) {
                 if (more) {
@@ -785,13 +793,16 @@ __global__ __launch_bounds__(Narrow<D>::THREADS, D <= 128 ? 2 : 1) void attentio
         const bool more = first + 32 < end;
         if (more) next.fetch(k, k_rows, first + 32, end, a.width);
         floatx4 s[2] = {floatx4{}, floatx4{}}, dp[2] = {floatx4{}, floatx4{}};
+        // (operands a step ahead of their products)
+        Pieces left = narrow_along<Tile>(ks, 0, 0), down = narrow_along<Tile>(vs, 0, 0);
 #pragma unroll
-        for (int step = 0; step < D / 32; ++step)
-#pragma unroll
-            for (int t = 0; t < 2; ++t) {
-                narrow_both(narrow_along<Tile>(ks, 16 * t, step), qf.step[step], s[t], narrow_along<Tile>(vs, 16 * t, step), gf.step[step], dp[t]);
-                __builtin_amdgcn_sched_barrier(0);
-            }
+        for (int i = 0; i < D / 16; ++i) {
+            Pieces left1 = left, down1 = down;
+            if (i + 1 < D / 16) left1 = narrow_along<Tile>(ks, 16 * ((i + 1) & 1), (i + 1) / 2), down1 = narrow_along<Tile>(vs, 16 * ((i + 1) & 1), (i + 1) / 2);
+            narrow_both(left, qf.step[i / 2], s[i & 1], down, gf.step[i / 2], dp[i & 1]);
+            __builtin_amdgcn_sched_barrier(0);
+            left = left1, down = down1;
+        }
         if (Z::STAGES == 2 && more) {
             next.store(to);
             next.fetch(v, v_rows, first + 32, end, a.width);
@@ -813,8 +824,15 @@ __global__ __launch_bounds__(Narrow<D>::THREADS, D <= 128 ? 2 : 1) void attentio
                     if (first + 16 * t + 4 * g + e >= end) dp[t][e] = 0.0f;
         }
         const Pieces ds = narrow_weights(dp);
+        left = narrow_across<Tile>(ks, 0), down = narrow_across<Tile>(ks, 16);
 #pragma unroll
-        for (int c = 0; c < D / 16; ++c) dq.acc[c] = narrow_mul(narrow_across<Tile>(ks, 16 * c), ds, dq.acc[c]);
+        for (int c = 0; c < D / 16; c += 2) {
+            Pieces left1 = left, down1 = down;
+            if (c + 2 < D / 16) left1 = narrow_across<Tile>(ks, 16 * c + 32), down1 = narrow_across<Tile>(ks, 16 * c + 48);
+            narrow_both(left, ds, dq.acc[c], down, ds, dq.acc[c + 1]);
+            __builtin_amdgcn_sched_barrier(0);
+            left = left1, down = down1;
+        }
         if (Z::STAGES == 2) {
             if (more) next.store(to + Tile::BYTES);
             __syncthreads();

@@ -358,7 +358,7 @@ __device__ __forceinline__ T level_of(T lse) {
 // KEYS, VALUES: which of dk and dv it forms.
 template <typename T, int D>
 struct StatesShape {
-    static constexpr int RT = 32, RK = D * sizeof(T) <= 256 ? 2 : 1;
+    static constexpr int RT = 32, RK = sizeof(T) == 8 && D <= 32 ? 2 : 1;  // (float: where pieces do not serve)
     static constexpr bool BOTH = D * sizeof(T) <= 1024;  // both gradients' sums and both operands fit a wave's registers
     static constexpr int LDS = 2 * Staged<T, D, RT>::BYTES + 2 * RT * (int)sizeof(T);
 };
@@ -493,7 +493,7 @@ __device__ __forceinline__ void states_gradient_tile(const Args& a, char* lds, i
 // The gradient of the rows: as the forward pass, with the weights known from lse.
 template <typename T, int D>
 struct RowsShape {
-    static constexpr int KT = 32, RQ = D * sizeof(T) <= 256 ? 2 : 1;
+    static constexpr int KT = 32, RQ = sizeof(T) == 8 && D <= 32 ? 2 : 1;
     static constexpr int LDS = 2 * Staged<T, D, KT>::BYTES;
 };
 
