@@ -9,6 +9,9 @@
 // The arrangement is that of attention_tiles.h with instructions of 32x32x16: states by rows, a row of the problem (or a state, for the gradients of states) to a lane
 // (lane % 32), whose scores leave the instruction in the order in which the next product takes them as its right operand. Left operands lie in LDS as three planes of rows,
 // padded: along a row they are read 16 bytes at a time, across rows by the transposing read, four rows of a column to a lane.
+//
+// What bounds it: products fill 0.29 (forward) to 0.48 (gradient of states, heads of 128) of the cycles; cutting, exponentials and waits for LDS beside them, which two waves to a
+// vector unit hide in part. us: 16x256x512 with 16 heads of 64 forward 55 (with fp32 instructions 84), its gradient 191 (280); 2x1999x4001, 8 heads on 2 of 128, gradient 1129 (2270).
 #ifndef DALI_HIP_ATTENTION_SPLIT_H
 #define DALI_HIP_ATTENTION_SPLIT_H
 
@@ -527,8 +530,9 @@ __global__ __launch_bounds__(256, 2) void attention_rows_gradient_split(Args a) 
 }
 
 // ------------------------------------------------------------------------------------------------ backward, wide heads
-// Heads of more than 64: 32 columns of two operands and their sums would leave a wave's vector unit to itself, with nobody to work while it waits (heads of 128: 802 and 628 us at
-// 2x1999x4001). So a wave takes 16 with instructions of 16x16x32: half the registers, and two waves to a unit where heads have 128; each value read from LDS is used half as often.
+// Heads of more than 64: 32 columns of two operands and their sums would leave a wave's vector unit to itself, with nobody to work while it waits (heads of 128: 802 and 628 us for the
+// states and the rows of 2x1999x4001, so 690 and 505). So a wave takes 16 with instructions of 16x16x32: half the registers, and two waves to a unit where heads have 128; each value
+// read from LDS is used half as often.
 // Lane l holds eight values of every 32 of its column l % 16, and of the results the rows 4 (l / 16) + (0..3).
 __device__ __forceinline__ floatx4 narrow_mul(const Pieces& a, const Pieces& b, floatx4 c) {
     constexpr int left[6] = {2, 0, 1, 1, 0, 0}, right[6] = {0, 2, 1, 0, 1, 0};

@@ -9,7 +9,11 @@
 //
 // A workgroup of four waves takes a tile of 128 x 128, a wave 64 x 64 of it as 2 x 2 sums of v_mfma_f32_32x32x16_bf16; slabs of 16 of the inner extent go through two stages of
 // 24 KiB, written by the loads themselves; 48 KiB and at most 168 registers, so that three workgroups share a compute unit and two multiply while one waits (three stages and two
-// workgroups: 2750 us against 2620 for [8192,1024].[1024,32000]). All six products go into one sum, four of the instruction's sums in turn.
+// workgroups: 2750 us against 2620 for [8192,1024].[1024,32000]). All six products go into one sum, four of the instruction's sums in turn. (sgemm_split.hip
+// keeps the small ones apart, which costs registers and vector work and comes closer to double precision: gradients of [8192,1024].[1024,32000] 2.3e-7 away from it, here 1.0e-6, products in
+// fp32 instructions 3.1e-6.)
+//
+// Bound by the matrix pipe: 0.81 of the cycles at the clock that the power limit leaves, 211 TFLOP/s in fp32 terms ([8192,1024].[1024,32000] 2550 us).
 //
 // A sum that is not finite (values from 2^111 and sums from 2^96 on, infinities, NaN): the tile is taken again with the fp32 instruction on the values, put together from their pieces.
 #ifndef DALI_HIP_PRODUCT_OF_PIECES_H

@@ -7,7 +7,8 @@
 // Many rows in fp32 go by products of matrices that are cut beforehand, with the softmax at their ends (further below). Else the vocabulary is taken in pieces, the rows in
 // blocks, so that a piece of logits holds at most kPieceBytes and stays in the 256 MiB cache between the product that
 // writes it and the kernel that reads it. Forward, every kSegment columns of a row leave a maximum and a sum of weights relative to it, and a last launch joins a
-// row's. Backward, the piece is formed again and becomes g in its place; the products add it up in the order of pieces and blocks.
+// row's (up to 1024 rows: the last workgroup of a row does). Backward, the piece is formed again and becomes g in its place; the products add it up in the order of pieces and
+// blocks. Bound by the products: [8,1024].[1024,50257] 47.5 us, of which 41 read w; fp64 gradients of [301,515].[515,10007] 313, of which 308 three products.
 #include <algorithm>
 #include <cmath>
 
@@ -344,7 +345,8 @@ int cross_entropy_backward(int64_t rows, int inputs, int vocab, const T* d_losse
 // ------------------------------------------------------------------------------------------------ many rows in fp32
 // Products of images (product_of_pieces.h): x is cut once for all pieces of the vocabulary, a piece of w once for all products with it. The logits come out transposed, a
 // row of them to a lane. Forward they are folded where they are and never leave the registers: every 64 columns leave a maximum and a sum. Backward they become g, which is
-// written as an image at once for both products with it.
+// written as an image at once for both products with it. Bound by the matrix pipe. [8192,1024].[1024,32000]: 2550 us forward (3580 through memory with products that cut
+// their operands themselves), gradients 8170 (10840): logits 690, dx 670 and dw 670 for each of four pieces of the vocabulary.
 constexpr size_t kWeightImageBytes = (size_t)256 << 20, kSlopeImageBytes = (size_t)512 << 20;
 
 struct ImageCut {

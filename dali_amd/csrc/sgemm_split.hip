@@ -49,6 +49,7 @@
 // flipped where bit 3 of r is set: eight neighbouring rows touch eight different 16-byte columns of 128 bytes, sixteen touch sixteen of
 // 256, when reading and when writing.
 #include <cstdlib>
+#include <optional>
 #include <type_traits>
 
 #include "runtime.h"
@@ -612,7 +613,11 @@ int choose_shares(const SplitArgs& g, int cus, double fp32_rate, bool long_rate,
 
 int launch_split(SplitArgs& g, void (*kernel)(SplitArgs)) {
     const long tiles = (long)g.tiles_m * g.tiles_n;
-    g.partials = (float*)(workspace() + kWorkspaceCounterBytes);
+    // (shares are left for another launch: another host thread's come before or after both)
+    static_assert(kCarriedBytes >= kWorkspacePartialBytes, "room for as many shares");
+    std::optional<Carried> carried;
+    if (g.shares > 1) carried.emplace();
+    g.partials = carried ? (float*)carried->data() : nullptr;
     hipLaunchKernelGGL(kernel, dim3((unsigned)(tiles * g.shares)), dim3(256), 0, stream(), g);
     hipError_t e = hipGetLastError();
     if (e == hipSuccess && g.shares > 1) {
