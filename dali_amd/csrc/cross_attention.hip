@@ -43,7 +43,7 @@ __global__ __launch_bounds__(256, D * sizeof(T) <= 512 ? 2 : 1) void attention_r
 
 // ------------------------------------------------------------------------------------------------ few rows
 // Up to 16 RQ rows: nobody shares a state with another wave, so each of the four takes states of its own, straight from memory into the operands (16 at a time,
-// 64-byte pieces of a state), and they are joined in LDS. Bound by reading the states: 32x1x2048 with 16 heads on 4 of 64, 101 MB, 28.7 us.
+// 64-byte pieces of a state), and they are joined in LDS. Bound by reading the states: 32x1x2048 with 16 heads on 4 of 64, 101 MB, 28.5 us.
 template <typename T, int D, int RQ>
 __global__ __launch_bounds__(256, D * sizeof(T) <= 512 ? 2 : 1) void attention_few(Args a) {
     typedef Matrix<T> M;
@@ -56,8 +56,11 @@ __global__ __launch_bounds__(256, D * sizeof(T) <= 512 ? 2 : 1) void attention_f
     const int id = on_die(blockIdx.x, gridDim.x);
     const int at = id / a.parts, part = id - at * a.parts, problem = a.first + at;
     const int b = problem / a.kv_heads, kvh = problem - b * a.kv_heads;
-    const int n = count_of(a, b), slabs = (n + 15) / 16, mine = part * 4 + wave;
-    const int begin = (int)((int64_t)slabs * mine / (4 * a.parts)), end = (int)((int64_t)slabs * (mine + 1) / (4 * a.parts));
+    // (a sequence with fewer states has fewer parts, not shorter ones)
+    const int n = count_of(a, b), slabs = (n + 15) / 16, mine = part * 4 + wave, most = ((a.keys + 15) / 16 + a.parts - 1) / a.parts;
+    const int parts = max(1, (slabs + most - 1) / max(most, 1));
+    if (part >= parts) return;
+    const int begin = (int)((int64_t)slabs * mine / (4 * parts)), end = (int)((int64_t)slabs * (mine + 1) / (4 * parts));
     const T* q = (const T*)a.q.p + b * a.q.batch + (int64_t)kvh * a.group * a.q.head;
     const T* k = (const T*)a.k.p + b * a.k.batch + kvh * a.k.head;
     const T* v = (const T*)a.v.p + b * a.v.batch + kvh * a.v.head;
@@ -182,7 +185,7 @@ __global__ __launch_bounds__(256, D * sizeof(T) <= 512 ? 2 : 1) void attention_f
             const int r = 16 * i + lane;
             sums[r] = all[i];  // from here on the row's own
             if (r >= a.rows) continue;
-            if (a.parts == 1) {
+            if (parts == 1) {
                 ((T*)a.lse_out)[dense_row<T>(a, b, kvh, r)] = all[i] == T(0) ? T(-INFINITY) : M::lse(best[i], all[i]);
             } else {
                 publish((T*)a.parts_m + part * pitch + own + r, best[i]);
@@ -192,7 +195,7 @@ __global__ __launch_bounds__(256, D * sizeof(T) <= 512 ? 2 : 1) void attention_f
     }
     __syncthreads();
     const int groups = a.rows * (D / N);
-    if (a.parts == 1) {
+    if (parts == 1) {
         for (int at = threadIdx.x; at < groups; at += 256) {
             const int r = at / (D / N), c = at % (D / N) * N;
             if (c >= a.width) continue;
@@ -210,15 +213,15 @@ __global__ __launch_bounds__(256, D * sizeof(T) <= 512 ? 2 : 1) void attention_f
         for (int e = 0; e < N; ++e) publish((T*)a.parts_y + (part * pitch + own + r) * D + c + e, ys[r * (D + N) + c + e]);
     }
     __shared__ unsigned ticket;
-    if (!last_to_arrive(a.counters + at * a.counter_step, a.parts, &ticket)) return;
+    if (!last_to_arrive(a.counters + at * a.counter_step, parts, &ticket)) return;
     const T *pm = (const T*)a.parts_m + own, *pl = (const T*)a.parts_l + own, *py = (const T*)a.parts_y + own * D;
     for (int at = threadIdx.x; at < groups; at += 256) {
         const int r = at / (D / N), c = at % (D / N) * N;
         T top = M::lowest, sum = 0, values[N] = {};
 #pragma unroll 4
-        for (int p = 0; p < a.parts; ++p) top = Max()(top, observe(pm + p * pitch + r));
+        for (int p = 0; p < parts; ++p) top = Max()(top, observe(pm + p * pitch + r));
 #pragma unroll 4
-        for (int p = 0; p < a.parts; ++p) {
+        for (int p = 0; p < parts; ++p) {
             const T f = M::weight(observe(pm + p * pitch + r) - top);
             sum += observe(pl + p * pitch + r) * f;
 #pragma unroll
@@ -305,8 +308,8 @@ constexpr int kUnits = 256;  // compute units that work is cut for
 
 // Parts that the states (or rows) are cut into, so that every compute unit has about `per_unit` workgroups, none with less than `least` slabs. As many to a unit as it holds at once
 // does best: gradients with heads of up to 64 two (4x1000x2000, heads of 64: 801 us with one, 686 with two, 738 with three), of more than 64 one (4x512x1024, heads of 256:
-// 501, 536, 565); single positions three,
-// whose states come from memory (32x1x2048: 30.3 us with two, 28.6 with three).
+// 501, 536, 565); single positions with heads of up to 64 floats three (32x1x2048: 30.3 us with two, 28.2 with three), wider ones two (8x1x4096, 32 heads
+// on 8 of 128: 59, 81), and at most 32 for a problem, since one workgroup joins them (1x1x8000, 16 heads of 64: 22 us, 26 with 48).
 int parts_for(int64_t workgroups, int slabs, int per_unit, int least) {
     if (workgroups >= kUnits * per_unit) return 1;
     const int64_t wanted = ((int64_t)kUnits * per_unit + workgroups - 1) / workgroups;
@@ -327,7 +330,7 @@ struct ForwardPlan {
         rq = a.rows <= 16 ? 1 : 2;
         const int rows = std::is_same_v<T, float> ? 128 : 64 * S::RQ;
         tiles = few ? 1 : (a.rows + rows - 1) / rows;
-        parts = few ? parts_for(problems, (a.keys + 63) / 64, 3, 2) : parts_for(problems * tiles, (a.keys + S::KT - 1) / S::KT, 2, 4);
+        parts = few ? std::min(32, parts_for(problems, (a.keys + 63) / 64, D * sizeof(T) <= 256 ? 3 : 2, 2)) : parts_for(problems * tiles, (a.keys + S::KT - 1) / S::KT, 2, 4);
     }
 };
 
