@@ -225,7 +225,7 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void attention_rows_split(Ar
     qf.load(q + q_rows.at(min(row, a.rows - 1)), a.width, (float)(a.scale * Matrix<float>::base * kUp));
     SplitColumns<D> y;
     y.clear();
-    float top = Matrix<float>::lowest, sum = 0;  // (of the scores as they are; of the lane's own states)
+    float top = Matrix<float>::lowest, sum = 0, lowest = 0;  // (of the scores as they are; of the lane's own states; of the scores times 2^32)
     Tile kt, vt;
     if (begin < end) {
         kt.fetch(k, k_rows, begin * KT, n, a.width);
@@ -247,6 +247,11 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void attention_rows_split(Ar
         for (int step = 0; step < D / 16; ++step)
 #pragma unroll
             for (int t = 0; t < KT / 32; ++t) s[t] = multiply(Tile::along(ks, 32 * t, step), qf.step[step], s[t]);
+        // (a sum that passed -2^128 on its way stays -inf and would weigh nothing; one that passed 2^128 makes its row NaN)
+#pragma unroll
+        for (int t = 0; t < KT / 32; ++t)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) lowest = fminf(lowest, s[t][e]);
         if ((slab + 1) * KT > n) {
             asm volatile("");  // (a branch that the other slabs jump over, no selection that they all make)
 #pragma unroll
@@ -286,7 +291,7 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void attention_rows_split(Ar
     }
     sum = fold_lanes<64, 32>(sum, Sum());
     // (a sum of 0: scores that are all -inf, or below what their pieces hold)
-    const bool bad = begin < end && (!(sum > 0.0f && sum < INFINITY) || !y.finite());
+    const bool bad = begin < end && (!(sum > 0.0f && sum < INFINITY) || lowest == -INFINITY || !y.finite());
     if (__syncthreads_or(bad)) {
         constexpr int STEP = 64 * ForwardShape<float, D>::RQ;
         for (int r = 0; r < 128 && tile * 128 + r < a.rows; r += STEP) {

@@ -1,0 +1,32 @@
+"""Attention to an encoder's states where values are extreme: scores whose partial sums pass what bf16 pieces hold, infinities in the last state. Bounds as in test_gpu_cross_attention.py."""
+import numpy as np
+import pytest
+
+from test_gpu_cross_attention import check_forward, make
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("width", [64, 100, 128, 200, 256])
+@pytest.mark.parametrize("queries,keys", [(70, 90), (150, 700)])
+@pytest.mark.parametrize("sign", [-1, 1])
+def test_scores_whose_partial_sums_are_large(gpu, D, rng, width, queries, keys, sign):
+    """The products of one state are 1.25 * 2^91 over 30 values of the width and the opposite over the next 30: every sum of them is exact in fp32 (a multiple of 1.25 * 2^91 of at most six
+    bits) and the score 0, but halfway it passes 2^96. So the results are those of a state of zeros. (The scale is ln 2, which times log2 e is 1: operands stay powers of two.)"""
+    q, k, v, counts = make(rng, np.float32, 2, queries, keys, 2, 1, width, [keys, keys // 2])
+    large = np.arange(width) % 16 != 15  # (fifteen of every sixteen values; the others are ordinary ones)
+    large[64:] = False
+    ordinary = ~large
+    q[..., large], k[..., large] = 0, 0
+    k[:, 7] = 0
+    big_q, big_k = q.copy(), k.copy()
+    big_q[..., large] = 2.0 ** 46
+    big_k[:, 7, :, :32][..., large[:32]] = sign * 1.25 * 2.0 ** 45
+    big_k[:, 7, :, 32:64][..., large[32:64]] = -sign * 1.25 * 2.0 ** 45
+    assert ordinary.any()
+    A = D.Array.from_numpy
+    check_forward(D, q, k, v, counts, np.log(2.0), D.op.cross_attention(A(big_q), A(big_k), A(v), A(counts), np.log(2.0)))
+    # smaller ordinary scores, so that the state weighs as much as others do whatever the width
+    for a in (q, big_q):
+        a[..., ordinary] *= np.float32(4.0 / width)
+    check_forward(D, q, k, v, counts, np.log(2.0), D.op.cross_attention(A(big_q), A(big_k), A(v), A(counts), np.log(2.0)))
