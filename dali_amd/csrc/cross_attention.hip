@@ -72,7 +72,7 @@ __global__ __launch_bounds__(256, D * sizeof(T) <= 512 ? 2 : 1) void attention_f
     Running<T> run[RQ];
 #pragma unroll
     for (int i = 0; i < RQ; ++i) y[i].clear();
-    // 16 states as left operands, along them and across them (states past the last one weigh nothing, but must not be infinite either: the last one stands in)
+    // 16 states as left operands, along them and across them (the last state stands in for those behind it, whose scores are -inf and whose values become zeros)
     struct Slab {
         typename Vec<T>::type left[C];
         typename Columns<T, D>::values across[4][Columns<T, D>::BLOCKS];
@@ -98,7 +98,7 @@ __global__ __launch_bounds__(256, D * sizeof(T) <= 512 ? 2 : 1) void attention_f
             }
         }
     };
-    auto take = [&](const Slab& from, int slab) {
+    auto take = [&](Slab& from, int slab) {
         typename M::acc s[RQ][1];
 #pragma unroll
         for (int i = 0; i < RQ; ++i) {
@@ -111,9 +111,12 @@ __global__ __launch_bounds__(256, D * sizeof(T) <= 512 ? 2 : 1) void attention_f
         if (slab * 16 + 16 > n) {
 #pragma unroll
             for (int e = 0; e < 4; ++e)
-                if (slab * 16 + M::row_of(e, g) >= n)
+                if (slab * 16 + M::row_of(e, g) >= n) {
 #pragma unroll
                     for (int i = 0; i < RQ; ++i) s[i][0][e] = T(-INFINITY);
+#pragma unroll
+                    for (int blk = 0; blk < Columns<T, D>::BLOCKS; ++blk) from.across[e][blk] = typename Columns<T, D>::values{};
+                }
         }
 #pragma unroll
         for (int i = 0; i < RQ; ++i) {

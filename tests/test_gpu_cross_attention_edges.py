@@ -30,3 +30,21 @@ def test_scores_whose_partial_sums_are_large(gpu, D, rng, width, queries, keys, 
     for a in (q, big_q):
         a[..., ordinary] *= np.float32(4.0 / width)
     check_forward(D, q, k, v, counts, np.log(2.0), D.op.cross_attention(A(big_q), A(big_k), A(v), A(counts), np.log(2.0)))
+
+
+@pytest.mark.parametrize("queries", [1, 12, 70])
+@pytest.mark.parametrize("dtype", [np.float32, np.float64])
+@pytest.mark.parametrize("keys", [1, 15, 33, 90, 700])
+def test_an_infinite_value_of_the_last_state(gpu, D, rng, queries, dtype, keys):
+    """It comes out in its own column, whatever the kernel puts in the places behind the last state."""
+    A, op = D.Array.from_numpy, D.op
+    for width in (8, 64, 128, 256):
+        q, k, v, _ = make(rng, dtype, 2, queries, keys, 2, 1, width)
+        counts = np.array([keys, max(1, keys - 9)], np.int32)
+        for b in range(2):
+            v[b, counts[b] - 1, 0, 3] = np.inf
+        y, lse = (a.numpy() for a in op.cross_attention(A(q), A(k), A(v), A(counts), 0.1))
+        assert np.isfinite(lse).all() and (y[..., 3] == np.inf).all()
+        clean = v.copy()
+        clean[..., 3], y[..., 3] = 0, 0
+        check_forward(D, q, k, clean, counts, 0.1, (A(y), A(lse)))
