@@ -75,9 +75,17 @@ __device__ __forceinline__ float together(const char* at) {
     return h == h ? (h + __uint_as_float(piece(1) << 16) + __uint_as_float(piece(2) << 16)) * kDown : __uint_as_float(piece(1) << 16 | piece(2));
 }
 
-// The image of a matrix [rows, cols]: rows `ld` values apart (BY_COLUMNS: columns), a thread eight neighbours of a row. Rows without a target are zeros, whatever they hold.
+// Which rows have a part in a gradient: those with a target and with weight (null: all of them)
+struct Takes {
+    const int32_t* targets;
+    const float* lse;
+    int vocab;
+    __device__ __forceinline__ bool row(int r) const { return !targets || ((unsigned)targets[r] < (unsigned)vocab && lse[r] != -INFINITY); }
+};
+
+// The image of a matrix [rows, cols]: rows `ld` values apart (BY_COLUMNS: columns), a thread eight neighbours of a row. Rows that are not taken are zeros, whatever they hold.
 template <bool BY_COLUMNS>
-__global__ __launch_bounds__(256) void make_image(const float* x, int64_t ld, int rows, int cols, int row_blocks, int col_blocks, const int32_t* targets, int vocab, char* image) {
+__global__ __launch_bounds__(256) void make_image(const float* x, int64_t ld, int rows, int cols, int row_blocks, int col_blocks, Takes takes, char* image) {
     const int t = threadIdx.x, r = BY_COLUMNS ? t & 15 : t >> 4, group = BY_COLUMNS ? t >> 4 : t & 15;
     const int across = (col_blocks + 7) / 8, rb = blockIdx.x / across, cb = (blockIdx.x - rb * across) * 8 + (group >> 1);
     if (rb >= row_blocks || cb >= col_blocks) return;
@@ -85,7 +93,7 @@ __global__ __launch_bounds__(256) void make_image(const float* x, int64_t ld, in
     float v[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[i] = 0.0f;
-    if (row < rows && (!targets || (unsigned)targets[row] < (unsigned)vocab)) {
+    if (row < rows && takes.row(row)) {
         if (BY_COLUMNS) {
 #pragma unroll
             for (int i = 0; i < 8; ++i)
@@ -112,10 +120,10 @@ __global__ __launch_bounds__(256) void make_image(const float* x, int64_t ld, in
 }
 
 template <bool BY_COLUMNS>
-int image_of(const char* what, const float* x, int64_t ld, int rows, int cols, const int32_t* targets, int vocab, char* image) {
+int image_of(const char* what, const float* x, int64_t ld, int rows, int cols, const Takes& takes, char* image) {
     const int row_blocks = blocks_of(rows), col_blocks = blocks_of(cols);
     const int64_t blocks = (int64_t)row_blocks * ((col_blocks + 7) / 8);
-    make_image<BY_COLUMNS><<<dim3((unsigned)blocks), dim3(256), 0, stream()>>>(x, ld, rows, cols, row_blocks, col_blocks, targets, vocab, image);
+    make_image<BY_COLUMNS><<<dim3((unsigned)blocks), dim3(256), 0, stream()>>>(x, ld, rows, cols, row_blocks, col_blocks, takes, image);
     return launched(what);
 }
 

@@ -231,12 +231,12 @@ int cross_entropy(int64_t rows, int inputs, int vocab, const T* x, int64_t x_str
 }
 
 // ------------------------------------------------------------------------------------------------ backward
-// x with zeros in the rows that have no target, whatever those hold: they have no part in dw
+// x with zeros in the rows that have no target or no weight, whatever those hold: they have no part in dw
 template <typename T>
-__global__ __launch_bounds__(256) void entropy_inputs(const T* x, int64_t x_stride, int inputs, const int32_t* targets, int vocab, T* kept) {
+__global__ __launch_bounds__(256) void entropy_inputs(const T* x, int64_t x_stride, int inputs, const int32_t* targets, const T* lse, int vocab, T* kept) {
     constexpr int N = Vec<T>::N;
     const int row = blockIdx.x, target = targets[row];
-    const bool there = target >= 0 && target < vocab;
+    const bool there = target >= 0 && target < vocab && lse[row] != T(-INFINITY);
     for (int c = threadIdx.x * N; c < inputs; c += 256 * N) {
         T v[N] = {};
         if (there) load_group(x + row * x_stride, c, inputs, T(0), v);
@@ -319,7 +319,7 @@ int cross_entropy_backward(int64_t rows, int inputs, int vocab, const T* d_losse
     }
     for (int64_t r = 0; r < rows; r += cut.block) {
         const int n = (int)std::min<int64_t>(cut.block, rows - r), chunks = (n + cut.chunk - 1) / cut.chunk;
-        entropy_inputs<T><<<dim3((unsigned)n), dim3(256), 0, stream()>>>(x + r * x_stride, x_stride, inputs, targets + r, vocab, kept);
+        entropy_inputs<T><<<dim3((unsigned)n), dim3(256), 0, stream()>>>(x + r * x_stride, x_stride, inputs, targets + r, lse + r, vocab, kept);
         if (launched(what)) return DALI_HIP_ERROR;
         for (int64_t v = 0; v < vocab; v += cut.piece) {
             const int width = (int)std::min<int64_t>(cut.piece, vocab - v);
@@ -523,7 +523,7 @@ __global__ __launch_bounds__(256, 3) void entropy_slopes(pieces::Product g, int 
 }
 
 int weight_image(const char* what, const float* w, int64_t w_stride, bool w_by_columns, int inputs, int width, char* image) {
-    return w_by_columns ? pieces::image_of<true>(what, w, w_stride, inputs, width, nullptr, 0, image) : pieces::image_of<false>(what, w, w_stride, inputs, width, nullptr, 0, image);
+    return w_by_columns ? pieces::image_of<true>(what, w, w_stride, inputs, width, {}, image) : pieces::image_of<false>(what, w, w_stride, inputs, width, {}, image);
 }
 
 int cross_entropy_by_images(int64_t rows, int inputs, int vocab, const float* x, int64_t x_stride, const float* w, int64_t w_stride, bool w_by_columns, const float* bias,
@@ -535,7 +535,7 @@ int cross_entropy_by_images(int64_t rows, int inputs, int vocab, const float* x,
     for (int64_t r = 0; r < rows; r += cut.block) {
         const int n = (int)std::min<int64_t>(cut.block, rows - r);
         const Image xs = {space + cut.x, blocks_of(n), blocks_of(inputs)};
-        if (image_of<false>(what, x + r * x_stride, x_stride, n, inputs, nullptr, 0, space + cut.x)) return DALI_HIP_ERROR;
+        if (image_of<false>(what, x + r * x_stride, x_stride, n, inputs, {}, space + cut.x)) return DALI_HIP_ERROR;
         for (int64_t v = 0; v < vocab; v += cut.piece) {
             const int width = (int)std::min<int64_t>(cut.piece, vocab - v);
             const Image ws = {space + cut.w, blocks_of(inputs), blocks_of(width)};
@@ -560,7 +560,7 @@ int cross_entropy_backward_by_images(int64_t rows, int inputs, int vocab, const 
     for (int64_t r = 0; r < rows; r += cut.block) {
         const int n = (int)std::min<int64_t>(cut.block, rows - r), chunks = (n + 63) / 64;
         const Image xs = {space + cut.x, blocks_of(n), blocks_of(inputs)};
-        if (image_of<false>(what, x + r * x_stride, x_stride, n, inputs, targets + r, vocab, space + cut.x)) return DALI_HIP_ERROR;
+        if (image_of<false>(what, x + r * x_stride, x_stride, n, inputs, {targets + r, lse + r, vocab}, space + cut.x)) return DALI_HIP_ERROR;
         for (int64_t v = 0; v < vocab; v += cut.piece) {
             const int width = (int)std::min<int64_t>(cut.piece, vocab - v);
             const Image ws = {space + cut.w, blocks_of(inputs), blocks_of(width)}, gs = {space + cut.slopes, blocks_of(n), blocks_of(width)};

@@ -298,8 +298,9 @@ def projected_cross_entropy(x, w, targets, bias=None, out=None):
 
 
 def projected_cross_entropy_backward(d_losses, x, w, targets, lse, bias=None, out=None):
-    """(dx, dw, dbias) from d_losses and the lse that ``projected_cross_entropy`` left; without bias, dbias is None. A row without a target has no part in them, whatever it
-    holds, nor has a row whose logits are all -inf. dw lies in memory as w does: where w is a transposed view, its destination may be one too."""
+    """(dx, dw, dbias) from d_losses and the lse that ``projected_cross_entropy`` left; without bias, dbias is None. A row without a target has no part in them, whatever x
+    holds there, nor has a row whose logits are all -inf. Words are taken out by a bias of -inf: an infinity of w multiplies weights of 0 as well, and makes NaN of dx.
+    dw lies in memory as w does: where w is a transposed view, its destination may be one too."""
     return _bind.projected_cross_entropy_backward(d_losses, x, w, targets, lse, bias, out)
 
 

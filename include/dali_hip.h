@@ -430,8 +430,8 @@ int dali_hip_projected_cross_entropy(int dtype, int64_t rows, int inputs, int vo
                                      const void* bias, const int32_t* targets, void* losses, void* lse, void* workspace);
 /*
  * Its gradients from d_losses and the lse of the forward pass: with g = d_losses (e^(logit - lse) - [target]), dx = g w^T [rows, inputs], dw = x^T g [inputs, vocab] or (dw_by_columns)
- * [vocab, inputs], dbias = sum of g over the rows; all dense; bias and dbias come together. A row without a target has no part in them whatever it holds (its dx is 0), nor has
- * one of logits of -inf alone.
+ * [vocab, inputs], dbias = sum of g over the rows; all dense; bias and dbias come together. A row without a target has no part in them whatever x holds there (its dx is 0), nor has
+ * one of logits of -inf alone. An infinity of w makes NaN of every row's dx in the place that it multiplies, also where its word has no weight: words are taken out by the bias.
  */
 int dali_hip_projected_cross_entropy_backward(int dtype, int64_t rows, int inputs, int vocab, const void* d_losses, const void* x, int64_t x_stride, const void* w,
                                               int64_t w_stride, int w_by_columns, const void* bias, const int32_t* targets, const void* lse, void* dx, void* dw,
