@@ -430,7 +430,8 @@ __global__ __launch_bounds__(256, D <= 64 ? 2 : 1) void attention_states_gradien
     if (key >= a.keys) return;
     const int64_t to = part * a.part_size + (((int64_t)b * a.keys + key) * a.kv_heads + kvh) * a.width;
     // (behind the last state: what its stand-in came to is not the gradient, which is zero)
-    dk.times(key < n ? (float)a.scale * kDownTwice : 0.0f);
+    dk.times(key < n ? kDownTwice : 0.0f);
+    dk.times((float)a.scale);  // (a factor of its own: the product of the two may be too small for its digits)
     dv.times(key < n ? kDownTwice : 0.0f);
     dk.each([&](int c, const auto& values) { store_run((float*)a.dk + to, c, a.width, values); });
     dv.each([&](int c, const auto& values) { store_run((float*)a.dv + to, c, a.width, values); });
@@ -530,7 +531,8 @@ __global__ __launch_bounds__(256, 2) void attention_rows_gradient_split(Args a) 
     }
     if (row >= a.rows) return;
     float* out = (float*)a.dq + part * a.part_size + own * a.width;
-    dq.times((float)a.scale * kDownTwice);
+    dq.times(kDownTwice);
+    dq.times((float)a.scale);
     dq.each([&](int c, const auto& values) { store_run(out, c, a.width, values); });
 }
 
@@ -617,11 +619,12 @@ struct NarrowColumns {
             for (int v = 0; v < 4; ++v) probe = fmaf(acc[b][v], 0.0f, probe);
         return probe == 0.0f;
     }
-    __device__ __forceinline__ void put(float* row, int width, float factor) const {
+    // times both factors, one after the other (their product may be too small for its digits)
+    __device__ __forceinline__ void put(float* row, int width, float first, float then) const {
         const int g = (threadIdx.x & 63) >> 4;
 #pragma unroll
         for (int b = 0; b < D / 16; ++b) {
-            const float run[4] = {acc[b][0] * factor, acc[b][1] * factor, acc[b][2] * factor, acc[b][3] * factor};
+            const float run[4] = {acc[b][0] * first * then, acc[b][1] * first * then, acc[b][2] * first * then, acc[b][3] * first * then};
             store_run(row, 16 * b + 4 * g, width, run);
         }
     }
@@ -760,8 +763,8 @@ __global__ __launch_bounds__(Narrow<D>::THREADS, D <= 128 ? 2 : 1) void attentio
     if (key >= a.keys) return;
     const int64_t to = part * a.part_size + (((int64_t)b * a.keys + key) * a.kv_heads + kvh) * a.width;
     // (behind the last state: what its stand-in came to is not the gradient, which is zero)
-    dk.put((float*)a.dk + to, a.width, key < n ? (float)a.scale * kDownTwice : 0.0f);
-    dv.put((float*)a.dv + to, a.width, key < n ? kDownTwice : 0.0f);
+    dk.put((float*)a.dk + to, a.width, key < n ? kDownTwice : 0.0f, (float)a.scale);
+    dv.put((float*)a.dv + to, a.width, key < n ? kDownTwice : 0.0f, 1.0f);
 }
 
 template <int D>
@@ -860,7 +863,7 @@ __global__ __launch_bounds__(Narrow<D>::THREADS, D <= 128 ? 2 : 1) void attentio
         return;
     }
     if (row >= a.rows) return;
-    dq.put((float*)a.dq + part * a.part_size + own * a.width, a.width, (float)a.scale * kDownTwice);
+    dq.put((float*)a.dq + part * a.part_size + own * a.width, a.width, kDownTwice, (float)a.scale);
 }
 
 }  // namespace

@@ -2,7 +2,7 @@
 import numpy as np
 import pytest
 
-from test_gpu_cross_attention import check_forward, make
+from test_gpu_cross_attention import check_backward, check_forward, make
 
 pytestmark = pytest.mark.gpu
 
@@ -48,3 +48,10 @@ def test_an_infinite_value_of_the_last_state(gpu, D, rng, queries, dtype, keys):
         clean = v.copy()
         clean[..., 3], y[..., 3] = 0, 0
         check_forward(D, q, k, clean, counts, 0.1, (A(y), A(lse)))
+
+
+@pytest.mark.parametrize("width", [32, 64, 128, 256])
+def test_gradients_with_a_small_scale(gpu, D, rng, width):
+    """A scale of 1e-33, whose gradients dy of about 2^60 brings back to ordinary numbers."""
+    q, k, v, counts = make(rng, np.float32, 2, 70, 90, 2, 1, width, [90, 47])
+    check_backward(D, (rng.randn(*q.shape) * 2.0 ** 60).astype(np.float32), q, k, v, counts, 1e-33)
