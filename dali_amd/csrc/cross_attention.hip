@@ -493,7 +493,8 @@ int check_extents(const char* what, int dtype, int batch, int queries, int keys,
     if (batch < 0 || queries < 0 || keys < 0) return fail("%s: %d sequences of %d positions and %d states", what, batch, queries, keys);
     if (heads < 1 || kv_heads < 1 || heads % kv_heads) return fail("%s: %d heads cannot share %d", what, heads, kv_heads);
     if (width < 1 || width > DALI_HIP_MAX_HEAD_WIDTH) return fail("%s: heads are from 1 to %d wide (got %d)", what, DALI_HIP_MAX_HEAD_WIDTH, width);
-    if (!std::isfinite(scale)) return fail("%s: the scale must be finite (got %g)", what, scale);
+    if (!holds_scale(dtype, scale) || (dtype == DALI_HIP_FLOAT && !holds_scale(dtype, scale * Matrix<float>::base)))
+        return fail("%s: the scale must be finite in its operands' type, in float times log2 e too (got %g)", what, scale);
     const int group = heads / kv_heads;
     if ((int64_t)queries * group > 1 << 28 || keys > 1 << 28 || (int64_t)batch * kv_heads > 2147483647LL)
         return fail("%s: %d sequences of %d positions and %d states with %d heads are too many", what, batch, queries, keys, heads);

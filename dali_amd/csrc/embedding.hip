@@ -242,7 +242,7 @@ int check_embedding(const char* what, int dtype, int64_t count, int rows, int wi
     if (count < 0 || count > 2147483647LL - 256) return fail("%s: %lld tokens", what, (long long)count);
     if (rows < 1) return fail("%s: a table of %d rows", what, rows);
     if (width < 1) return fail("%s: rows of %d values", what, width);
-    if (!std::isfinite(scale)) return fail("%s: the scale must be finite (got %g)", what, scale);
+    if (!holds_scale(dtype, scale)) return fail("%s: the scale must be finite in its operands' type (got %g)", what, scale);
     return DALI_HIP_OK;
 }
 

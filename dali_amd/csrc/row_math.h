@@ -5,6 +5,7 @@
 
 #include <hip/hip_runtime.h>
 
+#include <cmath>
 #include <cstdint>
 #include <initializer_list>
 #include <type_traits>
@@ -231,6 +232,8 @@ inline bool off_elements(std::initializer_list<const void*> pointers, size_t siz
 }
 
 inline bool is_real(int dtype) { return dtype == DALI_HIP_FLOAT || dtype == DALI_HIP_DOUBLE; }
+// whether a factor, given in double, is a finite number of the operands' type as well
+inline bool holds_scale(int dtype, double scale) { return std::isfinite(dtype == DALI_HIP_FLOAT ? (double)(float)scale : scale); }
 
 inline int launched(const char* what) {
     const hipError_t e = hipGetLastError();

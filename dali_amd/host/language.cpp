@@ -66,6 +66,11 @@ Array destination(const char* what, const char* name, const Array& given, const 
     return given;
 }
 
+void check_scale(const char* what, double scale, DType dtype) {
+    DALI_ASSERT(std::isfinite(dtype == DTYPE_FLOAT ? (double)(float)scale : scale),
+                make_message(what, ": the scale must be finite (got ", scale, " for ", dtype_to_cpp_name(dtype), ")"));
+}
+
 // what an entry of the library keeps beside its operands for the time of a call (or as long as a recording holds it)
 template <typename Bytes>
 Array workspace(const char* what, const Bytes& bytes) {
@@ -268,7 +273,7 @@ Array embedding(const Array& table, const Array& tokens, double scale, const Arr
     DALI_ASSERT(table.ndim() == 2 && is_real(table) && table.shape()[0] >= 1 && table.shape()[1] >= 1,
                 make_message(what, ": the table must be a float or double matrix that is not empty"));
     DALI_ASSERT(tokens.dtype() == DTYPE_INT32, make_message(what, ": tokens must be int"));
-    DALI_ASSERT(std::isfinite(scale), make_message(what, ": the scale must be finite (got ", scale, ")"));
+    check_scale(what, scale, table.dtype());
     const DType dtype = table.dtype();
     std::vector<int> shape = tokens.shape();
     shape.push_back(table.shape()[1]);
@@ -291,7 +296,7 @@ Array embedding_backward(const Array& dy, const Array& tokens, int rows, double 
     DALI_ASSERT(dy.ndim() >= 1 && is_real(dy) && dy.shape().back() >= 1, make_message(what, ": dy must be float or double and have a last axis that is not empty"));
     check_shape(what, "tokens", tokens, leading(dy), DTYPE_INT32);
     DALI_ASSERT(rows >= 1, make_message(what, ": a table has at least one row (got ", rows, ")"));
-    DALI_ASSERT(std::isfinite(scale), make_message(what, ": the scale must be finite (got ", scale, ")"));
+    check_scale(what, scale, dy.dtype());
     const DType dtype = dy.dtype();
     const int width = dy.shape().back();
     const Array r = destination(what, "dtable", out, {rows, width}, dtype);
@@ -324,7 +329,7 @@ struct AttentionSizes {
         check_shape(what, "values", v, k.shape(), dtype);
         DALI_ASSERT(heads >= 1 && kv_heads >= 1 && heads % kv_heads == 0, make_message(what, ": ", heads, " heads cannot share ", kv_heads));
         if (!counts.is_stateless()) check_shape(what, "key_counts", counts, {batch}, DTYPE_INT32);
-        DALI_ASSERT(std::isfinite(scale), make_message(what, ": the scale must be finite (got ", scale, ")"));
+        check_scale(what, scale, dtype);
     }
 };
 

@@ -388,6 +388,7 @@ int dali_hip_token_log_probs_backward(int dtype, int64_t rows, int vocab, const 
  * Operators of an encoder-decoder language model; the reference has none of them. dtype: DALI_HIP_FLOAT or DALI_HIP_DOUBLE, of every operand that is not int32. They allocate
  * nothing: where a function ..._workspace is declared, `workspace` is device memory of the bytes that it answers for the same extents, on 256 bytes, which must not
  * overlap anything and holds nothing before or after the call. Destinations must not overlap operands or each other. Results do not depend on the order of arrivals.
+ * A scale is rounded to the type and has to be finite in it (attention in float: times log2 e too).
  */
 
 /*
