@@ -144,12 +144,52 @@ __global__ __launch_bounds__(64) void embedding_chunks(const T* dy, int64_t stri
     leave(end, end < count && keys[end] == token);
 }
 
-// A workgroup sees to `per` neighbouring rows of the table (at most 15): zeros where no token names one, and the parts of a run that lies in several chunks, in their order.
-// A wave takes every fourth 64 groups of columns.
-template <typename T, bool PAST>
+// What the chunks `first` to `last` of a row's run have come to, in their order, by a wave: columns from c0 on, the next ones `step` further. NARROW: the row has at most 32 groups; as many
+// lanes read its groups as it takes, a power of two, and others parts further on, which are handed over in their order (a token of 1550 places in rows of 27: 23 us, so 16).
+template <typename T, bool NARROW, bool PAST>
+__device__ __forceinline__ void join_run(int width, int chunk, int from, int to, const T* partials, T scale, T* row, int c0, int step) {
+    constexpr int N = Vec<T>::N, DEEP = 8;
+    const int lane = threadIdx.x & 63, first = from / chunk, last = (to - 1) / chunk;
+    const T* head = partials + ((int64_t)first * 2 + (from % chunk ? 1 : 0)) * width;
+    int lanes = NARROW ? 1 : 64;
+    if (NARROW)
+        while (lanes * N < width) lanes *= 2;
+    const int teams = 64 / lanes, team = lane / lanes;
+    for (int c = c0 + lane % lanes * N; c < width || NARROW; c += step) {
+        T sum[N];
+        load_group(head, c, width, T(0), sum);
+        for (int p = first + 1; p <= last; p += DEEP * teams) {
+            typename Vec<T>::type g[DEEP];
+#pragma unroll
+            for (int j = 0; j < DEEP; ++j) g[j] = ask_group(partials + (int64_t)min(p + j * teams + team, last) * 2 * width, c, width);
+#pragma unroll
+            for (int j = 0; j < DEEP; ++j) {
+                if (p + j * teams > last) break;
+                T v[N];
+                take_group(g[j], c, width, T(0), v);
+                if constexpr (NARROW) {
+                    for (int t = 0; t < teams && p + j * teams + t <= last; ++t)
+#pragma unroll
+                        for (int e = 0; e < N; ++e) sum[e] += __shfl(v[e], t * lanes + lane % lanes);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < N; ++e) sum[e] += v[e];
+                }
+            }
+        }
+#pragma unroll
+        for (int e = 0; e < N; ++e) sum[e] *= scale;
+        if (team == 0) store_group<PAST>(row, c, width, sum);
+        if (NARROW) break;
+    }
+}
+
+// A workgroup sees to `per` neighbouring rows of the table (at most 15): zeros where no token names one, and the parts of a run that lies in several chunks. A wave takes every fourth 64
+// groups of columns, or, NARROW, every fourth row.
+template <typename T, bool NARROW, bool PAST>
 __global__ __launch_bounds__(256) void embedding_gradient(int width, const int32_t* keys, int count, int rows, int chunk, int first_row, int per, const T* partials, T scale,
                                                           T* dtable) {
-    constexpr int N = Vec<T>::N, DEEP = 8;
+    constexpr int N = Vec<T>::N;
     __shared__ int begin[16];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int r0 = first_row + blockIdx.x * per, here = min(per, rows - r0);
@@ -158,32 +198,88 @@ __global__ __launch_bounds__(256) void embedding_gradient(int width, const int32
         if (threadIdx.x % 16 == 0) begin[i] = at;
     }
     __syncthreads();
-    for (int r = 0; r < here; ++r) {
-        const int from = begin[r], to = begin[r + 1];
-        const int first = from / chunk, last = (to - 1) / chunk;
-        if (from < to && first == last) continue;  // written already
+    for (int r = NARROW ? wave : 0; r < here; r += NARROW ? 4 : 1) {
+        const int from = begin[r], to = begin[r + 1], c0 = NARROW ? 0 : wave * 64 * N;
         T* out = dtable + (int64_t)(r0 + r) * width;
-        for (int c = (wave * 64 + lane) * N; c < width; c += 256 * N) {
-            T sum[N] = {};
-            if (from < to) {
-                load_group(partials + ((int64_t)first * 2 + (from % chunk ? 1 : 0)) * width, c, width, T(0), sum);
-                for (int p = first + 1; p <= last; p += DEEP) {
-                    typename Vec<T>::type g[DEEP];
+        if (from < to) {
+            if (from / chunk != (to - 1) / chunk) join_run<T, NARROW, PAST>(width, chunk, from, to, partials, scale, out, c0, 256 * N);  // (else written already)
+            continue;
+        }
+        const T zeros[N] = {};
+        for (int c = c0 + lane * N; c < width; c += (NARROW ? 64 : 256) * N) store_group<PAST>(out, c, width, zeros);
+    }
+}
+
+// The same for tables most of whose rows no token names: up to 1024 rows or 32 KiB to a workgroup, whose zeros go over them as over one array, in groups on 16 bytes.
+constexpr int kMostRowsEach = 1024, kBytesEach = 32768;
+
+template <typename T, bool NARROW>
+__global__ __launch_bounds__(256) void embedding_gradient_sparse(int width, unsigned width_m, int width_s, const int32_t* keys, int count, int rows, int chunk, int first_row, int per,
+                                                                 const T* partials, T scale, T* dtable) {
+    constexpr int N = Vec<T>::N;
+    __shared__ int begin[kMostRowsEach + 1];
+    __shared__ int ends[2];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int r0 = first_row + blockIdx.x * per, here = min(per, rows - r0);
+    if (wave == 0) {
+        const int at = lower_bound(keys, count, (unsigned)(r0 + (lane < 16 ? 0 : here)));
+        if (lane == 0 || lane == 16) ends[lane / 16] = at;
+    }
+    __syncthreads();
+    const int low = ends[0], high = ends[1];
+    T* out = dtable + (int64_t)r0 * width;
+    const int n = here * width;                                                                        // (of many rows at most kBytesEach, else a row's width)
+    const int head = (int)((16 - (uintptr_t)out % 16) % 16 / sizeof(T)), start = head ? head - N : 0;  // (the first group may begin before the rows)
+    typedef T aligned_group __attribute__((ext_vector_type(N)));
+    const auto zeros = [&](int64_t e) { *reinterpret_cast<aligned_group*>(out + e) = aligned_group{}; };
+    if (low == high) {  // no token of these rows
+        for (int64_t e = start + (int)threadIdx.x * N; e < n; e += 256 * N) {
+            if (e >= 0 && e + N <= n) {
+                zeros(e);
+            } else {
 #pragma unroll
-                    for (int j = 0; j < DEEP; ++j) g[j] = ask_group(partials + (int64_t)min(p + j, last) * 2 * width, c, width);
-#pragma unroll
-                    for (int j = 0; j < DEEP; ++j) {
-                        if (p + j > last) break;
-                        T v[N];
-                        take_group(g[j], c, width, T(0), v);
-#pragma unroll
-                        for (int e = 0; e < N; ++e) sum[e] += v[e];
-                    }
-                }
+                for (int i = 0; i < N; ++i)
+                    if (e + i >= 0 && e + i < n) out[e + i] = T(0);
             }
+        }
+        return;
+    }
+    for (int i = threadIdx.x; i <= here; i += 256) {
+        int lo = low, hi = high;
+        while (lo < hi) {
+            const int mid = lo + (hi - lo) / 2;
+            if ((unsigned)keys[mid] < (unsigned)(r0 + i)) lo = mid + 1;
+            else hi = mid;
+        }
+        begin[i] = lo;
+    }
+    __syncthreads();
+    for (int64_t e = start + (int)threadIdx.x * N; e < n; e += 256 * N) {
+        const int a = (int)max(e, (int64_t)0), b = (int)min(e + N, (int64_t)n) - 1;
+        int r = (int)sgemm_row_map_div((unsigned)a, width_m, width_s);
+        const bool one = r == (int)sgemm_row_map_div((unsigned)b, width_m, width_s);
+        if (one && begin[r] != begin[r + 1]) continue;
+        if (one && e >= 0 && e + N <= n) {
+            zeros(e);
+            continue;
+        }
+        int64_t end = (int64_t)(r + 1) * width;  // of row r
 #pragma unroll
-            for (int e = 0; e < N; ++e) sum[e] *= scale;
-            store_group<PAST>(out, c, width, sum);
+        for (int i = 0; i < N; ++i) {
+            const int64_t x = e + i;
+            if (x < a || x > b) continue;
+            while (x >= end) ++r, end += width;
+            if (begin[r] == begin[r + 1]) out[x] = T(0);
+        }
+    }
+    for (int base = 0, k = 0; base < here; base += 64) {
+        const int mine = base + lane;
+        unsigned long long rest = __ballot(mine < here && begin[min(mine, here - 1)] < begin[min(mine, here - 1) + 1] &&
+                                           begin[min(mine, here - 1)] / chunk != (begin[min(mine, here - 1) + 1] - 1) / chunk);
+        for (; rest; rest &= rest - 1, ++k) {
+            const int r = base + __ffsll((long long)rest) - 1;
+            if (!NARROW || (k & 3) == wave)
+                join_run<T, NARROW, false>(width, chunk, begin[r], begin[r + 1], partials, scale, out + (int64_t)r * width, NARROW ? 0 : wave * 64 * N, 256 * N);
         }
     }
 }
@@ -224,13 +320,25 @@ int embedding_backward(int64_t count, int rows, int width, const T* dy, int64_t 
                                                                                                                  first, (T)scale, dtable, partials);
         if (launched(what)) return DALI_HIP_ERROR;
     }
-    const int per = std::max(1, std::min(15, rows / 2048));
+    // A large table of which few rows are named is zeros for the most part: [44681,2199] for 34 tokens 134 us row by row, 90 (zeros alone 73), [119465,128] for one 59 and 20. Where the
+    // named rows are more, the first launch has brought much of the table into the caches, and rows past them row by row are quicker ([43264,1344] fp64 for 5312 tokens 129 us, 150);
+    // short rows gain as long as there are more of them than tokens ([79168,10] for 20084: 76, 47).
+    const bool narrow = width <= 32 * Vec<T>::N, sparse = rows >= 16384 && (rows >= 16 * count || (narrow && rows > count));
+    const int per = sparse ? std::max(1, std::min({(int)(kBytesEach / sizeof(T) / width), kMostRowsEach, rows / 1024})) : std::max(1, std::min(15, rows / 2048));
+    int shift = 0;
+    while (((int64_t)1 << shift) < width) ++shift;
+    const unsigned times = (unsigned)((((uint64_t)1 << (31 + shift)) + width - 1) / width);  // (of an exact division by the width)
     const bool past = past_caches((double)rows * width * sizeof(T));
     for (int64_t first = 0; first < rows; first += (int64_t)most * per) {
-        const int64_t blocks = std::min((rows - first + per - 1) / per, (int64_t)most);
-        either_way(past, [&](auto p) {
-            embedding_gradient<T, decltype(p)::value>
-                <<<dim3((unsigned)blocks), dim3(256), 0, stream()>>>(width, keys, (int)count, rows, chunk, (int)first, per, partials, (T)scale, dtable);
+        const dim3 grid((unsigned)std::min((rows - first + per - 1) / per, (int64_t)most));
+        either_way(narrow, [&](auto n) {
+            constexpr bool NARROW = decltype(n)::value;
+            if (sparse)
+                embedding_gradient_sparse<T, NARROW><<<grid, dim3(256), 0, stream()>>>(width, times, shift, keys, (int)count, rows, chunk, (int)first, per, partials, (T)scale, dtable);
+            else
+                either_way(past, [&](auto p) {
+                    embedding_gradient<T, NARROW, decltype(p)::value><<<grid, dim3(256), 0, stream()>>>(width, keys, (int)count, rows, chunk, (int)first, per, partials, (T)scale, dtable);
+                });
         });
         if (launched(what)) return DALI_HIP_ERROR;
     }
