@@ -293,7 +293,7 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void attention_rows_split(Ar
     // (a sum of 0: scores that are all -inf, or below what their pieces hold)
     const bool bad = begin < end && (!(sum > 0.0f && sum < INFINITY) || lowest == -INFINITY || !y.finite());
     if (__syncthreads_or(bad)) {
-        constexpr int STEP = 64 * ForwardShape<float, D>::RQ;
+        constexpr int STEP = ForwardShape<float, D>::ROWS;
         for (int r = 0; r < 128 && tile * 128 + r < a.rows; r += STEP) {
             __syncthreads();
             rows_tile<float, D>(a, attention_lds, problem, part, tile * 128 + r);
@@ -420,10 +420,10 @@ __global__ __launch_bounds__(256, D <= 64 ? 2 : 1) void attention_states_gradien
         }
     }
     if (__syncthreads_or(extreme == INFINITY || !dk.finite() || !dv.finite())) {
-        constexpr int STEP = 64 * StatesShape<float, D>::RK;
+        constexpr int STEP = StatesShape<float, D>::STATES;
         for (int r = 0; r < 128; r += STEP) {
             __syncthreads();
-            states_gradient_tile<float, D, true, true>(a, attention_lds, problem, part, tile * 128 + r);
+            states_gradient_tile<float, D>(a, attention_lds, problem, part, tile * 128 + r);
         }
         return;
     }
@@ -522,7 +522,7 @@ __global__ __launch_bounds__(256, 2) void attention_rows_gradient_split(Args a) 
         __syncthreads();
     }
     if (__syncthreads_or(extreme == INFINITY || !dq.finite())) {
-        constexpr int STEP = 64 * RowsShape<float, D>::RQ;
+        constexpr int STEP = RowsShape<float, D>::ROWS;
         for (int r = 0; r < 128 && tile * 128 + r < a.rows; r += STEP) {
             __syncthreads();
             rows_gradient_tile<float, D>(a, attention_lds, problem, part, tile * 128 + r);
@@ -757,7 +757,7 @@ __global__ __launch_bounds__(Narrow<D>::THREADS, D <= 128 ? 2 : 1) void attentio
         }
     }
     if (__syncthreads_or(extreme == INFINITY || !dk.finite() || !dv.finite())) {
-        states_gradient_tile<float, D, true, true, Z::THREADS>(a, attention_lds, problem, part, tile * Z::MINE);
+        states_gradient_tile<float, D, Z::THREADS>(a, attention_lds, problem, part, tile * Z::MINE);
         return;
     }
     if (key >= a.keys) return;

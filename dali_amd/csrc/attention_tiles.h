@@ -99,40 +99,115 @@ __device__ __forceinline__ typename Vec<T>::type row_group(const T* row, int c, 
     }
     return g;
 }
+// LATE, below: heads of more than 128 doubles that are not 256 wide. All that a thread brings is asked for before any is put in its place. (Put there at once, each group is waited for:
+// gradients of 23x420x102 with 2 heads of 187 535 us, and 302. Narrower heads are quicker without, their registers are full; for whole rows there is nothing to put in its place, and a kernel
+// that does either at run time spills.)
 
-// What a lane holds of 16 rows as a right operand: row lane % 16, groups lane / 16 of every four
-template <typename T, int D>
+// What a lane holds of 16 rows as a right operand: row lane % 16, groups lane / 16 of every four, from value c0 of W on
+template <typename T, int D, int W = D, bool LATE = false>
 struct Fragment {
     static constexpr int N = Vec<T>::N, C = D / (4 * N);
     typename Vec<T>::type g[C];
-    __device__ __forceinline__ void load(const T* row, int width, T factor) {
+    __device__ __forceinline__ void load(const T* row, int width, T factor, int c0 = 0) {
         const int lane = threadIdx.x & 63;
+        if constexpr (!LATE) {
 #pragma unroll
-        for (int c = 0; c < C; ++c) g[c] = row_group<D>(row, (4 * c + (lane >> 4)) * N, width) * factor;
+            for (int c = 0; c < C; ++c) g[c] = row_group<W>(row, c0 + (4 * c + (lane >> 4)) * N, width) * factor;
+        } else {
+#pragma unroll
+            for (int c = 0; c < C; ++c) g[c] = ask_group<true>(row, c0 + (4 * c + (lane >> 4)) * N, width);
+#pragma unroll
+            for (int c = 0; c < C; ++c) {
+                T v[N];
+                take_group<true>(g[c], c0 + (4 * c + (lane >> 4)) * N, width, T(0), v);
+#pragma unroll
+                for (int e = 0; e < N; ++e) g[c][e] = v[e] * factor;
+            }
+        }
+    }
+};
+
+// Heads of more than 128 doubles: two waves share 16 rows (or states), each with half of the width, since operands and sums of all of it do not fit a wave's registers (up to 696 of them
+// were spilled, and the gradients of the states took two launches). Each forms half of a score's sum, and they meet in LDS; results are the half's own. The halves are whole blocks of 32,
+// as even as that allows. Gradients of 3x878x3987, 4 heads of 256: 9990 us, so 3790; forward 4x500x1000, 8 heads on 4 of 256: 977, 502. Bound by the matrix pipe for half of the
+// time (one wave to a vector unit: nobody works while it waits).
+template <typename T, int D>
+struct Halves {
+    static constexpr int H = D * sizeof(T) > 1024 ? 2 : 1, W = D / H;  // waves that share rows, and the most that one has of the width
+    static constexpr int GROUPS = 4 / H;                              // of waves in a workgroup of four
+    int wave, group, c0, mine;                                        // the wave; its group; what it has of the width: from c0 on, `mine`
+    __device__ __forceinline__ explicit Halves(int width) : wave(threadIdx.x >> 6) {
+        group = wave / H;
+        mine = H == 1 ? D : (width + 63) / 64 * 32;
+        c0 = wave % H * mine;
+    }
+    // whether the wave's share ends before its value c
+    __device__ __forceinline__ bool ends(int c) const { return H > 1 && c >= mine; }
+    static constexpr int bytes(int tiles) { return H == 1 ? 0 : 2 * 4 * tiles * 256 * (int)sizeof(T); }
+    // the sums of both halves, by way of `space` ([2][4 waves][tiles][4][64], whose halves are written in turn: with one barrier a time nobody writes what another still reads)
+    template <int TILES>
+    __device__ __forceinline__ void meet(T* space, int& turn, typename Matrix<T>::acc* (&s)[TILES]) const {
+        if constexpr (H > 1) {
+            const int lane = threadIdx.x & 63;
+            T* all = space + turn * 4 * TILES * 256 + lane;
+#pragma unroll
+            for (int t = 0; t < TILES; ++t)
+#pragma unroll
+                for (int v = 0; v < 4; ++v) all[((wave * TILES + t) * 4 + v) * 64] = (*s[t])[v];
+            __syncthreads();
+#pragma unroll
+            for (int t = 0; t < TILES; ++t)
+#pragma unroll
+                for (int v = 0; v < 4; ++v) (*s[t])[v] += all[(((wave ^ 1) * TILES + t) * 4 + v) * 64];
+            turn ^= 1;
+        }
     }
 };
 
 // A tile of R rows of D values in LDS, a group of padding behind each row: sixteen rows' groups at one place lie in different banks
-template <typename T, int D, int R, int THREADS = 256>
+template <typename T, int D, int R, int THREADS = 256, bool LATE = false>
 struct Staged {
     static constexpr int N = Vec<T>::N, PITCH = D + N, GROUPS = D / N, EACH = R * GROUPS / THREADS;
     static constexpr int BYTES = R * PITCH * sizeof(T);
     static_assert(R * GROUPS % THREADS == 0, "whole groups to every thread");
     typename Vec<T>::type g[EACH];
-    // rows [first, first + R) of those below `end`, zeros elsewhere
+    int there;  // rows of the tile
+    // rows [first, first + R) of those below `end` (first is), zeros elsewhere
     __device__ __forceinline__ void fetch(const T* base, const Rows& rows, int first, int end, int width) {
+        there = end - first;
+        if constexpr (!LATE) {
 #pragma unroll
-        for (int i = 0; i < EACH; ++i) {
-            const int at = threadIdx.x + i * THREADS, r = first + at / GROUPS, c = at % GROUPS * N;
-            g[i] = r < end ? row_group<D>(base + rows.at(r), c, width) : typename Vec<T>::type{};
+            for (int i = 0; i < EACH; ++i) {
+                const int at = threadIdx.x + i * THREADS, r = first + at / GROUPS;
+                g[i] = r < end ? row_group<D>(base + rows.at(r), at % GROUPS * N, width) : typename Vec<T>::type{};
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < EACH; ++i) {
+                const int at = threadIdx.x + i * THREADS;
+                g[i] = ask_group<true>(base + rows.at(min(first + at / GROUPS, end - 1)), at % GROUPS * N, width);
+            }
         }
     }
-    __device__ __forceinline__ void store(T* lds) const {
+    __device__ __forceinline__ void store(T* lds, int width) const {
+        typedef T aligned_group __attribute__((ext_vector_type(16 / sizeof(T))));
+        if constexpr (!LATE) {
 #pragma unroll
-        for (int i = 0; i < EACH; ++i) {
-            const int at = threadIdx.x + i * THREADS;
-            typedef T aligned_group __attribute__((ext_vector_type(16 / sizeof(T))));
-            *reinterpret_cast<aligned_group*>(lds + at / GROUPS * PITCH + at % GROUPS * N) = g[i];
+            for (int i = 0; i < EACH; ++i) {
+                const int at = threadIdx.x + i * THREADS;
+                *reinterpret_cast<aligned_group*>(lds + at / GROUPS * PITCH + at % GROUPS * N) = g[i];
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < EACH; ++i) {
+                const int at = threadIdx.x + i * THREADS, c = at % GROUPS * N;
+                T v[N];
+                take_group<true>(g[i], c, width, T(0), v);
+                aligned_group to;
+#pragma unroll
+                for (int e = 0; e < N; ++e) to[e] = at / GROUPS < there ? v[e] : T(0);
+                *reinterpret_cast<aligned_group*>(lds + at / GROUPS * PITCH + c) = to;
+            }
         }
     }
     // the left operand along the rows: row r + lane % 16, group 4 c + lane / 16
@@ -238,20 +313,26 @@ __device__ __forceinline__ int64_t dense_row(const Args& a, int b, int kvh, int 
 }
 
 // ------------------------------------------------------------------------------------------------ forward
-// A workgroup of four waves takes 64 RQ rows of a problem, a wave 16 RQ of them, over a part of the states, KT at a time through LDS.
+// A workgroup of four waves takes 64 RQ rows of a problem, a wave (or two) 16 RQ of them, over a part of the states, KT at a time through LDS.
 template <typename T, int D>
 struct ForwardShape {
-    static constexpr int KT = D * sizeof(T) <= 256 ? 64 : 32, RQ = D * sizeof(T) <= 512 ? 2 : 1;
-    static constexpr int LDS = 2 * Staged<T, D, KT>::BYTES;
+    static constexpr int KT = D * sizeof(T) <= 256 ? 64 : D * sizeof(T) <= 1024 ? 32 : 16, RQ = D * sizeof(T) <= 512 ? 2 : 1, ROWS = 16 * RQ * Halves<T, D>::GROUPS;
+    static constexpr int TILES = 2 * Staged<T, D, KT>::BYTES, LDS = TILES + Halves<T, D>::bytes(KT / 16);
 };
 
-template <typename T, int D>
+// (LATE: see above; else heads of more than 128 doubles are 256 wide)
+template <typename T, int D, bool LATE = false>
 __device__ __forceinline__ void rows_tile(const Args& a, char* lds, int problem, int part, int first_row) {
     typedef Matrix<T> M;
     typedef ForwardShape<T, D> S;
-    constexpr int KT = S::KT, RQ = S::RQ, N = Vec<T>::N, C = D / (4 * N);
+    typedef Halves<T, D> Z;
+    constexpr int KT = S::KT, RQ = S::RQ, N = Vec<T>::N, W = Z::W, C = W / (4 * N);
+    static_assert(Z::H == 1 || (RQ == 1 && KT == 16), "one tile of scores meets at a time");
     T *ks = reinterpret_cast<T*>(lds), *vs = ks + KT * Staged<T, D, KT>::PITCH;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4;
+    const int lane = threadIdx.x & 63, g = lane >> 4;
+    const int width = Z::H > 1 && !LATE ? D : a.width;
+    const Z z(width);
+    int turn = 0;
     const int b = problem / a.kv_heads, kvh = problem - b * a.kv_heads;
     const int n = count_of(a, b), slabs = (n + KT - 1) / KT;
     const int begin = (int)((int64_t)slabs * part / a.parts), end = (int)((int64_t)slabs * (part + 1) / a.parts);
@@ -259,27 +340,27 @@ __device__ __forceinline__ void rows_tile(const Args& a, char* lds, int problem,
     const T* k = (const T*)a.k.p + b * a.k.batch + kvh * a.k.head;
     const T* v = (const T*)a.v.p + b * a.v.batch + kvh * a.v.head;
     const Rows q_rows(a, a.q), k_rows(a.k), v_rows(a.v);
-    const int r0 = first_row + wave * 16 * RQ;
-    Fragment<T, D> qf[RQ];
+    const int r0 = first_row + z.group * 16 * RQ;
+    Fragment<T, W, D, LATE> qf[RQ];
 #pragma unroll
-    for (int i = 0; i < RQ; ++i) qf[i].load(q + q_rows.at(min(r0 + 16 * i + (lane & 15), a.rows - 1)), a.width, (T)(a.scale * M::base));
-    Columns<T, D> y[RQ];
+    for (int i = 0; i < RQ; ++i) qf[i].load(q + q_rows.at(min(r0 + 16 * i + (lane & 15), a.rows - 1)), width, (T)(a.scale * M::base), z.c0);
+    Columns<T, W> y[RQ];
     Running<T> run[RQ];
 #pragma unroll
     for (int i = 0; i < RQ; ++i) y[i].clear();
-    Staged<T, D, KT> kt, vt;
+    Staged<T, D, KT, 256, LATE> kt, vt;
     if (begin < end) {
-        kt.fetch(k, k_rows, begin * KT, n, a.width);
-        vt.fetch(v, v_rows, begin * KT, n, a.width);
+        kt.fetch(k, k_rows, begin * KT, n, width);
+        vt.fetch(v, v_rows, begin * KT, n, width);
     }
     for (int slab = begin; slab < end; ++slab) {
         __syncthreads();
-        kt.store(ks);
-        vt.store(vs);
+        kt.store(ks, width);
+        vt.store(vs, width);
         __syncthreads();
         if (slab + 1 < end) {
-            kt.fetch(k, k_rows, (slab + 1) * KT, n, a.width);
-            vt.fetch(v, v_rows, (slab + 1) * KT, n, a.width);
+            kt.fetch(k, k_rows, (slab + 1) * KT, n, width);
+            vt.fetch(v, v_rows, (slab + 1) * KT, n, width);
         }
         typename M::acc s[RQ][KT / 16];
 #pragma unroll
@@ -288,12 +369,17 @@ __device__ __forceinline__ void rows_tile(const Args& a, char* lds, int problem,
             for (int i = 0; i < RQ; ++i) s[i][t] = typename M::acc{};
 #pragma unroll
             for (int c = 0; c < C; ++c) {
-                const typename Vec<T>::type left = Staged<T, D, KT>::along(ks, 16 * t, c);
+                if (z.ends(c * 4 * N)) break;
+                const typename Vec<T>::type left = Staged<T, D, KT>::along(ks + z.c0, 16 * t, c);
 #pragma unroll
                 for (int e = 0; e < N; ++e)
 #pragma unroll
                     for (int i = 0; i < RQ; ++i) s[i][t] = M::mul(left[e], qf[i].g[c][e], s[i][t]);
             }
+        }
+        if constexpr (Z::H > 1) {
+            typename M::acc* halves[1] = {&s[0][0]};
+            z.meet(reinterpret_cast<T*>(lds + S::TILES), turn, halves);
         }
         if ((slab + 1) * KT > n) {
 #pragma unroll
@@ -313,12 +399,13 @@ __device__ __forceinline__ void rows_tile(const Args& a, char* lds, int problem,
         for (int t = 0; t < KT / 16; ++t)
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                const T* row = vs + (16 * t + M::row_of(e, g)) * Staged<T, D, KT>::PITCH;
+                const T* row = vs + (16 * t + M::row_of(e, g)) * Staged<T, D, KT>::PITCH + z.c0;
 #pragma unroll
-                for (int blk = 0; blk < Columns<T, D>::BLOCKS; ++blk) {
-                    const auto left = Columns<T, D>::across(row, blk);
+                for (int blk = 0; blk < Columns<T, W>::BLOCKS; ++blk) {
+                    if (z.ends(blk * 16 * Columns<T, W>::NV)) break;
+                    const auto left = Columns<T, W>::across(row, blk);
 #pragma unroll
-                    for (int c = 0; c < Columns<T, D>::NV; ++c)
+                    for (int c = 0; c < Columns<T, W>::NV; ++c)
 #pragma unroll
                         for (int i = 0; i < RQ; ++i) y[i].acc[blk][c] = M::mul(left[c], s[i][t][e], y[i].acc[blk][c]);
                 }
@@ -332,14 +419,18 @@ __device__ __forceinline__ void rows_tile(const Args& a, char* lds, int problem,
         if (a.parts == 1) {
             const int64_t to = dense_row<T>(a, b, kvh, r);
             y[i].times(sum == T(0) ? T(0) : T(1) / sum);
-            T* out = (T*)a.y_out + to * a.width;
-            y[i].each([&](int c, const auto& values) { store_run(out, c, a.width, values); });
-            if (g == 0) ((T*)a.lse_out)[to] = sum == T(0) ? T(-INFINITY) : M::lse(run[i].top, sum);
+            T* out = (T*)a.y_out + to * width;
+            y[i].each([&](int c, const auto& values) {
+                if (c < z.mine) store_run(out, z.c0 + c, width, values);
+            });
+            if (g == 0 && z.c0 == 0) ((T*)a.lse_out)[to] = sum == T(0) ? T(-INFINITY) : M::lse(run[i].top, sum);
         } else {
             const int64_t to = ((int64_t)part * a.batch * a.kv_heads + problem) * a.rows + r;
             T* out = (T*)a.parts_y + to * D;
-            y[i].each([&](int c, const auto& values) { store_run(out, c, D, values); });
-            if (g == 0) ((T*)a.parts_m)[to] = run[i].top, ((T*)a.parts_l)[to] = sum;
+            y[i].each([&](int c, const auto& values) {
+                if (c < z.mine) store_run(out, z.c0 + c, D, values);
+            });
+            if (g == 0 && z.c0 == 0) ((T*)a.parts_m)[to] = run[i].top, ((T*)a.parts_l)[to] = sum;
         }
     }
 }
@@ -354,50 +445,51 @@ __device__ __forceinline__ T level_of(T lse) {
     return lse == T(-INFINITY) ? T(INFINITY) : lse * (T)Matrix<T>::base;
 }
 
-// The gradients of the states: a workgroup takes 64 RK states (of four waves), a wave 16 RK of them in its registers, and walks over the rows of a part of them, RT at a time through LDS.
-// KEYS, VALUES: which of dk and dv it forms.
+// The gradients of the states: a workgroup takes 64 RK states (of four waves), a wave (or two) 16 RK of them in its registers, and walks over the rows of a part of them, RT at a time
+// through LDS.
 template <typename T, int D>
 struct StatesShape {
-    static constexpr int RT = 32, RK = sizeof(T) == 8 && D <= 32 ? 2 : 1;  // (float: where pieces do not serve)
-    static constexpr bool BOTH = D * sizeof(T) <= 1024;  // both gradients' sums and both operands fit a wave's registers
-    static constexpr int LDS = 2 * Staged<T, D, RT>::BYTES + 2 * RT * (int)sizeof(T);
+    typedef Halves<T, D> Z;
+    static constexpr int RT = Z::H == 1 ? 32 : 16, RK = sizeof(T) == 8 && D <= 32 ? 2 : 1, STATES = 16 * RK * Z::GROUPS;  // (float: where pieces do not serve)
+    static constexpr int TILES = 2 * Staged<T, D, RT>::BYTES + 2 * RT * (int)sizeof(T), LDS = TILES + Z::bytes(2);
 };
 
-template <typename T, int D, bool KEYS, bool VALUES, int THREADS = 256>
+template <typename T, int D, int THREADS = 256, bool LATE = false>
 __device__ __forceinline__ void states_gradient_tile(const Args& a, char* lds, int problem, int part, int first_state) {
     typedef Matrix<T> M;
     typedef StatesShape<T, D> S;
-    constexpr int RT = S::RT, RK = S::RK, N = Vec<T>::N, C = D / (4 * N), PITCH = Staged<T, D, RT, THREADS>::PITCH;
+    typedef Halves<T, D> Z;
+    constexpr int RT = S::RT, RK = S::RK, N = Vec<T>::N, W = Z::W, C = W / (4 * N), PITCH = Staged<T, D, RT, THREADS>::PITCH;
+    static_assert(Z::H == 1 || (RK == 1 && THREADS == 256), "two tiles of scores meet at a time");
     T *qs = reinterpret_cast<T*>(lds), *gs = qs + RT * PITCH, *levels = gs + RT * PITCH, *deltas = levels + RT;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4;
+    const int lane = threadIdx.x & 63, g = lane >> 4;
+    const int width = Z::H > 1 && !LATE ? D : a.width;
+    const Z z(a.width);  // (asked at every step whether its share ends, also where that is known: without the branches the compiler reads further ahead and spills 64 registers)
+    int turn = 0;
     const int b = problem / a.kv_heads, kvh = problem - b * a.kv_heads;
-    const int n = count_of(a, b), k0 = first_state + wave * 16 * RK;
+    const int n = count_of(a, b), k0 = first_state + z.group * 16 * RK;
     const int begin = part_of(a, part, a.rows, RT), end = part_of(a, part + 1, a.rows, RT);
     const T* q = (const T*)a.q.p + b * a.q.batch + (int64_t)kvh * a.group * a.q.head;
     const T* dy = (const T*)a.dy.p + b * a.dy.batch + (int64_t)kvh * a.group * a.dy.head;
     const T* k = (const T*)a.k.p + b * a.k.batch + kvh * a.k.head;
     const T* v = (const T*)a.v.p + b * a.v.batch + kvh * a.v.head;
     const Rows q_rows(a, a.q), dy_rows(a, a.dy);
-    Columns<T, D> dk[KEYS ? RK : 1], dv[VALUES ? RK : 1];
-    if (KEYS)
+    Columns<T, W> dk[RK], dv[RK];
 #pragma unroll
-        for (int i = 0; i < RK; ++i) dk[i].clear();
-    if (VALUES)
-#pragma unroll
-        for (int i = 0; i < RK; ++i) dv[i].clear();
+    for (int i = 0; i < RK; ++i) dk[i].clear(), dv[i].clear();
     if (first_state < n) {
-        Fragment<T, D> kf[RK], vf[KEYS ? RK : 1];
+        Fragment<T, W, D, LATE> kf[RK], vf[RK];
 #pragma unroll
         for (int i = 0; i < RK; ++i) {
             const int key = min(k0 + 16 * i + (lane & 15), n - 1);
-            kf[i].load(k + key * a.k.row, a.width, (T)(a.scale * M::base));
-            if (KEYS) vf[i].load(v + key * a.v.row, a.width, T(1));
+            kf[i].load(k + key * a.k.row, width, (T)(a.scale * M::base), z.c0);
+            vf[i].load(v + key * a.v.row, width, T(1), z.c0);
         }
-        Staged<T, D, RT, THREADS> qt, gt;
+        Staged<T, D, RT, THREADS, LATE> qt, gt;
         T level = 0, delta = 0;
         auto fetch = [&](int r0) {
-            qt.fetch(q, q_rows, r0, end, a.width);
-            gt.fetch(dy, dy_rows, r0, end, a.width);
+            qt.fetch(q, q_rows, r0, end, width);
+            gt.fetch(dy, dy_rows, r0, end, width);
             if (threadIdx.x < RT) {
                 const int r = r0 + threadIdx.x;
                 level = T(INFINITY), delta = 0;
@@ -408,11 +500,11 @@ __device__ __forceinline__ void states_gradient_tile(const Args& a, char* lds, i
                 }
             }
         };
-        fetch(begin);
+        if (begin < end) fetch(begin);
         for (int r0 = begin; r0 < end; r0 += RT) {
             __syncthreads();
-            qt.store(qs);
-            gt.store(gs);
+            qt.store(qs, width);
+            gt.store(gs, width);
             if (threadIdx.x < RT) levels[threadIdx.x] = level, deltas[threadIdx.x] = delta;
             __syncthreads();
             if (r0 + RT < end) fetch(r0 + RT);
@@ -423,23 +515,25 @@ __device__ __forceinline__ void states_gradient_tile(const Args& a, char* lds, i
                 for (int i = 0; i < RK; ++i) s[i] = dp[i] = typename M::acc{};
 #pragma unroll
                 for (int c = 0; c < C; ++c) {
-                    const typename Vec<T>::type left = Staged<T, D, RT, THREADS>::along(qs, 16 * t, c);
+                    if (z.ends(c * 4 * N)) break;
+                    const typename Vec<T>::type left = Staged<T, D, RT, THREADS>::along(qs + z.c0, 16 * t, c), down = Staged<T, D, RT, THREADS>::along(gs + z.c0, 16 * t, c);
 #pragma unroll
                     for (int e = 0; e < N; ++e)
 #pragma unroll
                         for (int i = 0; i < RK; ++i) s[i] = M::mul(left[e], kf[i].g[c][e], s[i]);
-                    if (KEYS) {
-                        const typename Vec<T>::type down = Staged<T, D, RT, THREADS>::along(gs, 16 * t, c);
 #pragma unroll
-                        for (int e = 0; e < N; ++e)
+                    for (int e = 0; e < N; ++e)
 #pragma unroll
-                            for (int i = 0; i < RK; ++i) dp[i] = M::mul(down[e], vf[i].g[c][e], dp[i]);
-                    }
+                        for (int i = 0; i < RK; ++i) dp[i] = M::mul(down[e], vf[i].g[c][e], dp[i]);
+                }
+                if constexpr (Z::H > 1) {
+                    typename M::acc* halves[2] = {&s[0], &dp[0]};
+                    z.meet(reinterpret_cast<T*>(lds + S::TILES), turn, halves);
                 }
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     const int r = 16 * t + M::row_of(e, g);
-                    const T lev = levels[r], del = KEYS ? deltas[r] : T(0);
+                    const T lev = levels[r], del = deltas[r];
 #pragma unroll
                     for (int i = 0; i < RK; ++i) {
                         s[i][e] = lev == T(INFINITY) ? T(0) : M::weight(s[i][e] - lev);
@@ -450,21 +544,17 @@ __device__ __forceinline__ void states_gradient_tile(const Args& a, char* lds, i
                 for (int e = 0; e < 4; ++e) {
                     const int r = 16 * t + M::row_of(e, g);
 #pragma unroll
-                    for (int blk = 0; blk < Columns<T, D>::BLOCKS; ++blk) {
-                        if (VALUES) {
-                            const auto left = Columns<T, D>::across(gs + r * PITCH, blk);
+                    for (int blk = 0; blk < Columns<T, W>::BLOCKS; ++blk) {
+                        if (z.ends(blk * 16 * Columns<T, W>::NV)) break;
+                        const auto of_values = Columns<T, W>::across(gs + r * PITCH + z.c0, blk), of_keys = Columns<T, W>::across(qs + r * PITCH + z.c0, blk);
 #pragma unroll
-                            for (int c = 0; c < Columns<T, D>::NV; ++c)
+                        for (int c = 0; c < Columns<T, W>::NV; ++c)
 #pragma unroll
-                                for (int i = 0; i < RK; ++i) dv[i].acc[blk][c] = M::mul(left[c], s[i][e], dv[i].acc[blk][c]);
-                        }
-                        if (KEYS) {
-                            const auto left = Columns<T, D>::across(qs + r * PITCH, blk);
+                            for (int i = 0; i < RK; ++i) dv[i].acc[blk][c] = M::mul(of_values[c], s[i][e], dv[i].acc[blk][c]);
 #pragma unroll
-                            for (int c = 0; c < Columns<T, D>::NV; ++c)
+                        for (int c = 0; c < Columns<T, W>::NV; ++c)
 #pragma unroll
-                                for (int i = 0; i < RK; ++i) dk[i].acc[blk][c] = M::mul(left[c], dp[i][e], dk[i].acc[blk][c]);
-                        }
+                            for (int i = 0; i < RK; ++i) dk[i].acc[blk][c] = M::mul(of_keys[c], dp[i][e], dk[i].acc[blk][c]);
                     }
                 }
             }
@@ -474,36 +564,42 @@ __device__ __forceinline__ void states_gradient_tile(const Args& a, char* lds, i
     for (int i = 0; i < RK; ++i) {
         const int key = k0 + 16 * i + (lane & 15);
         if (key >= a.keys) continue;
-        const int64_t to = part * a.part_size + (((int64_t)b * a.keys + key) * a.kv_heads + kvh) * a.width;
+        const int64_t to = part * a.part_size + (((int64_t)b * a.keys + key) * a.kv_heads + kvh) * width;
         // (behind the last state: what its stand-in came to is not the gradient, which is zero)
         const bool there = key < n;
-        auto put = [&](T* out, const Columns<T, D>& sums, T factor) {
+        auto put = [&](T* out, const Columns<T, W>& sums, T factor) {
             sums.each([&](int c, const auto& values) {
-                T run[Columns<T, D>::NV];
+                T run[Columns<T, W>::NV];
 #pragma unroll
-                for (int e = 0; e < Columns<T, D>::NV; ++e) run[e] = there ? values[e] * factor : T(0);
-                store_run(out + to, c, a.width, run);
+                for (int e = 0; e < Columns<T, W>::NV; ++e) run[e] = there ? values[e] * factor : T(0);
+                if (c < z.mine) store_run(out + to, z.c0 + c, width, run);
             });
         };
-        if (KEYS) put((T*)a.dk, dk[i], (T)a.scale);
-        if (VALUES) put((T*)a.dv, dv[i], T(1));
+        put((T*)a.dk, dk[i], (T)a.scale);
+        put((T*)a.dv, dv[i], T(1));
     }
 }
 
 // The gradient of the rows: as the forward pass, with the weights known from lse.
 template <typename T, int D>
 struct RowsShape {
-    static constexpr int KT = 32, RQ = sizeof(T) == 8 && D <= 32 ? 2 : 1;
-    static constexpr int LDS = 2 * Staged<T, D, KT>::BYTES;
+    typedef Halves<T, D> Z;
+    static constexpr int KT = Z::H == 1 ? 32 : 16, RQ = sizeof(T) == 8 && D <= 32 ? 2 : 1, ROWS = 16 * RQ * Z::GROUPS;
+    static constexpr int TILES = 2 * Staged<T, D, KT>::BYTES, LDS = TILES + Z::bytes(2);
 };
 
-template <typename T, int D, int THREADS = 256>
+template <typename T, int D, int THREADS = 256, bool LATE = false>
 __device__ __forceinline__ void rows_gradient_tile(const Args& a, char* lds, int problem, int part, int first_row) {
     typedef Matrix<T> M;
     typedef RowsShape<T, D> S;
-    constexpr int KT = S::KT, RQ = S::RQ, N = Vec<T>::N, C = D / (4 * N), PITCH = Staged<T, D, KT, THREADS>::PITCH;
+    typedef Halves<T, D> Z;
+    constexpr int KT = S::KT, RQ = S::RQ, N = Vec<T>::N, W = Z::W, C = W / (4 * N), PITCH = Staged<T, D, KT, THREADS>::PITCH;
+    static_assert(Z::H == 1 || (RQ == 1 && THREADS == 256), "two tiles of scores meet at a time");
     T *ks = reinterpret_cast<T*>(lds), *vs = ks + KT * PITCH;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4;
+    const int lane = threadIdx.x & 63, g = lane >> 4;
+    const int width = Z::H > 1 && !LATE ? D : a.width;
+    const Z z(width);
+    int turn = 0;
     const int b = problem / a.kv_heads, kvh = problem - b * a.kv_heads;
     const int n = count_of(a, b), begin = part_of(a, part, n, KT), end = part_of(a, part + 1, n, KT);
     const T* q = (const T*)a.q.p + b * a.q.batch + (int64_t)kvh * a.group * a.q.head;
@@ -511,33 +607,33 @@ __device__ __forceinline__ void rows_gradient_tile(const Args& a, char* lds, int
     const T* k = (const T*)a.k.p + b * a.k.batch + kvh * a.k.head;
     const T* v = (const T*)a.v.p + b * a.v.batch + kvh * a.v.head;
     const Rows q_rows(a, a.q), dy_rows(a, a.dy), k_rows(a.k), v_rows(a.v);
-    const int r0 = first_row + wave * 16 * RQ;
-    Fragment<T, D> qf[RQ], gf[RQ];
-    Columns<T, D> dq[RQ];
+    const int r0 = first_row + z.group * 16 * RQ;
+    Fragment<T, W, D, LATE> qf[RQ], gf[RQ];
+    Columns<T, W> dq[RQ];
     T level[RQ], delta[RQ];
 #pragma unroll
     for (int i = 0; i < RQ; ++i) {
         const int r = min(r0 + 16 * i + (lane & 15), a.rows - 1);
-        qf[i].load(q + q_rows.at(r), a.width, (T)(a.scale * M::base));
-        gf[i].load(dy + dy_rows.at(r), a.width, T(1));
+        qf[i].load(q + q_rows.at(r), width, (T)(a.scale * M::base), z.c0);
+        gf[i].load(dy + dy_rows.at(r), width, T(1), z.c0);
         const int64_t at = dense_row<T>(a, b, kvh, r);
         level[i] = level_of(((const T*)a.lse)[at]);
         delta[i] = ((const T*)a.delta)[at];
         dq[i].clear();
     }
-    Staged<T, D, KT, THREADS> kt, vt;
+    Staged<T, D, KT, THREADS, LATE> kt, vt;
     if (begin < end) {
-        kt.fetch(k, k_rows, begin, end, a.width);
-        vt.fetch(v, v_rows, begin, end, a.width);
+        kt.fetch(k, k_rows, begin, end, width);
+        vt.fetch(v, v_rows, begin, end, width);
     }
     for (int first = begin; first < end; first += KT) {
         __syncthreads();
-        kt.store(ks);
-        vt.store(vs);
+        kt.store(ks, width);
+        vt.store(vs, width);
         __syncthreads();
         if (first + KT < end) {
-            kt.fetch(k, k_rows, first + KT, end, a.width);
-            vt.fetch(v, v_rows, first + KT, end, a.width);
+            kt.fetch(k, k_rows, first + KT, end, width);
+            vt.fetch(v, v_rows, first + KT, end, width);
         }
 #pragma unroll
         for (int t = 0; t < KT / 16; ++t) {
@@ -546,7 +642,8 @@ __device__ __forceinline__ void rows_gradient_tile(const Args& a, char* lds, int
             for (int i = 0; i < RQ; ++i) s[i] = dp[i] = typename M::acc{};
 #pragma unroll
             for (int c = 0; c < C; ++c) {
-                const typename Vec<T>::type left = Staged<T, D, KT, THREADS>::along(ks, 16 * t, c), down = Staged<T, D, KT, THREADS>::along(vs, 16 * t, c);
+                if (z.ends(c * 4 * N)) break;
+                const typename Vec<T>::type left = Staged<T, D, KT, THREADS>::along(ks + z.c0, 16 * t, c), down = Staged<T, D, KT, THREADS>::along(vs + z.c0, 16 * t, c);
 #pragma unroll
                 for (int e = 0; e < N; ++e)
 #pragma unroll
@@ -554,6 +651,10 @@ __device__ __forceinline__ void rows_gradient_tile(const Args& a, char* lds, int
                         s[i] = M::mul(left[e], qf[i].g[c][e], s[i]);
                         dp[i] = M::mul(down[e], gf[i].g[c][e], dp[i]);
                     }
+            }
+            if constexpr (Z::H > 1) {
+                typename M::acc* halves[2] = {&s[0], &dp[0]};
+                z.meet(reinterpret_cast<T*>(lds + S::TILES), turn, halves);
             }
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
@@ -563,12 +664,13 @@ __device__ __forceinline__ void rows_gradient_tile(const Args& a, char* lds, int
             }
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                const T* row = ks + (16 * t + M::row_of(e, g)) * PITCH;
+                const T* row = ks + (16 * t + M::row_of(e, g)) * PITCH + z.c0;
 #pragma unroll
-                for (int blk = 0; blk < Columns<T, D>::BLOCKS; ++blk) {
-                    const auto left = Columns<T, D>::across(row, blk);
+                for (int blk = 0; blk < Columns<T, W>::BLOCKS; ++blk) {
+                    if (z.ends(blk * 16 * Columns<T, W>::NV)) break;
+                    const auto left = Columns<T, W>::across(row, blk);
 #pragma unroll
-                    for (int c = 0; c < Columns<T, D>::NV; ++c)
+                    for (int c = 0; c < Columns<T, W>::NV; ++c)
 #pragma unroll
                         for (int i = 0; i < RQ; ++i) dq[i].acc[blk][c] = M::mul(left[c], dp[i][e], dq[i].acc[blk][c]);
                 }
@@ -579,9 +681,11 @@ __device__ __forceinline__ void rows_gradient_tile(const Args& a, char* lds, int
     for (int i = 0; i < RQ; ++i) {
         const int r = r0 + 16 * i + (lane & 15);
         if (r >= a.rows) continue;
-        T* out = (T*)a.dq + part * a.part_size + dense_row<T>(a, b, kvh, r) * a.width;
+        T* out = (T*)a.dq + part * a.part_size + dense_row<T>(a, b, kvh, r) * width;
         dq[i].times((T)a.scale);
-        dq[i].each([&](int c, const auto& values) { store_run(out, c, a.width, values); });
+        dq[i].each([&](int c, const auto& values) {
+            if (c < z.mine) store_run(out, z.c0 + c, width, values);
+        });
     }
 }
 

@@ -20,25 +20,25 @@ namespace dali_hip {
 namespace {
 
 // ------------------------------------------------------------------------------------------------ many rows
-template <typename T, int D>
+template <typename T, int D, bool LATE>
 __global__ __launch_bounds__(256, D * sizeof(T) <= 1024 ? 2 : 1) void attention_rows(Args a) {
     extern __shared__ __attribute__((aligned(16))) char attention_lds[];
     const int id = on_die(blockIdx.x, gridDim.x), at = id / (a.tiles * a.parts), rest = id - at * a.tiles * a.parts, part = rest / a.tiles, tile = rest - part * a.tiles;
-    rows_tile<T, D>(a, attention_lds, a.first + at, part, tile * 64 * ForwardShape<T, D>::RQ);
+    rows_tile<T, D, LATE>(a, attention_lds, a.first + at, part, tile * ForwardShape<T, D>::ROWS);
 }
 
-template <typename T, int D, bool KEYS, bool VALUES>
+template <typename T, int D, bool LATE>
 __global__ __launch_bounds__(256, D * sizeof(T) <= 512 ? 2 : 1) void attention_states_gradient(Args a) {
     extern __shared__ __attribute__((aligned(16))) char attention_lds[];
     const int id = on_die(blockIdx.x, gridDim.x), at = id / (a.tiles * a.parts), rest = id - at * a.tiles * a.parts, part = rest / a.tiles, tile = rest - part * a.tiles;
-    states_gradient_tile<T, D, KEYS, VALUES>(a, attention_lds, a.first + at, part, tile * 64 * StatesShape<T, D>::RK);
+    states_gradient_tile<T, D, 256, LATE>(a, attention_lds, a.first + at, part, tile * StatesShape<T, D>::STATES);
 }
 
-template <typename T, int D>
+template <typename T, int D, bool LATE>
 __global__ __launch_bounds__(256, D * sizeof(T) <= 512 ? 2 : 1) void attention_rows_gradient(Args a) {
     extern __shared__ __attribute__((aligned(16))) char attention_lds[];
     const int id = on_die(blockIdx.x, gridDim.x), at = id / (a.tiles * a.parts), rest = id - at * a.tiles * a.parts, part = rest / a.tiles, tile = rest - part * a.tiles;
-    rows_gradient_tile<T, D>(a, attention_lds, a.first + at, part, tile * 64 * RowsShape<T, D>::RQ);
+    rows_gradient_tile<T, D, 256, LATE>(a, attention_lds, a.first + at, part, tile * RowsShape<T, D>::ROWS);
 }
 
 // ------------------------------------------------------------------------------------------------ few rows
@@ -331,9 +331,9 @@ struct ForwardPlan {
         const int64_t problems = (int64_t)a.batch * a.kv_heads;
         few = a.rows <= (D * sizeof(T) <= 512 ? 32 : 16);  // (wider rows: 32 would not fit a wave's registers)
         rq = a.rows <= 16 ? 1 : 2;
-        const int rows = std::is_same_v<T, float> ? 128 : 64 * S::RQ;
+        const int rows = std::is_same_v<T, float> ? 128 : S::ROWS;
         tiles = few ? 1 : (a.rows + rows - 1) / rows;
-        parts = few ? std::min(32, parts_for(problems, (a.keys + 63) / 64, D * sizeof(T) <= 256 ? 3 : 2, 2)) : parts_for(problems * tiles, (a.keys + S::KT - 1) / S::KT, 2, 4);
+        parts = few ? std::min(32, parts_for(problems, (a.keys + 63) / 64, D * sizeof(T) <= 256 ? 3 : 2, 2)) : parts_for(problems * tiles, (a.keys + S::KT - 1) / S::KT, Halves<T, D>::H == 1 ? 2 : 4, 4);
     }
 };
 
@@ -345,10 +345,15 @@ struct BackwardPlan {
     void set(const Args& a) {
         const int64_t problems = (int64_t)a.batch * a.kv_heads;
         // (float: rows and states of a tile by the kernels of attention_split.h)
-        constexpr int states = !std::is_same_v<T, float> ? 64 * StatesShape<T, D>::RK : D <= 128 ? 128 : 64, rows = !std::is_same_v<T, float> ? 64 * RowsShape<T, D>::RQ : states;
+        constexpr bool exact = !std::is_same_v<T, float>;
+        constexpr int states = exact ? StatesShape<T, D>::STATES : D <= 128 ? 128 : 64, rows = exact ? RowsShape<T, D>::ROWS : states;
         state_tiles = (a.keys + states - 1) / states, row_tiles = (a.rows + rows - 1) / rows;
-        state_parts = a.keys && a.rows ? parts_for(problems * state_tiles, (a.rows + 31) / 32, D <= 64 ? 2 : 1, 8) : 1;
-        row_parts = a.keys && a.rows ? parts_for(problems * row_tiles, (a.keys + 31) / 32, D <= 64 ? 2 : 1, 8) : 1;
+        // (Heads of more than 128 doubles: a slab of 16 is 3.4 us of work, so two make a part; four workgroups to a unit, one after the other, even out lengths: gradients of 3x878x3987,
+        // 4 heads of 256, 4780 us with one, 4190 with four)
+        constexpr int slab = exact ? StatesShape<T, D>::RT : 32, least = Halves<T, D>::H == 1 ? 8 : 2, per_unit = Halves<T, D>::H > 1 ? 4 : D <= 64 ? 2 : 1;
+        static_assert(!exact || slab == RowsShape<T, D>::KT, "the same slabs of rows and states");
+        state_parts = a.keys && a.rows ? parts_for(problems * state_tiles, (a.rows + slab - 1) / slab, per_unit, least) : 1;
+        row_parts = a.keys && a.rows ? parts_for(problems * row_tiles, (a.keys + slab - 1) / slab, per_unit, least) : 1;
         const auto round = [](int64_t n) { return (n + 63) / 64 * 64; };
         state_size = round((int64_t)a.batch * a.keys * a.kv_heads * a.width), row_size = round((int64_t)a.batch * a.queries * a.heads * a.width);
     }
@@ -410,6 +415,14 @@ int launch(const char* what, K kernel, int64_t problems, int64_t each, int lds, 
     return DALI_HIP_OK;
 }
 
+// f(false_type), or f(true_type) where attention_tiles.h has a form of its own for heads that do not fill D
+template <typename T, int D, typename F>
+int by_fill(int width, F f) {
+    if constexpr (Halves<T, D>::H > 1)
+        if (width != D) return f(std::true_type());
+    return f(std::false_type());
+}
+
 template <typename T, int D>
 int forward(const char* what, Args a) {
     ForwardPlan plan;
@@ -421,17 +434,19 @@ int forward(const char* what, Args a) {
         a.counter_step = counter_step(problems);
     }
     const int few_lds = 16 * plan.rq * (D + Vec<T>::N + 8) * (int)sizeof(T);
+    if (plan.few) {
+        if constexpr (D * sizeof(T) <= 512)
+            if (plan.rq == 2) return launch(what, attention_few<T, D, 2>, problems, plan.parts, few_lds, a);
+        return launch(what, attention_few<T, D, 1>, problems, plan.parts, few_lds, a);
+    }
     int status;
-    if (plan.few && plan.rq == 1)
-        status = launch(what, attention_few<T, D, 1>, problems, plan.parts, few_lds, a);
-    else if (plan.few) {
-        if constexpr (D * sizeof(T) <= 512) status = launch(what, attention_few<T, D, 2>, problems, plan.parts, few_lds, a);
-        else status = fail("%s: no kernel for %d rows", what, a.rows);  // (a plan makes none)
-    } else if constexpr (std::is_same_v<T, float>)
+    if constexpr (std::is_same_v<T, float>)
         status = launch(what, attention_rows_split<D>, problems, plan.tiles * plan.parts, SplitForward<D>::LDS, a);
     else
-        status = launch(what, attention_rows<T, D>, problems, plan.tiles * plan.parts, ForwardShape<T, D>::LDS, a);
-    if (status || plan.parts == 1 || plan.few) return status;
+        status = by_fill<T, D>(a.width, [&](auto late) {
+            return launch(what, attention_rows<T, D, decltype(late)::value>, problems, plan.tiles * plan.parts, ForwardShape<T, D>::LDS, a);
+        });
+    if (status || plan.parts == 1) return status;
     return launch(what, attention_join<T, D>, 1, (problems * a.rows + 3) / 4, 0, a);
 }
 
@@ -455,7 +470,6 @@ int backward(const char* what, Args a) {
     constexpr bool split = std::is_same_v<T, float>;
     T* parts = (T*)a.parts_y;
     if (a.keys > 0) {
-        typedef StatesShape<T, D> S;
         Args b = a;
         b.tiles = plan.state_tiles, b.parts = plan.state_parts;
         if (b.parts > 1) b.part_size = plan.state_size, b.dk = parts, b.dv = parts + b.parts * plan.state_size;
@@ -464,11 +478,9 @@ int backward(const char* what, Args a) {
             if (launch(what, attention_states_gradient_narrow<D>, problems, each, Narrow<D>::STATES_LDS, b, Narrow<D>::THREADS)) return DALI_HIP_ERROR;
         } else if constexpr (split) {
             if (launch(what, attention_states_gradient_split<D>, problems, each, SplitStates<D>::LDS, b)) return DALI_HIP_ERROR;
-        } else if constexpr (S::BOTH) {
-            if (launch(what, attention_states_gradient<T, D, true, true>, problems, each, S::LDS, b)) return DALI_HIP_ERROR;
         } else {
-            if (launch(what, attention_states_gradient<T, D, true, false>, problems, each, S::LDS, b)) return DALI_HIP_ERROR;
-            if (launch(what, attention_states_gradient<T, D, false, true>, problems, each, S::LDS, b)) return DALI_HIP_ERROR;
+            if (by_fill<T, D>(a.width, [&](auto late) { return launch(what, attention_states_gradient<T, D, decltype(late)::value>, problems, each, StatesShape<T, D>::LDS, b); }))
+                return DALI_HIP_ERROR;
         }
         if (b.parts > 1) {
             const int64_t size = (int64_t)a.batch * a.keys * a.kv_heads * a.width;
@@ -483,7 +495,7 @@ int backward(const char* what, Args a) {
     int status;
     if constexpr (split && D > 64) status = launch(what, attention_rows_gradient_narrow<D>, problems, each, Narrow<D>::ROWS_LDS, b, Narrow<D>::THREADS);
     else if constexpr (split) status = launch(what, attention_rows_gradient_split<D>, problems, each, SplitRows<D>::LDS, b);
-    else status = launch(what, attention_rows_gradient<T, D>, problems, each, RowsShape<T, D>::LDS, b);
+    else status = by_fill<T, D>(a.width, [&](auto late) { return launch(what, attention_rows_gradient<T, D, decltype(late)::value>, problems, each, RowsShape<T, D>::LDS, b); });
     return status || b.parts == 1 ? status : join(what, (const T*)parts, b.part_size, b.parts, rows * a.width, a.dq);
 }
 
