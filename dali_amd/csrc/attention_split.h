@@ -247,24 +247,24 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void attention_rows_split(Ar
         for (int step = 0; step < D / 16; ++step)
 #pragma unroll
             for (int t = 0; t < KT / 32; ++t) s[t] = multiply(Tile::along(ks, 32 * t, step), qf.step[step], s[t]);
-        // (a sum that passed -2^128 on its way stays -inf and would weigh nothing; one that passed 2^128 makes its row NaN)
-#pragma unroll
-        for (int t = 0; t < KT / 32; ++t)
-#pragma unroll
-            for (int e = 0; e < 16; ++e) lowest = fminf(lowest, s[t][e]);
+        float best = -INFINITY;
+        // (lowest: a sum that passed -2^128 on its way stays -inf and would weigh nothing; one that passed 2^128 makes its row NaN)
         if ((slab + 1) * KT > n) {
             asm volatile("");  // (a branch that the other slabs jump over, no selection that they all make)
 #pragma unroll
             for (int t = 0; t < KT / 32; ++t)
 #pragma unroll
-                for (int e = 0; e < 16; ++e)
+                for (int e = 0; e < 16; ++e) {
+                    lowest = fminf(lowest, s[t][e]);
                     if (slab * KT + 32 * t + split_row(e, h) >= n) s[t][e] = -INFINITY;
+                    best = fmaxf(best, s[t][e]);
+                }
+        } else {
+#pragma unroll
+            for (int t = 0; t < KT / 32; ++t)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) lowest = fminf(lowest, s[t][e]), best = fmaxf(best, s[t][e]);
         }
-        float best = -INFINITY;
-#pragma unroll
-        for (int t = 0; t < KT / 32; ++t)
-#pragma unroll
-            for (int e = 0; e < 16; ++e) best = fmaxf(best, s[t][e]);
         best = fmaxf(top, fold_lanes<64, 32>(best, Max()) * kDownTwice);
         if (__any(best > top)) {
             const float again = Matrix<float>::weight(top - best);
