@@ -165,7 +165,7 @@ __global__ __launch_bounds__(256) void dgemm_fold(const double* parts, int share
     *p = beta == 0.0 ? sum : sum + beta * *p;
 }
 
-constexpr int kShareTiles = 512;  // workgroups that a product is cut for
+constexpr int kShareTiles = 1024;  // workgroups that a product is cut for: four to a compute unit (gradients of [11401,723].[723,1078] 1483 us with two, so 1320)
 
 int share_of(int M, int N, int K, int* shares) {
     const long tiles = (long)((M + 63) / 64) * ((N + 63) / 64);
@@ -228,14 +228,17 @@ extern "C" int dali_hip_dgemm(int transB, int transA, int m, int n, int k, doubl
     a.A = A; a.ai = transA ? 1 : lda; a.ak = transA ? lda : 1;
     a.B = B; a.bk = transB ? 1 : ldb; a.bj = transB ? ldb : 1;
     a.C = C; a.ldc = ldc; a.alpha = alpha; a.beta = beta;
-    // 128 x 128 tiles when they still give every compute unit one, 64 x 64 otherwise
+    // 128 x 128 tiles where they come in nearly whole rounds of two to a compute unit, 64 x 64 otherwise: a unit that has one more than the others works alone with four times as much, and
+    // one by itself has nobody to work while it waits. us with the large and the small ones: 4096^3 2190 and 2320, 4096x2048x1024 283 and 301; 2048^3 330 and 305, 1238x7528x1583
+    // 1003 and 631, 5428x2432x3500 2540 and 1795, 3840x2880x1344 651 and 535, 11401x723x1078 589 and 398. (The sums are the same, in the same order.)
     static int cus = 0;
     if (cus == 0) {
         hipDeviceProp_t prop;
         cus = hipGetDeviceProperties(&prop, bound_device()) == hipSuccess ? prop.multiProcessorCount : 256;
     }
     const long tiles128 = (long)((rows + 127) / 128) * ((cols + 127) / 128);
-    const int T = tiles128 >= cus ? 4 : 2;
+    const long rounds = (tiles128 + 2 * cus - 1) / (2 * cus);
+    const int T = 16 * tiles128 >= 15 * rounds * 2 * cus ? 4 : 2;
     const int BM = 32 * T;
     const long tiles = (long)((rows + BM - 1) / BM) * ((cols + BM - 1) / BM);
     if (tiles > 0x7fffffffL) return fail("dali_hip_dgemm: too many tiles");
