@@ -11,7 +11,8 @@
 // padded: along a row they are read 16 bytes at a time, across rows by the transposing read, four rows of a column to a lane.
 //
 // What bounds it: products fill 0.29 (forward) to 0.48 (gradient of states, heads of 128) of the cycles; cutting, exponentials and waits for LDS beside them, which two waves to a
-// vector unit hide in part. us: 16x256x512 with 16 heads of 64 forward 55 (with fp32 instructions 84), its gradient 191 (280); 2x1999x4001, 8 heads on 2 of 128, gradient 1129 (2270).
+// vector unit hide in part. us: 16x256x512 with 16 heads of 64 forward 53 (with fp32 instructions 84), its gradient 187 (280); 2x1999x4001, 8 heads on 2 of 128, gradient 1060 (2270).
+// Registers decide how many waves that is: two to a unit, one with heads of 256, and some are spilled (84 and 73 of the forward pass with heads of 128 and 256).
 #ifndef DALI_HIP_ATTENTION_SPLIT_H
 #define DALI_HIP_ATTENTION_SPLIT_H
 

@@ -43,7 +43,8 @@ __global__ __launch_bounds__(256, D * sizeof(T) <= 512 ? 2 : 1) void attention_r
 
 // ------------------------------------------------------------------------------------------------ few rows
 // Up to 16 RQ rows: nobody shares a state with another wave, so each of the four takes states of its own, straight from memory into the operands (16 at a time,
-// 64-byte pieces of a state), and they are joined in LDS. Bound by reading the states: 32x1x2048 with 16 heads on 4 of 64, 101 MB, 28.5 us.
+// 64-byte pieces of a state), and they are joined in LDS. 32x1x2048 with 16 heads on 4 of 64, 101 MB: 28.4 us, of which reading at the rate of a copy takes 20 and the start of a launch and
+// the meeting of its parts 8.
 template <typename T, int D, int RQ>
 __global__ __launch_bounds__(256, D * sizeof(T) <= 512 ? 2 : 1) void attention_few(Args a) {
     typedef Matrix<T> M;

@@ -7,8 +7,8 @@
 // order, not by rows: a wave adds up the rows of dy at 16 to 128 neighbouring places, eight loads under way, and writes the runs that lie within them. A second launch
 // joins the parts of longer runs and writes the rows that no token names. What is summed in which order depends on the tokens alone, never on arrival.
 //
-// Bound by memory. 65536 tokens of 1024 floats: rows 57 us (268 MB written past the caches, 4.7 TB/s); gradient 136: ordering the tokens 14 to 28 in six launches, 83 for reading dy
-// (250 MB in the tokens' order, 3.0 TB/s), 34 for the second launch (131 MB written by both). 8 tokens: 3.9 us, the launch. fp64, 3001 tokens into 97 rows of 515: 36 us.
+// Bound by memory. 65536 tokens of 1024 floats: rows 57 us (268 MB written past the caches, 4.7 TB/s); gradient 136: ordering the tokens 14 to 28 in six launches, 84 for reading dy
+// (250 MB in the tokens' order, 3.0 TB/s), 31 for the second launch (131 MB written by both). 8 tokens: 3.9 us, the launch. fp64, 3001 tokens into 97 rows of 515: 36 us.
 #include <algorithm>
 #include <cmath>
 

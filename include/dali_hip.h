@@ -408,7 +408,8 @@ int dali_hip_embedding_backward(int dtype, int64_t count, int rows, int width, c
  * Attention of positions q [batch, queries, heads, width] to states k, v [batch, keys, kv_heads, width] of another length: head h looks at kv head h / (heads / kv_heads), and
  * sequence b has counts[b] states (held inside [0, keys]; counts NULL: all of them), what lies behind them is not read. With s = scale * q.k: lse = ln sum e^s
  * [batch, queries, heads], y = sum e^(s - lse) v [batch, queries, heads, width], both dense. A row without states, or with scores of -inf alone, has y = 0 and lse = -inf; a
- * score of +inf or NaN makes its row NaN. Strides are in values, of the first three axes; the last one is dense. width is at most DALI_HIP_MAX_HEAD_WIDTH.
+ * score of +inf or NaN makes its row NaN (in float scores are counted in powers of two: from 2.3e38 on they are infinite). Strides are in values, of the first
+ * three axes; the last one is dense. width is at most DALI_HIP_MAX_HEAD_WIDTH.
  */
 int dali_hip_cross_attention_workspace(int dtype, int batch, int queries, int keys, int heads, int kv_heads, int width, int backward, size_t* bytes);
 int dali_hip_cross_attention(int dtype, int batch, int queries, int keys, int heads, int kv_heads, int width, const void* q, const int64_t* q_strides, const void* k,
@@ -424,7 +425,8 @@ int dali_hip_cross_attention_backward(int dtype, int batch, int queries, int key
 /*
  * Softmax cross entropy of rows x [rows, inputs] (x_stride values apart) against the logits x w + bias, which are formed in pieces and not kept: lse = ln sum e^logit,
  * losses = lse - logit[target], both [rows]. w holds rows of the vocabulary's logits [inputs, vocab] w_stride values apart, or (w_by_columns) [vocab, inputs]; bias [vocab]
- * may be NULL. A target outside [0, vocab) stands for none: loss 0. A logit of -inf has probability 0; a row of -inf alone has lse -inf and loss +inf.
+ * may be NULL. A target outside [0, vocab) stands for none: loss 0. A logit of -inf has probability 0; a row of -inf alone has lse -inf and loss +inf; a
+ * logit of +inf or NaN makes its row NaN.
  */
 int dali_hip_projected_cross_entropy_workspace(int dtype, int64_t rows, int inputs, int vocab, int backward, int with_bias, size_t* bytes);
 int dali_hip_projected_cross_entropy(int dtype, int64_t rows, int inputs, int vocab, const void* x, int64_t x_stride, const void* w, int64_t w_stride, int w_by_columns,

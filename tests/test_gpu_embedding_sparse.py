@@ -23,8 +23,8 @@ def near_and_far(rng, count, rows):
 @pytest.mark.parametrize("rows,width,count", SIZES)
 @pytest.mark.parametrize("dtype", [np.float32, np.float64])
 def test_gradient(gpu, D, rng, rows, width, count, dtype):
-    if rows * width > 4000000 and dtype == np.float64:
-        rows = 16384
+    if width > 8192 and dtype == np.float64:
+        width //= 2
     dy, tokens = rng.randn(count, width).astype(dtype), near_and_far(rng, count, rows)
     out = D.Array.from_numpy(np.full((rows, width), np.nan, dtype))
     D.op.embedding_backward(D.Array.from_numpy(dy), D.Array.from_numpy(tokens), rows, 1.5, out=out)

@@ -10,12 +10,13 @@ from test_gpu_projected_cross_entropy import case, check_forward, check_gradient
 pytestmark = pytest.mark.gpu
 
 F, G = np.float32, np.float64
-CASES = [(F, 1100, 24, 90), (F, 2050, 5, 1030), (F, 16500, 7, 90), (F, 400, 12, 90001),  # (a second launch joins; two blocks; two pieces)
-         (G, 1100, 24, 130), (G, 1100, 5, 16001), (G, 16500, 6, 130), (G, 16500, 3, 1100), (G, 200, 4, 90000)]  # (... two pieces in two blocks; two pieces of few rows)
+# a second launch joins; two blocks; two pieces; both. With bias and rows of w, or without bias and columns
+CASES = [(F, 1100, 24, 90, True, False), (F, 1100, 24, 90, False, True), (F, 2050, 5, 1030, True, True), (F, 16500, 7, 90, True, False), (F, 16500, 7, 90, False, True),
+         (F, 400, 12, 90001, True, False), (F, 400, 12, 90001, False, True), (G, 1100, 24, 130, True, False), (G, 1100, 5, 16001, True, False), (G, 16500, 6, 130, True, False),
+         (G, 16500, 3, 1100, False, True)]
 
 
-@pytest.mark.parametrize("dtype,rows,inputs,vocab", CASES)
-@pytest.mark.parametrize("biased,by_columns", [(True, False), (False, True)])
+@pytest.mark.parametrize("dtype,rows,inputs,vocab,biased,by_columns", CASES)
 def test_both_directions(gpu, D, rng, dtype, rows, inputs, vocab, biased, by_columns):
     A, op = D.Array.from_numpy, D.op
     x, w, bias, targets = case(rng, dtype, rows, inputs, vocab)
