@@ -55,3 +55,40 @@ def test_gradients_with_a_small_scale(gpu, D, rng, width):
     """A scale of 1e-33, whose gradients dy of about 2^60 brings back to ordinary numbers."""
     q, k, v, counts = make(rng, np.float32, 2, 70, 90, 2, 1, width, [90, 47])
     check_backward(D, (rng.randn(*q.shape) * 2.0 ** 60).astype(np.float32), q, k, v, counts, 1e-33)
+
+
+@pytest.mark.parametrize("width", [129, 160, 187, 192, 193, 256])
+@pytest.mark.parametrize("queries,keys", [(40, 90), (19, 333)])
+def test_wide_heads_in_double_precision(gpu, D, rng, width, queries, keys):
+    """Two waves to a row: padded batches, views, destinations between other values, recordings."""
+    A, op = D.Array.from_numpy, D.op
+    q, k, v, counts = make(rng, np.float64, 4, queries, keys, 4, 2, width, [0, 1, keys, 33])
+    dy = rng.randn(*q.shape)
+    behind = np.arange(keys)[None, :] >= counts[:, None]
+    k[behind], v[behind] = np.nan, np.inf
+    scale = 1 / np.sqrt(width)
+    y, lse = check_forward(D, q, k, v, counts, scale)
+    grads = check_backward(D, dy, q, k, v, counts, scale)
+    turned = lambda a: A(np.ascontiguousarray(a.transpose(0, 2, 1, 3))).transpose(0, 2, 1, 3)  # noqa: E731
+    wider = A(np.concatenate([v, k, np.full(k.shape[:3] + (1,), np.nan)], 3))
+    views = (A(q[:, ::-1].copy())[:, ::-1], wider[:, :, :, width:2 * width], turned(v))
+    for a, b in zip((y, lse), op.cross_attention(*views, A(counts), scale)):
+        assert np.array_equal(a.numpy(), b.numpy())
+    for a, b in zip(grads, op.cross_attention_backward(turned(dy), *views, y, lse, A(counts), scale)):
+        assert np.array_equal(a.numpy(), b.numpy())
+    # destinations inside longer arrays: what lies before and behind stays
+    longer = [A(np.full((6,) + s[1:], 7.0)) for s in (q.shape, q.shape[:3], q.shape, k.shape, k.shape)]
+    inside = [a[1:5] for a in longer]
+    ins = [A(a) for a in (dy, q, k, v, counts)]
+    rec = D.Recording()
+    with rec:
+        op.cross_attention(*ins[1:], scale, out=inside[:2])
+        op.cross_attention_backward(*ins[:4], *inside[:2], ins[4], scale, out=inside[2:])
+    rec.make_graph()
+    for _ in range(3):
+        for a in inside:
+            a.assign(a * 0.0)
+        op.cross_attention(ins[1] * 2.0, ins[2], ins[3], ins[4])[0].numpy()  # the program's own work in between
+        rec.replay()
+        for got, want in zip(longer, (y, lse) + tuple(grads)):
+            assert (got.numpy()[[0, 5]] == 7).all() and np.array_equal(got.numpy()[1:5], want.numpy())
