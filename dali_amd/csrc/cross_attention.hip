@@ -314,9 +314,10 @@ constexpr int kUnits = 256;  // compute units that work is cut for
 // does best: gradients with heads of up to 64 two (4x1000x2000, heads of 64: 801 us with one, 686 with two, 738 with three), of more than 64 one (4x512x1024, heads of 256:
 // 501, 536, 565); single positions with heads of up to 64 floats three (32x1x2048: 30.3 us with two, 28.2 with three), wider ones two (8x1x4096, 32 heads
 // on 8 of 128: 59, 81), and at most 32 for a problem, since one workgroup joins them (1x1x8000, 16 heads of 64: 22 us, 26 with 48).
-int parts_for(int64_t workgroups, int slabs, int per_unit, int least) {
+// within: no more workgroups than those, since one to a unit that is left for a second round takes as long as the first
+int parts_for(int64_t workgroups, int slabs, int per_unit, int least, bool within = false) {
     if (workgroups >= kUnits * per_unit) return 1;
-    const int64_t wanted = ((int64_t)kUnits * per_unit + workgroups - 1) / workgroups;
+    const int64_t wanted = ((int64_t)kUnits * per_unit + (within ? 0 : workgroups - 1)) / workgroups;
     return (int)std::max<int64_t>(1, std::min<int64_t>({wanted, slabs / least, 64}));
 }
 
@@ -349,12 +350,13 @@ struct BackwardPlan {
         constexpr bool exact = !std::is_same_v<T, float>;
         constexpr int states = exact ? StatesShape<T, D>::STATES : D <= 128 ? 128 : 64, rows = exact ? RowsShape<T, D>::ROWS : states;
         state_tiles = (a.keys + states - 1) / states, row_tiles = (a.rows + rows - 1) / rows;
-        // (Heads of more than 128 doubles: a slab of 16 is 3.4 us of work, so two make a part; four workgroups to a unit, one after the other, even out lengths: gradients of 3x878x3987,
-        // 4 heads of 256, 4780 us with one, 4190 with four)
-        constexpr int slab = exact ? StatesShape<T, D>::RT : 32, least = Halves<T, D>::H == 1 ? 8 : 2, per_unit = Halves<T, D>::H > 1 ? 4 : D <= 64 ? 2 : 1;
+        // (Heads of more than 64 doubles: a slab is 3.4 to 6.8 us of work, so two make a part: gradients of 1x448x969, one head of 128, 299 us with eight, 98 with two. More than 128: four
+        // workgroups to a unit, one after the other, even out lengths: gradients of 3x878x3987, 4 heads of 256, 4780 us with one, 4190 with four)
+        constexpr int slab = exact ? StatesShape<T, D>::RT : 32, least = exact && D > 64 ? 2 : 8, per_unit = Halves<T, D>::H > 1 ? 4 : D <= 64 ? 2 : 1;
+        constexpr bool within = exact && D > 64 && per_unit == 1;
         static_assert(!exact || slab == RowsShape<T, D>::KT, "the same slabs of rows and states");
-        state_parts = a.keys && a.rows ? parts_for(problems * state_tiles, (a.rows + slab - 1) / slab, per_unit, least) : 1;
-        row_parts = a.keys && a.rows ? parts_for(problems * row_tiles, (a.keys + slab - 1) / slab, per_unit, least) : 1;
+        state_parts = a.keys && a.rows ? parts_for(problems * state_tiles, (a.rows + slab - 1) / slab, per_unit, least, within) : 1;
+        row_parts = a.keys && a.rows ? parts_for(problems * row_tiles, (a.keys + slab - 1) / slab, per_unit, least, within) : 1;
         const auto round = [](int64_t n) { return (n + 63) / 64 * 64; };
         state_size = round((int64_t)a.batch * a.keys * a.kv_heads * a.width), row_size = round((int64_t)a.batch * a.queries * a.heads * a.width);
     }

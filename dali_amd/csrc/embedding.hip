@@ -323,12 +323,12 @@ int embedding_backward(int64_t count, int rows, int width, const T* dy, int64_t 
     // A large table of which few rows are named is zeros for the most part: [44681,2199] for 34 tokens 134 us row by row, 90 (zeros alone 73), [119465,128] for one 59 and 20. Where the
     // named rows are more, the first launch has brought much of the table into the caches, and rows past them row by row are quicker ([43264,1344] fp64 for 5312 tokens 129 us, 150);
     // short rows gain as long as there are more of them than tokens ([79168,10] for 20084: 76, 47).
-    const bool narrow = width <= 32 * Vec<T>::N, sparse = rows >= 16384 && (rows >= 16 * count || (narrow && rows > count));
+    const bool narrow = width <= 32 * Vec<T>::N, past = past_caches((double)rows * width * sizeof(T));
+    const bool sparse = (rows >= 16384 || past) && (rows >= 16 * count || (narrow && rows > count));
     const int per = sparse ? std::max(1, std::min({(int)(kBytesEach / sizeof(T) / width), kMostRowsEach, rows / 1024})) : std::max(1, std::min(15, rows / 2048));
     int shift = 0;
     while (((int64_t)1 << shift) < width) ++shift;
     const unsigned times = (unsigned)((((uint64_t)1 << (31 + shift)) + width - 1) / width);  // (of an exact division by the width)
-    const bool past = past_caches((double)rows * width * sizeof(T));
     for (int64_t first = 0; first < rows; first += (int64_t)most * per) {
         const dim3 grid((unsigned)std::min((rows - first + per - 1) / per, (int64_t)most));
         either_way(narrow, [&](auto n) {
