@@ -6,9 +6,10 @@ from test_gpu_embedding import check_gradient, tokens_of
 
 pytestmark = pytest.mark.gpu
 
-# rows, width, tokens: around a row of one group, 32 groups, 64 groups; short rows with nearly as many tokens as rows; a row of more than 32 KiB
+# rows, width, tokens: around a row of one group, 32 groups, 64 groups; short rows with nearly as many tokens as rows; a row of more than 32 KiB; fewer rows,
+# of more than 256 MiB
 SIZES = [(16384, 1, 300), (16384, 3, 16000), (20011, 4, 900), (20000, 5, 19000), (16400, 33, 1000), (17000, 64, 40), (16500, 65, 1000), (16384, 129, 900), (16391, 131, 1), (20000, 257, 500),
-         (16384, 513, 300), (16500, 1030, 200), (16384, 8200, 20)]
+         (16384, 513, 300), (16500, 1030, 200), (16384, 8200, 20), (8000, 8500, 20)]
 
 
 def near_and_far(rng, count, rows):
